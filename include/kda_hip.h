@@ -323,6 +323,74 @@ int kda_log_decay_fwd(const void* alpha, float* g, int64_t n, float g_min, int d
 int kda_log_decay_bwd(const void* alpha, const float* dg, void* dalpha, int64_t n, float g_min, int dtype,
                       void* stream);
 
+/* Linear maps with an epilogue (the blocks' MLPs and projections,
+ * nope_gdn_mlx.py:216-262, 4009-4091):
+ *   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]
+ * for m < M, n < N, k < K; z (may be NULL) receives the value before act, which
+ * the backward pass reads.  act: 0 none, 1 gelu (z Phi(z)), 2 silu.  All of
+ * dtype; sums, epilogue and activation in fp32.  Matrices are rows of ld_*
+ * elements (at most 2^21), unit column stride.  bf16 with more than 64 rows: x
+ * and w 16-byte aligned, ld_x and ld_w multiples of 8 that cover K rounded up
+ * to 8, and that many elements of the last row readable; other operands and
+ * smaller or fp32 ones: any stride, aligned to their element. */
+#define KDA_ACT_NONE 0
+#define KDA_ACT_GELU 1
+#define KDA_ACT_SILU 2
+int kda_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
+                   const void* residual, int64_t ld_r, void* y, int64_t ld_y, void* z, int64_t ld_z,
+                   int M, int N, int K, int act, int dtype, void* stream);
+/* dx[m][k] = (sum_n dz[m][n] w[n][k]) * act'(z[m][k]), w [N][K]: the gradient of
+ * a map's input, times the derivative of the activation that made that input
+ * (act 0: none, z unused).  bf16: dz and w as x and w above. */
+int kda_linear_dgrad(const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, const void* z, int64_t ld_z,
+                     void* dx, int64_t ld_dx, int M, int N, int K, int act, int dtype, void* stream);
+/* fp32 weight and bias gradients dw[n][k] = sum_m dz[m][n] x[m][k], db[n] =
+ * sum_m dz[m][n] (db may be NULL), dw and db contiguous, sums in a fixed order.
+ * M >= 1; workspace: at least kda_linear_wgrad_workspace_size bytes, 16-byte
+ * aligned.  bf16: kda_weight_grad. */
+size_t kda_linear_wgrad_workspace_size(int M, int N, int K);
+int kda_linear_wgrad(const float* dz, int64_t ld_dz, const float* x, int64_t ld_x, float* dw, float* db,
+                     int M, int N, int K, void* workspace, size_t ws_bytes, void* stream);
+/* dz[m][n] = dy[m][n] act'(z[m][n]), act 1 or 2 */
+int kda_linear_act_bwd(const void* dy, int64_t ld_dy, const void* z, int64_t ld_z, void* dz, int64_t ld_dz,
+                       int M, int N, int act, int dtype, void* stream);
+
+/* The update of a training step over many tensors (the reference's clip and
+ * AdamW, train_mlx_k400.py:241-252, 548-549).  A tensor: its weights p and
+ * gradients g (n elements each, contiguous, of dtype) and where its moments
+ * begin, `offset` elements (a multiple of 256) into the moments' buffers.  Those
+ * buffers hold whole blocks of 256 elements: a tensor owns n rounded up to 256
+ * of them, and those past n are written as zeros (from zeros).  Tensors must
+ * not overlap.  Kernels take up to 120 tensors a launch. */
+typedef struct kda_adamw_tensor {
+    void* p;
+    const void* g;
+    int64_t n, offset, dtype;
+} kda_adamw_tensor;
+/* out[0] = sqrt(sum of g^2 over all tensors), out[1] = min(max_norm / (out[0] +
+ * 1e-6), 1), fp32, in a fixed order (p and offset unused). */
+size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count);
+int kda_grad_norm(const kda_adamw_tensor* tensors, int count, double max_norm, float* out,
+                  void* workspace, size_t ws_bytes, void* stream);
+/* g' = clip[1] g (clip: kda_grad_norm's out, or NULL for g itself);
+ *   m <- beta1 m + (1 - beta1) g';  v <- beta2 v + (1 - beta2) g'^2;
+ *   p <- p (1 - lr weight_decay) - lr correct1 m / (sqrt(v correct2) + eps)
+ * (correct1 = correct2 = 1: no bias correction).  master (may be NULL): fp32
+ * copies of the weights, laid out as the moments, updated in p's place, p their
+ * rounding.  states 0: m, v fp32.  states 1: 8 bits, one scale for 256 elements:
+ *   m int8,  value m_scale (k / 127) |k / 127|, m_scale the block's largest |m|;
+ *   v uint8, value (v_scale (k / 255)^2)^2, v_scale the block's largest sqrt(v),
+ *   k >= 1 where v > 0.
+ * m, v, master 16-byte aligned. */
+#define KDA_ADAMW_F32 0
+#define KDA_ADAMW_INT8 1
+int kda_adamw_step(const kda_adamw_tensor* tensors, int count, int states, void* m, void* v, float* m_scale,
+                   float* v_scale, float* master, const float* clip, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, double correct1, double correct2, void* stream);
+/* the values that n (a multiple of 256) 8-bit moments stand for */
+int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale,
+                      void* m_out, void* v_out, int64_t n, int dtype, void* stream);
+
 #define KDA_LAYER_PRODUCER 0
 #define KDA_LAYER_RMSNORM 1
 size_t kda_layer_workspace_size(int which, int B, int T, int H, int D);

@@ -9,6 +9,8 @@ from .kda import (ChunkKDAFunction, chunk_gdn, chunk_kda, gated_supported, kda_b
 from .layer import (ChunkKDAGatedFunction, GatedDeltaLayer, GatedRMSNormFunction, ProducerFunction, RMSNormGated,
                     ShortCausalConv1d, gated_rmsnorm_backward, gated_rmsnorm_forward, producer_backward,
                     producer_forward)
+from .linear import LinearActFunction, MLPFunction, linear_act, mlp
+from .optim import FusedAdamW
 from .recurrence import GDN_HIP_PATH, HIP_PATH, KDA_PATHS, KDARecurrence
 
 __all__ = [
@@ -17,5 +19,6 @@ __all__ = [
     "workspace_bytes", "workspace_offsets", "train_kept_bytes", "KDARecurrence", "HIP_PATH", "GDN_HIP_PATH", "KDA_PATHS",
     "GatedDeltaLayer", "ShortCausalConv1d", "RMSNormGated", "ProducerFunction", "GatedRMSNormFunction",
     "ChunkKDAGatedFunction",
+    "linear_act", "mlp", "LinearActFunction", "MLPFunction", "FusedAdamW",
     "producer_forward", "producer_backward", "gated_rmsnorm_forward", "gated_rmsnorm_backward",
 ]

@@ -35,7 +35,7 @@ WS_REGIONS = ("W", "U", "Qp", "QpT", "Kb", "KbT", "WT", "Aqk", "AqkT", "Akk", "T
 
 # every function the header declares, with its ctypes signature
 _P, _I, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
-_L, _F = ctypes.c_int64, ctypes.c_float
+_L, _F, _D = ctypes.c_int64, ctypes.c_float, ctypes.c_double
 SIGNATURES = {
     "kda_abi_version": ([], _I),
     "kda_last_error": ([], ctypes.c_char_p),
@@ -60,6 +60,15 @@ SIGNATURES = {
     "kda_layer_pack": ([_P, _I, _P], _I),
     "kda_log_decay_fwd": ([_P, _P, _L, _F, _I, _P], _I),
     "kda_log_decay_bwd": ([_P, _P, _P, _L, _F, _I, _P], _I),
+    "kda_linear_fwd": ([_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _L] + [_I] * 5 + [_P], _I),
+    "kda_linear_dgrad": ([_P, _L] * 4 + [_I] * 5 + [_P], _I),
+    "kda_linear_wgrad_workspace_size": ([_I] * 3, _Z),
+    "kda_linear_wgrad": ([_P, _L, _P, _L, _P, _P] + [_I] * 3 + [_P, _Z, _P], _I),
+    "kda_linear_act_bwd": ([_P, _L] * 3 + [_I] * 4 + [_P], _I),
+    "kda_grad_norm_workspace_size": ([_P, _I], _Z),
+    "kda_grad_norm": ([_P, _I, _D, _P, _P, _Z, _P], _I),
+    "kda_adamw_step": ([_P, _I, _I] + [_P] * 6 + [_D] * 7 + [_P], _I),
+    "kda_adamw_moments": ([_P] * 6 + [_L, _I, _P], _I),
     "kda_layer_workspace_size": ([_I] * 5, _Z),
     "kda_profile_enable": ([_I], _I),
     "kda_profile_name": ([_I], ctypes.c_char_p),

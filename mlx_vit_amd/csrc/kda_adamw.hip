@@ -1,0 +1,418 @@
+// kda_adamw.hip -- the training step's update over all of a model's tensors:
+// the gradients' global norm with the clip factor, AdamW with moments in fp32
+// or in 8 bits, and the C ABI around them.
+//
+//   G = sqrt(sum g^2), c = min(max_norm / (G + 1e-6), 1), g' = c g
+//   m <- b1 m + (1 - b1) g',  v <- b2 v + (1 - b2) g'^2
+//   p <- p (1 - lr wd) - lr c1 m / (sqrt(v) sqrt(c2) + eps)
+//
+// (the reference's AdamW, train_mlx_k400.py:548-549, without bias correction
+// c1 = c2 = 1).  Everything between the loads and the stores is fp32.
+//
+// The moments of all tensors lie in one buffer each, a tensor's beginning on a
+// multiple of 256 elements.  In 8 bits 256 consecutive elements share a scale:
+//   m = s (k / 127) |k / 127|, k in [-127, 127], s the block's largest |m|
+//   sqrt(v) = s (k / 255)^2,   k in [0, 255],    s the block's largest sqrt(v)
+// Both laws spend their codes on small values (v over ten decades); v's holds
+// the root that the update divides by, and a v above zero keeps a code above
+// zero, so no weight is divided by eps alone.  The update itself uses the new
+// moments before they are rounded to codes.
+#include <math.h>
+
+#include "kda_hip.h"
+#include "kda_internal.h"
+
+namespace kda {
+
+namespace {
+
+constexpr int QB = 256;            // elements that share a scale
+constexpr int PER_WG = 4096;       // elements of one tensor a workgroup updates
+constexpr int NORM_PER_WG = 16384; // and sums the squares of
+constexpr int PER_LAUNCH = 120;    // tensors of one launch (their descriptors travel as kernel arguments)
+
+struct Tensor {
+    void* p;
+    const void* g;
+    int64_t n;
+    uint32_t blk0;                 // first block of 256 in the moments
+    uint32_t wg0;                  // first workgroup
+};
+struct StepArgs {
+    Tensor t[PER_LAUNCH];
+    uint8_t flags[PER_LAUNCH];     // 1: bf16, 2: p and g 16-byte aligned
+    int count;
+    float b1, omb1, b2, omb2, decay, lr, eps, rc2;
+    const float* clip;
+    void *m, *v;
+    float *ms, *vs, *master;
+};
+static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
+struct NormArgs2 {
+    Tensor t[PER_LAUNCH];
+    uint8_t flags[PER_LAUNCH];
+    int count;
+    float* part;
+};
+
+// the tensor of workgroup b: the last whose first workgroup is at most b.  All
+// lanes look at once (a binary search is seven dependent scalar loads).
+template <typename Args>
+__device__ __forceinline__ int tensor_of(const Args& a, uint32_t b) {
+    const int l = lane_id();
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER_LAUNCH; i += 64)
+        n += __popcll(__ballot(i + l < a.count && a.t[min(i + l, PER_LAUNCH - 1)].wg0 <= b));
+    return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+// eight elements at p, of which `left` exist
+template <typename T>
+__device__ __forceinline__ void ld8(const T* p, int64_t left, bool vec, float (&x)[8]) {
+    if (vec && left >= 8) {
+        if constexpr (std::is_same<T, float>::value) {
+            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            x[0] = bf_lo(a.x); x[1] = bf_hi(a.x); x[2] = bf_lo(a.y); x[3] = bf_hi(a.y);
+            x[4] = bf_lo(a.z); x[5] = bf_hi(a.z); x[6] = bf_lo(a.w); x[7] = bf_hi(a.w);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < left ? ld1<T>(p + e) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void st8(T* p, int64_t left, bool vec, const float (&x)[8]) {
+    if (vec && left >= 8) {
+        if constexpr (std::is_same<T, float>::value) {
+            *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            *reinterpret_cast<uint4*>(p) =
+                make_uint4(pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7]));
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < left) st1<T>(p + e, x[e]);
+}
+
+// The largest of 32 lanes' values by their bits: of non-negative floats this is
+// the largest value, and a NaN, whose bits are larger than infinity's, wins, so
+// that a block with one decodes to NaN instead of to something finite.
+__device__ __forceinline__ uint32_t max32(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, true));   // row_half_mirror
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, true));   // row_mirror
+    return max(x, (uint32_t)__builtin_amdgcn_ds_swizzle((int)x, 0x401F));                  // lane ^ 16
+}
+
+// a scale's reciprocal; below the smallest normal the block counts as zero
+constexpr uint32_t MIN_NORMAL = 0x00800000u;
+__device__ __forceinline__ float inv_scale(uint32_t s) {
+    return s < MIN_NORMAL ? 0.f : __builtin_amdgcn_rcpf(__uint_as_float(s));
+}
+
+template <typename T, bool SMALL, bool MASTER>
+__device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, bool vec, float c, int64_t e0) {
+    const int64_t left = t.n - e0;
+    const size_t at = (size_t)t.blk0 * QB + e0;      // in the moments
+    T* p = static_cast<T*>(t.p) + e0;
+    float g[8], w[8], m[8], v[8];
+    ld8<T>(static_cast<const T*>(t.g) + e0, left, vec, g);
+    if constexpr (MASTER) ld8<float>(a.master + at, 8, true, w);
+    else ld8<T>(p, left, vec, w);
+    if constexpr (SMALL) {
+        const uint2 km = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.m) + at);
+        const uint2 kv = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + at);
+        const float sm = a.ms[at / QB] * (1.f / (127.f * 127.f)), sv = a.vs[at / QB] * (1.f / (255.f * 255.f));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float k = (float)(int8_t)((e < 4 ? km.x : km.y) >> (8 * (e & 3)));
+            const float q = (float)(uint8_t)((e < 4 ? kv.x : kv.y) >> (8 * (e & 3)));
+            m[e] = sm * k * fabsf(k);
+            const float r = sv * q * q;
+            v[e] = r * r;
+        }
+    } else {
+        ld8<float>(static_cast<const float*>(a.m) + at, 8, true, m);
+        ld8<float>(static_cast<const float*>(a.v) + at, 8, true, v);
+    }
+    uint32_t top_m = 0, top_r = 0;
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        g[e] *= c;
+        m[e] = fmaf(a.b1, m[e], a.omb1 * g[e]);
+        v[e] = fmaf(a.b2, v[e], a.omb2 * g[e] * g[e]);
+        r[e] = __builtin_amdgcn_sqrtf(v[e]);
+        // lr holds the bias correction c1, rc2 is sqrt(c2)
+        w[e] = fmaf(w[e], a.decay, -a.lr * m[e] * __builtin_amdgcn_rcpf(fmaf(r[e], a.rc2, a.eps)));
+        if constexpr (SMALL) {
+            top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
+            top_r = max(top_r, __float_as_uint(r[e]) & 0x7fffffffu);
+        }
+    }
+    st8<T>(p, left, vec, w);
+    if constexpr (MASTER) st8<float>(a.master + at, 8, true, w);
+    if constexpr (SMALL) {
+        top_m = max32(top_m);
+        top_r = max32(top_r);
+        const float im = inv_scale(top_m), ir = inv_scale(top_r);
+        uint32_t km[2] = {0u, 0u}, kv[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m[e]) * im));
+            const int k = (int)copysignf(x, m[e]);
+            const float y = rintf(255.f * __builtin_amdgcn_sqrtf(r[e] * ir));
+            const int q = r[e] * ir > 0.f ? max((int)y, 1) : 0;
+            km[e >> 2] |= (uint32_t)(k & 255) << (8 * (e & 3));
+            kv[e >> 2] |= (uint32_t)q << (8 * (e & 3));
+        }
+        *reinterpret_cast<uint2*>(static_cast<int8_t*>(a.m) + at) = make_uint2(km[0], km[1]);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + at) = make_uint2(kv[0], kv[1]);
+        if ((lane_id() & 31) == 0) {
+            a.ms[at / QB] = top_m < MIN_NORMAL ? 0.f : __uint_as_float(top_m);
+            a.vs[at / QB] = top_r < MIN_NORMAL ? 0.f : __uint_as_float(top_r);
+        }
+    } else {
+        st8<float>(static_cast<float*>(a.m) + at, 8, true, m);
+        st8<float>(static_cast<float*>(a.v) + at, 8, true, v);
+    }
+}
+
+template <bool SMALL, bool MASTER>
+__global__ __launch_bounds__(256) void kda_adamw_kernel(const StepArgs a) {
+    const int i = tensor_of(a, blockIdx.x);
+    const Tensor& t = a.t[i];
+    const int f = a.flags[i];
+    const float c = a.clip ? a.clip[1] : 1.f;
+    const int64_t b0 = (int64_t)(blockIdx.x - t.wg0) * PER_WG, end = min((t.n + QB - 1) / QB * QB, b0 + (int64_t)PER_WG);
+    for (int64_t e = b0 + 8 * (int64_t)threadIdx.x; e < end; e += 8 * 256) {   // whole blocks: half waves stay together
+        if (f & 1) update<uint16_t, SMALL, MASTER>(a, t, f & 2, c, e);
+        else update<float, SMALL, MASTER>(a, t, f & 2, c, e);
+    }
+}
+
+__device__ __forceinline__ float wg_sum(float s, float* lds) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    if (lane_id() == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+__global__ __launch_bounds__(256) void kda_grad_norm_kernel(const NormArgs2 a) {
+    __shared__ float lds[4];
+    const int i = tensor_of(a, blockIdx.x);
+    const Tensor& t = a.t[i];
+    const int f = a.flags[i];
+    const int64_t b0 = (int64_t)(blockIdx.x - t.wg0) * NORM_PER_WG, end = min(t.n, b0 + (int64_t)NORM_PER_WG);
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, x[8];
+    for (int64_t e = b0 + 8 * (int64_t)threadIdx.x; e < end; e += 8 * 256) {
+        if (f & 1) ld8<uint16_t>(static_cast<const uint16_t*>(t.g) + e, t.n - e, f & 2, x);
+        else ld8<float>(static_cast<const float*>(t.g) + e, t.n - e, f & 2, x);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s[q] = fmaf(x[q], x[q], s[q]);
+    }
+    const float sum = wg_sum(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])), lds);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = sum;
+}
+
+// out[0] = G, out[1] = the clip factor (a NaN stays one)
+__global__ __launch_bounds__(1024) void kda_grad_norm_finish_kernel(const float* __restrict__ part, int n, float max_norm,
+                                                                    float* __restrict__ out) {
+    __shared__ double lds[16];
+    double s = 0.;
+    for (int i = threadIdx.x; i < n; i += 1024) s += (double)part[i];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    if (lane_id() == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < 16; ++i) s += lds[i];
+    const float g = (float)sqrt(s), c = max_norm / (g + 1e-6f);
+    out[0] = g;
+    out[1] = c > 1.f ? 1.f : c;
+}
+
+// what 8-bit moments stand for, eight a thread
+template <typename T>
+__global__ __launch_bounds__(256) void kda_adamw_moments_kernel(const int8_t* __restrict__ m, const uint8_t* __restrict__ v,
+                                                                const float* __restrict__ ms, const float* __restrict__ vs,
+                                                                T* __restrict__ mo, T* __restrict__ vo, size_t n) {
+    for (size_t at = 8 * ((size_t)blockIdx.x * 256 + threadIdx.x); at < n; at += 8 * 256 * (size_t)gridDim.x) {
+        const uint2 km = *reinterpret_cast<const uint2*>(m + at), kv = *reinterpret_cast<const uint2*>(v + at);
+        const float sm = ms[at / QB] * (1.f / (127.f * 127.f)), sv = vs[at / QB] * (1.f / (255.f * 255.f));
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float k = (float)(int8_t)((e < 4 ? km.x : km.y) >> (8 * (e & 3)));
+            const float q = (float)(uint8_t)((e < 4 ? kv.x : kv.y) >> (8 * (e & 3)));
+            x[e] = sm * k * fabsf(k);
+            const float r = sv * q * q;
+            y[e] = r * r;
+        }
+        st8<T>(mo + at, 8, true, x);
+        st8<T>(vo + at, 8, true, y);
+    }
+}
+
+int check_tensors(const kda_adamw_tensor* t, int count, bool step) {
+    if (count < 0 || (count > 0 && !t)) return api_fail(KDA_E_INVALID, "count=%d tensors at %p", count, (const void*)t);
+    for (int i = 0; i < count; ++i) {
+        if (t[i].dtype != KDA_DTYPE_F32 && t[i].dtype != KDA_DTYPE_BF16)
+            return api_fail(KDA_E_UNSUPPORTED, "tensor %d: dtype=%lld: expected 0 (fp32) or 1 (bf16)", i, (long long)t[i].dtype);
+        if (t[i].n < 0 || t[i].n > ((int64_t)1 << 36)) return api_fail(KDA_E_INVALID, "tensor %d: n=%lld", i, (long long)t[i].n);
+        if (t[i].n == 0) continue;
+        const uintptr_t es = t[i].dtype == KDA_DTYPE_BF16 ? 2 : 4;
+        if (!t[i].g || reinterpret_cast<uintptr_t>(t[i].g) % es != 0 ||
+            (step && (!t[i].p || reinterpret_cast<uintptr_t>(t[i].p) % es != 0)))
+            return api_fail(KDA_E_INVALID, "tensor %d: p or g is NULL or misaligned", i);
+        if (step && (t[i].offset < 0 || t[i].offset % QB != 0 || t[i].offset / QB > 0xffffffffLL))
+            return api_fail(KDA_E_INVALID, "tensor %d: offset=%lld: expected a multiple of %d", i, (long long)t[i].offset, QB);
+    }
+    return KDA_OK;
+}
+
+// the next tensors of a launch (from *i on), workgroups of `per` elements; returns the workgroups
+template <typename Args>
+uint32_t fill(Args& a, const kda_adamw_tensor* t, int count, int* i, int per, bool step) {
+    a.count = 0;
+    uint32_t wg = 0;
+    for (; *i < count && a.count < PER_LAUNCH; ++*i) {
+        const kda_adamw_tensor& q = t[*i];
+        if (q.n == 0) continue;
+        const uint32_t need = (uint32_t)((q.n + per - 1) / per);
+        if (wg + need > (1u << 23) && a.count > 0) break;   // 256 threads each: below 2^32 in all
+        const uintptr_t both = reinterpret_cast<uintptr_t>(q.g) | (step ? reinterpret_cast<uintptr_t>(q.p) : 0);
+        a.t[a.count] = Tensor{q.p, q.g, q.n, (uint32_t)(step ? q.offset / QB : 0), wg};
+        a.flags[a.count] = (uint8_t)((q.dtype == KDA_DTYPE_BF16 ? 1 : 0) | (both % 16 == 0 ? 2 : 0));
+        ++a.count;
+        wg += need;
+    }
+    return wg;
+}
+
+size_t norm_parts(const kda_adamw_tensor* t, int count) {
+    size_t n = 0;
+    for (int i = 0; i < count; ++i) n += (size_t)((t[i].n + NORM_PER_WG - 1) / NORM_PER_WG);
+    return n;
+}
+
+}  // namespace
+
+}  // namespace kda
+
+using namespace kda;
+
+extern "C" {
+
+size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count) {
+    if (check_tensors(tensors, count, false) != KDA_OK) return 0;
+    return norm_parts(tensors, count) * sizeof(float);
+}
+
+int kda_grad_norm(const kda_adamw_tensor* tensors, int count, double max_norm, float* out, void* workspace, size_t ws_bytes,
+                  void* stream) {
+    const int rc = check_tensors(tensors, count, false);
+    if (rc != KDA_OK) return rc;
+    if (!out || reinterpret_cast<uintptr_t>(out) % 4 != 0) return api_fail(KDA_E_INVALID, "out is NULL or misaligned");
+    if (!(max_norm > 0.)) return api_fail(KDA_E_INVALID, "max_norm=%g: expected a positive number", max_norm);
+    const size_t parts = norm_parts(tensors, count);
+    if (parts > 0x7fffffffu) return api_fail(KDA_E_UNSUPPORTED, "%zu partial sums", parts);
+    if (parts > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0))
+        return api_fail(KDA_E_INVALID, "workspace is NULL or misaligned");
+    if (ws_bytes < parts * sizeof(float))
+        return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, parts * sizeof(float));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    NormArgs2 a;
+    float* part = static_cast<float*>(workspace);
+    for (int i = 0; i < count;) {
+        a.part = part;
+        const uint32_t wg = fill(a, tensors, count, &i, NORM_PER_WG, false);
+        if (wg == 0) continue;
+        hipLaunchKernelGGL(kda_grad_norm_kernel, dim3(wg), dim3(256), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return api_hip_fail(e, "kda_grad_norm");
+        part += wg;
+    }
+    hipLaunchKernelGGL(kda_grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float*>(workspace),
+                       (int)parts, (float)max_norm, out);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_grad_norm");
+}
+
+int kda_adamw_step(const kda_adamw_tensor* tensors, int count, int states, void* m, void* v, float* m_scale, float* v_scale,
+                   float* master, const float* clip, double lr, double beta1, double beta2, double eps, double weight_decay,
+                   double correct1, double correct2, void* stream) {
+    const int rc = check_tensors(tensors, count, true);
+    if (rc != KDA_OK) return rc;
+    if (states != KDA_ADAMW_F32 && states != KDA_ADAMW_INT8)
+        return api_fail(KDA_E_UNSUPPORTED, "states=%d: expected 0 (fp32) or 1 (8 bits)", states);
+    if (!(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1. && eps >= 0. && correct1 > 0. && correct2 > 0.))
+        return api_fail(KDA_E_INVALID, "beta1=%g beta2=%g eps=%g correct1=%g correct2=%g", beta1, beta2, eps, correct1,
+                        correct2);
+    if (count == 0) return KDA_OK;
+    const bool small = states == KDA_ADAMW_INT8;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(master);
+    if (!m || !v || all % 16 != 0) return api_fail(KDA_E_INVALID, "m, v or master is NULL or not 16-byte aligned");
+    if (small && (!m_scale || !v_scale || (reinterpret_cast<uintptr_t>(m_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 4 != 0))
+        return api_fail(KDA_E_INVALID, "m_scale or v_scale is NULL or misaligned");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    StepArgs a;
+    a.b1 = (float)beta1; a.omb1 = (float)(1. - beta1);
+    a.b2 = (float)beta2; a.omb2 = (float)(1. - beta2);
+    a.decay = (float)(1. - lr * weight_decay);
+    a.lr = (float)(lr * correct1);
+    a.eps = (float)eps;
+    a.rc2 = (float)sqrt(correct2);
+    a.clip = clip;
+    a.m = m; a.v = v; a.ms = m_scale; a.vs = v_scale; a.master = master;
+    for (int i = 0; i < count;) {
+        const uint32_t wg = fill(a, tensors, count, &i, PER_WG, true);
+        if (wg == 0) continue;
+        const dim3 grid(wg), block(256);
+        if (small && master) hipLaunchKernelGGL((kda_adamw_kernel<true, true>), grid, block, 0, st, a);
+        else if (small) hipLaunchKernelGGL((kda_adamw_kernel<true, false>), grid, block, 0, st, a);
+        else if (master) hipLaunchKernelGGL((kda_adamw_kernel<false, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((kda_adamw_kernel<false, false>), grid, block, 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return api_hip_fail(e, "kda_adamw_step");
+    }
+    return KDA_OK;
+}
+
+int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale, void* m_out, void* v_out,
+                      int64_t n, int dtype, void* stream) {
+    if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_BF16)
+        return api_fail(KDA_E_UNSUPPORTED, "dtype=%d: expected 0 (fp32) or 1 (bf16)", dtype);
+    if (n < 0 || n % QB != 0) return api_fail(KDA_E_INVALID, "n=%lld: expected a multiple of %d", (long long)n, QB);
+    if (n == 0) return KDA_OK;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(m_out) |
+                          reinterpret_cast<uintptr_t>(v_out);
+    if (!m || !v || !m_out || !v_out || all % 16 != 0)
+        return api_fail(KDA_E_INVALID, "m, v, m_out or v_out is NULL or not 16-byte aligned");
+    if (!m_scale || !v_scale || (reinterpret_cast<uintptr_t>(m_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 4 != 0)
+        return api_fail(KDA_E_INVALID, "m_scale or v_scale is NULL or misaligned");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid((unsigned)std::min<int64_t>((n / 8 + 255) / 256, 8192)), block(256);
+    const int8_t* km = static_cast<const int8_t*>(m);
+    const uint8_t* kv = static_cast<const uint8_t*>(v);
+    if (dtype == KDA_DTYPE_BF16)
+        hipLaunchKernelGGL((kda_adamw_moments_kernel<uint16_t>), grid, block, 0, st, km, kv, m_scale, v_scale,
+                           static_cast<uint16_t*>(m_out), static_cast<uint16_t*>(v_out), (size_t)n);
+    else
+        hipLaunchKernelGGL((kda_adamw_moments_kernel<float>), grid, block, 0, st, km, kv, m_scale, v_scale,
+                           static_cast<float*>(m_out), static_cast<float*>(v_out), (size_t)n);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_adamw_moments");
+}
+
+}  // extern "C"

@@ -24,8 +24,11 @@ from typing import List, Optional, Tuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .layer import GatedDeltaLayer
+from .layer_fused import _plain_module
+from .linear import mlp
 
 BF16_KEEP_FP32 = ("A_log", "dt_bias")
 
@@ -123,6 +126,27 @@ def _mlp(dim: int, ratio: float, dropout: float) -> nn.Sequential:
     return nn.Sequential(nn.Linear(dim, h), nn.GELU(), nn.Dropout(dropout), nn.Linear(h, dim), nn.Dropout(dropout))
 
 
+def _mlp_residual(block: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """x + drop_path(mlp(norm2(x))).  With ``block.fused_mlp`` the two maps run as
+    ``mlp`` where that computes the same: plain modules with biases, no dropout, one
+    dtype, on a ROCm device, outside autocast and tracing."""
+    h = block.norm2(x)
+    seq = block.mlp
+    if not (block.fused_mlp and type(seq) is nn.Sequential and len(seq) == 5 and h.device.type == "cuda"
+            and h.dtype in (torch.bfloat16, torch.float32) and not torch.is_autocast_enabled("cuda")
+            and not torch.compiler.is_compiling() and not torch._C._is_tracing()
+            and forward_ad._current_level < 0 and _plain_module(seq, nn.Sequential)
+            and all(_plain_module(m, c) for m, c in zip(seq, (nn.Linear, nn.GELU, nn.Dropout, nn.Linear, nn.Dropout)))
+            and seq[1].approximate == "none" and not any(m.p > 0 and m.training for m in (seq[2], seq[4]))
+            and all(type(p) is nn.Parameter and p.dtype == h.dtype and p.device == h.device for p in seq.parameters())
+            and seq[0].bias is not None and seq[3].bias is not None):
+        return x + block.drop_path(seq(h))
+    params = seq[0].weight, seq[0].bias, seq[3].weight, seq[3].bias
+    if x.dtype != h.dtype or (isinstance(block.drop_path, DropPath) and block.training):
+        return x + block.drop_path(mlp(h, *params))
+    return mlp(h, *params, residual=x)
+
+
 class NoPEViTBlock(nn.Module):
     """Pre-norm ViT block, optional spatial-only attention (nope_gdn_mlx.py:216-262)."""
 
@@ -135,6 +159,7 @@ class NoPEViTBlock(nn.Module):
         self.drop_path = DropPath(drop_path) if drop_path > 0 else nn.Identity()
         self.norm2 = nn.LayerNorm(embed_dim, eps=1e-6)
         self.mlp = _mlp(embed_dim, mlp_ratio, dropout)
+        self.fused_mlp = False   # set_fused_mlp
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, N, D = x.shape
@@ -145,7 +170,7 @@ class NoPEViTBlock(nn.Module):
         else:
             a = self.attn(normed, mask=mask)
         x = x + self.drop_path(a)
-        return x + self.drop_path(self.mlp(self.norm2(x)))
+        return _mlp_residual(self, x)
 
 
 class NoPEVideoEncoder(nn.Module):
@@ -198,6 +223,7 @@ class HybridBlock(nn.Module):
             self.layer = NoPEMultiheadAttention(dim, num_heads, dropout)
         self.norm2 = nn.LayerNorm(dim, eps=1e-6)
         self.mlp = _mlp(dim, mlp_ratio, dropout)
+        self.fused_mlp = False   # set_fused_mlp
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None,
                 state: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -222,8 +248,7 @@ class HybridBlock(nn.Module):
             out = self.layer(normed, mask=mask)
             new_state = state
         x = x + self.drop_path(out)
-        x = x + self.drop_path(self.mlp(self.norm2(x)))
-        return x, new_state
+        return _mlp_residual(self, x), new_state
 
 
 class NoPEGDNVideoBackbone(nn.Module):
@@ -350,6 +375,16 @@ def to_bf16(model: nn.Module, keep_fp32: Tuple[str, ...] = BF16_KEEP_FP32) -> nn
     for name, p in model.named_parameters():
         if p.dtype == torch.float32 and not any(s in name for s in keep_fp32):
             p.data = p.data.to(torch.bfloat16)
+    return model
+
+
+def set_fused_mlp(model: nn.Module, on: bool = True) -> nn.Module:
+    """Run the MLP of every block of ``model`` as ``linear.mlp`` (off by default: the
+    results differ from the separate modules' in the rounding of the value before
+    the activation and of the residual's sum).  In place; returns the model."""
+    for m in model.modules():
+        if isinstance(m, (NoPEViTBlock, HybridBlock)):
+            m.fused_mlp = on
     return model
 
 

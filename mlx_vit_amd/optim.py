@@ -1,0 +1,197 @@
+"""AdamW over all of a model's tensors in a few launches: ``FusedAdamW``.
+
+The update is ``train.AdamW``'s (the reference's, train_mlx_k400.py:548-549), with
+the gradients' global norm and clip (train_mlx_k400.py:241-252) folded into it:
+the norm is one pass over the gradients, and the update multiplies each gradient
+by the clip factor as it reads it, so no gradient is rewritten.  What differs is
+what the moments are held in: fp32 whatever the weights' dtype, or 8 bits with a
+scale for each 256 elements, and on request an fp32 copy of the weights
+(``master_weights``) that bf16 weights are the rounding of, so that updates below
+half a bf16 step add up.
+
+8-bit moments: m = s (k / 127) |k / 127|, k in [-127, 127], s the block's largest
+|m|; v = (s (k / 255)^2)^2, k in [0, 255], s the block's largest sqrt(v).  The
+update uses the new moments before they are rounded.  A gradient that is not
+finite makes its whole block of 8-bit moments NaN.
+"""
+from __future__ import annotations
+
+from array import array
+from typing import Dict, Iterable, List, Optional, Tuple
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from .kda import _DTYPE_CODE, _ptr, _stream
+from .linear import _on
+
+BLOCK = 256      # elements that share a scale; a tensor's moments begin on a multiple of it
+_STATES = {"fp32": 0, "int8": 1}
+_data_ptr, _contiguous, _numel = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
+
+
+class FusedAdamW:
+    """AdamW with moments of their own dtype.
+
+    ``states``: "fp32" or "int8"; ``master_weights``: keep and update fp32 copies of
+    the weights; ``bias_correction``: divide the moments by 1 - beta^step (off in
+    the reference).  ``state``: buffers to use (not copied), as the attribute
+    ``state`` of an optimizer over the same tensors holds them: "m", "v" (fp32, or
+    int8 and uint8 with "m_scale" and "v_scale"), "master"; parameter i's part
+    begins at ``offsets[i]`` and what lies between two parameters' is zero.
+
+    Parameters are contiguous fp32 or bf16 tensors on one ROCm device; those
+    without a gradient at a step are left out of it."""
+
+    def __init__(self, params: Iterable[nn.Parameter], lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8,
+                 weight_decay: float = 0.05, states: str = "fp32", master_weights: bool = False,
+                 bias_correction: bool = False, state: Optional[Dict[str, torch.Tensor]] = None):
+        if states not in _STATES:
+            raise ValueError(f"states={states!r}: expected one of {tuple(_STATES)}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or not eps >= 0.0:
+            raise ValueError(f"betas={betas}, eps={eps}: expected betas in [0, 1) and eps >= 0")
+        self.params: List[nn.Parameter] = [p for p in params if p.requires_grad]
+        if not self.params:
+            raise ValueError("no parameters to optimise")
+        self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.states, self.bias_correction = states, bias_correction
+        self.steps = 0
+        self.device = self.params[0].device
+        for p in self.params:
+            if p.device.type != "cuda" or p.device != self.device:
+                raise ValueError(f"FusedAdamW runs on one ROCm device; got parameters on {p.device} and {self.device}")
+            if p.dtype not in _DTYPE_CODE or not p.is_contiguous():
+                raise ValueError("parameters must be contiguous float32 or bfloat16 tensors; got "
+                                 f"{p.dtype}, shape {tuple(p.shape)}, strides {p.stride()}")
+        spans = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("parameters overlap in memory (one of them is given twice, or two share a storage)")
+        self._dtypes = [p.dtype for p in self.params]
+        self._numels = [p.numel() for p in self.params]
+        self.offsets: List[int] = []
+        at = 0
+        for n in self._numels:
+            self.offsets.append(at)
+            at += -(-n // BLOCK) * BLOCK
+        self.total = at
+        self.state = self._new_state(master_weights) if state is None else self._given_state(state, master_weights)
+        # p, g, n, offset, dtype of each parameter
+        self._table = array("q", [v for n, o, t in zip(self._numels, self.offsets, self._dtypes)
+                                  for v in (0, 0, n, o, _DTYPE_CODE[t])])
+
+    # ---- state -----------------------------------------------------------
+    def _specs(self, master: bool) -> Dict[str, Tuple[torch.dtype, int]]:
+        n = self.total
+        if self.states == "fp32":
+            specs = {"m": (torch.float32, n), "v": (torch.float32, n)}
+        else:
+            specs = {"m": (torch.int8, n), "v": (torch.uint8, n), "m_scale": (torch.float32, n // BLOCK),
+                     "v_scale": (torch.float32, n // BLOCK)}
+        if master:
+            specs["master"] = (torch.float32, n)
+        return specs
+
+    def _new_state(self, master: bool) -> Dict[str, torch.Tensor]:
+        state = {k: torch.zeros(n, dtype=t, device=self.device) for k, (t, n) in self._specs(master).items()}
+        if master:
+            with torch.no_grad():
+                torch._foreach_copy_(self.views(state["master"]), self.params)
+        return state
+
+    def _given_state(self, state: Dict[str, torch.Tensor], master: bool) -> Dict[str, torch.Tensor]:
+        specs = self._specs(master)
+        if set(state) != set(specs):
+            raise ValueError(f"state holds {sorted(state)}; expected {sorted(specs)}")
+        for k, (t, n) in specs.items():
+            s = state[k]
+            if (s.dtype != t or tuple(s.shape) != (n,) or s.device != self.device or not s.is_contiguous()
+                    or s.data_ptr() & 15):
+                raise ValueError(f"state[{k!r}] must be a contiguous 16-byte aligned {t} tensor of {n} elements on "
+                                 f"{self.device}; got {s.dtype}, shape {tuple(s.shape)} on {s.device}")
+        return dict(state)
+
+    def views(self, flat: torch.Tensor) -> List[torch.Tensor]:
+        """Each parameter's part of a buffer laid out as the moments."""
+        return [flat[o:o + n].view(p.shape) for p, o, n in zip(self.params, self.offsets, self._numels)]
+
+    def moments(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(m, v) as buffers of values (``views`` gives the parameters' parts): with
+        fp32 states the state's own buffers, in another dtype copies."""
+        m, v = self.state["m"], self.state["v"]
+        if self.states == "fp32":
+            return m.to(dtype), v.to(dtype)
+        if dtype not in _DTYPE_CODE:
+            raise ValueError(f"dtype {dtype} unsupported: use float32 or bfloat16")
+        mo = torch.empty(self.total, dtype=dtype, device=self.device)
+        vo = torch.empty_like(mo)
+        with _on(self.device):
+            _lib.check(_lib.load().kda_adamw_moments(
+                _ptr(m), _ptr(v), _ptr(self.state["m_scale"]), _ptr(self.state["v_scale"]), _ptr(mo), _ptr(vo),
+                self.total, _DTYPE_CODE[dtype], _stream(self.device)), "kda_adamw_moments")
+        return mo, vo
+
+    def state_dict(self) -> dict:
+        return {"steps": self.steps, **self.state}
+
+    def load_state_dict(self, state: dict) -> None:
+        """Copy a ``state_dict`` of an optimizer over the same tensors into this one's buffers."""
+        if set(state) != {"steps", *self.state}:
+            raise ValueError(f"state holds {sorted(state)}; expected {sorted(('steps', *self.state))}")
+        for k, t in self.state.items():
+            if state[k].dtype != t.dtype or state[k].shape != t.shape:
+                raise ValueError(f"state[{k!r}] is {state[k].dtype} {tuple(state[k].shape)}; expected {t.dtype} "
+                                 f"{tuple(t.shape)}")
+        for k, t in self.state.items():
+            t.copy_(state[k])
+        self.steps = int(state["steps"])
+
+    # ---- the step --------------------------------------------------------
+    def _tensors(self):
+        """(descriptors, count, gradients kept until the launch) of the parameters with a gradient."""
+        ps = self.params
+        if [p.dtype for p in ps] != self._dtypes or list(map(_numel, ps)) != self._numels or not all(map(_contiguous, ps)):
+            raise ValueError("a parameter's dtype, size or layout is not what the optimizer was made for")
+        gs = [p.grad for p in ps]
+        table, dtypes = self._table, self._dtypes
+        table[0::5] = array("q", map(_data_ptr, ps))
+        if any(g is None for g in gs):
+            keep = [i for i, g in enumerate(gs) if g is not None]
+            table = array("q", [v for i in keep for v in table[5 * i:5 * i + 5]])
+            gs, dtypes = [gs[i] for i in keep], [dtypes[i] for i in keep]
+        if [g.dtype for g in gs] != dtypes:
+            raise ValueError("a gradient's dtype is not its parameter's")
+        if not all(map(_contiguous, gs)):
+            gs = [g.contiguous() for g in gs]
+        table[1::5] = array("q", map(_data_ptr, gs))
+        return table, len(gs), gs
+
+    @torch.no_grad()
+    def step(self, max_norm: Optional[float] = None) -> Optional[torch.Tensor]:
+        """One update.  With ``max_norm`` the gradients count scaled by
+        min(max_norm / (G + 1e-6), 1), G their global norm, which is returned (0-d
+        fp32); the gradients themselves stay as they are."""
+        if max_norm is not None and not max_norm > 0.0:
+            raise ValueError(f"max_norm={max_norm}: expected a positive number or None")
+        table, count, gs = self._tensors()
+        self.steps += 1
+        b1, b2 = self.betas
+        c1 = 1.0 / (1.0 - b1 ** self.steps) if self.bias_correction else 1.0
+        c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
+        lib, st, at = _lib.load(), self.state, table.buffer_info()[0]
+        clip = None
+        with _on(self.device):
+            stream = _stream(self.device)
+            if max_norm is not None:
+                clip = torch.empty(2, dtype=torch.float32, device=self.device)
+                ws = torch.empty(max(lib.kda_grad_norm_workspace_size(at, count), 4), dtype=torch.uint8, device=self.device)
+                _lib.check(lib.kda_grad_norm(at, count, max_norm, _ptr(clip), _ptr(ws), ws.numel(), stream), "kda_grad_norm")
+            _lib.check(lib.kda_adamw_step(
+                at, count, _STATES[self.states], _ptr(st["m"]), _ptr(st["v"]), _ptr(st.get("m_scale")),
+                _ptr(st.get("v_scale")), _ptr(st.get("master")), _ptr(clip), self.lr, b1, b2, self.eps, self.weight_decay,
+                c1, c2, stream), "kda_adamw_step")
+        return None if clip is None else clip[0]
+
+    def zero_grad(self) -> None:
+        for p in self.params:
+            p.grad = None

@@ -23,6 +23,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .optim import FusedAdamW
+
 
 def cosine_warmup_lr(step: int, total_steps: int, warmup_steps: int, base_lr: float) -> float:
     if step < warmup_steps:
@@ -110,13 +112,24 @@ class TrainStep:
     reference sets it before each step, train_mlx_k400.py:427-429); without it
     the rate stays ``lr``.  ``ema`` (a ``checkpoint.ModelEMA``) is updated after
     every optimiser step (train_mlx_k400.py:440-441).  ``global_step`` starts at
-    ``step_offset`` and advances by one per call."""
+    ``step_offset`` and advances by one per call.
+
+    ``optimizer_states`` "fp32" or "int8" takes the clip and the update through
+    ``FusedAdamW`` with such moments (and, with ``master_weights``, fp32 copies of the
+    weights); None keeps ``AdamW``, whose moments have the parameters' dtype."""
 
     def __init__(self, model: nn.Module, lr: float = 3e-4, weight_decay: float = 0.05, betas=(0.9, 0.95),
                  grad_clip: float = 1.0, label_smoothing: float = 0.1, total_steps: Optional[int] = None,
-                 warmup_steps: int = 0, ema=None, step_offset: int = 0):
+                 warmup_steps: int = 0, ema=None, step_offset: int = 0, optimizer_states: Optional[str] = None,
+                 master_weights: bool = False):
         self.model = model
-        self.opt = AdamW(model.parameters(), lr=lr, betas=betas, weight_decay=weight_decay)
+        if optimizer_states is not None:
+            self.opt = FusedAdamW(model.parameters(), lr=lr, betas=betas, weight_decay=weight_decay,
+                                  states=optimizer_states, master_weights=master_weights)
+        elif master_weights:
+            raise ValueError("master_weights needs optimizer_states 'fp32' or 'int8'")
+        else:
+            self.opt = AdamW(model.parameters(), lr=lr, betas=betas, weight_decay=weight_decay)
         self.base_lr = lr
         self.grad_clip = grad_clip
         self.label_smoothing = label_smoothing
@@ -130,9 +143,12 @@ class TrainStep:
         self.opt.zero_grad()
         loss = loss_fn(self.model(video), target, self.label_smoothing)
         loss.backward()
-        if self.grad_clip > 0:
-            clip_grads_by_norm(self.opt.params, self.grad_clip)
-        self.opt.step()
+        if isinstance(self.opt, FusedAdamW):
+            self.opt.step(max_norm=self.grad_clip if self.grad_clip > 0 else None)
+        else:
+            if self.grad_clip > 0:
+                clip_grads_by_norm(self.opt.params, self.grad_clip)
+            self.opt.step()
         if self.ema is not None:
             self.ema.update(self.model)
         self.global_step += 1

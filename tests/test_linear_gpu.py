@@ -1,0 +1,316 @@
+"""linear_act and mlp against 64-bit formulas with a bound for every element
+(linear_reference): sizes that end inside a tile, rows of every alignment, one
+row to several tiles, each activation, dtype and optional operand; strided and
+expanded operands, frozen inputs, no rows, graph replays, finite differences."""
+import pytest
+import torch
+
+import linear_reference as L
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+# M, K, N
+SIZES = [(1, 8, 1), (1, 384, 174), (3, 5, 7), (17, 33, 19), (64, 40, 130), (65, 8, 8), (65, 7, 9), (128, 64, 128),
+         (129, 100, 257), (131, 31, 33), (200, 384, 520), (300, 772, 395), (257, 520, 136), (70, 1536, 384)]
+
+
+def _mk(seed, *shape, dt, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g)).to(dt).to(DEV)
+
+
+def _inputs(M, K, N, dt, bias=True, res=True, seed=0):
+    return (_mk(seed, M, K, dt=dt), _mk(seed + 1, N, K, dt=dt, scale=K ** -0.5),
+            _mk(seed + 2, N, dt=dt, scale=0.1) if bias else None, _mk(seed + 3, M, N, dt=dt) if res else None,
+            _mk(seed + 4, M, N, dt=dt))
+
+
+def _leaves(*ts):
+    for t in ts:
+        if t is not None:
+            t.requires_grad_(True)
+    return [t for t in ts if t is not None]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_linear_act_forward_and_gradients(size, dtype):
+    from mlx_vit_amd import linear_act
+    M, K, N = size
+    i = SIZES.index(size)
+    for act, bias, res in ((None, True, False), ("gelu", i % 3 != 0, i % 2 == 0), ("silu", i % 3 != 1, i % 2 == 1)):
+        print(size, dtype, act, bias, res, flush=True)
+        x, w, b, r, dy = _inputs(M, K, N, DT[dtype], bias, res, seed=10 * i)
+        want = L.linear_act(x, w, b, r, act, dy)
+        with torch.no_grad():
+            plain = linear_act(x, w, b, r, act)
+        L.check("y without gradients", plain, want["y"])
+        leaves = _leaves(x, w, b, r)
+        y = linear_act(x, w, b, r, act)
+        assert torch.equal(y, plain)
+        names = ["dx", "dw"] + ["db"] * (b is not None) + ["dr"] * (r is not None)
+        for n, g, leaf in zip(names, torch.autograd.grad(y, leaves, dy), leaves):
+            assert g.shape == leaf.shape and g.dtype == leaf.dtype
+            L.check(n, g, want[n])
+
+
+# M, K, hidden
+MLP_SIZES = [(1, 64, 128), (5, 9, 27), (64, 96, 384), (66, 72, 144), (130, 67, 201), (300, 384, 1536), (257, 128, 520)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("size", MLP_SIZES, ids=str)
+def test_mlp_forward_and_gradients(size, dtype):
+    from mlx_vit_amd import mlp
+    M, K, N = size
+    i, dt = MLP_SIZES.index(size), DT[dtype]
+    for act, res in (("gelu", i % 2 == 0), ("silu", i % 2 == 1), (None, True)):
+        print(size, dtype, act, res, flush=True)
+        x, w1, b1, _, _ = _inputs(M, K, N, dt, i % 4 != 3, False, seed=100 + 10 * i)
+        _, w2, b2, r, dy = _inputs(M, N, K, dt, i % 4 != 2, res, seed=500 + 10 * i)
+        want = L.mlp(x, w1, b1, w2, b2, r, act, dy)
+        with torch.no_grad():
+            plain = mlp(x, w1, b1, w2, b2, r, act)
+        leaves = _leaves(x, w1, b1, w2, b2, r)
+        y = mlp(x, w1, b1, w2, b2, r, act)
+        assert torch.equal(y, plain)
+        L.check("y", y, want["y"])
+        names = ["dx", "dw1"] + ["db1"] * (b1 is not None) + ["dw2"] + ["db2"] * (b2 is not None) + ["dr"] * (r is not None)
+        for n, g in zip(names, torch.autograd.grad(y, leaves, dy)):
+            L.check(n, g, want[n])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_strided_operands(dtype):
+    """Column slices, a transposed weight, a 3-d input, rows behind an offset of one
+    element, an expanded cotangent."""
+    from mlx_vit_amd import linear_act
+    dt = DT[dtype]
+    B, T, K, N = 3, 37, 72, 56
+    wide = _mk(1, B, T, 3 * K + 1, dt=dt)
+    wt = _mk(2, K, N, dt=dt, scale=K ** -0.5)
+    b, r = _mk(3, 2 * N, dt=dt)[::2], _mk(4, B, T, 2 * N, dt=dt)[..., N:]
+    for at in (0, 1, K):
+        x = wide[..., at:at + K]
+        want = L.linear_act(x.reshape(-1, K), wt.t(), b, r.reshape(-1, N), "gelu", torch.ones(B * T, N, dtype=dt))
+        leaves = [t.detach().requires_grad_(True) for t in (x, wt, b, r)]
+        y = linear_act(leaves[0], leaves[1].t(), leaves[2], leaves[3], "gelu")
+        assert y.shape == (B, T, N)
+        L.check("y", y.reshape(-1, N), want["y"])
+        dx, dwt, db, dr = torch.autograd.grad(y.sum(), leaves)     # its cotangent is one expanded element
+        L.check("dx", dx.reshape(-1, K), want["dx"])
+        L.check("dw", dwt.t(), want["dw"])
+        L.check("db", db, want["db"])
+        L.check("dr", dr.reshape(-1, N), want["dr"])
+    one = _mk(5, 1, K, dt=dt).expand(80, K)                        # rows at a stride of zero
+    L.check("expanded rows", linear_act(one, wt.t()), L.linear_act(one, wt.t(), None, None, None)["y"])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_shared_operands(dtype):
+    """x as its own residual, and one weight for both maps: the gradients add up."""
+    from mlx_vit_amd import mlp
+    dt = DT[dtype]
+    M, K = 90, 64
+    x, w, b, _, dy = _inputs(M, K, K, dt, True, False, seed=30)
+    want = L.mlp(x, w, b, w, b, x, "gelu", dy)
+    leaves = _leaves(x, w, b)
+    y = mlp(x, w, b, w, b, x, "gelu")
+    L.check("y", y, want["y"])
+    for n, g in zip(("x", "w", "b"), torch.autograd.grad(y, leaves, dy)):
+        parts = {"x": ("dx", "dr"), "w": ("dw1", "dw2"), "b": ("db1", "db2")}[n]
+        L.check(n, g, (want[parts[0]] + want[parts[1]]).round(dt))
+
+
+def test_frozen_inputs_get_no_gradient():
+    from mlx_vit_amd import linear_act, mlp
+    x, w, b, r, dy = _inputs(70, 64, 96, torch.bfloat16)
+    want = L.linear_act(x, w, b, r, "silu", dy)
+    for i, n in enumerate(("dx", "dw", "db", "dr")):
+        ts = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, w, b, r))]
+        linear_act(*ts, "silu").backward(dy)
+        assert [t.grad is not None for t in ts] == [i == j for j in range(4)]
+        L.check(n, ts[i].grad, want[n])
+    x, w1, b1, _, _ = _inputs(70, 64, 96, torch.bfloat16, seed=1)
+    _, w2, b2, r, dy = _inputs(70, 96, 64, torch.bfloat16, seed=2)
+    want = L.mlp(x, w1, b1, w2, b2, r, "gelu", dy)
+    for i, n in enumerate(("dx", "dw1", "db1", "dw2", "db2", "dr")):
+        ts = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, w1, b1, w2, b2, r))]
+        mlp(*ts, "gelu").backward(dy)
+        assert [t.grad is not None for t in ts] == [i == j for j in range(6)]
+        L.check(n, ts[i].grad, want[n])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_no_rows(dtype):
+    from mlx_vit_amd import linear_act, mlp
+    dt = DT[dtype]
+    x, w1, b1, _, _ = _inputs(0, 16, 24, dt, True, False)
+    _, w2, b2, r, dy = _inputs(0, 24, 16, dt)
+    leaves = _leaves(x, w1, b1, w2, b2, r)
+    for y, ls in ((mlp(x, w1, b1, w2, b2, r), leaves), (linear_act(x, w1, b1, None, "gelu"), leaves[:3])):
+        assert y.shape[0] == 0
+        for g, t in zip(torch.autograd.grad(y.sum(), ls), ls):
+            assert g.shape == t.shape and not g.any()
+
+
+def test_non_finite_values_stay_in_their_rows():
+    """A NaN or infinite row of x makes that row of y non-finite and no other, also
+    where the row ends inside a tile of the contracted index."""
+    from mlx_vit_amd import linear_act
+    for dt in (torch.bfloat16, torch.float32):
+        for M, K, N in ((70, 36, 40), (200, 136, 130), (9, 20, 24)):
+            x, w, b, r, _ = _inputs(M, K, N, dt, seed=7)
+            clean = linear_act(x, w, b, r, "gelu")
+            x[3, K - 1] = float("nan")
+            x[5, 0] = float("inf")
+            y = linear_act(x, w, b, r, "gelu")
+            rows = torch.ones(M, dtype=torch.bool, device=DEV)
+            rows[3] = rows[5] = False
+            assert y[3].isnan().all() and not y[5].isfinite().all()
+            assert torch.equal(y[rows], clean[rows])
+
+
+def test_gelu_over_its_range():
+    """Values from -40 to 40 through the epilogue and its derivative (K = 1)."""
+    from mlx_vit_amd import linear_act
+    for dt in (torch.bfloat16, torch.float32):
+        for act in ("gelu", "silu"):
+            x = torch.linspace(-40, 40, 4001, device=DEV).to(dt).unsqueeze(1).requires_grad_(True)
+            w = torch.ones(1, 1, dtype=dt, device=DEV)
+            want = L.linear_act(x, w, None, None, act, torch.ones(4001, 1, dtype=dt))
+            y = linear_act(x, w, None, None, act)
+            L.check("y", y, want["y"])
+            L.check("dx", torch.autograd.grad(y.sum(), x)[0], want["dx"])
+
+
+def test_gradients_against_differences():
+    """Central differences of sum(y dy) along a random direction of each input, fp32.
+    Truncation: h^2 / 6 times a third derivative of order the slope itself (h = 1/64:
+    4e-5); rounding: each y is off by at most 2^-24 of its terms' sum, some 2^-20,
+    and 90 x 48 of them of random sign add up to 66 * 2^-20 / (2 h) = 2e-3, against
+    slopes of order 66: 1e-3 relative to the largest slope covers both."""
+    from mlx_vit_amd import mlp
+    M, K, N = 90, 48, 80
+    x, w1, b1, _, _ = _inputs(M, K, N, torch.float32, True, False, seed=40)
+    _, w2, b2, r, dy = _inputs(M, N, K, torch.float32, seed=41)
+    ts = _leaves(x, w1, b1, w2, b2, r)
+    grads = torch.autograd.grad(mlp(*ts), ts, dy)
+    h = 2.0 ** -6
+    got, want = [], []
+    with torch.no_grad():
+        for i, t in enumerate(ts):
+            d = _mk(50 + i, *t.shape, dt=torch.float32)
+            d = d / d.norm() * 8
+            f = [(mlp(*[s + e * h * d if j == i else s for j, s in enumerate(ts)]).double() * dy.double()).sum().item()
+                 for e in (1, -1)]
+            want.append((f[0] - f[1]) / (2 * h))
+            got.append((grads[i].double() * d.double()).sum().item())
+    print("slopes", got, want, flush=True)
+    scale = max(abs(v) for v in want)
+    assert all(abs(a - b) <= 1e-3 * max(scale, 66.0) for a, b in zip(got, want))
+
+
+def test_second_derivative_is_refused():
+    from mlx_vit_amd import linear_act
+    x, w, b, r, dy = _inputs(5, 16, 8, torch.float32)
+    x.requires_grad_(True)
+    (g,) = torch.autograd.grad(linear_act(x, w, b, r, "gelu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_graph_replays(dtype):
+    """A captured inference pass and a captured training pass replay on new inputs,
+    the program's own eager work between the replays."""
+    from mlx_vit_amd import mlp
+    dt = DT[dtype]
+    for M in (9, 150):
+        x, w1, b1, _, _ = _inputs(M, 64, 132, dt, True, False, seed=60)
+        _, w2, b2, r, dy = _inputs(M, 132, 64, dt, seed=61)
+        ts = [t.detach().requires_grad_(True) for t in (x, w1, b1, w2, b2, r)]
+
+        def step():
+            y = mlp(*ts)
+            return [y.detach(), *torch.autograd.grad(y, ts, dy)]
+
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        for k in range(3):
+            with torch.no_grad():
+                ts[0].copy_(_mk(70 + k, M, 64, dt=dt))
+            g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, step()):
+                assert torch.equal(a, b)
+
+
+def test_other_stream():
+    from mlx_vit_amd import mlp
+    x, w1, b1, _, _ = _inputs(300, 64, 128, torch.bfloat16, True, False, seed=80)
+    _, w2, b2, r, dy = _inputs(300, 128, 64, torch.bfloat16, seed=81)
+    ref = mlp(x, w1, b1, w2, b2, r)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = mlp(x, w1, b1, w2, b2, r)
+    s.synchronize()
+    assert torch.equal(y, ref)
+
+
+def test_results_repeat_bit_for_bit():
+    from mlx_vit_amd import mlp
+    for dt in (torch.bfloat16, torch.float32):
+        x, w1, b1, _, _ = _inputs(1000, 96, 200, dt, True, False, seed=90)
+        _, w2, b2, r, dy = _inputs(1000, 200, 96, dt, seed=91)
+        ts = _leaves(x, w1, b1, w2, b2, r)
+        a, b = (torch.autograd.grad(mlp(*ts), ts, dy) for _ in range(2))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_blocks_mlp_as_one_operator():
+    """A block with ``set_fused_mlp`` against itself without: the separate modules round
+    the value before the activation and each map's result too.  And the cases that
+    keep the modules: dropout in training, a hook."""
+    from mlx_vit_amd import model as M
+    for dt in (torch.bfloat16, torch.float32):
+        torch.manual_seed(0)
+        blk = M.NoPEViTBlock(64, 2, 4.0, dropout=0.1).to(DEV).to(dt).eval()
+        x = _mk(1, 2, 50, 64, dt=dt).requires_grad_(True)
+        ps = [x, *blk.parameters()]
+        outs = []
+        for on in (False, True):
+            M.set_fused_mlp(blk, on)
+            y = blk(x)
+            outs.append([y, *torch.autograd.grad(y.float().square().sum(), ps)])
+        # relative to each tensor's norm: a few roundings of u, at random
+        tol = 8 * torch.finfo(dt).eps
+        for a, b in zip(*outs):
+            assert (a.double() - b.double()).norm() <= tol * b.double().norm()
+        calls = []
+        import mlx_vit_amd.model as mod
+        real, mod.mlp = mod.mlp, lambda *a, **k: calls.append(1) or real(*a, **k)
+        try:
+            blk(x)
+            assert calls == [1]
+            blk.train()
+            blk(x)
+            h = blk.eval().mlp[0].register_forward_hook(lambda *a: None)
+            blk(x)
+            h.remove()
+            assert calls == [1]
+            blk(x)
+            assert calls == [1, 1]
+        finally:
+            mod.mlp = real
