@@ -339,21 +339,31 @@ int kda_log_decay_bwd(const void* alpha, const float* dg, void* dalpha, int64_t 
 int kda_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
                    const void* residual, int64_t ld_r, void* y, int64_t ld_y, void* z, int64_t ld_z,
                    int M, int N, int K, int act, int dtype, void* stream);
-/* dx[m][k] = (sum_n dz[m][n] w[n][k]) * act'(z[m][k]), w [N][K]: the gradient of
- * a map's input, times the derivative of the activation that made that input
- * (act 0: none, z unused).  bf16: dz and w as x and w above. */
-int kda_linear_dgrad(const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, const void* z, int64_t ld_z,
-                     void* dx, int64_t ld_dx, int M, int N, int K, int act, int dtype, void* stream);
-/* fp32 weight and bias gradients dw[n][k] = sum_m dz[m][n] x[m][k], db[n] =
- * sum_m dz[m][n] (db may be NULL), dw and db contiguous, sums in a fixed order.
- * M >= 1; workspace: at least kda_linear_wgrad_workspace_size bytes, 16-byte
- * aligned.  bf16: kda_weight_grad. */
-size_t kda_linear_wgrad_workspace_size(int M, int N, int K);
-int kda_linear_wgrad(const float* dz, int64_t ld_dz, const float* x, int64_t ld_x, float* dw, float* db,
-                     int M, int N, int K, void* workspace, size_t ws_bytes, void* stream);
-/* dz[m][n] = dy[m][n] act'(z[m][n]), act 1 or 2 */
-int kda_linear_act_bwd(const void* dy, int64_t ld_dy, const void* z, int64_t ld_z, void* dz, int64_t ld_dz,
-                       int M, int N, int act, int dtype, void* stream);
+/* Copies of one or two bf16 matrices (the second's pointers may be NULL) as
+ * contiguous rows of cols rounded up to 8 elements, zero past cols: what x and w
+ * above have to be where they are not. */
+int kda_linear_pad(const void* src0, int64_t ld0, int rows0, int cols0, void* dst0,
+                   const void* src1, int64_t ld1, int rows1, int cols1, void* dst1, void* stream);
+/* The gradients of kda_linear_fwd from dy [M][N], with dz = dy act'(z):
+ *   dx = dz w,  dw[n][k] = sum_m dz[m][n] x[m][k],  db[n] = sum_m dz[m][n]
+ * (each may be NULL; db only with dw).  z as the forward wrote it (act 0:
+ * unused).  dw [N][K] and db [N] contiguous, sums in a fixed order.  bf16: x and
+ * w as for more than 64 rows above (the part of x that pads K is read and not
+ * used), dw 16-byte aligned where K is a multiple of 8.  M >= 1; workspace: at
+ * least kda_linear_bwd_workspace_size bytes, 16-byte aligned. */
+size_t kda_linear_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N, int K, int act, int dtype);
+int kda_linear_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                   const void* z, int64_t ld_z, void* dx, int64_t ld_dx, void* dw, void* db,
+                   int M, int N, int K, int act, int dtype, void* workspace, size_t ws_bytes, void* stream);
+/* The gradients of two maps in a row, h = act(z), z = x w1^T + b1 [M][N], y = h
+ * w2^T + b2 [M][O], from dy [M][O]: the activation's derivative is applied as
+ * dy w2 is stored, and both weight gradients are one launch (bf16).  Outputs may
+ * be NULL (a bias gradient only with its weight's); requirements as above. */
+size_t kda_mlp_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N, int K, int O, int act, int dtype);
+int kda_mlp_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* w1, int64_t ld_w1,
+                const void* z, int64_t ld_z, const void* h, int64_t ld_h, const void* w2, int64_t ld_w2,
+                void* dx, int64_t ld_dx, void* dw1, void* db1, void* dw2, void* db2,
+                int M, int N, int K, int O, int act, int dtype, void* workspace, size_t ws_bytes, void* stream);
 
 /* The update of a training step over many tensors (the reference's clip and
  * AdamW, train_mlx_k400.py:241-252, 548-549).  A tensor: its weights p and

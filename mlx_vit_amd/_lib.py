@@ -61,10 +61,11 @@ SIGNATURES = {
     "kda_log_decay_fwd": ([_P, _P, _L, _F, _I, _P], _I),
     "kda_log_decay_bwd": ([_P, _P, _P, _L, _F, _I, _P], _I),
     "kda_linear_fwd": ([_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _L] + [_I] * 5 + [_P], _I),
-    "kda_linear_dgrad": ([_P, _L] * 4 + [_I] * 5 + [_P], _I),
-    "kda_linear_wgrad_workspace_size": ([_I] * 3, _Z),
-    "kda_linear_wgrad": ([_P, _L, _P, _L, _P, _P] + [_I] * 3 + [_P, _Z, _P], _I),
-    "kda_linear_act_bwd": ([_P, _L] * 3 + [_I] * 4 + [_P], _I),
+    "kda_linear_pad": ([_P, _L, _I, _I, _P] * 2 + [_P], _I),
+    "kda_linear_bwd_workspace_size": ([_P, _L] + [_I] * 5, _Z),
+    "kda_linear_bwd": ([_P, _L] * 5 + [_P] * 2 + [_I] * 5 + [_P, _Z, _P], _I),
+    "kda_mlp_bwd_workspace_size": ([_P, _L] + [_I] * 6, _Z),
+    "kda_mlp_bwd": ([_P, _L] * 7 + [_P] * 4 + [_I] * 6 + [_P, _Z, _P], _I),
     "kda_grad_norm_workspace_size": ([_P, _I], _Z),
     "kda_grad_norm": ([_P, _I, _D, _P, _P, _Z, _P], _I),
     "kda_adamw_step": ([_P, _I, _I] + [_P] * 6 + [_D] * 7 + [_P], _I),

@@ -23,7 +23,7 @@ struct GemmArgs {
     int64_t lda, ldb, ldc, ldr, ldzi, ldzo;
     int M, N, K;
     int mt, nt;             // tiles
-    int vec;                // C, bias, res, zin, zout: groups of four columns are aligned, N % 4 == 0
+    int vec;                // C, bias, res, zin, zout: 16-byte accesses, N % 8 == 0 (wgrad's parts: N % 4)
     int vec_a, vec_b;       // fp32: rows of A, B can be read four floats at a time
     int splits, k_per;      // fp32 wgrad: parts of the contracted index, k_per (a multiple of the step) each
     float *part, *bpart;    // and their partial sums, [split][M][N] and [split][M]
@@ -33,50 +33,56 @@ struct GemmArgs {
 // activations: 0 none, 1 gelu (z Phi(z)), 2 silu (z sigma(z))
 // ----------------------------------------------------------------------------
 
-// Phi(z) and e^{-z^2/2}.  EXACT: the library's erf and exp.  Otherwise, for
-// results rounded to bf16, Phi(-|z|) = e^{-u^2} P(t) / 2, u = |z| / sqrt 2,
-// t = 1 / (1 + 0.3275911 u), Abramowitz & Stegun 7.1.26 (|error| of erf <=
-// 1.5e-7, 1 / 13000 of a bf16 half step of Phi near 1).
-template <bool EXACT>
-__device__ __forceinline__ float phi_exp(float z, float& e) {
-    if constexpr (EXACT) {
-        e = expf(-0.5f * z * z);
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    } else {
-        const float u = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.f));
-        e = __builtin_amdgcn_exp2f(-1.4426950408889634f * u * u);
-        float p = fmaf(1.061405429f, t, -1.453152027f);
-        p = fmaf(p, t, 1.421413741f);
-        p = fmaf(p, t, -0.284496736f);
-        p = fmaf(p, t, 0.254829592f);
-        const float tail = 0.5f * p * t * e;
-        return z >= 0.f ? 1.f - tail : tail;
-    }
+// Results rounded to bf16 (EXACT false) take fitted forms, because the epilogue
+// is VALU-bound with erf: 38.5 million values cost a 25088 x 1536 product 25 us
+// with Abramowitz & Stegun's 7.1.26 (25 issue slots a value, exp2 and rcp four
+// each) where the product's data need 20.
+//   gelu:  Phi(z) = 1 / (1 + 2^{-z R(z^2)}), R the minimax fit of log2(Phi / (1 -
+//          Phi)) / z up to |z| = 5 (18 slots): gelu is off by at most 4e-4 of its
+//          value, a tenth of a bf16 half step, and by 4e-7 below -5.
+//   gelu': 1/2 + z Q(t), t = 2 z^2 / 4.8^2 - 1, the minimax fit of an odd function up
+//          to |z| = 4.8 and its end beyond (14 slots): off by at most 3e-5.
+__device__ __forceinline__ float sigma_fast(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
 }
-template <bool EXACT>
-__device__ __forceinline__ float sigma(float z) {
-    if constexpr (EXACT) return 1.f / (1.f + expf(-z));
-    else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+__device__ __forceinline__ float gelu_fast(float z) {
+    const float s = fminf(z * z, 25.f);
+    float r = fmaf(-2.9020036e-08f, s, 2.0529139e-06f);
+    r = fmaf(r, s, -3.9314848e-05f);
+    r = fmaf(r, s, -8.4793003e-04f);
+    r = fmaf(r, s, 1.0687304e-01f);
+    r = fmaf(r, s, 2.3006303f);
+    return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z * r));
+}
+__device__ __forceinline__ float gelu_grad_fast(float z) {
+    // these minimum and maximum keep a NaN
+    const float c = __builtin_elementwise_maximum(__builtin_elementwise_minimum(z, 4.8f), -4.8f);
+    const float t = fmaf(c, c * 0.086805556f, -1.f);
+    float q = fmaf(2.4953399e-02f, t, -5.5430472e-02f);
+    q = fmaf(q, t, 3.6742341e-02f);
+    q = fmaf(q, t, -3.1934381e-02f);
+    q = fmaf(q, t, 7.8190073e-02f);
+    q = fmaf(q, t, -1.0049784e-01f);
+    q = fmaf(q, t, 8.8953942e-02f);
+    q = fmaf(q, t, -7.8604877e-02f);
+    q = fmaf(q, t, 7.3644958e-02f);
+    q = fmaf(q, t, -8.0312975e-02f);
+    q = fmaf(q, t, 1.4847238e-01f);
+    return fmaf(c, q, 0.5f);
 }
 template <int ACT, bool EXACT>
 __device__ __forceinline__ float act(float z) {
-    if constexpr (ACT == 1) {
-        float e;
-        return z * phi_exp<EXACT>(z, e);
-    } else if constexpr (ACT == 2) {
-        return z * sigma<EXACT>(z);
-    } else {
-        return z;
-    }
+    if constexpr (ACT == 1) return EXACT ? z * (0.5f * (1.f + erff(z * 0.70710678118654752f))) : gelu_fast(z);
+    else if constexpr (ACT == 2) return EXACT ? z / (1.f + expf(-z)) : z * sigma_fast(z);
+    else return z;
 }
 template <int ACT, bool EXACT>
 __device__ __forceinline__ float act_grad(float z) {
     if constexpr (ACT == 1) {
-        float e;
-        const float p = phi_exp<EXACT>(z, e);
-        return fmaf(z * e, 0.39894228040143268f, p);
+        if constexpr (!EXACT) return gelu_grad_fast(z);
+        return fmaf(z * expf(-0.5f * z * z), 0.39894228040143268f, 0.5f * (1.f + erff(z * 0.70710678118654752f)));
     } else if constexpr (ACT == 2) {
-        const float s = sigma<EXACT>(z);
+        const float s = EXACT ? 1.f / (1.f + expf(-z)) : sigma_fast(z);
         return s * fmaf(z, 1.f - s, 1.f);
     } else {
         return 1.f;
@@ -107,39 +113,106 @@ __device__ __forceinline__ void stc4(T* p, const float4& v, int n, bool vec) {
     if (n > 3) st1<T>(p + 3, v.w);
 }
 
-// The epilogue of four columns n..n+3 of row m: DG: times act'(zin) (zin null:
+// eight columns at p (n of them exist): vec: 16-byte accesses
+template <typename T>
+__device__ __forceinline__ void ldc8(const T* p, int n, bool vec, float (&v)[8]) {
+    if (vec) {
+        if constexpr (std::is_same<T, float>::value) {
+            const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+            v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+        } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(p);
+            v[0] = bf_lo(x.x); v[1] = bf_hi(x.x); v[2] = bf_lo(x.y); v[3] = bf_hi(x.y);
+            v[4] = bf_lo(x.z); v[5] = bf_hi(x.z); v[6] = bf_lo(x.w); v[7] = bf_hi(x.w);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? ld1<T>(p + e) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void stc8(T* p, const float (&v)[8], int n, bool vec) {
+    if (vec) {
+        if constexpr (std::is_same<T, float>::value) {
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            *reinterpret_cast<uint4*>(p) =
+                make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) st1<T>(p + e, v[e]);
+}
+
+// The epilogue of eight columns n..n+7 of row m.  DG: times act'(zin) (zin null:
 // nothing); else bias, z out, activation, residual
 template <typename T, int ACT, bool DG, bool EXACT>
-__device__ __forceinline__ void finish4(const GemmArgs& a, int m, int n, f32x4 acc, const float4& bias) {
+__device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (&v)[8], const float (&bias)[8]) {
     const int left = a.N - n;
     const bool vec = a.vec;
-    float4 v = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    float t[8];
     if constexpr (DG) {
         if constexpr (ACT != 0) {
-            const float4 z = ldc4<T>(static_cast<const T*>(a.zin) + (size_t)m * a.ldzi + n, left, vec);
-            v.x *= act_grad<ACT, EXACT>(z.x);
-            v.y *= act_grad<ACT, EXACT>(z.y);
-            v.z *= act_grad<ACT, EXACT>(z.z);
-            v.w *= act_grad<ACT, EXACT>(z.w);
+            ldc8<T>(static_cast<const T*>(a.zin) + (size_t)m * a.ldzi + n, left, vec, t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= act_grad<ACT, EXACT>(t[e]);
         }
     } else {
-        v.x += bias.x; v.y += bias.y; v.z += bias.z; v.w += bias.w;
-        if (a.zout) stc4<T>(static_cast<T*>(a.zout) + (size_t)m * a.ldzo + n, v, left, vec);
-        v.x = act<ACT, EXACT>(v.x);
-        v.y = act<ACT, EXACT>(v.y);
-        v.z = act<ACT, EXACT>(v.z);
-        v.w = act<ACT, EXACT>(v.w);
-        if (a.res) {
-            const float4 r = ldc4<T>(static_cast<const T*>(a.res) + (size_t)m * a.ldr + n, left, vec);
-            v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
-        }
+        if (a.res) ldc8<T>(static_cast<const T*>(a.res) + (size_t)m * a.ldr + n, left, vec, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += bias[e];
+        if (a.zout) stc8<T>(static_cast<T*>(a.zout) + (size_t)m * a.ldzo + n, v, left, vec);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = act<ACT, EXACT>(v[e]);
+        if (a.res)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += t[e];
     }
-    stc4<T>(static_cast<T*>(a.c) + (size_t)m * a.ldc + n, v, left, vec);
+    stc8<T>(static_cast<T*>(a.c) + (size_t)m * a.ldc + n, v, left, vec);
 }
 template <typename T, bool DG>
-__device__ __forceinline__ float4 bias4(const GemmArgs& a, int n) {
-    if (DG || !a.bias || n >= a.N) return make_float4(0.f, 0.f, 0.f, 0.f);
-    return ldc4<T>(static_cast<const T*>(a.bias) + n, a.N - n, a.vec);
+__device__ __forceinline__ void bias8(const GemmArgs& a, int n, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (!DG && a.bias && n < a.N) ldc8<T>(static_cast<const T*>(a.bias) + n, a.N - n, a.vec, v);
+}
+
+// The epilogue of a wave's 64 columns from n0 and 16 FM rows from m0, 32 rows at a
+// time through 8 KB of LDS of its own: the accumulators hold four columns of 16
+// rows a fragment, and leave as whole 128-byte (bf16) rows of 16-byte pieces.
+// Rows of 64 floats, the 16-byte piece c of row r at c ^ (r & 15), so that both
+// the fragments' writes (16 rows of a piece) and the reads are spread over the
+// banks.  acc[i][j]: columns 16 i, rows 16 j.
+template <typename T, int ACT, bool DG, bool EXACT, int FM>
+__device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, const f32x4 (&acc)[4][FM], char* lds) {
+    const int l = lane_id(), r16 = l & 15, g4 = l >> 4, q = l & 7;
+    const int n = n0 + 8 * q;
+    float bias[8];
+    bias8<T, DG>(a, n, bias);
+#pragma unroll
+    for (int h = 0; h < FM; h += 2) {
+        wave_sync();   // the last part's reads come first
+#pragma unroll
+        for (int j = h; j < h + 2; ++j) {
+            const int r = 16 * (j - h) + r16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(lds + 256 * r + (((4 * i + g4) ^ r16) << 4)) = acc[i][j];
+        }
+        wave_sync();
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const int r = 8 * it + (l >> 3), m = m0 + 16 * h + r;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(lds + 256 * r + (((2 * q) ^ (r & 15)) << 4));
+            const f32x4 y = *reinterpret_cast<const f32x4*>(lds + 256 * r + (((2 * q + 1) ^ (r & 15)) << 4));
+            float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            if (m < a.M && n < a.N) finish8<T, ACT, DG, EXACT>(a, m, n, v, bias);
+        }
+    }
 }
 
 // tile (mi, ni) of block bid: each XCD takes a run of consecutive tiles, ordered
@@ -163,7 +236,7 @@ template <int RB>
 __device__ __forceinline__ int key_k(int r) {
     return RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
-__device__ __forceinline__ int key_t(int r) { return ((r & 3) << 1) | (r & 8); }
+__device__ __forceinline__ int key_t(int r) { return ((r & 3) << 1) | (r & 8); }   // 16 chunks at least
 
 template <int RB>
 __device__ __forceinline__ bf16x8 frag_k(const char* tile, int row0, int chunk) {
@@ -312,17 +385,8 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_bf16_kernel(const 
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j], acc[i][j], 0, 0, 0);
         }
     }
-    // B's fragment first: a lane holds four consecutive columns n of one row m
-#pragma unroll
-    for (int i = 0; i < FN; ++i) {
-        const int n = n0 + wn + 16 * i + 4 * g4;
-        const float4 bias = bias4<uint16_t, DG>(a, n);
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int m = m0 + wm + 16 * j + r16;
-            if (m < a.M && n < a.N) finish4<uint16_t, ACT, DG, false>(a, m, n, acc[i][j], bias);
-        }
-    }
+    lds_barrier();   // every wave has read the last step
+    finish_wave<uint16_t, ACT, DG, false, FM>(a, m0 + wm, n0 + wn, acc, lds + 8192 * w);
 }
 
 // ----------------------------------------------------------------------------
@@ -477,16 +541,8 @@ __global__ __launch_bounds__(256, 2) void kda_linear_f32_kernel(const GemmArgs a
             }
         }
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = n0 + wn + 16 * i + 4 * g4;
-            const float4 bias = bias4<float, DG>(a, n);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int m = m0 + wm + 16 * j + r16;
-                if (m < a.M && n < a.N) finish4<float, ACT, DG, true>(a, m, n, acc[i][j], bias);
-            }
-        }
+        lds_barrier();
+        finish_wave<float, ACT, DG, true, 4>(a, m0 + wm, n0 + wn, acc, lds + 8192 * w);
     }
 }
 
@@ -519,7 +575,7 @@ __device__ __forceinline__ bf16x8 row8(const uint16_t* row, int k, int K, bool v
     return __builtin_bit_cast(bf16x8, v);
 }
 
-constexpr int FEW_WAVES = 8;
+constexpr int FEW_WAVES = 8, FEW_ROWS = 64;
 
 // 16 rows x 16 columns a workgroup; wave w takes steps w, w + 8, ... of the
 // contracted index (32 of bf16, 16 of fp32) and the partial tiles meet in LDS
@@ -550,41 +606,78 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const Ge
     }
     part[w][l] = acc;
     __syncthreads();
-    if (w != 0) return;
+    if (threadIdx.x >= 32) return;
+    // row m, columns n..n+7: two lanes' pieces of each wave
+    const int r = threadIdx.x >> 1, c = 2 * (threadIdx.x & 1);
+    f32x4 x = part[0][16 * c + r], y = part[0][16 * (c + 1) + r];
 #pragma unroll
-    for (int i = 1; i < FEW_WAVES; ++i) acc += part[i][l];
-    const int m = m0 + r16, n = n0 + 4 * g4;
-    if (m < a.M && n < a.N)
-        finish4<T, ACT, false, std::is_same<T, float>::value>(a, m, n, acc, bias4<T, false>(a, n));
+    for (int i = 1; i < FEW_WAVES; ++i) {
+        x += part[i][16 * c + r];
+        y += part[i][16 * (c + 1) + r];
+    }
+    const int m = m0 + r, n = n0 + 4 * c;
+    if (m >= a.M || n >= a.N) return;
+    float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, bias[8];
+    bias8<T, false>(a, n, bias);
+    finish8<T, ACT, false, std::is_same<T, float>::value>(a, m, n, v, bias);
 }
 
-// dz = dy act'(z)
+// dz = dy act'(z) (ACT 0: dy), rows of ld_dz elements whose columns from N to the
+// next multiple of eight are zero
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ z,
                                                                  T* __restrict__ dz, int64_t ld_dy, int64_t ld_z,
-                                                                 int64_t ld_dz, int M, int N, int vec) {
+                                                                 int64_t ld_dz, int M, int N, int vec_in) {
     constexpr bool EXACT = std::is_same<T, float>::value;
-    const int groups = (N + 3) / 4;
+    const int groups = (N + 7) / 8;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)M * groups; i += (size_t)gridDim.x * 256) {
-        const int m = (int)(i / groups), n = 4 * (int)(i - (size_t)m * groups), left = N - n;
-        const float4 g = ldc4<T>(dy + (size_t)m * ld_dy + n, left, vec), x = ldc4<T>(z + (size_t)m * ld_z + n, left, vec);
-        stc4<T>(dz + (size_t)m * ld_dz + n,
-                make_float4(g.x * act_grad<ACT, EXACT>(x.x), g.y * act_grad<ACT, EXACT>(x.y),
-                            g.z * act_grad<ACT, EXACT>(x.z), g.w * act_grad<ACT, EXACT>(x.w)),
-                left, vec);
+        const int m = (int)(i / groups), n = 8 * (int)(i - (size_t)m * groups), left = N - n;
+        float g[8], x[8];
+        ldc8<T>(dy + (size_t)m * ld_dy + n, left, vec_in, g);
+        if constexpr (ACT != 0) {
+            ldc8<T>(z + (size_t)m * ld_z + n, left, vec_in, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] *= act_grad<ACT, EXACT>(x[e]);
+        }
+        stc8<T>(dz + (size_t)m * ld_dz + n, g, 8, true);
     }
+}
+
+// one or two matrices copied into rows of a multiple of eight columns, zero past theirs
+struct PadArgs {
+    const uint16_t* src[2];
+    uint16_t* dst[2];
+    int64_t ld[2];
+    int rows[2], cols[2];
+};
+__global__ __launch_bounds__(256) void kda_linear_pad_kernel(const PadArgs a) {
+    const int j = blockIdx.y, groups = (a.cols[j] + 7) / 8;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)a.rows[j] * groups; i += (size_t)gridDim.x * 256) {
+        const int m = (int)(i / groups), n = 8 * (int)(i - (size_t)m * groups);
+        float v[8];
+        ldc8<uint16_t>(a.src[j] + (size_t)m * a.ld[j] + n, a.cols[j] - n, false, v);
+        stc8<uint16_t>(a.dst[j] + 8 * i, v, 8, true);
+    }
+}
+
+// the first K columns of rows of ld elements, as contiguous rows
+__global__ __launch_bounds__(256) void kda_linear_compact_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
+                                                                 int64_t ld, int K, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256)
+        dst[i] = src[i / K * ld + i % K];
 }
 
 // ----------------------------------------------------------------------------
 // launches
 // ----------------------------------------------------------------------------
+// rows that can be read and written 16 bytes at a time
 bool groups_ok(const void* p, int64_t ld, int es) {
-    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % (4 * es) == 0 && ld % 4 == 0);
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (16 / es) == 0);
 }
 
 template <bool BT, int ACT, bool DG>
 hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
-    constexpr int BM = 128, BN = 128, BK = 32, NST = 4, WR = 2, WC = 2;
+    constexpr int BM = 128, BN = 128, BK = 64, NST = 2, WR = 4, WC = 2;
     constexpr size_t LDS = (size_t)NST * (BM + BN) * 2 * BK;
     a.mt = (a.M + BM - 1) / BM;
     a.nt = (a.N + BN - 1) / BN;
@@ -595,7 +688,7 @@ hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
 
 template <int ACT>
 hipError_t launch_fwd(GemmArgs& a, int bf16, hipStream_t st) {
-    if (a.M <= 64) {
+    if (a.M <= FEW_ROWS) {
         a.nt = (a.N + 15) / 16;
         a.mt = (a.M + 15) / 16;
         const dim3 grid((unsigned)a.mt * a.nt), block(64 * FEW_WAVES);
@@ -621,18 +714,25 @@ hipError_t launch_dgrad(GemmArgs& a, int bf16, hipStream_t st) {
     return hipGetLastError();
 }
 
+hipError_t dgrad(int act, int bf16, GemmArgs& a, hipStream_t st) {
+    return act == 1 ? launch_dgrad<1>(a, bf16, st) : act == 2 ? launch_dgrad<2>(a, bf16, st) : launch_dgrad<0>(a, bf16, st);
+}
+
 template <typename T>
 hipError_t launch_act_bwd(const void* dy, const void* z, void* dz, int64_t ld_dy, int64_t ld_z, int64_t ld_dz, int M, int N,
-                          int act, int vec, hipStream_t st) {
-    const size_t n = (size_t)M * ((N + 3) / 4);
+                          int act, hipStream_t st) {
+    constexpr int ES = sizeof(T);
+    const size_t n = (size_t)M * ((N + 7) / 8);
+    const int vec = N % 8 == 0 && groups_ok(dy, ld_dy, ES) && groups_ok(act ? z : nullptr, ld_z, ES);
     const dim3 grid((unsigned)std::min<size_t>((n + 255) / 256, 4096)), block(256);
     const T *pdy = static_cast<const T*>(dy), *pz = static_cast<const T*>(z);
+    T* pdz = static_cast<T*>(dz);
     if (act == 1)
-        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 1>), grid, block, 0, st, pdy, pz, static_cast<T*>(dz), ld_dy, ld_z,
-                           ld_dz, M, N, vec);
+        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 1>), grid, block, 0, st, pdy, pz, pdz, ld_dy, ld_z, ld_dz, M, N, vec);
+    else if (act == 2)
+        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 2>), grid, block, 0, st, pdy, pz, pdz, ld_dy, ld_z, ld_dz, M, N, vec);
     else
-        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 2>), grid, block, 0, st, pdy, pz, static_cast<T*>(dz), ld_dy, ld_z,
-                           ld_dz, M, N, vec);
+        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 0>), grid, block, 0, st, pdy, pz, pdz, ld_dy, ld_z, ld_dz, M, N, vec);
     return hipGetLastError();
 }
 
@@ -645,6 +745,107 @@ void wgrad_plan(int M, int N, int K, int* splits, int* per) {
     *splits = (M + *per - 1) / *per;
 }
 
+// a matrix: pointer, row stride, columns
+struct Mat {
+    const void* p;
+    int64_t ld;
+    int n;
+};
+// the weight gradient dw [n][k] (and db [n]) of one map
+struct Wgrad {
+    Mat dz, x;
+    void *dw, *db;
+};
+
+int64_t up8(int64_t n) { return (n + 7) & ~(int64_t)7; }
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// rows that the LDS DMA can read: 16-byte aligned, whole pieces
+bool dma_ok(const Mat& m) { return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0 && m.n % 8 == 0; }
+
+// bytes of `count` gradients' partial sums and padded results
+size_t wgrads_bytes(const Wgrad* g, int count, int M, int bf16) {
+    size_t n = 0;
+    if (bf16) {
+        WgradProblem q[2] = {};
+        for (int j = 0; j < count; ++j) {
+            q[j] = WgradProblem{g[j].dz.p, g[j].x.p, g[j].dw, g[j].db, g[j].dz.ld, g[j].x.ld, g[j].dz.n, up8(g[j].x.n)};
+            if (g[j].x.n % 8 != 0) n += up256((size_t)g[j].dz.n * up8(g[j].x.n) * 2);
+        }
+        return n + up256(wgrad_ws_floats(q, count, M) * sizeof(float));
+    }
+    for (int j = 0; j < count; ++j) {
+        int splits, per;
+        wgrad_plan(M, g[j].dz.n, g[j].x.n, &splits, &per);
+        n = std::max(n, up256(((size_t)splits * g[j].dz.n * (g[j].x.n + 1)) * sizeof(float)));
+    }
+    return n;
+}
+
+hipError_t wgrad_f32(const Wgrad& g, int M, char* ws, hipStream_t st) {
+    const int N = g.dz.n, K = g.x.n;
+    GemmArgs a = {};   // C[n][k] = sum_m A[m][n] B[m][k]
+    a.a = g.dz.p; a.b = g.x.p;
+    a.lda = g.dz.ld; a.ldb = g.x.ld;
+    a.M = N; a.N = K; a.K = M;
+    a.mt = (N + 127) / 128;
+    a.nt = (K + 127) / 128;
+    wgrad_plan(M, N, K, &a.splits, &a.k_per);
+    a.part = reinterpret_cast<float*>(ws);
+    float* bpart = a.part + (size_t)a.splits * N * K;
+    a.bpart = g.db ? bpart : nullptr;
+    a.vec = K % 4 == 0;
+    a.vec_a = reinterpret_cast<uintptr_t>(a.a) % 16 == 0 && a.lda % 4 == 0;
+    a.vec_b = reinterpret_cast<uintptr_t>(a.b) % 16 == 0 && a.ldb % 4 == 0;
+    hipLaunchKernelGGL((kda_linear_f32_kernel<true, true, 0, false, true>), dim3((unsigned)(a.mt * a.nt * a.splits)),
+                       dim3(256), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const size_t total = (size_t)N * K + N;
+    hipLaunchKernelGGL(kda_linear_sum_parts_kernel, dim3((unsigned)std::min<size_t>((total + 255) / 256, 4096)), dim3(256), 0,
+                       st, a.part, bpart, static_cast<float*>(g.dw), static_cast<float*>(g.db), (size_t)N * K, N, a.splits);
+    return hipGetLastError();
+}
+
+hipError_t wgrads(const Wgrad* g, int count, int M, int bf16, char* ws, hipStream_t st) {
+    if (count == 0) return hipSuccess;
+    hipError_t e = hipSuccess;
+    if (!bf16) {
+        for (int j = 0; j < count && e == hipSuccess; ++j) e = wgrad_f32(g[j], M, ws, st);
+        return e;
+    }
+    WgradProblem q[2];
+    for (int j = 0; j < count; ++j) {
+        const int64_t k = up8(g[j].x.n);
+        q[j] = WgradProblem{g[j].dz.p, g[j].x.p, g[j].dw, g[j].db, g[j].dz.ld, g[j].x.ld, g[j].dz.n, k};
+        if (k != g[j].x.n) {
+            q[j].dw = ws;
+            ws += up256((size_t)g[j].dz.n * k * 2);
+        }
+    }
+    e = launch_wgrad(q, count, M, reinterpret_cast<float*>(ws), st);
+    for (int j = 0; j < count && e == hipSuccess; ++j)
+        if (q[j].dw != g[j].dw) {
+            const size_t n = (size_t)g[j].dz.n * g[j].x.n;
+            hipLaunchKernelGGL(kda_linear_compact_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 2048)), dim3(256), 0,
+                               st, static_cast<const uint16_t*>(q[j].dw), static_cast<uint16_t*>(g[j].dw), q[j].k, g[j].x.n, n);
+            e = hipGetLastError();
+        }
+    return e;
+}
+
+// dx = dz w (* act'(z))
+GemmArgs dgrad_args(const Mat& dz, const Mat& w, const void* z, int64_t ld_z, void* dx, int64_t ld_dx, int M, int es) {
+    GemmArgs a = {};   // C[m][k] = sum_n A[m][n] B[n][k]
+    a.a = dz.p; a.b = w.p; a.c = dx; a.zin = z;
+    a.lda = dz.ld; a.ldb = w.ld; a.ldc = ld_dx; a.ldzi = ld_z;
+    a.M = M; a.N = w.n; a.K = dz.n;
+    a.vec = w.n % 8 == 0 && groups_ok(dx, ld_dx, es) && groups_ok(z, ld_z, es);
+    a.vec_a = reinterpret_cast<uintptr_t>(a.a) % 16 == 0 && a.lda % 4 == 0;
+    a.vec_b = reinterpret_cast<uintptr_t>(a.b) % 16 == 0 && a.ldb % 4 == 0;
+    return a;
+}
+
 int check_map(int M, int N, int K, int act, int dtype) {
     if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_BF16)
         return api_fail(KDA_E_UNSUPPORTED, "dtype=%d: expected 0 (fp32) or 1 (bf16)", dtype);
@@ -652,9 +853,9 @@ int check_map(int M, int N, int K, int act, int dtype) {
         return api_fail(KDA_E_UNSUPPORTED, "act=%d: expected 0 (none), 1 (gelu) or 2 (silu)", act);
     if (M < 0 || N < 1 || K < 1 || N > (1 << 20) || K > (1 << 20))
         return api_fail(KDA_E_INVALID, "M=%d N=%d K=%d: expected M >= 0, N and K from 1 to 2^20", M, N, K);
-    // tiles of 128 x 128 by 256 threads: below 2^32 threads
-    if (((int64_t)M + 127) / 128 * ((std::max(N, K) + 127) / 128) > (1 << 23))
-        return api_fail(KDA_E_UNSUPPORTED, "M=%d N=%d K=%d: more than 2^23 tiles of 128 x 128", M, N, K);
+    // tiles of 64 x 128 by at most 512 threads: below 2^32 threads
+    if (((int64_t)M + 63) / 64 * ((std::max(N, K) + 127) / 128) > (1 << 22))
+        return api_fail(KDA_E_UNSUPPORTED, "M=%d N=%d K=%d: more than 2^22 tiles of 64 x 128", M, N, K);
     return KDA_OK;
 }
 
@@ -664,12 +865,19 @@ int check_rows(const void* p, const char* name, int64_t ld, int cols, int dtype,
     if (!p) return api_fail(KDA_E_INVALID, "%s is NULL", name);
     if (reinterpret_cast<uintptr_t>(p) % (dma ? 16 : es) != 0)
         return api_fail(KDA_E_INVALID, "%s is not %d-byte aligned", name, dma ? 16 : es);
-    if (ld < (dma ? (cols + 7) & ~7 : cols) || ld > (1 << 21) || (dma && ld % 8 != 0))
+    if (ld < (dma ? up8(cols) : cols) || ld > (1 << 21) || (dma && ld % 8 != 0))
         return api_fail(KDA_E_INVALID, "%s: row stride %lld for %d columns", name, (long long)ld, cols);
     return KDA_OK;
 }
 int check_opt(const void* p, const char* name, int64_t ld, int cols, int dtype) {
     return p ? check_rows(p, name, ld, cols, dtype, false) : KDA_OK;
+}
+int check_ws(const void* ws, size_t have, size_t need) {
+    if (need == 0) return KDA_OK;
+    if (!ws || reinterpret_cast<uintptr_t>(ws) % 16 != 0)
+        return api_fail(KDA_E_INVALID, "workspace is NULL or not 16-byte aligned");
+    if (have < need) return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", have, need);
+    return KDA_OK;
 }
 
 #define LIN_TRY(x)                       \
@@ -677,6 +885,27 @@ int check_opt(const void* p, const char* name, int64_t ld, int cols, int dtype) 
         const int rc_ = (x);             \
         if (rc_ != KDA_OK) return rc_;   \
     } while (0)
+#define LIN_HIP(x, what)                                       \
+    do {                                                       \
+        const hipError_t e_ = (x);                             \
+        if (e_ != hipSuccess) return api_hip_fail(e_, what);   \
+    } while (0)
+
+// dz's bytes in the workspace: where an activation's derivative is applied, or dy cannot be read as it is
+size_t dz_bytes(const Mat& dy, int M, int act, int bf16) {
+    return act || (bf16 && !dma_ok(dy)) ? up256((size_t)M * up8(dy.n) * (bf16 ? 2 : 4)) : 0;
+}
+// dy act'(z) as dz_bytes' part of the workspace, or dy itself
+hipError_t make_dz(Mat* dy, const void* z, int64_t ld_z, int M, int act, int bf16, char** ws, hipStream_t st) {
+    const size_t n = dz_bytes(*dy, M, act, bf16);
+    if (n == 0) return hipSuccess;
+    const Mat dz = {*ws, up8(dy->n), dy->n};
+    const hipError_t e = bf16 ? launch_act_bwd<uint16_t>(dy->p, z, *ws, dy->ld, ld_z, dz.ld, M, dy->n, act, st)
+                              : launch_act_bwd<float>(dy->p, z, *ws, dy->ld, ld_z, dz.ld, M, dy->n, act, st);
+    *ws += n;
+    *dy = dz;
+    return e;
+}
 
 }  // namespace
 
@@ -692,7 +921,7 @@ int kda_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, con
     LIN_TRY(check_map(M, N, K, act, dtype));
     if (M == 0) return KDA_OK;
     const int es = dtype == KDA_DTYPE_BF16 ? 2 : 4;
-    const bool dma = dtype == KDA_DTYPE_BF16 && M > 64;
+    const bool dma = dtype == KDA_DTYPE_BF16 && M > FEW_ROWS;
     LIN_TRY(check_rows(x, "x", ld_x, K, dtype, dma));
     LIN_TRY(check_rows(w, "w", ld_w, K, dtype, dma));
     LIN_TRY(check_opt(bias, "bias", N, N, dtype));
@@ -703,98 +932,146 @@ int kda_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, con
     a.a = x; a.b = w; a.c = y; a.bias = bias; a.res = residual; a.zout = z;
     a.lda = ld_x; a.ldb = ld_w; a.ldc = ld_y; a.ldr = ld_r; a.ldzo = ld_z;
     a.M = M; a.N = N; a.K = K;
-    a.vec = N % 4 == 0 && groups_ok(y, ld_y, es) && groups_ok(bias, 0, es) && groups_ok(residual, ld_r, es) && groups_ok(z, ld_z, es);
-    const int row = es == 2 ? 8 : 4;   // elements of a 16-byte read
-    a.vec_a = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x % row == 0;
-    a.vec_b = reinterpret_cast<uintptr_t>(w) % 16 == 0 && ld_w % row == 0;
+    a.vec = N % 8 == 0 && groups_ok(y, ld_y, es) && groups_ok(bias, 0, es) && groups_ok(residual, ld_r, es) && groups_ok(z, ld_z, es);
+    a.vec_a = groups_ok(x, ld_x, es);
+    a.vec_b = groups_ok(w, ld_w, es);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const hipError_t e = act == 1   ? launch_fwd<1>(a, es == 2, st)
-                         : act == 2 ? launch_fwd<2>(a, es == 2, st)
-                                    : launch_fwd<0>(a, es == 2, st);
-    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_linear_fwd");
+    LIN_HIP(act == 1   ? launch_fwd<1>(a, es == 2, st)
+            : act == 2 ? launch_fwd<2>(a, es == 2, st)
+                       : launch_fwd<0>(a, es == 2, st),
+            "kda_linear_fwd");
+    return KDA_OK;
 }
 
-int kda_linear_dgrad(const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, const void* z, int64_t ld_z, void* dx,
-                     int64_t ld_dx, int M, int N, int K, int act, int dtype, void* stream) {
+int kda_linear_pad(const void* src0, int64_t ld0, int rows0, int cols0, void* dst0, const void* src1, int64_t ld1, int rows1,
+                   int cols1, void* dst1, void* stream) {
+    PadArgs a = {};
+    const void* src[2] = {src0, src1};
+    void* dst[2] = {dst0, dst1};
+    const int64_t ld[2] = {ld0, ld1};
+    const int rows[2] = {rows0, rows1}, cols[2] = {cols0, cols1};
+    int n = 0;
+    size_t most = 0;
+    for (int j = 0; j < 2; ++j) {
+        if (!src[j] && !dst[j]) continue;
+        if (rows[j] < 0 || cols[j] < 1 || cols[j] > (1 << 20)) return api_fail(KDA_E_INVALID, "matrix %d: %d x %d", j, rows[j], cols[j]);
+        LIN_TRY(check_rows(src[j], "src", ld[j], cols[j], KDA_DTYPE_BF16, false));
+        if (!dst[j] || reinterpret_cast<uintptr_t>(dst[j]) % 16 != 0)
+            return api_fail(KDA_E_INVALID, "dst is NULL or not 16-byte aligned");
+        a.src[n] = static_cast<const uint16_t*>(src[j]);
+        a.dst[n] = static_cast<uint16_t*>(dst[j]);
+        a.ld[n] = ld[j];
+        a.rows[n] = rows[j];
+        a.cols[n] = cols[j];
+        most = std::max(most, (size_t)rows[j] * ((cols[j] + 7) / 8));
+        ++n;
+    }
+    if (n == 0 || most == 0) return KDA_OK;
+    hipLaunchKernelGGL(kda_linear_pad_kernel, dim3((unsigned)std::min<size_t>((most + 255) / 256, 4096), n), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), a);
+    LIN_HIP(hipGetLastError(), "kda_linear_pad");
+    return KDA_OK;
+}
+
+size_t kda_linear_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N, int K, int act, int dtype) {
+    if (check_map(M, N, K, act, dtype) != KDA_OK || M == 0) return 0;
+    const int bf16 = dtype == KDA_DTYPE_BF16;
+    const Mat d = {dy, ld_dy, N};
+    const Wgrad g = {d, {nullptr, up8(K), K}, nullptr, const_cast<void*>(dy)};
+    return dz_bytes(d, M, act, bf16) + wgrads_bytes(&g, 1, M, bf16);
+}
+
+int kda_linear_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* z,
+                   int64_t ld_z, void* dx, int64_t ld_dx, void* dw, void* db, int M, int N, int K, int act, int dtype,
+                   void* workspace, size_t ws_bytes, void* stream) {
     LIN_TRY(check_map(M, N, K, act, dtype));
-    if (M == 0) return KDA_OK;
-    const int es = dtype == KDA_DTYPE_BF16 ? 2 : 4;
-    const bool dma = dtype == KDA_DTYPE_BF16;
-    LIN_TRY(check_rows(dz, "dz", ld_dz, N, dtype, dma));
-    LIN_TRY(check_rows(w, "w", ld_w, K, dtype, dma));
-    LIN_TRY(check_rows(dx, "dx", ld_dx, K, dtype, false));
-    if (act != KDA_ACT_NONE) LIN_TRY(check_rows(z, "z", ld_z, K, dtype, false));
-    GemmArgs a = {};   // C[m][k] = sum_n A[m][n] B[n][k]
-    a.a = dz; a.b = w; a.c = dx; a.zin = act != KDA_ACT_NONE ? z : nullptr;
-    a.lda = ld_dz; a.ldb = ld_w; a.ldc = ld_dx; a.ldzi = ld_z;
-    a.M = M; a.N = K; a.K = N;
-    a.vec = K % 4 == 0 && groups_ok(dx, ld_dx, es) && groups_ok(a.zin, ld_z, es);
-    a.vec_a = reinterpret_cast<uintptr_t>(dz) % 16 == 0 && ld_dz % 4 == 0;
-    a.vec_b = reinterpret_cast<uintptr_t>(w) % 16 == 0 && ld_w % 4 == 0;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const hipError_t e = act == 1   ? launch_dgrad<1>(a, es == 2, st)
-                         : act == 2 ? launch_dgrad<2>(a, es == 2, st)
-                                    : launch_dgrad<0>(a, es == 2, st);
-    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_linear_dgrad");
-}
-
-size_t kda_linear_wgrad_workspace_size(int M, int N, int K) {
-    if (M < 1 || N < 1 || K < 1 || N > (1 << 20) || K > (1 << 20)) return 0;
-    int splits, per;
-    wgrad_plan(M, N, K, &splits, &per);
-    return ((size_t)splits * N * K + (size_t)splits * N) * sizeof(float);
-}
-
-int kda_linear_wgrad(const float* dz, int64_t ld_dz, const float* x, int64_t ld_x, float* dw, float* db, int M, int N, int K,
-                     void* workspace, size_t ws_bytes, void* stream) {
-    LIN_TRY(check_map(M, N, K, KDA_ACT_NONE, KDA_DTYPE_F32));
     if (M < 1) return api_fail(KDA_E_INVALID, "M=%d: expected at least one row", M);
-    LIN_TRY(check_rows(dz, "dz", ld_dz, N, KDA_DTYPE_F32, false));
-    LIN_TRY(check_rows(x, "x", ld_x, K, KDA_DTYPE_F32, false));
-    LIN_TRY(check_rows(dw, "dw", K, K, KDA_DTYPE_F32, false));
-    const size_t need = kda_linear_wgrad_workspace_size(M, N, K);
-    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
-        return api_fail(KDA_E_INVALID, "workspace is NULL or not 16-byte aligned");
-    if (ws_bytes < need) return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, need);
-    GemmArgs a = {};   // C[n][k] = sum_m A[m][n] B[m][k]
-    a.a = dz; a.b = x;
-    a.lda = ld_dz; a.ldb = ld_x;
-    a.M = N; a.N = K; a.K = M;
-    a.mt = (N + 127) / 128;
-    a.nt = (K + 127) / 128;
-    wgrad_plan(M, N, K, &a.splits, &a.k_per);
-    a.part = static_cast<float*>(workspace);
-    float* bpart = a.part + (size_t)a.splits * N * K;
-    a.bpart = db ? bpart : nullptr;
-    a.vec = K % 4 == 0;
-    a.vec_a = reinterpret_cast<uintptr_t>(dz) % 16 == 0 && ld_dz % 4 == 0;
-    a.vec_b = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x % 4 == 0;
+    const int bf16 = dtype == KDA_DTYPE_BF16, es = bf16 ? 2 : 4;
+    LIN_TRY(check_rows(dy, "dy", ld_dy, N, dtype, false));
+    if (act) LIN_TRY(check_rows(z, "z", ld_z, N, dtype, false));
+    if (dx) {
+        LIN_TRY(check_rows(w, "w", ld_w, K, dtype, bf16));
+        LIN_TRY(check_rows(dx, "dx", ld_dx, K, dtype, false));
+    }
+    if (dw) {
+        LIN_TRY(check_rows(x, "x", ld_x, K, dtype, bf16));
+        LIN_TRY(check_rows(dw, "dw", K, K, dtype, bf16 && K % 8 == 0));
+    } else if (db) {
+        return api_fail(KDA_E_INVALID, "db without dw");
+    }
+    LIN_TRY(check_ws(workspace, ws_bytes, kda_linear_bwd_workspace_size(dy, ld_dy, M, N, K, act, dtype)));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL((kda_linear_f32_kernel<true, true, 0, false, true>), dim3((unsigned)(a.mt * a.nt * a.splits)),
-                       dim3(256), 0, st, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return api_hip_fail(e, "kda_linear_wgrad");
-    const size_t total = (size_t)N * K + N;
-    hipLaunchKernelGGL(kda_linear_sum_parts_kernel, dim3((unsigned)std::min<size_t>((total + 255) / 256, 4096)), dim3(256), 0,
-                       st, a.part, bpart, dw, db, (size_t)N * K, N, a.splits);
-    e = hipGetLastError();
-    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_linear_wgrad");
+    char* ws = static_cast<char*>(workspace);
+    Mat dz = {dy, ld_dy, N};
+    LIN_HIP(make_dz(&dz, z, ld_z, M, act, bf16, &ws, st), "kda_linear_bwd");
+    if (dx) {
+        GemmArgs a = dgrad_args(dz, {w, ld_w, K}, nullptr, 0, dx, ld_dx, M, es);
+        LIN_HIP(dgrad(0, bf16, a, st), "kda_linear_bwd");
+    }
+    const Wgrad g = {dz, {x, ld_x, K}, dw, db};
+    LIN_HIP(wgrads(&g, dw ? 1 : 0, M, bf16, ws, st), "kda_linear_bwd");
+    return KDA_OK;
 }
 
-int kda_linear_act_bwd(const void* dy, int64_t ld_dy, const void* z, int64_t ld_z, void* dz, int64_t ld_dz, int M, int N,
-                       int act, int dtype, void* stream) {
-    LIN_TRY(check_map(M, N, 1, act, dtype));
-    if (act == KDA_ACT_NONE) return api_fail(KDA_E_UNSUPPORTED, "act=0 has no gradient kernel");
-    if (M == 0) return KDA_OK;
-    LIN_TRY(check_rows(dy, "dy", ld_dy, N, dtype, false));
-    LIN_TRY(check_rows(z, "z", ld_z, N, dtype, false));
-    LIN_TRY(check_rows(dz, "dz", ld_dz, N, dtype, false));
-    const int es = dtype == KDA_DTYPE_BF16 ? 2 : 4;
-    const int vec = N % 4 == 0 && groups_ok(dy, ld_dy, es) && groups_ok(z, ld_z, es) && groups_ok(dz, ld_dz, es);
+size_t kda_mlp_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N, int K, int O, int act, int dtype) {
+    if (check_map(M, N, K, act, dtype) != KDA_OK || check_map(M, O, N, act, dtype) != KDA_OK || M == 0) return 0;
+    const int bf16 = dtype == KDA_DTYPE_BF16;
+    const Mat d = {dy, ld_dy, O}, d1 = {nullptr, up8(N), N};
+    void* b = const_cast<void*>(dy);
+    const Wgrad g[2] = {{d, {nullptr, up8(N), N}, nullptr, b}, {d1, {nullptr, up8(K), K}, nullptr, b}};
+    size_t one = wgrads_bytes(g, 2, M, bf16);
+    for (int j = 0; j < 2; ++j) one = std::max(one, wgrads_bytes(g + j, 1, M, bf16));
+    return dz_bytes(d, M, 0, bf16) + up256((size_t)M * up8(N) * (bf16 ? 2 : 4)) + one;
+}
+
+int kda_mlp_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* w1, int64_t ld_w1, const void* z,
+                int64_t ld_z, const void* h, int64_t ld_h, const void* w2, int64_t ld_w2, void* dx, int64_t ld_dx, void* dw1,
+                void* db1, void* dw2, void* db2, int M, int N, int K, int O, int act, int dtype, void* workspace,
+                size_t ws_bytes, void* stream) {
+    LIN_TRY(check_map(M, N, K, act, dtype));
+    LIN_TRY(check_map(M, O, N, act, dtype));
+    if (M < 1) return api_fail(KDA_E_INVALID, "M=%d: expected at least one row", M);
+    const int bf16 = dtype == KDA_DTYPE_BF16, es = bf16 ? 2 : 4;
+    const bool first = dx || dw1;
+    LIN_TRY(check_rows(dy, "dy", ld_dy, O, dtype, false));
+    if (first) {
+        LIN_TRY(check_rows(w2, "w2", ld_w2, N, dtype, bf16));
+        if (act) LIN_TRY(check_rows(z, "z", ld_z, N, dtype, false));
+    }
+    if (dx) {
+        LIN_TRY(check_rows(w1, "w1", ld_w1, K, dtype, bf16));
+        LIN_TRY(check_rows(dx, "dx", ld_dx, K, dtype, false));
+    }
+    if (dw1) {
+        LIN_TRY(check_rows(x, "x", ld_x, K, dtype, bf16));
+        LIN_TRY(check_rows(dw1, "dw1", K, K, dtype, bf16 && K % 8 == 0));
+    }
+    if (dw2) {
+        LIN_TRY(check_rows(h, "h", ld_h, N, dtype, bf16));
+        LIN_TRY(check_rows(dw2, "dw2", N, N, dtype, bf16 && N % 8 == 0));
+    }
+    if ((db1 && !dw1) || (db2 && !dw2)) return api_fail(KDA_E_INVALID, "a bias gradient without its weight's");
+    LIN_TRY(check_ws(workspace, ws_bytes, kda_mlp_bwd_workspace_size(dy, ld_dy, M, N, K, O, act, dtype)));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const hipError_t e = es == 2 ? launch_act_bwd<uint16_t>(dy, z, dz, ld_dy, ld_z, ld_dz, M, N, act, vec, st)
-                                 : launch_act_bwd<float>(dy, z, dz, ld_dy, ld_z, ld_dz, M, N, act, vec, st);
-    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_linear_act_bwd");
+    char* ws = static_cast<char*>(workspace);
+    Mat d2 = {dy, ld_dy, O};
+    LIN_HIP(make_dz(&d2, nullptr, 0, M, 0, bf16, &ws, st), "kda_mlp_bwd");
+    const Mat d1 = {ws, up8(N), N};
+    if (first) {   // dz1 = (dy w2) act'(z)
+        GemmArgs a = dgrad_args(d2, {w2, ld_w2, N}, act ? z : nullptr, ld_z, ws, d1.ld, M, es);
+        LIN_HIP(dgrad(act, bf16, a, st), "kda_mlp_bwd");
+        ws += up256((size_t)M * d1.ld * es);
+    }
+    if (dx) {
+        GemmArgs a = dgrad_args(d1, {w1, ld_w1, K}, nullptr, 0, dx, ld_dx, M, es);
+        LIN_HIP(dgrad(0, bf16, a, st), "kda_mlp_bwd");
+    }
+    Wgrad g[2];
+    int count = 0;
+    if (dw1) g[count++] = Wgrad{d1, {x, ld_x, K}, dw1, db1};
+    if (dw2) g[count++] = Wgrad{d2, {h, ld_h, N}, dw2, db2};
+    LIN_HIP(wgrads(g, count, M, bf16, ws, st), "kda_mlp_bwd");
+    return KDA_OK;
 }
 
 }  // extern "C"

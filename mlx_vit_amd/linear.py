@@ -30,12 +30,13 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kda import _DTYPE_CODE, _ptr, _stream
+from .kda import _DTYPE_CODE
 
 ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2}
 FEW_ROWS = 64        # up to here a forward's operands may have any alignment (kda_linear_fwd)
 MAX_STRIDE = 1 << 21
 _NULL = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _on(dev: torch.device):
@@ -43,138 +44,104 @@ def _on(dev: torch.device):
     return _NULL if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _padded(M: int, n: int, like: torch.Tensor) -> torch.Tensor:
-    """An (M, n) matrix whose rows begin on 16 bytes and can be read in whole
-    16-byte pieces (n rounded up to 8)."""
-    return torch.empty((M, -(-n // 8) * 8), dtype=like.dtype, device=like.device)[:, :n]
+def _up8(n: int) -> int:
+    return -(-n // 8) * 8
 
 
-def _mat(t: torch.Tensor, dma: bool) -> torch.Tensor:
-    """t (M, n) as the kernels read it: rows at an even stride, with ``dma`` as
-    ``_padded`` lays them out; a copy where it is not."""
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t (M, n) with unit column stride and rows at an even stride; a copy where it is not."""
     M, n = t.shape
-    if (n > 1 and t.stride(1) != 1) or (M > 1 and not n <= t.stride(0) <= MAX_STRIDE):
-        t = t.contiguous()
-    if dma and (t.data_ptr() & 15 or n & 7 or (M > 1 and t.stride(0) & 7)):
-        return _padded(M, n, t).copy_(t)
+    s0, s1 = t.stride()
+    if (n > 1 and s1 != 1) or (M > 1 and not n <= s0 <= MAX_STRIDE):
+        return t.contiguous()
     return t
 
 
 def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
+    return t.stride(0) if t.shape[0] > 1 else _up8(t.shape[1])
 
 
-def _forward(x2: torch.Tensor, w: torch.Tensor, bias, res2, act: int, want_z: bool, pad: bool = False):
-    """(y, z or None, x2, w) of matrices x2 (M, K), w (N, K): the last two as the
-    kernel read them.  pad: y and z with rows as ``_padded`` lays them out."""
-    M, K = x2.shape
-    N = w.shape[0]
-    code = _DTYPE_CODE[x2.dtype]
-    dma = code == 1 and M > FEW_ROWS
-    x2, w = _mat(x2, dma), _mat(w, dma)
-    new = _padded if pad else lambda m, n, like: torch.empty((m, n), dtype=like.dtype, device=like.device)
-    y = new(M, N, x2)
-    z = new(M, N, x2) if want_z else None
+def _whole(t: torch.Tensor) -> bool:
+    """Rows begin on 16 bytes and are whole 16-byte pieces."""
+    return not (t.shape[1] & 7 or t.data_ptr() & 15 or (t.shape[0] > 1 and t.stride(0) & 7))
+
+
+def _whole_rows(x: torch.Tensor, w: torch.Tensor, stream: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16 matrices as the tiles' DMA reads them: copies, in one launch, of those
+    that are not, their columns rounded up to 8."""
+    jobs, out = [], [x, w]
+    for i, t in enumerate((x, w)):
+        if not _whole(t):
+            M, n = t.shape
+            out[i] = torch.empty((M, _up8(n)), dtype=t.dtype, device=t.device)
+            jobs += [t.data_ptr(), _ld(t), M, n, out[i].data_ptr()]
+    if jobs:
+        jobs += [None, 0, 0, 0, None] * (2 - len(jobs) // 5)
+        _lib.check(_lib.load().kda_linear_pad(*jobs, stream), "kda_linear_pad")
+    return out[0], out[1]
+
+
+def _forward(x2: torch.Tensor, K: int, w: torch.Tensor, bias, res2, act: int, y: torch.Tensor,
+             z: Optional[torch.Tensor], train: bool):
+    """y <- act(x2 w^T + bias) + res2 for x2 (M, K or wider), w (N, K), y and z (M, N
+    or wider).  Returns x2 and w as the kernels read them, with ``train`` also the
+    backward's."""
+    M, N = x2.shape[0], w.shape[0]
+    code = _DTYPE_CODE[w.dtype]
+    stream = _raw_stream(w.device.index)
+    x2, w = _rows(x2), _rows(w)
+    if code and (train or M > FEW_ROWS):
+        x2, w = _whole_rows(x2, w, stream)
     if M:
-        if bias is not None:
+        if bias is not None and not bias.is_contiguous():
             bias = bias.contiguous()
         if res2 is not None:
-            res2 = _mat(res2, False)
+            res2 = _rows(res2)
         rc = _lib.load().kda_linear_fwd(
-            _ptr(x2), _ld(x2), _ptr(w), _ld(w), _ptr(bias), _ptr(res2), 0 if res2 is None else _ld(res2), _ptr(y), _ld(y),
-            _ptr(z), 0 if z is None else _ld(z), M, N, K, act, code, _stream(x2.device))
-        _lib.check(rc, "kda_linear_fwd")
-    return y, z, x2, w
-
-
-def _dgrad(dz: torch.Tensor, w: torch.Tensor, z: Optional[torch.Tensor], act: int, pad: bool = False) -> torch.Tensor:
-    """(dz w) * act'(z) for dz (M, N), w (N, K)."""
-    M, N = dz.shape
-    K = w.shape[1]
-    code = _DTYPE_CODE[dz.dtype]
-    dz, w = _mat(dz, code == 1), _mat(w, code == 1)
-    dx = _padded(M, K, dz) if pad else torch.empty((M, K), dtype=dz.dtype, device=dz.device)
-    rc = _lib.load().kda_linear_dgrad(_ptr(dz), _ld(dz), _ptr(w), _ld(w), _ptr(z) if act else None, _ld(z) if act else 0,
-                                      _ptr(dx), _ld(dx), M, N, K, act, code, _stream(dz.device))
-    _lib.check(rc, "kda_linear_dgrad")
-    return dx
-
-
-def _act_bwd(dy: torch.Tensor, z: torch.Tensor, act: int) -> torch.Tensor:
-    M, N = dy.shape
-    dz = _padded(M, N, dy)
-    dy = _mat(dy, False)
-    rc = _lib.load().kda_linear_act_bwd(_ptr(dy), _ld(dy), _ptr(z), _ld(z), _ptr(dz), _ld(dz), M, N, act,
-                                        _DTYPE_CODE[dy.dtype], _stream(dy.device))
-    _lib.check(rc, "kda_linear_act_bwd")
-    return dz
-
-
-def _wgrad(problems, M: int):
-    """[(dw, db or None)] for each (dz (M, N), x (M, K), bias)."""
-    dev = problems[0][0].device
-    if M == 0:
-        z = dict(dtype=problems[0][0].dtype, device=dev)
-        return [(torch.zeros((d.shape[1], x.shape[1]), **z), torch.zeros(d.shape[1], **z) if b else None)
-                for d, x, b in problems]
-    if problems[0][0].dtype == torch.bfloat16:
-        from .layer import weight_grads
-        wide, ks = [], []
-        for d, x, b in problems:
-            k = x.shape[1]
-            ks.append(k)
-            if k & 7:   # rows of whole 16-byte pieces: the columns past k give columns of dw that are left out
-                x = _mat(x, True)
-                x = x.as_strided((M, -(-k // 8) * 8), (_ld(x), 1))
-            wide.append((d, x, b))
-        return [(dw if dw.shape[1] == k else dw[:, :k].contiguous(), db) for (dw, db), k in zip(weight_grads(wide, M), ks)]
-    out = []
-    lib = _lib.load()
-    for d, x, b in problems:
-        d, x = _mat(d, False), _mat(x, False)
-        N, K = d.shape[1], x.shape[1]
-        dw = torch.empty((N, K), dtype=torch.float32, device=dev)
-        db = torch.empty((N,), dtype=torch.float32, device=dev) if b else None
-        ws = torch.empty(lib.kda_linear_wgrad_workspace_size(M, N, K), dtype=torch.uint8, device=dev)
-        rc = lib.kda_linear_wgrad(_ptr(d), _ld(d), _ptr(x), _ld(x), _ptr(dw), _ptr(db), M, N, K, _ptr(ws), ws.numel(),
-                                  _stream(dev))
-        _lib.check(rc, "kda_linear_wgrad")
-        out.append((dw, db))
-    return out
+            x2.data_ptr(), _ld(x2), w.data_ptr(), _ld(w), None if bias is None else bias.data_ptr(),
+            None if res2 is None else res2.data_ptr(), 0 if res2 is None else _ld(res2), y.data_ptr(), y.stride(0),
+            None if z is None else z.data_ptr(), 0 if z is None else z.stride(0), M, N, K, act, code, stream)
+        if rc:
+            _lib.check(rc, "kda_linear_fwd")
+    return x2, w
 
 
 def _check(what: str, x: torch.Tensor, maps, residual: Optional[torch.Tensor], activation) -> int:
     """Validate x (..., K), the maps' (weight, bias) in turn and the residual;
     returns the activation's code."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation, -1)
+    if act < 0:
         raise ValueError(f"{what}: activation={activation!r}: expected one of {tuple(ACTIVATIONS)}")
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: x must be a torch.Tensor")
-    if x.dtype not in _DTYPE_CODE:
-        raise ValueError(f"{what}: x dtype {x.dtype} unsupported: use float32 or bfloat16")
-    if x.dim() < 1:
-        raise ValueError(f"{what}: x must be (..., K); got shape {tuple(x.shape)}")
-    n, named = x.shape[-1], []
-    for i, (w, b) in enumerate(maps):
-        tag = str(i + 1) if len(maps) > 1 else ""
-        if w.dim() != 2 or w.shape[1] != n or w.shape[0] < 1 or n < 1:
-            raise ValueError(f"{what}: weight{tag} shape {tuple(w.shape)} does not take {n} columns")
-        n = w.shape[0]
-        if b is not None and tuple(b.shape) != (n,):
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    if dtype not in _DTYPE_CODE:
+        raise ValueError(f"{what}: x dtype {dtype} unsupported: use float32 or bfloat16")
+    if len(shape) < 1:
+        raise ValueError(f"{what}: x must be (..., K); got shape {tuple(shape)}")
+    n = shape[-1]
+    named = []
+    for w, b in maps:
+        ws = w.shape
+        if len(ws) != 2 or ws[1] != n or ws[0] < 1 or n < 1:
+            tag = str(len(named) // 2 + 1) if len(maps) > 1 else ""
+            raise ValueError(f"{what}: weight{tag} shape {tuple(ws)} does not take {n} columns")
+        n = ws[0]
+        if b is not None and b.shape != (n,):
+            tag = str(len(named) // 2 + 1) if len(maps) > 1 else ""
             raise ValueError(f"{what}: bias{tag} shape {tuple(b.shape)} != {(n,)}")
-        named += [("weight" + tag, w), ("bias" + tag, b)]
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], n):
-        raise ValueError(f"{what}: residual shape {tuple(residual.shape)} != {(*x.shape[:-1], n)}")
-    for name, t in (*named, ("residual", residual)):
-        if t is None:
-            continue
-        if t.dtype != x.dtype:
-            raise ValueError(f"{what}: {name} has dtype {t.dtype}; expected {x.dtype}")
-        if t.device != x.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
-    if x.device.type != "cuda":
-        raise ValueError(f"{what} runs on a ROCm device; got tensors on {x.device}")
-    return ACTIVATIONS[activation]
+        named += (w, b)
+    if residual is not None and (residual.shape[-1:] != (n,) or residual.shape[:-1] != shape[:-1]):
+        raise ValueError(f"{what}: residual shape {tuple(residual.shape)} != {(*shape[:-1], n)}")
+    for i, t in enumerate((*named, residual)):
+        if t is not None and (t.dtype != dtype or t.device != dev):
+            name = "residual" if i == len(named) else ("weight", "bias")[i & 1] + (str(i // 2 + 1) if len(maps) > 1 else "")
+            if t.dtype != dtype:
+                raise ValueError(f"{what}: {name} has dtype {t.dtype}; expected {dtype}")
+            raise ValueError(f"{what}: {name} is on {t.device}, x on {dev}")
+    if dev.type != "cuda":
+        raise ValueError(f"{what} runs on a ROCm device; got tensors on {dev}")
+    return act
 
 
 def _needs_grad(*tensors) -> bool:
@@ -182,7 +149,20 @@ def _needs_grad(*tensors) -> bool:
 
 
 def _flat(t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
-    return None if t is None else t.reshape(-1, n)
+    return t if t is None or t.dim() == 2 else t.reshape(-1, n)
+
+
+def _new(like: torch.Tensor, *shape) -> torch.Tensor:
+    return torch.empty(shape, dtype=like.dtype, device=like.device)
+
+
+def _out(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _zeros(like: torch.Tensor, *wanted):
+    """Gradients over no rows: (shape, whether it is wanted)."""
+    return [like.new_zeros(shape) if need else None for shape, need in wanted]
 
 
 class LinearActFunction(torch.autograd.Function):
@@ -193,31 +173,41 @@ class LinearActFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         N, K = weight.shape
         with _on(x.device):
-            y, z, x2, w = _forward(_flat(x, K), weight, bias, _flat(residual, N), act, bool(act))
+            x2 = _flat(x, K)
+            M = x2.shape[0]
+            y = _new(x, *x.shape[:-1], N)
+            z = _new(x, M, _up8(N)) if act else None
+            x2, w = _forward(x2, K, weight, bias, _flat(residual, N), act, y.view(M, N), z, True)
         ctx.save_for_backward(x2, w, z)
-        ctx.act, ctx.bias, ctx.shape = act, bias is not None, x.shape
-        return y.view(*x.shape[:-1], N)
+        ctx.act, ctx.shape, ctx.N = act, x.shape, N
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x2, w, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        M, N = x2.shape[0], w.shape[0]
+        act, N, K, M = ctx.act, ctx.N, ctx.shape[-1], x2.shape[0]
         dx = dw = db = None
-        with _on(x2.device):
-            if M == 0:
-                dx = x2.new_zeros(ctx.shape) if need_x else None
-                if need_w or need_b:
-                    ((dw, db),) = _wgrad([(dy.reshape(M, N), x2, ctx.bias)], M)
-            elif need_x or need_w or need_b:
-                dz = dy.reshape(M, N)
-                dz = _act_bwd(dz, z, ctx.act) if ctx.act else _mat(dz, dz.dtype == torch.bfloat16)
+        if M == 0:
+            dx, dw, db = _zeros(x2, (ctx.shape, need_x), ((N, K), need_w), ((N,), need_b))
+        elif need_x or need_w or need_b:
+            with _on(x2.device):
+                d = _rows(_flat(dy, N))
                 if need_x:
-                    dx = _dgrad(dz, w, None, 0).view(ctx.shape)
+                    dx = _new(x2, *ctx.shape)
                 if need_w or need_b:
-                    ((dw, db),) = _wgrad([(dz, x2, ctx.bias and need_b)], M)
-        return dx, dw if need_w else None, db if need_b else None, dy if need_r else None, None
+                    dw = _new(x2, N, K)
+                    db = _new(x2, N) if need_b else None
+                lib, code, pd, ld = _lib.load(), _DTYPE_CODE[x2.dtype], d.data_ptr(), _ld(d)
+                n = lib.kda_linear_bwd_workspace_size(pd, ld, M, N, K, act, code)
+                ws = torch.empty(n, dtype=torch.uint8, device=x2.device)
+                rc = lib.kda_linear_bwd(pd, ld, x2.data_ptr(), _ld(x2), w.data_ptr(), _ld(w), _out(z),
+                                        z.stride(0) if act else 0, _out(dx), K, _out(dw), _out(db), M, N, K, act, code,
+                                        ws.data_ptr(), n, _raw_stream(x2.device.index))
+                if rc:
+                    _lib.check(rc, "kda_linear_bwd")
+        return dx, dw if need_w else None, db, dy if need_r else None, None
 
 
 class MLPFunction(torch.autograd.Function):
@@ -226,44 +216,49 @@ class MLPFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w1, b1, w2, b2, residual, act):
-        N, K = w1.shape
-        out = w2.shape[0]
+        (N, K), O = w1.shape, w2.shape[0]
         with _on(x.device):
-            h, z, x2, w1 = _forward(_flat(x, K), w1, b1, None, act, bool(act), pad=True)
-            y, _, _, w2 = _forward(h, w2, b2, _flat(residual, out), 0, False)
+            x2 = _flat(x, K)
+            M = x2.shape[0]
+            h = _new(x, M, _up8(N))
+            z = _new(x, M, _up8(N)) if act else None
+            y = _new(x, *x.shape[:-1], O)
+            x2, w1 = _forward(x2, K, w1, b1, None, act, h, z, True)
+            h, w2 = _forward(h, N, w2, b2, _flat(residual, O), 0, y.view(M, O), None, True)
         ctx.save_for_backward(x2, w1, z, h, w2)
-        ctx.act, ctx.biases, ctx.shape = act, (b1 is not None, b2 is not None), x.shape
-        return y.view(*x.shape[:-1], out)
+        ctx.act, ctx.shape, ctx.sizes = act, x.shape, (N, O)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x2, w1, z, h, w2 = ctx.saved_tensors
         need_x, need_w1, need_b1, need_w2, need_b2, need_r = ctx.needs_input_grad[:6]
-        M, out = x2.shape[0], w2.shape[0]
+        act, (N, O), K, M = ctx.act, ctx.sizes, ctx.shape[-1], x2.shape[0]
         dx = dw1 = db1 = dw2 = db2 = None
-        with _on(x2.device):
-            dy2 = dy.reshape(M, out)
-            first, second = need_w1 or need_b1, need_w2 or need_b2
-            problems = []
-            if M == 0:
-                dx = x2.new_zeros(ctx.shape) if need_x else None
-                dz = x2.new_zeros((0, w1.shape[0]))
-            else:
-                dy2 = _mat(dy2, dy2.dtype == torch.bfloat16)
-                if need_x or first:
-                    dz = _dgrad(dy2, w2, z, ctx.act, pad=True)
+        if M == 0:
+            dx, dw1, db1, dw2, db2 = _zeros(x2, (ctx.shape, need_x), ((N, K), need_w1), ((N,), need_b1),
+                                            ((O, N), need_w2), ((O,), need_b2))
+        elif need_x or need_w1 or need_b1 or need_w2 or need_b2:
+            with _on(x2.device):
+                d = _rows(_flat(dy, O))
                 if need_x:
-                    dx = _dgrad(dz, w1, None, 0).view(ctx.shape)
-            if first:
-                problems.append((dz, x2, ctx.biases[0] and need_b1))
-            if second:
-                problems.append((dy2, h, ctx.biases[1] and need_b2))
-            grads = _wgrad(problems, M) if problems else []
-            if second:
-                dw2, db2 = grads.pop()
-            if first:
-                dw1, db1 = grads.pop()
+                    dx = _new(x2, *ctx.shape)
+                if need_w1 or need_b1:
+                    dw1 = _new(x2, N, K)
+                    db1 = _new(x2, N) if need_b1 else None
+                if need_w2 or need_b2:
+                    dw2 = _new(x2, O, N)
+                    db2 = _new(x2, O) if need_b2 else None
+                lib, code, pd, ld = _lib.load(), _DTYPE_CODE[x2.dtype], d.data_ptr(), _ld(d)
+                n = lib.kda_mlp_bwd_workspace_size(pd, ld, M, N, K, O, act, code)
+                ws = torch.empty(n, dtype=torch.uint8, device=x2.device)
+                rc = lib.kda_mlp_bwd(pd, ld, x2.data_ptr(), _ld(x2), w1.data_ptr(), _ld(w1), _out(z),
+                                     z.stride(0) if act else 0, h.data_ptr(), _ld(h), w2.data_ptr(), _ld(w2), _out(dx), K,
+                                     _out(dw1), _out(db1), _out(dw2), _out(db2), M, N, K, O, act, code, ws.data_ptr(), n,
+                                     _raw_stream(x2.device.index))
+                if rc:
+                    _lib.check(rc, "kda_mlp_bwd")
         return (dx, dw1 if need_w1 else None, db1, dw2 if need_w2 else None, db2, dy if need_r else None, None)
 
 
@@ -273,13 +268,17 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     bias (N,), residual (..., N), all bf16 or all fp32; ``activation`` None, "gelu"
     (z Phi(z)) or "silu".  Rows and weights at any stride; bf16 rows that do not
     begin on 16 bytes, or whose K is no multiple of 8, are copied first when there
-    are more than 64 of them."""
+    are more than 64 of them or a gradient is needed."""
     act = _check("linear_act", x, ((weight, bias),), residual, activation)
     if _needs_grad(x, weight, bias, residual):
         return LinearActFunction.apply(x, weight, bias, residual, act)
     N, K = weight.shape
     with _on(x.device):
-        return _forward(_flat(x, K), weight, bias, _flat(residual, N), act, False)[0].view(*x.shape[:-1], N)
+        x2 = _flat(x, K)
+        M = x2.shape[0]
+        y = _new(x, *x.shape[:-1], N)
+        _forward(x2, K, weight, bias, _flat(residual, N), act, y.view(M, N), None, False)
+    return y
 
 
 def mlp(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: torch.Tensor, b2: Optional[torch.Tensor],
@@ -290,7 +289,11 @@ def mlp(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: torch
     act = _check("mlp", x, ((w1, b1), (w2, b2)), residual, activation)
     if _needs_grad(x, w1, b1, w2, b2, residual):
         return MLPFunction.apply(x, w1, b1, w2, b2, residual, act)
-    out = w2.shape[0]
+    (N, K), O = w1.shape, w2.shape[0]
     with _on(x.device):
-        h = _forward(_flat(x, w1.shape[1]), w1, b1, None, act, False, pad=True)[0]
-        return _forward(h, w2, b2, _flat(residual, out), 0, False)[0].view(*x.shape[:-1], out)
+        x2 = _flat(x, K)
+        M = x2.shape[0]
+        h, y = _new(x, M, _up8(N)), _new(x, *x.shape[:-1], O)
+        _forward(x2, K, w1, b1, None, act, h, None, False)
+        _forward(h, N, w2, b2, _flat(residual, O), 0, y.view(M, O), None, False)
+    return y

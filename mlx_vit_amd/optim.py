@@ -24,11 +24,12 @@ import torch.nn as nn
 
 from . import _lib
 from .kda import _DTYPE_CODE, _ptr, _stream
-from .linear import _on
+from .linear import _on, _raw_stream
 
 BLOCK = 256      # elements that share a scale; a tensor's moments begin on a multiple of it
+NORM_PART = 16384   # elements of a partial sum of the norm (kda_grad_norm_workspace_size)
 _STATES = {"fp32": 0, "int8": 1}
-_data_ptr, _contiguous, _numel = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
+_data_ptr, _contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 
 
 class FusedAdamW:
@@ -64,9 +65,6 @@ class FusedAdamW:
             if p.dtype not in _DTYPE_CODE or not p.is_contiguous():
                 raise ValueError("parameters must be contiguous float32 or bfloat16 tensors; got "
                                  f"{p.dtype}, shape {tuple(p.shape)}, strides {p.stride()}")
-        spans = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel())
-        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
-            raise ValueError("parameters overlap in memory (one of them is given twice, or two share a storage)")
         self._dtypes = [p.dtype for p in self.params]
         self._numels = [p.numel() for p in self.params]
         self.offsets: List[int] = []
@@ -77,8 +75,11 @@ class FusedAdamW:
         self.total = at
         self.state = self._new_state(master_weights) if state is None else self._given_state(state, master_weights)
         # p, g, n, offset, dtype of each parameter
+        self._parts = sum(-(-n // NORM_PART) for n in self._numels)
+        self._ptrs: List[int] = []
         self._table = array("q", [v for n, o, t in zip(self._numels, self.offsets, self._dtypes)
                                   for v in (0, 0, n, o, _DTYPE_CODE[t])])
+        self._check_params(list(map(_data_ptr, self.params)))
 
     # ---- state -----------------------------------------------------------
     def _specs(self, master: bool) -> Dict[str, Tuple[torch.dtype, int]]:
@@ -147,24 +148,41 @@ class FusedAdamW:
         self.steps = int(state["steps"])
 
     # ---- the step --------------------------------------------------------
+    def _check_params(self, ptrs: List[int]) -> None:
+        """The parameters' addresses are new: are they still what the optimizer was made for?"""
+        for p, t, n in zip(self.params, self._dtypes, self._numels):
+            if p.dtype != t or p.numel() != n or not p.is_contiguous() or p.device != self.device:
+                raise ValueError(f"a parameter of {n} elements of {t} is now {tuple(p.shape)}, {p.dtype}, strides "
+                                 f"{p.stride()} on {p.device}: make a new optimizer")
+        spans = sorted((a, p.nbytes) for a, p in zip(ptrs, self.params) if p.nbytes)
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("parameters overlap in memory (one of them is given twice, or two share a storage)")
+        self._ptrs = ptrs
+        # while these are held no other tensor can come to lie at the same address
+        self._storages = [p.untyped_storage() for p in self.params]
+        self._table[0::5] = array("q", ptrs)
+
     def _tensors(self):
-        """(descriptors, count, gradients kept until the launch) of the parameters with a gradient."""
-        ps = self.params
-        if [p.dtype for p in ps] != self._dtypes or list(map(_numel, ps)) != self._numels or not all(map(_contiguous, ps)):
-            raise ValueError("a parameter's dtype, size or layout is not what the optimizer was made for")
-        gs = [p.grad for p in ps]
-        table, dtypes = self._table, self._dtypes
-        table[0::5] = array("q", map(_data_ptr, ps))
-        if any(g is None for g in gs):
-            keep = [i for i, g in enumerate(gs) if g is not None]
+        """(descriptors, count, workgroups of the norm, gradients to keep until the launch) of the
+        parameters with a gradient."""
+        ptrs = list(map(_data_ptr, self.params))
+        if ptrs != self._ptrs:
+            self._check_params(ptrs)
+        gs = [p.grad for p in self.params]
+        table, dtypes, parts = self._table, self._dtypes, self._parts
+        missing = [i for i, g in enumerate(gs) if g is None]
+        if missing:
+            skip = set(missing)
+            keep = [i for i in range(len(gs)) if i not in skip]
             table = array("q", [v for i in keep for v in table[5 * i:5 * i + 5]])
             gs, dtypes = [gs[i] for i in keep], [dtypes[i] for i in keep]
+            parts = sum(-(-self._numels[i] // NORM_PART) for i in keep)
         if [g.dtype for g in gs] != dtypes:
             raise ValueError("a gradient's dtype is not its parameter's")
         if not all(map(_contiguous, gs)):
             gs = [g.contiguous() for g in gs]
-        table[1::5] = array("q", map(_data_ptr, gs))
-        return table, len(gs), gs
+        table[1::5] = array("q", list(map(_data_ptr, gs)))
+        return table, len(gs), parts, gs
 
     @torch.no_grad()
     def step(self, max_norm: Optional[float] = None) -> Optional[torch.Tensor]:
@@ -173,23 +191,27 @@ class FusedAdamW:
         fp32); the gradients themselves stay as they are."""
         if max_norm is not None and not max_norm > 0.0:
             raise ValueError(f"max_norm={max_norm}: expected a positive number or None")
-        table, count, gs = self._tensors()
+        table, count, parts, gs = self._tensors()   # gs: alive until the launches
         self.steps += 1
         b1, b2 = self.betas
         c1 = 1.0 / (1.0 - b1 ** self.steps) if self.bias_correction else 1.0
         c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
-        lib, st, at = _lib.load(), self.state, table.buffer_info()[0]
-        clip = None
+        lib, at = _lib.load(), table.buffer_info()[0]
+        buffers = [_ptr(self.state.get(k)) for k in ("m", "v", "m_scale", "v_scale", "master")]
+        clip = pc = None
         with _on(self.device):
-            stream = _stream(self.device)
+            stream = _raw_stream(self.device.index)
             if max_norm is not None:
-                clip = torch.empty(2, dtype=torch.float32, device=self.device)
-                ws = torch.empty(max(lib.kda_grad_norm_workspace_size(at, count), 4), dtype=torch.uint8, device=self.device)
-                _lib.check(lib.kda_grad_norm(at, count, max_norm, _ptr(clip), _ptr(ws), ws.numel(), stream), "kda_grad_norm")
-            _lib.check(lib.kda_adamw_step(
-                at, count, _STATES[self.states], _ptr(st["m"]), _ptr(st["v"]), _ptr(st.get("m_scale")),
-                _ptr(st.get("v_scale")), _ptr(st.get("master")), _ptr(clip), self.lr, b1, b2, self.eps, self.weight_decay,
-                c1, c2, stream), "kda_adamw_step")
+                # the norm, the clip factor, the norm's partial sums
+                clip = torch.empty(2 + parts, dtype=torch.float32, device=self.device)
+                pc = clip.data_ptr()
+                rc = lib.kda_grad_norm(at, count, max_norm, pc, pc + 8, 4 * parts, stream)
+                if rc:
+                    _lib.check(rc, "kda_grad_norm")
+            rc = lib.kda_adamw_step(at, count, _STATES[self.states], *buffers, pc, self.lr, b1, b2, self.eps,
+                                    self.weight_decay, c1, c2, stream)
+            if rc:
+                _lib.check(rc, "kda_adamw_step")
         return None if clip is None else clip[0]
 
     def zero_grad(self) -> None:

@@ -77,29 +77,41 @@ def test_c_abi_linear_fwd_refuses(kw, rc):
 def test_c_abi_linear_nothing_to_do():
     lib = _lib.load()
     assert _fwd(lib, M=0, x=None) == 0
-    assert lib.kda_linear_wgrad_workspace_size(0, 4, 4) == 0
-    assert lib.kda_linear_wgrad_workspace_size(100, 16, 24) >= 4 * (16 * 24 + 16)
+    assert lib.kda_linear_bwd_workspace_size(4096, 16, 0, 16, 16, 0, 0) == 0
+    assert lib.kda_linear_pad(None, 0, 0, 0, None, None, 0, 0, 0, None, None) == 0
+
+
+def test_c_abi_backward_workspace():
+    """fp32: at least one partial gradient; dz where an activation is, or a bf16 dy cannot be read as it is."""
+    lib = _lib.load()
+    size = lambda dy=4096, ld=32, M=100, N=32, K=64, act=0, dtype=1: lib.kda_linear_bwd_workspace_size(dy, ld, M, N, K, act, dtype)  # noqa: E731
+    assert size(dtype=0) >= 4 * (32 * 64 + 32)
+    assert size(act=1) >= size() + 2 * 100 * 32
+    assert size(dy=4098) >= size() + 2 * 100 * 32 and size(ld=33) >= size() + 2 * 100 * 32
+    assert size(K=63) >= size() + 2 * 32 * 64
+    assert lib.kda_mlp_bwd_workspace_size(4096, 32, 100, 128, 64, 32, 1, 1) >= 2 * 100 * 128
 
 
 def test_c_abi_backward_refuses():
     lib = _lib.load()
-    ok = [4096, 32, 8192, 64, 4096, 64, 16384, 64, 100, 32, 64, 1, 1, None]   # dz, w, z, dx, M, N, K, act, dtype
-    for i, v, rc in ((0, None, -1), (2, None, -1), (4, None, -1), (6, None, -1), (1, 31, -1), (3, 60, -1), (0, 4104, -1),
-                     (11, 5, -2), (12, 7, -2), (8, -1, -1)):
-        a = list(ok)
-        a[i] = v
-        assert lib.kda_linear_dgrad(*a) == rc, (i, v)
-    ok = [4096, 32, 8192, 64, 16384, 32768, 100, 32, 64, 65536, 1 << 20, None]
-    for i, v, rc in ((0, None, -1), (2, None, -1), (4, None, -1), (9, None, -1), (9, 65540, -1), (10, 16, -3), (6, 0, -1),
-                     (0, 4098, -1)):
-        a = list(ok)
-        a[i] = v
-        assert lib.kda_linear_wgrad(*a) == rc, (i, v)
-    ok = [4096, 32, 8192, 32, 16384, 32, 100, 32, 1, 1, None]
-    for i, v, rc in ((8, 0, -2), (0, None, -1), (2, None, -1), (4, 16385, -1), (5, 8, -1)):
-        a = list(ok)
-        a[i] = v
-        assert lib.kda_linear_act_bwd(*a) == rc, (i, v)
+    a0 = dict(dy=4096, ld_dy=32, x=4096, ld_x=64, w=8192, ld_w=64, z=4096, ld_z=32, dx=16384, ld_dx=64, dw=4096, db=4096,
+              M=100, N=32, K=64, act=1, dtype=1, ws=4096, n=1 << 30, st=None)
+    for kw, rc in ((dict(dy=None), -1), (dict(x=None), -1), (dict(w=None), -1), (dict(z=None), -1), (dict(dw=None), -1),
+                   (dict(ld_dy=31), -1), (dict(ld_x=60), -1), (dict(x=4104), -1), (dict(w=8200), -1), (dict(ld_dx=63), -1),
+                   (dict(dw=4104), -1), (dict(act=5), -2), (dict(dtype=7), -2), (dict(M=0), -1), (dict(ws=None), -1),
+                   (dict(ws=4100), -1), (dict(n=16), -3), (dict(dtype=0, dy=4098), -1)):
+        assert lib.kda_linear_bwd(*{**a0, **kw}.values()) == rc, kw
+    m0 = dict(dy=4096, ld_dy=32, x=4096, ld_x=64, w1=8192, ld_w1=64, z=4096, ld_z=128, h=4096, ld_h=128, w2=4096, ld_w2=128,
+              dx=16384, ld_dx=64, dw1=4096, db1=4096, dw2=4096, db2=4096, M=100, N=128, K=64, O=32, act=1, dtype=1, ws=4096,
+              n=1 << 30, st=None)
+    for kw, rc in ((dict(dy=None), -1), (dict(x=None), -1), (dict(w1=None), -1), (dict(w2=None), -1), (dict(z=None), -1),
+                   (dict(h=None), -1), (dict(dw1=None), -1), (dict(dw2=None), -1), (dict(h=4104), -1), (dict(ld_h=127), -1),
+                   (dict(O=0), -1), (dict(M=-1), -1), (dict(act=3), -2), (dict(ws=None), -1), (dict(n=16), -3)):
+        assert lib.kda_mlp_bwd(*{**m0, **kw}.values()) == rc, kw
+    p0 = dict(s0=4096, ld0=10, r0=4, c0=9, d0=4096, s1=None, ld1=0, r1=0, c1=0, d1=None, st=None)
+    for kw, rc in ((dict(s0=None), -1), (dict(d0=None), -1), (dict(d0=4104), -1), (dict(ld0=8), -1), (dict(c0=0), -1),
+                   (dict(r0=-1), -1), (dict(d1=4096), -1)):
+        assert lib.kda_linear_pad(*{**p0, **kw}.values()) == rc, kw
 
 
 def _tensor(p=4096, g=8192, n=10, offset=0, dtype=1):
