@@ -371,16 +371,22 @@ int kda_mlp_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, cons
  * begin, `offset` elements (a multiple of 256) into the moments' buffers.  Those
  * buffers hold whole blocks of 256 elements: a tensor owns n rounded up to 256
  * of them, and those past n are written as zeros (from zeros).  Tensors must
- * not overlap.  Kernels take up to 120 tensors a launch. */
+ * not overlap.  g NULL: the tensor is left out of the call. */
 typedef struct kda_adamw_tensor {
     void* p;
     const void* g;
     int64_t n, offset, dtype;
 } kda_adamw_tensor;
+/* What does not change from step to step (p, n, offset and dtype of the tensors),
+ * as the kernels read it: kda_adamw_plan fills kda_adamw_plan_size bytes of host
+ * memory, which the caller copies to the device once (8-byte aligned) and passes
+ * with the same tensors, whose g may differ, to the two calls below. */
+size_t kda_adamw_plan_size(const kda_adamw_tensor* tensors, int count);
+int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, size_t bytes);
 /* out[0] = sqrt(sum of g^2 over all tensors), out[1] = min(max_norm / (out[0] +
- * 1e-6), 1), fp32, in a fixed order (p and offset unused). */
+ * 1e-6), 1), fp32, in a fixed order.  workspace 4-byte aligned. */
 size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count);
-int kda_grad_norm(const kda_adamw_tensor* tensors, int count, double max_norm, float* out,
+int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, double max_norm, float* out,
                   void* workspace, size_t ws_bytes, void* stream);
 /* g' = clip[1] g (clip: kda_grad_norm's out, or NULL for g itself);
  *   m <- beta1 m + (1 - beta1) g';  v <- beta2 v + (1 - beta2) g'^2;
@@ -394,9 +400,9 @@ int kda_grad_norm(const kda_adamw_tensor* tensors, int count, double max_norm, f
  * m, v, master 16-byte aligned. */
 #define KDA_ADAMW_F32 0
 #define KDA_ADAMW_INT8 1
-int kda_adamw_step(const kda_adamw_tensor* tensors, int count, int states, void* m, void* v, float* m_scale,
-                   float* v_scale, float* master, const float* clip, double lr, double beta1, double beta2,
-                   double eps, double weight_decay, double correct1, double correct2, void* stream);
+int kda_adamw_step(const kda_adamw_tensor* tensors, int count, const void* plan, int states, void* m, void* v,
+                   float* m_scale, float* v_scale, float* master, const float* clip, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, double correct1, double correct2, void* stream);
 /* the values that n (a multiple of 256) 8-bit moments stand for */
 int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale,
                       void* m_out, void* v_out, int64_t n, int dtype, void* stream);

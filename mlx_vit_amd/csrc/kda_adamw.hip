@@ -27,45 +27,35 @@ namespace kda {
 namespace {
 
 constexpr int QB = 256;            // elements that share a scale
-constexpr int PER_WG = 4096;       // elements of one tensor a workgroup updates
-constexpr int NORM_PER_WG = 16384; // and sums the squares of
-constexpr int PER_LAUNCH = 120;    // tensors of one launch (their descriptors travel as kernel arguments)
+constexpr int PER_WG = 4096;       // elements of one tensor a workgroup takes
+constexpr int PER_LAUNCH = 480;    // tensors of one launch: their gradients' addresses travel as kernel arguments
 
+// What does not change from step to step lies in device memory, the plan: the
+// tensors, then for each workgroup its tensor.  A step's own part, the gradients'
+// addresses, fits one launch for most models (as whole descriptors in the
+// arguments, 120 tensors a launch, the default classifier's 436 took four
+// launches and 6 us more for each).
 struct Tensor {
     void* p;
-    const void* g;
     int64_t n;
     uint32_t blk0;                 // first block of 256 in the moments
     uint32_t wg0;                  // first workgroup
+    int64_t bf16;
+};
+struct Grads {
+    const Tensor* tensors;
+    const uint32_t* owner;         // [workgroup] its tensor
+    int first;                     // tensor of g[0]
+    uint32_t wg;                   // workgroup of block 0
+    const void* g[PER_LAUNCH];     // null: the tensor is left out
 };
 struct StepArgs {
-    Tensor t[PER_LAUNCH];
-    uint8_t flags[PER_LAUNCH];     // 1: bf16, 2: p and g 16-byte aligned
-    int count;
     float b1, omb1, b2, omb2, decay, lr, eps, rc2;
     const float* clip;
     void *m, *v;
     float *ms, *vs, *master;
 };
-static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
-struct NormArgs2 {
-    Tensor t[PER_LAUNCH];
-    uint8_t flags[PER_LAUNCH];
-    int count;
-    float* part;
-};
-
-// the tensor of workgroup b: the last whose first workgroup is at most b.  All
-// lanes look at once (a binary search is seven dependent scalar loads).
-template <typename Args>
-__device__ __forceinline__ int tensor_of(const Args& a, uint32_t b) {
-    const int l = lane_id();
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < PER_LAUNCH; i += 64)
-        n += __popcll(__ballot(i + l < a.count && a.t[min(i + l, PER_LAUNCH - 1)].wg0 <= b));
-    return __builtin_amdgcn_readfirstlane(n - 1);
-}
+static_assert(sizeof(Grads) + sizeof(StepArgs) <= 4096, "kernel arguments");
 
 // eight elements at p, of which `left` exist
 template <typename T>
@@ -120,12 +110,12 @@ __device__ __forceinline__ float inv_scale(uint32_t s) {
 }
 
 template <typename T, bool SMALL, bool MASTER>
-__device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, bool vec, float c, int64_t e0) {
+__device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, const void* grad, bool vec, float c, int64_t e0) {
     const int64_t left = t.n - e0;
     const size_t at = (size_t)t.blk0 * QB + e0;      // in the moments
     T* p = static_cast<T*>(t.p) + e0;
     float g[8], w[8], m[8], v[8];
-    ld8<T>(static_cast<const T*>(t.g) + e0, left, vec, g);
+    ld8<T>(static_cast<const T*>(grad) + e0, left, vec, g);
     if constexpr (MASTER) ld8<float>(a.master + at, 8, true, w);
     else ld8<T>(p, left, vec, w);
     if constexpr (SMALL) {
@@ -188,15 +178,18 @@ __device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, bool 
 }
 
 template <bool SMALL, bool MASTER>
-__global__ __launch_bounds__(256) void kda_adamw_kernel(const StepArgs a) {
-    const int i = tensor_of(a, blockIdx.x);
-    const Tensor& t = a.t[i];
-    const int f = a.flags[i];
+__global__ __launch_bounds__(256) void kda_adamw_kernel(const StepArgs a, const Grads q) {
+    const uint32_t wg = q.wg + blockIdx.x;
+    const int i = (int)q.owner[wg];
+    const Tensor t = q.tensors[i];
+    const void* g = q.g[i - q.first];
+    if (!g) return;
+    const bool vec = ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(t.p)) & 15) == 0;
     const float c = a.clip ? a.clip[1] : 1.f;
-    const int64_t b0 = (int64_t)(blockIdx.x - t.wg0) * PER_WG, end = min((t.n + QB - 1) / QB * QB, b0 + (int64_t)PER_WG);
+    const int64_t b0 = (int64_t)(wg - t.wg0) * PER_WG, end = min((t.n + QB - 1) / QB * QB, b0 + (int64_t)PER_WG);
     for (int64_t e = b0 + 8 * (int64_t)threadIdx.x; e < end; e += 8 * 256) {   // whole blocks: half waves stay together
-        if (f & 1) update<uint16_t, SMALL, MASTER>(a, t, f & 2, c, e);
-        else update<float, SMALL, MASTER>(a, t, f & 2, c, e);
+        if (t.bf16) update<uint16_t, SMALL, MASTER>(a, t, g, vec, c, e);
+        else update<float, SMALL, MASTER>(a, t, g, vec, c, e);
     }
 }
 
@@ -208,21 +201,30 @@ __device__ __forceinline__ float wg_sum(float s, float* lds) {
     return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-__global__ __launch_bounds__(256) void kda_grad_norm_kernel(const NormArgs2 a) {
+__global__ __launch_bounds__(256) void kda_grad_norm_kernel(float* __restrict__ part, const Grads q) {
     __shared__ float lds[4];
-    const int i = tensor_of(a, blockIdx.x);
-    const Tensor& t = a.t[i];
-    const int f = a.flags[i];
-    const int64_t b0 = (int64_t)(blockIdx.x - t.wg0) * NORM_PER_WG, end = min(t.n, b0 + (int64_t)NORM_PER_WG);
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, x[8];
-    for (int64_t e = b0 + 8 * (int64_t)threadIdx.x; e < end; e += 8 * 256) {
-        if (f & 1) ld8<uint16_t>(static_cast<const uint16_t*>(t.g) + e, t.n - e, f & 2, x);
-        else ld8<float>(static_cast<const float*>(t.g) + e, t.n - e, f & 2, x);
+    const uint32_t wg = q.wg + blockIdx.x;
+    const int i = (int)q.owner[wg];
+    const Tensor t = q.tensors[i];
+    const void* g = q.g[i - q.first];
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (g) {
+        const bool vec = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+        const int64_t b0 = (int64_t)(wg - t.wg0) * PER_WG;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) s[q] = fmaf(x[q], x[q], s[q]);
+        for (int u = 0; u < PER_WG / 2048; ++u) {
+            const int64_t e = b0 + 2048 * u + 8 * (int64_t)threadIdx.x, left = t.n - e;
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (left > 0) {
+                if (t.bf16) ld8<uint16_t>(static_cast<const uint16_t*>(g) + e, left, vec, x);
+                else ld8<float>(static_cast<const float*>(g) + e, left, vec, x);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[k] = fmaf(x[k], x[k], s[k]);
+        }
     }
     const float sum = wg_sum(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])), lds);
-    if (threadIdx.x == 0) a.part[blockIdx.x] = sum;
+    if (threadIdx.x == 0) part[wg] = sum;
 }
 
 // out[0] = G, out[1] = the clip factor (a NaN stays one)
@@ -230,6 +232,7 @@ __global__ __launch_bounds__(1024) void kda_grad_norm_finish_kernel(const float*
                                                                     float* __restrict__ out) {
     __shared__ double lds[16];
     double s = 0.;
+#pragma unroll 8
     for (int i = threadIdx.x; i < n; i += 1024) s += (double)part[i];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
@@ -266,44 +269,53 @@ __global__ __launch_bounds__(256) void kda_adamw_moments_kernel(const int8_t* __
 
 int check_tensors(const kda_adamw_tensor* t, int count, bool step) {
     if (count < 0 || (count > 0 && !t)) return api_fail(KDA_E_INVALID, "count=%d tensors at %p", count, (const void*)t);
+    int64_t wgs = 0;
     for (int i = 0; i < count; ++i) {
         if (t[i].dtype != KDA_DTYPE_F32 && t[i].dtype != KDA_DTYPE_BF16)
             return api_fail(KDA_E_UNSUPPORTED, "tensor %d: dtype=%lld: expected 0 (fp32) or 1 (bf16)", i, (long long)t[i].dtype);
         if (t[i].n < 0 || t[i].n > ((int64_t)1 << 36)) return api_fail(KDA_E_INVALID, "tensor %d: n=%lld", i, (long long)t[i].n);
+        wgs += (t[i].n + PER_WG - 1) / PER_WG;
         if (t[i].n == 0) continue;
         const uintptr_t es = t[i].dtype == KDA_DTYPE_BF16 ? 2 : 4;
-        if (!t[i].g || reinterpret_cast<uintptr_t>(t[i].g) % es != 0 ||
+        if (reinterpret_cast<uintptr_t>(t[i].g) % es != 0 ||
             (step && (!t[i].p || reinterpret_cast<uintptr_t>(t[i].p) % es != 0)))
-            return api_fail(KDA_E_INVALID, "tensor %d: p or g is NULL or misaligned", i);
+            return api_fail(KDA_E_INVALID, "tensor %d: p is NULL, or p or g is misaligned", i);
         if (step && (t[i].offset < 0 || t[i].offset % QB != 0 || t[i].offset / QB > 0xffffffffLL))
             return api_fail(KDA_E_INVALID, "tensor %d: offset=%lld: expected a multiple of %d", i, (long long)t[i].offset, QB);
     }
+    if (wgs > (1 << 23))   // 256 threads each: below 2^32 in a launch
+        return api_fail(KDA_E_UNSUPPORTED, "more than 2^23 * %d elements", PER_WG);
     return KDA_OK;
 }
 
-// the next tensors of a launch (from *i on), workgroups of `per` elements; returns the workgroups
-template <typename Args>
-uint32_t fill(Args& a, const kda_adamw_tensor* t, int count, int* i, int per, bool step) {
-    a.count = 0;
-    uint32_t wg = 0;
-    for (; *i < count && a.count < PER_LAUNCH; ++*i) {
-        const kda_adamw_tensor& q = t[*i];
-        if (q.n == 0) continue;
-        const uint32_t need = (uint32_t)((q.n + per - 1) / per);
-        if (wg + need > (1u << 23) && a.count > 0) break;   // 256 threads each: below 2^32 in all
-        const uintptr_t both = reinterpret_cast<uintptr_t>(q.g) | (step ? reinterpret_cast<uintptr_t>(q.p) : 0);
-        a.t[a.count] = Tensor{q.p, q.g, q.n, (uint32_t)(step ? q.offset / QB : 0), wg};
-        a.flags[a.count] = (uint8_t)((q.dtype == KDA_DTYPE_BF16 ? 1 : 0) | (both % 16 == 0 ? 2 : 0));
-        ++a.count;
-        wg += need;
-    }
-    return wg;
+uint32_t workgroups(const kda_adamw_tensor* t, int count) {
+    uint32_t n = 0;
+    for (int i = 0; i < count; ++i) n += (uint32_t)((t[i].n + PER_WG - 1) / PER_WG);
+    return n;
+}
+const uint32_t* owners(const void* plan, int count) {
+    return reinterpret_cast<const uint32_t*>(static_cast<const Tensor*>(plan) + count);
 }
 
-size_t norm_parts(const kda_adamw_tensor* t, int count) {
-    size_t n = 0;
-    for (int i = 0; i < count; ++i) n += (size_t)((t[i].n + NORM_PER_WG - 1) / NORM_PER_WG);
-    return n;
+// launch(grads, workgroups) for each run of PER_LAUNCH tensors
+template <typename F>
+hipError_t each_launch(const kda_adamw_tensor* t, int count, const void* plan, F&& launch) {
+    Grads q;
+    q.tensors = static_cast<const Tensor*>(plan);
+    q.owner = owners(plan, count);
+    q.wg = 0;
+    for (q.first = 0; q.first < count; q.first += PER_LAUNCH) {
+        const int n = std::min(PER_LAUNCH, count - q.first);
+        for (int i = 0; i < n; ++i) q.g[i] = t[q.first + i].g;
+        const uint32_t wg = workgroups(t + q.first, n);
+        if (wg > 0) {
+            launch(q, dim3(wg));
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        q.wg += wg;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -314,44 +326,61 @@ using namespace kda;
 
 extern "C" {
 
-size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count) {
-    if (check_tensors(tensors, count, false) != KDA_OK) return 0;
-    return norm_parts(tensors, count) * sizeof(float);
+size_t kda_adamw_plan_size(const kda_adamw_tensor* tensors, int count) {
+    if (check_tensors(tensors, count, true) != KDA_OK) return 0;
+    return count * sizeof(Tensor) + workgroups(tensors, count) * sizeof(uint32_t);
 }
 
-int kda_grad_norm(const kda_adamw_tensor* tensors, int count, double max_norm, float* out, void* workspace, size_t ws_bytes,
-                  void* stream) {
+int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, size_t bytes) {
+    const int rc = check_tensors(tensors, count, true);
+    if (rc != KDA_OK) return rc;
+    if (count == 0) return KDA_OK;
+    if (!host_plan || reinterpret_cast<uintptr_t>(host_plan) % 8 != 0)
+        return api_fail(KDA_E_INVALID, "host_plan is NULL or not 8-byte aligned");
+    if (bytes < kda_adamw_plan_size(tensors, count))
+        return api_fail(KDA_E_WORKSPACE, "the plan has %zu bytes, needs %zu", bytes, kda_adamw_plan_size(tensors, count));
+    Tensor* t = static_cast<Tensor*>(host_plan);
+    uint32_t* owner = const_cast<uint32_t*>(owners(host_plan, count));
+    uint32_t wg = 0;
+    for (int i = 0; i < count; ++i) {
+        t[i] = Tensor{tensors[i].p, tensors[i].n, (uint32_t)(tensors[i].offset / QB), wg, tensors[i].dtype};
+        for (const uint32_t end = wg + workgroups(tensors + i, 1); wg < end; ++wg) owner[wg] = (uint32_t)i;
+    }
+    return KDA_OK;
+}
+
+size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count) {
+    if (check_tensors(tensors, count, false) != KDA_OK) return 0;
+    return workgroups(tensors, count) * sizeof(float);
+}
+
+int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, double max_norm, float* out, void* workspace,
+                  size_t ws_bytes, void* stream) {
     const int rc = check_tensors(tensors, count, false);
     if (rc != KDA_OK) return rc;
     if (!out || reinterpret_cast<uintptr_t>(out) % 4 != 0) return api_fail(KDA_E_INVALID, "out is NULL or misaligned");
     if (!(max_norm > 0.)) return api_fail(KDA_E_INVALID, "max_norm=%g: expected a positive number", max_norm);
-    const size_t parts = norm_parts(tensors, count);
-    if (parts > 0x7fffffffu) return api_fail(KDA_E_UNSUPPORTED, "%zu partial sums", parts);
+    const size_t parts = workgroups(tensors, count);
+    if (parts > 0 && (!plan || reinterpret_cast<uintptr_t>(plan) % 8 != 0))
+        return api_fail(KDA_E_INVALID, "plan is NULL or not 8-byte aligned");
     if (parts > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0))
         return api_fail(KDA_E_INVALID, "workspace is NULL or misaligned");
     if (ws_bytes < parts * sizeof(float))
         return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, parts * sizeof(float));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    NormArgs2 a;
     float* part = static_cast<float*>(workspace);
-    for (int i = 0; i < count;) {
-        a.part = part;
-        const uint32_t wg = fill(a, tensors, count, &i, NORM_PER_WG, false);
-        if (wg == 0) continue;
-        hipLaunchKernelGGL(kda_grad_norm_kernel, dim3(wg), dim3(256), 0, st, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return api_hip_fail(e, "kda_grad_norm");
-        part += wg;
-    }
-    hipLaunchKernelGGL(kda_grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float*>(workspace),
-                       (int)parts, (float)max_norm, out);
-    const hipError_t e = hipGetLastError();
+    hipError_t e = each_launch(tensors, count, plan, [&](const Grads& q, dim3 grid) {
+        hipLaunchKernelGGL(kda_grad_norm_kernel, grid, dim3(256), 0, st, part, q);
+    });
+    if (e != hipSuccess) return api_hip_fail(e, "kda_grad_norm");
+    hipLaunchKernelGGL(kda_grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)parts, (float)max_norm, out);
+    e = hipGetLastError();
     return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_grad_norm");
 }
 
-int kda_adamw_step(const kda_adamw_tensor* tensors, int count, int states, void* m, void* v, float* m_scale, float* v_scale,
-                   float* master, const float* clip, double lr, double beta1, double beta2, double eps, double weight_decay,
-                   double correct1, double correct2, void* stream) {
+int kda_adamw_step(const kda_adamw_tensor* tensors, int count, const void* plan, int states, void* m, void* v,
+                   float* m_scale, float* v_scale, float* master, const float* clip, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, double correct1, double correct2, void* stream) {
     const int rc = check_tensors(tensors, count, true);
     if (rc != KDA_OK) return rc;
     if (states != KDA_ADAMW_F32 && states != KDA_ADAMW_INT8)
@@ -360,6 +389,8 @@ int kda_adamw_step(const kda_adamw_tensor* tensors, int count, int states, void*
         return api_fail(KDA_E_INVALID, "beta1=%g beta2=%g eps=%g correct1=%g correct2=%g", beta1, beta2, eps, correct1,
                         correct2);
     if (count == 0) return KDA_OK;
+    if (!plan || reinterpret_cast<uintptr_t>(plan) % 8 != 0)
+        return api_fail(KDA_E_INVALID, "plan is NULL or not 8-byte aligned");
     const bool small = states == KDA_ADAMW_INT8;
     const uintptr_t all = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(master);
     if (!m || !v || all % 16 != 0) return api_fail(KDA_E_INVALID, "m, v or master is NULL or not 16-byte aligned");
@@ -375,18 +406,14 @@ int kda_adamw_step(const kda_adamw_tensor* tensors, int count, int states, void*
     a.rc2 = (float)sqrt(correct2);
     a.clip = clip;
     a.m = m; a.v = v; a.ms = m_scale; a.vs = v_scale; a.master = master;
-    for (int i = 0; i < count;) {
-        const uint32_t wg = fill(a, tensors, count, &i, PER_WG, true);
-        if (wg == 0) continue;
-        const dim3 grid(wg), block(256);
-        if (small && master) hipLaunchKernelGGL((kda_adamw_kernel<true, true>), grid, block, 0, st, a);
-        else if (small) hipLaunchKernelGGL((kda_adamw_kernel<true, false>), grid, block, 0, st, a);
-        else if (master) hipLaunchKernelGGL((kda_adamw_kernel<false, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((kda_adamw_kernel<false, false>), grid, block, 0, st, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return api_hip_fail(e, "kda_adamw_step");
-    }
-    return KDA_OK;
+    const hipError_t e = each_launch(tensors, count, plan, [&](const Grads& q, dim3 grid) {
+        const dim3 block(256);
+        if (small && master) hipLaunchKernelGGL((kda_adamw_kernel<true, true>), grid, block, 0, st, a, q);
+        else if (small) hipLaunchKernelGGL((kda_adamw_kernel<true, false>), grid, block, 0, st, a, q);
+        else if (master) hipLaunchKernelGGL((kda_adamw_kernel<false, true>), grid, block, 0, st, a, q);
+        else hipLaunchKernelGGL((kda_adamw_kernel<false, false>), grid, block, 0, st, a, q);
+    });
+    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_adamw_step");
 }
 
 int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale, void* m_out, void* v_out,

@@ -27,7 +27,6 @@ from .kda import _DTYPE_CODE, _ptr, _stream
 from .linear import _on, _raw_stream
 
 BLOCK = 256      # elements that share a scale; a tensor's moments begin on a multiple of it
-NORM_PART = 16384   # elements of a partial sum of the norm (kda_grad_norm_workspace_size)
 _STATES = {"fp32": 0, "int8": 1}
 _data_ptr, _contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 
@@ -75,8 +74,8 @@ class FusedAdamW:
         self.total = at
         self.state = self._new_state(master_weights) if state is None else self._given_state(state, master_weights)
         # p, g, n, offset, dtype of each parameter
-        self._parts = sum(-(-n // NORM_PART) for n in self._numels)
         self._ptrs: List[int] = []
+        self._plan: Optional[torch.Tensor] = None
         self._table = array("q", [v for n, o, t in zip(self._numels, self.offsets, self._dtypes)
                                   for v in (0, 0, n, o, _DTYPE_CODE[t])])
         self._check_params(list(map(_data_ptr, self.params)))
@@ -161,28 +160,34 @@ class FusedAdamW:
         # while these are held no other tensor can come to lie at the same address
         self._storages = [p.untyped_storage() for p in self.params]
         self._table[0::5] = array("q", ptrs)
+        lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
+        plan = torch.empty(lib.kda_adamw_plan_size(at, count), dtype=torch.uint8)
+        _lib.check(lib.kda_adamw_plan(at, count, plan.data_ptr(), plan.numel()), "kda_adamw_plan")
+        if self._plan is not None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("parameters were moved since the last step: take one outside the capture first")
+            torch.cuda.synchronize(self.device)   # a step may be reading the old plan, on any stream
+        self._plan = plan.to(self.device)
+        self._parts = lib.kda_grad_norm_workspace_size(at, count) // 4
 
-    def _tensors(self):
-        """(descriptors, count, workgroups of the norm, gradients to keep until the launch) of the
-        parameters with a gradient."""
+    def _gradients(self) -> List[Optional[torch.Tensor]]:
+        """Fill the descriptors for a step; returns the gradients, to be kept until the launches."""
         ptrs = list(map(_data_ptr, self.params))
         if ptrs != self._ptrs:
             self._check_params(ptrs)
-        gs = [p.grad for p in self.params]
-        table, dtypes, parts = self._table, self._dtypes, self._parts
+        gs = present = [p.grad for p in self.params]
+        dtypes = self._dtypes
         missing = [i for i, g in enumerate(gs) if g is None]
         if missing:
-            skip = set(missing)
-            keep = [i for i in range(len(gs)) if i not in skip]
-            table = array("q", [v for i in keep for v in table[5 * i:5 * i + 5]])
-            gs, dtypes = [gs[i] for i in keep], [dtypes[i] for i in keep]
-            parts = sum(-(-self._numels[i] // NORM_PART) for i in keep)
-        if [g.dtype for g in gs] != dtypes:
+            present = [g for g in gs if g is not None]
+            dtypes = [t for t, g in zip(dtypes, gs) if g is not None]
+        if [g.dtype for g in present] != dtypes:
             raise ValueError("a gradient's dtype is not its parameter's")
-        if not all(map(_contiguous, gs)):
-            gs = [g.contiguous() for g in gs]
-        table[1::5] = array("q", list(map(_data_ptr, gs)))
-        return table, len(gs), parts, gs
+        if not all(map(_contiguous, present)):
+            gs = present = [g if g is None else g.contiguous() for g in gs]
+        self._table[1::5] = array("q", [0 if g is None else g.data_ptr() for g in gs] if missing
+                                  else list(map(_data_ptr, gs)))
+        return gs
 
     @torch.no_grad()
     def step(self, max_norm: Optional[float] = None) -> Optional[torch.Tensor]:
@@ -191,24 +196,25 @@ class FusedAdamW:
         fp32); the gradients themselves stay as they are."""
         if max_norm is not None and not max_norm > 0.0:
             raise ValueError(f"max_norm={max_norm}: expected a positive number or None")
-        table, count, parts, gs = self._tensors()   # gs: alive until the launches
+        gs = self._gradients()   # noqa: F841 (alive until the launches)
         self.steps += 1
         b1, b2 = self.betas
         c1 = 1.0 / (1.0 - b1 ** self.steps) if self.bias_correction else 1.0
         c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
-        lib, at = _lib.load(), table.buffer_info()[0]
+        lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
+        plan = self._plan.data_ptr()
         buffers = [_ptr(self.state.get(k)) for k in ("m", "v", "m_scale", "v_scale", "master")]
         clip = pc = None
         with _on(self.device):
             stream = _raw_stream(self.device.index)
             if max_norm is not None:
                 # the norm, the clip factor, the norm's partial sums
-                clip = torch.empty(2 + parts, dtype=torch.float32, device=self.device)
+                clip = torch.empty(2 + self._parts, dtype=torch.float32, device=self.device)
                 pc = clip.data_ptr()
-                rc = lib.kda_grad_norm(at, count, max_norm, pc, pc + 8, 4 * parts, stream)
+                rc = lib.kda_grad_norm(at, count, plan, max_norm, pc, pc + 8, 4 * self._parts, stream)
                 if rc:
                     _lib.check(rc, "kda_grad_norm")
-            rc = lib.kda_adamw_step(at, count, _STATES[self.states], *buffers, pc, self.lr, b1, b2, self.eps,
+            rc = lib.kda_adamw_step(at, count, plan, _STATES[self.states], *buffers, pc, self.lr, b1, b2, self.eps,
                                     self.weight_decay, c1, c2, stream)
             if rc:
                 _lib.check(rc, "kda_adamw_step")

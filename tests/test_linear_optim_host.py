@@ -118,24 +118,30 @@ def _tensor(p=4096, g=8192, n=10, offset=0, dtype=1):
     return (ctypes.c_int64 * 5)(p, g, n, offset, dtype)
 
 
-def _step(lib, t, count=1, states=0, m=4096, v=8192, ms=None, vs=None, master=None, b1=0.9, b2=0.95, eps=1e-8, c1=1.0, c2=1.0):
-    return lib.kda_adamw_step(t, count, states, m, v, ms, vs, master, None, 1e-3, b1, b2, eps, 0.05, c1, c2, None)
+def _step(lib, t, count=1, states=0, m=4096, v=8192, ms=None, vs=None, master=None, b1=0.9, b2=0.95, eps=1e-8, c1=1.0, c2=1.0, plan=4096):
+    return lib.kda_adamw_step(t, count, plan, states, m, v, ms, vs, master, None, 1e-3, b1, b2, eps, 0.05, c1, c2, None)
 
 
 def test_c_abi_adamw_refuses():
     lib = _lib.load()
-    for t, rc in ((_tensor(p=0), -1), (_tensor(g=0), -1), (_tensor(p=4097), -1), (_tensor(g=8194, dtype=0), -1),
-                  (_tensor(n=-1), -1), (_tensor(offset=100), -1), (_tensor(offset=-256), -1), (_tensor(dtype=2), -2)):
+    for t, rc in ((_tensor(p=0), -1), (_tensor(p=4097), -1), (_tensor(g=8194, dtype=0), -1),
+                  (_tensor(n=-1), -1), (_tensor(offset=100), -1), (_tensor(offset=-256), -1), (_tensor(dtype=2), -2), (_tensor(n=1 << 36), -2)):
         assert _step(lib, t) == rc, list(t)
     t = _tensor()
     for kw, rc in ((dict(count=-1), -1), (dict(states=2), -2), (dict(m=None), -1), (dict(v=8196), -1), (dict(master=4100), -1),
                    (dict(states=1), -1), (dict(states=1, ms=4096, vs=4098), -1), (dict(b1=1.0), -1), (dict(b2=-0.1), -1),
-                   (dict(eps=-1.0), -1), (dict(c1=0.0), -1), (dict(c2=float("nan")), -1)):
+                   (dict(eps=-1.0), -1), (dict(c1=0.0), -1), (dict(c2=float("nan")), -1), (dict(plan=None), -1), (dict(plan=4100), -1)):
         assert _step(lib, t, **kw) == rc, kw
+    buf = ctypes.create_string_buffer(4096)
+    at = (ctypes.addressof(buf) + 15) & ~15
+    n = lib.kda_adamw_plan_size(t, 1)
+    assert 0 < n <= 64 and lib.kda_adamw_plan(t, 1, at, n) == 0
+    assert lib.kda_adamw_plan(t, 1, at, n - 1) == -3 and lib.kda_adamw_plan(t, 1, None, n) == -1
+    assert lib.kda_adamw_plan(_tensor(p=0), 1, at, n) == -1
     assert _step(lib, None, count=1) == -1 and _step(lib, None, count=0) == 0
-    norm = lambda **kw: lib.kda_grad_norm(*{**dict(t=t, count=1, max_norm=1.0, out=4096, ws=8192, n=1 << 10, st=None), **kw}.values())  # noqa: E731
+    norm = lambda **kw: lib.kda_grad_norm(*{**dict(t=t, count=1, plan=4096, max_norm=1.0, out=4096, ws=8192, n=1 << 10, st=None), **kw}.values())  # noqa: E731
     for kw, rc in ((dict(out=None), -1), (dict(out=4098), -1), (dict(max_norm=0.0), -1), (dict(max_norm=float("nan")), -1),
-                   (dict(ws=None), -1), (dict(n=0), -3), (dict(count=-1), -1)):
+                   (dict(ws=None), -1), (dict(n=0), -3), (dict(count=-1), -1), (dict(plan=None), -1), (dict(plan=4100), -1)):
         assert norm(**kw) == rc, kw
     assert lib.kda_grad_norm_workspace_size(_tensor(n=100000), 1) >= 4
     mom = lambda **kw: lib.kda_adamw_moments(*{**dict(m=4096, v=4096, ms=4096, vs=4096, mo=4096, vo=4096, n=256, dt=1, st=None), **kw}.values())  # noqa: E731

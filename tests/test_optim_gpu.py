@@ -347,3 +347,33 @@ def test_train_step_of_a_classifier(states):
         # u = (1 - b1) g / (sqrt(1 - b2) |g| + eps): at most 0.45, within 1e-4 of it for the clip factor
         assert ((ma.double() - W).abs() <= 2.0 ** -20 * W.abs() + step.opt.lr * 1e-4).all()
         assert torch.equal(p.detach(), ma.to(p.dtype))
+
+
+def test_moved_parameters():
+    """Weights that were given new memory between two steps; one of another size is refused, as are
+    parameters that share memory."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.bfloat16] * len(SIZES), seed=8) for _ in range(2))
+    oa, ob = FusedAdamW(a), FusedAdamW(b)
+    for k in range(2):
+        for ps, o in ((a, oa), (b, ob)):
+            _grads(ps, 40 + k)
+            o.step(1.0)
+        for p in a:
+            p.data = p.data.clone()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    a[3].grad = None
+    a[3].data = torch.zeros(5, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="make a new optimizer"):
+        oa.step()
+    buf = torch.zeros(300, device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        FusedAdamW([torch.nn.Parameter(buf[:200]), torch.nn.Parameter(buf[100:])])
+    with pytest.raises(ValueError, match="overlap"):
+        FusedAdamW([b[0], b[0]])
+    with pytest.raises(ValueError, match="contiguous"):
+        FusedAdamW([torch.nn.Parameter(buf.view(30, 10).t())])
+    with pytest.raises(ValueError, match="state"):
+        FusedAdamW(b, state={"m": buf})
+    with pytest.raises(ValueError, match="elements"):
+        FusedAdamW(b, state={"m": buf, "v": buf})
