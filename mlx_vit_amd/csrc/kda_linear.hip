@@ -181,34 +181,35 @@ __device__ __forceinline__ void bias8(const GemmArgs& a, int n, float (&v)[8]) {
     if (!DG && a.bias && n < a.N) ldc8<T>(static_cast<const T*>(a.bias) + n, a.N - n, a.vec, v);
 }
 
-// The epilogue of a wave's 64 columns from n0 and 16 FM rows from m0, 32 rows at a
-// time through 8 KB of LDS of its own: the accumulators hold four columns of 16
-// rows a fragment, and leave as whole 128-byte (bf16) rows of 16-byte pieces.
-// Rows of 64 floats, the 16-byte piece c of row r at c ^ (r & 15), so that both
-// the fragments' writes (16 rows of a piece) and the reads are spread over the
-// banks.  acc[i][j]: columns 16 i, rows 16 j.
-template <typename T, int ACT, bool DG, bool EXACT, int FM>
-__device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, const f32x4 (&acc)[4][FM], char* lds) {
-    const int l = lane_id(), r16 = l & 15, g4 = l >> 4, q = l & 7;
+// The epilogue of a wave's 16 FN columns from n0 and 16 FM rows from m0, R rows (16
+// or 32) at a time through 64 FN R bytes of LDS of its own: the accumulators hold
+// four columns of 16 rows a fragment, and leave as whole rows (128 bytes of bf16
+// at FN = 4) of 16-byte pieces.  The 16-byte piece c of row r lies at c ^ (r's low
+// bits), so that both the fragments' writes (16 rows of a piece) and the reads
+// are spread over the banks.  acc[i][j]: columns 16 i, rows 16 j.
+template <typename T, int ACT, bool DG, bool EXACT, int R, int FN, int FM>
+__device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, const f32x4 (&acc)[FN][FM], char* lds) {
+    constexpr int RB = 64 * FN, KEY = 4 * FN - 1, LR = 2 * FN, RI = 64 / LR;   // row bytes, lanes a row, rows a read
+    const int l = lane_id(), r16 = l & 15, g4 = l >> 4, q = l % LR;
     const int n = n0 + 8 * q;
     float bias[8];
     bias8<T, DG>(a, n, bias);
 #pragma unroll
-    for (int h = 0; h < FM; h += 2) {
+    for (int h = 0; h < FM; h += R / 16) {
         wave_sync();   // the last part's reads come first
 #pragma unroll
-        for (int j = h; j < h + 2; ++j) {
+        for (int j = h; j < h + R / 16; ++j) {
             const int r = 16 * (j - h) + r16;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f32x4*>(lds + 256 * r + (((4 * i + g4) ^ r16) << 4)) = acc[i][j];
+            for (int i = 0; i < FN; ++i)
+                *reinterpret_cast<f32x4*>(lds + RB * r + (((4 * i + g4) ^ (r16 & KEY)) << 4)) = acc[i][j];
         }
         wave_sync();
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            const int r = 8 * it + (l >> 3), m = m0 + 16 * h + r;
-            const f32x4 x = *reinterpret_cast<const f32x4*>(lds + 256 * r + (((2 * q) ^ (r & 15)) << 4));
-            const f32x4 y = *reinterpret_cast<const f32x4*>(lds + 256 * r + (((2 * q + 1) ^ (r & 15)) << 4));
+        for (int it = 0; it < R / RI; ++it) {
+            const int r = RI * it + l / LR, m = m0 + 16 * h + r;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(lds + RB * r + (((2 * q) ^ (r & KEY)) << 4));
+            const f32x4 y = *reinterpret_cast<const f32x4*>(lds + RB * r + (((2 * q + 1) ^ (r & KEY)) << 4));
             float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             if (m < a.M && n < a.N) finish8<T, ACT, DG, EXACT>(a, m, n, v, bias);
         }
@@ -230,13 +231,15 @@ __device__ __forceinline__ void tile_of(int bid, int nb, int mt, int nt, int& mi
 // ----------------------------------------------------------------------------
 
 // chunk key of row r: rows of RB bytes along the contracted index (a fragment
-// read takes 16 rows of one chunk), or rows across it of at least 256 bytes (a
-// transposing read takes rows 8 g .. 8 g + 3 of 32 bytes)
+// read takes 16 rows of one chunk), or rows across it (a transposing read takes
+// rows 8 g .. 8 g + 3 of 32 bytes; of 128-byte rows two share a bank)
 template <int RB>
 __device__ __forceinline__ int key_k(int r) {
-    return RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+    // of 64-byte rows: a 16-byte read's 16 lanes are 0-3 and 12-15 of one quarter of the
+    // wave and 4-11 of the next, so the four keys pair up accordingly
+    return RB == 128 ? (r >> 1) & 7 : -(r >> 2) & 3;
 }
-__device__ __forceinline__ int key_t(int r) { return ((r & 3) << 1) | (r & 8); }   // 16 chunks at least
+__device__ __forceinline__ int key_t(int r) { return ((r & 3) << 1) | (r & 8); }
 
 template <int RB>
 __device__ __forceinline__ bf16x8 frag_k(const char* tile, int row0, int chunk) {
@@ -247,7 +250,7 @@ __device__ __forceinline__ bf16x8 frag_k(const char* tile, int row0, int chunk) 
 template <int RB>
 __device__ __forceinline__ bf16x8 frag_t(const char* tile, int n0, int k0) {
     const int l = lane_id(), j = l & 15, g = l >> 4, r = k0 + 8 * g + (j >> 2), b = 2 * (n0 + 4 * (j & 3));
-    const int at = (((b >> 4) ^ key_t(r)) << 4) + (b & 15);   // row r + 4 has the same key
+    const int at = (((b >> 4) ^ (key_t(r) & (RB / 16 - 1))) << 4) + (b & 15);   // row r + 4 has the same key
     const short4v x = ld_tr4(reinterpret_cast<const uint16_t*>(tile + r * RB + at));
     const short4v y = ld_tr4(reinterpret_cast<const uint16_t*>(tile + (r + 4) * RB + at));
     return __builtin_bit_cast(bf16x8, short8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
@@ -263,7 +266,7 @@ struct Dma {
     __device__ __forceinline__ static void place(int i, int w, int& r, int& c) {
         const int p = 1024 * (w + W * i) + 16 * lane_id();
         r = p / RB;
-        c = ((p % RB) >> 4) ^ (TR ? key_t(r) : key_k<RB>(r));
+        c = ((p % RB) >> 4) ^ (TR ? key_t(r) & (RB / 16 - 1) : key_k<RB>(r));
     }
     // rows and 16-byte chunks past the last read the last (not stored, or zeroed below)
     __device__ __forceinline__ void init(int64_t ld, int last_row, int last_chunk, int w) {
@@ -386,7 +389,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_bf16_kernel(const 
         }
     }
     lds_barrier();   // every wave has read the last step
-    finish_wave<uint16_t, ACT, DG, false, FM>(a, m0 + wm, n0 + wn, acc, lds + 8192 * w);
+    finish_wave<uint16_t, ACT, DG, false, 32>(a, m0 + wm, n0 + wn, acc, lds + 2048 * FN * w);
 }
 
 // ----------------------------------------------------------------------------
@@ -412,20 +415,35 @@ __device__ __forceinline__ void split3(const float4& x, uint2& h, uint2& m, uint
     l = make_uint2(__builtin_amdgcn_perm(c[1], c[0], HI), __builtin_amdgcn_perm(c[3], c[2], HI));
 }
 
-// A 128 x 32 (or, TR, 32 x 128) tile of fp32 rows through registers into three
-// bf16 planes of 8 KB
-template <bool TR>
+// An EDGE x 32 (or, TR, 32 x EDGE) tile of fp32 rows through TH threads' registers
+// into three bf16 planes
+template <int EDGE, int TH, bool TR>
 struct Stage32 {
-    static constexpr int RB = TR ? 256 : 64, PLANE = 8192;
-    float4 v[4];
+    static constexpr int RB = TR ? 2 * EDGE : 64, PLANE = 64 * EDGE, TPR = TR ? EDGE / 4 : 8;   // threads a row
+    static constexpr int STEP = TH / TPR, PER = 8 * EDGE / TH;                                  // rows apart, pieces a thread
+    float4 v[PER];
+    uint32_t off[PER];
+    // Byte offsets of this thread's pieces in a whole step; across the contracted
+    // index, what is past the last (`edge` exist) reads the last: not stored
+    __device__ __forceinline__ void init(int64_t ld, int edge) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            off[i] = 4u * (TR ? (uint32_t)row(i) * (uint32_t)ld + (uint32_t)min(col(), edge - 4)
+                              : (uint32_t)min(row(i), edge - 1) * (uint32_t)ld + (uint32_t)col());
+    }
+    __device__ __forceinline__ void load_whole(const float* base) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            v[i] = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(base) + off[i]);
+    }
     // row and first column of this thread's piece i
-    __device__ __forceinline__ static int row(int i) { return TR ? (threadIdx.x >> 5) + 8 * i : (threadIdx.x >> 3) + 32 * i; }
-    __device__ __forceinline__ static int col() { return TR ? 4 * (threadIdx.x & 31) : 4 * (threadIdx.x & 7); }
+    __device__ __forceinline__ static int row(int i) { return (int)threadIdx.x / TPR + STEP * i; }
+    __device__ __forceinline__ static int col() { return 4 * ((int)threadIdx.x % TPR); }
     // rows, cols: how many of them exist past (r0, c0); what does not is zero
     __device__ __forceinline__ void load(const float* base, int64_t ld, int rows, int cols, bool vec) {
         const int c = col();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < PER; ++i) {
             const int r = row(i);
             v[i] = r < rows && c < cols ? ldc4<float>(base + (size_t)r * ld + c, cols - c, vec && c + 4 <= cols)
                                         : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -434,9 +452,9 @@ struct Stage32 {
     __device__ __forceinline__ void store(char* tile) const {
         const int b = 2 * col();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < PER; ++i) {
             const int r = row(i);
-            char* p = tile + r * RB + (((b >> 4) ^ (TR ? key_t(r) : key_k<RB>(r))) << 4) + (b & 15);
+            char* p = tile + r * RB + (((b >> 4) ^ (TR ? key_t(r) & (RB / 16 - 1) : key_k<RB>(r))) << 4) + (b & 15);
             uint2 h, m, l;
             split3(v[i], h, m, l);
             *reinterpret_cast<uint2*>(p) = h;
@@ -446,103 +464,120 @@ struct Stage32 {
     }
 };
 
-// C tile of 128 x 128 by 2 x 2 waves, 32 of the contracted index a step.  AT, BT:
+// C tile of BM x BN by WR x WC waves, 32 of the contracted index a step.  AT, BT:
 // the operand's rows run across the contracted index.  PART: one of a.splits
 // parts of it, into a.part (and with a.bpart A's column sums).
-template <bool AT, bool BT, int ACT, bool DG, bool PART>
-__global__ __launch_bounds__(256, 2) void kda_linear_f32_kernel(const GemmArgs a) {
-    constexpr int BK = 32, RBA = AT ? 256 : 64, RBB = BT ? 256 : 64, PL = 8192;
-    __shared__ __attribute__((aligned(1024))) char lds[6 * PL];
+template <int BM, int BN, int WR, int WC, bool AT, bool BT, int ACT, bool DG, bool PART>
+__global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_f32_kernel(const GemmArgs a) {
+    constexpr int BK = 32, TH = 64 * WR * WC, FM = BM / WR / 16, FN = BN / WC / 16;
+    constexpr int RBA = AT ? 2 * BM : 64, RBB = BT ? 2 * BN : 64, PA = 64 * BM, PB = 64 * BN, LDS = 3 * (PA + PB);
+    static_assert(TH / 64 * 64 * FN * 16 <= LDS, "the epilogue's rows");
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), r16 = l & 15, g4 = l >> 4;
-    const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
+    const int wm = (w / WC) * (BM / WR), wn = (w % WC) * (BN / WC);
     const int tiles = a.mt * a.nt, split = PART ? (int)blockIdx.x / tiles : 0;
     int mi, ni;
     tile_of((int)blockIdx.x - split * tiles, tiles, a.mt, a.nt, mi, ni);
-    const int m0 = mi * 128, n0 = ni * 128;
+    const int m0 = mi * BM, n0 = ni * BN;
     const int k0 = PART ? split * a.k_per : 0, k1 = PART ? min(a.K, k0 + a.k_per) : a.K;
     const float *A = static_cast<const float*>(a.a), *B = static_cast<const float*>(a.b);
-    Stage32<AT> sa;
-    Stage32<BT> sb;
+    Stage32<BM, TH, AT> sa;
+    Stage32<BN, TH, BT> sb;
+    const bool whole_a = a.vec_a && (!AT || a.M % 4 == 0), whole_b = a.vec_b && (!BT || a.N % 4 == 0);
+    sa.init(a.lda, a.M - m0);
+    sb.init(a.ldb, a.N - n0);
     auto load = [&](int k) {
-        if constexpr (AT) sa.load(A + (size_t)k * a.lda + m0, a.lda, k1 - k, a.M - m0, a.vec_a);
-        else sa.load(A + (size_t)m0 * a.lda + k, a.lda, a.M - m0, k1 - k, a.vec_a);
-        if constexpr (BT) sb.load(B + (size_t)k * a.ldb + n0, a.ldb, k1 - k, a.N - n0, a.vec_b);
-        else sb.load(B + (size_t)n0 * a.ldb + k, a.ldb, a.N - n0, k1 - k, a.vec_b);
+        const float* pa = AT ? A + (size_t)k * a.lda + m0 : A + (size_t)m0 * a.lda + k;
+        const float* pb = BT ? B + (size_t)k * a.ldb + n0 : B + (size_t)n0 * a.ldb + k;
+        const bool whole = k + BK <= k1;
+        if (whole && whole_a) sa.load_whole(pa);
+        else if constexpr (AT) sa.load(pa, a.lda, k1 - k, a.M - m0, a.vec_a);
+        else sa.load(pa, a.lda, a.M - m0, k1 - k, a.vec_a);
+        if (whole && whole_b) sb.load_whole(pb);
+        else if constexpr (BT) sb.load(pb, a.ldb, k1 - k, a.N - n0, a.vec_b);
+        else sb.load(pb, a.ldb, a.N - n0, k1 - k, a.vec_b);
     };
-    f32x4 acc[4][4];
+    f32x4 acc[FN][FM];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = zero4();
+        for (int j = 0; j < FM; ++j) acc[i][j] = zero4();
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     const bool sums = PART && a.bpart && ni == 0;
     load(k0);
     for (int k = k0; k < k1; k += BK) {
         if (k > k0) lds_barrier();   // every wave has read the step before
         sa.store(lds);
-        sb.store(lds + 3 * PL);
+        sb.store(lds + 3 * PA);
         if (sums)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < Stage32<BM, TH, AT>::PER; ++i) {
                 sum.x += sa.v[i].x; sum.y += sa.v[i].y; sum.z += sa.v[i].z; sum.w += sa.v[i].w;
             }
         lds_barrier();
         if (k + BK < k1) load(k + BK);
         // products of parts down to 2^-16 of the largest: hh, hm, mh, hl, lh, mm
-        bf16x8 fb[3][4];
+        bf16x8 fb[3][FN];
 #pragma unroll
         for (int p = 0; p < 3; ++p)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const char* t = lds + (3 + p) * PL;
+            for (int i = 0; i < FN; ++i) {
+                const char* t = lds + 3 * PA + p * PB;
                 if constexpr (BT) fb[p][i] = frag_t<RBB>(t, wn + 16 * i, 0);
                 else fb[p][i] = frag_k<RBB>(t, wn + 16 * i, 0);
             }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < FM; ++j) {
             bf16x8 fa[3];
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
-                if constexpr (AT) fa[p] = frag_t<RBA>(lds + p * PL, wm + 16 * j, 0);
-                else fa[p] = frag_k<RBA>(lds + p * PL, wm + 16 * j, 0);
+                if constexpr (AT) fa[p] = frag_t<RBA>(lds + p * PA, wm + 16 * j, 0);
+                else fa[p] = frag_k<RBA>(lds + p * PA, wm + 16 * j, 0);
             }
-            // smallest first
+            // A step's products sum from zero, smallest first, and join the accumulator by
+            // an ordinary addition: the matrix unit rounds its sums downwards, and 72
+            // such steps (K = 384) left a bias that a sum over 6272 rows showed (1.1e-6
+            // of a bias gradient, 4e-7 in fp32 arithmetic).
+            f32x4 t[FN];
 #pragma unroll
             for (int q = 0; q < 6; ++q) {
-                constexpr int PB[6] = {0, 2, 1, 0, 1, 0}, PA[6] = {2, 0, 1, 1, 0, 0};
+                constexpr int QB[6] = {0, 2, 1, 0, 1, 0}, QA[6] = {2, 0, 1, 1, 0, 0};
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[PB[q]][i], fa[PA[q]], acc[i][j], 0, 0, 0);
+                for (int i = 0; i < FN; ++i)
+                    t[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[QB[q]][i], fa[QA[q]], q == 0 ? zero4() : t[i], 0, 0, 0);
             }
+#pragma unroll
+            for (int i = 0; i < FN; ++i) acc[i][j] += t[i];
         }
     }
     if constexpr (PART) {
         float* part = a.part + (size_t)split * a.M * a.N;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < FN; ++i) {
             const int n = n0 + wn + 16 * i + 4 * g4;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < FM; ++j) {
                 const int m = m0 + wm + 16 * j + r16;
                 if (m < a.M && n < a.N)
                     stc4<float>(part + (size_t)m * a.N + n, make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]),
                                 a.N - n, a.vec);
             }
         }
-        if (sums) {   // the eight threads of a column in order (AT: 32 threads a row)
+        if (sums) {   // the threads of a column in order
             lds_barrier();
             reinterpret_cast<float4*>(lds)[threadIdx.x] = sum;
             lds_barrier();
-            if (threadIdx.x < 128 && m0 + (int)threadIdx.x < a.M) {
+            if (threadIdx.x < BM && m0 + (int)threadIdx.x < a.M) {
                 float s = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s += reinterpret_cast<const float*>(lds)[128 * i + threadIdx.x];
+                for (int i = 0; i < 4 * TH / BM; ++i) s += reinterpret_cast<const float*>(lds)[BM * i + threadIdx.x];
                 a.bpart[(size_t)split * a.M + m0 + threadIdx.x] = s;
             }
         }
     } else {
+        constexpr int R = 64 * FN * 32 * TH / 64 <= LDS && FM % 2 == 0 ? 32 : 16;
         lds_barrier();
-        finish_wave<float, ACT, DG, true, 4>(a, m0 + wm, n0 + wn, acc, lds + 8192 * w);
+        finish_wave<float, ACT, DG, true, R>(a, m0 + wm, n0 + wn, acc, lds + 64 * FN * R * w);
     }
 }
 
@@ -686,6 +721,31 @@ hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
+// fp32 tiles, by how many there are for 256 CUs (6272 rows: 384 -> 1536, 588 tiles of
+// 128 x 128: 65 us, 1176 of 128 x 64: 52, 2352 of 64 x 64: 56; 1536 -> 384, a quarter
+// as many: 94, 74, 62; 4096 x 4096 x 4096, 1024 of 128 x 128: 663, 727, 815)
+template <bool BT, int ACT, bool DG>
+hipError_t launch_f32(GemmArgs& a, hipStream_t st) {
+    const int64_t m128 = (a.M + 127) / 128, n128 = (a.N + 127) / 128, n64 = (a.N + 63) / 64;
+    if (m128 * n128 >= 1024) {
+        a.mt = (int)m128;
+        a.nt = (int)n128;
+        hipLaunchKernelGGL((kda_linear_f32_kernel<128, 128, 2, 2, false, BT, ACT, DG, false>), dim3((unsigned)a.mt * a.nt),
+                           dim3(256), 0, st, a);
+    } else if (m128 * n64 >= 512) {
+        a.mt = (int)m128;
+        a.nt = (int)n64;
+        hipLaunchKernelGGL((kda_linear_f32_kernel<128, 64, 2, 2, false, BT, ACT, DG, false>), dim3((unsigned)a.mt * a.nt),
+                           dim3(256), 0, st, a);
+    } else {
+        a.mt = (a.M + 63) / 64;
+        a.nt = (int)n64;
+        hipLaunchKernelGGL((kda_linear_f32_kernel<64, 64, 2, 2, false, BT, ACT, DG, false>), dim3((unsigned)a.mt * a.nt),
+                           dim3(256), 0, st, a);
+    }
+    return hipGetLastError();
+}
+
 template <int ACT>
 hipError_t launch_fwd(GemmArgs& a, int bf16, hipStream_t st) {
     if (a.M <= FEW_ROWS) {
@@ -696,22 +756,12 @@ hipError_t launch_fwd(GemmArgs& a, int bf16, hipStream_t st) {
         else hipLaunchKernelGGL((kda_linear_few_kernel<float, ACT>), grid, block, 0, st, a);
         return hipGetLastError();
     }
-    if (bf16) return launch_bf16<false, ACT, false>(a, st);
-    a.mt = (a.M + 127) / 128;
-    a.nt = (a.N + 127) / 128;
-    hipLaunchKernelGGL((kda_linear_f32_kernel<false, false, ACT, false, false>), dim3((unsigned)a.mt * a.nt), dim3(256), 0,
-                       st, a);
-    return hipGetLastError();
+    return bf16 ? launch_bf16<false, ACT, false>(a, st) : launch_f32<false, ACT, false>(a, st);
 }
 
 template <int ACT>
 hipError_t launch_dgrad(GemmArgs& a, int bf16, hipStream_t st) {
-    if (bf16) return launch_bf16<true, ACT, true>(a, st);
-    a.mt = (a.M + 127) / 128;
-    a.nt = (a.N + 127) / 128;
-    hipLaunchKernelGGL((kda_linear_f32_kernel<false, true, ACT, true, false>), dim3((unsigned)a.mt * a.nt), dim3(256), 0,
-                       st, a);
-    return hipGetLastError();
+    return bf16 ? launch_bf16<true, ACT, true>(a, st) : launch_f32<true, ACT, true>(a, st);
 }
 
 hipError_t dgrad(int act, int bf16, GemmArgs& a, hipStream_t st) {
@@ -736,11 +786,12 @@ hipError_t launch_act_bwd(const void* dy, const void* z, void* dz, int64_t ld_dy
     return hipGetLastError();
 }
 
-// Parts of the m rows that wgrad's sum is split into: two workgroups on each
-// of 256 CUs, at least 8 steps each
+// Parts of the m rows that wgrad's sum is split into: a workgroup on each of 256
+// CUs, at least 8 steps each (6272 rows, 1536 x 384: 7 parts in tiles of 128 x 128
+// by eight waves 50 us, 14 by four waves 53 and twice the partial sums)
 void wgrad_plan(int M, int N, int K, int* splits, int* per) {
     const int tiles = ((N + 127) / 128) * ((K + 127) / 128), steps = (M + 31) / 32;
-    const int s = std::max(1, std::min(512 / std::max(tiles, 1), steps / 8));
+    const int s = std::max(1, std::min(256 / std::max(tiles, 1), steps / 8));
     *per = (steps + s - 1) / s * 32;
     *splits = (M + *per - 1) / *per;
 }
@@ -797,8 +848,8 @@ hipError_t wgrad_f32(const Wgrad& g, int M, char* ws, hipStream_t st) {
     a.vec = K % 4 == 0;
     a.vec_a = reinterpret_cast<uintptr_t>(a.a) % 16 == 0 && a.lda % 4 == 0;
     a.vec_b = reinterpret_cast<uintptr_t>(a.b) % 16 == 0 && a.ldb % 4 == 0;
-    hipLaunchKernelGGL((kda_linear_f32_kernel<true, true, 0, false, true>), dim3((unsigned)(a.mt * a.nt * a.splits)),
-                       dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kda_linear_f32_kernel<128, 128, 4, 2, true, true, 0, false, true>), dim3((unsigned)(a.mt * a.nt * a.splits)),
+                       dim3(512), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const size_t total = (size_t)N * K + N;
