@@ -389,6 +389,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_bf16_kernel(const 
         }
     }
     lds_barrier();   // every wave has read the last step
+    static_assert(W * 64 * FN * 32 <= NST * STAGE, "the epilogue's rows");
     finish_wave<uint16_t, ACT, DG, false, 32>(a, m0 + wm, n0 + wn, acc, lds + 2048 * FN * w);
 }
 
@@ -710,15 +711,42 @@ bool groups_ok(const void* p, int64_t ld, int es) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (16 / es) == 0);
 }
 
-template <bool BT, int ACT, bool DG>
-hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
-    constexpr int BM = 128, BN = 128, BK = 64, NST = 2, WR = 4, WC = 2;
+template <int BM, int BN, int WR, int WC, bool BT, int ACT, bool DG>
+hipError_t launch_tiles(GemmArgs& a, hipStream_t st) {
+    constexpr int BK = 64, NST = 2;
     constexpr size_t LDS = (size_t)NST * (BM + BN) * 2 * BK;
+    const auto kernel = kda_linear_bf16_kernel<BM, BN, BK, NST, WR, WC, BT, ACT, DG>;
+    if constexpr (LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
+        if (e != hipSuccess) return e;
+    }
     a.mt = (a.M + BM - 1) / BM;
     a.nt = (a.N + BN - 1) / BN;
-    hipLaunchKernelGGL((kda_linear_bf16_kernel<BM, BN, BK, NST, WR, WC, BT, ACT, DG>), dim3((unsigned)a.mt * a.nt),
-                       dim3(64 * WR * WC), LDS, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.mt * a.nt), dim3(64 * WR * WC), LDS, st, a);
     return hipGetLastError();
+}
+
+// bf16 tiles, by how many there are for 256 CUs and what a tile's way in and out
+// costs beside its steps (us):
+//                              256 x 256  128 x 128  64 x 128  64 x 64
+//   16384 x 8192, K 2048             490        616       628      738
+//   25088 x  384, K 1536              36         42        39       47
+//   12544 x 2048, K 768, gelu         53         57        58       69
+//   25088 x 1536, K 384, gelu         56         51        53       61
+//   the same, times gelu'(z)          58         65        64       67
+//    4096 x 1024, K 1024              25         14        13       15
+//    1571 x  400, K 776               26         12        10        8
+// One workgroup of 256 x 256 fills a CU, so nothing runs beside its epilogue: it
+// takes half the data a product, and pays where the steps outweigh the epilogue
+// (K from 512) or the epilogue reads as much as it writes, and most CUs have one.
+template <bool BT, int ACT, bool DG>
+hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
+    const int64_t m256 = (a.M + 255) / 256, n256 = (a.N + 255) / 256, m64 = (a.M + 63) / 64, n128 = (a.N + 127) / 128;
+    if (m256 * n256 >= 192 && (a.K >= 512 || (DG && ACT != 0))) return launch_tiles<256, 256, 4, 4, BT, ACT, DG>(a, st);
+    if ((a.M + 127) / 128 * n128 >= 1024) return launch_tiles<128, 128, 4, 2, BT, ACT, DG>(a, st);
+    if (m64 * n128 >= 256) return launch_tiles<64, 128, 2, 2, BT, ACT, DG>(a, st);
+    return launch_tiles<64, 64, 2, 2, BT, ACT, DG>(a, st);
 }
 
 // fp32 tiles, by how many there are for 256 CUs (6272 rows: 384 -> 1536, 588 tiles of

@@ -78,14 +78,15 @@ class Val:
         return Val(self.v * d.v, self.e * d.mag + self.v.abs() * d.e + 2.0 ** -23 * self.mag * d.mag)
 
 
-def _val(t):
-    return None if t is None else Val(t.detach().double().cpu())
+def _val(t, dev):
+    return None if t is None else Val(t.detach().to(dev).double())
 
 
 def linear_act(x, w, b, r, name, dy=None):
     """{"y", "dx", "dw", "db", "dr"}: Val each, rounded as the op rounds (gradients with dy)."""
     dt = x.dtype
-    x, w, b, r, dy = (_val(t) for t in (x, w, b, r, dy))
+    dev = x.device
+    x, w, b, r, dy = (_val(t, dev) for t in (x, w, b, r, dy))
     z = x.mm(w.t())
     if b is not None:
         z = z + Val(b.v.expand(z.v.shape))
@@ -102,7 +103,8 @@ def linear_act(x, w, b, r, name, dy=None):
 def mlp(x, w1, b1, w2, b2, r, name, dy=None):
     """{"y", "dx", "dw1", "db1", "dw2", "db2", "dr"}."""
     dt = x.dtype
-    x, w1, b1, w2, b2, r, dy = (_val(t) for t in (x, w1, b1, w2, b2, r, dy))
+    dev = x.device
+    x, w1, b1, w2, b2, r, dy = (_val(t, dev) for t in (x, w1, b1, w2, b2, r, dy))
     z = x.mm(w1.t())
     if b1 is not None:
         z = z + Val(b1.v.expand(z.v.shape))
@@ -121,7 +123,7 @@ def mlp(x, w1, b1, w2, b2, r, name, dy=None):
 
 
 def check(name, got, want):
-    got = got.detach().double().cpu().reshape(want.v.shape)
+    got = got.detach().double().to(want.v.device).reshape(want.v.shape)
     off = (got - want.v).abs() - want.e
     assert torch.isfinite(got).all(), f"{name}: not finite"
     worst = off.max().item() if off.numel() else 0.0

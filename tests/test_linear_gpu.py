@@ -83,6 +83,35 @@ def test_mlp_forward_and_gradients(size, dtype):
             L.check(n, g, want[n])
 
 
+# Shapes for each tile size the launches choose from (by the number of tiles), ending inside one:
+# bf16 256 x 256 (K from 512, and the activation's derivative at any K), 128 x 128, 64 x 128, 64 x 64;
+# fp32 128 x 128, 128 x 64, 64 x 64
+TILED = [(6210, 2049, 520, "bf16", "gelu"), (5000, 3300, 72, "bf16", "silu"), (2100, 1030, 200, "bf16", None),
+         (5000, 3300, 40, "fp32", "gelu"), (4200, 1030, 72, "fp32", None), (700, 513, 136, "fp32", "silu")]
+
+
+@pytest.mark.parametrize("M,N,K,dtype,act", TILED)
+def test_every_tile_size(M, N, K, dtype, act):
+    from mlx_vit_amd import linear_act, mlp
+    dt = DT[dtype]
+    x, w, b, r, dy = _inputs(M, K, N, dt, seed=200)
+    want = L.linear_act(x, w, b, r, act, dy)
+    leaves = _leaves(x, w, b, r)
+    y = linear_act(x, w, b, r, act)
+    L.check("y", y, want["y"])
+    for n, g in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves[:3], dy)):
+        L.check(n, g, want[n])
+    # as a block's second map: dgrad over K' = K with the derivative of the first's activation, N wide
+    x, w1, b1, _, _ = _inputs(M, 24, N, dt, True, False, seed=210)
+    _, w2, b2, _, dy = _inputs(M, N, K, dt, True, False, seed=220)
+    want = L.mlp(x, w1, b1, w2, b2, None, "gelu", dy)
+    leaves = _leaves(x, w1, b1, w2, b2)
+    y = mlp(x, w1, b1, w2, b2)
+    L.check("y", y, want["y"])
+    for n, g in zip(("dx", "dw1", "db1", "dw2", "db2"), torch.autograd.grad(y, leaves, dy)):
+        L.check(n, g, want[n])
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_strided_operands(dtype):
     """Column slices, a transposed weight, a 3-d input, rows behind an offset of one
