@@ -301,27 +301,24 @@ __device__ __forceinline__ void zero_tail(char* tile, int valid) {
     }
 }
 
-// at most n of the last steps' DMA (L instructions each) outstanding
-template <int L, int MAX>
-__device__ __forceinline__ void wait_steps(int n) {
-    if constexpr (MAX > 0) {
-        if (n >= MAX) {
-            dma_wait<MAX * L>();
-            return;
-        }
-        wait_steps<L, MAX - 1>(n);
-    } else {
-        dma_wait<0>();
-    }
-}
-
-// C tile of BM x BN by WR x WC waves, BK of the contracted index a step, NST
-// buffers.  BT: B's rows run across the contracted index (dgrad).
-template <int BM, int BN, int BK, int NST, int WR, int WC, bool BT, int ACT, bool DG>
-__global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_bf16_kernel(const GemmArgs a) {
-    constexpr int W = WR * WC, RBA = 2 * BK, RBB = BT ? 2 * BN : 2 * BK, ROWB = BT ? BK : BN;
+// C tile of BM x BN by WR x WC waves, 64 of the contracted index a step, two
+// buffers.  BT: B's rows run across the contracted index (dgrad).  WPE: waves a
+// SIMD that the registers have to leave room for.
+//
+// AHEAD: a step is two halves of 32, and a wave reads a half's fragments before the
+// products of the half before, so that the matrix unit need not wait for LDS.
+// There is one barrier a step, in its middle: by then a wave holds its second
+// half in registers and its share of the next step has landed, so behind it the
+// next step's first half can be read and this step's buffer filled with the step
+// after the next.  (16384 x 2048 x 8192 in tiles of 128 x 128: 622 -> 526 us.)  It
+// takes a second set of fragments, which sixteen waves of 64 x 64 have no
+// registers for: there four waves a SIMD hide the reads.
+template <int BM, int BN, int WR, int WC, int WPE, bool AHEAD, bool BT, int ACT, bool DG>
+__global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(const GemmArgs a) {
+    constexpr int BK = 64, W = WR * WC, RBA = 2 * BK, RBB = BT ? 2 * BN : 2 * BK, ROWB = BT ? BK : BN;
     constexpr int SA = BM * RBA, STAGE = SA + ROWB * RBB;
     constexpr int FM = BM / WR / 16, FN = BN / WC / 16;
+    static_assert(W * 64 * FN * 32 <= 2 * STAGE && FM % 2 == 0 && FN <= 4, "the epilogue's rows");
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), r16 = l & 15, g4 = l >> 4;
     const int wm = (w / WC) * (BM / WR), wn = (w % WC) * (BN / WC);
@@ -339,57 +336,115 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_bf16_kernel(const 
     const char* ga = static_cast<const char*>(a.a) + (size_t)m0 * (2 * a.lda);
     const char* gb = static_cast<const char*>(a.b) + (BT ? (size_t)n0 * 2 : (size_t)n0 * (2 * a.ldb));
     const int64_t stepb = BT ? 2 * BK * a.ldb : 2 * BK;
-    const int steps = (a.K + BK - 1) / BK, tail = a.K - (steps - 1) * BK;
-    auto issue = [&](int s) {
-        const uint32_t st = base + (uint32_t)((s % NST) * STAGE);
-        if (s == steps - 1 && tail < BK) {
-            da.init(a.lda, a.M - 1 - m0, (tail - 1) / 8, w);
-            if constexpr (BT) db.init(a.ldb, tail - 1, (a.N - 1 - n0) / 8, w);
-            else db.init(a.ldb, a.N - 1 - n0, (tail - 1) / 8, w);
-        }
+    const int steps = a.K / BK, tail = a.K % BK;
+    auto issue = [&](int buf) {
+        const uint32_t st = base + (uint32_t)(buf * STAGE);
         da.issue(ga, st, w);
         db.issue(gb, st + SA, w);
         ga += 2 * BK;
         gb += stepb;
     };
-    for (int s = 0; s < min(steps, NST - 1); ++s) issue(s);
     f32x4 acc[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = zero4();
-    // Each step: this wave's share of it has landed (the later steps' stays in
-    // flight), barrier -- so every wave's has, and every wave has read the step
-    // before, whose buffer is filled next -- then issue and compute.
-    for (int s = 0; s < steps; ++s) {
-        wait_steps<L, NST - 2>(min(NST - 2, steps - 1 - s));
-        lds_barrier();
-        char* st = lds + (s % NST) * STAGE;
-        if (s == steps - 1 && tail < BK) {
-            zero_tail<BM, RBA, false, 64 * W>(st, tail);
-            zero_tail<ROWB, RBB, BT, 64 * W>(st + SA, tail);
-            lds_barrier();
+    // A fragment's place within its half depends on the lane alone (frag_k's key on
+    // r16): buffer and fragment are immediate offsets
+    const char *pa[2], *pb[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int at = r16 * 128 + (((4 * h + g4) ^ key_k<128>(r16)) << 4);
+        pa[h] = lds + wm * RBA + at;
+        pb[h] = lds + SA + wn * 128 + at;   // !BT
+    }
+    struct Frags {
+        bf16x8 a[FM], b[FN];
+    };
+    auto read = [&](Frags& f, int buf, int h) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            if constexpr (BT) f.b[i] = frag_t<RBB>(lds + buf * STAGE + SA, wn + 16 * i, 32 * h);
+            else f.b[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(pb[h] + buf * STAGE + 16 * i * 128));
         }
-        if (s + NST - 1 < steps) issue(s + NST - 1);
 #pragma unroll
-        for (int ks = 0; ks < BK / 32; ++ks) {
-            bf16x8 fa[FM], fb[FN];
+        for (int j = 0; j < FM; ++j)
+            f.a[j] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(pa[h] + buf * STAGE + 16 * j * 128));
+    };
+    auto multiply = [&](const Frags& f) {
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                if constexpr (BT) fb[i] = frag_t<RBB>(st + SA, wn + 16 * i, 32 * ks);
-                else fb[i] = frag_k<RBB>(st + SA, wn + 16 * i, 4 * ks);
-            }
-#pragma unroll
-            for (int j = 0; j < FM; ++j) fa[j] = frag_k<RBA>(st, wm + 16 * j, 4 * ks);
+        for (int j = 0; j < FM; ++j)
 #pragma unroll
             for (int i = 0; i < FN; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b[i], f.a[j], acc[i][j], 0, 0, 0);
+    };
+    // Before each barrier this wave's share of the step has landed; behind it every
+    // wave's has, and every wave has read the step before (AHEAD: its second half is
+    // in registers)
+    if constexpr (AHEAD) {
+        if (steps > 0) {
+            issue(0);
+            if (steps > 1) {
+                issue(1);
+                dma_wait<L>();
+            } else {
+                dma_wait<0>();
+            }
+            lds_barrier();
+            Frags f, g;
+            read(f, 0, 0);
+            auto step = [&](int s, int buf) {
+                read(g, buf, 1);
+                multiply(f);
+                if (s + 1 < steps) {
+                    dma_wait<0>();
+                    lds_barrier();
+                    if (s + 2 < steps) issue(buf);
+                    read(f, 1 - buf, 0);
+                }
+                multiply(g);
+            };
+            int s = 0;
+            for (; s + 1 < steps; s += 2) {
+                step(s, 0);
+                step(s + 1, 1);
+            }
+            if (s < steps) step(s, 0);
+        }
+    } else {
+        if (steps > 0) issue(0);
+#pragma unroll 1
+        for (int s = 0; s < steps; ++s) {
+            dma_wait<0>();
+            lds_barrier();
+            if (s + 1 < steps) issue(1 - (s & 1));
 #pragma unroll
-                for (int j = 0; j < FM; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j], acc[i][j], 0, 0, 0);
+            for (int h = 0; h < 2; ++h) {
+                Frags f;
+                read(f, s & 1, h);
+                multiply(f);
+            }
+        }
+    }
+    if (tail > 0) {   // the part of a step: what lies past K zero in both operands
+        lds_barrier();
+        da.init(a.lda, a.M - 1 - m0, (tail - 1) / 8, w);
+        if constexpr (BT) db.init(a.ldb, tail - 1, (a.N - 1 - n0) / 8, w);
+        else db.init(a.ldb, a.N - 1 - n0, (tail - 1) / 8, w);
+        issue(0);
+        dma_wait<0>();
+        lds_barrier();
+        zero_tail<BM, RBA, false, 64 * W>(lds, tail);
+        zero_tail<ROWB, RBB, BT, 64 * W>(lds + SA, tail);
+        lds_barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Frags f;
+            read(f, 0, h);
+            multiply(f);
         }
     }
     lds_barrier();   // every wave has read the last step
-    static_assert(W * 64 * FN * 32 <= NST * STAGE, "the epilogue's rows");
     finish_wave<uint16_t, ACT, DG, false, 32>(a, m0 + wm, n0 + wn, acc, lds + 2048 * FN * w);
 }
 
@@ -711,11 +766,10 @@ bool groups_ok(const void* p, int64_t ld, int es) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (16 / es) == 0);
 }
 
-template <int BM, int BN, int WR, int WC, bool BT, int ACT, bool DG>
+template <int BM, int BN, int WR, int WC, int WPE, bool AHEAD, bool BT, int ACT, bool DG>
 hipError_t launch_tiles(GemmArgs& a, hipStream_t st) {
-    constexpr int BK = 64, NST = 2;
-    constexpr size_t LDS = (size_t)NST * (BM + BN) * 2 * BK;
-    const auto kernel = kda_linear_bf16_kernel<BM, BN, BK, NST, WR, WC, BT, ACT, DG>;
+    constexpr size_t LDS = 2 * (BM + BN) * 128;
+    const auto kernel = kda_linear_bf16_kernel<BM, BN, WR, WC, WPE, AHEAD, BT, ACT, DG>;
     if constexpr (LDS > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
@@ -727,26 +781,26 @@ hipError_t launch_tiles(GemmArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-// bf16 tiles, by how many there are for 256 CUs and what a tile's way in and out
-// costs beside its steps (us):
-//                              256 x 256  128 x 128  64 x 128  64 x 64
-//   16384 x 8192, K 2048             490        616       628      738
-//   25088 x  384, K 1536              36         42        39       47
-//   12544 x 2048, K 768, gelu         53         57        58       69
-//   25088 x 1536, K 384, gelu         56         51        53       61
-//   the same, times gelu'(z)          58         65        64       67
-//    4096 x 1024, K 1024              25         14        13       15
-//    1571 x  400, K 776               26         12        10        8
+// bf16 tiles, by how many there are for 256 CUs (us):
+//                               256 x 256   128 x 128   64 x 64
+//   16384 x 8192, K 2048              503         526       740
+//   25088 x  384, K 1536               38          41        47
+//   12544 x  768, K 768                22          25        26   (147 of the largest)
+//   25088 x 1536, K 384, gelu          60          54        61
+//   the same, times gelu'(z)           62          57        65
+//    4096 x 1024, K 1024               25          11        14
+//    2048 x 2048, K 512                16           8.0       9.3
+//    2048 x 1024, K 1024               24          10         7.8
+//    6272 x  384, K 1536               33          19        15
 // One workgroup of 256 x 256 fills a CU, so nothing runs beside its epilogue: it
 // takes half the data a product, and pays where the steps outweigh the epilogue
-// (K from 512) or the epilogue reads as much as it writes, and most CUs have one.
+// and most CUs have one.
 template <bool BT, int ACT, bool DG>
 hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
-    const int64_t m256 = (a.M + 255) / 256, n256 = (a.N + 255) / 256, m64 = (a.M + 63) / 64, n128 = (a.N + 127) / 128;
-    if (m256 * n256 >= 192 && (a.K >= 512 || (DG && ACT != 0))) return launch_tiles<256, 256, 4, 4, BT, ACT, DG>(a, st);
-    if ((a.M + 127) / 128 * n128 >= 1024) return launch_tiles<128, 128, 4, 2, BT, ACT, DG>(a, st);
-    if (m64 * n128 >= 256) return launch_tiles<64, 128, 2, 2, BT, ACT, DG>(a, st);
-    return launch_tiles<64, 64, 2, 2, BT, ACT, DG>(a, st);
+    const int64_t m256 = (a.M + 255) / 256, n256 = (a.N + 255) / 256, m128 = (a.M + 127) / 128, n128 = (a.N + 127) / 128;
+    if (m256 * n256 >= 144 && a.K >= 512) return launch_tiles<256, 256, 4, 4, 4, false, BT, ACT, DG>(a, st);
+    if (m128 * n128 >= 192) return launch_tiles<128, 128, 2, 4, 4, true, BT, ACT, DG>(a, st);
+    return launch_tiles<64, 64, 2, 2, 4, true, BT, ACT, DG>(a, st);
 }
 
 // fp32 tiles, by how many there are for 256 CUs (6272 rows: 384 -> 1536, 588 tiles of

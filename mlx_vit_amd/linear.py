@@ -36,12 +36,13 @@ ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2}
 FEW_ROWS = 64        # up to here a forward's operands may have any alignment (kda_linear_fwd)
 MAX_STRIDE = 1 << 21
 _NULL = contextlib.nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_grad_enabled = torch.is_grad_enabled
 
 
 def _on(dev: torch.device):
     """Launches go to the tensors' device, whatever the current one is."""
-    return _NULL if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _NULL if dev.index == _current_device() else torch.cuda.device(dev)
 
 
 def _up8(n: int) -> int:
@@ -81,14 +82,14 @@ def _whole_rows(x: torch.Tensor, w: torch.Tensor, stream: int) -> Tuple[torch.Te
     return out[0], out[1]
 
 
-def _forward(x2: torch.Tensor, K: int, w: torch.Tensor, bias, res2, act: int, y: torch.Tensor,
-             z: Optional[torch.Tensor], train: bool):
-    """y <- act(x2 w^T + bias) + res2 for x2 (M, K or wider), w (N, K), y and z (M, N
-    or wider).  Returns x2 and w as the kernels read them, with ``train`` also the
-    backward's."""
+def _forward(x2: torch.Tensor, K: int, w: torch.Tensor, bias, res2, act: int, y: int, ld_y: int, z: Optional[int],
+             ld_z: int, train: bool):
+    """y <- act(x2 w^T + bias) + res2 for x2 (M, K or wider), w (N, K); y and z: addresses
+    and row strides of (M, N) outputs.  Returns x2 and w as the kernels read them,
+    with ``train`` also the backward's."""
     M, N = x2.shape[0], w.shape[0]
     code = _DTYPE_CODE[w.dtype]
-    stream = _raw_stream(w.device.index)
+    stream = _raw_stream(w.get_device())
     x2, w = _rows(x2), _rows(w)
     if code and (train or M > FEW_ROWS):
         x2, w = _whole_rows(x2, w, stream)
@@ -99,8 +100,8 @@ def _forward(x2: torch.Tensor, K: int, w: torch.Tensor, bias, res2, act: int, y:
             res2 = _rows(res2)
         rc = _lib.load().kda_linear_fwd(
             x2.data_ptr(), _ld(x2), w.data_ptr(), _ld(w), None if bias is None else bias.data_ptr(),
-            None if res2 is None else res2.data_ptr(), 0 if res2 is None else _ld(res2), y.data_ptr(), y.stride(0),
-            None if z is None else z.data_ptr(), 0 if z is None else z.stride(0), M, N, K, act, code, stream)
+            None if res2 is None else res2.data_ptr(), 0 if res2 is None else _ld(res2), y, ld_y, z, ld_z, M, N, K, act,
+            code, stream)
         if rc:
             _lib.check(rc, "kda_linear_fwd")
     return x2, w
@@ -144,10 +145,6 @@ def _check(what: str, x: torch.Tensor, maps, residual: Optional[torch.Tensor], a
     return act
 
 
-def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 def _flat(t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
     return t if t is None or t.dim() == 2 else t.reshape(-1, n)
 
@@ -177,7 +174,7 @@ class LinearActFunction(torch.autograd.Function):
             M = x2.shape[0]
             y = _new(x, *x.shape[:-1], N)
             z = _new(x, M, _up8(N)) if act else None
-            x2, w = _forward(x2, K, weight, bias, _flat(residual, N), act, y.view(M, N), z, True)
+            x2, w = _forward(x2, K, weight, bias, _flat(residual, N), act, y.data_ptr(), N, _out(z), _up8(N), True)
         ctx.save_for_backward(x2, w, z)
         ctx.act, ctx.shape, ctx.N = act, x.shape, N
         return y
@@ -223,8 +220,8 @@ class MLPFunction(torch.autograd.Function):
             h = _new(x, M, _up8(N))
             z = _new(x, M, _up8(N)) if act else None
             y = _new(x, *x.shape[:-1], O)
-            x2, w1 = _forward(x2, K, w1, b1, None, act, h, z, True)
-            h, w2 = _forward(h, N, w2, b2, _flat(residual, O), 0, y.view(M, O), None, True)
+            x2, w1 = _forward(x2, K, w1, b1, None, act, h.data_ptr(), _up8(N), _out(z), _up8(N), True)
+            h, w2 = _forward(h, N, w2, b2, _flat(residual, O), 0, y.data_ptr(), O, None, 0, True)
         ctx.save_for_backward(x2, w1, z, h, w2)
         ctx.act, ctx.shape, ctx.sizes = act, x.shape, (N, O)
         return y
@@ -270,14 +267,13 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     begin on 16 bytes, or whose K is no multiple of 8, are copied first when there
     are more than 64 of them or a gradient is needed."""
     act = _check("linear_act", x, ((weight, bias),), residual, activation)
-    if _needs_grad(x, weight, bias, residual):
+    if _grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                            or (residual is not None and residual.requires_grad)):
         return LinearActFunction.apply(x, weight, bias, residual, act)
     N, K = weight.shape
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
     with _on(x.device):
-        x2 = _flat(x, K)
-        M = x2.shape[0]
-        y = _new(x, *x.shape[:-1], N)
-        _forward(x2, K, weight, bias, _flat(residual, N), act, y.view(M, N), None, False)
+        _forward(_flat(x, K), K, weight, bias, _flat(residual, N), act, y.data_ptr(), N, None, 0, False)
     return y
 
 
@@ -287,13 +283,12 @@ def mlp(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: torch
     w2 (K', N), biases or None, residual (..., K'), all bf16 or all fp32.  The hidden
     layer is rounded to their dtype between the two maps."""
     act = _check("mlp", x, ((w1, b1), (w2, b2)), residual, activation)
-    if _needs_grad(x, w1, b1, w2, b2, residual):
+    if _grad_enabled() and any(t is not None and t.requires_grad for t in (x, w1, b1, w2, b2, residual)):
         return MLPFunction.apply(x, w1, b1, w2, b2, residual, act)
     (N, K), O = w1.shape, w2.shape[0]
     with _on(x.device):
         x2 = _flat(x, K)
-        M = x2.shape[0]
-        h, y = _new(x, M, _up8(N)), _new(x, *x.shape[:-1], O)
-        _forward(x2, K, w1, b1, None, act, h, None, False)
-        _forward(h, N, w2, b2, _flat(residual, O), 0, y.view(M, O), None, False)
+        h, y = _new(x, x2.shape[0], _up8(N)), _new(x, *x.shape[:-1], O)
+        _forward(x2, K, w1, b1, None, act, h.data_ptr(), _up8(N), None, 0, False)
+        _forward(h, N, w2, b2, _flat(residual, O), 0, y.data_ptr(), O, None, 0, False)
     return y

@@ -184,12 +184,11 @@ class FusedAdamW:
         if [g.dtype for g in present] != dtypes:
             raise ValueError("a gradient's dtype is not its parameter's")
         if not all(map(_contiguous, present)):
-            gs = present = [g if g is None else g.contiguous() for g in gs]
+            gs = [g if g is None else g.detach().contiguous() for g in gs]
         self._table[1::5] = array("q", [0 if g is None else g.data_ptr() for g in gs] if missing
                                   else list(map(_data_ptr, gs)))
         return gs
 
-    @torch.no_grad()
     def step(self, max_norm: Optional[float] = None) -> Optional[torch.Tensor]:
         """One update.  With ``max_norm`` the gradients count scaled by
         min(max_norm / (G + 1e-6), 1), G their global norm, which is returned (0-d
@@ -203,7 +202,9 @@ class FusedAdamW:
         c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
         lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
         plan = self._plan.data_ptr()
-        buffers = [_ptr(self.state.get(k)) for k in ("m", "v", "m_scale", "v_scale", "master")]
+        get = self.state.get
+        buffers = [None if t is None else t.data_ptr()
+                   for t in (get("m"), get("v"), get("m_scale"), get("v_scale"), get("master"))]
         clip = pc = None
         with _on(self.device):
             stream = _raw_stream(self.device.index)
