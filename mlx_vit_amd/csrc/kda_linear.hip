@@ -33,7 +33,7 @@ struct GemmArgs {
 // activations: 0 none, 1 gelu (z Phi(z)), 2 silu (z sigma(z))
 // ----------------------------------------------------------------------------
 
-// Results rounded to bf16 (EXACT false) take fitted forms, because the epilogue
+// Results rounded to bf16 take fitted forms, because the epilogue
 // is VALU-bound with erf: 38.5 million values cost a 25088 x 1536 product 25 us
 // with Abramowitz & Stegun's 7.1.26 (25 issue slots a value, exp2 and rcp four
 // each) where the product's data need 20.
@@ -42,8 +42,22 @@ struct GemmArgs {
 //          value, a tenth of a bf16 half step, and by 4e-7 below -5.
 //   gelu': 1/2 + z Q(t), t = 2 z^2 / 4.8^2 - 1, the minimax fit of an odd function up
 //          to |z| = 4.8 and its end beyond (14 slots): off by at most 3e-5.
-__device__ __forceinline__ float sigma_fast(float z) {
+// fp32 results take Abramowitz & Stegun's 7.1.26: with u = |z| / sqrt 2, t = 1 / (1 +
+// 0.3275911 u), Phi(-|z|) = e^{-u^2} P(t) / 2 within 7.5e-8, the rounding of 1 + erf
+// itself; the library's erf has two branches that a wave takes both.
+__device__ __forceinline__ float sigma(float z) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+}
+// Phi(z), and e = e^{-z^2/2}
+__device__ __forceinline__ float phi_exp(float z, float& e) {
+    const float u = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.f));
+    e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float tail = 0.5f * p * t * e;
+    return z >= 0.f ? 1.f - tail : tail;
 }
 __device__ __forceinline__ float gelu_fast(float z) {
     const float s = fminf(z * z, 25.f);
@@ -70,19 +84,27 @@ __device__ __forceinline__ float gelu_grad_fast(float z) {
     q = fmaf(q, t, 1.4847238e-01f);
     return fmaf(c, q, 0.5f);
 }
-template <int ACT, bool EXACT>
+// F32: for results kept in fp32
+template <int ACT, bool F32>
 __device__ __forceinline__ float act(float z) {
-    if constexpr (ACT == 1) return EXACT ? z * (0.5f * (1.f + erff(z * 0.70710678118654752f))) : gelu_fast(z);
-    else if constexpr (ACT == 2) return EXACT ? z / (1.f + expf(-z)) : z * sigma_fast(z);
-    else return z;
+    if constexpr (ACT == 1) {
+        float e;
+        return F32 ? z * phi_exp(z, e) : gelu_fast(z);
+    } else if constexpr (ACT == 2) {
+        return z * sigma(z);
+    } else {
+        return z;
+    }
 }
-template <int ACT, bool EXACT>
+template <int ACT, bool F32>
 __device__ __forceinline__ float act_grad(float z) {
     if constexpr (ACT == 1) {
-        if constexpr (!EXACT) return gelu_grad_fast(z);
-        return fmaf(z * expf(-0.5f * z * z), 0.39894228040143268f, 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+        if constexpr (!F32) return gelu_grad_fast(z);
+        float e;
+        const float p = phi_exp(z, e);
+        return fmaf(z * e, 0.39894228040143268f, p);
     } else if constexpr (ACT == 2) {
-        const float s = EXACT ? 1.f / (1.f + expf(-z)) : sigma_fast(z);
+        const float s = sigma(z);
         return s * fmaf(z, 1.f - s, 1.f);
     } else {
         return 1.f;
@@ -150,7 +172,7 @@ __device__ __forceinline__ void stc8(T* p, const float (&v)[8], int n, bool vec)
 
 // The epilogue of eight columns n..n+7 of row m.  DG: times act'(zin) (zin null:
 // nothing); else bias, z out, activation, residual
-template <typename T, int ACT, bool DG, bool EXACT>
+template <typename T, int ACT, bool DG, bool F32>
 __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (&v)[8], const float (&bias)[8]) {
     const int left = a.N - n;
     const bool vec = a.vec;
@@ -159,7 +181,7 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (
         if constexpr (ACT != 0) {
             ldc8<T>(static_cast<const T*>(a.zin) + (size_t)m * a.ldzi + n, left, vec, t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= act_grad<ACT, EXACT>(t[e]);
+            for (int e = 0; e < 8; ++e) v[e] *= act_grad<ACT, F32>(t[e]);
         }
     } else {
         if (a.res) ldc8<T>(static_cast<const T*>(a.res) + (size_t)m * a.ldr + n, left, vec, t);
@@ -167,7 +189,7 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (
         for (int e = 0; e < 8; ++e) v[e] += bias[e];
         if (a.zout) stc8<T>(static_cast<T*>(a.zout) + (size_t)m * a.ldzo + n, v, left, vec);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = act<ACT, EXACT>(v[e]);
+        for (int e = 0; e < 8; ++e) v[e] = act<ACT, F32>(v[e]);
         if (a.res)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += t[e];
@@ -187,7 +209,7 @@ __device__ __forceinline__ void bias8(const GemmArgs& a, int n, float (&v)[8]) {
 // at FN = 4) of 16-byte pieces.  The 16-byte piece c of row r lies at c ^ (r's low
 // bits), so that both the fragments' writes (16 rows of a piece) and the reads
 // are spread over the banks.  acc[i][j]: columns 16 i, rows 16 j.
-template <typename T, int ACT, bool DG, bool EXACT, int R, int FN, int FM>
+template <typename T, int ACT, bool DG, bool F32, int R, int FN, int FM>
 __device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, const f32x4 (&acc)[FN][FM], char* lds) {
     constexpr int RB = 64 * FN, KEY = 4 * FN - 1, LR = 2 * FN, RI = 64 / LR;   // row bytes, lanes a row, rows a read
     const int l = lane_id(), r16 = l & 15, g4 = l >> 4, q = l % LR;
@@ -211,7 +233,7 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, c
             const f32x4 x = *reinterpret_cast<const f32x4*>(lds + RB * r + (((2 * q) ^ (r & KEY)) << 4));
             const f32x4 y = *reinterpret_cast<const f32x4*>(lds + RB * r + (((2 * q + 1) ^ (r & KEY)) << 4));
             float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            if (m < a.M && n < a.N) finish8<T, ACT, DG, EXACT>(a, m, n, v, bias);
+            if (m < a.M && n < a.N) finish8<T, ACT, DG, F32>(a, m, n, v, bias);
         }
     }
 }
@@ -719,7 +741,7 @@ template <typename T, int ACT>
 __global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ z,
                                                                  T* __restrict__ dz, int64_t ld_dy, int64_t ld_z,
                                                                  int64_t ld_dz, int M, int N, int vec_in) {
-    constexpr bool EXACT = std::is_same<T, float>::value;
+    constexpr bool F32 = std::is_same<T, float>::value;
     const int groups = (N + 7) / 8;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)M * groups; i += (size_t)gridDim.x * 256) {
         const int m = (int)(i / groups), n = 8 * (int)(i - (size_t)m * groups), left = N - n;
@@ -728,7 +750,7 @@ __global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __rest
         if constexpr (ACT != 0) {
             ldc8<T>(z + (size_t)m * ld_z + n, left, vec_in, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] *= act_grad<ACT, EXACT>(x[e]);
+            for (int e = 0; e < 8; ++e) g[e] *= act_grad<ACT, F32>(x[e]);
         }
         stc8<T>(dz + (size_t)m * ld_dz + n, g, 8, true);
     }
