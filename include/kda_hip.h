@@ -384,7 +384,7 @@ typedef struct kda_adamw_tensor {
 size_t kda_adamw_plan_size(const kda_adamw_tensor* tensors, int count);
 int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, size_t bytes);
 /* out[0] = sqrt(sum of g^2 over all tensors), out[1] = min(max_norm / (out[0] +
- * 1e-6), 1), fp32, in a fixed order.  workspace 4-byte aligned. */
+ * 1e-6), 1), rounded to fp32 from fp64 sums.  workspace 8-byte aligned. */
 size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count);
 int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, double max_norm, float* out,
                   void* workspace, size_t ws_bytes, void* stream);
@@ -396,7 +396,8 @@ int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, 
  * rounding.  states 0: m, v fp32.  states 1: 8 bits, one scale for 256 elements:
  *   m int8,  value m_scale (k / 127) |k / 127|, m_scale the block's largest |m|;
  *   v uint8, value (v_scale (k / 255)^2)^2, v_scale the block's largest sqrt(v),
- *   k >= 1 where v > 0.
+ *   k >= 1 where v > 0; the codes are those of fp32 arithmetic rounded operation by
+ *   operation.
  * m, v, master 16-byte aligned. */
 #define KDA_ADAMW_F32 0
 #define KDA_ADAMW_INT8 1

@@ -103,14 +103,32 @@ __device__ __forceinline__ uint32_t max32(uint32_t x) {
     return max(x, (uint32_t)__builtin_amdgcn_ds_swizzle((int)x, 0x401F));                  // lane ^ 16
 }
 
-// a scale's reciprocal; below the smallest normal the block counts as zero
 constexpr uint32_t MIN_NORMAL = 0x00800000u;
-__device__ __forceinline__ float inv_scale(uint32_t s) {
-    return s < MIN_NORMAL ? 0.f : __builtin_amdgcn_rcpf(__uint_as_float(s));
+
+// m and v from their codes, each operation rounded as written
+__device__ __forceinline__ void decode8(const uint2& km, const uint2& kv, float sm, float sv, float (&m)[8], float (&v)[8]) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float k = (float)(int8_t)((e < 4 ? km.x : km.y) >> (8 * (e & 3))) * (1.f / 127.f);
+        const float q = (float)(uint8_t)((e < 4 ? kv.x : kv.y) >> (8 * (e & 3))) * (1.f / 255.f);
+        m[e] = sm * k * fabsf(k);
+        const float r = sv * q * q;
+        v[e] = r * r;
+    }
 }
+
+// The code of a companded value, x = top sqrt(value / scale): `fast` is x with the
+// hardware's square root and reciprocal, within 9e-5 (3.3e-7 of 255); where it lies
+// that near a border between two codes, about once in 3000, x is formed with
+// correctly rounded operations.  So the codes are those of fp32 arithmetic operation
+// by operation, whatever computes them, and two programs that take the same steps
+// keep the same moments.
+constexpr float BORDER = 0.5f - 1.5e-4f;
 
 template <typename T, bool SMALL, bool MASTER>
 __device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, const void* grad, bool vec, float c, int64_t e0) {
+#pragma clang fp contract(off)
     const int64_t left = t.n - e0;
     const size_t at = (size_t)t.blk0 * QB + e0;      // in the moments
     T* p = static_cast<T*>(t.p) + e0;
@@ -119,57 +137,52 @@ __device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, const
     if constexpr (MASTER) ld8<float>(a.master + at, 8, true, w);
     else ld8<T>(p, left, vec, w);
     if constexpr (SMALL) {
-        const uint2 km = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.m) + at);
-        const uint2 kv = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + at);
-        const float sm = a.ms[at / QB] * (1.f / (127.f * 127.f)), sv = a.vs[at / QB] * (1.f / (255.f * 255.f));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float k = (float)(int8_t)((e < 4 ? km.x : km.y) >> (8 * (e & 3)));
-            const float q = (float)(uint8_t)((e < 4 ? kv.x : kv.y) >> (8 * (e & 3)));
-            m[e] = sm * k * fabsf(k);
-            const float r = sv * q * q;
-            v[e] = r * r;
-        }
+        decode8(*reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.m) + at),
+                *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + at), a.ms[at / QB], a.vs[at / QB], m, v);
     } else {
         ld8<float>(static_cast<const float*>(a.m) + at, 8, true, m);
         ld8<float>(static_cast<const float*>(a.v) + at, 8, true, v);
     }
-    uint32_t top_m = 0, top_r = 0;
+    uint32_t top_m = 0, top_v = 0;
     float r[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         g[e] *= c;
-        m[e] = fmaf(a.b1, m[e], a.omb1 * g[e]);
-        v[e] = fmaf(a.b2, v[e], a.omb2 * g[e] * g[e]);
+        m[e] = a.b1 * m[e] + a.omb1 * g[e];
+        v[e] = a.b2 * v[e] + a.omb2 * g[e] * g[e];
         r[e] = __builtin_amdgcn_sqrtf(v[e]);
         // lr holds the bias correction c1, rc2 is sqrt(c2)
         w[e] = fmaf(w[e], a.decay, -a.lr * m[e] * __builtin_amdgcn_rcpf(fmaf(r[e], a.rc2, a.eps)));
         if constexpr (SMALL) {
             top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
-            top_r = max(top_r, __float_as_uint(r[e]) & 0x7fffffffu);
+            top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
         }
     }
     st8<T>(p, left, vec, w);
     if constexpr (MASTER) st8<float>(a.master + at, 8, true, w);
     if constexpr (SMALL) {
         top_m = max32(top_m);
-        top_r = max32(top_r);
-        const float im = inv_scale(top_m), ir = inv_scale(top_r);
+        top_v = max32(top_v);
+        // below the smallest normal number a block counts as zero
+        const float sm = top_m < MIN_NORMAL ? 0.f : __uint_as_float(top_m);
+        const float sv = top_v < MIN_NORMAL ? 0.f : sqrtf(__uint_as_float(top_v));
+        const float im = sm == 0.f ? 0.f : __builtin_amdgcn_rcpf(sm), ir = sv == 0.f ? 0.f : __builtin_amdgcn_rcpf(sv);
         uint32_t km[2] = {0u, 0u}, kv[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float x = rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m[e]) * im));
-            const int k = (int)copysignf(x, m[e]);
-            const float y = rintf(255.f * __builtin_amdgcn_sqrtf(r[e] * ir));
-            const int q = r[e] * ir > 0.f ? max((int)y, 1) : 0;
-            km[e >> 2] |= (uint32_t)(k & 255) << (8 * (e & 3));
-            kv[e >> 2] |= (uint32_t)q << (8 * (e & 3));
+            const float x = 127.f * __builtin_amdgcn_sqrtf(fabsf(m[e]) * im), y = 255.f * __builtin_amdgcn_sqrtf(r[e] * ir);
+            float k = rintf(x), q = rintf(y);
+            if (fabsf(x - k) > BORDER) k = rintf(127.f * sqrtf(fabsf(m[e]) / sm));
+            if (fabsf(y - q) > BORDER) q = rintf(255.f * sqrtf(sqrtf(v[e]) / sv));
+            const int ik = (int)copysignf(k, m[e]), iq = v[e] * ir > 0.f ? max((int)q, 1) : 0;
+            km[e >> 2] |= (uint32_t)(ik & 255) << (8 * (e & 3));
+            kv[e >> 2] |= (uint32_t)iq << (8 * (e & 3));
         }
         *reinterpret_cast<uint2*>(static_cast<int8_t*>(a.m) + at) = make_uint2(km[0], km[1]);
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + at) = make_uint2(kv[0], kv[1]);
         if ((lane_id() & 31) == 0) {
-            a.ms[at / QB] = top_m < MIN_NORMAL ? 0.f : __uint_as_float(top_m);
-            a.vs[at / QB] = top_r < MIN_NORMAL ? 0.f : __uint_as_float(top_r);
+            a.ms[at / QB] = sm;
+            a.vs[at / QB] = sv;
         }
     } else {
         st8<float>(static_cast<float*>(a.m) + at, 8, true, m);
@@ -193,21 +206,17 @@ __global__ __launch_bounds__(256) void kda_adamw_kernel(const StepArgs a, const 
     }
 }
 
-__device__ __forceinline__ float wg_sum(float s, float* lds) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    if (lane_id() == 0) lds[threadIdx.x >> 6] = s;
-    __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
-}
-
-__global__ __launch_bounds__(256) void kda_grad_norm_kernel(float* __restrict__ part, const Grads q) {
-    __shared__ float lds[4];
+// The norm's sums are fp64 from the first square on: the clip factor then is the
+// exact one rounded, and does not depend on the order (the conversion and the
+// addition cost two more operations a value than fp32 sums, in a pass that waits
+// for memory).
+__global__ __launch_bounds__(256) void kda_grad_norm_kernel(double* __restrict__ part, const Grads q) {
+    __shared__ double lds[4];
     const uint32_t wg = q.wg + blockIdx.x;
     const int i = (int)q.owner[wg];
     const Tensor t = q.tensors[i];
     const void* g = q.g[i - q.first];
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    double s[4] = {0., 0., 0., 0.};
     if (g) {
         const bool vec = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
         const int64_t b0 = (int64_t)(wg - t.wg0) * PER_WG;
@@ -220,29 +229,33 @@ __global__ __launch_bounds__(256) void kda_grad_norm_kernel(float* __restrict__ 
                 else ld8<float>(static_cast<const float*>(g) + e, left, vec, x);
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s[k] = fmaf(x[k], x[k], s[k]);
+            for (int k = 0; k < 8; ++k) s[k & 3] = fma((double)x[k], (double)x[k], s[k & 3]);
         }
     }
-    const float sum = wg_sum(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])), lds);
-    if (threadIdx.x == 0) part[wg] = sum;
+    double sum = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    if (lane_id() == 0) lds[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) part[wg] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
 // out[0] = G, out[1] = the clip factor (a NaN stays one)
-__global__ __launch_bounds__(1024) void kda_grad_norm_finish_kernel(const float* __restrict__ part, int n, float max_norm,
+__global__ __launch_bounds__(1024) void kda_grad_norm_finish_kernel(const double* __restrict__ part, int n, double max_norm,
                                                                     float* __restrict__ out) {
     __shared__ double lds[16];
     double s = 0.;
 #pragma unroll 8
-    for (int i = threadIdx.x; i < n; i += 1024) s += (double)part[i];
+    for (int i = threadIdx.x; i < n; i += 1024) s += part[i];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
     if (lane_id() == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int i = 1; i < 16; ++i) s += lds[i];
-    const float g = (float)sqrt(s), c = max_norm / (g + 1e-6f);
-    out[0] = g;
-    out[1] = c > 1.f ? 1.f : c;
+    const double g = sqrt(s), c = max_norm / (g + 1e-6);
+    out[0] = (float)g;
+    out[1] = (float)(c > 1. ? 1. : c);
 }
 
 // what 8-bit moments stand for, eight a thread
@@ -251,17 +264,8 @@ __global__ __launch_bounds__(256) void kda_adamw_moments_kernel(const int8_t* __
                                                                 const float* __restrict__ ms, const float* __restrict__ vs,
                                                                 T* __restrict__ mo, T* __restrict__ vo, size_t n) {
     for (size_t at = 8 * ((size_t)blockIdx.x * 256 + threadIdx.x); at < n; at += 8 * 256 * (size_t)gridDim.x) {
-        const uint2 km = *reinterpret_cast<const uint2*>(m + at), kv = *reinterpret_cast<const uint2*>(v + at);
-        const float sm = ms[at / QB] * (1.f / (127.f * 127.f)), sv = vs[at / QB] * (1.f / (255.f * 255.f));
         float x[8], y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float k = (float)(int8_t)((e < 4 ? km.x : km.y) >> (8 * (e & 3)));
-            const float q = (float)(uint8_t)((e < 4 ? kv.x : kv.y) >> (8 * (e & 3)));
-            x[e] = sm * k * fabsf(k);
-            const float r = sv * q * q;
-            y[e] = r * r;
-        }
+        decode8(*reinterpret_cast<const uint2*>(m + at), *reinterpret_cast<const uint2*>(v + at), ms[at / QB], vs[at / QB], x, y);
         st8<T>(mo + at, 8, true, x);
         st8<T>(vo + at, 8, true, y);
     }
@@ -351,7 +355,7 @@ int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, 
 
 size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count) {
     if (check_tensors(tensors, count, false) != KDA_OK) return 0;
-    return workgroups(tensors, count) * sizeof(float);
+    return workgroups(tensors, count) * sizeof(double);
 }
 
 int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, double max_norm, float* out, void* workspace,
@@ -363,17 +367,17 @@ int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, 
     const size_t parts = workgroups(tensors, count);
     if (parts > 0 && (!plan || reinterpret_cast<uintptr_t>(plan) % 8 != 0))
         return api_fail(KDA_E_INVALID, "plan is NULL or not 8-byte aligned");
-    if (parts > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0))
+    if (parts > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0))
         return api_fail(KDA_E_INVALID, "workspace is NULL or misaligned");
-    if (ws_bytes < parts * sizeof(float))
-        return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, parts * sizeof(float));
+    if (ws_bytes < parts * sizeof(double))
+        return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, parts * sizeof(double));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    float* part = static_cast<float*>(workspace);
+    double* part = static_cast<double*>(workspace);
     hipError_t e = each_launch(tensors, count, plan, [&](const Grads& q, dim3 grid) {
         hipLaunchKernelGGL(kda_grad_norm_kernel, grid, dim3(256), 0, st, part, q);
     });
     if (e != hipSuccess) return api_hip_fail(e, "kda_grad_norm");
-    hipLaunchKernelGGL(kda_grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)parts, (float)max_norm, out);
+    hipLaunchKernelGGL(kda_grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)parts, max_norm, out);
     e = hipGetLastError();
     return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_grad_norm");
 }

@@ -26,7 +26,8 @@ struct GemmArgs {
     int vec;                // C, bias, res, zin, zout: 16-byte accesses, N % 8 == 0 (wgrad's parts: N % 4)
     int vec_a, vec_b;       // fp32: rows of A, B can be read four floats at a time
     int splits, k_per;      // fp32 wgrad: parts of the contracted index, k_per (a multiple of the step) each
-    float *part, *bpart;    // and their partial sums, [split][M][N] and [split][M]
+    float *part, *bpart;    // and their partial sums, [split][M][N] and [split][M]; dgrad with an activation:
+                            // bpart, C's column sums before rounding, [row of waves][N]
 };
 
 // ----------------------------------------------------------------------------
@@ -170,10 +171,11 @@ __device__ __forceinline__ void stc8(T* p, const float (&v)[8], int n, bool vec)
         if (e < n) st1<T>(p + e, v[e]);
 }
 
-// The epilogue of eight columns n..n+7 of row m.  DG: times act'(zin) (zin null:
-// nothing); else bias, z out, activation, residual
+// The epilogue of eight columns n..n+7 of row m.  DG: times act'(zin) and added to
+// `bias`, the rows' sums (no activation: nothing); else bias, z out, activation,
+// residual
 template <typename T, int ACT, bool DG, bool F32>
-__device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (&v)[8], const float (&bias)[8]) {
+__device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (&v)[8], float (&bias)[8]) {
     const int left = a.N - n;
     const bool vec = a.vec;
     float t[8];
@@ -181,7 +183,10 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (
         if constexpr (ACT != 0) {
             ldc8<T>(static_cast<const T*>(a.zin) + (size_t)m * a.ldzi + n, left, vec, t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= act_grad<ACT, F32>(t[e]);
+            for (int e = 0; e < 8; ++e) {
+                v[e] *= act_grad<ACT, F32>(t[e]);
+                bias[e] += v[e];
+            }
         }
     } else {
         if (a.res) ldc8<T>(static_cast<const T*>(a.res) + (size_t)m * a.ldr + n, left, vec, t);
@@ -210,7 +215,8 @@ __device__ __forceinline__ void bias8(const GemmArgs& a, int n, float (&v)[8]) {
 // bits), so that both the fragments' writes (16 rows of a piece) and the reads
 // are spread over the banks.  acc[i][j]: columns 16 i, rows 16 j.
 template <typename T, int ACT, bool DG, bool F32, int R, int FN, int FM>
-__device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, const f32x4 (&acc)[FN][FM], char* lds) {
+__device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, const f32x4 (&acc)[FN][FM], char* lds,
+                                            int wave_row = 0) {
     constexpr int RB = 64 * FN, KEY = 4 * FN - 1, LR = 2 * FN, RI = 64 / LR;   // row bytes, lanes a row, rows a read
     const int l = lane_id(), r16 = l & 15, g4 = l >> 4, q = l % LR;
     const int n = n0 + 8 * q;
@@ -234,6 +240,16 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, c
             const f32x4 y = *reinterpret_cast<const f32x4*>(lds + RB * r + (((2 * q + 1) ^ (r & KEY)) << 4));
             float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             if (m < a.M && n < a.N) finish8<T, ACT, DG, F32>(a, m, n, v, bias);
+        }
+    }
+    if constexpr (DG && ACT != 0) {
+        if (a.bpart) {   // the lanes of a column
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                for (int d = LR; d < 64; d <<= 1) bias[e] += __shfl_xor(bias[e], d);
+                if (l < LR && n + e < a.N) a.bpart[(size_t)wave_row * a.N + n + e] = bias[e];
+            }
         }
     }
 }
@@ -467,7 +483,7 @@ __global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(cons
         }
     }
     lds_barrier();   // every wave has read the last step
-    finish_wave<uint16_t, ACT, DG, false, 32>(a, m0 + wm, n0 + wn, acc, lds + 2048 * FN * w);
+    finish_wave<uint16_t, ACT, DG, false, 32>(a, m0 + wm, n0 + wn, acc, lds + 2048 * FN * w, mi * WR + w / WC);
 }
 
 // ----------------------------------------------------------------------------
@@ -477,13 +493,15 @@ __global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(cons
 // x = h + m + l, each the next 8 bits of x's 24 (truncation, so nothing
 // overflows and every difference is exact); the four values' parts packed.
 // An infinite x gives a NaN part.
-__device__ __forceinline__ void split3(const float4& x, uint2& h, uint2& m, uint2& l) {
-    const float v[4] = {x.x, x.y, x.z, x.w};
+// flip: the sign bit to change in each.
+__device__ __forceinline__ void split3(const float4& x, uint32_t flip, uint2& h, uint2& m, uint2& l) {
+    const uint32_t v[4] = {__float_as_uint(x.x) ^ flip, __float_as_uint(x.y) ^ flip, __float_as_uint(x.z) ^ flip,
+                           __float_as_uint(x.w) ^ flip};
     uint32_t a[4], b[4], c[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        a[e] = __float_as_uint(v[e]) & 0xffff0000u;
-        const float r = v[e] - __uint_as_float(a[e]);
+        a[e] = v[e] & 0xffff0000u;
+        const float r = __uint_as_float(v[e]) - __uint_as_float(a[e]);
         b[e] = __float_as_uint(r) & 0xffff0000u;
         c[e] = __float_as_uint(r - __uint_as_float(b[e]));
     }
@@ -527,14 +545,14 @@ struct Stage32 {
                                         : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
-    __device__ __forceinline__ void store(char* tile) const {
+    __device__ __forceinline__ void store(char* tile, uint32_t flip) const {
         const int b = 2 * col();
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int r = row(i);
             char* p = tile + r * RB + (((b >> 4) ^ (TR ? key_t(r) & (RB / 16 - 1) : key_k<RB>(r))) << 4) + (b & 15);
             uint2 h, m, l;
-            split3(v[i], h, m, l);
+            split3(v[i], flip, h, m, l);
             *reinterpret_cast<uint2*>(p) = h;
             *reinterpret_cast<uint2*>(p + PLANE) = m;
             *reinterpret_cast<uint2*>(p + 2 * PLANE) = l;
@@ -585,8 +603,9 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_f32_kernel(const G
     load(k0);
     for (int k = k0; k < k1; k += BK) {
         if (k > k0) lds_barrier();   // every wave has read the step before
-        sa.store(lds);
-        sb.store(lds + 3 * PA);
+        const bool odd = ((k - k0) / BK) & 1;
+        sa.store(lds, odd ? 0x80000000u : 0u);
+        sb.store(lds + 3 * PA, 0u);
         if (sums)
 #pragma unroll
             for (int i = 0; i < Stage32<BM, TH, AT>::PER; ++i) {
@@ -594,6 +613,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_f32_kernel(const G
             }
         lds_barrier();
         if (k + BK < k1) load(k + BK);
+        const float sign = odd ? -1.f : 1.f;
         // products of parts down to 2^-16 of the largest: hh, hm, mh, hl, lh, mm
         bf16x8 fb[3][FN];
 #pragma unroll
@@ -612,10 +632,11 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_f32_kernel(const G
                 if constexpr (AT) fa[p] = frag_t<RBA>(lds + p * PA, wm + 16 * j, 0);
                 else fa[p] = frag_k<RBA>(lds + p * PA, wm + 16 * j, 0);
             }
-            // A step's products sum from zero, smallest first, and join the accumulator by
-            // an ordinary addition: the matrix unit rounds its sums downwards, and 72
-            // such steps (K = 384) left a bias that a sum over 6272 rows showed (1.1e-6
-            // of a bias gradient, 4e-7 in fp32 arithmetic).
+            // The matrix unit rounds its sums downwards, which a sum over many rows of the
+            // results shows (a bias gradient over 6272 rows: off by 1.1e-6, 4e-7 in fp32
+            // arithmetic).  So a step's products sum from zero, smallest first, join the
+            // accumulator by an ordinary addition, and every other step is formed of A
+            // negated and subtracted, which turns its rounding upwards.
             f32x4 t[FN];
 #pragma unroll
             for (int q = 0; q < 6; ++q) {
@@ -625,7 +646,9 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_f32_kernel(const G
                     t[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[QB[q]][i], fa[QA[q]], q == 0 ? zero4() : t[i], 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < FN; ++i) acc[i][j] += t[i];
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sign, t[i][e], acc[i][j][e]);
         }
     }
     if constexpr (PART) {
@@ -736,24 +759,62 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const Ge
 }
 
 // dz = dy act'(z) (ACT 0: dy), rows of ld_dz elements whose columns from N to the
-// next multiple of eight are zero
+// next multiple of eight are zero; 64 rows x 256 columns a workgroup.  part: the
+// columns' sums before dz is rounded, [row of workgroups][N].
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ z,
-                                                                 T* __restrict__ dz, int64_t ld_dy, int64_t ld_z,
-                                                                 int64_t ld_dz, int M, int N, int vec_in) {
+                                                                 T* __restrict__ dz, float* __restrict__ part,
+                                                                 int64_t ld_dy, int64_t ld_z, int64_t ld_dz, int M, int N,
+                                                                 int vec_in) {
     constexpr bool F32 = std::is_same<T, float>::value;
-    const int groups = (N + 7) / 8;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)M * groups; i += (size_t)gridDim.x * 256) {
-        const int m = (int)(i / groups), n = 8 * (int)(i - (size_t)m * groups), left = N - n;
-        float g[8], x[8];
-        ldc8<T>(dy + (size_t)m * ld_dy + n, left, vec_in, g);
-        if constexpr (ACT != 0) {
-            ldc8<T>(z + (size_t)m * ld_z + n, left, vec_in, x);
+    __shared__ float sums[8][256];
+    const int nb = (N + 255) / 256, rb = (int)blockIdx.x / nb, r0 = threadIdx.x >> 5, c = threadIdx.x & 31;
+    const int n = 256 * ((int)blockIdx.x - rb * nb) + 8 * c, left = N - n;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (left > 0)
+        for (int m = 64 * rb + r0; m < min(M, 64 * rb + 64); m += 8) {
+            float g[8], x[8];
+            ldc8<T>(dy + (size_t)m * ld_dy + n, left, vec_in, g);
+            if constexpr (ACT != 0) {
+                ldc8<T>(z + (size_t)m * ld_z + n, left, vec_in, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] *= act_grad<ACT, F32>(x[e]);
+                for (int e = 0; e < 8; ++e) {
+                    g[e] *= act_grad<ACT, F32>(x[e]);
+                    s[e] += g[e];
+                }
+            }
+            stc8<T>(dz + (size_t)m * ld_dz + n, g, 8, true);
         }
-        stc8<T>(dz + (size_t)m * ld_dz + n, g, 8, true);
+    if (!part) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[r0][8 * c + e] = s[e];
+    __syncthreads();
+    const int col = 256 * ((int)blockIdx.x - rb * nb) + (int)threadIdx.x;
+    if (col >= N) return;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += sums[i][threadIdx.x];
+    part[(size_t)rb * N + col] = t;
+}
+
+// db: the column sums of `rows` rows of partial sums, in a fixed order (32 columns x 8
+// runs of rows a workgroup)
+__global__ __launch_bounds__(256) void kda_linear_colsum_kernel(const float* __restrict__ part, uint16_t* __restrict__ db,
+                                                                int rows, int N) {
+    __shared__ float sums[8][32];
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, n = 32 * (int)blockIdx.x + c;
+    float s = 0.f;
+    if (n < N) {
+        const int per = (rows + 7) / 8, r1 = min(rows, per * (g + 1));
+#pragma unroll 4
+        for (int r = per * g; r < r1; ++r) s += part[(size_t)r * N + n];
     }
+    sums[g][c] = s;
+    __syncthreads();
+    if (g != 0 || n >= N) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += sums[i][c];
+    db[n] = f2bf(s);
 }
 
 // one or two matrices copied into rows of a multiple of eight columns, zero past theirs
@@ -817,12 +878,22 @@ hipError_t launch_tiles(GemmArgs& a, hipStream_t st) {
 // One workgroup of 256 x 256 fills a CU, so nothing runs beside its epilogue: it
 // takes half the data a product, and pays where the steps outweigh the epilogue
 // and most CUs have one.
+int bf16_tile(int M, int N, int K) {   // its edge
+    const int64_t m256 = (M + 255) / 256, n256 = (N + 255) / 256, m128 = (M + 127) / 128, n128 = (N + 127) / 128;
+    return m256 * n256 >= 144 && K >= 512 ? 256 : m128 * n128 >= 192 ? 128 : 64;
+}
 template <bool BT, int ACT, bool DG>
 hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
-    const int64_t m256 = (a.M + 255) / 256, n256 = (a.N + 255) / 256, m128 = (a.M + 127) / 128, n128 = (a.N + 127) / 128;
-    if (m256 * n256 >= 144 && a.K >= 512) return launch_tiles<256, 256, 4, 4, 4, false, BT, ACT, DG>(a, st);
-    if (m128 * n128 >= 192) return launch_tiles<128, 128, 2, 4, 4, true, BT, ACT, DG>(a, st);
-    return launch_tiles<64, 64, 2, 2, 4, true, BT, ACT, DG>(a, st);
+    switch (bf16_tile(a.M, a.N, a.K)) {
+        case 256: return launch_tiles<256, 256, 4, 4, 4, false, BT, ACT, DG>(a, st);
+        case 128: return launch_tiles<128, 128, 2, 4, 4, true, BT, ACT, DG>(a, st);
+        default: return launch_tiles<64, 64, 2, 2, 4, true, BT, ACT, DG>(a, st);
+    }
+}
+// rows of waves of such a product, each with its column sums
+int wave_rows(int M, int N, int K) {
+    const int t = bf16_tile(M, N, K);
+    return (M + t - 1) / t * (t == 256 ? 4 : 2);
 }
 
 // fp32 tiles, by how many there are for 256 CUs (6272 rows: 384 -> 1536, 588 tiles of
@@ -873,20 +944,22 @@ hipError_t dgrad(int act, int bf16, GemmArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-hipError_t launch_act_bwd(const void* dy, const void* z, void* dz, int64_t ld_dy, int64_t ld_z, int64_t ld_dz, int M, int N,
-                          int act, hipStream_t st) {
+hipError_t launch_act_bwd(const void* dy, const void* z, void* dz, float* part, int64_t ld_dy, int64_t ld_z, int64_t ld_dz,
+                          int M, int N, int act, hipStream_t st) {
     constexpr int ES = sizeof(T);
-    const size_t n = (size_t)M * ((N + 7) / 8);
     const int vec = N % 8 == 0 && groups_ok(dy, ld_dy, ES) && groups_ok(act ? z : nullptr, ld_z, ES);
-    const dim3 grid((unsigned)std::min<size_t>((n + 255) / 256, 4096)), block(256);
+    const dim3 grid((unsigned)((M + 63) / 64) * ((N + 255) / 256)), block(256);
     const T *pdy = static_cast<const T*>(dy), *pz = static_cast<const T*>(z);
     T* pdz = static_cast<T*>(dz);
-    if (act == 1)
-        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 1>), grid, block, 0, st, pdy, pz, pdz, ld_dy, ld_z, ld_dz, M, N, vec);
-    else if (act == 2)
-        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 2>), grid, block, 0, st, pdy, pz, pdz, ld_dy, ld_z, ld_dz, M, N, vec);
-    else
-        hipLaunchKernelGGL((kda_linear_act_bwd_kernel<T, 0>), grid, block, 0, st, pdy, pz, pdz, ld_dy, ld_z, ld_dz, M, N, vec);
+    const auto kernel = act == 1   ? kda_linear_act_bwd_kernel<T, 1>
+                        : act == 2 ? kda_linear_act_bwd_kernel<T, 2>
+                                   : kda_linear_act_bwd_kernel<T, 0>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, pdy, pz, pdz, part, ld_dy, ld_z, ld_dz, M, N, vec);
+    return hipGetLastError();
+}
+
+hipError_t launch_colsum(const float* part, void* db, int rows, int N, hipStream_t st) {
+    hipLaunchKernelGGL(kda_linear_colsum_kernel, dim3((N + 31) / 32), dim3(256), 0, st, part, static_cast<uint16_t*>(db), rows, N);
     return hipGetLastError();
 }
 
@@ -1050,17 +1123,21 @@ int check_ws(const void* ws, size_t have, size_t need) {
 size_t dz_bytes(const Mat& dy, int M, int act, int bf16) {
     return act || (bf16 && !dma_ok(dy)) ? up256((size_t)M * up8(dy.n) * (bf16 ? 2 : 4)) : 0;
 }
-// dy act'(z) as dz_bytes' part of the workspace, or dy itself
-hipError_t make_dz(Mat* dy, const void* z, int64_t ld_z, int M, int act, int bf16, char** ws, hipStream_t st) {
+// dy act'(z) as dz_bytes' part of the workspace, or dy itself; part: launch_act_bwd's
+hipError_t make_dz(Mat* dy, const void* z, int64_t ld_z, int M, int act, int bf16, char** ws, float* part, hipStream_t st) {
     const size_t n = dz_bytes(*dy, M, act, bf16);
     if (n == 0) return hipSuccess;
     const Mat dz = {*ws, up8(dy->n), dy->n};
-    const hipError_t e = bf16 ? launch_act_bwd<uint16_t>(dy->p, z, *ws, dy->ld, ld_z, dz.ld, M, dy->n, act, st)
-                              : launch_act_bwd<float>(dy->p, z, *ws, dy->ld, ld_z, dz.ld, M, dy->n, act, st);
+    const hipError_t e = bf16 ? launch_act_bwd<uint16_t>(dy->p, z, *ws, part, dy->ld, ld_z, dz.ld, M, dy->n, act, st)
+                              : launch_act_bwd<float>(dy->p, z, *ws, part, dy->ld, ld_z, dz.ld, M, dy->n, act, st);
     *ws += n;
     *dy = dz;
     return e;
 }
+
+// A bf16 bias gradient behind an activation sums dz before it is rounded: from its
+// rounded values the sum would be off by as much again as its own rounding.
+bool sums_apart(int act, int bf16) { return act && bf16; }
 
 }  // namespace
 
@@ -1133,7 +1210,8 @@ size_t kda_linear_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N
     const int bf16 = dtype == KDA_DTYPE_BF16;
     const Mat d = {dy, ld_dy, N};
     const Wgrad g = {d, {nullptr, up8(K), K}, nullptr, const_cast<void*>(dy)};
-    return dz_bytes(d, M, act, bf16) + wgrads_bytes(&g, 1, M, bf16);
+    const size_t sums = sums_apart(act, bf16) ? up256((size_t)((M + 63) / 64) * N * sizeof(float)) : 0;
+    return dz_bytes(d, M, act, bf16) + sums + wgrads_bytes(&g, 1, M, bf16);
 }
 
 int kda_linear_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* z,
@@ -1158,7 +1236,14 @@ int kda_linear_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, c
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
     Mat dz = {dy, ld_dy, N};
-    LIN_HIP(make_dz(&dz, z, ld_z, M, act, bf16, &ws, st), "kda_linear_bwd");
+    float* part = db && sums_apart(act, bf16) ? reinterpret_cast<float*>(ws + dz_bytes(dz, M, act, bf16)) : nullptr;
+    LIN_HIP(make_dz(&dz, z, ld_z, M, act, bf16, &ws, part, st), "kda_linear_bwd");
+    if (part) {
+        const int rows = (M + 63) / 64;
+        LIN_HIP(launch_colsum(part, db, rows, N, st), "kda_linear_bwd");
+        ws += up256((size_t)rows * N * sizeof(float));
+        db = nullptr;
+    }
     if (dx) {
         GemmArgs a = dgrad_args(dz, {w, ld_w, K}, nullptr, 0, dx, ld_dx, M, es);
         LIN_HIP(dgrad(0, bf16, a, st), "kda_linear_bwd");
@@ -1176,7 +1261,8 @@ size_t kda_mlp_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N, i
     const Wgrad g[2] = {{d, {nullptr, up8(N), N}, nullptr, b}, {d1, {nullptr, up8(K), K}, nullptr, b}};
     size_t one = wgrads_bytes(g, 2, M, bf16);
     for (int j = 0; j < 2; ++j) one = std::max(one, wgrads_bytes(g + j, 1, M, bf16));
-    return dz_bytes(d, M, 0, bf16) + up256((size_t)M * up8(N) * (bf16 ? 2 : 4)) + one;
+    const size_t sums = sums_apart(act, bf16) ? up256((size_t)wave_rows(M, N, O) * N * sizeof(float)) : 0;
+    return dz_bytes(d, M, 0, bf16) + up256((size_t)M * up8(N) * (bf16 ? 2 : 4)) + sums + one;
 }
 
 int kda_mlp_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* w1, int64_t ld_w1, const void* z,
@@ -1210,12 +1296,20 @@ int kda_mlp_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, cons
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
     Mat d2 = {dy, ld_dy, O};
-    LIN_HIP(make_dz(&d2, nullptr, 0, M, 0, bf16, &ws, st), "kda_mlp_bwd");
+    LIN_HIP(make_dz(&d2, nullptr, 0, M, 0, bf16, &ws, nullptr, st), "kda_mlp_bwd");
     const Mat d1 = {ws, up8(N), N};
     if (first) {   // dz1 = (dy w2) act'(z)
         GemmArgs a = dgrad_args(d2, {w2, ld_w2, N}, act ? z : nullptr, ld_z, ws, d1.ld, M, es);
-        LIN_HIP(dgrad(act, bf16, a, st), "kda_mlp_bwd");
         ws += up256((size_t)M * d1.ld * es);
+        const bool apart = db1 && sums_apart(act, bf16);
+        if (apart) a.bpart = reinterpret_cast<float*>(ws);
+        LIN_HIP(dgrad(act, bf16, a, st), "kda_mlp_bwd");
+        if (apart) {
+            const int rows = wave_rows(M, N, O);
+            LIN_HIP(launch_colsum(a.bpart, db1, rows, N, st), "kda_mlp_bwd");
+            ws += up256((size_t)rows * N * sizeof(float));
+            db1 = nullptr;
+        }
     }
     if (dx) {
         GemmArgs a = dgrad_args(d1, {w1, ld_w1, K}, nullptr, 0, dx, ld_dx, M, es);

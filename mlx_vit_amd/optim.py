@@ -168,7 +168,7 @@ class FusedAdamW:
                 raise RuntimeError("parameters were moved since the last step: take one outside the capture first")
             torch.cuda.synchronize(self.device)   # a step may be reading the old plan, on any stream
         self._plan = plan.to(self.device)
-        self._parts = lib.kda_grad_norm_workspace_size(at, count) // 4
+        self._parts = lib.kda_grad_norm_workspace_size(at, count) // 8
 
     def _gradients(self) -> List[Optional[torch.Tensor]]:
         """Fill the descriptors for a step; returns the gradients, to be kept until the launches."""
@@ -209,10 +209,10 @@ class FusedAdamW:
         with _on(self.device):
             stream = _raw_stream(self.device.index)
             if max_norm is not None:
-                # the norm, the clip factor, the norm's partial sums
-                clip = torch.empty(2 + self._parts, dtype=torch.float32, device=self.device)
+                # the norm, the clip factor, the norm's partial sums (fp64)
+                clip = torch.empty(2 + 2 * self._parts, dtype=torch.float32, device=self.device)
                 pc = clip.data_ptr()
-                rc = lib.kda_grad_norm(at, count, plan, max_norm, pc, pc + 8, 4 * self._parts, stream)
+                rc = lib.kda_grad_norm(at, count, plan, max_norm, pc, pc + 8, 8 * self._parts, stream)
                 if rc:
                     _lib.check(rc, "kda_grad_norm")
             rc = lib.kda_adamw_step(at, count, plan, _STATES[self.states], *buffers, pc, self.lr, b1, b2, self.eps,

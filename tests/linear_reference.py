@@ -95,8 +95,10 @@ def linear_act(x, w, b, r, name, dy=None):
         y = y + r
     out = {"y": y.round(dt)}
     if dy is not None:
-        dz = dy if name is None else dy.times_act_grad(z.round(dt), name, dt).round(dt)
-        out.update(dx=dz.mm(w).round(dt), dw=dz.t().mm(x).round(dt), db=dz.sum0().round(dt), dr=dy)
+        exact = dy if name is None else dy.times_act_grad(z.round(dt), name, dt)
+        dz = exact if name is None else exact.round(dt)
+        # the bias gradient sums dz before it is rounded
+        out.update(dx=dz.mm(w).round(dt), dw=dz.t().mm(x).round(dt), db=exact.sum0().round(dt), dr=dy)
     return out
 
 
@@ -116,8 +118,10 @@ def mlp(x, w1, b1, w2, b2, r, name, dy=None):
         y = y + r
     out = {"y": y.round(dt)}
     if dy is not None:
-        dz = dy.mm(w2).times_act_grad(z.round(dt), name, dt).round(dt)
-        out.update(dx=dz.mm(w1).round(dt), dw1=dz.t().mm(x).round(dt), db1=dz.sum0().round(dt),
+        exact = dy.mm(w2).times_act_grad(z.round(dt), name, dt)
+        dz = exact.round(dt)
+        # behind an activation the first bias gradient sums dz before it is rounded
+        out.update(dx=dz.mm(w1).round(dt), dw1=dz.t().mm(x).round(dt), db1=(dz if name is None else exact).sum0().round(dt),
                    dw2=dy.t().mm(h).round(dt), db2=dy.sum0().round(dt), dr=dy)
     return out
 

@@ -141,7 +141,7 @@ def test_c_abi_adamw_refuses():
     assert _step(lib, None, count=1) == -1 and _step(lib, None, count=0) == 0
     norm = lambda **kw: lib.kda_grad_norm(*{**dict(t=t, count=1, plan=4096, max_norm=1.0, out=4096, ws=8192, n=1 << 10, st=None), **kw}.values())  # noqa: E731
     for kw, rc in ((dict(out=None), -1), (dict(out=4098), -1), (dict(max_norm=0.0), -1), (dict(max_norm=float("nan")), -1),
-                   (dict(ws=None), -1), (dict(n=0), -3), (dict(count=-1), -1), (dict(plan=None), -1), (dict(plan=4100), -1)):
+                   (dict(ws=None), -1), (dict(ws=8196), -1), (dict(n=0), -3), (dict(count=-1), -1), (dict(plan=None), -1), (dict(plan=4100), -1)):
         assert norm(**kw) == rc, kw
     assert lib.kda_grad_norm_workspace_size(_tensor(n=100000), 1) >= 4
     mom = lambda **kw: lib.kda_adamw_moments(*{**dict(m=4096, v=4096, ms=4096, vs=4096, mo=4096, vo=4096, n=256, dt=1, st=None), **kw}.values())  # noqa: E731

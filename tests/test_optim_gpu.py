@@ -225,6 +225,37 @@ def test_tiny_and_large_gradients_in_8_bits():
     assert p.isfinite().all() and all(t.isfinite().all() for t in opt.moments())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_codes_are_those_of_fp32_arithmetic(dtype):
+    """Codes and scales, over steps with the clip at work, equal those of torch's fp32
+    operations in the same order, each rounded by itself: two programs that take the
+    same steps keep the same moments."""
+    from mlx_vit_amd import FusedAdamW
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    n, b1, b2 = 3_000_064, 0.9, 0.95
+    (p,) = _params([(n,)], [dt], seed=11)
+    opt = FusedAdamW([p], betas=(b1, b2), states="int8")
+    k, s, q, t = (opt.state[i].clone() for i in ("m", "m_scale", "v", "v_scale"))
+    rows = lambda x: torch.nn.functional.pad(x, (0, -n % BLOCK)).view(-1, BLOCK)  # noqa: E731
+    for step in range(4):
+        g = torch.Generator(device=DEV).manual_seed(step)
+        p.grad = (torch.randn(n, generator=g, device=DEV) * torch.rand(n, generator=g, device=DEV) ** 4).to(dt)
+        norm = p.grad.double().square().sum().sqrt()
+        c = torch.clamp(0.5 / (norm + 1e-6), max=1.0).float()
+        assert opt.step(max_norm=0.5).item() == norm.float().item()
+        x = rows(p.grad.float() * c)
+        f = k.float().view(-1, BLOCK) / 127
+        m = b1 * (s.view(-1, 1) * f * f.abs()) + (1 - b1) * x
+        f = q.float().view(-1, BLOCK) / 255
+        v = b2 * (t.view(-1, 1) * f * f).square() + (1 - b2) * x * x
+        r = v.sqrt()
+        s, t = m.abs().amax(1, keepdim=True), r.amax(1, keepdim=True)
+        k = (torch.round(127 * torch.sqrt(m.abs() / s)) * m.sign()).to(torch.int8).view(-1)
+        q = torch.maximum(torch.round(255 * torch.sqrt(r / t)), (r > 0).float()).to(torch.uint8).view(-1)
+        for name, want in (("m_scale", s.view(-1)), ("v_scale", t.view(-1)), ("m", k), ("v", q)):
+            assert torch.equal(opt.state[name], want), (step, name, (opt.state[name] != want).sum().item())
+
+
 @pytest.mark.parametrize("states", ["fp32", "int8"])
 def test_state_is_carried(states):
     """The state of one optimizer, given or copied to another, continues it bit for bit."""
