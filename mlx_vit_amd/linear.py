@@ -27,6 +27,7 @@ import contextlib
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -34,7 +35,7 @@ from .kda import _DTYPE_CODE
 
 ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2}
 FEW_ROWS = 64        # up to here a forward's operands may have any alignment (kda_linear_fwd)
-MAX_STRIDE = 1 << 21
+MAX_STRIDE, MAX_ROWS = 1 << 21, (1 << 31) - 1
 _NULL = contextlib.nullcontext()
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _grad_enabled = torch.is_grad_enabled
@@ -142,6 +143,8 @@ def _check(what: str, x: torch.Tensor, maps, residual: Optional[torch.Tensor], a
             raise ValueError(f"{what}: {name} is on {t.device}, x on {dev}")
     if dev.type != "cuda":
         raise ValueError(f"{what} runs on a ROCm device; got tensors on {dev}")
+    if x.numel() > MAX_ROWS * shape[-1]:
+        raise ValueError(f"{what}: x of shape {tuple(shape)} has more than {MAX_ROWS} rows")
     return act
 
 
@@ -267,8 +270,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     begin on 16 bytes, or whose K is no multiple of 8, are copied first when there
     are more than 64 of them or a gradient is needed."""
     act = _check("linear_act", x, ((weight, bias),), residual, activation)
+    # (a forward-mode tangent: the node refuses it, the kernels would drop it)
     if _grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                            or (residual is not None and residual.requires_grad)):
+                            or (residual is not None and residual.requires_grad)) or forward_ad._current_level >= 0:
         return LinearActFunction.apply(x, weight, bias, residual, act)
     N, K = weight.shape
     y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
@@ -283,7 +287,8 @@ def mlp(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: torch
     w2 (K', N), biases or None, residual (..., K'), all bf16 or all fp32.  The hidden
     layer is rounded to their dtype between the two maps."""
     act = _check("mlp", x, ((w1, b1), (w2, b2)), residual, activation)
-    if _grad_enabled() and any(t is not None and t.requires_grad for t in (x, w1, b1, w2, b2, residual)):
+    if (_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w1, b1, w2, b2, residual))
+            or forward_ad._current_level >= 0):
         return MLPFunction.apply(x, w1, b1, w2, b2, residual, act)
     (N, K), O = w1.shape, w2.shape[0]
     with _on(x.device):

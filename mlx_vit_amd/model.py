@@ -27,7 +27,7 @@ import torch.nn.functional as F
 from torch.autograd import forward_ad
 
 from .layer import GatedDeltaLayer
-from .layer_fused import _plain_module
+from .layer_fused import _nn_module, _plain_module
 from .linear import mlp
 
 BF16_KEEP_FP32 = ("A_log", "dt_bias")
@@ -135,7 +135,10 @@ def _mlp_residual(block: nn.Module, x: torch.Tensor) -> torch.Tensor:
     if not (block.fused_mlp and type(seq) is nn.Sequential and len(seq) == 5 and h.device.type == "cuda"
             and h.dtype in (torch.bfloat16, torch.float32) and not torch.is_autocast_enabled("cuda")
             and not torch.compiler.is_compiling() and not torch._C._is_tracing()
-            and forward_ad._current_level < 0 and _plain_module(seq, nn.Sequential)
+            and forward_ad._current_level < 0 and not (_nn_module._global_forward_hooks or _nn_module._global_forward_pre_hooks
+                                                       or _nn_module._global_backward_hooks
+                                                       or _nn_module._global_backward_pre_hooks)
+            and _plain_module(seq, nn.Sequential)
             and all(_plain_module(m, c) for m, c in zip(seq, (nn.Linear, nn.GELU, nn.Dropout, nn.Linear, nn.Dropout)))
             and seq[1].approximate == "none" and not any(m.p > 0 and m.training for m in (seq[2], seq[4]))
             and all(type(p) is nn.Parameter and p.dtype == h.dtype and p.device == h.device for p in seq.parameters())

@@ -32,7 +32,8 @@ _data_ptr, _contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 
 
 class FusedAdamW:
-    """AdamW with moments of their own dtype.
+    """AdamW with moments of their own dtype.  A captured step replays with the learning
+    rate, and the bias corrections, that it was captured with.
 
     ``states``: "fp32" or "int8"; ``master_weights``: keep and update fp32 copies of
     the weights; ``bias_correction``: divide the moments by 1 - beta^step (off in
@@ -72,7 +73,7 @@ class FusedAdamW:
             self.offsets.append(at)
             at += -(-n // BLOCK) * BLOCK
         self.total = at
-        self.state = self._new_state(master_weights) if state is None else self._given_state(state, master_weights)
+        self._state = self._new_state(master_weights) if state is None else self._given_state(state, master_weights)
         # p, g, n, offset, dtype of each parameter
         self._ptrs: List[int] = []
         self._plan: Optional[torch.Tensor] = None
@@ -111,6 +112,11 @@ class FusedAdamW:
                                  f"{self.device}; got {s.dtype}, shape {tuple(s.shape)} on {s.device}")
         return dict(state)
 
+    @property
+    def state(self) -> Dict[str, torch.Tensor]:
+        """The buffers of moments (and masters) by name."""
+        return dict(self._state)
+
     def views(self, flat: torch.Tensor) -> List[torch.Tensor]:
         """Each parameter's part of a buffer laid out as the moments."""
         return [flat[o:o + n].view(p.shape) for p, o, n in zip(self.params, self.offsets, self._numels)]
@@ -118,7 +124,7 @@ class FusedAdamW:
     def moments(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
         """(m, v) as buffers of values (``views`` gives the parameters' parts): with
         fp32 states the state's own buffers, in another dtype copies."""
-        m, v = self.state["m"], self.state["v"]
+        m, v = self._state["m"], self._state["v"]
         if self.states == "fp32":
             return m.to(dtype), v.to(dtype)
         if dtype not in _DTYPE_CODE:
@@ -127,22 +133,22 @@ class FusedAdamW:
         vo = torch.empty_like(mo)
         with _on(self.device):
             _lib.check(_lib.load().kda_adamw_moments(
-                _ptr(m), _ptr(v), _ptr(self.state["m_scale"]), _ptr(self.state["v_scale"]), _ptr(mo), _ptr(vo),
+                _ptr(m), _ptr(v), _ptr(self._state["m_scale"]), _ptr(self._state["v_scale"]), _ptr(mo), _ptr(vo),
                 self.total, _DTYPE_CODE[dtype], _stream(self.device)), "kda_adamw_moments")
         return mo, vo
 
     def state_dict(self) -> dict:
-        return {"steps": self.steps, **self.state}
+        return {"steps": self.steps, **self._state}
 
     def load_state_dict(self, state: dict) -> None:
         """Copy a ``state_dict`` of an optimizer over the same tensors into this one's buffers."""
-        if set(state) != {"steps", *self.state}:
-            raise ValueError(f"state holds {sorted(state)}; expected {sorted(('steps', *self.state))}")
-        for k, t in self.state.items():
+        if set(state) != {"steps", *self._state}:
+            raise ValueError(f"state holds {sorted(state)}; expected {sorted(('steps', *self._state))}")
+        for k, t in self._state.items():
             if state[k].dtype != t.dtype or state[k].shape != t.shape:
                 raise ValueError(f"state[{k!r}] is {state[k].dtype} {tuple(state[k].shape)}; expected {t.dtype} "
                                  f"{tuple(t.shape)}")
-        for k, t in self.state.items():
+        for k, t in self._state.items():
             t.copy_(state[k])
         self.steps = int(state["steps"])
 
@@ -202,7 +208,7 @@ class FusedAdamW:
         c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
         lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
         plan = self._plan.data_ptr()
-        get = self.state.get
+        get = self._state.get
         buffers = [None if t is None else t.data_ptr()
                    for t in (get("m"), get("v"), get("m_scale"), get("v_scale"), get("master"))]
         clip = pc = None

@@ -285,6 +285,31 @@ def test_graph_replays(dtype):
                 assert torch.equal(a, b)
 
 
+def test_graph_replays_of_large_tiles():
+    """The tiles of 256 x 256 take more LDS than a kernel gets by default."""
+    from mlx_vit_amd import linear_act
+    x, w, b, r, _ = _inputs(6200, 640, 2560, torch.bfloat16, seed=65)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = linear_act(x, w, b, r, "gelu")
+    for k in range(3):
+        x.copy_(_mk(75 + k, 6200, 640, dt=torch.bfloat16))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, linear_act(x, w, b, r, "gelu"))
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+    from mlx_vit_amd import linear_act, mlp
+    x, w, b, _, _ = _inputs(9, 16, 16, torch.float32)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: linear_act(d, w, b), lambda: mlp(d, w, b, w, b)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                f()
+
+
 def test_other_stream():
     from mlx_vit_amd import mlp
     x, w1, b1, _, _ = _inputs(300, 64, 128, torch.bfloat16, True, False, seed=80)
