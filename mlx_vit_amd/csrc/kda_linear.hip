@@ -171,17 +171,33 @@ __device__ __forceinline__ void stc8(T* p, const float (&v)[8], int n, bool vec)
         if (e < n) st1<T>(p + e, v[e]);
 }
 
-// The epilogue of eight columns n..n+7 of row m.  DG: times act'(zin) and added to
-// `bias`, the rows' sums (no activation: nothing); else bias, z out, activation,
-// residual
+// Where an epilogue reads and writes: column n of row m in each matrix, moved down a
+// few rows at a time (a multiplication by each row stride for every eight values
+// was a fifth of the epilogue's instructions)
+template <typename T, bool DG>
+struct Place {
+    const T* in;   // DG: zin, else the residual
+    T *z, *c;
+    __device__ __forceinline__ Place(const GemmArgs& a, int m, int n)
+        : in(static_cast<const T*>(DG ? a.zin : a.res) + (size_t)m * (DG ? a.ldzi : a.ldr) + n),
+          z(static_cast<T*>(a.zout) + (size_t)m * a.ldzo + n), c(static_cast<T*>(a.c) + (size_t)m * a.ldc + n) {}
+    __device__ __forceinline__ void down(const GemmArgs& a, int rows) {
+        in += rows * (DG ? a.ldzi : a.ldr);
+        if constexpr (!DG) z += rows * a.ldzo;
+        c += rows * a.ldc;
+    }
+};
+
+// The epilogue of eight columns from `at`, of which `left` exist.  DG: times act'(zin)
+// and added to `bias`, the rows' sums (no activation: nothing); else bias, z out,
+// activation, residual
 template <typename T, int ACT, bool DG, bool F32>
-__device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (&v)[8], float (&bias)[8]) {
-    const int left = a.N - n;
+__device__ __forceinline__ void finish8(const GemmArgs& a, const Place<T, DG>& at, int left, float (&v)[8], float (&bias)[8]) {
     const bool vec = a.vec;
     float t[8];
     if constexpr (DG) {
         if constexpr (ACT != 0) {
-            ldc8<T>(static_cast<const T*>(a.zin) + (size_t)m * a.ldzi + n, left, vec, t);
+            ldc8<T>(at.in, left, vec, t);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[e] *= act_grad<ACT, F32>(t[e]);
@@ -189,17 +205,17 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, float (
             }
         }
     } else {
-        if (a.res) ldc8<T>(static_cast<const T*>(a.res) + (size_t)m * a.ldr + n, left, vec, t);
+        if (a.res) ldc8<T>(at.in, left, vec, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bias[e];
-        if (a.zout) stc8<T>(static_cast<T*>(a.zout) + (size_t)m * a.ldzo + n, v, left, vec);
+        if (a.zout) stc8<T>(at.z, v, left, vec);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = act<ACT, F32>(v[e]);
         if (a.res)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += t[e];
     }
-    stc8<T>(static_cast<T*>(a.c) + (size_t)m * a.ldc + n, v, left, vec);
+    stc8<T>(at.c, v, left, vec);
 }
 template <typename T, bool DG>
 __device__ __forceinline__ void bias8(const GemmArgs& a, int n, float (&v)[8]) {
@@ -222,6 +238,8 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, c
     const int n = n0 + 8 * q;
     float bias[8];
     bias8<T, DG>(a, n, bias);
+    int m = m0 + l / LR;
+    Place<T, DG> at(a, m, n);
 #pragma unroll
     for (int h = 0; h < FM; h += R / 16) {
         wave_sync();   // the last part's reads come first
@@ -235,11 +253,13 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int m0, int n0, c
         wave_sync();
 #pragma unroll
         for (int it = 0; it < R / RI; ++it) {
-            const int r = RI * it + l / LR, m = m0 + 16 * h + r;
+            const int r = RI * it + l / LR;
             const f32x4 x = *reinterpret_cast<const f32x4*>(lds + RB * r + (((2 * q) ^ (r & KEY)) << 4));
             const f32x4 y = *reinterpret_cast<const f32x4*>(lds + RB * r + (((2 * q + 1) ^ (r & KEY)) << 4));
             float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            if (m < a.M && n < a.N) finish8<T, ACT, DG, F32>(a, m, n, v, bias);
+            if (m < a.M && n < a.N) finish8<T, ACT, DG, F32>(a, at, a.N - n, v, bias);
+            m += RI;
+            at.down(a, RI);
         }
     }
     if constexpr (DG && ACT != 0) {
@@ -755,7 +775,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const Ge
     if (m >= a.M || n >= a.N) return;
     float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, bias[8];
     bias8<T, false>(a, n, bias);
-    finish8<T, ACT, false, std::is_same<T, float>::value>(a, m, n, v, bias);
+    finish8<T, ACT, false, std::is_same<T, float>::value>(a, Place<T, false>(a, m, n), a.N - n, v, bias);
 }
 
 // dz = dy act'(z) (ACT 0: dy), rows of ld_dz elements whose columns from N to the
