@@ -329,10 +329,11 @@ int kda_log_decay_bwd(const void* alpha, const float* dg, void* dalpha, int64_t 
  * for m < M, n < N, k < K; z (may be NULL) receives the value before act, which
  * the backward pass reads.  act: 0 none, 1 gelu (z Phi(z)), 2 silu.  All of
  * dtype; sums, epilogue and activation in fp32.  Matrices are rows of ld_*
- * elements (at most 2^21), unit column stride.  bf16 with more than 64 rows: x
- * and w 16-byte aligned, ld_x and ld_w multiples of 8 that cover K rounded up
- * to 8, and that many elements of the last row readable; other operands and
- * smaller or fp32 ones: any stride, aligned to their element. */
+ * elements (at most 2^21), unit column stride.  bf16 with ceil(M / 16) ceil(N / 16)
+ * above 512: x and w 16-byte aligned, ld_x and ld_w multiples of 8 that cover K
+ * rounded up to 8, and that many elements of the last row readable; other
+ * operands and smaller or fp32 ones: any stride, aligned to their element.
+ * Outputs overlap neither each other nor an input, here and below. */
 #define KDA_ACT_NONE 0
 #define KDA_ACT_GELU 1
 #define KDA_ACT_SILU 2
@@ -348,7 +349,7 @@ int kda_linear_pad(const void* src0, int64_t ld0, int rows0, int cols0, void* ds
  *   dx = dz w,  dw[n][k] = sum_m dz[m][n] x[m][k],  db[n] = sum_m dz[m][n]
  * (each may be NULL; db only with dw).  z as the forward wrote it (act 0:
  * unused).  dw [N][K] and db [N] contiguous, sums in a fixed order.  bf16: x and
- * w as for more than 64 rows above (the part of x that pads K is read and not
+ * w as for many pieces above (the part of x that pads K is read and not
  * used), dw 16-byte aligned where K is a multiple of 8.  M >= 1; workspace: at
  * least kda_linear_bwd_workspace_size bytes, 16-byte aligned. */
 size_t kda_linear_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N, int K, int act, int dtype);
@@ -380,15 +381,13 @@ typedef struct kda_adamw_tensor {
 /* What does not change from step to step (p, n, offset and dtype of the tensors),
  * as the kernels read it: kda_adamw_plan fills kda_adamw_plan_size bytes of host
  * memory, which the caller copies to the device once (8-byte aligned) and passes
- * with the same tensors, whose g may differ, to the two calls below. */
+ * with the same tensors, whose g may differ, to kda_adamw_step. */
 size_t kda_adamw_plan_size(const kda_adamw_tensor* tensors, int count);
 int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, size_t bytes);
-/* out[0] = sqrt(sum of g^2 over all tensors), out[1] = min(max_norm / (out[0] +
- * 1e-6), 1), rounded to fp32 from fp64 sums.  workspace 8-byte aligned. */
-size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count);
-int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, double max_norm, float* out,
-                  void* workspace, size_t ws_bytes, void* stream);
-/* g' = clip[1] g (clip: kda_grad_norm's out, or NULL for g itself);
+/* One step.  max_norm > 0: clip[0] = G = sqrt(sum of g^2 over all tensors), clip[1] =
+ * min(max_norm / (G + 1e-6), 1), each rounded to fp32 from fp64 sums, g' = clip[1] g
+ * and a workspace of kda_adamw_step_workspace_size bytes, 8-byte aligned; max_norm 0:
+ * g' = g, clip and workspace unused.
  *   m <- beta1 m + (1 - beta1) g';  v <- beta2 v + (1 - beta2) g'^2;
  *   p <- p (1 - lr weight_decay) - lr correct1 m / (sqrt(v correct2) + eps)
  * (correct1 = correct2 = 1: no bias correction).  master (may be NULL): fp32
@@ -401,9 +400,11 @@ int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, 
  * m, v, master 16-byte aligned. */
 #define KDA_ADAMW_F32 0
 #define KDA_ADAMW_INT8 1
+size_t kda_adamw_step_workspace_size(const kda_adamw_tensor* tensors, int count);
 int kda_adamw_step(const kda_adamw_tensor* tensors, int count, const void* plan, int states, void* m, void* v,
-                   float* m_scale, float* v_scale, float* master, const float* clip, double lr, double beta1,
-                   double beta2, double eps, double weight_decay, double correct1, double correct2, void* stream);
+                   float* m_scale, float* v_scale, float* master, double max_norm, float* clip, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, double correct1, double correct2,
+                   void* workspace, size_t ws_bytes, void* stream);
 /* the values that n (a multiple of 256) 8-bit moments stand for */
 int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale,
                       void* m_out, void* v_out, int64_t n, int dtype, void* stream);

@@ -66,11 +66,10 @@ SIGNATURES = {
     "kda_linear_bwd": ([_P, _L] * 5 + [_P] * 2 + [_I] * 5 + [_P, _Z, _P], _I),
     "kda_mlp_bwd_workspace_size": ([_P, _L] + [_I] * 6, _Z),
     "kda_mlp_bwd": ([_P, _L] * 7 + [_P] * 4 + [_I] * 6 + [_P, _Z, _P], _I),
-    "kda_grad_norm_workspace_size": ([_P, _I], _Z),
     "kda_adamw_plan_size": ([_P, _I], _Z),
     "kda_adamw_plan": ([_P, _I, _P, _Z], _I),
-    "kda_grad_norm": ([_P, _I, _P, _D, _P, _P, _Z, _P], _I),
-    "kda_adamw_step": ([_P, _I, _P, _I] + [_P] * 6 + [_D] * 7 + [_P], _I),
+    "kda_adamw_step_workspace_size": ([_P, _I], _Z),
+    "kda_adamw_step": ([_P, _I, _P, _I] + [_P] * 5 + [_D, _P] + [_D] * 7 + [_P, _Z, _P], _I),
     "kda_adamw_moments": ([_P] * 6 + [_L, _I, _P], _I),
     "kda_layer_workspace_size": ([_I] * 5, _Z),
     "kda_profile_enable": ([_I], _I),

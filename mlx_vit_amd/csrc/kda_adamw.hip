@@ -27,7 +27,14 @@ namespace kda {
 namespace {
 
 constexpr int QB = 256;            // elements that share a scale
-constexpr int PER_WG = 4096;       // elements of one tensor a workgroup takes
+// elements of one tensor a workgroup takes (bf16 weights in 16 tensors, a step with
+// the norm, us for 2048 | 4096 | 8192: 2^18 elements 7.1 | 8.2 | 10.5, where the host
+// takes 20; 2^23 38.3 | 35.4 | 36.1; 2^26 302 | 310 | 316, in 8 bits 156 | 153 | 157)
+constexpr int PER_WG = 4096;
+// up to so many partial sums of the norm every workgroup of the update adds them
+// itself (8 a thread); beyond, a launch between the two does (us, itself | launch:
+// 64 sums 8.2 | 9.1, 256 10.1 | 10.9, 2048 35.4 | 36.7, 8192 168 | 154, 16384 388 | 314)
+constexpr int SUM_PARTS = 2048;
 constexpr int PER_LAUNCH = 480;    // tensors of one launch: their gradients' addresses travel as kernel arguments
 
 // What does not change from step to step lies in device memory, the plan: the
@@ -51,7 +58,10 @@ struct Grads {
 };
 struct StepArgs {
     float b1, omb1, b2, omb2, decay, lr, eps, rc2;
-    const float* clip;
+    float* clip;                   // the norm and the clip factor, or null
+    const double* part;            // non-null: to be formed from these partial sums
+    int parts;
+    double max_norm;
     void *m, *v;
     float *ms, *vs, *master;
 };
@@ -190,15 +200,43 @@ __device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, const
     }
 }
 
+// The clip factor of all partial sums, by TH threads (all of them get it); out
+// non-null: out[0] = G, out[1] = the factor (a NaN stays one)
+template <int TH>
+__device__ __forceinline__ float clip_factor(const double* __restrict__ part, int n, double max_norm, double* lds, float* out) {
+    double s = 0.;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += TH) s += part[i];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    if (lane_id() == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = lds[0];
+#pragma unroll
+    for (int i = 1; i < TH / 64; ++i) s += lds[i];
+    const double g = sqrt(s), c = max_norm / (g + 1e-6), f = c > 1. ? 1. : c;
+    if (out && threadIdx.x == 0) {
+        out[0] = (float)g;
+        out[1] = (float)f;
+    }
+    return (float)f;
+}
+
 template <bool SMALL, bool MASTER>
 __global__ __launch_bounds__(256) void kda_adamw_kernel(const StepArgs a, const Grads q) {
     const uint32_t wg = q.wg + blockIdx.x;
     const int i = (int)q.owner[wg];
     const Tensor t = q.tensors[i];
     const void* g = q.g[i - q.first];
-    if (!g) return;
     const bool vec = ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(t.p)) & 15) == 0;
-    const float c = a.clip ? a.clip[1] : 1.f;
+    float c = 1.f;
+    if (a.part) {
+        __shared__ double lds[4];
+        c = clip_factor<256>(a.part, a.parts, a.max_norm, lds, blockIdx.x == 0 && q.wg == 0 ? a.clip : nullptr);
+    } else if (a.clip) {
+        c = a.clip[1];
+    }
+    if (!g) return;
     const int64_t b0 = (int64_t)(wg - t.wg0) * PER_WG, end = min((t.n + QB - 1) / QB * QB, b0 + (int64_t)PER_WG);
     for (int64_t e = b0 + 8 * (int64_t)threadIdx.x; e < end; e += 8 * 256) {   // whole blocks: half waves stay together
         if (t.bf16) update<uint16_t, SMALL, MASTER>(a, t, g, vec, c, e);
@@ -240,22 +278,10 @@ __global__ __launch_bounds__(256) void kda_grad_norm_kernel(double* __restrict__
     if (threadIdx.x == 0) part[wg] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-// out[0] = G, out[1] = the clip factor (a NaN stays one)
 __global__ __launch_bounds__(1024) void kda_grad_norm_finish_kernel(const double* __restrict__ part, int n, double max_norm,
                                                                     float* __restrict__ out) {
     __shared__ double lds[16];
-    double s = 0.;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < n; i += 1024) s += part[i];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    if (lane_id() == 0) lds[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int i = 1; i < 16; ++i) s += lds[i];
-    const double g = sqrt(s), c = max_norm / (g + 1e-6);
-    out[0] = (float)g;
-    out[1] = (float)(c > 1. ? 1. : c);
+    clip_factor<1024>(part, n, max_norm, lds, out);
 }
 
 // what 8-bit moments stand for, eight a thread
@@ -271,7 +297,7 @@ __global__ __launch_bounds__(256) void kda_adamw_moments_kernel(const int8_t* __
     }
 }
 
-int check_tensors(const kda_adamw_tensor* t, int count, bool step) {
+int check_tensors(const kda_adamw_tensor* t, int count) {
     if (count < 0 || (count > 0 && !t)) return api_fail(KDA_E_INVALID, "count=%d tensors at %p", count, (const void*)t);
     int64_t wgs = 0;
     for (int i = 0; i < count; ++i) {
@@ -281,10 +307,9 @@ int check_tensors(const kda_adamw_tensor* t, int count, bool step) {
         wgs += (t[i].n + PER_WG - 1) / PER_WG;
         if (t[i].n == 0) continue;
         const uintptr_t es = t[i].dtype == KDA_DTYPE_BF16 ? 2 : 4;
-        if (reinterpret_cast<uintptr_t>(t[i].g) % es != 0 ||
-            (step && (!t[i].p || reinterpret_cast<uintptr_t>(t[i].p) % es != 0)))
+        if (reinterpret_cast<uintptr_t>(t[i].g) % es != 0 || !t[i].p || reinterpret_cast<uintptr_t>(t[i].p) % es != 0)
             return api_fail(KDA_E_INVALID, "tensor %d: p is NULL, or p or g is misaligned", i);
-        if (step && (t[i].offset < 0 || t[i].offset % QB != 0 || t[i].offset / QB > 0xffffffffLL))
+        if (t[i].offset < 0 || t[i].offset % QB != 0 || t[i].offset / QB > 0xffffffffLL)
             return api_fail(KDA_E_INVALID, "tensor %d: offset=%lld: expected a multiple of %d", i, (long long)t[i].offset, QB);
     }
     if (wgs > (1 << 23))   // 256 threads each: below 2^32 in a launch
@@ -331,12 +356,12 @@ using namespace kda;
 extern "C" {
 
 size_t kda_adamw_plan_size(const kda_adamw_tensor* tensors, int count) {
-    if (check_tensors(tensors, count, true) != KDA_OK) return 0;
+    if (check_tensors(tensors, count) != KDA_OK) return 0;
     return count * sizeof(Tensor) + workgroups(tensors, count) * sizeof(uint32_t);
 }
 
 int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, size_t bytes) {
-    const int rc = check_tensors(tensors, count, true);
+    const int rc = check_tensors(tensors, count);
     if (rc != KDA_OK) return rc;
     if (count == 0) return KDA_OK;
     if (!host_plan || reinterpret_cast<uintptr_t>(host_plan) % 8 != 0)
@@ -353,52 +378,38 @@ int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, 
     return KDA_OK;
 }
 
-size_t kda_grad_norm_workspace_size(const kda_adamw_tensor* tensors, int count) {
-    if (check_tensors(tensors, count, false) != KDA_OK) return 0;
+size_t kda_adamw_step_workspace_size(const kda_adamw_tensor* tensors, int count) {
+    if (check_tensors(tensors, count) != KDA_OK) return 0;
     return workgroups(tensors, count) * sizeof(double);
 }
 
-int kda_grad_norm(const kda_adamw_tensor* tensors, int count, const void* plan, double max_norm, float* out, void* workspace,
-                  size_t ws_bytes, void* stream) {
-    const int rc = check_tensors(tensors, count, false);
-    if (rc != KDA_OK) return rc;
-    if (!out || reinterpret_cast<uintptr_t>(out) % 4 != 0) return api_fail(KDA_E_INVALID, "out is NULL or misaligned");
-    if (!(max_norm > 0.)) return api_fail(KDA_E_INVALID, "max_norm=%g: expected a positive number", max_norm);
-    const size_t parts = workgroups(tensors, count);
-    if (parts > 0 && (!plan || reinterpret_cast<uintptr_t>(plan) % 8 != 0))
-        return api_fail(KDA_E_INVALID, "plan is NULL or not 8-byte aligned");
-    if (parts > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0))
-        return api_fail(KDA_E_INVALID, "workspace is NULL or misaligned");
-    if (ws_bytes < parts * sizeof(double))
-        return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, parts * sizeof(double));
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    double* part = static_cast<double*>(workspace);
-    hipError_t e = each_launch(tensors, count, plan, [&](const Grads& q, dim3 grid) {
-        hipLaunchKernelGGL(kda_grad_norm_kernel, grid, dim3(256), 0, st, part, q);
-    });
-    if (e != hipSuccess) return api_hip_fail(e, "kda_grad_norm");
-    hipLaunchKernelGGL(kda_grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)parts, max_norm, out);
-    e = hipGetLastError();
-    return e == hipSuccess ? KDA_OK : api_hip_fail(e, "kda_grad_norm");
-}
-
 int kda_adamw_step(const kda_adamw_tensor* tensors, int count, const void* plan, int states, void* m, void* v,
-                   float* m_scale, float* v_scale, float* master, const float* clip, double lr, double beta1, double beta2,
-                   double eps, double weight_decay, double correct1, double correct2, void* stream) {
-    const int rc = check_tensors(tensors, count, true);
+                   float* m_scale, float* v_scale, float* master, double max_norm, float* clip, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, double correct1, double correct2, void* workspace,
+                   size_t ws_bytes, void* stream) {
+    const int rc = check_tensors(tensors, count);
     if (rc != KDA_OK) return rc;
     if (states != KDA_ADAMW_F32 && states != KDA_ADAMW_INT8)
         return api_fail(KDA_E_UNSUPPORTED, "states=%d: expected 0 (fp32) or 1 (8 bits)", states);
     if (!(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1. && eps >= 0. && correct1 > 0. && correct2 > 0.))
         return api_fail(KDA_E_INVALID, "beta1=%g beta2=%g eps=%g correct1=%g correct2=%g", beta1, beta2, eps, correct1,
                         correct2);
-    if (count == 0) return KDA_OK;
-    if (!plan || reinterpret_cast<uintptr_t>(plan) % 8 != 0)
+    if (!(max_norm >= 0.)) return api_fail(KDA_E_INVALID, "max_norm=%g: expected 0 (no clip) or a positive number", max_norm);
+    const size_t parts = workgroups(tensors, count);
+    if (max_norm > 0.) {
+        if (!clip || reinterpret_cast<uintptr_t>(clip) % 4 != 0) return api_fail(KDA_E_INVALID, "clip is NULL or misaligned");
+        if (parts > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0))
+            return api_fail(KDA_E_INVALID, "workspace is NULL or misaligned");
+        if (ws_bytes < parts * sizeof(double))
+            return api_fail(KDA_E_WORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, parts * sizeof(double));
+    }
+    if (parts > 0 && (!plan || reinterpret_cast<uintptr_t>(plan) % 8 != 0))
         return api_fail(KDA_E_INVALID, "plan is NULL or not 8-byte aligned");
     const bool small = states == KDA_ADAMW_INT8;
     const uintptr_t all = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(master);
-    if (!m || !v || all % 16 != 0) return api_fail(KDA_E_INVALID, "m, v or master is NULL or not 16-byte aligned");
-    if (small && (!m_scale || !v_scale || (reinterpret_cast<uintptr_t>(m_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 4 != 0))
+    if (parts > 0 && (!m || !v || all % 16 != 0)) return api_fail(KDA_E_INVALID, "m, v or master is NULL or not 16-byte aligned");
+    if (parts > 0 && small &&
+        (!m_scale || !v_scale || (reinterpret_cast<uintptr_t>(m_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 4 != 0))
         return api_fail(KDA_E_INVALID, "m_scale or v_scale is NULL or misaligned");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StepArgs a;
@@ -408,8 +419,24 @@ int kda_adamw_step(const kda_adamw_tensor* tensors, int count, const void* plan,
     a.lr = (float)(lr * correct1);
     a.eps = (float)eps;
     a.rc2 = (float)sqrt(correct2);
-    a.clip = clip;
     a.m = m; a.v = v; a.ms = m_scale; a.vs = v_scale; a.master = master;
+    a.clip = nullptr; a.part = nullptr; a.parts = 0; a.max_norm = max_norm;
+    if (max_norm > 0.) {
+        double* part = static_cast<double*>(workspace);
+        hipError_t e = each_launch(tensors, count, plan, [&](const Grads& q, dim3 grid) {
+            hipLaunchKernelGGL(kda_grad_norm_kernel, grid, dim3(256), 0, st, part, q);
+        });
+        if (e != hipSuccess) return api_hip_fail(e, "kda_adamw_step");
+        a.clip = clip;
+        if (parts > 0 && parts <= SUM_PARTS) {
+            a.part = part;
+            a.parts = (int)parts;
+        } else {
+            hipLaunchKernelGGL(kda_grad_norm_finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)parts, max_norm, clip);
+            e = hipGetLastError();
+            if (e != hipSuccess) return api_hip_fail(e, "kda_adamw_step");
+        }
+    }
     const hipError_t e = each_launch(tensors, count, plan, [&](const Grads& q, dim3 grid) {
         const dim3 block(256);
         if (small && master) hipLaunchKernelGGL((kda_adamw_kernel<true, true>), grid, block, 0, st, a, q);

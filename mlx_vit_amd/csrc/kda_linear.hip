@@ -721,43 +721,64 @@ __global__ __launch_bounds__(256) void kda_linear_sum_parts_kernel(const float* 
 // few rows: operands straight from memory, the waves share the contracted index
 // ----------------------------------------------------------------------------
 
-// eight (bf16) or four (fp32) elements k.. of a row; past K zero
-__device__ __forceinline__ bf16x8 row8(const uint16_t* row, int k, int K, bool vec) {
-    if (vec && k + 8 <= K) return __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(row + k));
+// eight elements k.. of a row; past K zero
+__device__ __forceinline__ bf16x8 row8(const uint16_t* row, int k, int K) {
     short8v v = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (k + e < K) v[e] = (short)row[k + e];
     return __builtin_bit_cast(bf16x8, v);
 }
+// acc += a step of the contracted index: 32 of it in bf16, 16 in fp32
+__device__ __forceinline__ f32x4 few_step(const uint4& x, const uint4& y, f32x4 acc, uint16_t) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, y), __builtin_bit_cast(bf16x8, x), acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 few_step(const uint4& x, const uint4& y, f32x4 acc, float) {
+    const float4 p = __builtin_bit_cast(float4, x), q = __builtin_bit_cast(float4, y);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(q.x, p.x, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(q.y, p.y, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(q.z, p.z, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(q.w, p.w, acc, 0, 0, 0);
+}
 
-constexpr int FEW_WAVES = 8, FEW_ROWS = 64;
+constexpr int FEW_WAVES = 8, FEW_AHEAD = 4;
 
 // 16 rows x 16 columns a workgroup; wave w takes steps w, w + 8, ... of the
-// contracted index (32 of bf16, 16 of fp32) and the partial tiles meet in LDS
+// contracted index, FEW_AHEAD of them loaded before the first is used, and the
+// partial tiles meet in LDS
 template <typename T, int ACT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const GemmArgs a) {
+    constexpr int E = 16 / sizeof(T), STEP = 4 * E;   // elements of a lane, of a step
     __shared__ f32x4 part[FEW_WAVES][64];
-    const int w = threadIdx.x >> 6, l = lane_id(), r16 = l & 15, g4 = l >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), r16 = l & 15, g4 = l >> 4;
     const int m0 = 16 * ((int)blockIdx.x / a.nt), n0 = 16 * ((int)blockIdx.x % a.nt);
     const T* ra = static_cast<const T*>(a.a) + (size_t)min(m0 + r16, a.M - 1) * a.lda;
     const T* rb = static_cast<const T*>(a.b) + (size_t)min(n0 + r16, a.N - 1) * a.ldb;
     f32x4 acc = zero4();
-    if constexpr (std::is_same<T, float>::value) {
-        for (int k = 16 * w; k < a.K; k += 16 * FEW_WAVES) {
-            const int kk = k + 4 * g4;
-            const float4 x = ldc4<float>(ra + kk, a.K - kk, a.vec_a && kk + 4 <= a.K);
-            const float4 y = ldc4<float>(rb + kk, a.K - kk, a.vec_b && kk + 4 <= a.K);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y.x, x.x, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y.y, x.y, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y.z, x.z, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y.w, x.w, acc, 0, 0, 0);
+    const int whole = a.vec_a && a.vec_b ? a.K / STEP : 0, steps = (a.K + STEP - 1) / STEP;
+    int i = w;
+    for (; i < whole; i += FEW_AHEAD * FEW_WAVES) {
+        uint4 x[FEW_AHEAD], y[FEW_AHEAD];
+#pragma unroll
+        for (int u = 0; u < FEW_AHEAD; ++u) {
+            x[u] = y[u] = make_uint4(0, 0, 0, 0);
+            if (i + u * FEW_WAVES < whole) {
+                const int k = STEP * (i + u * FEW_WAVES) + E * g4;
+                x[u] = *reinterpret_cast<const uint4*>(ra + k);
+                y[u] = *reinterpret_cast<const uint4*>(rb + k);
+            }
         }
-    } else {
-#pragma unroll 4
-        for (int k = 32 * w; k < a.K; k += 32 * FEW_WAVES) {
-            const bf16x8 x = row8(ra, k + 8 * g4, a.K, a.vec_a), y = row8(rb, k + 8 * g4, a.K, a.vec_b);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, x, acc, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < FEW_AHEAD; ++u) acc = few_step(x[u], y[u], acc, T());
+    }
+    // a step that ends past K, or all of them where rows begin off 16 bytes
+    for (i = whole + (w + FEW_WAVES - whole % FEW_WAVES) % FEW_WAVES; i < steps; i += FEW_WAVES) {
+        const int k = STEP * i + E * g4;
+        if constexpr (std::is_same<T, float>::value) {
+            acc = few_step(__builtin_bit_cast(uint4, ldc4<float>(ra + k, a.K - k, false)),
+                           __builtin_bit_cast(uint4, ldc4<float>(rb + k, a.K - k, false)), acc, T());
+        } else {
+            acc = few_step(__builtin_bit_cast(uint4, row8(ra, k, a.K)), __builtin_bit_cast(uint4, row8(rb, k, a.K)), acc, T());
         }
     }
     part[w][l] = acc;
@@ -941,9 +962,24 @@ hipError_t launch_f32(GemmArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Pieces of 16 x 16 instead of tiles: while they are few enough for all CUs at once,
+// of bf16 two a CU, of fp32 (products on the fp32 matrix unit here) four.  us, pieces
+// against tiles:
+//   rows, product          pieces        bf16            fp32
+//      1, 384 -> 1536          96      3.2    4.3      3.9   12.1
+//     64, 384 -> 1536         384      4.2    4.5      5.8   12.6
+//    128, 384 -> 1536         768      5.9    4.5      9.2   12.6
+//     16, 2048 -> 8192        512     10.4   16.3     17.7   53.7
+//     32, 2048 -> 8192       1024     17.7   16.8     31.7   54.4
+//     64, 2048 -> 8192       2048     33.3   17.2     59.7   54.7
+//     64, 8192 -> 2048        512     31.0   56.6     59.3  203.9
+//    128, 8192 -> 2048       1024     58.5   56.7    114.9  204.5
+//    256, 8192 -> 2048       2048    113.7   57.2    226.4  202.4
+bool few(int M, int N, int bf16) { return ((int64_t)M + 15) / 16 * ((N + 15) / 16) <= (bf16 ? 512 : 1024); }
+
 template <int ACT>
 hipError_t launch_fwd(GemmArgs& a, int bf16, hipStream_t st) {
-    if (a.M <= FEW_ROWS) {
+    if (few(a.M, a.N, bf16)) {
         a.nt = (a.N + 15) / 16;
         a.mt = (a.M + 15) / 16;
         const dim3 grid((unsigned)a.mt * a.nt), block(64 * FEW_WAVES);
@@ -1173,7 +1209,7 @@ int kda_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, con
     LIN_TRY(check_map(M, N, K, act, dtype));
     if (M == 0) return KDA_OK;
     const int es = dtype == KDA_DTYPE_BF16 ? 2 : 4;
-    const bool dma = dtype == KDA_DTYPE_BF16 && M > FEW_ROWS;
+    const bool dma = dtype == KDA_DTYPE_BF16 && !few(M, N, 1);
     LIN_TRY(check_rows(x, "x", ld_x, K, dtype, dma));
     LIN_TRY(check_rows(w, "w", ld_w, K, dtype, dma));
     LIN_TRY(check_opt(bias, "bias", N, N, dtype));

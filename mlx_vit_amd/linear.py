@@ -34,7 +34,7 @@ from . import _lib
 from .kda import _DTYPE_CODE
 
 ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2}
-FEW_ROWS = 64        # up to here a forward's operands may have any alignment (kda_linear_fwd)
+FEW = 512            # up to so many pieces of 16 x 16 a forward's operands may have any alignment (kda_linear_fwd)
 MAX_STRIDE, MAX_ROWS = 1 << 21, (1 << 31) - 1
 _NULL = contextlib.nullcontext()
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
@@ -44,6 +44,10 @@ _grad_enabled = torch.is_grad_enabled
 def _on(dev: torch.device):
     """Launches go to the tensors' device, whatever the current one is."""
     return _NULL if dev.index == _current_device() else torch.cuda.device(dev)
+
+
+def _few(M: int, N: int) -> bool:
+    return (M + 15 >> 4) * (N + 15 >> 4) <= FEW
 
 
 def _up8(n: int) -> int:
@@ -92,7 +96,7 @@ def _forward(x2: torch.Tensor, K: int, w: torch.Tensor, bias, res2, act: int, y:
     code = _DTYPE_CODE[w.dtype]
     stream = _raw_stream(w.get_device())
     x2, w = _rows(x2), _rows(w)
-    if code and (train or M > FEW_ROWS):
+    if code and (train or not _few(M, N)):
         x2, w = _whole_rows(x2, w, stream)
     if M:
         if bias is not None and not bias.is_contiguous():
@@ -267,8 +271,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     """act(x weight^T + bias) + residual, differentiable.  x (..., K), weight (N, K),
     bias (N,), residual (..., N), all bf16 or all fp32; ``activation`` None, "gelu"
     (z Phi(z)) or "silu".  Rows and weights at any stride; bf16 rows that do not
-    begin on 16 bytes, or whose K is no multiple of 8, are copied first when there
-    are more than 64 of them or a gradient is needed."""
+    begin on 16 bytes, or whose K is no multiple of 8, are copied first when y has
+    more than 512 pieces of 16 x 16 or a gradient is needed."""
     act = _check("linear_act", x, ((weight, bias),), residual, activation)
     # (a forward-mode tangent: the node refuses it, the kernels would drop it)
     if _grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
@@ -276,6 +280,17 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         return LinearActFunction.apply(x, weight, bias, residual, act)
     N, K = weight.shape
     y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    px, pw, M, code = x.data_ptr(), weight.data_ptr(), x.numel() // K, _DTYPE_CODE[x.dtype]
+    if (M and x.is_contiguous() and weight.is_contiguous() and (bias is None or bias.is_contiguous())
+            and (residual is None or residual.is_contiguous()) and not (code and ((px | pw) & 15 or K & 7) and not _few(M, N))
+            and K <= MAX_STRIDE and N <= MAX_STRIDE and x.get_device() == _current_device()):
+        # as they lie: half the time of such a call is the host's
+        rc = _lib.load().kda_linear_fwd(
+            px, K, pw, K, None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), N,
+            y.data_ptr(), N, None, 0, M, N, K, act, code, _raw_stream(x.get_device()))
+        if rc:
+            _lib.check(rc, "kda_linear_fwd")
+        return y
     with _on(x.device):
         _forward(_flat(x, K), K, weight, bias, _flat(residual, N), act, y.data_ptr(), N, None, 0, False)
     return y

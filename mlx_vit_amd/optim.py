@@ -17,6 +17,7 @@ finite makes its whole block of 8-bit moments NaN.
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 from typing import Dict, Iterable, List, Optional, Tuple
 
 import torch
@@ -28,7 +29,13 @@ from .linear import _on, _raw_stream
 
 BLOCK = 256      # elements that share a scale; a tensor's moments begin on a multiple of it
 _STATES = {"fp32": 0, "int8": 1}
-_data_ptr, _contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_data_ptr, _contiguous, _nbytes = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, attrgetter("nbytes")
+
+
+def _overlap(spans: List[Tuple[int, int]]) -> bool:
+    """Do any two of these (address, bytes) share memory?"""
+    spans = sorted(s for s in spans if s[1])
+    return any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:]))
 
 
 class FusedAdamW:
@@ -41,6 +48,9 @@ class FusedAdamW:
     ``state`` of an optimizer over the same tensors holds them: "m", "v" (fp32, or
     int8 and uint8 with "m_scale" and "v_scale"), "master"; parameter i's part
     begins at ``offsets[i]`` and what lies between two parameters' is zero.
+
+    With ``master_weights`` a weight that is changed other than by ``step`` gets its
+    master's value back at the next one.
 
     Parameters are contiguous fp32 or bf16 tensors on one ROCm device; those
     without a gradient at a step are left out of it."""
@@ -67,6 +77,7 @@ class FusedAdamW:
                                  f"{p.dtype}, shape {tuple(p.shape)}, strides {p.stride()}")
         self._dtypes = [p.dtype for p in self.params]
         self._numels = [p.numel() for p in self.params]
+        self._bytes = [p.nbytes for p in self.params]
         self.offsets: List[int] = []
         at = 0
         for n in self._numels:
@@ -77,6 +88,7 @@ class FusedAdamW:
         # p, g, n, offset, dtype of each parameter
         self._ptrs: List[int] = []
         self._plan: Optional[torch.Tensor] = None
+        self._captured: List[torch.Tensor] = []
         self._table = array("q", [v for n, o, t in zip(self._numels, self.offsets, self._dtypes)
                                   for v in (0, 0, n, o, _DTYPE_CODE[t])])
         self._check_params(list(map(_data_ptr, self.params)))
@@ -110,6 +122,8 @@ class FusedAdamW:
                     or s.data_ptr() & 15):
                 raise ValueError(f"state[{k!r}] must be a contiguous 16-byte aligned {t} tensor of {n} elements on "
                                  f"{self.device}; got {s.dtype}, shape {tuple(s.shape)} on {s.device}")
+        if _overlap([(s.data_ptr(), s.nbytes) for s in state.values()]):
+            raise ValueError("state's buffers overlap in memory")
         return dict(state)
 
     @property
@@ -159,8 +173,7 @@ class FusedAdamW:
             if p.dtype != t or p.numel() != n or not p.is_contiguous() or p.device != self.device:
                 raise ValueError(f"a parameter of {n} elements of {t} is now {tuple(p.shape)}, {p.dtype}, strides "
                                  f"{p.stride()} on {p.device}: make a new optimizer")
-        spans = sorted((a, p.nbytes) for a, p in zip(ptrs, self.params) if p.nbytes)
-        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+        if _overlap([(a, p.nbytes) for a, p in zip(ptrs, self.params)]):
             raise ValueError("parameters overlap in memory (one of them is given twice, or two share a storage)")
         self._ptrs = ptrs
         # while these are held no other tensor can come to lie at the same address
@@ -174,7 +187,7 @@ class FusedAdamW:
                 raise RuntimeError("parameters were moved since the last step: take one outside the capture first")
             torch.cuda.synchronize(self.device)   # a step may be reading the old plan, on any stream
         self._plan = plan.to(self.device)
-        self._parts = lib.kda_grad_norm_workspace_size(at, count) // 8
+        self._parts = lib.kda_adamw_step_workspace_size(at, count) // 8
 
     def _gradients(self) -> List[Optional[torch.Tensor]]:
         """Fill the descriptors for a step; returns the gradients, to be kept until the launches."""
@@ -182,14 +195,18 @@ class FusedAdamW:
         if ptrs != self._ptrs:
             self._check_params(ptrs)
         gs = present = [p.grad for p in self.params]
-        dtypes = self._dtypes
-        missing = [i for i, g in enumerate(gs) if g is None]
+        sizes = self._bytes
+        missing = any(g is None for g in gs)
         if missing:
             present = [g for g in gs if g is not None]
-            dtypes = [t for t, g in zip(dtypes, gs) if g is not None]
-        if [g.dtype for g in present] != dtypes:
-            raise ValueError("a gradient's dtype is not its parameter's")
+            sizes = [n for n, g in zip(sizes, gs) if g is not None]
+        # (each such look at 436 tensors is 15 us of the host's)
+        if list(map(_nbytes, present)) != sizes:
+            raise ValueError("a gradient's size or dtype is not that of its parameter when the optimizer was made")
         if not all(map(_contiguous, present)):
+            # gradients lie as their parameters do
+            if not all(map(_contiguous, self.params)):
+                raise ValueError("a parameter is no longer contiguous: make a new optimizer")
             gs = [g if g is None else g.detach().contiguous() for g in gs]
         self._table[1::5] = array("q", [0 if g is None else g.data_ptr() for g in gs] if missing
                                   else list(map(_data_ptr, gs)))
@@ -207,22 +224,22 @@ class FusedAdamW:
         c1 = 1.0 / (1.0 - b1 ** self.steps) if self.bias_correction else 1.0
         c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
         lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
+        if torch.cuda.is_current_stream_capturing() and not any(t is self._plan for t in self._captured):
+            self._captured.append(self._plan)   # the graph reads it at each replay, also after parameters moved
         plan = self._plan.data_ptr()
         get = self._state.get
         buffers = [None if t is None else t.data_ptr()
                    for t in (get("m"), get("v"), get("m_scale"), get("v_scale"), get("master"))]
-        clip = pc = None
+        clip, pc, pw, parts = None, None, None, 0
         with _on(self.device):
-            stream = _raw_stream(self.device.index)
             if max_norm is not None:
                 # the norm, the clip factor, the norm's partial sums (fp64)
-                clip = torch.empty(2 + 2 * self._parts, dtype=torch.float32, device=self.device)
+                parts = self._parts
+                clip = torch.empty(2 + 2 * parts, dtype=torch.float32, device=self.device)
                 pc = clip.data_ptr()
-                rc = lib.kda_grad_norm(at, count, plan, max_norm, pc, pc + 8, 8 * self._parts, stream)
-                if rc:
-                    _lib.check(rc, "kda_grad_norm")
-            rc = lib.kda_adamw_step(at, count, plan, _STATES[self.states], *buffers, pc, self.lr, b1, b2, self.eps,
-                                    self.weight_decay, c1, c2, stream)
+                pw = pc + 8
+            rc = lib.kda_adamw_step(at, count, plan, _STATES[self.states], *buffers, max_norm or 0.0, pc, self.lr, b1, b2,
+                                    self.eps, self.weight_decay, c1, c2, pw, 8 * parts, _raw_stream(self.device.index))
             if rc:
                 _lib.check(rc, "kda_adamw_step")
         return None if clip is None else clip[0]

@@ -56,7 +56,7 @@ def test_fused_adamw_refuses():
 
 
 def _fwd(lib, **kw):
-    a = dict(x=4096, ld_x=64, w=8192, ld_w=64, bias=None, res=None, ld_r=0, y=16384, ld_y=32, z=None, ld_z=0, M=100, N=32,
+    a = dict(x=4096, ld_x=64, w=8192, ld_w=64, bias=None, res=None, ld_r=0, y=16384, ld_y=32, z=None, ld_z=0, M=9000, N=32,
              K=64, act=0, dtype=1, stream=None)
     a.update(kw)
     return lib.kda_linear_fwd(*a.values())
@@ -118,8 +118,10 @@ def _tensor(p=4096, g=8192, n=10, offset=0, dtype=1):
     return (ctypes.c_int64 * 5)(p, g, n, offset, dtype)
 
 
-def _step(lib, t, count=1, states=0, m=4096, v=8192, ms=None, vs=None, master=None, b1=0.9, b2=0.95, eps=1e-8, c1=1.0, c2=1.0, plan=4096):
-    return lib.kda_adamw_step(t, count, plan, states, m, v, ms, vs, master, None, 1e-3, b1, b2, eps, 0.05, c1, c2, None)
+def _step(lib, t, count=1, states=0, m=4096, v=8192, ms=None, vs=None, master=None, b1=0.9, b2=0.95, eps=1e-8, c1=1.0, c2=1.0, plan=4096,
+          norm=0.0, clip=4096, ws=8192, n=1 << 10):
+    return lib.kda_adamw_step(t, count, plan, states, m, v, ms, vs, master, norm, clip, 1e-3, b1, b2, eps, 0.05, c1, c2, ws, n,
+                              None)
 
 
 def test_c_abi_adamw_refuses():
@@ -139,11 +141,10 @@ def test_c_abi_adamw_refuses():
     assert lib.kda_adamw_plan(t, 1, at, n - 1) == -3 and lib.kda_adamw_plan(t, 1, None, n) == -1
     assert lib.kda_adamw_plan(_tensor(p=0), 1, at, n) == -1
     assert _step(lib, None, count=1) == -1 and _step(lib, None, count=0) == 0
-    norm = lambda **kw: lib.kda_grad_norm(*{**dict(t=t, count=1, plan=4096, max_norm=1.0, out=4096, ws=8192, n=1 << 10, st=None), **kw}.values())  # noqa: E731
-    for kw, rc in ((dict(out=None), -1), (dict(out=4098), -1), (dict(max_norm=0.0), -1), (dict(max_norm=float("nan")), -1),
-                   (dict(ws=None), -1), (dict(ws=8196), -1), (dict(n=0), -3), (dict(count=-1), -1), (dict(plan=None), -1), (dict(plan=4100), -1)):
-        assert norm(**kw) == rc, kw
-    assert lib.kda_grad_norm_workspace_size(_tensor(n=100000), 1) >= 4
+    for kw, rc in ((dict(clip=None), -1), (dict(clip=4098), -1), (dict(norm=-1.0), -1), (dict(norm=float("nan")), -1),
+                   (dict(ws=None), -1), (dict(ws=8196), -1), (dict(n=0), -3)):
+        assert _step(lib, t, **{"norm": 1.0, **kw}) == rc, kw
+    assert lib.kda_adamw_step_workspace_size(_tensor(n=100000), 1) >= 8
     mom = lambda **kw: lib.kda_adamw_moments(*{**dict(m=4096, v=4096, ms=4096, vs=4096, mo=4096, vo=4096, n=256, dt=1, st=None), **kw}.values())  # noqa: E731
     for kw, rc in ((dict(n=100), -1), (dict(n=-256), -1), (dict(dt=3), -2), (dict(m=None), -1), (dict(mo=4100), -1), (dict(ms=None), -1)):
         assert mom(**kw) == rc, kw

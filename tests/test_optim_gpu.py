@@ -408,3 +408,61 @@ def test_moved_parameters():
         FusedAdamW(b, state={"m": buf})
     with pytest.raises(ValueError, match="elements"):
         FusedAdamW(b, state={"m": buf, "v": buf})
+    with pytest.raises(ValueError, match="buffers overlap"):
+        FusedAdamW([torch.nn.Parameter(torch.zeros(256, device=DEV))], state={"m": buf[:256], "v": buf[:256]})
+
+
+def test_parameters_changed_in_place_are_refused():
+    """The same address, other elements: a part of the parameter, its transpose."""
+    from mlx_vit_amd import FusedAdamW
+    p = torch.nn.Parameter(torch.zeros(32, 16, device=DEV))
+    whole = p.data
+    opt = FusedAdamW([p])
+    for other, match in ((whole[:8], "size or dtype"), (whole.t(), "make a new optimizer")):
+        p.grad = None
+        p.data = other
+        p.grad = torch.ones_like(p)
+        with pytest.raises(ValueError, match=match):
+            opt.step()
+    assert opt.steps == 0 and bool((whole == 0).all())
+    p.grad = None
+    p.data = whole
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert bool((whole != 0).all())
+
+
+def test_graph_of_a_step_before_parameters_moved():
+    """A captured step goes on updating the memory that it was captured with."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.bfloat16] * len(SIZES), seed=9) for _ in range(2))
+    oa, ob = FusedAdamW(a), FusedAdamW(b)
+    for ps in (a, b):
+        _grads(ps, 3)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        norm = oa.step(0.5)
+    old = [p.data for p in a]
+    grads = [p.grad for p in a]
+    for p in a:
+        p.grad = None
+        p.data = p.data.clone()
+    oa.step()      # the plan is made again; no gradients: nothing moves
+    for k in range(3):
+        junk = [torch.full((4096,), -1, dtype=torch.int64, device=DEV) for _ in range(8)]   # noqa: F841 (takes freed memory)
+        g.replay()
+        assert torch.equal(norm, ob.step(0.5))
+        assert all(torch.equal(x, q) for x, q in zip(old, b)) and len(grads) == len(a)
+
+
+@pytest.mark.parametrize("n", [(1 << 23) - 5, (1 << 23) + 5])
+def test_norm_of_many_elements(n):
+    """2048 partial sums of the norm and 2049: joined by the update itself, by a launch before it."""
+    from mlx_vit_amd import FusedAdamW
+    (p,) = params = _params([(n,)], [torch.bfloat16], seed=10)
+    _grads(params, 4)
+    opt = FusedAdamW(params, lr=1e-2)
+    _check_step(opt, _before(opt, params), Plain(1e-2, (0.9, 0.95), 1e-8, 0.05), 1.0, params)
+    exact = p.grad.double().square().sum().sqrt()
+    assert torch.equal(opt.step(1.0), exact.float())
