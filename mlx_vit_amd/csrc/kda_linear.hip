@@ -800,20 +800,20 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const Ge
 }
 
 // dz = dy act'(z) (ACT 0: dy), rows of ld_dz elements whose columns from N to the
-// next multiple of eight are zero; 64 rows x 256 columns a workgroup.  part: the
+// next multiple of eight are zero; `rows` rows x 256 columns a workgroup.  part: the
 // columns' sums before dz is rounded, [row of workgroups][N].
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ z,
                                                                  T* __restrict__ dz, float* __restrict__ part,
                                                                  int64_t ld_dy, int64_t ld_z, int64_t ld_dz, int M, int N,
-                                                                 int vec_in) {
+                                                                 int rows, int vec_in) {
     constexpr bool F32 = std::is_same<T, float>::value;
     __shared__ float sums[8][256];
     const int nb = (N + 255) / 256, rb = (int)blockIdx.x / nb, r0 = threadIdx.x >> 5, c = threadIdx.x & 31;
     const int n = 256 * ((int)blockIdx.x - rb * nb) + 8 * c, left = N - n;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (left > 0)
-        for (int m = 64 * rb + r0; m < min(M, 64 * rb + 64); m += 8) {
+        for (int m = rows * rb + r0; m < min(M, rows * rb + rows); m += 8) {
             float g[8], x[8];
             ldc8<T>(dy + (size_t)m * ld_dy + n, left, vec_in, g);
             if constexpr (ACT != 0) {
@@ -999,18 +999,25 @@ hipError_t dgrad(int act, int bf16, GemmArgs& a, hipStream_t st) {
     return act == 1 ? launch_dgrad<1>(a, bf16, st) : act == 2 ? launch_dgrad<2>(a, bf16, st) : launch_dgrad<0>(a, bf16, st);
 }
 
+// Rows a workgroup of it takes, by how many there are for 256 CUs (a backward pass
+// without dx, us, 64 rows | 16: 1571 x 395, 50 of 64 rows, 35 | 26; 4096 x 1024, 256,
+// 32 | 29; 3136 x 1536, 294, 34 | 31; 8192 x 1024, 512, 39 | 40; 12544 x 1536, 1176,
+// 52 | 58): more workgroups against fewer partial sums
+int act_rows(int M, int N) { return ((int64_t)M + 63) / 64 * ((N + 255) / 256) >= 512 ? 64 : 16; }
+int act_parts(int M, int N) { return (int)(((int64_t)M + act_rows(M, N) - 1) / act_rows(M, N)); }
+
 template <typename T>
 hipError_t launch_act_bwd(const void* dy, const void* z, void* dz, float* part, int64_t ld_dy, int64_t ld_z, int64_t ld_dz,
                           int M, int N, int act, hipStream_t st) {
     constexpr int ES = sizeof(T);
     const int vec = N % 8 == 0 && groups_ok(dy, ld_dy, ES) && groups_ok(act ? z : nullptr, ld_z, ES);
-    const dim3 grid((unsigned)((M + 63) / 64) * ((N + 255) / 256)), block(256);
+    const dim3 grid((unsigned)act_parts(M, N) * ((N + 255) / 256)), block(256);
     const T *pdy = static_cast<const T*>(dy), *pz = static_cast<const T*>(z);
     T* pdz = static_cast<T*>(dz);
     const auto kernel = act == 1   ? kda_linear_act_bwd_kernel<T, 1>
                         : act == 2 ? kda_linear_act_bwd_kernel<T, 2>
                                    : kda_linear_act_bwd_kernel<T, 0>;
-    hipLaunchKernelGGL(kernel, grid, block, 0, st, pdy, pz, pdz, part, ld_dy, ld_z, ld_dz, M, N, vec);
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, pdy, pz, pdz, part, ld_dy, ld_z, ld_dz, M, N, act_rows(M, N), vec);
     return hipGetLastError();
 }
 
@@ -1266,7 +1273,7 @@ size_t kda_linear_bwd_workspace_size(const void* dy, int64_t ld_dy, int M, int N
     const int bf16 = dtype == KDA_DTYPE_BF16;
     const Mat d = {dy, ld_dy, N};
     const Wgrad g = {d, {nullptr, up8(K), K}, nullptr, const_cast<void*>(dy)};
-    const size_t sums = sums_apart(act, bf16) ? up256((size_t)((M + 63) / 64) * N * sizeof(float)) : 0;
+    const size_t sums = sums_apart(act, bf16) ? up256((size_t)act_parts(M, N) * N * sizeof(float)) : 0;
     return dz_bytes(d, M, act, bf16) + sums + wgrads_bytes(&g, 1, M, bf16);
 }
 
@@ -1295,7 +1302,7 @@ int kda_linear_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, c
     float* part = db && sums_apart(act, bf16) ? reinterpret_cast<float*>(ws + dz_bytes(dz, M, act, bf16)) : nullptr;
     LIN_HIP(make_dz(&dz, z, ld_z, M, act, bf16, &ws, part, st), "kda_linear_bwd");
     if (part) {
-        const int rows = (M + 63) / 64;
+        const int rows = act_parts(M, N);
         LIN_HIP(launch_colsum(part, db, rows, N, st), "kda_linear_bwd");
         ws += up256((size_t)rows * N * sizeof(float));
         db = nullptr;
