@@ -330,9 +330,10 @@ int kda_log_decay_bwd(const void* alpha, const float* dg, void* dalpha, int64_t 
  * the backward pass reads.  act: 0 none, 1 gelu (z Phi(z)), 2 silu.  All of
  * dtype; sums, epilogue and activation in fp32.  Matrices are rows of ld_*
  * elements (at most 2^21), unit column stride.  bf16 with ceil(M / 16) ceil(N / 16)
- * above 512: x and w 16-byte aligned, ld_x and ld_w multiples of 8 that cover K
- * rounded up to 8, and that many elements of the last row readable; other
- * operands and smaller or fp32 ones: any stride, aligned to their element.
+ * above 256 (above 512 where M <= 8): x and w 16-byte aligned, ld_x and ld_w
+ * multiples of 8 that cover K rounded up to 8, and that many elements of the last
+ * row readable; other operands and smaller or fp32 ones: any stride, aligned to
+ * their element.
  * Outputs overlap neither each other nor an input, here and below. */
 #define KDA_ACT_NONE 0
 #define KDA_ACT_GELU 1

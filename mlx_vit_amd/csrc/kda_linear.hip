@@ -359,7 +359,7 @@ __device__ __forceinline__ void zero_tail(char* tile, int valid) {
     }
 }
 
-// C tile of BM x BN by WR x WC waves, 64 of the contracted index a step, two
+// C tile of BM x BN by WR x WC waves, 64 of the contracted index a step, NB
 // buffers.  BT: B's rows run across the contracted index (dgrad).  WPE: waves a
 // SIMD that the registers have to leave room for.
 //
@@ -368,15 +368,15 @@ __device__ __forceinline__ void zero_tail(char* tile, int valid) {
 // There is one barrier a step, in its middle: by then a wave holds its second
 // half in registers and its share of the next step has landed, so behind it the
 // next step's first half can be read and this step's buffer filled with the step
-// after the next.  (16384 x 2048 x 8192 in tiles of 128 x 128: 622 -> 526 us.)  It
+// NB after it.  (16384 x 2048 x 8192 in tiles of 128 x 128: 622 -> 526 us.)  It
 // takes a second set of fragments, which sixteen waves of 64 x 64 have no
 // registers for: there four waves a SIMD hide the reads.
-template <int BM, int BN, int WR, int WC, int WPE, bool AHEAD, bool BT, int ACT, bool DG>
+template <int BM, int BN, int WR, int WC, int WPE, int NB, bool AHEAD, bool BT, int ACT, bool DG>
 __global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(const GemmArgs a) {
     constexpr int BK = 64, W = WR * WC, RBA = 2 * BK, RBB = BT ? 2 * BN : 2 * BK, ROWB = BT ? BK : BN;
     constexpr int SA = BM * RBA, STAGE = SA + ROWB * RBB;
     constexpr int FM = BM / WR / 16, FN = BN / WC / 16;
-    static_assert(W * 64 * FN * 32 <= 2 * STAGE && FM % 2 == 0 && FN <= 4, "the epilogue's rows");
+    static_assert(W * 64 * FN * 32 <= NB * STAGE && FM % 2 == 0 && FN <= 4, "the epilogue's rows");
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), r16 = l & 15, g4 = l >> 4;
     const int wm = (w / WC) * (BM / WR), wn = (w % WC) * (BN / WC);
@@ -440,14 +440,13 @@ __global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(cons
     // wave's has, and every wave has read the step before (AHEAD: its second half is
     // in registers)
     if constexpr (AHEAD) {
+        static_assert(NB == 2 || NB == 4, "the waits");
         if (steps > 0) {
-            issue(0);
-            if (steps > 1) {
-                issue(1);
-                dma_wait<L>();
-            } else {
-                dma_wait<0>();
-            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (b < steps) issue(b);
+            if (steps >= NB) dma_wait<(NB - 1) * L>();
+            else dma_wait<0>();
             lds_barrier();
             Frags f, g;
             read(f, 0, 0);
@@ -455,21 +454,23 @@ __global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(cons
                 read(g, buf, 1);
                 multiply(f);
                 if (s + 1 < steps) {
-                    dma_wait<0>();
+                    dma_wait_chunks<L>(min(NB - 2, steps - 2 - s));   // what is issued behind step s + 1
                     lds_barrier();
-                    if (s + 2 < steps) issue(buf);
-                    read(f, 1 - buf, 0);
+                    if (s + NB < steps) issue(buf);
+                    read(f, (buf + 1) % NB, 0);
                 }
                 multiply(g);
             };
             int s = 0;
-            for (; s + 1 < steps; s += 2) {
-                step(s, 0);
-                step(s + 1, 1);
-            }
-            if (s < steps) step(s, 0);
+            for (; s + NB <= steps; s += NB)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) step(s + b, b);
+#pragma unroll
+            for (int b = 0; b < NB - 1; ++b)
+                if (s + b < steps) step(s + b, b);
         }
     } else {
+        static_assert(NB == 2, "two buffers");
         if (steps > 0) issue(0);
 #pragma unroll 1
         for (int s = 0; s < steps; ++s) {
@@ -890,10 +891,10 @@ bool groups_ok(const void* p, int64_t ld, int es) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (16 / es) == 0);
 }
 
-template <int BM, int BN, int WR, int WC, int WPE, bool AHEAD, bool BT, int ACT, bool DG>
+template <int BM, int BN, int WR, int WC, int WPE, int NB, bool AHEAD, bool BT, int ACT, bool DG>
 hipError_t launch_tiles(GemmArgs& a, hipStream_t st) {
-    constexpr size_t LDS = 2 * (BM + BN) * 128;
-    const auto kernel = kda_linear_bf16_kernel<BM, BN, WR, WC, WPE, AHEAD, BT, ACT, DG>;
+    constexpr size_t LDS = NB * (BM + BN) * 128;
+    const auto kernel = kda_linear_bf16_kernel<BM, BN, WR, WC, WPE, NB, AHEAD, BT, ACT, DG>;
     if constexpr (LDS > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
@@ -923,13 +924,20 @@ int bf16_tile(int M, int N, int K) {   // its edge
     const int64_t m256 = (M + 255) / 256, n256 = (N + 255) / 256, m128 = (M + 127) / 128, n128 = (N + 127) / 128;
     return m256 * n256 >= 144 && K >= 512 ? 256 : m128 * n128 >= 192 ? 128 : 64;
 }
+// Four buffers instead of two for tiles of 64 x 64: where a CU has one of them, a step
+// takes as long as a load, and four steps' loads then overlap (us, 2 | 4 buffers:
+// 64 tiles, K 8192, 55 | 27; 128, K 2048, 16.3 | 9.3; 256, K 1024, 6.6 | 6.2; 294, K 1536,
+// 12.7 | 11.5); more tiles hide each other's loads and need the room, and few steps fill
+// no four buffers (588, K 768, 8.7 | 10.3; 312, K 384, 4.9 | 5.3; 96, K 384, 4.0 | 4.1)
+bool deep(int M, int N, int K) { return ((int64_t)M + 63) / 64 * ((N + 63) / 64) <= 320 && K >= 512; }
 template <bool BT, int ACT, bool DG>
 hipError_t launch_bf16(GemmArgs& a, hipStream_t st) {
     switch (bf16_tile(a.M, a.N, a.K)) {
-        case 256: return launch_tiles<256, 256, 4, 4, 4, false, BT, ACT, DG>(a, st);
-        case 128: return launch_tiles<128, 128, 2, 4, 4, true, BT, ACT, DG>(a, st);
-        default: return launch_tiles<64, 64, 2, 2, 4, true, BT, ACT, DG>(a, st);
+        case 256: return launch_tiles<256, 256, 4, 4, 4, 2, false, BT, ACT, DG>(a, st);
+        case 128: return launch_tiles<128, 128, 2, 4, 4, 2, true, BT, ACT, DG>(a, st);
     }
+    return deep(a.M, a.N, a.K) ? launch_tiles<64, 64, 2, 2, 4, 4, true, BT, ACT, DG>(a, st)
+                               : launch_tiles<64, 64, 2, 2, 4, 2, true, BT, ACT, DG>(a, st);
 }
 // rows of waves of such a product, each with its column sums
 int wave_rows(int M, int N, int K) {
@@ -963,19 +971,24 @@ hipError_t launch_f32(GemmArgs& a, hipStream_t st) {
 }
 
 // Pieces of 16 x 16 instead of tiles: while they are few enough for all CUs at once,
-// of bf16 two a CU, of fp32 (products on the fp32 matrix unit here) four.  us, pieces
-// against tiles:
-//   rows, product          pieces        bf16            fp32
-//      1, 384 -> 1536          96      3.2    4.3      3.9   12.1
+// and twice as many up to 8 rows, whose x the CUs' caches hold.  In fp32 the pieces
+// have the fp32 matrix unit's products and no splitting.  us, pieces | tiles:
+//   rows, product          pieces        bf16             fp32
+//      1, 384 -> 1536          96      3.3    4.3      3.9   12.1
+//    128, 384 -> 384          192      3.6    4.5      4.5   12.5
+//     32, 8192 -> 2048        256     17.2   27.5     33.2  203.3
 //     64, 384 -> 1536         384      4.2    4.5      5.8   12.6
-//    128, 384 -> 1536         768      5.9    4.5      9.2   12.6
-//     16, 2048 -> 8192        512     10.4   16.3     17.7   53.7
-//     32, 2048 -> 8192       1024     17.7   16.8     31.7   54.4
-//     64, 2048 -> 8192       2048     33.3   17.2     59.7   54.7
-//     64, 8192 -> 2048        512     31.0   56.6     59.3  203.9
-//    128, 8192 -> 2048       1024     58.5   56.7    114.9  204.5
-//    256, 8192 -> 2048       2048    113.7   57.2    226.4  202.4
-bool few(int M, int N, int bf16) { return ((int64_t)M + 15) / 16 * ((N + 15) / 16) <= (bf16 ? 512 : 1024); }
+//     48, 8192 -> 2048        384     31.0   27.5
+//      8, 2048 -> 8192        512      9.0    9.4     15.9   53.8
+//     16, 2048 -> 8192        512     10.3    9.4     17.9   53.9
+//      1, 4096 -> 16384      1024     24.0   20.6     48.4  118.7
+//     32, 2048 -> 8192       1024     17.8    9.8     31.7   54.4
+//    128, 8192 -> 2048       1024     58.7   27.3    114.9  204.5
+//      8, 1024 -> 32768      2048     18.8   14.0     31.3   57.0
+//     64, 2048 -> 8192       2048     33.1   10.0     59.7   54.7
+bool few(int M, int N, int bf16) {
+    return ((int64_t)M + 15) / 16 * ((N + 15) / 16) <= (bf16 ? 256 : 1024) * (M <= 8 ? 2 : 1);
+}
 
 template <int ACT>
 hipError_t launch_fwd(GemmArgs& a, int bf16, hipStream_t st) {

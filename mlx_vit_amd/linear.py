@@ -34,7 +34,6 @@ from . import _lib
 from .kda import _DTYPE_CODE
 
 ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2}
-FEW = 512            # up to so many pieces of 16 x 16 a forward's operands may have any alignment (kda_linear_fwd)
 MAX_STRIDE, MAX_ROWS = 1 << 21, (1 << 31) - 1
 _NULL = contextlib.nullcontext()
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
@@ -47,7 +46,8 @@ def _on(dev: torch.device):
 
 
 def _few(M: int, N: int) -> bool:
-    return (M + 15 >> 4) * (N + 15 >> 4) <= FEW
+    """A bf16 forward's operands may have any alignment (kda_linear_fwd)."""
+    return (M + 15 >> 4) * (N + 15 >> 4) <= (512 if M <= 8 else 256)
 
 
 def _up8(n: int) -> int:
@@ -272,7 +272,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     bias (N,), residual (..., N), all bf16 or all fp32; ``activation`` None, "gelu"
     (z Phi(z)) or "silu".  Rows and weights at any stride; bf16 rows that do not
     begin on 16 bytes, or whose K is no multiple of 8, are copied first when y has
-    more than 512 pieces of 16 x 16 or a gradient is needed."""
+    more than 256 pieces of 16 x 16 (512 up to 8 rows) or a gradient is needed."""
     act = _check("linear_act", x, ((weight, bias),), residual, activation)
     # (a forward-mode tangent: the node refuses it, the kernels would drop it)
     if _grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)

@@ -15,8 +15,9 @@ DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
 # M, K, N
 SIZES = [(1, 8, 1), (1, 384, 174), (3, 5, 7), (17, 33, 19), (64, 40, 130), (65, 8, 8), (65, 7, 9), (128, 64, 128),
          (129, 100, 257), (131, 31, 33), (200, 384, 520), (300, 772, 395), (257, 520, 136), (70, 1536, 384),
-         # forwards in tiles of 64 x 64 (bf16 alone; both)
-         (700, 33, 200), (2100, 41, 130), (3000, 96, 7), (2060, 130, 136)]
+         # forwards in tiles of 64 x 64 (bf16 alone or both; few steps and many), the largest in pieces
+         (700, 33, 200), (2100, 41, 130), (3000, 96, 7), (2060, 130, 136), (2050, 1501, 130), (9, 600, 5000),
+         (8, 70, 8200)]
 
 
 def _mk(seed, *shape, dt, scale=1.0):
