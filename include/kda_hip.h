@@ -327,9 +327,10 @@ int kda_log_decay_bwd(const void* alpha, const float* dg, void* dalpha, int64_t 
  * nope_gdn_mlx.py:216-262, 4009-4091):
  *   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]
  * for m < M, n < N, k < K; z (may be NULL) receives the value before act, which
- * the backward pass reads.  act: 0 none, 1 gelu (z Phi(z)), 2 silu.  All of
- * dtype; sums, epilogue and activation in fp32.  Matrices are rows of ld_*
- * elements (at most 2^21), unit column stride.  bf16 with ceil(M / 16) ceil(N / 16)
+ * the backward pass reads: fp32, or fp16 beside bf16 (infinite past its range).
+ * act: 0 none, 1 gelu (z Phi(z)), 2 silu.  The others are of dtype; sums, epilogue
+ * and activation in fp32.  Matrices are rows of ld_* elements (at most 2^21), unit
+ * column stride.  bf16 with ceil(M / 16) ceil(N / 16)
  * above 256 (above 512 where M <= 8): x and w 16-byte aligned, ld_x and ld_w
  * multiples of 8 that cover K rounded up to 8, and that many elements of the last
  * row readable; other operands and smaller or fp32 ones: any stride, aligned to

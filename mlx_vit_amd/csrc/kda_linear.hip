@@ -42,7 +42,7 @@ struct GemmArgs {
 //          Phi)) / z up to |z| = 5 (18 slots): gelu is off by at most 4e-4 of its
 //          value, a tenth of a bf16 half step, and by 4e-7 below -5.
 //   gelu': 1/2 + z Q(t), t = 2 z^2 / 4.8^2 - 1, the minimax fit of an odd function up
-//          to |z| = 4.8 and its end beyond (14 slots): off by at most 3e-5.
+//          to |z| = 4.8 and its end beyond (14 slots): off by at most 3e-5, beyond by 5e-5.
 // fp32 results take Abramowitz & Stegun's 7.1.26: with u = |z| / sqrt 2, t = 1 / (1 +
 // 0.3275911 u), Phi(-|z|) = e^{-u^2} P(t) / 2 within 7.5e-8, the rounding of 1 + erf
 // itself; the library's erf has two branches that a wave takes both.
@@ -105,6 +105,8 @@ __device__ __forceinline__ float act_grad(float z) {
         const float p = phi_exp(z, e);
         return fmaf(z * e, 0.39894228040143268f, p);
     } else if constexpr (ACT == 2) {
+        // (bf16's z may be past its range: infinite)
+        if constexpr (!F32) z = __builtin_elementwise_maximum(__builtin_elementwise_minimum(z, 65504.f), -65504.f);
         const float s = sigma(z);
         return s * fmaf(z, 1.f - s, 1.f);
     } else {
@@ -136,39 +138,70 @@ __device__ __forceinline__ void stc4(T* p, const float4& v, int n, bool vec) {
     if (n > 3) st1<T>(p + 3, v.w);
 }
 
+// What z is kept in beside bf16 results: fp16, three more bits in the same room.  As
+// bf16 it put a fifth of its rounding's size on top of dz's own in every gradient
+// (off by 1.46 half steps where 1.41 is two roundings).  Past fp16's range it is
+// infinite, where both derivatives are at their ends.
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+template <typename T>
+using Pre = typename std::conditional<std::is_same<T, float>::value, float, _Float16>::type;
+
 // eight columns at p (n of them exist): vec: 16-byte accesses
 template <typename T>
 __device__ __forceinline__ void ldc8(const T* p, int n, bool vec, float (&v)[8]) {
-    if (vec) {
-        if constexpr (std::is_same<T, float>::value) {
-            const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-            v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    if constexpr (std::is_same<T, _Float16>::value) {
+        if (vec) {
+            const half8v h = *reinterpret_cast<const half8v*>(p);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
         } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(p);
-            v[0] = bf_lo(x.x); v[1] = bf_hi(x.x); v[2] = bf_lo(x.y); v[3] = bf_hi(x.y);
-            v[4] = bf_lo(x.z); v[5] = bf_hi(x.z); v[6] = bf_lo(x.w); v[7] = bf_hi(x.w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.f;
         }
         return;
-    }
+    } else {
+        if (vec) {
+            if constexpr (std::is_same<T, float>::value) {
+                const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+            } else {
+                const uint4 x = *reinterpret_cast<const uint4*>(p);
+                v[0] = bf_lo(x.x); v[1] = bf_hi(x.x); v[2] = bf_lo(x.y); v[3] = bf_hi(x.y);
+                v[4] = bf_lo(x.z); v[5] = bf_hi(x.z); v[6] = bf_lo(x.w); v[7] = bf_hi(x.w);
+            }
+            return;
+        }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? ld1<T>(p + e) : 0.f;
+        for (int e = 0; e < 8; ++e) v[e] = e < n ? ld1<T>(p + e) : 0.f;
+    }
 }
 template <typename T>
 __device__ __forceinline__ void stc8(T* p, const float (&v)[8], int n, bool vec) {
-    if (vec) {
-        if constexpr (std::is_same<T, float>::value) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4*>(p) =
-                make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
-        }
-        return;
-    }
+    if constexpr (std::is_same<T, _Float16>::value) {
+        half8v h;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < n) st1<T>(p + e, v[e]);
+        for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
+        if (vec) *reinterpret_cast<half8v*>(p) = h;
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < n) p[e] = h[e];
+    } else {
+        if (vec) {
+            if constexpr (std::is_same<T, float>::value) {
+                *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                *reinterpret_cast<uint4*>(p) =
+                    make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) st1<T>(p + e, v[e]);
+    }
 }
 
 // Where an epilogue reads and writes: column n of row m in each matrix, moved down a
@@ -176,11 +209,13 @@ __device__ __forceinline__ void stc8(T* p, const float (&v)[8], int n, bool vec)
 // was a fifth of the epilogue's instructions)
 template <typename T, bool DG>
 struct Place {
-    const T* in;   // DG: zin, else the residual
-    T *z, *c;
+    typedef typename std::conditional<DG, Pre<T>, T>::type In;
+    const In* in;   // DG: zin, else the residual
+    Pre<T>* z;
+    T* c;
     __device__ __forceinline__ Place(const GemmArgs& a, int m, int n)
-        : in(static_cast<const T*>(DG ? a.zin : a.res) + (size_t)m * (DG ? a.ldzi : a.ldr) + n),
-          z(static_cast<T*>(a.zout) + (size_t)m * a.ldzo + n), c(static_cast<T*>(a.c) + (size_t)m * a.ldc + n) {}
+        : in(static_cast<const In*>(DG ? a.zin : a.res) + (size_t)m * (DG ? a.ldzi : a.ldr) + n),
+          z(static_cast<Pre<T>*>(a.zout) + (size_t)m * a.ldzo + n), c(static_cast<T*>(a.c) + (size_t)m * a.ldc + n) {}
     __device__ __forceinline__ void down(const GemmArgs& a, int rows) {
         in += rows * (DG ? a.ldzi : a.ldr);
         if constexpr (!DG) z += rows * a.ldzo;
@@ -197,7 +232,7 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, const Place<T, DG>& a
     float t[8];
     if constexpr (DG) {
         if constexpr (ACT != 0) {
-            ldc8<T>(at.in, left, vec, t);
+            ldc8<Pre<T>>(at.in, left, vec, t);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[e] *= act_grad<ACT, F32>(t[e]);
@@ -208,7 +243,7 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, const Place<T, DG>& a
         if (a.res) ldc8<T>(at.in, left, vec, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bias[e];
-        if (a.zout) stc8<T>(at.z, v, left, vec);
+        if (a.zout) stc8<Pre<T>>(at.z, v, left, vec);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = act<ACT, F32>(v[e]);
         if (a.res)
@@ -804,7 +839,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const Ge
 // next multiple of eight are zero; `rows` rows x 256 columns a workgroup.  part: the
 // columns' sums before dz is rounded, [row of workgroups][N].
 template <typename T, int ACT>
-__global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ z,
+__global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __restrict__ dy, const Pre<T>* __restrict__ z,
                                                                  T* __restrict__ dz, float* __restrict__ part,
                                                                  int64_t ld_dy, int64_t ld_z, int64_t ld_dz, int M, int N,
                                                                  int rows, int vec_in) {
@@ -818,7 +853,7 @@ __global__ __launch_bounds__(256) void kda_linear_act_bwd_kernel(const T* __rest
             float g[8], x[8];
             ldc8<T>(dy + (size_t)m * ld_dy + n, left, vec_in, g);
             if constexpr (ACT != 0) {
-                ldc8<T>(z + (size_t)m * ld_z + n, left, vec_in, x);
+                ldc8<Pre<T>>(z + (size_t)m * ld_z + n, left, vec_in, x);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     g[e] *= act_grad<ACT, F32>(x[e]);
@@ -1025,7 +1060,8 @@ hipError_t launch_act_bwd(const void* dy, const void* z, void* dz, float* part, 
     constexpr int ES = sizeof(T);
     const int vec = N % 8 == 0 && groups_ok(dy, ld_dy, ES) && groups_ok(act ? z : nullptr, ld_z, ES);
     const dim3 grid((unsigned)act_parts(M, N) * ((N + 255) / 256)), block(256);
-    const T *pdy = static_cast<const T*>(dy), *pz = static_cast<const T*>(z);
+    const T* pdy = static_cast<const T*>(dy);
+    const Pre<T>* pz = static_cast<const Pre<T>*>(z);
     T* pdz = static_cast<T*>(dz);
     const auto kernel = act == 1   ? kda_linear_act_bwd_kernel<T, 1>
                         : act == 2 ? kda_linear_act_bwd_kernel<T, 2>

@@ -12,9 +12,9 @@ and ``mlp`` two of them, the reference's block MLP with its skip connection
 One kernel forms a product and its epilogue; the backward pass applies the
 activation's derivative in the epilogue of the product that needs it, and forms
 weight and bias gradients in one launch.  Sums, epilogues and activations are
-fp32; each tensor that is stored (y, and for the backward pass the value before
-the activation and the hidden layer) is rounded once to the inputs' dtype, bf16
-or fp32.  fp32 products split each operand exactly into three bf16 parts and
+fp32; each tensor that is stored (y, and for the backward pass the hidden layer) is
+rounded once to the inputs' dtype, bf16 or fp32, the value before the activation to
+fp16 where that is bf16.  fp32 products split each operand exactly into three bf16 parts and
 keep what is at least 2^-16 of the largest product, fp32's own accuracy; an
 infinite fp32 operand gives NaN where fp32 arithmetic may give an infinity.
 
@@ -34,6 +34,7 @@ from . import _lib
 from .kda import _DTYPE_CODE
 
 ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2}
+_PRE = {torch.float32: torch.float32, torch.bfloat16: torch.float16}    # what the value before the activation is kept in
 MAX_STRIDE, MAX_ROWS = 1 << 21, (1 << 31) - 1
 _NULL = contextlib.nullcontext()
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
@@ -180,7 +181,7 @@ class LinearActFunction(torch.autograd.Function):
             x2 = _flat(x, K)
             M = x2.shape[0]
             y = _new(x, *x.shape[:-1], N)
-            z = _new(x, M, _up8(N)) if act else None
+            z = torch.empty((M, _up8(N)), dtype=_PRE[x.dtype], device=x.device) if act else None
             x2, w = _forward(x2, K, weight, bias, _flat(residual, N), act, y.data_ptr(), N, _out(z), _up8(N), True)
         ctx.save_for_backward(x2, w, z)
         ctx.act, ctx.shape, ctx.N = act, x.shape, N
@@ -225,7 +226,7 @@ class MLPFunction(torch.autograd.Function):
             x2 = _flat(x, K)
             M = x2.shape[0]
             h = _new(x, M, _up8(N))
-            z = _new(x, M, _up8(N)) if act else None
+            z = torch.empty((M, _up8(N)), dtype=_PRE[x.dtype], device=x.device) if act else None
             y = _new(x, *x.shape[:-1], O)
             x2, w1 = _forward(x2, K, w1, b1, None, act, h.data_ptr(), _up8(N), _out(z), _up8(N), True)
             h, w2 = _forward(h, N, w2, b2, _flat(residual, O), 0, y.data_ptr(), O, None, 0, True)

@@ -313,6 +313,29 @@ def test_forward_mode_tangents_are_refused():
                 f()
 
 
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("M", [5, 4100])
+def test_values_past_fp16(M, act):
+    """z of +-3 10^5: the activation is z or nothing there, its derivative 1 or 0."""
+    from mlx_vit_amd import linear_act
+    x = torch.full((M, 8), 300000.0, dtype=torch.bfloat16, device=DEV)
+    x[1::2] = -x[1::2]
+    w = torch.eye(8, dtype=torch.bfloat16, device=DEV)
+    dy = _mk(90, M, 8, dt=torch.bfloat16)
+    leaves = _leaves(x, w)
+    y = linear_act(x, w, activation=act)
+    assert torch.equal(y, x.clamp(min=0))
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    # gelu's derivative is off by at most 6e-5 (the sum in linear_reference: the fit's 2.92e-5 and 1.83e-5 between the
+    # true one's value where the fit ends and here), silu's by nothing here; dw's rounding, and its sum by 2^-20 of its terms
+    d = 6e-5 if act == "gelu" else 0.0
+    with torch.no_grad():
+        dz = torch.where(x > 0, dy, 0).double()
+        assert ((dx.double() - dz).abs() <= d * dy.double().abs()).all()
+        want, size = dz.t() @ x.double(), 3e5 * dy.double().abs().sum(0).unsqueeze(1)
+        assert ((dw.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -20 + d) * size).all()
+
+
 def test_other_stream():
     from mlx_vit_amd import mlp
     x, w1, b1, _, _ = _inputs(300, 64, 128, torch.bfloat16, True, False, seed=80)
