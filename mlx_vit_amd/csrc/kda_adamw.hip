@@ -17,6 +17,11 @@
 // the root that the update divides by, and a v above zero keeps a code above
 // zero, so no weight is divided by eps alone.  The update itself uses the new
 // moments before they are rounded to codes.
+//
+// All are one pass over memory.  A copy of 1 GiB moves 5.1 TB/s here, a sum that
+// only reads 3.9: 3.1 10^8 bf16 weights with fp32 moments (22 bytes each) take 1264 us
+// at 5.4 TB/s, in 8 bits (10 bytes) 595 at 5.2, the norm (2 bytes) 151 at 4.1, reading
+// the 8-bit moments into bf16 (6 bytes) 373 at 5.0.
 #include <math.h>
 
 #include "kda_hip.h"
@@ -247,7 +252,8 @@ __global__ __launch_bounds__(256) void kda_adamw_kernel(const StepArgs a, const 
 // The norm's sums are fp64 from the first square on: the clip factor then is the
 // exact one rounded, and does not depend on the order (the conversion and the
 // addition cost two more operations a value than fp32 sums, in a pass that waits
-// for memory).
+// for memory; four pieces a workgroup with their loads in flight together measured the
+// same: 2^28 elements with the update 1226 us and 1225).
 __global__ __launch_bounds__(256) void kda_grad_norm_kernel(double* __restrict__ part, const Grads q) {
     __shared__ double lds[4];
     const uint32_t wg = q.wg + blockIdx.x;

@@ -5,9 +5,19 @@
 //   dgrad     dx[m][k] = (sum_n dz[m][n] W[n][k]) * act'(zin[m][k])
 //   wgrad     dW[n][k] = sum_m dz[m][n] x[m][k], db[n] = sum_m dz[m][n]   (fp32; bf16: kda_wgrad.hip)
 //
-// Both are one product C[m][n] = sum_k A[m][k] B(k, n); the operand whose rows
-// run along the contracted index (W in dgrad, both in wgrad) reaches the MFMA
+// All are one product C[m][n] = sum_k A[m][k] B(k, n); the operand whose rows
+// run across the contracted index (W in dgrad, both in wgrad) reaches the MFMA
 // through transposing LDS reads, so nothing is transposed in memory.
+//
+// What bounds them: 2 M N K operations against the matrix unit (1391 TFLOP/s of
+// bf16 in an 8192^3 product by the library here), the rows' bytes where K or N is
+// a few hundred (the 25088 x 1536 hidden layer of a block: 77 MB, 15 us a pass at a
+// copy's 5.1 TB/s), the epilogue's instructions beside them, and a load's latency
+// where there are fewer tiles than CUs.  Measured (forward, bias and activation
+// within): 16384 x 2048 -> 8192 gelu 495 us, 1110 TFLOP/s (without activation 461; the
+// library's bare product 404); 25088 x 384 -> 1536 gelu 51 us and 1536 -> 384 with the
+// residual 37 (the library's bare products 61 and 38); 196 x 384 -> 1536 5 us; 1 x 384 ->
+// 174 4 us.
 #include "kda_hip.h"
 #include "kda_internal.h"
 
@@ -619,6 +629,12 @@ struct Stage32 {
 // C tile of BM x BN by WR x WC waves, 32 of the contracted index a step.  AT, BT:
 // the operand's rows run across the contracted index.  PART: one of a.splits
 // parts of it, into a.part (and with a.bpart A's column sums).
+//
+// Six bf16 products for one: at 1391 TFLOP/s of those no more than 232 of fp32's,
+// where the library's fp32 products reach 154 at 8192^3 and 85 at 6272 x 384 <-> 1536.
+// Here 6272 x 384 -> 1536 takes 54 us (137 TFLOP/s), 4096^3 663 (207).  What bounds it
+// is the way to LDS: each value is loaded, split (nine instructions) and stored once
+// a tile, in one buffer, the next step's loads in flight over the products.
 template <int BM, int BN, int WR, int WC, bool AT, bool BT, int ACT, bool DG, bool PART>
 __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_f32_kernel(const GemmArgs a) {
     constexpr int BK = 32, TH = 64 * WR * WC, FM = BM / WR / 16, FN = BN / WC / 16;
@@ -781,7 +797,9 @@ constexpr int FEW_WAVES = 8, FEW_AHEAD = 4;
 
 // 16 rows x 16 columns a workgroup; wave w takes steps w, w + 8, ... of the
 // contracted index, FEW_AHEAD of them loaded before the first is used, and the
-// partial tiles meet in LDS
+// partial tiles meet in LDS.  Bound by the weights' bytes where there are many of
+// them (1 x 2048 -> 8192: 33.6 MB in 7.7 us, 4.4 TB/s) and by the chain of a launch, a
+// load and the LDS round where there are few (1 x 384 -> 174: 3 us).
 template <typename T, int ACT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const GemmArgs a) {
     constexpr int E = 16 / sizeof(T), STEP = 4 * E;   // elements of a lane, of a step
@@ -835,6 +853,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const Ge
     finish8<T, ACT, false, std::is_same<T, float>::value>(a, Place<T, false>(a, m, n), a.N - n, v, bias);
 }
 
+// (Memory-bound: 25088 x 1536 reads and writes 231 MB in about 50 us.)
 // dz = dy act'(z) (ACT 0: dy), rows of ld_dz elements whose columns from N to the
 // next multiple of eight are zero; `rows` rows x 256 columns a workgroup.  part: the
 // columns' sums before dz is rounded, [row of workgroups][N].
