@@ -9,15 +9,15 @@
 // run across the contracted index (W in dgrad, both in wgrad) reaches the MFMA
 // through transposing LDS reads, so nothing is transposed in memory.
 //
-// What bounds them: 2 M N K operations against the matrix unit (1391 TFLOP/s of
-// bf16 in an 8192^3 product by the library here), the rows' bytes where K or N is
-// a few hundred (the 25088 x 1536 hidden layer of a block: 77 MB, 15 us a pass at a
+// What bounds them: 2 M N K operations against the matrix unit (1391 to 1634
+// TFLOP/s of bf16 in an 8192^3 product by the library here, as the card's clock
+// allows), the rows' bytes where K or N is a few hundred (the 25088 x 1536 hidden layer of a block: 77 MB, 15 us a pass at a
 // copy's 5.1 TB/s), the epilogue's instructions beside them, and a load's latency
 // where there are fewer tiles than CUs.  Measured (forward, bias and activation
-// within): 16384 x 2048 -> 8192 gelu 495 us, 1110 TFLOP/s (without activation 461; the
-// library's bare product 404); 25088 x 384 -> 1536 gelu 51 us and 1536 -> 384 with the
-// residual 37 (the library's bare products 61 and 38); 196 x 384 -> 1536 5 us; 1 x 384 ->
-// 174 4 us.
+// within): 16384 x 2048 -> 8192 gelu 483 us, 1138 TFLOP/s (without activation 450; the
+// library's bare product 371); 25088 x 384 -> 1536 gelu 53 us and 1536 -> 384 with the
+// residual 38 (the library's bare products 56 and 33); 196 x 384 -> 1536 4.6 us; 1 x 384 ->
+// 174 3.4 us.
 #include "kda_hip.h"
 #include "kda_internal.h"
 
@@ -415,7 +415,10 @@ __device__ __forceinline__ void zero_tail(char* tile, int valid) {
 // next step's first half can be read and this step's buffer filled with the step
 // NB after it.  (16384 x 2048 x 8192 in tiles of 128 x 128: 622 -> 526 us.)  It
 // takes a second set of fragments, which sixteen waves of 64 x 64 have no
-// registers for: there four waves a SIMD hide the reads.
+// registers for: there four waves a SIMD hide the reads.  (Eight waves of 128 x 64 with
+// fragments a quarter of a step ahead instead: 8192^3 833 us against 865, 16384 x 2048
+// -> 8192 499 and 503, but 12544 x 768 -> 3200 92 and 88, where eight waves are fewer for
+// the epilogue.)
 template <int BM, int BN, int WR, int WC, int WPE, int NB, bool AHEAD, bool BT, int ACT, bool DG>
 __global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(const GemmArgs a) {
     constexpr int BK = 64, W = WR * WC, RBA = 2 * BK, RBB = BT ? 2 * BN : 2 * BK, ROWB = BT ? BK : BN;
@@ -630,11 +633,12 @@ struct Stage32 {
 // the operand's rows run across the contracted index.  PART: one of a.splits
 // parts of it, into a.part (and with a.bpart A's column sums).
 //
-// Six bf16 products for one: at 1391 TFLOP/s of those no more than 232 of fp32's,
+// Six bf16 products for one: at 1634 TFLOP/s of those no more than 272 of fp32's,
 // where the library's fp32 products reach 154 at 8192^3 and 85 at 6272 x 384 <-> 1536.
-// Here 6272 x 384 -> 1536 takes 54 us (137 TFLOP/s), 4096^3 663 (207).  What bounds it
-// is the way to LDS: each value is loaded, split (nine instructions) and stored once
-// a tile, in one buffer, the next step's loads in flight over the products.
+// Here 6272 x 384 -> 1536 takes 52 us (142 TFLOP/s), 4096^3 684 (201; the library
+// 913).  What bounds it is the way to LDS: each value is loaded, split (nine
+// instructions) and stored once a tile, in one buffer, the next step's loads in
+// flight over the products.
 template <int BM, int BN, int WR, int WC, bool AT, bool BT, int ACT, bool DG, bool PART>
 __global__ __launch_bounds__(64 * WR * WC, 2) void kda_linear_f32_kernel(const GemmArgs a) {
     constexpr int BK = 32, TH = 64 * WR * WC, FM = BM / WR / 16, FN = BN / WC / 16;
@@ -853,7 +857,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kda_linear_few_kernel(const Ge
     finish8<T, ACT, false, std::is_same<T, float>::value>(a, Place<T, false>(a, m, n), a.N - n, v, bias);
 }
 
-// (Memory-bound: 25088 x 1536 reads and writes 231 MB in about 50 us.)
+// (Bound by memory: 25088 x 1536 reads and writes 231 MB in 38.5 us, 6.0 TB/s.)
 // dz = dy act'(z) (ACT 0: dy), rows of ld_dz elements whose columns from N to the
 // next multiple of eight are zero; `rows` rows x 256 columns a workgroup.  part: the
 // columns' sums before dz is rounded, [row of workgroups][N].
