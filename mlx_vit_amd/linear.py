@@ -18,8 +18,9 @@ fp16 where that is bf16.  fp32 products split each operand exactly into three bf
 keep what is at least 2^-16 of the largest product, fp32's own accuracy; an
 infinite fp32 operand gives NaN where fp32 arithmetic may give an infinity.
 
-Differentiable in every tensor; a second derivative is refused.  There is no CPU
-path.
+Differentiable in every tensor; a second derivative and tracing are refused.  There
+is no CPU path.  A backward pass is captured into a graph as torch's own nodes are:
+while no eager graph of the same leaves is alive.
 """
 from __future__ import annotations
 
@@ -38,7 +39,7 @@ _PRE = {torch.float32: torch.float32, torch.bfloat16: torch.float16}    # what t
 MAX_STRIDE, MAX_ROWS = 1 << 21, (1 << 31) - 1
 _NULL = contextlib.nullcontext()
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-_grad_enabled = torch.is_grad_enabled
+_grad_enabled, _is_tracing = torch.is_grad_enabled, torch._C._is_tracing
 
 
 def _on(dev: torch.device):
@@ -148,6 +149,8 @@ def _check(what: str, x: torch.Tensor, maps, residual: Optional[torch.Tensor], a
             raise ValueError(f"{what}: {name} is on {t.device}, x on {dev}")
     if dev.type != "cuda":
         raise ValueError(f"{what} runs on a ROCm device; got tensors on {dev}")
+    if _is_tracing():
+        raise RuntimeError(f"{what} cannot be traced: its launches are no part of a traced graph")
     if x.numel() > MAX_ROWS * shape[-1]:
         raise ValueError(f"{what}: x of shape {tuple(shape)} has more than {MAX_ROWS} rows")
     return act

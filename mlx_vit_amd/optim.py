@@ -29,6 +29,7 @@ from .linear import _on, _raw_stream
 
 BLOCK = 256      # elements that share a scale; a tensor's moments begin on a multiple of it
 _STATES = {"fp32": 0, "int8": 1}
+_increment_version = torch._C._increment_version
 _data_ptr, _contiguous, _nbytes = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, attrgetter("nbytes")
 
 
@@ -196,12 +197,14 @@ class FusedAdamW:
             self._check_params(ptrs)
         gs = present = [p.grad for p in self.params]
         sizes = self._bytes
-        missing = any(g is None for g in gs)
-        if missing:
-            present = [g for g in gs if g is not None]
-            sizes = [n for n, g in zip(sizes, gs) if g is not None]
         # (each such look at 436 tensors is 15 us of the host's)
-        if list(map(_nbytes, present)) != sizes:
+        try:
+            fits, missing = list(map(_nbytes, gs)) == sizes, False
+        except AttributeError:   # None
+            missing = True
+            present = [g for g in gs if g is not None]
+            fits = [g.nbytes for g in present] == [n for n, g in zip(sizes, gs) if g is not None]
+        if not fits:
             raise ValueError("a gradient's size or dtype is not that of its parameter when the optimizer was made")
         if not all(map(_contiguous, present)):
             # gradients lie as their parameters do
@@ -242,6 +245,8 @@ class FusedAdamW:
                                     self.eps, self.weight_decay, c1, c2, pw, 8 * parts, _raw_stream(self.device.index))
             if rc:
                 _lib.check(rc, "kda_adamw_step")
+        # a graph that holds the weights as they were has to notice
+        _increment_version(self.params)
         return None if clip is None else clip[0]
 
     def zero_grad(self) -> None:

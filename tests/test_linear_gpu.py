@@ -394,3 +394,11 @@ def test_blocks_mlp_as_one_operator():
             assert calls == [1, 1]
         finally:
             mod.mlp = real
+
+
+def test_tracing_is_refused():
+    from mlx_vit_amd import linear_act, mlp
+    x, w, b, _, _ = _inputs(9, 16, 16, torch.float32)
+    for f in (lambda t: linear_act(t, w, b), lambda t: mlp(t, w, b, w, b)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (x,))

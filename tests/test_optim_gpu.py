@@ -466,3 +466,15 @@ def test_norm_of_many_elements(n):
     _check_step(opt, _before(opt, params), Plain(1e-2, (0.9, 0.95), 1e-8, 0.05), 1.0, params)
     exact = p.grad.double().square().sum().sqrt()
     assert torch.equal(opt.step(1.0), exact.float())
+
+
+def test_autograd_sees_that_weights_changed():
+    from mlx_vit_amd import FusedAdamW
+    p = torch.nn.Parameter(torch.ones(16, device=DEV))
+    x = torch.ones(16, device=DEV, requires_grad=True)
+    opt = FusedAdamW([p])
+    y = (x * p).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
