@@ -190,8 +190,9 @@ class FusedAdamW:
         self._plan = plan.to(self.device)
         self._parts = lib.kda_adamw_step_workspace_size(at, count) // 8
 
-    def _gradients(self) -> List[Optional[torch.Tensor]]:
-        """Fill the descriptors for a step; returns the gradients, to be kept until the launches."""
+    def _gradients(self) -> Tuple[List[Optional[torch.Tensor]], List[nn.Parameter]]:
+        """Fill the descriptors for a step; returns the gradients, to be kept until the
+        launches, and the parameters that have one."""
         ptrs = list(map(_data_ptr, self.params))
         if ptrs != self._ptrs:
             self._check_params(ptrs)
@@ -213,7 +214,7 @@ class FusedAdamW:
             gs = [g if g is None else g.detach().contiguous() for g in gs]
         self._table[1::5] = array("q", [0 if g is None else g.data_ptr() for g in gs] if missing
                                   else list(map(_data_ptr, gs)))
-        return gs
+        return gs, [p for p, g in zip(self.params, gs) if g is not None] if missing else self.params
 
     def step(self, max_norm: Optional[float] = None) -> Optional[torch.Tensor]:
         """One update.  With ``max_norm`` the gradients count scaled by
@@ -221,32 +222,36 @@ class FusedAdamW:
         fp32); the gradients themselves stay as they are."""
         if max_norm is not None and not max_norm > 0.0:
             raise ValueError(f"max_norm={max_norm}: expected a positive number or None")
-        gs = self._gradients()   # noqa: F841 (alive until the launches)
+        gs, updated = self._gradients()   # (gs: alive until the launches)
         self.steps += 1
         b1, b2 = self.betas
         c1 = 1.0 / (1.0 - b1 ** self.steps) if self.bias_correction else 1.0
         c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
         lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
-        if torch.cuda.is_current_stream_capturing() and not any(t is self._plan for t in self._captured):
-            self._captured.append(self._plan)   # the graph reads it at each replay, also after parameters moved
         plan = self._plan.data_ptr()
         get = self._state.get
         buffers = [None if t is None else t.data_ptr()
                    for t in (get("m"), get("v"), get("m_scale"), get("v_scale"), get("master"))]
         clip, pc, pw, parts = None, None, None, 0
         with _on(self.device):
+            if torch.cuda.is_current_stream_capturing() and not any(t is self._plan for t in self._captured):
+                self._captured.append(self._plan)   # the graph reads it at each replay, also after parameters moved
             if max_norm is not None:
-                # the norm, the clip factor, the norm's partial sums (fp64)
+                # the norm and the clip factor; the norm's partial sums (fp64), behind them while they
+                # are few, since who keeps the norm keeps what it lies in
                 parts = self._parts
-                clip = torch.empty(2 + 2 * parts, dtype=torch.float32, device=self.device)
+                clip = torch.empty(2 + 2 * parts if parts < 256 else 2, dtype=torch.float32, device=self.device)
                 pc = clip.data_ptr()
                 pw = pc + 8
+                if parts >= 256:
+                    sums = torch.empty(parts, dtype=torch.float64, device=self.device)
+                    pw = sums.data_ptr()
             rc = lib.kda_adamw_step(at, count, plan, _STATES[self.states], *buffers, max_norm or 0.0, pc, self.lr, b1, b2,
                                     self.eps, self.weight_decay, c1, c2, pw, 8 * parts, _raw_stream(self.device.index))
             if rc:
                 _lib.check(rc, "kda_adamw_step")
         # a graph that holds the weights as they were has to notice
-        _increment_version(self.params)
+        _increment_version(updated)
         return None if clip is None else clip[0]
 
     def zero_grad(self) -> None:

@@ -478,3 +478,16 @@ def test_autograd_sees_that_weights_changed():
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+    q = torch.nn.Parameter(torch.ones(16, device=DEV))
+    opt = FusedAdamW([p, q])
+    y = (x * q).sum()
+    opt.step()               # q has no gradient: it stays
+    y.backward()
+    assert torch.equal(x.grad, q.detach())
+
+
+def test_a_kept_norm_keeps_little():
+    from mlx_vit_amd import FusedAdamW
+    params = _params([(1 << 21,)], [torch.bfloat16], seed=11)
+    _grads(params, 5)
+    assert FusedAdamW(params).step(1.0).untyped_storage().nbytes() <= 4096
