@@ -402,3 +402,28 @@ def test_tracing_is_refused():
     for f in (lambda t: linear_act(t, w, b), lambda t: mlp(t, w, b, w, b)):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, (x,))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_offsets_past_32_bits(dtype):
+    """More than 2^31 elements in y, z, dy and dz: the first and the last rows, and what sums over all."""
+    from mlx_vit_amd import linear_act
+    M, K, N = 131142, 16, 16392
+    dt = DT[dtype]
+    x, w = _mk(300, M, K, dt=dt), _mk(301, N, K, dt=dt, scale=0.25)
+    row = _mk(302, N, dt=dt)
+    leaves = _leaves(x, w)
+    y = linear_act(x, w, activation="silu")
+    dx, dw = torch.autograd.grad(y, leaves, row.expand(M, N))
+    with torch.no_grad():
+        for rows in (slice(0, 70), slice(M - 70, M)):
+            want = L.linear_act(x[rows], w, None, None, "silu", row.expand(70, N).contiguous())
+            L.check("y", y[rows], want["y"])
+            L.check("dx", dx[rows], want["dx"])
+        # the last 8 columns' dw: half a step for dz's rounding and one for its own, and the sum's 2 M 2^-24
+        z = x.double() @ w[-8:].double().t()
+        sg = torch.sigmoid(z)
+        dz = row[-8:].double() * sg * (1 + z * (1 - sg))
+        want, size = dz.t() @ x.double(), dz.abs().t() @ x.double().abs()
+        tol = (2 * M + 16) * 2.0 ** -24 * size + torch.finfo(dt).eps * (size + want.abs())
+        assert ((dw[-8:].double() - want).abs() <= tol).all()

@@ -491,3 +491,29 @@ def test_a_kept_norm_keeps_little():
     params = _params([(1 << 21,)], [torch.bfloat16], seed=11)
     _grads(params, 5)
     assert FusedAdamW(params).step(1.0).untyped_storage().nbytes() <= 4096
+
+
+@pytest.mark.parametrize("states", ["fp32", "int8"])
+def test_offsets_past_32_bits(states):
+    """A tensor of more than 2^31 elements and one behind it: what a small one of the same values gets."""
+    from mlx_vit_amd import FusedAdamW
+    n = (1 << 31) + 300
+
+    def params(*sizes):
+        ps = [torch.nn.Parameter(torch.full((k,), 0.25, dtype=torch.bfloat16, device=DEV)) for k in sizes]
+        for p in ps:
+            p.grad = torch.full_like(p, 0.5)
+        return ps
+
+    (big, behind), (small,) = params(n, 300), params(300)
+    opt, ref = FusedAdamW([big, behind], lr=1e-2, states=states), FusedAdamW([small], lr=1e-2, states=states)
+    opt.step()
+    ref.step()
+    assert bool((small != 0.25).all())
+    assert bool((big == small[0]).all()) and torch.equal(behind, small)
+    for k in opt.state:
+        a, b = opt.state[k], ref.state[k]
+        assert torch.equal(a[-b.numel():], b), k
+    norm = opt.step(1.0)
+    exact = 0.5 * (n + 300) ** 0.5
+    assert abs(norm.item() - exact) <= 2.0 ** -23 * exact
