@@ -153,6 +153,8 @@ def _mlp_residual(block: nn.Module, x: torch.Tensor) -> torch.Tensor:
 class NoPEViTBlock(nn.Module):
     """Pre-norm ViT block, optional spatial-only attention (nope_gdn_mlx.py:216-262)."""
 
+    fused_mlp = False   # set_fused_mlp
+
     def __init__(self, embed_dim: int, num_heads: int, mlp_ratio: float = 4.0, dropout: float = 0.0,
                  spatial_tokens: Optional[int] = None, drop_path: float = 0.0):
         super().__init__()
@@ -162,7 +164,6 @@ class NoPEViTBlock(nn.Module):
         self.drop_path = DropPath(drop_path) if drop_path > 0 else nn.Identity()
         self.norm2 = nn.LayerNorm(embed_dim, eps=1e-6)
         self.mlp = _mlp(embed_dim, mlp_ratio, dropout)
-        self.fused_mlp = False   # set_fused_mlp
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, N, D = x.shape
@@ -207,6 +208,8 @@ class NoPEVideoEncoder(nn.Module):
 class HybridBlock(nn.Module):
     """One processor block, GDN or NoPE attention (nope_gdn_mlx.py:4009-4091)."""
 
+    fused_mlp = False   # set_fused_mlp
+
     def __init__(self, dim: int, num_heads: int, block_type: str = "gdn", head_dim: Optional[int] = None,
                  chunk_size: int = 64, mlp_ratio: float = 4.0, dropout: float = 0.0,
                  channel_wise_decay: bool = True, allow_neg_eigval: bool = False,
@@ -226,7 +229,6 @@ class HybridBlock(nn.Module):
             self.layer = NoPEMultiheadAttention(dim, num_heads, dropout)
         self.norm2 = nn.LayerNorm(dim, eps=1e-6)
         self.mlp = _mlp(dim, mlp_ratio, dropout)
-        self.fused_mlp = False   # set_fused_mlp
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None,
                 state: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
