@@ -147,6 +147,8 @@ class FusedAdamW:
         mo = torch.empty(self.total, dtype=dtype, device=self.device)
         vo = torch.empty_like(mo)
         with _on(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                self._use(_raw_stream(self.device.index))
             _lib.check(_lib.load().kda_adamw_moments(
                 _ptr(m), _ptr(v), _ptr(self._state["m_scale"]), _ptr(self._state["v_scale"]), _ptr(mo), _ptr(vo),
                 self.total, _DTYPE_CODE[dtype], _stream(self.device)), "kda_adamw_moments")
@@ -188,7 +190,16 @@ class FusedAdamW:
                 raise RuntimeError("parameters were moved since the last step: take one outside the capture first")
             torch.cuda.synchronize(self.device)   # a step may be reading the old plan, on any stream
         self._plan = plan.to(self.device)
+        self._home = _raw_stream(self.device.index)
         self._parts = lib.kda_adamw_step_workspace_size(at, count) // 8
+
+    def _use(self, stream: int, *more: torch.Tensor) -> None:
+        """Launches on ``stream`` read the buffers: if it is not the one they were made on, their
+        memory must not be given away before they have ended, even if the optimizer is dropped."""
+        if stream != self._home:
+            current = torch.cuda.current_stream(self.device)
+            for t in (*self._state.values(), *more):
+                t.record_stream(current)
 
     def _gradients(self) -> Tuple[List[Optional[torch.Tensor]], List[nn.Parameter]]:
         """Fill the descriptors for a step; returns the gradients, to be kept until the
@@ -234,7 +245,10 @@ class FusedAdamW:
                    for t in (get("m"), get("v"), get("m_scale"), get("v_scale"), get("master"))]
         clip, pc, pw, parts = None, None, None, 0
         with _on(self.device):
-            if torch.cuda.is_current_stream_capturing() and not any(t is self._plan for t in self._captured):
+            stream = _raw_stream(self.device.index)
+            if not torch.cuda.is_current_stream_capturing():
+                self._use(stream, self._plan)
+            elif not any(t is self._plan for t in self._captured):
                 self._captured.append(self._plan)   # the graph reads it at each replay, also after parameters moved
             if max_norm is not None:
                 # the norm and the clip factor; the norm's partial sums (fp64), behind them while they
@@ -247,7 +261,7 @@ class FusedAdamW:
                     sums = torch.empty(parts, dtype=torch.float64, device=self.device)
                     pw = sums.data_ptr()
             rc = lib.kda_adamw_step(at, count, plan, _STATES[self.states], *buffers, max_norm or 0.0, pc, self.lr, b1, b2,
-                                    self.eps, self.weight_decay, c1, c2, pw, 8 * parts, _raw_stream(self.device.index))
+                                    self.eps, self.weight_decay, c1, c2, pw, 8 * parts, stream)
             if rc:
                 _lib.check(rc, "kda_adamw_step")
         # a graph that holds the weights as they were has to notice

@@ -328,6 +328,27 @@ def test_other_stream():
     assert torch.equal(na, ob.step(1.0)) and all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("states", ["fp32", "int8"])
+def test_optimizer_dropped_behind_a_step_on_another_stream(states):
+    """Its memory is not given to others before the step has ended."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.float32] * len(SIZES), seed=12) for _ in range(2))
+    for ps in (a, b):
+        _grads(ps, 6)
+    FusedAdamW(b, states=states).step(1.0)
+    opt = FusedAdamW(a, states=states)
+    sizes = [t.numel() * t.element_size() for t in (*opt.state.values(), opt._plan)]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)   # some milliseconds
+        opt.step(1.0)
+    del opt
+    others = [torch.full((n,), 1, dtype=torch.uint8, device=DEV) for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and len(others) == 4 * len(sizes)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("states", ["fp32", "int8"])
 def test_training_step_of_a_block(states, dtype):
