@@ -44,15 +44,15 @@ struct GemmArgs {
 // activations: 0 none, 1 gelu (z Phi(z)), 2 silu (z sigma(z))
 // ----------------------------------------------------------------------------
 
-// Results rounded to bf16 take fitted forms, because the epilogue
-// is VALU-bound with erf: 38.5 million values cost a 25088 x 1536 product 25 us
-// with Abramowitz & Stegun's 7.1.26 (25 issue slots a value, exp2 and rcp four
-// each) where the product's data need 20.
-//   gelu:  Phi(z) = 1 / (1 + 2^{-z R(z^2)}), R the minimax fit of log2(Phi / (1 -
-//          Phi)) / z up to |z| = 5 (18 slots): gelu is off by at most 4e-4 of its
-//          value, a tenth of a bf16 half step, and by 4e-7 below -5.
-//   gelu': 1/2 + z Q(t), t = 2 z^2 / 4.8^2 - 1, the minimax fit of an odd function up
-//          to |z| = 4.8 and its end beyond (14 slots): off by at most 3e-5, beyond by 5e-5.
+// Results rounded to bf16 take a fit for gelu, because the epilogue is VALU-bound
+// there: with e = e^{-z^2/2}, t = 1 / (1 + 0.338 |z|),
+//   Phi(-|z|) = e P(t),  P the minimax polynomial of degree 5 for e^{z^2/2} Phi(-|z|),
+// 1.6e-6 of its value off up to |z| = 3.5 and 1e-5 up to 6, so that
+//   gelu  = z Phi(z): within 1e-5 of its value down to z = -6 (a 200th of a bf16 half
+//           step), where it is 6e-9; 1e-11 below;
+//   gelu' = Phi(z) + z phi(z), below zero e (P(t) - |z| / sqrt(2 pi)): within 3e-6 of
+//           its terms, so a unit far below zero gets a gradient that vanishes with e.
+// 20 and 21 issue slots a value (exp2 and rcp four each); a degree less is off by 1e-4.
 // fp32 results take Abramowitz & Stegun's 7.1.26: with u = |z| / sqrt 2, t = 1 / (1 +
 // 0.3275911 u), Phi(-|z|) = e^{-u^2} P(t) / 2 within 7.5e-8, the rounding of 1 + erf
 // itself; the library's erf has two branches that a wave takes both.
@@ -70,30 +70,24 @@ __device__ __forceinline__ float phi_exp(float z, float& e) {
     const float tail = 0.5f * p * t * e;
     return z >= 0.f ? 1.f - tail : tail;
 }
+// P(t), a = |z|
+__device__ __forceinline__ float tail_fast(float a) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.338f, a, 1.f));
+    float p = fmaf(-1.1298490e-01f, t, 3.6227307e-01f);
+    p = fmaf(p, t, -8.4105216e-02f);
+    p = fmaf(p, t, 2.1490058e-01f);
+    p = fmaf(p, t, 1.1856889e-01f);
+    return fmaf(p, t, 1.3469618e-03f);
+}
 __device__ __forceinline__ float gelu_fast(float z) {
-    const float s = fminf(z * z, 25.f);
-    float r = fmaf(-2.9020036e-08f, s, 2.0529139e-06f);
-    r = fmaf(r, s, -3.9314848e-05f);
-    r = fmaf(r, s, -8.4793003e-04f);
-    r = fmaf(r, s, 1.0687304e-01f);
-    r = fmaf(r, s, 2.3006303f);
-    return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z * r));
+    const float x = __builtin_amdgcn_exp2f(-0.72134752044448170f * (z * z)) * tail_fast(fabsf(z));
+    return z * (z < 0.f ? x : 1.f - x);
 }
 __device__ __forceinline__ float gelu_grad_fast(float z) {
-    // these minimum and maximum keep a NaN
-    const float c = __builtin_elementwise_maximum(__builtin_elementwise_minimum(z, 4.8f), -4.8f);
-    const float t = fmaf(c, c * 0.086805556f, -1.f);
-    float q = fmaf(2.4953399e-02f, t, -5.5430472e-02f);
-    q = fmaf(q, t, 3.6742341e-02f);
-    q = fmaf(q, t, -3.1934381e-02f);
-    q = fmaf(q, t, 7.8190073e-02f);
-    q = fmaf(q, t, -1.0049784e-01f);
-    q = fmaf(q, t, 8.8953942e-02f);
-    q = fmaf(q, t, -7.8604877e-02f);
-    q = fmaf(q, t, 7.3644958e-02f);
-    q = fmaf(q, t, -8.0312975e-02f);
-    q = fmaf(q, t, 1.4847238e-01f);
-    return fmaf(c, q, 0.5f);
+    // (bf16's z may be past its range, infinite: 0 times a finite value then; e keeps a NaN)
+    const float a = fminf(fabsf(z), 64.f), e = __builtin_amdgcn_exp2f(-0.72134752044448170f * (z * z));
+    const float x = e * fmaf(-0.39894228040143268f, a, tail_fast(a));
+    return z < 0.f ? x : 1.f - x;
 }
 // F32: for results kept in fp32
 template <int ACT, bool F32>
