@@ -85,3 +85,26 @@ def test_gelu_in_bf16(N):
            (_half_step(want, torch.bfloat16) + 1.5e-5 * want.abs() + 2e-11).unsqueeze(1).expand(y.shape))
     want = _gelu_grad(z)
     _check("gelu'", dx, want, _half_step(want, torch.bfloat16) + (4e-6 + 2e-7 * z * z) * _terms(z) + 2.0 ** -24 * (z > 0))
+
+
+def _dense(lo, hi, n=50001):
+    """fp32 values between lo and hi, none of them zero."""
+    return torch.linspace(lo, hi, n, dtype=torch.float64).to(DEV).float().add(2.0 ** -12)
+
+
+@pytest.mark.parametrize("N", [1, 72, 0], ids=["pieces", "tiles", "mlp"])
+def test_gelu_in_fp32(N):
+    """Phi(-a), a = |z|, relative: the fit 8.4e-9 up to 2.5 and e^(a - 2.5) of it beyond; e by three roundings of its
+    argument, 3 2^-24 a^2 / 2 = 9e-8 a^2, and its own 2^-23; w = c / (1 + c) by 2 2^-23 (the sum, the reciprocal's 2^-23,
+    the product), of which the polynomial P(w) passes on w P' / P, at most 0.8 a times; its roundings, each 2^-24 of a
+    partial value, 2.75 (a + 1) P 2^-24 in all; the product with e 2^-24: 3.5e-7 + 3.6e-7 a + 9e-8 a^2 + the fit.  Above zero
+    1 - x adds 2^-24, and gelu's product one more."""
+    x = _dense(-12, 40)
+    y, dx = _map(x, N, "gelu", torch.float32) if N else _mlp(x, "gelu", torch.float32)
+    z = x.double()
+    a = z.abs()
+    rel = 3.5e-7 + 3.6e-7 * a + 9e-8 * a * a + 8.4e-9 * torch.exp((a - 2.5).clamp(min=0, max=10))
+    want = _gelu(z)
+    tol = torch.where(z < 0, (rel + 2.0 ** -24) * want.abs(), z * (rel * _phi(-a) + 2.0 ** -23))
+    _check("gelu", y, want.unsqueeze(1).expand(y.shape), tol.unsqueeze(1).expand(y.shape))
+    _check("gelu'", dx, _gelu_grad(z), (rel + 2.0 ** -24) * _terms(z) + 2.0 ** -24 * (z > 0))
