@@ -57,7 +57,11 @@ struct GemmArgs {
 // |z|), which is 1/2 at w = 0: 8.4e-9 of its value off up to |z| = 2.5, so that what is
 // left is fp32 arithmetic (measured: Phi within 1.0e-7, at z = -5 within 2e-6 of its
 // value; (1 + erf) / 2 of fp32 values within 1.1e-7, of which nothing is left at -5).
+// sigma of an fp32 result takes the accurate functions: the rounding of log2(e) z alone
+// puts |z| 2^-24 of its value on the other (a 1000th of a bf16 half step at z = -40)
+template <bool F32>
 __device__ __forceinline__ float sigma(float z) {
+    if constexpr (F32) return 1.f / (1.f + expf(-z));
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
 }
 // e^{z^2/2} Phi(-a), a = |z|
@@ -102,7 +106,7 @@ __device__ __forceinline__ float act(float z) {
     if constexpr (ACT == 1) {
         return gelu<F32>(z);
     } else if constexpr (ACT == 2) {
-        return z * sigma(z);
+        return z * sigma<F32>(z);
     } else {
         return z;
     }
@@ -114,7 +118,7 @@ __device__ __forceinline__ float act_grad(float z) {
     } else if constexpr (ACT == 2) {
         // (bf16's z may be past its range: infinite)
         if constexpr (!F32) z = __builtin_elementwise_maximum(__builtin_elementwise_minimum(z, 65504.f), -65504.f);
-        const float s = sigma(z);
+        const float s = sigma<F32>(z);
         return s * fmaf(z, 1.f - s, 1.f);
     } else {
         return 1.f;

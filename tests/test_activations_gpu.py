@@ -108,3 +108,25 @@ def test_gelu_in_fp32(N):
     tol = torch.where(z < 0, (rel + 2.0 ** -24) * want.abs(), z * (rel * _phi(-a) + 2.0 ** -23))
     _check("gelu", y, want.unsqueeze(1).expand(y.shape), tol.unsqueeze(1).expand(y.shape))
     _check("gelu'", dx, _gelu_grad(z), (rel + 2.0 ** -24) * _terms(z) + 2.0 ** -24 * (z > 0))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("N", [1, 72, 0], ids=["pieces", "tiles", "mlp"])
+def test_silu(N, dtype):
+    """fp32: sigma is an exponential within 2^-23 of its value, a sum, a quotient of 2^-24 each, and one product:
+    2.5 2^-23.  bf16's argument of exp2 adds |z| 2^-24 twice, its exp2 and reciprocal 2^-23 each.  The derivative is
+    sigma (1 + z (1 - sigma)), where 1 - sigma is off by 2^-24 and what sigma is."""
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    x = _points(-60, 60) if dtype == "bf16" else _dense(-80, 80)
+    y, dx = _map(x, N, "silu", dt) if N else _mlp(x, "silu", dt)
+    z = x.double()
+    s = torch.special.expit(z)
+    rel = 2.0 ** -22 if dtype == "fp32" else 2.0 ** -21 + 2.0 ** -23 * z.abs()
+    own = (lambda v: _half_step(v, dt)) if dtype == "bf16" else lambda v: 0.0
+    want = z * s
+    tol = own(want) + (rel + 2.0 ** -24) * want.abs()
+    _check("silu", y, want.unsqueeze(1).expand(y.shape), tol.unsqueeze(1).expand(y.shape))
+    t = torch.special.expit(-z)
+    want = s * (1 + z * t)
+    tol = s * ((1 + z.abs() * t) * (rel + 2.0 ** -22) + z.abs() * (2.0 ** -23 + rel * s))
+    _check("silu'", dx, want, own(want) + tol)
