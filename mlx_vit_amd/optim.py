@@ -178,20 +178,23 @@ class FusedAdamW:
                                  f"{p.stride()} on {p.device}: make a new optimizer")
         if _overlap([(a, p.nbytes) for a, p in zip(ptrs, self.params)]):
             raise ValueError("parameters overlap in memory (one of them is given twice, or two share a storage)")
-        self._ptrs = ptrs
-        # while these are held no other tensor can come to lie at the same address
-        self._storages = [p.untyped_storage() for p in self.params]
-        self._table[0::5] = array("q", ptrs)
-        lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
-        plan = torch.empty(lib.kda_adamw_plan_size(at, count), dtype=torch.uint8)
-        _lib.check(lib.kda_adamw_plan(at, count, plan.data_ptr(), plan.numel()), "kda_adamw_plan")
+        if self._plan is not None and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("parameters were moved since the last step: take one outside the capture first")
+        table = array("q", self._table)
+        table[0::5] = array("q", ptrs)
+        lib, at, count = _lib.load(), table.buffer_info()[0], len(self.params)
+        host = torch.empty(lib.kda_adamw_plan_size(at, count), dtype=torch.uint8)
+        _lib.check(lib.kda_adamw_plan(at, count, host.data_ptr(), host.numel()), "kda_adamw_plan")
+        parts = lib.kda_adamw_step_workspace_size(at, count) // 8
+        storages = [p.untyped_storage() for p in self.params]
         if self._plan is not None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("parameters were moved since the last step: take one outside the capture first")
             torch.cuda.synchronize(self.device)   # a step may be reading the old plan, on any stream
-        self._plan = plan.to(self.device)
+        plan = host.to(self.device)
+        # all at once, the addresses last: after a failure above the next step comes here again
+        # (while the storages are held no other tensor can come to lie at the same address)
+        self._table, self._plan, self._parts, self._storages = table, plan, parts, storages
         self._home = _raw_stream(self.device.index)
-        self._parts = lib.kda_adamw_step_workspace_size(at, count) // 8
+        self._ptrs = ptrs
 
     def _use(self, stream: int, *more: torch.Tensor) -> None:
         """Launches on ``stream`` read the buffers: if it is not the one they were made on, their

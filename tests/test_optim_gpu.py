@@ -538,3 +538,52 @@ def test_offsets_past_32_bits(states):
     norm = opt.step(1.0)
     exact = 0.5 * (n + 300) ** 0.5
     assert abs(norm.item() - exact) <= 2.0 ** -23 * exact
+
+
+@pytest.mark.parametrize("states", ["fp32", "int8"])
+def test_moved_parameters_in_a_capture(states):
+    """A step in a capture refuses weights that were moved, as often as it is asked; the step outside that it asks
+    for updates the new ones, and the memory that they were moved from stays as it was."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.bfloat16] * len(SIZES), seed=13) for _ in range(2))
+    oa, ob = (FusedAdamW(ps, states=states, master_weights=True) for ps in (a, b))
+    for ps, o in ((a, oa), (b, ob)):
+        _grads(ps, 50)
+        o.step(1.0)
+    old = [p.data for p in a]
+    for p in a:
+        p.data = p.data.clone()
+    kept = [t.clone() for t in old]
+    for ps in (a, b):
+        _grads(ps, 51)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="outside the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                oa.step(1.0)
+    assert oa.steps == 1
+    for k in range(2):
+        for ps, o in ((a, oa), (b, ob)):
+            _grads(ps, 52 + k)
+            o.step(1.0)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and oa.steps == ob.steps
+    assert all(torch.equal(oa.state[k], ob.state[k]) for k in oa.state)
+    assert all(torch.equal(p, q) for p, q in zip(old, kept))
+
+
+def test_a_plan_that_cannot_be_made(monkeypatch):
+    """Whatever fails while the plan of moved weights is made, the next step makes it."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.float32] * len(SIZES), seed=14) for _ in range(2))
+    oa, ob = FusedAdamW(a), FusedAdamW(b)
+    for p in a:
+        p.data = p.data.clone()
+    for ps in (a, b):
+        _grads(ps, 60)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "synchronize", lambda *_: (_ for _ in ()).throw(RuntimeError("no memory")))
+        with pytest.raises(RuntimeError, match="no memory"):
+            oa.step(1.0)
+    oa.step(1.0)
+    ob.step(1.0)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and oa.steps == 1
