@@ -86,6 +86,8 @@ class FusedAdamW:
             at += -(-n // BLOCK) * BLOCK
         self.total = at
         self._state = self._new_state(master_weights) if state is None else self._given_state(state, master_weights)
+        # the streams that the buffers' memory waits for (the one it was allocated on; of given ones that is not known)
+        self._state_streams = {_raw_stream(self.device.index)} if state is None else set()
         # p, g, n, offset, dtype of each parameter
         self._ptrs: List[int] = []
         self._plan: Optional[torch.Tensor] = None
@@ -140,6 +142,8 @@ class FusedAdamW:
         """(m, v) as buffers of values (``views`` gives the parameters' parts): with
         fp32 states the state's own buffers, in another dtype copies."""
         m, v = self._state["m"], self._state["v"]
+        with _on(self.device):
+            self._use()
         if self.states == "fp32":
             return m.to(dtype), v.to(dtype)
         if dtype not in _DTYPE_CODE:
@@ -147,8 +151,6 @@ class FusedAdamW:
         mo = torch.empty(self.total, dtype=dtype, device=self.device)
         vo = torch.empty_like(mo)
         with _on(self.device):
-            if not torch.cuda.is_current_stream_capturing():
-                self._use(_raw_stream(self.device.index))
             _lib.check(_lib.load().kda_adamw_moments(
                 _ptr(m), _ptr(v), _ptr(self._state["m_scale"]), _ptr(self._state["v_scale"]), _ptr(mo), _ptr(vo),
                 self.total, _DTYPE_CODE[dtype], _stream(self.device)), "kda_adamw_moments")
@@ -165,6 +167,8 @@ class FusedAdamW:
             if state[k].dtype != t.dtype or state[k].shape != t.shape:
                 raise ValueError(f"state[{k!r}] is {state[k].dtype} {tuple(state[k].shape)}; expected {t.dtype} "
                                  f"{tuple(t.shape)}")
+        with _on(self.device):
+            self._use()
         for k, t in self._state.items():
             t.copy_(state[k])
         self.steps = int(state["steps"])
@@ -193,16 +197,23 @@ class FusedAdamW:
         # all at once, the addresses last: after a failure above the next step comes here again
         # (while the storages are held no other tensor can come to lie at the same address)
         self._table, self._plan, self._parts, self._storages = table, plan, parts, storages
-        self._home = _raw_stream(self.device.index)
+        self._plan_streams = {_raw_stream(self.device.index)}
         self._ptrs = ptrs
 
-    def _use(self, stream: int, *more: torch.Tensor) -> None:
-        """Launches on ``stream`` read the buffers: if it is not the one they were made on, their
-        memory must not be given away before they have ended, even if the optimizer is dropped."""
-        if stream != self._home:
-            current = torch.cuda.current_stream(self.device)
-            for t in (*self._state.values(), *more):
-                t.record_stream(current)
+    def _use(self) -> bool:
+        """Work on the device's current stream uses the buffers: their memory must not be given away
+        before it has ended, even if the optimizer is dropped.  A stream once recorded stays so.
+        Returns whether the stream is being captured (a graph's user keeps the optimizer)."""
+        if torch.cuda.is_current_stream_capturing():
+            return True
+        stream = _raw_stream(self.device.index)
+        for known, buffers in ((self._state_streams, self._state.values()), (self._plan_streams, (self._plan,))):
+            if stream not in known:
+                current = torch.cuda.current_stream(self.device)
+                for t in buffers:
+                    t.record_stream(current)
+                known.add(stream)
+        return False
 
     def _gradients(self) -> Tuple[List[Optional[torch.Tensor]], List[nn.Parameter]]:
         """Fill the descriptors for a step; returns the gradients, to be kept until the
@@ -249,9 +260,7 @@ class FusedAdamW:
         clip, pc, pw, parts = None, None, None, 0
         with _on(self.device):
             stream = _raw_stream(self.device.index)
-            if not torch.cuda.is_current_stream_capturing():
-                self._use(stream, self._plan)
-            elif not any(t is self._plan for t in self._captured):
+            if self._use() and not any(t is self._plan for t in self._captured):
                 self._captured.append(self._plan)   # the graph reads it at each replay, also after parameters moved
             if max_norm is not None:
                 # the norm and the clip factor; the norm's partial sums (fp64), behind them while they

@@ -587,3 +587,50 @@ def test_a_plan_that_cannot_be_made(monkeypatch):
     oa.step(1.0)
     ob.step(1.0)
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and oa.steps == 1
+
+
+@pytest.mark.parametrize("states", ["fp32", "int8"])
+@pytest.mark.parametrize("how", ["moved", "given", "given-moved", "loaded"])
+def test_optimizer_dropped_behind_work_on_another_stream(how, states):
+    """The same where the weights' plan is made on that stream, where the moments came from a caller who made
+    them on a third one, and behind a state that is being loaded."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.float32] * len(SIZES), seed=15) for _ in range(2))
+    for ps in (a, b):
+        _grads(ps, 70)
+    ref = FusedAdamW(b, states=states)
+    made, stepped = torch.cuda.Stream(), torch.cuda.Stream()
+    if how.startswith("given"):
+        with torch.cuda.stream(made):
+            given = {k: torch.zeros_like(t) for k, t in ref.state.items()}
+        torch.cuda.synchronize()
+        opt = FusedAdamW(a, states=states, state=given)
+        del given
+    else:
+        opt = FusedAdamW(a, states=states)
+    sizes = [t.nbytes for t in (*opt.state.values(), opt._plan)]
+    state = ref.state_dict() if how == "loaded" else None
+    ref.step(1.0)
+    if how.endswith("moved"):
+        for p in a:
+            p.data = p.data.clone()
+    torch.cuda.synchronize()
+    if how == "given":
+        stepped = torch.cuda.default_stream()
+    with torch.cuda.stream(stepped):
+        torch.cuda._sleep(20_000_000)   # some milliseconds (over before the plan of moved weights: it waits)
+        if how == "loaded":
+            opt.load_state_dict({k: t if k == "steps" else t.clone() for k, t in state.items()})
+        else:
+            opt.step(1.0)
+            torch.cuda._sleep(20_000_000)
+            opt.moments(torch.bfloat16)
+    del opt
+    others = []
+    for s in (torch.cuda.default_stream(), made):
+        with torch.cuda.stream(s):
+            others += [torch.full((n,), 1, dtype=torch.uint8, device=DEV) for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(bool((t == 1).all()) for t in others)
+    if how != "loaded":
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
