@@ -41,7 +41,8 @@ def _overlap(spans: List[Tuple[int, int]]) -> bool:
 
 class FusedAdamW:
     """AdamW with moments of their own dtype.  A captured step replays with the learning
-    rate, and the bias corrections, that it was captured with.
+    rate, and the bias corrections, that it was captured with, on the weights' memory of
+    then, which the optimizer keeps; it needs the optimizer and those gradients alive.
 
     ``states``: "fp32" or "int8"; ``master_weights``: keep and update fp32 copies of
     the weights; ``bias_correction``: divide the moments by 1 - beta^step (off in
@@ -91,7 +92,7 @@ class FusedAdamW:
         # p, g, n, offset, dtype of each parameter
         self._ptrs: List[int] = []
         self._plan: Optional[torch.Tensor] = None
-        self._captured: List[torch.Tensor] = []
+        self._captured: List[tuple] = []
         self._table = array("q", [v for n, o, t in zip(self._numels, self.offsets, self._dtypes)
                                   for v in (0, 0, n, o, _DTYPE_CODE[t])])
         self._check_params(list(map(_data_ptr, self.params)))
@@ -260,8 +261,9 @@ class FusedAdamW:
         clip, pc, pw, parts = None, None, None, 0
         with _on(self.device):
             stream = _raw_stream(self.device.index)
-            if self._use() and not any(t is self._plan for t in self._captured):
-                self._captured.append(self._plan)   # the graph reads it at each replay, also after parameters moved
+            if self._use() and not any(kept[0] is self._plan for kept in self._captured):
+                # the graph reads the plan at each replay, and writes the weights that it names, also after they moved
+                self._captured.append((self._plan, self._storages))
             if max_norm is not None:
                 # the norm and the clip factor; the norm's partial sums (fp64), behind them while they
                 # are few, since who keeps the norm keeps what it lies in

@@ -634,3 +634,32 @@ def test_optimizer_dropped_behind_work_on_another_stream(how, states):
     assert all(bool((t == 1).all()) for t in others)
     if how != "loaded":
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_graph_of_a_step_keeps_the_weights_it_writes():
+    """Nobody but the optimizer holds the memory that the weights were moved from: no other tensor comes to lie
+    there, and a replay goes on updating it."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.bfloat16] * len(SIZES), seed=16) for _ in range(2))
+    oa, ob = FusedAdamW(a), FusedAdamW(b)
+    for ps in (a, b):
+        _grads(ps, 80)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        norm = oa.step(0.5)
+    grads = [p.grad for p in a]
+    spans = [(p.data_ptr(), p.nbytes) for p in a]
+    for p in a:
+        p.grad = None
+        p.data = p.data.clone()
+    oa.step()      # the plan is made again; no gradients: nothing moves
+    moved = [p.detach().clone() for p in a]
+    junk = [torch.full((n,), 7, dtype=torch.uint8, device=DEV) for _, n in spans for _ in range(16)]
+    for x, n in ((t.data_ptr(), t.nbytes) for t in junk):
+        assert not any(x < y + m and y < x + n for y, m in spans)
+    for _ in range(3):
+        g.replay()
+        assert torch.equal(norm, ob.step(0.5))
+    assert all(bool((t == 7).all()) for t in junk) and all(torch.equal(p, q) for p, q in zip(a, moved))
+    assert len(grads) == len(a)
