@@ -126,6 +126,11 @@ def _mlp(dim: int, ratio: float, dropout: float) -> nn.Sequential:
     return nn.Sequential(nn.Linear(dim, h), nn.GELU(), nn.Dropout(dropout), nn.Linear(h, dim), nn.Dropout(dropout))
 
 
+def _keeps(m: nn.Module) -> bool:
+    """m, a block's drop_path, returns what it is given, and does nothing else."""
+    return _plain_module(m, nn.Identity) or (_plain_module(m, DropPath) and (m.drop_prob == 0.0 or not m.training))
+
+
 def _mlp_residual(block: nn.Module, x: torch.Tensor) -> torch.Tensor:
     """x + drop_path(mlp(norm2(x))).  With ``block.fused_mlp`` the two maps run as
     ``mlp`` where that computes the same: plain modules with biases, no dropout, one
@@ -145,9 +150,9 @@ def _mlp_residual(block: nn.Module, x: torch.Tensor) -> torch.Tensor:
             and seq[0].bias is not None and seq[3].bias is not None):
         return x + block.drop_path(seq(h))
     params = seq[0].weight, seq[0].bias, seq[3].weight, seq[3].bias
-    if x.dtype != h.dtype or (isinstance(block.drop_path, DropPath) and block.training):
-        return x + block.drop_path(mlp(h, *params))
-    return mlp(h, *params, residual=x)
+    if x.dtype == h.dtype and _keeps(block.drop_path):
+        return mlp(h, *params, residual=x)
+    return x + block.drop_path(mlp(h, *params))
 
 
 class NoPEViTBlock(nn.Module):

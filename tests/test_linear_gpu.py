@@ -427,3 +427,43 @@ def test_offsets_past_32_bits(dtype):
         want, size = dz.t() @ x.double(), dz.abs().t() @ x.double().abs()
         tol = (2 * M + 16) * 2.0 ** -24 * size + torch.finfo(dt).eps * (size + want.abs())
         assert ((dw[-8:].double() - want).abs() <= tol).all()
+
+
+class _Scale(torch.nn.Identity):
+    def forward(self, x):
+        return 0.5 * x
+
+
+def _drop_paths():
+    """What a block's drop_path may be, by name, as it comes out of ``block.eval()``."""
+    from mlx_vit_amd.model import DropPath
+    train = DropPath(0.5)
+    hooked, own = torch.nn.Identity(), DropPath(0.3)
+    hooked.register_forward_hook(lambda m, args, out: 0.25 * out)
+    own.forward = lambda x: 2 * x
+    return {"identity": torch.nn.Identity(), "evaluated": DropPath(0.5), "training": train, "a scale": _Scale(),
+            "a linear map": torch.nn.Linear(64, 64), "hooked": hooked, "its own forward": own, "never": DropPath(0.0)}
+
+
+@pytest.mark.parametrize("name", list(_drop_paths()))
+@pytest.mark.parametrize("kind", ["NoPEViTBlock", "HybridBlock"])
+def test_blocks_mlp_and_what_follows_it(kind, name):
+    """A block's drop_path sees the MLP's result with ``set_fused_mlp`` as without: stochastic depth that is on in an
+    evaluated block, another module in its place, hooks.  Tolerances as in test_blocks_mlp_as_one_operator."""
+    from mlx_vit_amd import model as M
+    torch.manual_seed(0)
+    blk = M.NoPEViTBlock(64, 2) if kind == "NoPEViTBlock" else M.HybridBlock(64, 2, "nope")
+    blk.drop_path = _drop_paths()[name]
+    blk = blk.to(DEV).eval()
+    if name in ("training", "never"):
+        blk.drop_path.train()
+    x = _mk(1, 16, 10, 64, dt=torch.float32)
+    outs = []
+    for on in (False, True):
+        M.set_fused_mlp(blk, on)
+        torch.manual_seed(1)
+        y = blk(x)
+        outs.append(y if kind == "NoPEViTBlock" else y[0])
+    a, b = (o.detach().double() for o in outs)
+    for i in range(16):
+        assert (a[i] - b[i]).norm() <= 8 * torch.finfo(torch.float32).eps * a[i].norm(), i
