@@ -134,12 +134,13 @@ def _keeps(m: nn.Module) -> bool:
 def _mlp_residual(block: nn.Module, x: torch.Tensor) -> torch.Tensor:
     """x + drop_path(mlp(norm2(x))).  With ``block.fused_mlp`` the two maps run as
     ``mlp`` where that computes the same: plain modules with biases, no dropout, one
-    dtype, on a ROCm device, outside autocast and tracing."""
+    dtype, on a ROCm device, outside autocast, tracing and torch.func's transforms."""
     h = block.norm2(x)
     seq = block.mlp
     if not (block.fused_mlp and type(seq) is nn.Sequential and len(seq) == 5 and h.device.type == "cuda"
             and h.dtype in (torch.bfloat16, torch.float32) and not torch.is_autocast_enabled("cuda")
             and not torch.compiler.is_compiling() and not torch._C._is_tracing()
+            and type(h) is torch.Tensor and torch._C._functorch.peek_interpreter_stack() is None
             and forward_ad._current_level < 0 and not (_nn_module._global_forward_hooks or _nn_module._global_forward_pre_hooks
                                                        or _nn_module._global_backward_hooks
                                                        or _nn_module._global_backward_pre_hooks)
@@ -391,7 +392,8 @@ def to_bf16(model: nn.Module, keep_fp32: Tuple[str, ...] = BF16_KEEP_FP32) -> nn
 def set_fused_mlp(model: nn.Module, on: bool = True) -> nn.Module:
     """Run the MLP of every block of ``model`` as ``linear.mlp`` (off by default: the
     results differ from the separate modules' in the rounding of the value before
-    the activation and of the residual's sum).  In place; returns the model."""
+    the activation and of the residual's sum, and ``mlp`` has no second derivative).  In
+    place; returns the model."""
     for m in model.modules():
         if isinstance(m, (NoPEViTBlock, HybridBlock)):
             m.fused_mlp = on

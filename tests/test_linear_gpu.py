@@ -467,3 +467,34 @@ def test_blocks_mlp_and_what_follows_it(kind, name):
     a, b = (o.detach().double() for o in outs)
     for i in range(16):
         assert (a[i] - b[i]).norm() <= 8 * torch.finfo(torch.float32).eps * a[i].norm(), i
+
+
+class _NoAttention(torch.nn.Module):
+    """(The library's attention has no second derivative of its own.)"""
+
+    def forward(self, x, mask=None):
+        return torch.sin(x)
+
+
+def test_blocks_mlp_under_transforms():
+    """torch.func's transforms take the modules: one block over several inputs, per-sample gradients, a Hessian."""
+    from mlx_vit_amd import model as M
+    torch.manual_seed(0)
+    blk = M.NoPEViTBlock(16, 2).to(DEV).eval()
+    blk.attn = _NoAttention()
+    x = _mk(1, 3, 2, 5, 16, dt=torch.float32)
+    outs = []
+    for on in (False, True):
+        M.set_fused_mlp(blk, on)
+        outs.append((torch.func.vmap(blk)(x), torch.func.vmap(torch.func.grad(lambda t: blk(t).square().sum()))(x),
+                     torch.func.vjp(blk, x[0])[1](x[1])[0],
+                     torch.func.hessian(lambda t: blk(t[None, None]).square().sum())(x[0, 0, 0])))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    calls = []
+    real, M.mlp = M.mlp, lambda *a, **k: calls.append(1) or real(*a, **k)
+    try:
+        blk(x[0])
+        assert calls == [1]
+    finally:
+        M.mlp = real
