@@ -161,8 +161,13 @@ __device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, const
     uint32_t top_m = 0, top_v = 0;
     float r[8];
 #pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] *= c;
+    if (left < 8)   // what lies past the tensor stays zero, whatever c is
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e >= left) g[e] = 0.f;
+#pragma unroll
     for (int e = 0; e < 8; ++e) {
-        g[e] *= c;
         m[e] = a.b1 * m[e] + a.omb1 * g[e];
         v[e] = a.b2 * v[e] + a.omb2 * g[e] * g[e];
         r[e] = __builtin_amdgcn_sqrtf(v[e]);
@@ -174,7 +179,13 @@ __device__ __forceinline__ void update(const StepArgs& a, const Tensor& t, const
         }
     }
     st8<T>(p, left, vec, w);
-    if constexpr (MASTER) st8<float>(a.master + at, 8, true, w);
+    if constexpr (MASTER) {
+        if (left < 8)   // (with eps 0: there 0 / 0)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e >= left) w[e] = 0.f;
+        st8<float>(a.master + at, 8, true, w);
+    }
     if constexpr (SMALL) {
         top_m = max32(top_m);
         top_v = max32(top_v);

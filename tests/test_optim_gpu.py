@@ -663,3 +663,29 @@ def test_graph_of_a_step_keeps_the_weights_it_writes():
         assert torch.equal(norm, ob.step(0.5))
     assert all(bool((t == 7).all()) for t in junk) and all(torch.equal(p, q) for p, q in zip(a, moved))
     assert len(grads) == len(a)
+
+
+@pytest.mark.parametrize("master", [False, True])
+@pytest.mark.parametrize("states", ["fp32", "int8"])
+@pytest.mark.parametrize("how", ["eps 0", "no factor", "infinite"])
+def test_what_lies_between_the_weights_stays_zero(how, states, master):
+    """With eps = 0 (0 / 0 there), with a clip factor that is NaN, with gradients that are infinite: whatever becomes
+    of the weights, the buffers are zero between them, and load as a state does."""
+    from mlx_vit_amd import FusedAdamW
+    params = _params(SIZES, [torch.bfloat16] * len(SIZES), seed=17)
+    opt = FusedAdamW(params, states=states, master_weights=master, eps=0.0 if how == "eps 0" else 1e-8)
+    for k in range(2):
+        _grads(params, 90 + k)
+        if how != "eps 0":
+            for p in params:
+                p.grad.view(-1)[-1] = float("nan" if how == "no factor" else "inf")
+        opt.step(1.0 if how == "no factor" else None)
+    between = torch.ones(opt.total, dtype=torch.bool, device=DEV)
+    for v in opt.views(between):
+        v.fill_(False)
+    assert between.any()
+    for name in ("m", "v", "master"):
+        if name in opt.state:
+            assert not opt.state[name][between].any(), name
+    if how == "eps 0":
+        assert all(p.isfinite().all() for p in params)
