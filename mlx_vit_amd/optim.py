@@ -249,10 +249,9 @@ class FusedAdamW:
         if max_norm is not None and not max_norm > 0.0:
             raise ValueError(f"max_norm={max_norm}: expected a positive number or None")
         gs, updated = self._gradients()   # (gs: alive until the launches)
-        self.steps += 1
         b1, b2 = self.betas
-        c1 = 1.0 / (1.0 - b1 ** self.steps) if self.bias_correction else 1.0
-        c2 = 1.0 / (1.0 - b2 ** self.steps) if self.bias_correction else 1.0
+        c1 = 1.0 / (1.0 - b1 ** (self.steps + 1)) if self.bias_correction else 1.0
+        c2 = 1.0 / (1.0 - b2 ** (self.steps + 1)) if self.bias_correction else 1.0
         lib, at, count = _lib.load(), self._table.buffer_info()[0], len(self.params)
         plan = self._plan.data_ptr()
         get = self._state.get
@@ -278,6 +277,7 @@ class FusedAdamW:
                                     self.eps, self.weight_decay, c1, c2, pw, 8 * parts, stream)
             if rc:
                 _lib.check(rc, "kda_adamw_step")
+        self.steps += 1
         # a graph that holds the weights as they were has to notice
         _increment_version(updated)
         return None if clip is None else clip[0]

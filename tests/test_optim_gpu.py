@@ -689,3 +689,26 @@ def test_what_lies_between_the_weights_stays_zero(how, states, master):
             assert not opt.state[name][between].any(), name
     if how == "eps 0":
         assert all(p.isfinite().all() for p in params)
+
+
+@pytest.mark.parametrize("max_norm", [None, 1.0])
+def test_a_step_that_fails_does_not_count(max_norm, monkeypatch):
+    """No memory for the norm, a rate that the library refuses: the next step is the one that failed."""
+    from mlx_vit_amd import FusedAdamW
+    a, b = (_params(SIZES, [torch.float32] * len(SIZES), seed=18) for _ in range(2))
+    oa, ob = (FusedAdamW(ps, bias_correction=True) for ps in (a, b))
+    for ps in (a, b):
+        _grads(ps, 95)
+    if max_norm is not None:
+        with monkeypatch.context() as m:
+            m.setattr(torch, "empty", lambda *a, **k: (_ for _ in ()).throw(RuntimeError("no memory")))
+            with pytest.raises(RuntimeError, match="no memory"):
+                oa.step(max_norm)
+    betas, oa.betas = oa.betas, (1.5, 0.95)
+    with pytest.raises((RuntimeError, ValueError)):
+        oa.step(max_norm)
+    oa.betas = betas
+    assert oa.steps == 0
+    oa.step(max_norm)
+    ob.step(max_norm)
+    assert oa.steps == 1 and all(torch.equal(p, q) for p, q in zip(a, b))
