@@ -54,8 +54,8 @@ class FusedAdamW:
     With ``master_weights`` a weight that is changed other than by ``step`` gets its
     master's value back at the next one.
 
-    Parameters are contiguous fp32 or bf16 tensors on one ROCm device; those
-    without a gradient at a step are left out of it."""
+    Parameters are contiguous fp32 or bf16 tensors on one ROCm device, and stay so;
+    gradients have their dtype.  Those without a gradient at a step are left out of it."""
 
     def __init__(self, params: Iterable[nn.Parameter], lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8,
                  weight_decay: float = 0.05, states: str = "fp32", master_weights: bool = False,
@@ -181,6 +181,9 @@ class FusedAdamW:
             if p.dtype != t or p.numel() != n or not p.is_contiguous() or p.device != self.device:
                 raise ValueError(f"a parameter of {n} elements of {t} is now {tuple(p.shape)}, {p.dtype}, strides "
                                  f"{p.stride()} on {p.device}: make a new optimizer")
+            # (a step looks at the gradients' sizes in bytes: half precision's are bf16's)
+            if getattr(p, "grad_dtype", t) != t:
+                raise ValueError(f"a parameter of {t} takes gradients of grad_dtype={p.grad_dtype}: expected its own dtype")
         if _overlap([(a, p.nbytes) for a, p in zip(ptrs, self.params)]):
             raise ValueError("parameters overlap in memory (one of them is given twice, or two share a storage)")
         if self._plan is not None and torch.cuda.is_current_stream_capturing():

@@ -712,3 +712,27 @@ def test_a_step_that_fails_does_not_count(max_norm, monkeypatch):
     oa.step(max_norm)
     ob.step(max_norm)
     assert oa.steps == 1 and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, None], ids=["half", "any"])
+def test_gradients_of_another_dtype_are_refused(dtype):
+    """Half precision's bytes would be read as bf16's."""
+    from mlx_vit_amd import FusedAdamW
+    (p,) = _params([(300,)], [torch.bfloat16], seed=19)
+    if not hasattr(p, "grad_dtype"):
+        pytest.skip("this torch lets no gradient have another dtype")
+    p.grad_dtype = dtype
+    with pytest.raises(ValueError, match="grad_dtype"):
+        FusedAdamW([p])
+    p.grad_dtype = torch.bfloat16
+    opt = FusedAdamW([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    p.grad = None
+    p.grad_dtype = dtype
+    p.data = p.data.clone()
+    p.grad = torch.ones(300, dtype=torch.float16, device=DEV)
+    w = p.detach().clone()
+    with pytest.raises(ValueError, match="grad_dtype"):
+        opt.step()
+    assert torch.equal(p, w)
