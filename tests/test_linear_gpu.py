@@ -498,3 +498,32 @@ def test_blocks_mlp_under_transforms():
         assert calls == [1]
     finally:
         M.mlp = real
+
+
+# M, K, hidden, outputs: outputs that are no multiple of 8 (dy is copied), few from many columns and the reverse, one,
+# and two whose first map's gradient takes tiles of 256 x 256 by one of the widths and smaller ones by the other
+OTHER_WIDTHS = [(131, 300, 520, 7), (70, 8, 72, 513), (257, 33, 64, 1), (1, 24, 40, 130), (9, 130, 96, 600),
+                (300, 96, 384, 200), (64, 1000, 24, 16), (6200, 24, 2560, 640), (6200, 640, 2560, 24)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("size", OTHER_WIDTHS, ids=str)
+def test_mlp_of_other_output_width(size, dtype):
+    from mlx_vit_amd import mlp
+    M, K, N, O = size
+    i, dt = OTHER_WIDTHS.index(size), DT[dtype]
+    for act, bias, res in (("gelu", True, i % 2 == 0), ("silu", i % 2 == 1, True), (None, True, False))[:1 if M > 6000 else 3]:
+        print(size, dtype, act, bias, res, flush=True)
+        x, w1, b1, _, _ = _inputs(M, K, N, dt, bias, False, seed=400 + 10 * i)
+        _, w2, b2, r, dy = _inputs(M, N, O, dt, True, res, seed=600 + 10 * i)
+        want = L.mlp(x, w1, b1, w2, b2, r, act, dy)
+        with torch.no_grad():
+            plain = mlp(x, w1, b1, w2, b2, r, act)
+        leaves = _leaves(x, w1, b1, w2, b2, r)
+        y = mlp(x, w1, b1, w2, b2, r, act)
+        assert y.shape == (M, O) and torch.equal(y, plain)
+        L.check("y", y, want["y"])
+        names = ["dx", "dw1"] + ["db1"] * (b1 is not None) + ["dw2", "db2"] + ["dr"] * (r is not None)
+        for n, g, leaf in zip(names, torch.autograd.grad(y, leaves, dy), leaves):
+            assert g.shape == leaf.shape
+            L.check(n, g, want[n])
