@@ -527,3 +527,32 @@ def test_mlp_of_other_output_width(size, dtype):
         for n, g, leaf in zip(names, torch.autograd.grad(y, leaves, dy), leaves):
             assert g.shape == leaf.shape
             L.check(n, g, want[n])
+
+
+def test_blocks_mlp_with_frozen_weights(monkeypatch):
+    """Where a bias is trained and its weight is not, the modules run: no weight's gradient is formed in vain."""
+    from mlx_vit_amd import model as M
+    torch.manual_seed(0)
+    blk = M.NoPEViTBlock(64, 2).to(DEV)
+    M.set_fused_mlp(blk)
+    x = _mk(1, 2, 50, 64, dt=torch.float32)
+    calls = []
+    real = M.mlp
+    monkeypatch.setattr(M, "mlp", lambda *a, **k: calls.append(1) or real(*a, **k))
+    for frozen, fused in (((), True), ((0, 3), False), ((0,), False), ((3,), False)):
+        blk.requires_grad_(True)
+        for i in frozen:
+            blk.mlp[i].weight.requires_grad_(False)
+        blk.zero_grad()
+        calls.clear()
+        blk(x).square().sum().backward()
+        assert bool(calls) == fused
+        assert all((p.grad is not None) == p.requires_grad for p in blk.mlp.parameters())
+        with torch.no_grad():
+            calls.clear()
+            blk(x)
+            assert calls
+    blk.mlp.requires_grad_(False)
+    calls.clear()
+    blk(x).square().sum().backward()
+    assert calls
