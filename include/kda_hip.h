@@ -329,8 +329,10 @@ int kda_log_decay_bwd(const void* alpha, const float* dg, void* dalpha, int64_t 
  * for m < M, n < N, k < K; z (may be NULL) receives the value before act, which
  * the backward pass reads: fp32, or fp16 beside bf16 (infinite past its range).
  * act: 0 none, 1 gelu (z Phi(z)), 2 silu.  The others are of dtype; sums, epilogue
- * and activation in fp32.  Matrices are rows of ld_* elements (at most 2^21), unit
- * column stride.  bf16 with ceil(M / 16) ceil(N / 16)
+ * and activation in fp32 (of bf16's gelu within 1e-5 of its value).  An infinite fp32
+ * operand gives NaN where fp32 arithmetic may give an infinity, except in a forward of
+ * ceil(M / 16) ceil(N / 16) up to 1024 (2048 where M <= 8).  Matrices are rows of ld_*
+ * elements (at most 2^21), unit column stride.  bf16 with ceil(M / 16) ceil(N / 16)
  * above 256 (above 512 where M <= 8): x and w 16-byte aligned, ld_x and ld_w
  * multiples of 8 that cover K rounded up to 8, and that many elements of the last
  * row readable; other operands and smaller or fp32 ones: any stride, aligned to
@@ -373,8 +375,8 @@ int kda_mlp_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, cons
  * gradients g (n elements each, contiguous, of dtype) and where its moments
  * begin, `offset` elements (a multiple of 256) into the moments' buffers.  Those
  * buffers hold whole blocks of 256 elements: a tensor owns n rounded up to 256
- * of them, and those past n are written as zeros (from zeros).  Tensors must
- * not overlap.  g NULL: the tensor is left out of the call. */
+ * of them, and those past n are written as zeros (from zeros, whatever the gradients
+ * are).  Tensors must not overlap.  g NULL: the tensor is left out of the call. */
 typedef struct kda_adamw_tensor {
     void* p;
     const void* g;
@@ -397,8 +399,9 @@ int kda_adamw_plan(const kda_adamw_tensor* tensors, int count, void* host_plan, 
  * rounding.  states 0: m, v fp32.  states 1: 8 bits, one scale for 256 elements:
  *   m int8,  value m_scale (k / 127) |k / 127|, m_scale the block's largest |m|;
  *   v uint8, value (v_scale (k / 255)^2)^2, v_scale the block's largest sqrt(v),
- *   k >= 1 where v > 0; the codes are those of fp32 arithmetic rounded operation by
- *   operation.
+ *   k >= 1 where v > 0; values and codes are those of fp32 arithmetic rounded operation
+ *   by operation, k / 127 and k / 255 products with the fp32 numbers next to 1 / 127 and
+ *   1 / 255 (a quotient is up to one step of fp32 off them).
  * m, v, master 16-byte aligned. */
 #define KDA_ADAMW_F32 0
 #define KDA_ADAMW_INT8 1

@@ -120,7 +120,8 @@ __device__ __forceinline__ uint32_t max32(uint32_t x) {
 
 constexpr uint32_t MIN_NORMAL = 0x00800000u;
 
-// m and v from their codes, each operation rounded as written
+// m and v from their codes, each operation rounded as written (a product with the rounded
+// reciprocal: a quotient would differ by a step of fp32 at most)
 __device__ __forceinline__ void decode8(const uint2& km, const uint2& kv, float sm, float sv, float (&m)[8], float (&v)[8]) {
 #pragma clang fp contract(off)
 #pragma unroll

@@ -14,10 +14,10 @@
 // allows), the rows' bytes where K or N is a few hundred (the 25088 x 1536 hidden layer of a block: 77 MB, 15 us a pass at a
 // copy's 5.1 TB/s), the epilogue's instructions beside them, and a load's latency
 // where there are fewer tiles than CUs.  Measured (forward, bias and activation
-// within): 16384 x 2048 -> 8192 gelu 483 us, 1138 TFLOP/s (without activation 450; the
-// library's bare product 371); 25088 x 384 -> 1536 gelu 53 us and 1536 -> 384 with the
-// residual 38 (the library's bare products 56 and 33); 196 x 384 -> 1536 4.6 us; 1 x 384 ->
-// 174 3.4 us.
+// within, twenty in a graph): 16384 x 2048 -> 8192 gelu 495 us, 1111 TFLOP/s (without
+// activation 453; the library's bare product 373); 25088 x 384 -> 1536 gelu 55 us and
+// 1536 -> 384 with the residual 39 (the library's bare products 56 and 32); 196 x 384 ->
+// 1536 4.5 us; 1 x 384 -> 174 3.2 us.
 #include "kda_hip.h"
 #include "kda_internal.h"
 
@@ -562,7 +562,8 @@ __global__ __launch_bounds__(64 * WR * WC, WPE) void kda_linear_bf16_kernel(cons
 
 // x = h + m + l, each the next 8 bits of x's 24 (truncation, so nothing
 // overflows and every difference is exact); the four values' parts packed.
-// An infinite x gives a NaN part.
+// An infinite x gives a NaN part: its products are NaN where fp32 arithmetic (and a
+// forward in pieces of 16 x 16, see few) may have an infinity.
 // flip: the sign bit to change in each.
 __device__ __forceinline__ void split3(const float4& x, uint32_t flip, uint2& h, uint2& m, uint2& l) {
     const uint32_t v[4] = {__float_as_uint(x.x) ^ flip, __float_as_uint(x.y) ^ flip, __float_as_uint(x.z) ^ flip,
@@ -636,8 +637,8 @@ struct Stage32 {
 //
 // Six bf16 products for one: at 1634 TFLOP/s of those no more than 272 of fp32's,
 // where the library's fp32 products reach 154 at 8192^3 and 85 at 6272 x 384 <-> 1536.
-// Here 6272 x 384 -> 1536 takes 52 us (142 TFLOP/s), 4096^3 684 (201; the library
-// 913).  What bounds it is the way to LDS: each value is loaded, split (nine
+// Here 6272 x 384 -> 1536 with gelu takes 50 us (147 TFLOP/s), 4096^3 617 (223; the
+// library 911).  What bounds it is the way to LDS: each value is loaded, split (nine
 // instructions) and stored once a tile, in one buffer, the next step's loads in
 // flight over the products.
 template <int BM, int BN, int WR, int WC, bool AT, bool BT, int ACT, bool DG, bool PART>
@@ -970,8 +971,8 @@ hipError_t launch_tiles(GemmArgs& a, hipStream_t st) {
 //   16384 x 8192, K 2048              503         526       740
 //   25088 x  384, K 1536               38          41        47
 //   12544 x  768, K 768                22          25        26   (147 of the largest)
-//   25088 x 1536, K 384, gelu          60          54        61
-//   the same, times gelu'(z)           62          57        65
+//   25088 x 1536, K 384, gelu          64          55        64
+//   the same, times gelu'(z)           72          59        64
 //    4096 x 1024, K 1024               25          11        14
 //    2048 x 2048, K 512                16           8.0       9.3
 //    2048 x 1024, K 1024               24          10         7.8

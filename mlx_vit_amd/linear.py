@@ -11,12 +11,16 @@ and ``mlp`` two of them, the reference's block MLP with its skip connection
 
 One kernel forms a product and its epilogue; the backward pass applies the
 activation's derivative in the epilogue of the product that needs it, and forms
-weight and bias gradients in one launch.  Sums, epilogues and activations are
-fp32; each tensor that is stored (y, and for the backward pass the hidden layer) is
-rounded once to the inputs' dtype, bf16 or fp32, the value before the activation to
-fp16 where that is bf16.  fp32 products split each operand exactly into three bf16 parts and
-keep what is at least 2^-16 of the largest product, fp32's own accuracy; an
-infinite fp32 operand gives NaN where fp32 arithmetic may give an infinity.
+weight and bias gradients in one launch.  Sums and epilogues are fp32, and so are
+activations: of fp32 results to its own accuracy, of bf16's gelu within 1e-5 of its
+value.  Each tensor that is stored is rounded once, y and the hidden layer to the
+inputs' dtype, bf16 or fp32; what the backward pass reads again too: the value before
+the activation to fp16 where that is bf16, its gradient to bf16, the operand of the
+next products.  So bf16 gradients are off by two roundings, 2^1/2 of one.  fp32
+products split each operand exactly into three bf16 parts and keep what is at least
+2^-16 of the largest product, fp32's own accuracy; there an infinite operand gives
+NaN where fp32 arithmetic may give an infinity, which forwards of at most 1024 pieces
+of 16 x 16 (2048 up to 8 rows), formed otherwise, do give.
 
 Differentiable in every tensor; a second derivative and tracing are refused.  There
 is no CPU path.  A backward pass is captured into a graph as torch's own nodes are:

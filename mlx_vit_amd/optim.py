@@ -10,9 +10,10 @@ scale for each 256 elements, and on request an fp32 copy of the weights
 half a bf16 step add up.
 
 8-bit moments: m = s (k / 127) |k / 127|, k in [-127, 127], s the block's largest
-|m|; v = (s (k / 255)^2)^2, k in [0, 255], s the block's largest sqrt(v).  The
-update uses the new moments before they are rounded.  A gradient that is not
-finite makes its whole block of 8-bit moments NaN.
+|m|; v = (s (k / 255)^2)^2, k in [0, 255], s the block's largest sqrt(v); k / 127 and
+k / 255 are products with the fp32 numbers next to 1 / 127 and 1 / 255.  The update
+uses the new moments before they are rounded.  A gradient that is not finite makes its
+whole block of 8-bit moments NaN.
 """
 from __future__ import annotations
 
