@@ -414,6 +414,83 @@ int kda_adamw_step(const kda_adamw_tensor* tensors, int count, const void* plan,
 int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale,
                       void* m_out, void* v_out, int64_t n, int dtype, void* stream);
 
+/* Linear attention with a decay for each head (no counterpart in the reference; the
+ * recurrence of its GDN without the delta rule, nope_gdn_mlx.py:641-650):
+ *   S_t = e^{g_t} S_{t-1} + v_t k_t^T,   o_t = S_t q_t
+ * for H heads of D = 32, 64, 96 or 128 channels, S [H][D][D] fp32 as S[i_v][j_k].
+ * q, k, v, dout: [B][T][heads][D] of dtype (fp32 or bf16), strides in elements, unit
+ * channel stride, pointers and strides whole 16-byte pieces; q, k and v may have
+ * fewer heads than H, which each serve H / heads heads of the state in a row (dout: H).
+ * g: fp32 log-decays with strides of their own (0: shared); below -200 as -200, whose
+ * e^g is zero.  s0, s_final, ds_final, ds0 [sequences][H][D][D] fp32, each may be NULL.
+ * cu (device memory, may be NULL): nseq + 1 limits of sequences that lie in one row
+ * (B = 1) one behind the other; each limit counts as at least the one before and
+ * as within [0, T]; rows of no sequence get zeros.
+ * o [B][T][H][D], dq, dk, dv contiguous [B][T][their heads][D], of dtype; dg fp32: [B][T][H],
+ * or with dg_heads != 0 [H], the sum over all tokens; NULL: not wanted.
+ * Sums and states are fp32; in bf16 the pairs' weights and the state enter the products
+ * with 16 bits of mantissa.  What a token gets from itself alone (T = 1, no s0) has a dg
+ * of exactly zero.  A value that is not finite reaches every output of its sequence from its
+ * block of 64 tokens on (in a gradient: up to it).
+ * Backward: gradients of <o, dout> + <s_final, ds_final>; reads s_final only for dg
+ * beside ds_final.  Nothing else is kept between the calls.  workspace: at least
+ * kda_decay_workspace_size(KDA_PASS_FWD or KDA_PASS_BWD, args) bytes for these sizes, heads, cu,
+ * nseq, dtype, dg and dg_heads, 16-byte aligned.  Results do not depend on how the
+ * sequence is shared out beyond rounding, and are the same from call to call. */
+typedef struct kda_decay_rows {
+    const void* p;
+    int64_t batch, token, head, heads;
+} kda_decay_rows;
+typedef struct kda_decay_args {
+    kda_decay_rows q, k, v, dout;
+    const float* g;
+    int64_t g_batch, g_token, g_head;
+    const float* s0;
+    const int32_t* cu;
+    int64_t nseq;
+    void* o;
+    float* s_final;
+    const float* ds_final;
+    void *dq, *dk, *dv;
+    float* dg;
+    int64_t dg_heads;
+    float* ds0;
+    int64_t B, T, H, D, dtype;
+    void* workspace;
+    int64_t ws_bytes;
+} kda_decay_args;
+size_t kda_decay_workspace_size(int pass, const kda_decay_args* args);
+int kda_decay_fwd(const kda_decay_args* args, void* stream);
+int kda_decay_bwd(const kda_decay_args* args, void* stream);
+/* One token of each of B rows (T = 1), on states that stay where they are: s0 [states]
+ * [H][D][D] is read and written, o [B][H][D] written; q, k, v: batch and head strides.
+ * slots (device memory, may be NULL: row b's state is b, states = B): the state of each
+ * row.  A row whose slot is not in [0, states) is left out, its o zero; rows of one slot
+ * follow each other in their order.  No workspace. */
+int kda_decay_step(const kda_decay_args* args, const int32_t* slots, int64_t states, void* stream);
+
+/* Rotary positions on up to KDA_ROTARY_AXES axes: of each row of D channels (even, at most
+ * 256) axis a has the next sections[a] (even) and turns their pair i by sign times the angle
+ * position_a 2 pi turns[...], the pairs numbered through all axes; channels behind
+ * the last axis are copied.  Pairs of an axis: (i, sections[a] / 2 + i), or with
+ * interleaved (2 i, 2 i + 1).  Angles are formed in fp64, rows in fp32.  turns: host memory,
+ * one for every pair.  Positions: of type 0 int32, 1 int64 or 2 fp32 with strides (axis,
+ * batch, token), or NULL: axes 0 to 2 are n / (grid_h grid_w), n / grid_w mod grid_h and n mod
+ * grid_w of n = start + token.  q and k (k.p NULL: none): as kda_decay's operands, of any alignment
+ * to their element; q_out, k_out contiguous [B][T][heads][D]. */
+#define KDA_ROTARY_AXES 4
+typedef struct kda_rotary_args {
+    kda_decay_rows q, k;
+    void *q_out, *k_out;
+    const void* positions;
+    int64_t type, axis, batch, token;
+    int64_t grid_h, grid_w, start;
+    int64_t axes, sections[KDA_ROTARY_AXES];
+    const double* turns;
+    int64_t interleaved, sign, B, T, D, dtype;
+} kda_rotary_args;
+int kda_rotary(const kda_rotary_args* args, void* stream);
+
 #define KDA_LAYER_PRODUCER 0
 #define KDA_LAYER_RMSNORM 1
 size_t kda_layer_workspace_size(int which, int B, int T, int H, int D);

@@ -71,6 +71,11 @@ SIGNATURES = {
     "kda_adamw_step_workspace_size": ([_P, _I], _Z),
     "kda_adamw_step": ([_P, _I, _P, _I] + [_P] * 5 + [_D, _P] + [_D] * 7 + [_P, _Z, _P], _I),
     "kda_adamw_moments": ([_P] * 6 + [_L, _I, _P], _I),
+    "kda_decay_workspace_size": ([_I, _P], _Z),
+    "kda_decay_fwd": ([_P, _P], _I),
+    "kda_decay_bwd": ([_P, _P], _I),
+    "kda_decay_step": ([_P, _P, _L, _P], _I),
+    "kda_rotary": ([_P, _P], _I),
     "kda_layer_workspace_size": ([_I] * 5, _Z),
     "kda_profile_enable": ([_I], _I),
     "kda_profile_name": ([_I], ctypes.c_char_p),

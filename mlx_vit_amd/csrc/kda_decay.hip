@@ -1,0 +1,1367 @@
+// kda_decay.hip -- linear attention with a decay for each head: the forward and backward
+// passes over whole sequences, one token's step, and the C ABI around them.
+//
+//   S_t = e^{g_t} S_{t-1} + v_t k_t^T,   o_t = S_t q_t        (S[i_v][j_k], fp32)
+//
+// A sequence is worked through in chunks of C tokens with the state in registers.
+// With G_t the sum of g over the chunk up to t,
+//   o_t = e^{G_t} S q_t + sum_{s <= t} e^{G_t - G_s} (q_t . k_s) v_s
+//   S'  = e^{G_C} S + sum_s e^{G_C - G_s} v_s k_s^T
+// so a chunk is four products of the matrix unit.  All of the backward pass is the
+// same form again.  With (X, Y, W) in the places of (q, k, v):
+//   dq  (do, v, k), the state transposed;
+//   dk  (v, do, q) and dv (k, q, do), backwards in time with the decay of the token
+//       behind, the state then being dS, the adjoint of S;
+//   dg_t = <S_T, dS_T> + sum_{s >= t} (q_s . dq_s - k_s . dk_s),
+// which is what reaches tokens from t on from before t.
+#include "kda_hip.h"
+#include "kda_internal.h"
+
+namespace kda {
+
+namespace {
+
+// One operand [batch][token][head][D]: strides in elements, `share` heads of the
+// state to one of its own
+struct Rows {
+    const void* p;
+    int64_t batch, token, head;
+    int share;
+};
+
+// A run of tokens that one workgroup takes through in order
+struct Slot {
+    int tok0, n, seq;   // seq -1: tokens of no sequence, -2: nothing
+    int first, last;    // of its sequence
+};
+
+struct DecayArgs {
+    Rows x, y, w, z;            // z: the fourth operand (mix: q beside dq; mix2: see there)
+    const float* g;
+    int64_t gb, gt, gh;
+    void *out, *out2;           // [B][T][H][D]
+    const float* s_in;          // the state that a slot starts from, by slot or by sequence
+    float* s_out;               // and ends with: by slot (states), by sequence (else); may be null
+    float *dots, *dots2;        // [H][B T]
+    float* anchors;             // [slot][H][its chunks]
+    float* seg;                 // states: e^{sum of g} of each slot and head
+    const int4* tab;            // packed: the slots
+    int in_by_slot;
+    int B, T, H, nseq, nslots, per_seq, seg_tokens;
+};
+
+__device__ __forceinline__ Slot slot_of(const DecayArgs& a, int j) {
+    Slot s;
+    if (a.tab) {
+        const int4 t = a.tab[j];
+        s.tok0 = t.x; s.n = t.y; s.seq = t.z; s.first = t.w & 1; s.last = (t.w >> 1) & 1;
+    } else {
+        s.seq = j / a.per_seq;
+        const int i = j - s.seq * a.per_seq;
+        s.tok0 = i * a.seg_tokens;
+        s.n = min(a.seg_tokens, a.T - s.tok0);
+        s.first = i == 0;
+        s.last = i == a.per_seq - 1;
+    }
+    return s;
+}
+
+// Products of two operands given as sums of bf16 planes, down to 2^-16 of the
+// largest, the smallest first
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mmp(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 c) {
+#pragma unroll
+    for (int s = 2; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
+    return c;
+}
+
+// eight fp32 values as N bf16 planes: with three, exactly
+template <int N>
+__device__ __forceinline__ void planes8(const float* v, bf16x8 (&f)[N]) {
+    uint32_t w[N][4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        float x = v[2 * p], y = v[2 * p + 1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            w[i][p] = pack2bf(x, y);
+            if (i + 1 < N) { x -= bf_lo(w[i][p]); y -= bf_hi(w[i][p]); }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = __builtin_bit_cast(bf16x8, make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]));
+}
+
+// bf16 operands are one plane, fp32 ones three.  Tiles [C][LD] of bf16 a plane in
+// LDS, rows 16 bytes mod 128 apart.
+template <int D_, bool F32_, int C_>
+struct Cfg {
+    static constexpr int D = D_, C = C_, NPL = F32_ ? 3 : 1, NW = D / 16, NTH = 64 * NW, LD = D + 8, LP = C + 8;
+    static constexpr int PLANE = C * LD, TILE = NPL * PLANE, PPL = C * LP, TT = C / 16, NT = TT * (TT + 1) / 2, DT = D / 16,
+                         KD = D / 32, KC = C / 32;
+    static constexpr bool F32 = F32_;
+    typedef typename std::conditional<F32_, float, uint16_t>::type ST;
+    static constexpr int ES = (int)sizeof(ST), VPR = D * ES / 16, NV = C * VPR, PER = NV / NTH;
+    static_assert(NV % NTH == 0 && C % 32 == 0 && D % 32 == 0, "whole pieces");
+};
+
+// C rows on their way from memory to LDS
+template <class K>
+struct Stage {
+    uint4 r[K::PER];
+    // row i at p + i * step; those from n (>= 1) on read the last and are stored as zeros
+    __device__ __forceinline__ void load(const typename K::ST* p, int64_t step, int n) {
+#pragma unroll
+        for (int i = 0; i < K::PER; ++i) {
+            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = (v - row * K::VPR) * (16 / K::ES);
+            r[i] = *reinterpret_cast<const uint4*>(p + min(row, n - 1) * step + c);
+        }
+    }
+    __device__ __forceinline__ void store(uint16_t* t, int n) const {
+#pragma unroll
+        for (int i = 0; i < K::PER; ++i) {
+            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = (v - row * K::VPR) * (16 / K::ES);
+            const uint4 x = row < n ? r[i] : make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (!K::F32) {
+                *reinterpret_cast<uint4*>(t + row * K::LD + c) = x;
+            } else {
+                // each part the next 8 bits of 24, cut off, so that nothing overflows
+                const uint32_t b[4] = {x.x, x.y, x.z, x.w};
+                uint32_t h[4], m[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h[e] = b[e] & 0xffff0000u;
+                    const float rest = __uint_as_float(b[e]) - __uint_as_float(h[e]);
+                    m[e] = __float_as_uint(rest) & 0xffff0000u;
+                    l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
+                }
+                constexpr uint32_t HI = 0x07060302u;
+                uint16_t* q = t + row * K::LD + c;
+                *reinterpret_cast<uint2*>(q) =
+                    make_uint2(__builtin_amdgcn_perm(h[1], h[0], HI), __builtin_amdgcn_perm(h[3], h[2], HI));
+                *reinterpret_cast<uint2*>(q + K::PLANE) =
+                    make_uint2(__builtin_amdgcn_perm(m[1], m[0], HI), __builtin_amdgcn_perm(m[3], m[2], HI));
+                *reinterpret_cast<uint2*>(q + 2 * K::PLANE) =
+                    make_uint2(__builtin_amdgcn_perm(l[1], l[0], HI), __builtin_amdgcn_perm(l[3], l[2], HI));
+            }
+        }
+    }
+};
+
+// fragments of a tile's planes: rows contiguous (c: the matrix unit's own order of
+// the contracted index), in the order of accumulators, and transposed
+template <class K>
+__device__ __forceinline__ void rows_c(const uint16_t* t, int row0, int k0, bf16x8 (&f)[K::NPL]) {
+#pragma unroll
+    for (int p = 0; p < K::NPL; ++p) f[p] = ldfrag_c<1, uint16_t>(t + p * K::PLANE, K::LD, row0, k0).h;
+}
+template <class K>
+__device__ __forceinline__ void rows_k(const uint16_t* t, int row0, int k0, bf16x8 (&f)[K::NPL]) {
+#pragma unroll
+    for (int p = 0; p < K::NPL; ++p) f[p] = ldfrag<1, uint16_t>(t + p * K::PLANE, K::LD, row0, k0).h;
+}
+template <class K>
+__device__ __forceinline__ void cols_k(const uint16_t* t, int n0, int k0, bf16x8 (&f)[K::NPL]) {
+#pragma unroll
+    for (int p = 0; p < K::NPL; ++p) f[p] = ldfragT(t + p * K::PLANE, K::LD, n0, k0).h;
+}
+
+// A chunk's decays.  Sums of g are formed in fp64 (a difference of two sums of
+// fast decays would lose what lies between neighbours) and kept as pairs of fp32,
+// in powers of two.
+template <int C>
+struct Decays {
+    float hi[C], lo[C], up[C], down[C];   // G_t; 2^{G_t}; 2^{G_C - G_t}
+    float all;                            // 2^{G_C}
+};
+constexpr double LOG2E = 1.4426950408889634;
+// e^-200 is zero in fp32, as e^-inf is, and its sums stay finite
+constexpr float G_MIN = -200.f;
+
+__device__ __forceinline__ float decay(float g) { return expf(g < G_MIN ? G_MIN : g); }
+
+// by one wave: lane r has g of row r (0 behind the last)
+template <int C>
+__device__ __forceinline__ double fill_decays(Decays<C>* d, float g) {
+    const int l = lane_id();
+    double x = (double)(g < G_MIN ? G_MIN : g) * LOG2E;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const double y = __shfl_up(x, k, 64);
+        if (l >= k) x += y;
+    }
+    const double all = __shfl(x, C - 1, 64);
+    if (l < C) {
+        const float h = (float)x;
+        d->hi[l] = h;
+        d->lo[l] = (float)(x - (double)h);
+        d->up[l] = __builtin_amdgcn_exp2f(h);
+        d->down[l] = __builtin_amdgcn_exp2f((float)(all - x));
+        if (l == C - 1) d->all = d->up[l];
+    }
+    return all;
+}
+template <int C>
+__device__ __forceinline__ float between(const Decays<C>& d, int t, int s) {
+    return __builtin_amdgcn_exp2f((d.hi[t] - d.hi[s]) + (d.lo[t] - d.lo[s]));
+}
+
+// tile id of the lower triangle -> (row of tiles, column)
+__device__ __forceinline__ void tile_of(int id, int& ti, int& si) {
+    ti = (id >= 1) + (id >= 3) + (id >= 6);
+    si = id - ti * (ti + 1) / 2;
+}
+
+// raw products of X's rows of tile ti with Y's of tile si: lane (c = l % 16, r = l / 16)
+// has X row 16 ti + c with Y rows 16 si + 4 r + i
+template <class K>
+__device__ __forceinline__ f32x4 pair_tile(const uint16_t* X, const uint16_t* Y, int ti, int si) {
+    f32x4 acc = zero4();
+#pragma unroll
+    for (int k = 0; k < K::KD; ++k) {
+        bf16x8 y[K::NPL], x[K::NPL];
+        rows_c<K>(Y, 16 * si, 32 * k, y);
+        rows_c<K>(X, 16 * ti, 32 * k, x);
+        acc = mmp(y, x, acc);
+    }
+    return acc;
+}
+template <class K>
+__device__ __forceinline__ f32x4 mask_tile(const Decays<K::C>& d, int ti, int si) {
+    const int l = lane_id(), t = 16 * ti + (l & 15), s0 = 16 * si + 4 * (l >> 4);
+    f32x4 m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = s0 + i <= t ? between(d, t, s0 + i) : 0.f;
+    return m;
+}
+// a tile of NP planes into P[t][s]
+template <class K, int NP>
+__device__ __forceinline__ void put_pair(uint16_t* P, const f32x4& v, int ti, int si) {
+    const int l = lane_id();
+    uint16_t* p = P + (16 * ti + (l & 15)) * K::LP + 16 * si + 4 * (l >> 4);
+    float x[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const uint32_t a = pack2bf(x[0], x[1]), b = pack2bf(x[2], x[3]);
+        *reinterpret_cast<uint2*>(p + i * K::PPL) = make_uint2(a, b);
+        if (i + 1 < NP) { x[0] -= bf_lo(a); x[1] -= bf_hi(a); x[2] -= bf_lo(b); x[3] -= bf_hi(b); }
+    }
+}
+// the tiles above the diagonal that products of 32 columns read
+template <class K, int NP>
+__device__ __forceinline__ void clear_upper(uint16_t* P) {
+    for (int v = threadIdx.x; v < NP * (K::TT / 2) * 16 * 4; v += K::NTH) {
+        const int c = v & 3, row = (v >> 2) & 15, b = (v >> 6) % (K::TT / 2), p = (v >> 6) / (K::TT / 2);
+        *reinterpret_cast<uint2*>(P + p * K::PPL + (32 * b + row) * K::LP + 32 * b + 16 + 4 * c) = make_uint2(0u, 0u);
+    }
+}
+
+// The state, columns 16 w .. + 15 of W for wave w: lane (c, r) holds St[16 j + 4 r + i]
+// [16 w + c] in s[j][i].  In memory [W's channel][Y's], or (swapped) [Y's][W's].
+template <class K>
+struct State {
+    f32x4 s[K::DT];
+    __device__ __forceinline__ void load(const float* p, bool swapped) {
+        const int l = lane_id(), dw = 16 * (int)(threadIdx.x >> 6) + (l & 15), r = l >> 4;
+#pragma unroll
+        for (int j = 0; j < K::DT; ++j) {
+            if (!p) { s[j] = zero4(); continue; }
+            if (!swapped) {
+                const float4 v = *reinterpret_cast<const float4*>(p + dw * K::D + 16 * j + 4 * r);
+                s[j] = f32x4{v.x, v.y, v.z, v.w};
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[j][i] = p[(16 * j + 4 * r + i) * K::D + dw];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* p, float scale) const {
+        const int l = lane_id(), dw = 16 * (int)(threadIdx.x >> 6) + (l & 15), r = l >> 4;
+#pragma unroll
+        for (int j = 0; j < K::DT; ++j)
+            *reinterpret_cast<float4*>(p + dw * K::D + 16 * j + 4 * r) =
+                make_float4(scale * s[j][0], scale * s[j][1], scale * s[j][2], scale * s[j][3]);
+    }
+    // S <- all S + Y^T (down W): the chunk's sum from zero, so that what the matrix unit
+    // loses (it rounds sums downwards) does not add up over the chunks
+    __device__ __forceinline__ void add(const uint16_t* Y, const uint16_t* W, const Decays<K::C>& d) {
+        const int l = lane_id(), r = l >> 4, n0 = 16 * (int)(threadIdx.x >> 6);
+        f32x4 u[K::DT];
+#pragma unroll
+        for (int j = 0; j < K::DT; ++j) u[j] = zero4();
+#pragma unroll
+        for (int k = 0; k < K::KC; ++k) {
+            bf16x8 w[K::NPL], ws[3];
+            cols_k<K>(W, n0, 32 * k, w);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = (float)w[0][e];
+                if constexpr (K::NPL == 3) v[e] += (float)w[1][e] + (float)w[2][e];
+                v[e] *= d.down[32 * k + kslot(r, e)];
+            }
+            planes8<3>(v, ws);
+#pragma unroll
+            for (int j = 0; j < K::DT; ++j) {
+                bf16x8 y[K::NPL];
+                cols_k<K>(Y, 16 * j, 32 * k, y);
+                u[j] = mmp(y, ws, u[j]);
+            }
+        }
+        const float all = d.all;
+#pragma unroll
+        for (int j = 0; j < K::DT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[j][i] = fmaf(all, s[j][i], u[j][i]);
+    }
+    // NS planes of the state for the products with X
+    template <int NS>
+    __device__ __forceinline__ void planes(bf16x8 (&f)[K::KD][NS]) const {
+#pragma unroll
+        for (int k = 0; k < K::KD; ++k) {
+            const float v[8] = {s[2 * k][0], s[2 * k][1], s[2 * k][2], s[2 * k][3],
+                                s[2 * k + 1][0], s[2 * k + 1][1], s[2 * k + 1][2], s[2 * k + 1][3]};
+            planes8<NS>(v, f[k]);
+        }
+    }
+    // up_t (St^T X_t) for every row: lane (c, r) has row 16 i + c, channels 16 w + 4 r ..
+    template <int NS>
+    __device__ __forceinline__ void apply(const uint16_t* X, const Decays<K::C>& d, f32x4 (&o)[K::TT]) const {
+        bf16x8 f[K::KD][NS];
+        planes<NS>(f);
+        const int c = lane_id() & 15;
+#pragma unroll
+        for (int i = 0; i < K::TT; ++i) {
+            f32x4 acc = zero4();
+#pragma unroll
+            for (int k = 0; k < K::KD; ++k) {
+                bf16x8 x[K::NPL];
+                rows_k<K>(X, 16 * i, 32 * k, x);
+                acc = mmp(f[k], x, acc);
+            }
+            const float up = d.up[16 * i + c];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = acc[e] * up;
+        }
+    }
+};
+
+// o_t += sum_s P[t][s] W_s, layout as State::apply
+template <class K, int NP>
+__device__ __forceinline__ void add_pairs(const uint16_t* P, const uint16_t* W, f32x4 (&o)[K::TT]) {
+    const int n0 = 16 * (int)(threadIdx.x >> 6);
+#pragma unroll
+    for (int k = 0; k < K::KC; ++k) {
+        bf16x8 w[K::NPL];
+        cols_k<K>(W, n0, 32 * k, w);
+#pragma unroll
+        for (int i = 2 * k; i < K::TT; ++i) {
+            bf16x8 p[NP];
+#pragma unroll
+            for (int q = 0; q < NP; ++q) p[q] = ldfrag<1, uint16_t>(P + q * K::PPL, K::LP, 16 * i, 32 * k).h;
+            o[i] = mmp(w, p, o[i]);
+        }
+    }
+}
+
+// four channels of a token's output
+template <typename T>
+__device__ __forceinline__ void put4(T* p, const f32x4& v) {
+    if constexpr (std::is_same<T, float>::value)
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
+}
+template <class K, typename OT>
+__device__ __forceinline__ void put_rows(OT* out, int64_t step, const f32x4 (&o)[K::TT], int n) {
+    const int l = lane_id(), ch = 16 * (int)(threadIdx.x >> 6) + 4 * (l >> 4);
+#pragma unroll
+    for (int i = 0; i < K::TT; ++i) {
+        const int t = 16 * i + (l & 15);
+        if (t < n) put4<OT>(out + t * step + ch, o[i]);
+    }
+}
+__device__ __forceinline__ float quad_sum(float x) {   // over the four lanes of equal l % 16
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+
+template <typename T>
+__device__ __forceinline__ const T* at(const Rows& r, int b, int tok, int h) {
+    return static_cast<const T*>(r.p) + b * r.batch + tok * r.token + (h / r.share) * r.head;
+}
+
+// rows of no sequence
+template <int D, typename OT>
+__device__ __forceinline__ void clear_rows(void* out, const DecayArgs& a, const Slot& s, int h) {
+    for (int v = threadIdx.x; v < s.n * D; v += blockDim.x)
+        static_cast<OT*>(out)[((int64_t)(s.tok0 + v / D) * a.H + h) * D + v % D] = OT(0);
+}
+
+template <class K, int NP>
+constexpr size_t mix_lds(bool states, bool dot) {
+    return (states ? 2 : 3) * (size_t)K::TILE * 2 + (states ? 0 : (size_t)NP * K::PPL * 2) + sizeof(Decays<K::C>) +
+           (dot ? (size_t)K::NW * K::C * 4 : 0);
+}
+
+// mix: out = the operator over a slot's tokens (REV: backwards in time).  STATES: only
+// what the slot adds to the state, and its whole decay.  DOT: dots[t] = z_t . (the part
+// of out_t that comes from the state before the chunk), which NS = 3 keeps to fp32.
+template <class K, typename OT, int NP, int NS, bool REV, bool STATES, bool DOT>
+__global__ __launch_bounds__(K::NTH) void kda_decay_mix_kernel(const DecayArgs a, const bool swapped) {
+    typedef typename K::ST ST;
+    __shared__ __attribute__((aligned(16))) char lds[mix_lds<K, NP>(STATES, DOT)];
+    uint16_t* X = reinterpret_cast<uint16_t*>(lds);
+    uint16_t* Y = X + (STATES ? 0 : K::TILE);
+    uint16_t* W = Y + K::TILE;
+    uint16_t* P = W + K::TILE;
+    Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : NP * K::PPL));
+    float* part = reinterpret_cast<float*>(dec + 1);   // DOT: [NW][C]
+
+    const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x), j = bid / a.H, h = bid - j * a.H;
+    const Slot s = slot_of(a, j);
+    if (s.seq < 0) {
+        if constexpr (!STATES) {
+            if (s.seq == -1) clear_rows<K::D, OT>(a.out, a, s, h);
+        }
+        return;
+    }
+    if (STATES && (REV ? s.first : s.last)) return;   // nothing follows
+    const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+    constexpr int DD = K::D * K::D;
+    State<K> st;
+    st.load(STATES || !a.s_in ? nullptr : a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD, swapped);
+
+    const int dir = REV ? -1 : 1, head = REV ? s.tok0 + s.n - 1 : s.tok0;   // the first row's token
+    const ST *x = at<ST>(a.x, b, head, h), *y = at<ST>(a.y, b, head, h), *w = at<ST>(a.w, b, head, h);
+    const float* g = a.g + b * a.gb + (int64_t)head * a.gt + h * a.gh;
+    const int64_t xs = dir * a.x.token, ys = dir * a.y.token, ws = dir * a.w.token, gs = dir * a.gt;
+    Stage<K> sx, sy, sw;
+    float gv = 0.f;
+    auto load = [&](int i0) {
+        const int n = s.n - i0;
+        if constexpr (!STATES) sx.load(x + i0 * xs, xs, n);
+        sy.load(y + i0 * ys, ys, n);
+        sw.load(w + i0 * ws, ws, n);
+        // backwards, row i decays by what its successor in time does; the first by nothing
+        const int i = i0 + l;
+        if (wave == 0) gv = l < K::C && i < s.n && !(REV && i == 0) ? g[(int64_t)(REV ? i - 1 : i) * gs] : 0.f;
+    };
+    if constexpr (!STATES) clear_upper<K, NP>(P);
+    double whole = 0.0;
+    if (s.n > 0) load(0);
+    for (int i0 = 0; i0 < s.n; i0 += K::C) {
+        const int n = s.n - i0;
+        if (i0) lds_barrier();   // every wave has read the chunk before
+        if constexpr (!STATES) sx.store(X, n);
+        sy.store(Y, n);
+        sw.store(W, n);
+        if (wave == 0) whole += fill_decays<K::C>(dec, gv);
+        lds_barrier();
+        if (i0 + K::C < s.n) load(i0 + K::C);
+        if constexpr (STATES) {
+            st.add(Y, W, *dec);
+        } else {
+#pragma unroll
+            for (int k = 0; k < (K::NT + K::NW - 1) / K::NW; ++k) {
+                const int id = wave + K::NW * k;
+                if (id < K::NT) {
+                    int ti, si;
+                    tile_of(id, ti, si);
+                    f32x4 p = pair_tile<K>(X, Y, ti, si);
+                    p *= mask_tile<K>(*dec, ti, si);
+                    put_pair<K, NP>(P, p, ti, si);
+                }
+            }
+            f32x4 o[K::TT];
+            st.template apply<NS>(X, *dec, o);
+            const int64_t row = (int64_t)b * a.T + head + dir * i0;   // of the chunk's first row
+            if constexpr (DOT) {
+                const ST* z = at<ST>(a.z, b, head + dir * i0, h) + 16 * wave + 4 * (l >> 4);
+#pragma unroll
+                for (int i = 0; i < K::TT; ++i) {
+                    const int t = 16 * i + (l & 15);
+                    const float4 q = ld4<ST>(z + (int64_t)min(t, n - 1) * dir * a.z.token);
+                    const float d = quad_sum(fmaf(q.x, o[i][0], q.y * o[i][1]) + fmaf(q.z, o[i][2], q.w * o[i][3]));
+                    if (l < 16) part[wave * K::C + t] = d;
+                }
+            }
+            st.add(Y, W, *dec);
+            lds_barrier();
+            add_pairs<K, NP>(P, W, o);
+            put_rows<K, OT>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, dir * (int64_t)a.H * K::D, o, n);
+            if constexpr (DOT) {
+                const int t = threadIdx.x;
+                if (t < K::C && t < n) {
+                    float d = 0.f;
+#pragma unroll
+                    for (int k = 0; k < K::NW; ++k) d += part[k * K::C + t];
+                    a.dots[(int64_t)h * a.B * a.T + row + dir * t] = d;
+                }
+            }
+        }
+    }
+    if constexpr (STATES) {
+        // backwards: to before the slot's first token
+        float last = 1.f;
+        if constexpr (REV) last = decay(g[(int64_t)(s.n - 1) * gs]);
+        if (threadIdx.x == 0) a.seg[(int64_t)j * a.H + h] = __builtin_amdgcn_exp2f((float)whole) * last;
+        st.store(a.s_out + ((int64_t)j * a.H + h) * DD, last);
+    } else if (a.s_out && (REV ? s.first : s.last)) {
+        float last = 1.f;
+        if constexpr (REV) last = s.n > 0 ? decay(g[(int64_t)(s.n - 1) * gs]) : 1.f;
+        st.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, last);
+    }
+}
+
+// e^{sum of g over a chunk} below which what passes through it is nothing beside what begins in it
+constexpr float ANCHOR_BELOW = 0x1p-32f;
+
+template <class K, int NP>
+constexpr size_t mix2_lds(bool dot) {
+    return 4 * (size_t)K::TILE * 2 + 2 * (size_t)NP * K::PPL * 2 + sizeof(Decays<K::C>) +
+           (dot ? (size_t)(K::NW + 2 * K::TT) * K::C * 4 : 0);
+}
+
+// mix2: dk and dv of a slot, backwards in time, from q (y), k (x), v (z) and do (w), with
+// dS in both orders: dv = mix(k, q, do), dk = mix(v, do, q).  DOT: dots[t] -= k_t . (the part
+// of dk_t from behind the chunk); dots2[t] = rows - columns of E, E_{ts} = e^{G_t - G_s}
+// (q_t . k_s) (do_t . v_s), whose sums over s and over t are what the chunk's own pairs
+// give q . dq and k . dk; and where nothing passes through a whole chunk anchors[chunk], all
+// that leaves it.
+template <class K, typename OT, int NP, int NS, bool DOT>
+__global__ __launch_bounds__(K::NTH) void kda_decay_mix2_kernel(const DecayArgs a) {
+    typedef typename K::ST ST;
+    __shared__ __attribute__((aligned(16))) char lds[mix2_lds<K, NP>(DOT)];
+    uint16_t* Kt = reinterpret_cast<uint16_t*>(lds);
+    uint16_t* Q = Kt + K::TILE;
+    uint16_t* V = Q + K::TILE;
+    uint16_t* O = V + K::TILE;
+    uint16_t* PA = O + K::TILE;
+    uint16_t* PD = PA + NP * K::PPL;
+    Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(PD + NP * K::PPL);
+    float* part = reinterpret_cast<float*>(dec + 1);   // DOT: [NW][C]; then E's [TT column tiles][C] and [TT row tiles][C]
+    float* e_own = part + K::NW * K::C;                // sums over the other tokens, of X rows (k, v)
+    float* e_oth = e_own + K::TT * K::C;               // and of Y rows (q, do)
+
+    const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x), j = bid / a.H, h = bid - j * a.H;
+    const Slot s = slot_of(a, j);
+    if (s.seq < 0) {
+        if (s.seq == -1) {
+            clear_rows<K::D, OT>(a.out, a, s, h);
+            clear_rows<K::D, OT>(a.out2, a, s, h);
+        }
+        return;
+    }
+    const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+    constexpr int DD = K::D * K::D;
+    const float* s_in = a.s_in ? a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD : nullptr;
+    State<K> sv, sk;   // dv's: [do][q]; dk's: [q][do]
+    sv.load(s_in, false);
+    sk.load(s_in, true);
+
+    const int head = s.tok0 + s.n - 1;
+    const ST *kp = at<ST>(a.x, b, head, h), *qp = at<ST>(a.y, b, head, h), *vp = at<ST>(a.z, b, head, h),
+             *op = at<ST>(a.w, b, head, h);
+    const float* g = a.g + b * a.gb + (int64_t)head * a.gt + h * a.gh;
+    Stage<K> rk, rq, rv, ro;
+    float gv = 0.f;
+    // the chunks are those of a pass forwards, so that dots and the sums of mix over them add up
+    const int n0 = s.n - (s.n - 1) / K::C * K::C;
+    auto load = [&](int i0) {
+        const int n = i0 ? K::C : n0, i = i0 + l;
+        rk.load(kp - i0 * a.x.token, -a.x.token, n);
+        rq.load(qp - i0 * a.y.token, -a.y.token, n);
+        rv.load(vp - i0 * a.z.token, -a.z.token, n);
+        ro.load(op - i0 * a.w.token, -a.w.token, n);
+        if (wave == 0) gv = l < n && i > 0 ? g[-(int64_t)(i - 1) * a.gt] : 0.f;
+    };
+    clear_upper<K, NP>(PA);
+    clear_upper<K, NP>(PD);
+    if constexpr (DOT)
+        for (int v = threadIdx.x; v < 2 * K::TT * K::C; v += K::NTH) e_own[v] = 0.f;
+    if (s.n > 0) load(0);
+    for (int i0 = 0, n = n0; i0 < s.n; i0 += n, n = K::C) {
+        if (i0) lds_barrier();
+        rk.store(Kt, n);
+        rq.store(Q, n);
+        rv.store(V, n);
+        ro.store(O, n);
+        if (wave == 0) fill_decays<K::C>(dec, gv);
+        lds_barrier();
+        if (i0 + n < s.n) load(i0 + n);
+#pragma unroll
+        for (int k = 0; k < (K::NT + K::NW - 1) / K::NW; ++k) {
+            const int id = wave + K::NW * k;
+            if (id < K::NT) {
+                int ti, si;
+                tile_of(id, ti, si);
+                const f32x4 m = mask_tile<K>(*dec, ti, si);
+                const f32x4 pa = pair_tile<K>(Kt, Q, ti, si) * m, d = pair_tile<K>(V, O, ti, si);
+                put_pair<K, NP>(PA, pa, ti, si);
+                put_pair<K, NP>(PD, d * m, ti, si);
+                if constexpr (DOT) {
+                    // a token's own pair passes no decay, and would drown what does where decays are fast
+                    f32x4 e = pa * d;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (ti == si && 4 * (l >> 4) + i == (l & 15)) e[i] = 0.f;
+                    const float own = quad_sum((e[0] + e[1]) + (e[2] + e[3]));
+                    if (l < 16) e_own[si * K::C + 16 * ti + l] = own;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float x = e[i];
+#pragma unroll
+                        for (int q = 1; q < 16; q <<= 1) x += __shfl_xor(x, q, 64);
+                        if ((l & 15) == 0) e_oth[ti * K::C + 16 * si + 4 * (l >> 4) + i] = x;
+                    }
+                }
+            }
+        }
+        const int64_t row = (int64_t)b * a.T + head - i0, step = -(int64_t)a.H * K::D;
+        const int ch = 16 * wave + 4 * (l >> 4);
+        f32x4 o[K::TT], o2[K::TT];
+        sv.template apply<NS>(Kt, *dec, o);
+        if constexpr (DOT) {
+#pragma unroll
+            for (int i = 0; i < K::TT; ++i) {
+                const int t = 16 * i + (l & 15);
+                float4 v = ld4<uint16_t>(V + t * K::LD + ch);
+                if constexpr (K::NPL == 3) {
+                    const float4 v1 = ld4<uint16_t>(V + K::PLANE + t * K::LD + ch),
+                                 v2 = ld4<uint16_t>(V + 2 * K::PLANE + t * K::LD + ch);
+                    v = make_float4(v.x + (v1.x + v2.x), v.y + (v1.y + v2.y), v.z + (v1.z + v2.z), v.w + (v1.w + v2.w));
+                }
+                const float d = quad_sum(fmaf(v.x, o[i][0], v.y * o[i][1]) + fmaf(v.z, o[i][2], v.w * o[i][3]));
+                if (l < 16) part[wave * K::C + t] = d;
+            }
+        }
+        sk.template apply<K::NPL == 3 ? 3 : NP>(V, *dec, o2);
+        sv.add(Q, O, *dec);
+        sk.add(O, Q, *dec);
+        lds_barrier();
+        add_pairs<K, NP>(PA, O, o);
+        add_pairs<K, NP>(PD, Q, o2);
+        put_rows<K, OT>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, step, o2, n);
+        put_rows<K, OT>(static_cast<OT*>(a.out2) + (row * a.H + h) * K::D, step, o, n);
+        if constexpr (DOT) {
+            const int t = threadIdx.x;
+            if (t < K::C && t < n) {
+                float own = 0.f, oth = 0.f, d = 0.f;
+#pragma unroll
+                for (int k = 0; k < K::TT; ++k) {
+                    own += e_own[k * K::C + t];
+                    oth += e_oth[k * K::C + t];
+                }
+#pragma unroll
+                for (int k = 0; k < K::NW; ++k) d += part[k * K::C + t];
+                const int64_t at = (int64_t)h * a.B * a.T + row - t;
+                a.dots[at] -= d;
+                a.dots2[at] = oth - own;
+                part[t] = d;   // (each thread has read its own column)
+            }
+            if (wave == 0) {
+                wave_sync();
+                float sum = l < K::C && l < n ? part[l] : 0.f;
+#pragma unroll
+                for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k, 64);
+                if (l == 0)
+                    a.anchors[((int64_t)j * a.H + h) * (a.seg_tokens / K::C) + (s.n - i0 - 1) / K::C] =
+                        dec->all < ANCHOR_BELOW ? sum : __builtin_nanf("");
+            }
+        }
+    }
+    if (a.s_out && s.first) {
+        const float last = s.n > 0 ? decay(g[-(int64_t)(s.n - 1) * a.gt]) : 1.f;
+        sv.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, last);
+    }
+}
+
+// ----------------------------------------------------------------------------
+// between the slots
+// ----------------------------------------------------------------------------
+
+// Slots of packed sequences, cu[0 .. nseq] their limits (taken as rising and within
+// [0, T], whatever they hold): tab as slot_of reads it, first[i] sequence i's first
+// slot.  What lies before the first and behind the last sequence becomes slots of
+// no sequence, after the others.
+constexpr int PLAN_TH = 1024;
+__global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, int nseq, int T, int seg_tokens, int4* tab,
+                                                                 int* first, int nslots) {
+    __shared__ int buf[PLAN_TH];
+    __shared__ int carry_end, carry_slots;
+    const int t = threadIdx.x;
+    if (t == 0) {
+        carry_end = min(max(cu[0], 0), T);
+        carry_slots = 0;
+    }
+    const int begin = min(max(cu[0], 0), T);
+    for (int i0 = 0; i0 < nseq; i0 += PLAN_TH) {
+        const int i = i0 + t;
+        // the largest limit so far
+        buf[t] = i < nseq ? min(max(cu[i + 1], 0), T) : 0;
+        __syncthreads();
+        for (int k = 1; k < PLAN_TH; k <<= 1) {
+            const int x = t >= k ? buf[t - k] : 0;
+            __syncthreads();
+            buf[t] = max(buf[t], x);
+            __syncthreads();
+        }
+        const int lo = max(carry_end, t ? buf[t - 1] : 0), hi = max(carry_end, buf[t]), top = max(carry_end, buf[PLAN_TH - 1]);
+        __syncthreads();
+        const int n = i < nseq ? hi - lo : 0, slots = i < nseq ? max(1, (n + seg_tokens - 1) / seg_tokens) : 0;
+        buf[t] = slots;
+        __syncthreads();
+        for (int k = 1; k < PLAN_TH; k <<= 1) {
+            const int x = t >= k ? buf[t - k] : 0;
+            __syncthreads();
+            buf[t] += x;
+            __syncthreads();
+        }
+        const int at = carry_slots + buf[t] - slots, total = carry_slots + buf[PLAN_TH - 1];
+        if (i < nseq) {
+            first[i] = at;
+            for (int k = 0; k < slots; ++k)
+                tab[at + k] = make_int4(lo + k * seg_tokens, min(seg_tokens, n - k * seg_tokens), i,
+                                        (k == 0) | (k == slots - 1) << 1);
+        }
+        __syncthreads();
+        if (t == 0) {
+            carry_end = top;
+            carry_slots = total;
+        }
+        __syncthreads();
+    }
+    const int used = carry_slots, end = carry_end;
+    if (t == 0) first[nseq] = used;
+    const int lead = (begin + seg_tokens - 1) / seg_tokens, trail = (T - end + seg_tokens - 1) / seg_tokens;
+    for (int k = t; k < nslots - used; k += PLAN_TH) {
+        int4 v = make_int4(0, 0, -2, 0);
+        if (k < lead) v = make_int4(k * seg_tokens, min(seg_tokens, begin - k * seg_tokens), -1, 0);
+        else if (k - lead < trail)
+            v = make_int4(end + (k - lead) * seg_tokens, min(seg_tokens, T - end - (k - lead) * seg_tokens), -1, 0);
+        tab[used + k] = v;
+    }
+}
+
+// The state at each slot's start (REV: its adjoint at each slot's end), in place of
+// what the slots add: one thread takes four elements through a sequence's slots, eight
+// loads at a time.
+template <bool REV>
+__global__ __launch_bounds__(256) void kda_decay_scan_kernel(float* u, const float* seg, const float* s0, const int* first,
+                                                             int per_seq, int H, int DD, int parts) {
+    const int part = blockIdx.x % parts, sh = blockIdx.x / parts, seq = sh / H, h = sh - seq * H;
+    const int e = 4 * (part * 256 + (int)threadIdx.x);
+    if (e >= DD) return;
+    const int lo = first ? first[seq] : seq * per_seq, count = (first ? first[seq + 1] : lo + per_seq) - lo;
+    float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s0) run = *reinterpret_cast<const float4*>(s0 + ((int64_t)seq * H + h) * DD + e);
+    auto slot = [&](int i) { return (int64_t)(REV ? lo + count - 1 - i : lo + i) * H + h; };
+    constexpr int AHEAD = 8;
+    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+        float4 v[AHEAD];
+        float f[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            // (the last one adds nothing to a start)
+            const int64_t at = slot(min(i0 + k, count - 1));
+            const bool any = i0 + k < count - 1;
+            v[k] = any ? *reinterpret_cast<const float4*>(u + at * DD + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            f[k] = any ? seg[at] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (i0 + k < count) {
+                *reinterpret_cast<float4*>(u + slot(i0 + k) * DD + e) = run;
+                run = make_float4(fmaf(f[k], run.x, v[k].x), fmaf(f[k], run.y, v[k].y), fmaf(f[k], run.z, v[k].z),
+                                  fmaf(f[k], run.w, v[k].w));
+            }
+        }
+    }
+}
+
+// dg of a slot: what passes from before token t to t or later,
+//   <S, dS> at the slot's end + sum_{s >= t} dots_s + sum_{s >= t, in t's chunk} dots2_s.
+// A chunk's dots2 add up to nothing, so their errors stay in it, and where nothing passes
+// through a chunk the first two begin anew at its end, with what leaves it: with all of
+// q . dq - k . dk in one sum over the slot, dg of fast decays was 2 to 60 times as far
+// off.  Sums in fp64.
+// s_end, ds_end: the state and its adjoint at a slot's end (the last slot's by sequence).
+// sums (not null): only the slot's whole sum.
+constexpr int DG_TH = 256;
+__global__ __launch_bounds__(DG_TH) void kda_decay_dg_kernel(const DecayArgs a, const float* starts, const float* dends,
+                                                             const float* s_final, const float* ds_final, float* dg,
+                                                             double* sums, int DD, int C) {
+    __shared__ double buf[DG_TH / 32];
+    const int j = blockIdx.x / a.H, h = blockIdx.x - j * a.H, t = threadIdx.x, l = t & 63, w = t >> 6;
+    const Slot s = slot_of(a, j);
+    if (s.seq < 0) {
+        if (s.seq == -1 && dg)
+            for (int i = t; i < s.n; i += DG_TH) dg[(int64_t)(s.tok0 + i) * a.H + h] = 0.f;
+        if (sums && t == 0) sums[(int64_t)j * a.H + h] = 0.0;
+        return;
+    }
+    auto all = [&](double x) {
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k, 64);
+        __syncthreads();
+        if (l == 0) buf[w] = x;
+        __syncthreads();
+        double y = 0.0;
+#pragma unroll
+        for (int k = 0; k < DG_TH / 64; ++k) y += buf[k];
+        return y;
+    };
+    const float *p = nullptr, *q = nullptr;
+    if (s.last) {
+        if (ds_final) {
+            p = s_final + ((int64_t)s.seq * a.H + h) * DD;
+            q = ds_final + ((int64_t)s.seq * a.H + h) * DD;
+        }
+    } else {
+        p = starts + ((int64_t)(j + 1) * a.H + h) * DD;
+        q = dends + ((int64_t)j * a.H + h) * DD;
+    }
+    double run = 0.0;
+    if (p) {
+        for (int e = 4 * t; e < DD; e += 4 * DG_TH) {
+            const float4 x = *reinterpret_cast<const float4*>(p + e), y = *reinterpret_cast<const float4*>(q + e);
+            run += ((double)x.x * y.x + (double)x.y * y.y) + ((double)x.z * y.z + (double)x.w * y.w);
+        }
+        run = all(run);
+    }
+    const int b = a.tab ? 0 : s.seq;
+    const int64_t base = (int64_t)h * a.B * a.T + (int64_t)b * a.T + s.tok0;
+    double whole = 0.0;
+    // 256 tokens a step from the last on; lane l of wave w has token i0 + 64 w + l
+    const float* anchors = a.anchors + ((int64_t)j * a.H + h) * (a.seg_tokens / C);
+    const int own = t / C;
+    for (int i0 = (s.n - 1) / DG_TH * DG_TH; i0 >= 0; i0 -= DG_TH) {
+        const int i = i0 + t;
+        double x = i < s.n ? (double)a.dots[base + i] : 0.0, e = i < s.n ? (double)a.dots2[base + i] : 0.0;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) {
+            const double y = __shfl_down(x, k, 64), f = __shfl_down(e, k, 64);
+            if ((l & (C - 1)) + k < C) { x += y; e += f; }
+        }
+        __syncthreads();
+        if (t % C == 0) buf[own] = x;
+        __syncthreads();
+        double behind = 0.0;
+        for (int k = DG_TH / C - 1; k >= 0; --k) {
+            if (i0 + k * C < s.n) {
+                const float anchor = anchors[i0 / C + k];
+                if (anchor == anchor) run = (double)anchor;
+            }
+            if (k == own) behind = run;
+            run += buf[k];
+        }
+        if (i < s.n) {
+            // (nothing passes a decay of zero: exactly)
+            const float g = a.g[b * a.gb + (int64_t)(s.tok0 + i) * a.gt + h * a.gh];
+            const double v = g < G_MIN ? 0.0 : (behind + x) + e;
+            if (dg) dg[((int64_t)b * a.T + s.tok0 + i) * a.H + h] = (float)v;
+            whole += v;
+        }
+    }
+    if (sums) {
+        whole = all(whole);
+        if (t == 0) sums[(int64_t)j * a.H + h] = whole;
+    }
+}
+// one decay a head: its gradient is the sum over the slots
+__global__ __launch_bounds__(64) void kda_decay_dg_sum_kernel(const double* sums, float* dg, int nslots, int H) {
+    double x = 0.0;
+    for (int j = threadIdx.x; j < nslots; j += 64) x += sums[(int64_t)j * H + blockIdx.x];
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k, 64);
+    if (threadIdx.x == 0) dg[blockIdx.x] = (float)x;
+}
+
+// gradients of a tensor whose heads are shared: sums over the state's heads, rounded once
+template <typename OT>
+__global__ __launch_bounds__(256) void kda_decay_group_kernel(const float* src, OT* dst, int64_t n4, int share, int D) {
+    const int per = D / 4;
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < n4; v += (int64_t)gridDim.x * 256) {
+        const int64_t head = v / per;
+        const float* p = src + (head * share) * D + 4 * (v - head * per);
+        f32x4 x = zero4();
+        for (int k = 0; k < share; ++k) {
+            const float4 y = *reinterpret_cast<const float4*>(p + (int64_t)k * D);
+            x += f32x4{y.x, y.y, y.z, y.w};
+        }
+        put4<OT>(dst + 4 * v, x);
+    }
+}
+
+
+// ----------------------------------------------------------------------------
+// one token
+// ----------------------------------------------------------------------------
+struct StepArgs {
+    Rows q, k, v;               // [row][head][D] (token: unused)
+    const float* g;
+    int64_t gb, gh;
+    float* s;                   // [N][H][D][D]
+    const int* slots;           // of each row, or null: its own number
+    void* o;                    // [B][H][D]
+    int B, H, N;
+};
+
+// A wave takes R rows of a state (rows of v's channels) through one token: loads of
+// 16 bytes a lane, L lanes a row, all in flight together.  The states' bytes, read and
+// written once, are all that counts.
+template <int D>
+struct StepCfg {
+    static constexpr int L = D == 32 ? 8 : D == 64 ? 16 : 32, RP = 64 / L, R = D == 32 ? 32 : 16, NP = R / RP, PARTS = D / R;
+};
+template <int D, typename ST>
+__global__ __launch_bounds__(256) void kda_decay_step_kernel(const StepArgs a) {
+    typedef StepCfg<D> C;
+    const int l = lane_id(), unit = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
+    const int part = unit % C::PARTS, bh = unit / C::PARTS, b = bh / a.H, h = bh - b * a.H;
+    if (b >= a.B) return;
+    const int col = 4 * (l % C::L), row0 = part * C::R + l / C::L;
+    const bool in = col < D;
+    const int n = a.slots ? a.slots[b] : b;
+    auto out = [&](int r) { return static_cast<ST*>(a.o) + ((int64_t)r * a.H + h) * D; };
+    if (n < 0 || n >= a.N) {
+        if (l < C::R) st1<ST>(out(b) + part * C::R + l, 0.f);
+        return;
+    }
+    if (a.slots) {   // rows of one state follow each other: the first of them does all
+        for (int i = l; i - l < b; i += 64)
+            if (__any(i < b && a.slots[min(i, b - 1)] == n)) return;
+    }
+    float* s = a.s + ((int64_t)n * a.H + h) * D * D + (int64_t)row0 * D + (in ? col : 0);
+    float4 x[C::NP];
+#pragma unroll
+    for (int i = 0; i < C::NP; ++i) x[i] = *reinterpret_cast<const float4*>(s + i * C::RP * D);
+    for (int r = b; r < a.B;) {
+        const ST *qp = static_cast<const ST*>(a.q.p) + r * a.q.batch + (h / a.q.share) * a.q.head,
+                 *kp = static_cast<const ST*>(a.k.p) + r * a.k.batch + (h / a.k.share) * a.k.head,
+                 *vp = static_cast<const ST*>(a.v.p) + r * a.v.batch + (h / a.v.share) * a.v.head;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 q = in ? ld4<ST>(qp + col) : zero, k = in ? ld4<ST>(kp + col) : zero;
+        const float f = decay(a.g[r * a.gb + h * a.gh]);
+        ST* o = out(r);
+#pragma unroll
+        for (int i = 0; i < C::NP; ++i) {
+            const int row = row0 + i * C::RP;
+            const float v = ld1<ST>(vp + row);
+            x[i] = make_float4(fmaf(f, x[i].x, v * k.x), fmaf(f, x[i].y, v * k.y), fmaf(f, x[i].z, v * k.z),
+                               fmaf(f, x[i].w, v * k.w));
+            float y = fmaf(x[i].x, q.x, x[i].y * q.y) + fmaf(x[i].z, q.z, x[i].w * q.w);
+            if (!in) y = 0.f;
+#pragma unroll
+            for (int m = 1; m < C::L; m <<= 1) y += __shfl_xor(y, m, 64);
+            if (l % C::L == 0) st1<ST>(o + row, y);
+        }
+        if (!a.slots) break;
+        int next = a.B;
+        for (int i0 = r + 1; i0 < a.B && next == a.B; i0 += 64) {
+            const uint64_t m = __ballot(i0 + l < a.B && a.slots[min(i0 + l, a.B - 1)] == n);
+            if (m) next = i0 + __builtin_ctzll(m);
+        }
+        r = next;
+    }
+    if (in)
+#pragma unroll
+        for (int i = 0; i < C::NP; ++i) *reinterpret_cast<float4*>(s + i * C::RP * D) = x[i];
+}
+
+// ----------------------------------------------------------------------------
+// host
+// ----------------------------------------------------------------------------
+typedef kda_decay_args Args;
+
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+struct Plan {
+    int seg_tokens, per_seq, nslots, packed;
+    bool multi;   // the states between slots are in memory
+};
+// Workgroups beside each other that fill the card: 256 CUs with four of head sizes up
+// to 64, two of larger ones.
+Plan plan_of(const Args& a, bool dg) {
+    Plan p;
+    const int64_t want = a.D <= 64 ? 1024 : 512, seqs = a.cu ? 1 : a.B, chunks = (a.T + 63) / 64;
+    int64_t per = 1;
+    if (seqs * a.H * 2 <= want && chunks > 4) per = std::min((chunks + 3) / 4, (want + seqs * a.H - 1) / (seqs * a.H));
+    int64_t seg = std::max<int64_t>(1, (chunks + per - 1) / per);
+    // dg is a sum over a slot's tokens, whose errors add up
+    if (dg) seg = std::min<int64_t>(seg, 32);
+    p.packed = a.cu != nullptr;
+    p.seg_tokens = (int)(64 * seg);
+    p.per_seq = p.packed ? 0 : (int)std::max<int64_t>(1, (chunks + seg - 1) / seg);
+    const int64_t n = p.packed ? a.nseq + 2 + a.T / p.seg_tokens : a.B * p.per_seq;
+    p.nslots = n * a.H > 0x7fffffff ? -1 : (int)n;
+    p.multi = p.packed || p.per_seq > 1;
+    return p;
+}
+
+// the workspace's parts, offsets in bytes
+struct Layout {
+    int64_t tab = -1, first = -1, s = -1, seg = -1, ds = -1, segd = -1, dots = -1, anchors = -1, sums = -1, g0 = -1, g1 = -1, bytes = 0;
+};
+bool shared(const Args& a, const kda_decay_rows& r) { return r.heads != a.H; }
+Layout layout_of(const Args& a, const Plan& p, bool bwd) {
+    Layout l;
+    auto take = [&](int64_t n) { const int64_t at = l.bytes; l.bytes += up16(n); return at; };
+    if (p.packed) {
+        l.tab = take(16 * (int64_t)p.nslots);
+        l.first = take(4 * (a.nseq + 1));
+    }
+    const int64_t st = 4 * (int64_t)p.nslots * a.H * a.D * a.D, sg = 4 * (int64_t)p.nslots * a.H;
+    if (p.multi) {
+        l.s = take(st);
+        l.seg = take(sg);
+    }
+    if (bwd) {
+        if (p.multi) {
+            l.ds = take(st);
+            l.segd = take(sg);
+        }
+        if (a.dg) {
+            l.dots = take(2 * 4 * a.H * a.B * a.T);
+            l.anchors = take(sg * (p.seg_tokens / 32));
+            if (a.dg_heads) l.sums = take(2 * sg);
+        }
+        const int64_t rows = 4 * a.B * a.T * a.H * a.D;
+        const bool kv = shared(a, a.k) || shared(a, a.v);
+        if (kv || shared(a, a.q)) l.g0 = take(rows);
+        if (kv) l.g1 = take(rows);
+    }
+    return l;
+}
+
+int check_operand(const Args& a, const kda_decay_rows& r, const char* name) {
+    const int64_t es = a.dtype == KDA_DTYPE_BF16 ? 2 : 4;
+    if (!r.p || reinterpret_cast<uintptr_t>(r.p) % 16 != 0)
+        return api_fail(KDA_E_INVALID, "%s is NULL or not 16-byte aligned", name);
+    if ((r.batch * es) % 16 || (r.token * es) % 16 || (r.head * es) % 16)
+        return api_fail(KDA_E_INVALID, "%s: strides %lld, %lld, %lld are not whole 16-byte pieces", name, (long long)r.batch,
+                        (long long)r.token, (long long)r.head);
+    return KDA_OK;
+}
+int check_sizes(const Args& a) {
+    if (a.dtype != KDA_DTYPE_F32 && a.dtype != KDA_DTYPE_BF16)
+        return api_fail(KDA_E_UNSUPPORTED, "dtype=%lld: expected 0 (fp32) or 1 (bf16)", (long long)a.dtype);
+    if (a.D != 32 && a.D != 64 && a.D != 96 && a.D != 128)
+        return api_fail(KDA_E_UNSUPPORTED, "D=%lld: expected 32, 64, 96 or 128", (long long)a.D);
+    if (a.B < 0 || a.T < 0 || a.H < 1 || a.H > 65535 || a.B > 0x7fffffff || a.T > 0x7fffffff - 4096 || a.nseq < 0 ||
+        a.nseq > 0x7fffffff)
+        return api_fail(KDA_E_INVALID, "B=%lld T=%lld H=%lld nseq=%lld", (long long)a.B, (long long)a.T, (long long)a.H,
+                        (long long)a.nseq);
+    if (a.cu && a.B != 1) return api_fail(KDA_E_INVALID, "B=%lld: packed sequences are one row", (long long)a.B);
+    const kda_decay_rows* r[3] = {&a.q, &a.k, &a.v};
+    for (int i = 0; i < 3; ++i)
+        if (r[i]->heads < 1 || a.H % r[i]->heads != 0)
+            return api_fail(KDA_E_INVALID, "%c has %lld heads, which do not divide H=%lld", "qkv"[i], (long long)r[i]->heads,
+                            (long long)a.H);
+    return KDA_OK;
+}
+int check_ptr(const void* p, const char* name, int align) {
+    if (!p || reinterpret_cast<uintptr_t>(p) % align != 0)
+        return api_fail(KDA_E_INVALID, "%s is NULL or not %d-byte aligned", name, align);
+    return KDA_OK;
+}
+#define DEC_TRY(x)                       \
+    do {                                 \
+        const int rc_ = (x);             \
+        if (rc_ != KDA_OK) return rc_;   \
+    } while (0)
+#define DEC_HIP(x)                                                   \
+    do {                                                             \
+        const hipError_t e_ = (x);                                   \
+        if (e_ != hipSuccess) return api_hip_fail(e_, "kda_decay");  \
+    } while (0)
+
+Rows rows_of(const Args& a, const kda_decay_rows& r) { return {r.p, r.batch, r.token, r.head, (int)(a.H / r.heads)}; }
+
+DecayArgs base_of(const Args& a, const Plan& p, const Layout& l) {
+    DecayArgs d = {};
+    char* ws = static_cast<char*>(a.workspace);
+    d.g = a.g; d.gb = a.g_batch; d.gt = a.g_token; d.gh = a.g_head;
+    d.B = (int)a.B; d.T = (int)a.T; d.H = (int)a.H;
+    d.nseq = (int)(a.cu ? a.nseq : a.B);
+    d.nslots = p.nslots; d.per_seq = p.per_seq; d.seg_tokens = p.seg_tokens;
+    d.tab = p.packed ? reinterpret_cast<const int4*>(ws + l.tab) : nullptr;
+    d.in_by_slot = p.multi;
+    return d;
+}
+
+template <class K, typename OT, int NP, int NS, bool REV, bool STATES, bool DOT>
+hipError_t launch_mix(const DecayArgs& d, bool swapped, hipStream_t st) {
+    hipLaunchKernelGGL((kda_decay_mix_kernel<K, OT, NP, NS, REV, STATES, DOT>), dim3((unsigned)(d.nslots * d.H)), dim3(K::NTH), 0,
+                       st, d, swapped);
+    return hipGetLastError();
+}
+
+hipError_t launch_plan(const Args& a, const Plan& p, const Layout& l, hipStream_t st) {
+    char* ws = static_cast<char*>(a.workspace);
+    hipLaunchKernelGGL(kda_decay_plan_kernel, dim3(1), dim3(PLAN_TH), 0, st, a.cu, (int)a.nseq, (int)a.T, p.seg_tokens,
+                       reinterpret_cast<int4*>(ws + l.tab), reinterpret_cast<int*>(ws + l.first), p.nslots);
+    return hipGetLastError();
+}
+
+// the states at the slots' limits: s at their starts, or (REV) their adjoints at the ends
+template <class K, bool REV>
+hipError_t states(const Args& a, const Plan& p, const Layout& l, DecayArgs d, const float* s0, hipStream_t st) {
+    char* ws = static_cast<char*>(a.workspace);
+    d.s_out = reinterpret_cast<float*>(ws + (REV ? l.ds : l.s));
+    d.seg = reinterpret_cast<float*>(ws + (REV ? l.segd : l.seg));
+    const hipError_t e = launch_mix<K, float, 1, 1, REV, true, false>(d, false, st);
+    if (e != hipSuccess || d.nseq == 0) return e;
+    const int DD = K::D * K::D, parts = (DD / 4 + 255) / 256;
+    hipLaunchKernelGGL(kda_decay_scan_kernel<REV>, dim3((unsigned)(d.nseq * d.H * parts)), dim3(256), 0, st, d.s_out, d.seg, s0,
+                       p.packed ? reinterpret_cast<const int*>(ws + l.first) : nullptr, p.per_seq, d.H, DD, parts);
+    return hipGetLastError();
+}
+
+template <typename OT>
+hipError_t launch_group(const float* src, void* dst, const Args& a, const kda_decay_rows& r, hipStream_t st) {
+    const int64_t n4 = a.B * a.T * r.heads * a.D / 4;
+    if (n4 == 0) return hipSuccess;
+    hipLaunchKernelGGL(kda_decay_group_kernel<OT>, dim3((unsigned)std::min<int64_t>((n4 + 255) / 256, 8192)), dim3(256), 0, st, src,
+                       static_cast<OT*>(dst), n4, (int)(a.H / r.heads), (int)a.D);
+    return hipGetLastError();
+}
+
+// Planes of the pairs' products and of the state in bf16's products with it: two make
+// what is lost there small beside the output's own rounding.
+template <int D, bool F32>
+int forward(const Args& a, hipStream_t st) {
+    typedef Cfg<D, F32, F32 ? 32 : 64> K;
+    constexpr int NP = F32 ? 3 : 2;
+    const Plan p = plan_of(a, false);
+    const Layout l = layout_of(a, p, false);
+    DecayArgs d = base_of(a, p, l);
+    if (p.packed) DEC_HIP(launch_plan(a, p, l, st));
+    if (p.multi) {
+        DecayArgs m = d;
+        m.y = rows_of(a, a.k);
+        m.w = rows_of(a, a.v);
+        DEC_HIP((states<K, false>(a, p, l, m, a.s0, st)));
+    }
+    d.x = rows_of(a, a.q);
+    d.y = rows_of(a, a.k);
+    d.w = rows_of(a, a.v);
+    d.out = a.o;
+    d.s_in = p.multi ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + l.s) : a.s0;
+    d.s_out = a.s_final;
+    DEC_HIP((launch_mix<K, typename K::ST, NP, NP, false, false, false>(d, false, st)));
+    return KDA_OK;
+}
+
+template <class K, typename OT, int NP, bool DOT>
+hipError_t launch_mix2(const DecayArgs& d, hipStream_t st) {
+    hipLaunchKernelGGL((kda_decay_mix2_kernel<K, OT, NP, DOT ? 3 : NP, DOT>), dim3((unsigned)(d.nslots * d.H)), dim3(K::NTH), 0, st,
+                       d);
+    return hipGetLastError();
+}
+
+template <int D, bool F32, bool DOT>
+int backward(const Args& a, hipStream_t st) {
+    typedef Cfg<D, F32, F32 ? 32 : 64> K;
+    typedef Cfg<D, F32, (F32 || D > 64) ? 32 : 64> K2;   // four operands in LDS
+    typedef typename K::ST ST;
+    typedef typename std::conditional<DOT, K2, K>::type K1;   // dg: the same chunks in both
+    constexpr int NP = F32 ? 3 : 2;
+    const Plan p = plan_of(a, DOT);
+    const Layout l = layout_of(a, p, true);
+    char* ws = static_cast<char*>(a.workspace);
+    const DecayArgs base = base_of(a, p, l);
+    const Rows q = rows_of(a, a.q), k = rows_of(a, a.k), v = rows_of(a, a.v);
+    kda_decay_rows dout = a.dout;
+    dout.heads = a.H;
+    const Rows o = rows_of(a, dout);
+    float* starts = p.multi ? reinterpret_cast<float*>(ws + l.s) : nullptr;
+    float* dends = p.multi ? reinterpret_cast<float*>(ws + l.ds) : nullptr;
+    float* dots = DOT ? reinterpret_cast<float*>(ws + l.dots) : nullptr;
+    float *g0 = l.g0 >= 0 ? reinterpret_cast<float*>(ws + l.g0) : nullptr,
+          *g1 = l.g1 >= 0 ? reinterpret_cast<float*>(ws + l.g1) : nullptr;
+    if (p.packed) DEC_HIP(launch_plan(a, p, l, st));
+    if (p.multi) {
+        DecayArgs m = base;
+        m.y = k; m.w = v;
+        DEC_HIP((states<K, false>(a, p, l, m, a.s0, st)));
+        m.y = q; m.w = o;
+        DEC_HIP((states<K, true>(a, p, l, m, a.ds_final, st)));
+    }
+    DecayArgs d = base;
+    d.x = o; d.y = v; d.w = k; d.z = q;
+    d.s_in = p.multi ? starts : a.s0;
+    d.dots = dots;
+    d.out = shared(a, a.q) ? g0 : a.dq;
+    if (shared(a, a.q)) {
+        DEC_HIP((launch_mix<K1, float, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
+        DEC_HIP(launch_group<ST>(g0, a.dq, a, a.q, st));
+    } else {
+        DEC_HIP((launch_mix<K1, ST, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
+    }
+    d = base;
+    d.x = k; d.y = q; d.z = v; d.w = o;
+    d.s_in = p.multi ? dends : a.ds_final;
+    d.s_out = a.ds0;
+    d.dots = dots;
+    d.dots2 = DOT ? dots + a.H * a.B * a.T : nullptr;
+    d.anchors = DOT ? reinterpret_cast<float*>(ws + l.anchors) : nullptr;
+    if (shared(a, a.k) || shared(a, a.v)) {
+        d.out = g0; d.out2 = g1;
+        DEC_HIP((launch_mix2<K2, float, NP, DOT>(d, st)));
+        DEC_HIP(launch_group<ST>(g0, a.dk, a, a.k, st));
+        DEC_HIP(launch_group<ST>(g1, a.dv, a, a.v, st));
+    } else {
+        d.out = a.dk; d.out2 = a.dv;
+        DEC_HIP((launch_mix2<K2, ST, NP, DOT>(d, st)));
+    }
+    if constexpr (DOT) {
+        d = base;
+        d.dots = dots;
+        d.dots2 = dots + a.H * a.B * a.T;
+        d.anchors = reinterpret_cast<float*>(ws + l.anchors);
+        double* sums = a.dg_heads ? reinterpret_cast<double*>(ws + l.sums) : nullptr;
+        hipLaunchKernelGGL(kda_decay_dg_kernel, dim3((unsigned)(d.nslots * d.H)), dim3(DG_TH), 0, st, d, starts, dends, a.s_final,
+                           a.ds_final, sums ? nullptr : a.dg, sums, D * D, K1::C);
+        DEC_HIP(hipGetLastError());
+        if (sums) {
+            hipLaunchKernelGGL(kda_decay_dg_sum_kernel, dim3((unsigned)d.H), dim3(64), 0, st, sums, a.dg, d.nslots, d.H);
+            DEC_HIP(hipGetLastError());
+        }
+    }
+    return KDA_OK;
+}
+
+template <int D>
+int forward_of(const Args& a, hipStream_t st) {
+    return a.dtype == KDA_DTYPE_F32 ? forward<D, true>(a, st) : forward<D, false>(a, st);
+}
+template <int D>
+int backward_of(const Args& a, hipStream_t st) {
+    if (a.dg) return a.dtype == KDA_DTYPE_F32 ? backward<D, true, true>(a, st) : backward<D, false, true>(a, st);
+    return a.dtype == KDA_DTYPE_F32 ? backward<D, true, false>(a, st) : backward<D, false, false>(a, st);
+}
+
+template <int D>
+hipError_t launch_step(const StepArgs& a, bool f32, hipStream_t st) {
+    const dim3 grid((unsigned)(((int64_t)a.B * a.H * StepCfg<D>::PARTS + 3) / 4));
+    if (f32) hipLaunchKernelGGL((kda_decay_step_kernel<D, float>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kda_decay_step_kernel<D, uint16_t>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+int check_common(const Args& a, bool bwd) {
+    DEC_TRY(check_sizes(a));
+    const Plan p = plan_of(a, bwd && a.dg);
+    if (p.nslots < 0) return api_fail(KDA_E_UNSUPPORTED, "B=%lld T=%lld H=%lld: too many workgroups", (long long)a.B, (long long)a.T, (long long)a.H);
+    if (a.B * a.T > 0) {
+        DEC_TRY(check_operand(a, a.q, "q"));
+        DEC_TRY(check_operand(a, a.k, "k"));
+        DEC_TRY(check_operand(a, a.v, "v"));
+        DEC_TRY(check_ptr(a.g, "g", 4));
+    }
+    if (a.cu) DEC_TRY(check_ptr(a.cu, "cu", 4));
+    if (a.s0) DEC_TRY(check_ptr(a.s0, "s0", 16));
+    const int64_t need = layout_of(a, p, bwd).bytes;
+    if (need) {
+        DEC_TRY(check_ptr(a.workspace, "workspace", 16));
+        if (a.ws_bytes < need)
+            return api_fail(KDA_E_WORKSPACE, "workspace has %lld bytes, needs %lld", (long long)a.ws_bytes, (long long)need);
+    }
+    return KDA_OK;
+}
+
+}  // namespace
+
+}  // namespace kda
+
+using namespace kda;
+
+extern "C" {
+
+size_t kda_decay_workspace_size(int pass, const kda_decay_args* args) {
+    if (!args || check_sizes(*args) != KDA_OK) return 0;
+    const bool bwd = pass == KDA_PASS_BWD;
+    const Plan p = plan_of(*args, bwd && args->dg);
+    return p.nslots < 0 ? 0 : (size_t)layout_of(*args, p, bwd).bytes;
+}
+
+int kda_decay_fwd(const kda_decay_args* args, void* stream) {
+    if (!args) return api_fail(KDA_E_INVALID, "args is NULL");
+    const Args& a = *args;
+    DEC_TRY(check_common(a, false));
+    if (a.B * a.T > 0) DEC_TRY(check_ptr(a.o, "o", 16));
+    if (a.s_final) DEC_TRY(check_ptr(a.s_final, "s_final", 16));
+    if (a.B == 0) return KDA_OK;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (a.D) {
+        case 32: return forward_of<32>(a, st);
+        case 64: return forward_of<64>(a, st);
+        case 96: return forward_of<96>(a, st);
+        default: return forward_of<128>(a, st);
+    }
+}
+
+int kda_decay_bwd(const kda_decay_args* args, void* stream) {
+    if (!args) return api_fail(KDA_E_INVALID, "args is NULL");
+    const Args& a = *args;
+    DEC_TRY(check_common(a, true));
+    if (a.B * a.T > 0) {
+        DEC_TRY(check_operand(a, a.dout, "dout"));
+        DEC_TRY(check_ptr(a.dq, "dq", 16));
+        DEC_TRY(check_ptr(a.dk, "dk", 16));
+        DEC_TRY(check_ptr(a.dv, "dv", 16));
+    }
+    if (a.ds_final) DEC_TRY(check_ptr(a.ds_final, "ds_final", 16));
+    if (a.ds0) DEC_TRY(check_ptr(a.ds0, "ds0", 16));
+    if (a.dg) {
+        DEC_TRY(check_ptr(a.dg, "dg", 4));
+        if (a.ds_final) DEC_TRY(check_ptr(a.s_final, "s_final (of the forward pass, for dg)", 16));
+    }
+    if (a.B == 0) return KDA_OK;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (a.D) {
+        case 32: return backward_of<32>(a, st);
+        case 64: return backward_of<64>(a, st);
+        case 96: return backward_of<96>(a, st);
+        default: return backward_of<128>(a, st);
+    }
+}
+
+int kda_decay_step(const kda_decay_args* args, const int32_t* slots, int64_t states, void* stream) {
+    if (!args) return api_fail(KDA_E_INVALID, "args is NULL");
+    const Args& a = *args;
+    DEC_TRY(check_sizes(a));
+    if (a.cu || a.T != 1) return api_fail(KDA_E_INVALID, "T=%lld: a step takes one token of each row", (long long)a.T);
+    if (a.B == 0) return KDA_OK;
+    if (states < 0 || states > 0x7fffffff || (!slots && states != a.B))
+        return api_fail(KDA_E_INVALID, "%lld states for %lld rows", (long long)states, (long long)a.B);
+    if (a.B * a.H > (1 << 28)) return api_fail(KDA_E_UNSUPPORTED, "B=%lld H=%lld: too many workgroups", (long long)a.B, (long long)a.H);
+    DEC_TRY(check_operand(a, a.q, "q"));
+    DEC_TRY(check_operand(a, a.k, "k"));
+    DEC_TRY(check_operand(a, a.v, "v"));
+    DEC_TRY(check_ptr(a.g, "g", 4));
+    DEC_TRY(check_ptr(a.o, "o", 16));
+    if (states) DEC_TRY(check_ptr(a.s0, "s0", 16));
+    if (slots) DEC_TRY(check_ptr(slots, "slots", 4));
+    StepArgs d = {};
+    d.q = rows_of(a, a.q); d.k = rows_of(a, a.k); d.v = rows_of(a, a.v);
+    d.g = a.g; d.gb = a.g_batch; d.gh = a.g_head;
+    d.s = const_cast<float*>(a.s0); d.slots = slots; d.o = a.o;
+    d.B = (int)a.B; d.H = (int)a.H; d.N = (int)states;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool f32 = a.dtype == KDA_DTYPE_F32;
+    switch (a.D) {
+        case 32: DEC_HIP(launch_step<32>(d, f32, st)); break;
+        case 64: DEC_HIP(launch_step<64>(d, f32, st)); break;
+        case 96: DEC_HIP(launch_step<96>(d, f32, st)); break;
+        default: DEC_HIP(launch_step<128>(d, f32, st));
+    }
+    return KDA_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,159 @@
+"""Rotary positions with several axes on MI355X: ``rotary``.
+
+Channels in pairs (x, y) are turned by the angle of their axis' position and their own
+frequency, x' = x cos - y sin, y' = x sin + y cos, for queries and keys in one launch.
+A token of a video has three axes, time, height and width, each with a section of the
+channels; ``grid`` numbers tokens as ``TubeletEmbedding3D`` lays them out
+(nope_gdn_mlx.py:98-150: frame by frame, rows of a frame, tokens of a row).  The
+reference's model has no positions; this is for what is built beside it.
+
+Angles are formed in fp64 (at a position p they are within 2^-52 p), rows in fp32 and
+rounded once.  Differentiable in q and k, by turning back; a second derivative and tracing are
+refused.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import math
+from array import array
+from functools import lru_cache
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .kda import _DTYPE_CODE
+from .linear import _grad_enabled, _is_tracing, _on, _raw_stream
+
+MAX_HEAD_DIM, MAX_AXES, MAX_TOKENS = 256, 4, (1 << 31) - 1
+_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+@lru_cache(maxsize=64)
+def _turns(sections: Tuple[int, ...], base: float) -> array:
+    """Turns a unit of position of every pair: base^(-2 i / section) / 2 pi."""
+    return array("d", [base ** (-2 * i / s) / (2 * math.pi) for s in sections for i in range(s // 2)])
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _rows(t: Optional[torch.Tensor]):
+    return (0, 0, 0, 0, 1) if t is None else (t.data_ptr(), *t.stride()[:3], t.shape[2])
+
+
+def _turn(q, k, how, sign: int):
+    """Queries and keys (either may be None) turned by ``how``, sign -1: back."""
+    positions, strides, grid, start, sections, base, interleaved = how
+    first = q if k is None or q is not None else k
+    B, T, _, D = first.shape
+    dev = first.device
+    with _on(dev):
+        q, k = (None if t is None else _unit(t) for t in (q, k))
+        out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k)]
+        ins, outs = (q, k) if q is not None else (k, None), out if q is not None else (out[1], None)
+        turns = _turns(sections, base)
+        args = array("q", [*_rows(ins[0]), *_rows(ins[1]), *(0 if t is None else t.data_ptr() for t in outs),
+                           *((0, 0, 0, 0, 0) if positions is None else (positions.data_ptr(), _POSITIONS[positions.dtype], *strides)),
+                           *grid, start, len(sections), *sections, *([0] * (MAX_AXES - len(sections))),
+                           turns.buffer_info()[0], int(interleaved), sign, B, T, D, _DTYPE_CODE[first.dtype]])
+        rc = _lib.load().kda_rotary(args.buffer_info()[0], _raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, "kda_rotary")
+    return out
+
+
+class RotaryFunction(torch.autograd.Function):
+    """``rotary`` as one node; keeps the positions."""
+
+    @staticmethod
+    def forward(ctx, q, k, how):
+        ctx.save_for_backward(how[0])
+        ctx.how = how[1:]
+        ctx.set_materialize_grads(False)
+        y = _turn(q, k, how, 1)
+        return y[0] if k is None else tuple(y)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        dq, dk = (d if need else None for d, need in zip((dq, dk), ctx.needs_input_grad))
+        if dq is None and dk is None:
+            return None, None, None
+        return (*_turn(dq, dk, (*ctx.saved_tensors, *ctx.how), -1), None)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, *,
+           grid: Optional[Tuple[int, int]] = None, start: int = 0, sections: Optional[Sequence[int]] = None,
+           base: float = 10000.0, interleaved: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """q (B, T, heads, D) and k (B, T, heads, D), bf16 or fp32, turned by their tokens' positions,
+    differentiable.  Returns q', or (q', k') with k.
+
+    ``positions``: (T,), (axes, T) or (axes, B, T), int32, int64 or fp32, on the same device; or
+    ``grid`` = (height, width), the tokens of a frame: token t is number n = start + t of its
+    video, with positions n // (height width), n // width % height and n % width.
+    ``sections``: the channels of each axis, even, in order (default: all for one axis); channels
+    behind them stay as they are.  Pair i of an axis with s channels turns by base^(-2 i / s) a
+    position; its channels are i and s / 2 + i of the section, or with ``interleaved`` 2 i and
+    2 i + 1.  D even, at most 256, at most 4 axes; any strides."""
+    what = "rotary"
+    if not isinstance(q, torch.Tensor) or not (k is None or isinstance(k, torch.Tensor)):
+        raise TypeError("rotary: q and k must be torch.Tensors")
+    if q.dim() != 4:
+        raise ValueError(f"{what}: q must be (B, T, heads, D); got shape {tuple(q.shape)}")
+    B, T, heads, D = q.shape
+    if q.dtype not in _DTYPE_CODE:
+        raise ValueError(f"{what}: q dtype {q.dtype} unsupported: use float32 or bfloat16")
+    if D < 2 or D % 2 or D > MAX_HEAD_DIM or heads < 1:
+        raise ValueError(f"{what}: {heads} heads of head_dim={D}: expected an even number up to {MAX_HEAD_DIM}")
+    if B * T > MAX_TOKENS:
+        raise ValueError(f"{what}: q of shape {tuple(q.shape)} has more than {MAX_TOKENS} tokens")
+    dev = q.device
+    if k is not None:
+        if k.dim() != 4 or k.shape[:2] != (B, T) or k.shape[3] != D or k.shape[2] < 1:
+            raise ValueError(f"{what}: k shape {tuple(k.shape)} does not match q's {tuple(q.shape)}")
+        if k.dtype != q.dtype:
+            raise ValueError(f"{what}: k has dtype {k.dtype}; expected {q.dtype}")
+        if k.device != dev:
+            raise ValueError(f"{what}: k is on {k.device}, q on {dev}")
+    sections = (D,) if sections is None else tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= MAX_AXES or any(s < 0 or s % 2 for s in sections) or sum(sections) > D:
+        raise ValueError(f"{what}: sections={sections}: expected 1 to {MAX_AXES} even numbers that make up at most {D}")
+    base = float(base)
+    if not 0.0 < base < math.inf:
+        raise ValueError(f"{what}: base={base}: expected a positive number")
+    strides = None
+    if (positions is None) == (grid is None):
+        raise ValueError(f"{what}: expected either positions or grid")
+    if grid is not None:
+        grid = tuple(int(n) for n in grid)
+        if len(grid) != 2 or min(grid) < 1 or max(grid) >= 1 << 31 or len(sections) > 3 or not 0 <= start < 1 << 62:
+            raise ValueError(f"{what}: grid={grid}, start={start} with {len(sections)} sections: expected (height, width), "
+                             "start >= 0 and at most 3 axes")
+    else:
+        if not isinstance(positions, torch.Tensor):
+            raise TypeError("rotary: positions must be a torch.Tensor")
+        if start:
+            raise ValueError(f"{what}: start={start} goes with grid, not with positions")
+        shape, n = tuple(positions.shape), len(sections)
+        if shape not in ((n, T), (n, B, T)) and not (n == 1 and shape == (T,)):
+            raise ValueError(f"{what}: positions shape {shape}: expected ({n}, {T}) or ({n}, {B}, {T})")
+        if positions.dtype not in _POSITIONS:
+            raise ValueError(f"{what}: positions dtype {positions.dtype} unsupported: use int32, int64 or float32")
+        if positions.device != dev:
+            raise ValueError(f"{what}: positions is on {positions.device}, q on {dev}")
+        if positions.requires_grad and _grad_enabled():
+            raise ValueError(f"{what} has no gradient for positions")
+        s = positions.stride()
+        strides = (0, 0, s[0]) if len(s) == 1 else (s[0], 0, s[1]) if len(s) == 2 else s
+    if dev.type != "cuda":
+        raise ValueError(f"{what} runs on a ROCm device; got tensors on {dev}")
+    if _is_tracing():
+        raise RuntimeError(f"{what} cannot be traced: its launches are no part of a traced graph")
+    how = positions, strides, grid or (1, 1), int(start), sections, base, bool(interleaved)
+    if _grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or forward_ad._current_level >= 0:
+        return RotaryFunction.apply(q, k, how)
+    y = _turn(q, k, how, 1)
+    return y[0] if k is None else tuple(y)
