@@ -419,7 +419,7 @@ int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const 
  *   S_t = e^{g_t} S_{t-1} + v_t k_t^T,   o_t = S_t q_t
  * for H heads of D = 32, 64, 96 or 128 channels, S [H][D][D] fp32 as S[i_v][j_k].
  * q, k, v, dout: [B][T][heads][D] of dtype (fp32 or bf16), strides in elements, unit
- * channel stride, pointers and strides whole 16-byte pieces; q, k and v may have
+ * channel stride, pointers and strides whole 16-byte pieces, token strides up to 2^24; q, k and v may have
  * fewer heads than H, which each serve H / heads heads of the state in a row (dout: H).
  * g: fp32 log-decays with strides of their own (0: shared); below -200 as -200, whose
  * e^g is zero.  s0, s_final, ds_final, ds0 [sequences][H][D][D] fp32, each may be NULL.
@@ -431,7 +431,7 @@ int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const 
  * Sums and states are fp32; in bf16 the pairs' weights and the state enter the products
  * with 16 bits of mantissa.  What a token gets from itself alone (T = 1, no s0) has a dg
  * of exactly zero.  A value that is not finite reaches every output of its sequence from its
- * block of 64 tokens on (in a gradient: up to it).
+ * block of 32 tokens on (in a gradient: up to it).
  * Backward: gradients of <o, dout> + <s_final, ds_final>; reads s_final only for dg
  * beside ds_final.  Nothing else is kept between the calls.  workspace: at least
  * kda_decay_workspace_size(KDA_PASS_FWD or KDA_PASS_BWD, args) bytes for these sizes, heads, cu,

@@ -95,38 +95,66 @@ __device__ __forceinline__ void planes8(const float* v, bf16x8 (&f)[N]) {
     for (int i = 0; i < N; ++i) f[i] = __builtin_bit_cast(bf16x8, make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]));
 }
 
-// bf16 operands are one plane, fp32 ones three.  Tiles [C][LD] of bf16 a plane in
-// LDS, rows 16 bytes mod 128 apart.
-template <int D_, bool F32_, int C_>
-struct Cfg {
-    static constexpr int D = D_, C = C_, NPL = F32_ ? 3 : 1, NW = D / 16, NTH = 64 * NW, LD = D + 8, LP = C + 8;
-    static constexpr int PLANE = C * LD, TILE = NPL * PLANE, PPL = C * LP, TT = C / 16, NT = TT * (TT + 1) / 2, DT = D / 16,
-                         KD = D / 32, KC = C / 32;
-    static constexpr bool F32 = F32_;
-    typedef typename std::conditional<F32_, float, uint16_t>::type ST;
-    static constexpr int ES = (int)sizeof(ST), VPR = D * ES / 16, NV = C * VPR, PER = NV / NTH;
-    static_assert(NV % NTH == 0 && C % 32 == 0 && D % 32 == 0, "whole pieces");
+// Tiles of rows in LDS, RB bytes each: 16-byte piece c of row r lies at c ^ key(r), so that
+// neither eight rows' reads of one piece nor a transposing read's four rows of two
+// pieces meet in a bank (with fewer than eight pieces to a row and its neighbour's: two bits).
+template <int RB>
+struct Sw {
+    __device__ __forceinline__ static int key(int r) {
+        return RB % 128 == 0 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
+    }
+    __device__ __forceinline__ static int at(int r, int c) { return r * RB + ((c ^ key(r)) << 4); }
+    // at(r, 4 k + q), q < 4, with k's part as a constant where k is one
+    __device__ __forceinline__ static int at(int r, int q, int k) {
+        const int o = r * RB + ((q ^ (key(r) & 3)) << 4);
+        return RB % 128 == 0 ? o + (((k & 1) ^ ((r >> 1) & 1)) << 6) + 64 * (k & ~1) : o + 64 * k;
+    }
 };
 
-// C rows on their way from memory to LDS
+// C tokens a chunk; a wave has CW tiles of 16 of W's channels (with two the LDS reads of
+// a chunk are half as many, but 65536 x 12 x 64 took 190 us instead of 175: too few
+// waves).  bf16 operands are one plane, fp32 ones three.  OCC: waves a SIMD that mix and
+// mix2 are held to.
+template <int D_, bool F32_, int C_ = 32, int CW_ = 1>
+struct Cfg {
+    static constexpr int D = D_, C = C_, CW = CW_, NPL = F32_ ? 3 : 1, NW = D / (16 * CW), NTH = 64 * NW;
+    static constexpr int RB = 2 * D, PLANE = C * RB, TILE = NPL * PLANE;    // bytes
+    static constexpr int RP = 2 * C, PPL = C * RP;                          // of the pairs'
+    static constexpr int TT = C / 16, NT = TT * (TT + 1) / 2, DT = D / 16, KD = D / 32, KC = C / 32;
+    static constexpr int OCC = F32_ ? 1 : 4, OCC2 = F32_ ? 1 : D > 64 ? 2 : 3;
+    static constexpr bool F32 = F32_;
+    typedef typename std::conditional<F32_, float, uint16_t>::type ST;
+    static constexpr int ES = (int)sizeof(ST), EPV = 16 / ES, VPR = D / EPV, NV = C * VPR, PER = NV / NTH;
+    static_assert(NV % NTH == 0 && C % 32 == 0 && D % (16 * CW) == 0, "whole pieces");
+};
+// the channel of W that row m of tile c of wave w stands for: two tiles' four rows are
+// eight channels in a row
 template <class K>
+__device__ __forceinline__ int channel(int w, int c, int m) {
+    return K::CW == 2 ? 32 * w + 8 * (m >> 2) + 4 * c + (m & 3) : 16 * w + m;
+}
+
+// C rows on their way from memory to LDS, forwards or backwards in time
+template <class K, bool REV>
 struct Stage {
     uint4 r[K::PER];
-    // row i at p + i * step; those from n (>= 1) on read the last and are stored as zeros
-    __device__ __forceinline__ void load(const typename K::ST* p, int64_t step, int n) {
+    // n >= 1 rows, the first in memory at p, `step` bytes apart; what is behind them reads the last
+    __device__ __forceinline__ void load(const typename K::ST* p, uint32_t step, int n) {
 #pragma unroll
         for (int i = 0; i < K::PER; ++i) {
-            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = (v - row * K::VPR) * (16 / K::ES);
-            r[i] = *reinterpret_cast<const uint4*>(p + min(row, n - 1) * step + c);
+            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = v - row * K::VPR, m = min(row, n - 1);
+            r[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + ((uint32_t)(REV ? n - 1 - m : m) * step + 16 * c));
         }
     }
-    __device__ __forceinline__ void store(uint16_t* t, int n) const {
+    // ... and is stored as zeros
+    __device__ __forceinline__ void store(char* t, int n) const {
 #pragma unroll
         for (int i = 0; i < K::PER; ++i) {
-            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = (v - row * K::VPR) * (16 / K::ES);
-            const uint4 x = row < n ? r[i] : make_uint4(0u, 0u, 0u, 0u);
+            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = v - row * K::VPR;
+            uint4 x = r[i];
+            if (n < K::C) x = row < n ? x : make_uint4(0u, 0u, 0u, 0u);
             if constexpr (!K::F32) {
-                *reinterpret_cast<uint4*>(t + row * K::LD + c) = x;
+                *reinterpret_cast<uint4*>(t + Sw<K::RB>::at(row, c)) = x;
             } else {
                 // each part the next 8 bits of 24, cut off, so that nothing overflows
                 const uint32_t b[4] = {x.x, x.y, x.z, x.w};
@@ -139,7 +167,7 @@ struct Stage {
                     l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
                 }
                 constexpr uint32_t HI = 0x07060302u;
-                uint16_t* q = t + row * K::LD + c;
+                char* q = t + Sw<K::RB>::at(row, c >> 1) + 8 * (c & 1);
                 *reinterpret_cast<uint2*>(q) =
                     make_uint2(__builtin_amdgcn_perm(h[1], h[0], HI), __builtin_amdgcn_perm(h[3], h[2], HI));
                 *reinterpret_cast<uint2*>(q + K::PLANE) =
@@ -151,22 +179,39 @@ struct Stage {
     }
 };
 
-// fragments of a tile's planes: rows contiguous (c: the matrix unit's own order of
-// the contracted index), in the order of accumulators, and transposed
-template <class K>
-__device__ __forceinline__ void rows_c(const uint16_t* t, int row0, int k0, bf16x8 (&f)[K::NPL]) {
+// Fragments, the contracted index in the matrix unit's own order (lane l has 8 (l / 16) ..
+// + 7 of 32).  Along the rows:
+template <int RB, int NPL, int PLANE>
+__device__ __forceinline__ void along(const char* t, int row0, int k, bf16x8 (&f)[NPL]) {
+    const int l = lane_id(), o = Sw<RB>::at(l & 15, l >> 4, k);
 #pragma unroll
-    for (int p = 0; p < K::NPL; ++p) f[p] = ldfrag_c<1, uint16_t>(t + p * K::PLANE, K::LD, row0, k0).h;
+    for (int p = 0; p < NPL; ++p)
+        f[p] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(t + p * PLANE + row0 * RB + o));
+}
+// and across them: 16 columns of rows 32 k .., the p-th four of them at o0 (o1: four rows on)
+template <class K>
+__device__ __forceinline__ void across(const char* t, int k, int o0, int o1, bf16x8 (&f)[K::NPL]) {
+#pragma unroll
+    for (int p = 0; p < K::NPL; ++p) {
+        const char* u = t + p * K::PLANE + 32 * k * K::RB;
+        f[p] = cat4(ld_tr4(reinterpret_cast<const uint16_t*>(u + o0)), ld_tr4(reinterpret_cast<const uint16_t*>(u + o1)));
+    }
+}
+// of W: tile c of the wave's; of Y: tile j, every other four of 32 channels
+template <class K>
+__device__ __forceinline__ void w_frag(const char* W, int k, int c, bf16x8 (&f)[K::NPL]) {
+    const int l = lane_id(), j = l & 15, row = 8 * (l >> 4) + (j >> 2), w = (int)(threadIdx.x >> 6);
+    if constexpr (K::CW == 2) {
+        across<K>(W, k, Sw<K::RB>::at(row, 4 * w + (j & 3)) + 8 * c, Sw<K::RB>::at(row + 4, 4 * w + (j & 3)) + 8 * c, f);
+    } else {
+        const int piece = 2 * w + ((j & 3) >> 1), b = 8 * (j & 1);
+        across<K>(W, k, Sw<K::RB>::at(row, piece) + b, Sw<K::RB>::at(row + 4, piece) + b, f);
+    }
 }
 template <class K>
-__device__ __forceinline__ void rows_k(const uint16_t* t, int row0, int k0, bf16x8 (&f)[K::NPL]) {
-#pragma unroll
-    for (int p = 0; p < K::NPL; ++p) f[p] = ldfrag<1, uint16_t>(t + p * K::PLANE, K::LD, row0, k0).h;
-}
-template <class K>
-__device__ __forceinline__ void cols_k(const uint16_t* t, int n0, int k0, bf16x8 (&f)[K::NPL]) {
-#pragma unroll
-    for (int p = 0; p < K::NPL; ++p) f[p] = ldfragT(t + p * K::PLANE, K::LD, n0, k0).h;
+__device__ __forceinline__ void y_frag(const char* Y, int k, int t, bf16x8 (&f)[K::NPL]) {
+    const int l = lane_id(), j = l & 15, row = 8 * (l >> 4) + (j >> 2);
+    across<K>(Y, k, Sw<K::RB>::at(row, j & 3, t >> 1) + 8 * (t & 1), Sw<K::RB>::at(row + 4, j & 3, t >> 1) + 8 * (t & 1), f);
 }
 
 // A chunk's decays.  Sums of g are formed in fp64 (a difference of two sums of
@@ -175,25 +220,32 @@ __device__ __forceinline__ void cols_k(const uint16_t* t, int n0, int k0, bf16x8
 template <int C>
 struct Decays {
     float hi[C], lo[C], up[C], down[C];   // G_t; 2^{G_t}; 2^{G_C - G_t}
-    float all;                            // 2^{G_C}
+    float all, pad[3];                    // 2^{G_C}
 };
 constexpr double LOG2E = 1.4426950408889634;
 // e^-200 is zero in fp32, as e^-inf is, and its sums stay finite
 constexpr float G_MIN = -200.f;
-
 __device__ __forceinline__ float decay(float g) { return expf(g < G_MIN ? G_MIN : g); }
 
-// by one wave: lane r has g of row r (0 behind the last)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double x) {   // 0 where there is no source lane
+    const uint2 u = __builtin_bit_cast(uint2, x);
+    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_update_dpp(0, u.x, CTRL, ROWS, 0xf, true),
+                                                 __builtin_amdgcn_update_dpp(0, u.y, CTRL, ROWS, 0xf, true)));
+}
+// by one wave: lane r has g of row r (0 behind the last); returns G_C
 template <int C>
 __device__ __forceinline__ double fill_decays(Decays<C>* d, float g) {
+    static_assert(C == 32, "two rows of 16 lanes");
     const int l = lane_id();
     double x = (double)(g < G_MIN ? G_MIN : g) * LOG2E;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const double y = __shfl_up(x, k, 64);
-        if (l >= k) x += y;
-    }
-    const double all = __shfl(x, C - 1, 64);
+    x += dpp<0x111, 0xf>(x);   // row_shr:1, 2, 4, 8
+    x += dpp<0x112, 0xf>(x);
+    x += dpp<0x114, 0xf>(x);
+    x += dpp<0x118, 0xf>(x);
+    x += dpp<0x142, 0xa>(x);   // row_bcast:15, into rows 1 and 3
+    const uint2 u = __builtin_bit_cast(uint2, x);
+    const double all = __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(u.x, 31), __builtin_amdgcn_readlane(u.y, 31)));
     if (l < C) {
         const float h = (float)x;
         d->hi[l] = h;
@@ -203,10 +255,6 @@ __device__ __forceinline__ double fill_decays(Decays<C>* d, float g) {
         if (l == C - 1) d->all = d->up[l];
     }
     return all;
-}
-template <int C>
-__device__ __forceinline__ float between(const Decays<C>& d, int t, int s) {
-    return __builtin_amdgcn_exp2f((d.hi[t] - d.hi[s]) + (d.lo[t] - d.lo[s]));
 }
 
 // tile id of the lower triangle -> (row of tiles, column)
@@ -218,13 +266,13 @@ __device__ __forceinline__ void tile_of(int id, int& ti, int& si) {
 // raw products of X's rows of tile ti with Y's of tile si: lane (c = l % 16, r = l / 16)
 // has X row 16 ti + c with Y rows 16 si + 4 r + i
 template <class K>
-__device__ __forceinline__ f32x4 pair_tile(const uint16_t* X, const uint16_t* Y, int ti, int si) {
+__device__ __forceinline__ f32x4 pair_tile(const char* X, const char* Y, int ti, int si) {
     f32x4 acc = zero4();
 #pragma unroll
     for (int k = 0; k < K::KD; ++k) {
         bf16x8 y[K::NPL], x[K::NPL];
-        rows_c<K>(Y, 16 * si, 32 * k, y);
-        rows_c<K>(X, 16 * ti, 32 * k, x);
+        along<K::RB, K::NPL, K::PLANE>(Y, 16 * si, k, y);
+        along<K::RB, K::NPL, K::PLANE>(X, 16 * ti, k, x);
         acc = mmp(y, x, acc);
     }
     return acc;
@@ -232,16 +280,19 @@ __device__ __forceinline__ f32x4 pair_tile(const uint16_t* X, const uint16_t* Y,
 template <class K>
 __device__ __forceinline__ f32x4 mask_tile(const Decays<K::C>& d, int ti, int si) {
     const int l = lane_id(), t = 16 * ti + (l & 15), s0 = 16 * si + 4 * (l >> 4);
+    const float h = d.hi[t], o = d.lo[t];
+    const float4 hs = *reinterpret_cast<const float4*>(d.hi + s0), ls = *reinterpret_cast<const float4*>(d.lo + s0);
+    const float hv[4] = {hs.x, hs.y, hs.z, hs.w}, lv[4] = {ls.x, ls.y, ls.z, ls.w};
     f32x4 m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = s0 + i <= t ? between(d, t, s0 + i) : 0.f;
+    for (int i = 0; i < 4; ++i) m[i] = s0 + i <= t ? __builtin_amdgcn_exp2f((h - hv[i]) + (o - lv[i])) : 0.f;
     return m;
 }
 // a tile of NP planes into P[t][s]
 template <class K, int NP>
-__device__ __forceinline__ void put_pair(uint16_t* P, const f32x4& v, int ti, int si) {
-    const int l = lane_id();
-    uint16_t* p = P + (16 * ti + (l & 15)) * K::LP + 16 * si + 4 * (l >> 4);
+__device__ __forceinline__ void put_pair(char* P, const f32x4& v, int ti, int si) {
+    const int l = lane_id(), g = l >> 4;
+    char* p = P + Sw<K::RP>::at(16 * ti + (l & 15), 2 * si + (g >> 1)) + 8 * (g & 1);
     float x[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -252,122 +303,137 @@ __device__ __forceinline__ void put_pair(uint16_t* P, const f32x4& v, int ti, in
 }
 // the tiles above the diagonal that products of 32 columns read
 template <class K, int NP>
-__device__ __forceinline__ void clear_upper(uint16_t* P) {
-    for (int v = threadIdx.x; v < NP * (K::TT / 2) * 16 * 4; v += K::NTH) {
-        const int c = v & 3, row = (v >> 2) & 15, b = (v >> 6) % (K::TT / 2), p = (v >> 6) / (K::TT / 2);
-        *reinterpret_cast<uint2*>(P + p * K::PPL + (32 * b + row) * K::LP + 32 * b + 16 + 4 * c) = make_uint2(0u, 0u);
+__device__ __forceinline__ void clear_upper(char* P) {
+    for (int v = threadIdx.x; v < NP * (K::TT / 2) * 16 * 2; v += K::NTH) {
+        const int c = v & 1, row = (v >> 1) & 15, b = (v >> 5) % (K::TT / 2), p = (v >> 5) / (K::TT / 2);
+        *reinterpret_cast<uint4*>(P + p * K::PPL + Sw<K::RP>::at(32 * b + row, 4 * b + 2 + c)) = make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
-// The state, columns 16 w .. + 15 of W for wave w: lane (c, r) holds St[16 j + 4 r + i]
-// [16 w + c] in s[j][i].  In memory [W's channel][Y's], or (swapped) [Y's][W's].
+// The state, the channels of W that are the wave's: lane (m = l % 16, r = l / 16) holds
+// St[32 (j / 2) + 8 r + 4 (j % 2) + i][channel(w, c, m)] in s[c][j][i].  In memory [W's channel]
+// [Y's], or (swapped) [Y's][W's].
 template <class K>
 struct State {
-    f32x4 s[K::DT];
+    f32x4 s[K::CW][K::DT];
     __device__ __forceinline__ void load(const float* p, bool swapped) {
-        const int l = lane_id(), dw = 16 * (int)(threadIdx.x >> 6) + (l & 15), r = l >> 4;
+        const int l = lane_id(), r = l >> 4;
 #pragma unroll
-        for (int j = 0; j < K::DT; ++j) {
-            if (!p) { s[j] = zero4(); continue; }
-            if (!swapped) {
-                const float4 v = *reinterpret_cast<const float4*>(p + dw * K::D + 16 * j + 4 * r);
-                s[j] = f32x4{v.x, v.y, v.z, v.w};
-            } else {
+        for (int c = 0; c < K::CW; ++c) {
+            const int dw = channel<K>(threadIdx.x >> 6, c, l & 15);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[j][i] = p[(16 * j + 4 * r + i) * K::D + dw];
+            for (int j = 0; j < K::DT; ++j) {
+                const int dy = 32 * (j >> 1) + 8 * r + 4 * (j & 1);
+                if (!p) { s[c][j] = zero4(); continue; }
+                if (!swapped) {
+                    const float4 v = *reinterpret_cast<const float4*>(p + dw * K::D + dy);
+                    s[c][j] = f32x4{v.x, v.y, v.z, v.w};
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[c][j][i] = p[(dy + i) * K::D + dw];
+                }
             }
         }
     }
     __device__ __forceinline__ void store(float* p, float scale) const {
-        const int l = lane_id(), dw = 16 * (int)(threadIdx.x >> 6) + (l & 15), r = l >> 4;
+        const int l = lane_id(), r = l >> 4;
 #pragma unroll
-        for (int j = 0; j < K::DT; ++j)
-            *reinterpret_cast<float4*>(p + dw * K::D + 16 * j + 4 * r) =
-                make_float4(scale * s[j][0], scale * s[j][1], scale * s[j][2], scale * s[j][3]);
+        for (int c = 0; c < K::CW; ++c) {
+            const int dw = channel<K>(threadIdx.x >> 6, c, l & 15);
+#pragma unroll
+            for (int j = 0; j < K::DT; ++j)
+                *reinterpret_cast<float4*>(p + dw * K::D + 32 * (j >> 1) + 8 * r + 4 * (j & 1)) =
+                    make_float4(scale * s[c][j][0], scale * s[c][j][1], scale * s[c][j][2], scale * s[c][j][3]);
+        }
     }
     // S <- all S + Y^T (down W): the chunk's sum from zero, so that what the matrix unit
-    // loses (it rounds sums downwards) does not add up over the chunks
-    __device__ __forceinline__ void add(const uint16_t* Y, const uint16_t* W, const Decays<K::C>& d) {
-        const int l = lane_id(), r = l >> 4, n0 = 16 * (int)(threadIdx.x >> 6);
-        f32x4 u[K::DT];
+    // loses (it rounds sums downwards) does not add up over the chunks.  w: w_frag of W.
+    __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::KC][K::CW][K::NPL], const Decays<K::C>& d) {
+        static_assert(K::KC == 1, "one step of the contracted index");
+        const int r = lane_id() >> 4;
+        const float4 d0 = *reinterpret_cast<const float4*>(d.down + 8 * r), d1 = *reinterpret_cast<const float4*>(d.down + 8 * r + 4);
+        const float dn[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+        bf16x8 ws[K::CW][3];
 #pragma unroll
-        for (int j = 0; j < K::DT; ++j) u[j] = zero4();
-#pragma unroll
-        for (int k = 0; k < K::KC; ++k) {
-            bf16x8 w[K::NPL], ws[3];
-            cols_k<K>(W, n0, 32 * k, w);
+        for (int c = 0; c < K::CW; ++c) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = (float)w[0][e];
-                if constexpr (K::NPL == 3) v[e] += (float)w[1][e] + (float)w[2][e];
-                v[e] *= d.down[32 * k + kslot(r, e)];
+                v[e] = (float)w[0][c][0][e];
+                if constexpr (K::NPL == 3) v[e] += (float)w[0][c][1][e] + (float)w[0][c][2][e];
+                v[e] *= dn[e];
             }
-            planes8<3>(v, ws);
-#pragma unroll
-            for (int j = 0; j < K::DT; ++j) {
-                bf16x8 y[K::NPL];
-                cols_k<K>(Y, 16 * j, 32 * k, y);
-                u[j] = mmp(y, ws, u[j]);
-            }
+            planes8<3>(v, ws[c]);
         }
         const float all = d.all;
 #pragma unroll
-        for (int j = 0; j < K::DT; ++j)
+        for (int j = 0; j < K::DT; ++j) {
+            bf16x8 y[K::NPL];
+            y_frag<K>(Y, 0, j, y);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = fmaf(all, s[j][i], u[j][i]);
-    }
-    // NS planes of the state for the products with X
-    template <int NS>
-    __device__ __forceinline__ void planes(bf16x8 (&f)[K::KD][NS]) const {
+            for (int c = 0; c < K::CW; ++c) {
+                const f32x4 u = mmp(y, ws[c], zero4());
 #pragma unroll
-        for (int k = 0; k < K::KD; ++k) {
-            const float v[8] = {s[2 * k][0], s[2 * k][1], s[2 * k][2], s[2 * k][3],
-                                s[2 * k + 1][0], s[2 * k + 1][1], s[2 * k + 1][2], s[2 * k + 1][3]};
-            planes8<NS>(v, f[k]);
+                for (int i = 0; i < 4; ++i) s[c][j][i] = fmaf(all, s[c][j][i], u[i]);
+            }
         }
     }
-    // up_t (St^T X_t) for every row: lane (c, r) has row 16 i + c, channels 16 w + 4 r ..
+    // up_t (St^T X_t) for every row, the state as NS planes: lane (m, r) has row 16 i + m, the
+    // channels of rows 4 r .. of tile c
     template <int NS>
-    __device__ __forceinline__ void apply(const uint16_t* X, const Decays<K::C>& d, f32x4 (&o)[K::TT]) const {
-        bf16x8 f[K::KD][NS];
-        planes<NS>(f);
-        const int c = lane_id() & 15;
+    __device__ __forceinline__ void apply(const char* X, const Decays<K::C>& d, f32x4 (&o)[K::TT][K::CW]) const {
+#pragma unroll
+        for (int i = 0; i < K::TT; ++i)
+#pragma unroll
+            for (int c = 0; c < K::CW; ++c) o[i][c] = zero4();
+#pragma unroll
+        for (int k = 0; k < K::KD; ++k) {
+            bf16x8 f[K::CW][NS];
+#pragma unroll
+            for (int c = 0; c < K::CW; ++c) {
+                const f32x4 &x = s[c][2 * k], &y = s[c][2 * k + 1];
+                const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                planes8<NS>(v, f[c]);
+            }
+#pragma unroll
+            for (int i = 0; i < K::TT; ++i) {
+                bf16x8 x[K::NPL];
+                along<K::RB, K::NPL, K::PLANE>(X, 16 * i, k, x);
+#pragma unroll
+                for (int c = 0; c < K::CW; ++c) o[i][c] = mmp(f[c], x, o[i][c]);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < K::TT; ++i) {
-            f32x4 acc = zero4();
+            const float up = d.up[16 * i + (lane_id() & 15)];
 #pragma unroll
-            for (int k = 0; k < K::KD; ++k) {
-                bf16x8 x[K::NPL];
-                rows_k<K>(X, 16 * i, 32 * k, x);
-                acc = mmp(f[k], x, acc);
-            }
-            const float up = d.up[16 * i + c];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] = acc[e] * up;
+            for (int c = 0; c < K::CW; ++c) o[i][c] *= up;
         }
     }
 };
 
 // o_t += sum_s P[t][s] W_s, layout as State::apply
 template <class K, int NP>
-__device__ __forceinline__ void add_pairs(const uint16_t* P, const uint16_t* W, f32x4 (&o)[K::TT]) {
-    const int n0 = 16 * (int)(threadIdx.x >> 6);
+__device__ __forceinline__ void add_pairs(const char* P, const bf16x8 (&w)[K::KC][K::CW][K::NPL], f32x4 (&o)[K::TT][K::CW]) {
 #pragma unroll
-    for (int k = 0; k < K::KC; ++k) {
-        bf16x8 w[K::NPL];
-        cols_k<K>(W, n0, 32 * k, w);
+    for (int k = 0; k < K::KC; ++k)
 #pragma unroll
         for (int i = 2 * k; i < K::TT; ++i) {
             bf16x8 p[NP];
+            along<K::RP, NP, K::PPL>(P, 16 * i, k, p);
 #pragma unroll
-            for (int q = 0; q < NP; ++q) p[q] = ldfrag<1, uint16_t>(P + q * K::PPL, K::LP, 16 * i, 32 * k).h;
-            o[i] = mmp(w, p, o[i]);
+            for (int c = 0; c < K::CW; ++c) o[i][c] = mmp(w[k][c], p, o[i][c]);
         }
-    }
+}
+template <class K>
+__device__ __forceinline__ void w_frags(const char* W, bf16x8 (&w)[K::KC][K::CW][K::NPL]) {
+#pragma unroll
+    for (int k = 0; k < K::KC; ++k)
+#pragma unroll
+        for (int c = 0; c < K::CW; ++c) w_frag<K>(W, k, c, w[k][c]);
 }
 
-// four channels of a token's output
+// a wave's channels of the rows of a chunk, the first in memory at out
 template <typename T>
 __device__ __forceinline__ void put4(T* p, const f32x4& v) {
     if constexpr (std::is_same<T, float>::value)
@@ -375,18 +441,29 @@ __device__ __forceinline__ void put4(T* p, const f32x4& v) {
     else
         *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
 }
-template <class K, typename OT>
-__device__ __forceinline__ void put_rows(OT* out, int64_t step, const f32x4 (&o)[K::TT], int n) {
-    const int l = lane_id(), ch = 16 * (int)(threadIdx.x >> 6) + 4 * (l >> 4);
+template <class K, typename OT, bool REV>
+__device__ __forceinline__ void put_rows(OT* out, uint32_t step, const f32x4 (&o)[K::TT][K::CW], int n) {
+    const int l = lane_id(), w = threadIdx.x >> 6, r = l >> 4;
 #pragma unroll
     for (int i = 0; i < K::TT; ++i) {
         const int t = 16 * i + (l & 15);
-        if (t < n) put4<OT>(out + t * step + ch, o[i]);
+        if (t >= n) continue;
+        OT* p = out + (uint32_t)(REV ? n - 1 - t : t) * step + channel<K>(w, 0, 4 * r);
+        if constexpr (K::CW == 2 && !std::is_same<OT, float>::value) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack2bf(o[i][0][0], o[i][0][1]), pack2bf(o[i][0][2], o[i][0][3]),
+                                                      pack2bf(o[i][1][0], o[i][1][1]), pack2bf(o[i][1][2], o[i][1][3]));
+        } else {
+#pragma unroll
+            for (int c = 0; c < K::CW; ++c) put4<OT>(p + 4 * c, o[i][c]);
+        }
     }
 }
 __device__ __forceinline__ float quad_sum(float x) {   // over the four lanes of equal l % 16
     x += __shfl_xor(x, 16, 64);
     return x + __shfl_xor(x, 32, 64);
+}
+__device__ __forceinline__ float dot4(const float4& a, const f32x4& b) {
+    return fmaf(a.x, b[0], a.y * b[1]) + fmaf(a.z, b[2], a.w * b[3]);
 }
 
 template <typename T>
@@ -403,23 +480,28 @@ __device__ __forceinline__ void clear_rows(void* out, const DecayArgs& a, const 
 
 template <class K, int NP>
 constexpr size_t mix_lds(bool states, bool dot) {
-    return (states ? 2 : 3) * (size_t)K::TILE * 2 + (states ? 0 : (size_t)NP * K::PPL * 2) + sizeof(Decays<K::C>) +
+    return (states ? 2 : 3) * (size_t)K::TILE + (states ? 0 : (size_t)NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
            (dot ? (size_t)K::NW * K::C * 4 : 0);
 }
 
 // mix: out = the operator over a slot's tokens (REV: backwards in time).  STATES: only
 // what the slot adds to the state, and its whole decay.  DOT: dots[t] = z_t . (the part
 // of out_t that comes from the state before the chunk), which NS = 3 keeps to fp32.
+//
+// A chunk: pairs, state and the state's part of out from LDS; a barrier; the pairs'
+// part from P and registers, and the next chunk into LDS; a barrier.  Its loads are in
+// flight for a whole chunk.  The last wave, which has the fewest pairs, forms the next
+// chunk's decays.
 template <class K, typename OT, int NP, int NS, bool REV, bool STATES, bool DOT>
-__global__ __launch_bounds__(K::NTH) void kda_decay_mix_kernel(const DecayArgs a, const bool swapped) {
+__global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const DecayArgs a, const bool swapped) {
     typedef typename K::ST ST;
     __shared__ __attribute__((aligned(16))) char lds[mix_lds<K, NP>(STATES, DOT)];
-    uint16_t* X = reinterpret_cast<uint16_t*>(lds);
-    uint16_t* Y = X + (STATES ? 0 : K::TILE);
-    uint16_t* W = Y + K::TILE;
-    uint16_t* P = W + K::TILE;
+    char* X = lds;
+    char* Y = X + (STATES ? 0 : K::TILE);
+    char* W = Y + K::TILE;
+    char* P = W + K::TILE;
     Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : NP * K::PPL));
-    float* part = reinterpret_cast<float*>(dec + 1);   // DOT: [NW][C]
+    float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]
 
     const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x), j = bid / a.H, h = bid - j * a.H;
     const Slot s = slot_of(a, j);
@@ -431,40 +513,62 @@ __global__ __launch_bounds__(K::NTH) void kda_decay_mix_kernel(const DecayArgs a
     }
     if (STATES && (REV ? s.first : s.last)) return;   // nothing follows
     const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
-    constexpr int DD = K::D * K::D;
+    constexpr int DD = K::D * K::D, LAST = K::NW - 1;
     State<K> st;
     st.load(STATES || !a.s_in ? nullptr : a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD, swapped);
 
-    const int dir = REV ? -1 : 1, head = REV ? s.tok0 + s.n - 1 : s.tok0;   // the first row's token
-    const ST *x = at<ST>(a.x, b, head, h), *y = at<ST>(a.y, b, head, h), *w = at<ST>(a.w, b, head, h);
-    const float* g = a.g + b * a.gb + (int64_t)head * a.gt + h * a.gh;
-    const int64_t xs = dir * a.x.token, ys = dir * a.y.token, ws = dir * a.w.token, gs = dir * a.gt;
-    Stage<K> sx, sy, sw;
+    const float* g = a.g + b * a.gb + (int64_t)s.tok0 * a.gt + h * a.gh;
+    Stage<K, REV> sx, sy, sw;
     float gv = 0.f;
+    // the first row in memory of the chunk at i0
+    auto lowest = [&](int i0, int n) { return s.tok0 + (REV ? s.n - i0 - n : i0); };
     auto load = [&](int i0) {
-        const int n = s.n - i0;
-        if constexpr (!STATES) sx.load(x + i0 * xs, xs, n);
-        sy.load(y + i0 * ys, ys, n);
-        sw.load(w + i0 * ws, ws, n);
-        // backwards, row i decays by what its successor in time does; the first by nothing
-        const int i = i0 + l;
-        if (wave == 0) gv = l < K::C && i < s.n && !(REV && i == 0) ? g[(int64_t)(REV ? i - 1 : i) * gs] : 0.f;
+        const int n = min(K::C, s.n - i0), t = lowest(i0, n);
+        if constexpr (!STATES) sx.load(at<ST>(a.x, b, t, h), (uint32_t)a.x.token * K::ES, n);
+        sy.load(at<ST>(a.y, b, t, h), (uint32_t)a.y.token * K::ES, n);
+        sw.load(at<ST>(a.w, b, t, h), (uint32_t)a.w.token * K::ES, n);
     };
-    if constexpr (!STATES) clear_upper<K, NP>(P);
-    double whole = 0.0;
-    if (s.n > 0) load(0);
-    for (int i0 = 0; i0 < s.n; i0 += K::C) {
-        const int n = s.n - i0;
-        if (i0) lds_barrier();   // every wave has read the chunk before
+    // backwards, row i decays by what its successor in time does; the first by nothing
+    auto load_g = [&](int i0) {
+        const int i = i0 + l;
+        gv = l < K::C && i < s.n && !(REV && i == 0) ? g[(int64_t)(REV ? s.n - i : i) * a.gt] : 0.f;
+    };
+    auto store = [&](int n) {
         if constexpr (!STATES) sx.store(X, n);
         sy.store(Y, n);
         sw.store(W, n);
-        if (wave == 0) whole += fill_decays<K::C>(dec, gv);
+    };
+    if constexpr (!STATES) clear_upper<K, NP>(P);
+    double whole = 0.0;
+    if (s.n > 0) {
+        load(0);
+        if (wave == LAST) {
+            load_g(0);
+            whole = fill_decays<K::C>(dec, gv);
+            load_g(K::C);
+        }
+        store(s.n);
+        if (K::C < s.n) load(K::C);
         lds_barrier();
-        if (i0 + K::C < s.n) load(i0 + K::C);
-        if constexpr (STATES) {
-            st.add(Y, W, *dec);
-        } else {
+    }
+    for (int i0 = 0; i0 < s.n; i0 += K::C) {
+        const int n = min(K::C, s.n - i0);
+        const Decays<K::C>& d = dec[i0 / K::C & 1];
+        const bool more = i0 + K::C < s.n;
+        bf16x8 w[K::KC][K::CW][K::NPL];
+        f32x4 o[K::TT][K::CW];
+        w_frags<K>(W, w);
+        float4 z[DOT ? K::TT : 1][K::CW];
+        if constexpr (DOT) {
+            const ST* p = at<ST>(a.z, b, lowest(i0, n), h) + channel<K>(wave, 0, 4 * (l >> 4));
+#pragma unroll
+            for (int i = 0; i < K::TT; ++i) {
+                const int m = min(16 * i + (l & 15), n - 1);
+#pragma unroll
+                for (int c = 0; c < K::CW; ++c) z[i][c] = ld4<ST>(p + (REV ? n - 1 - m : m) * (int)a.z.token + 4 * c);
+            }
+        }
+        if constexpr (!STATES) {
 #pragma unroll
             for (int k = 0; k < (K::NT + K::NW - 1) / K::NW; ++k) {
                 const int id = wave + K::NW * k;
@@ -472,59 +576,68 @@ __global__ __launch_bounds__(K::NTH) void kda_decay_mix_kernel(const DecayArgs a
                     int ti, si;
                     tile_of(id, ti, si);
                     f32x4 p = pair_tile<K>(X, Y, ti, si);
-                    p *= mask_tile<K>(*dec, ti, si);
+                    p *= mask_tile<K>(d, ti, si);
                     put_pair<K, NP>(P, p, ti, si);
                 }
             }
-            f32x4 o[K::TT];
-            st.template apply<NS>(X, *dec, o);
-            const int64_t row = (int64_t)b * a.T + head + dir * i0;   // of the chunk's first row
+            st.template apply<NS>(X, d, o);
             if constexpr (DOT) {
-                const ST* z = at<ST>(a.z, b, head + dir * i0, h) + 16 * wave + 4 * (l >> 4);
 #pragma unroll
                 for (int i = 0; i < K::TT; ++i) {
-                    const int t = 16 * i + (l & 15);
-                    const float4 q = ld4<ST>(z + (int64_t)min(t, n - 1) * dir * a.z.token);
-                    const float d = quad_sum(fmaf(q.x, o[i][0], q.y * o[i][1]) + fmaf(q.z, o[i][2], q.w * o[i][3]));
-                    if (l < 16) part[wave * K::C + t] = d;
-                }
-            }
-            st.add(Y, W, *dec);
-            lds_barrier();
-            add_pairs<K, NP>(P, W, o);
-            put_rows<K, OT>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, dir * (int64_t)a.H * K::D, o, n);
-            if constexpr (DOT) {
-                const int t = threadIdx.x;
-                if (t < K::C && t < n) {
-                    float d = 0.f;
+                    float x = 0.f;
 #pragma unroll
-                    for (int k = 0; k < K::NW; ++k) d += part[k * K::C + t];
-                    a.dots[(int64_t)h * a.B * a.T + row + dir * t] = d;
+                    for (int c = 0; c < K::CW; ++c) x += dot4(z[i][c], o[i][c]);
+                    x = quad_sum(x);
+                    if (l < 16) part[wave * K::C + 16 * i + l] = x;
                 }
             }
         }
+        st.add(Y, w, d);
+        if (wave == LAST && more) {
+            whole += fill_decays<K::C>(dec + ((i0 / K::C + 1) & 1), gv);
+            load_g(i0 + 2 * K::C);
+        }
+        lds_barrier();
+        if (more) {
+            store(s.n - i0 - K::C);
+            if (i0 + 2 * K::C < s.n) load(i0 + 2 * K::C);
+        }
+        if constexpr (!STATES) {
+            const int64_t row = (int64_t)b * a.T + lowest(i0, n);
+            add_pairs<K, NP>(P, w, o);
+            put_rows<K, OT, REV>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, n);
+            if constexpr (DOT) {
+                const int t = threadIdx.x;
+                if (t < n) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int k = 0; k < K::NW; ++k) x += part[k * K::C + t];
+                    a.dots[(int64_t)h * a.B * a.T + row + (REV ? n - 1 - t : t)] = x;
+                }
+            }
+        }
+        if (more) lds_barrier();
     }
     if constexpr (STATES) {
         // backwards: to before the slot's first token
         float last = 1.f;
-        if constexpr (REV) last = decay(g[(int64_t)(s.n - 1) * gs]);
-        if (threadIdx.x == 0) a.seg[(int64_t)j * a.H + h] = __builtin_amdgcn_exp2f((float)whole) * last;
+        if constexpr (REV) last = decay(g[0]);
+        if (wave == LAST && l == 0) a.seg[(int64_t)j * a.H + h] = __builtin_amdgcn_exp2f((float)whole) * last;
         st.store(a.s_out + ((int64_t)j * a.H + h) * DD, last);
     } else if (a.s_out && (REV ? s.first : s.last)) {
         float last = 1.f;
-        if constexpr (REV) last = s.n > 0 ? decay(g[(int64_t)(s.n - 1) * gs]) : 1.f;
+        if constexpr (REV) last = s.n > 0 ? decay(g[0]) : 1.f;
         st.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, last);
     }
 }
 
-// e^{sum of g over a chunk} below which what passes through it is nothing beside what begins in it
-constexpr float ANCHOR_BELOW = 0x1p-32f;
-
 template <class K, int NP>
 constexpr size_t mix2_lds(bool dot) {
-    return 4 * (size_t)K::TILE * 2 + 2 * (size_t)NP * K::PPL * 2 + sizeof(Decays<K::C>) +
+    return 4 * (size_t)K::TILE + 2 * (size_t)NP * K::PPL + 2 * sizeof(Decays<K::C>) +
            (dot ? (size_t)(K::NW + 2 * K::TT) * K::C * 4 : 0);
 }
+// e^{sum of g over a chunk} below which what passes through it is nothing beside what begins in it
+constexpr float ANCHOR_BELOW = 0x1p-32f;
 
 // mix2: dk and dv of a slot, backwards in time, from q (y), k (x), v (z) and do (w), with
 // dS in both orders: dv = mix(k, q, do), dk = mix(v, do, q).  DOT: dots[t] -= k_t . (the part
@@ -533,17 +646,17 @@ constexpr size_t mix2_lds(bool dot) {
 // give q . dq and k . dk; and where nothing passes through a whole chunk anchors[chunk], all
 // that leaves it.
 template <class K, typename OT, int NP, int NS, bool DOT>
-__global__ __launch_bounds__(K::NTH) void kda_decay_mix2_kernel(const DecayArgs a) {
+__global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const DecayArgs a) {
     typedef typename K::ST ST;
     __shared__ __attribute__((aligned(16))) char lds[mix2_lds<K, NP>(DOT)];
-    uint16_t* Kt = reinterpret_cast<uint16_t*>(lds);
-    uint16_t* Q = Kt + K::TILE;
-    uint16_t* V = Q + K::TILE;
-    uint16_t* O = V + K::TILE;
-    uint16_t* PA = O + K::TILE;
-    uint16_t* PD = PA + NP * K::PPL;
+    char* Kt = lds;
+    char* Q = Kt + K::TILE;
+    char* V = Q + K::TILE;
+    char* O = V + K::TILE;
+    char* PA = O + K::TILE;
+    char* PD = PA + NP * K::PPL;
     Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(PD + NP * K::PPL);
-    float* part = reinterpret_cast<float*>(dec + 1);   // DOT: [NW][C]; then E's [TT column tiles][C] and [TT row tiles][C]
+    float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]; then E's [TT column tiles][C] and [TT row tiles][C]
     float* e_own = part + K::NW * K::C;                // sums over the other tokens, of X rows (k, v)
     float* e_oth = e_own + K::TT * K::C;               // and of Y rows (q, do)
 
@@ -557,55 +670,70 @@ __global__ __launch_bounds__(K::NTH) void kda_decay_mix2_kernel(const DecayArgs 
         return;
     }
     const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
-    constexpr int DD = K::D * K::D;
+    constexpr int DD = K::D * K::D, LAST = K::NW - 1;
     const float* s_in = a.s_in ? a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD : nullptr;
     State<K> sv, sk;   // dv's: [do][q]; dk's: [q][do]
     sv.load(s_in, false);
     sk.load(s_in, true);
 
-    const int head = s.tok0 + s.n - 1;
-    const ST *kp = at<ST>(a.x, b, head, h), *qp = at<ST>(a.y, b, head, h), *vp = at<ST>(a.z, b, head, h),
-             *op = at<ST>(a.w, b, head, h);
-    const float* g = a.g + b * a.gb + (int64_t)head * a.gt + h * a.gh;
-    Stage<K> rk, rq, rv, ro;
+    const float* g = a.g + b * a.gb + (int64_t)s.tok0 * a.gt + h * a.gh;
+    Stage<K, true> rk, rq, rv, ro;
     float gv = 0.f;
-    // the chunks are those of a pass forwards, so that dots and the sums of mix over them add up
+    // the chunks are those of a pass forwards, so that dots and the sums of mix over them add up:
+    // rows [i0, i0 + n) backwards, all but the first C of them
     const int n0 = s.n - (s.n - 1) / K::C * K::C;
-    auto load = [&](int i0) {
-        const int n = i0 ? K::C : n0, i = i0 + l;
-        rk.load(kp - i0 * a.x.token, -a.x.token, n);
-        rq.load(qp - i0 * a.y.token, -a.y.token, n);
-        rv.load(vp - i0 * a.z.token, -a.z.token, n);
-        ro.load(op - i0 * a.w.token, -a.w.token, n);
-        if (wave == 0) gv = l < n && i > 0 ? g[-(int64_t)(i - 1) * a.gt] : 0.f;
+    auto load = [&](int i0, int n) {
+        const int t = s.tok0 + s.n - i0 - n;
+        rk.load(at<ST>(a.x, b, t, h), (uint32_t)a.x.token * K::ES, n);
+        rq.load(at<ST>(a.y, b, t, h), (uint32_t)a.y.token * K::ES, n);
+        rv.load(at<ST>(a.z, b, t, h), (uint32_t)a.z.token * K::ES, n);
+        ro.load(at<ST>(a.w, b, t, h), (uint32_t)a.w.token * K::ES, n);
+    };
+    auto load_g = [&](int i0, int n) {
+        const int i = i0 + l;
+        gv = l < n && i > 0 && i < s.n ? g[(int64_t)(s.n - i) * a.gt] : 0.f;
+    };
+    auto store = [&](int n) {
+        rk.store(Kt, n);
+        rq.store(Q, n);
+        rv.store(V, n);
+        ro.store(O, n);
     };
     clear_upper<K, NP>(PA);
     clear_upper<K, NP>(PD);
     if constexpr (DOT)
         for (int v = threadIdx.x; v < 2 * K::TT * K::C; v += K::NTH) e_own[v] = 0.f;
-    if (s.n > 0) load(0);
-    for (int i0 = 0, n = n0; i0 < s.n; i0 += n, n = K::C) {
-        if (i0) lds_barrier();
-        rk.store(Kt, n);
-        rq.store(Q, n);
-        rv.store(V, n);
-        ro.store(O, n);
-        if (wave == 0) fill_decays<K::C>(dec, gv);
+    if (s.n > 0) {
+        load(0, n0);
+        if (wave == LAST) {
+            load_g(0, n0);
+            fill_decays<K::C>(dec, gv);
+            load_g(n0, K::C);
+        }
+        store(n0);
+        if (n0 < s.n) load(n0, K::C);
         lds_barrier();
-        if (i0 + n < s.n) load(i0 + n);
+    }
+    int turn = 0;
+    for (int i0 = 0, n = n0; i0 < s.n; i0 += n, n = K::C, turn ^= 1) {
+        const Decays<K::C>& d = dec[turn];
+        const bool more = i0 + n < s.n;
+        bf16x8 wo[K::KC][K::CW][K::NPL], wq[K::KC][K::CW][K::NPL];
+        w_frags<K>(O, wo);
+        w_frags<K>(Q, wq);
 #pragma unroll
         for (int k = 0; k < (K::NT + K::NW - 1) / K::NW; ++k) {
             const int id = wave + K::NW * k;
             if (id < K::NT) {
                 int ti, si;
                 tile_of(id, ti, si);
-                const f32x4 m = mask_tile<K>(*dec, ti, si);
-                const f32x4 pa = pair_tile<K>(Kt, Q, ti, si) * m, d = pair_tile<K>(V, O, ti, si);
+                const f32x4 m = mask_tile<K>(d, ti, si);
+                const f32x4 pa = pair_tile<K>(Kt, Q, ti, si) * m, pd = pair_tile<K>(V, O, ti, si);
                 put_pair<K, NP>(PA, pa, ti, si);
-                put_pair<K, NP>(PD, d * m, ti, si);
+                put_pair<K, NP>(PD, pd * m, ti, si);
                 if constexpr (DOT) {
                     // a token's own pair passes no decay, and would drown what does where decays are fast
-                    f32x4 e = pa * d;
+                    f32x4 e = pa * pd;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (ti == si && 4 * (l >> 4) + i == (l & 15)) e[i] = 0.f;
@@ -621,63 +749,74 @@ __global__ __launch_bounds__(K::NTH) void kda_decay_mix2_kernel(const DecayArgs 
                 }
             }
         }
-        const int64_t row = (int64_t)b * a.T + head - i0, step = -(int64_t)a.H * K::D;
-        const int ch = 16 * wave + 4 * (l >> 4);
-        f32x4 o[K::TT], o2[K::TT];
-        sv.template apply<NS>(Kt, *dec, o);
+        f32x4 o[K::TT][K::CW], o2[K::TT][K::CW];
+        sv.template apply<NS>(Kt, d, o);
         if constexpr (DOT) {
+            const int ch = channel<K>(wave, 0, 4 * (l >> 4));
 #pragma unroll
             for (int i = 0; i < K::TT; ++i) {
                 const int t = 16 * i + (l & 15);
-                float4 v = ld4<uint16_t>(V + t * K::LD + ch);
-                if constexpr (K::NPL == 3) {
-                    const float4 v1 = ld4<uint16_t>(V + K::PLANE + t * K::LD + ch),
-                                 v2 = ld4<uint16_t>(V + 2 * K::PLANE + t * K::LD + ch);
-                    v = make_float4(v.x + (v1.x + v2.x), v.y + (v1.y + v2.y), v.z + (v1.z + v2.z), v.w + (v1.w + v2.w));
+                float x = 0.f;
+#pragma unroll
+                for (int c = 0; c < K::CW; ++c) {
+                    const char* p = V + Sw<K::RB>::at(t, (ch + 4 * c) >> 3) + 2 * ((ch + 4 * c) & 7);
+                    float4 v = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p));
+                    if constexpr (K::NPL == 3) {
+                        const float4 v1 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + K::PLANE)),
+                                     v2 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + 2 * K::PLANE));
+                        v = make_float4(v.x + (v1.x + v2.x), v.y + (v1.y + v2.y), v.z + (v1.z + v2.z), v.w + (v1.w + v2.w));
+                    }
+                    x += dot4(v, o[i][c]);
                 }
-                const float d = quad_sum(fmaf(v.x, o[i][0], v.y * o[i][1]) + fmaf(v.z, o[i][2], v.w * o[i][3]));
-                if (l < 16) part[wave * K::C + t] = d;
+                x = quad_sum(x);
+                if (l < 16) part[wave * K::C + t] = x;
             }
         }
-        sk.template apply<K::NPL == 3 ? 3 : NP>(V, *dec, o2);
-        sv.add(Q, O, *dec);
-        sk.add(O, Q, *dec);
+        sk.template apply<K::NPL == 3 ? 3 : NP>(V, d, o2);
+        sv.add(Q, wo, d);
+        sk.add(O, wq, d);
+        if (wave == LAST && more) {
+            fill_decays<K::C>(dec + (turn ^ 1), gv);
+            load_g(i0 + n + K::C, K::C);
+        }
+        const float all = d.all;
         lds_barrier();
-        add_pairs<K, NP>(PA, O, o);
-        add_pairs<K, NP>(PD, Q, o2);
-        put_rows<K, OT>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, step, o2, n);
-        put_rows<K, OT>(static_cast<OT*>(a.out2) + (row * a.H + h) * K::D, step, o, n);
+        if (more) {
+            store(K::C);
+            if (i0 + n + K::C < s.n) load(i0 + n + K::C, K::C);
+        }
+        const int64_t row = (int64_t)b * a.T + s.tok0 + s.n - i0 - n, out = (row * a.H + h) * K::D;
+        add_pairs<K, NP>(PA, wo, o);
+        add_pairs<K, NP>(PD, wq, o2);
+        put_rows<K, OT, true>(static_cast<OT*>(a.out) + out, (uint32_t)(a.H * K::D), o2, n);
+        put_rows<K, OT, true>(static_cast<OT*>(a.out2) + out, (uint32_t)(a.H * K::D), o, n);
         if constexpr (DOT) {
-            const int t = threadIdx.x;
-            if (t < K::C && t < n) {
-                float own = 0.f, oth = 0.f, d = 0.f;
+            if (wave == 0) {
+                const int t = l;
+                float x = 0.f;
+                if (t < n) {
+                    float own = 0.f, oth = 0.f;
 #pragma unroll
-                for (int k = 0; k < K::TT; ++k) {
-                    own += e_own[k * K::C + t];
-                    oth += e_oth[k * K::C + t];
+                    for (int k = 0; k < K::TT; ++k) {
+                        own += e_own[k * K::C + t];
+                        oth += e_oth[k * K::C + t];
+                    }
+#pragma unroll
+                    for (int k = 0; k < K::NW; ++k) x += part[k * K::C + t];
+                    const int64_t at = (int64_t)h * a.B * a.T + row + (n - 1 - t);
+                    a.dots[at] -= x;
+                    a.dots2[at] = oth - own;
                 }
 #pragma unroll
-                for (int k = 0; k < K::NW; ++k) d += part[k * K::C + t];
-                const int64_t at = (int64_t)h * a.B * a.T + row - t;
-                a.dots[at] -= d;
-                a.dots2[at] = oth - own;
-                part[t] = d;   // (each thread has read its own column)
-            }
-            if (wave == 0) {
-                wave_sync();
-                float sum = l < K::C && l < n ? part[l] : 0.f;
-#pragma unroll
-                for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k, 64);
+                for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k, 64);
                 if (l == 0)
                     a.anchors[((int64_t)j * a.H + h) * (a.seg_tokens / K::C) + (s.n - i0 - 1) / K::C] =
-                        dec->all < ANCHOR_BELOW ? sum : __builtin_nanf("");
+                        all < ANCHOR_BELOW ? x : __builtin_nanf("");
             }
         }
+        if (more) lds_barrier();
     }
-    if (a.s_out && s.first) {
-        const float last = s.n > 0 ? decay(g[-(int64_t)(s.n - 1) * a.gt]) : 1.f;
-        sv.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, last);
-    }
+    if (a.s_out && s.first) sv.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, s.n > 0 ? decay(g[0]) : 1.f);
 }
 
 // ----------------------------------------------------------------------------
@@ -748,7 +887,7 @@ __global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, 
 }
 
 // The state at each slot's start (REV: its adjoint at each slot's end), in place of
-// what the slots add: one thread takes four elements through a sequence's slots, eight
+// what the slots add: one thread takes four elements through a sequence's slots, sixteen
 // loads at a time.
 template <bool REV>
 __global__ __launch_bounds__(256) void kda_decay_scan_kernel(float* u, const float* seg, const float* s0, const int* first,
@@ -760,7 +899,7 @@ __global__ __launch_bounds__(256) void kda_decay_scan_kernel(float* u, const flo
     float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
     if (s0) run = *reinterpret_cast<const float4*>(s0 + ((int64_t)seq * H + h) * DD + e);
     auto slot = [&](int i) { return (int64_t)(REV ? lo + count - 1 - i : lo + i) * H + h; };
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 16;
     for (int i0 = 0; i0 < count; i0 += AHEAD) {
         float4 v[AHEAD];
         float f[AHEAD];
@@ -984,19 +1123,30 @@ struct Plan {
     int seg_tokens, per_seq, nslots, packed;
     bool multi;   // the states between slots are in memory
 };
-// Workgroups beside each other that fill the card: 256 CUs with four of head sizes up
-// to 64, two of larger ones.
-Plan plan_of(const Args& a, bool dg) {
+// How many chunks of 64 tokens a slot has.  Sequences that fill the card by themselves are
+// one slot each; else what is shared out costs a pass for the slots' states and a scan
+// over them, and the workgroups come in rounds of as many as fit beside each other
+// (measured at D = 64: a chunk takes 0.4 of a full card's time in a workgroup alone, a
+// slot 1 / 40 of it in the scan): the least of all counts.
+Plan plan_of(const Args& a, bool bwd) {
     Plan p;
-    const int64_t want = a.D <= 64 ? 1024 : 512, seqs = a.cu ? 1 : a.B, chunks = (a.T + 63) / 64;
-    int64_t per = 1;
-    if (seqs * a.H * 2 <= want && chunks > 4) per = std::min((chunks + 3) / 4, (want + seqs * a.H - 1) / (seqs * a.H));
-    int64_t seg = std::max<int64_t>(1, (chunks + per - 1) / per);
-    // dg is a sum over a slot's tokens, whose errors add up
-    if (dg) seg = std::min<int64_t>(seg, 32);
     p.packed = a.cu != nullptr;
+    const int64_t seqs = p.packed ? a.nseq : a.B, rows = p.packed ? 1 : a.B, chunks = std::max<int64_t>(1, (a.T + 63) / 64);
+    // dg is a sum over a slot's tokens, whose errors add up
+    const int64_t most = bwd && a.dg ? 32 : chunks, fit = a.D <= 64 ? 1024 : 512;
+    double best = 0.0;
+    int64_t seg = 0;
+    for (int64_t c = 1; c <= most; c = c == chunks ? most + 1 : c >= 64 ? chunks : c + 1) {
+        const int64_t per = (chunks + c - 1) / c, n = (p.packed ? per + seqs / 2 : rows * per) * a.H, rest = n % fit;
+        const double turns = (double)(n / fit) + (rest ? 0.4 + 0.6 * (double)rest / fit : 0.0);
+        const double cost = (double)c * turns * (p.packed || per > 1 ? 1.5 : 1.0) + (per > 1 ? 0.5 + 0.025 * per : 0.0);
+        if (!seg || cost < best) {
+            best = cost;
+            seg = c;
+        }
+    }
     p.seg_tokens = (int)(64 * seg);
-    p.per_seq = p.packed ? 0 : (int)std::max<int64_t>(1, (chunks + seg - 1) / seg);
+    p.per_seq = p.packed ? 0 : (int)((chunks + seg - 1) / seg);
     const int64_t n = p.packed ? a.nseq + 2 + a.T / p.seg_tokens : a.B * p.per_seq;
     p.nslots = n * a.H > 0x7fffffff ? -1 : (int)n;
     p.multi = p.packed || p.per_seq > 1;
@@ -1038,6 +1188,7 @@ Layout layout_of(const Args& a, const Plan& p, bool bwd) {
     return l;
 }
 
+constexpr int MAX_TOKEN_STRIDE = 1 << 24;
 int check_operand(const Args& a, const kda_decay_rows& r, const char* name) {
     const int64_t es = a.dtype == KDA_DTYPE_BF16 ? 2 : 4;
     if (!r.p || reinterpret_cast<uintptr_t>(r.p) % 16 != 0)
@@ -1045,6 +1196,9 @@ int check_operand(const Args& a, const kda_decay_rows& r, const char* name) {
     if ((r.batch * es) % 16 || (r.token * es) % 16 || (r.head * es) % 16)
         return api_fail(KDA_E_INVALID, "%s: strides %lld, %lld, %lld are not whole 16-byte pieces", name, (long long)r.batch,
                         (long long)r.token, (long long)r.head);
+    // (a chunk's rows are addressed by 32 bits)
+    if (r.token < 0 || r.token > MAX_TOKEN_STRIDE)
+        return api_fail(KDA_E_INVALID, "%s: token stride %lld: expected 0 to %d", name, (long long)r.token, MAX_TOKEN_STRIDE);
     return KDA_OK;
 }
 int check_sizes(const Args& a) {
@@ -1135,7 +1289,7 @@ hipError_t launch_group(const float* src, void* dst, const Args& a, const kda_de
 // what is lost there small beside the output's own rounding.
 template <int D, bool F32>
 int forward(const Args& a, hipStream_t st) {
-    typedef Cfg<D, F32, F32 ? 32 : 64> K;
+    typedef Cfg<D, F32> K;
     constexpr int NP = F32 ? 3 : 2;
     const Plan p = plan_of(a, false);
     const Layout l = layout_of(a, p, false);
@@ -1166,12 +1320,10 @@ hipError_t launch_mix2(const DecayArgs& d, hipStream_t st) {
 
 template <int D, bool F32, bool DOT>
 int backward(const Args& a, hipStream_t st) {
-    typedef Cfg<D, F32, F32 ? 32 : 64> K;
-    typedef Cfg<D, F32, (F32 || D > 64) ? 32 : 64> K2;   // four operands in LDS
+    typedef Cfg<D, F32> K;
     typedef typename K::ST ST;
-    typedef typename std::conditional<DOT, K2, K>::type K1;   // dg: the same chunks in both
     constexpr int NP = F32 ? 3 : 2;
-    const Plan p = plan_of(a, DOT);
+    const Plan p = plan_of(a, true);
     const Layout l = layout_of(a, p, true);
     char* ws = static_cast<char*>(a.workspace);
     const DecayArgs base = base_of(a, p, l);
@@ -1198,10 +1350,10 @@ int backward(const Args& a, hipStream_t st) {
     d.dots = dots;
     d.out = shared(a, a.q) ? g0 : a.dq;
     if (shared(a, a.q)) {
-        DEC_HIP((launch_mix<K1, float, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
+        DEC_HIP((launch_mix<K, float, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
         DEC_HIP(launch_group<ST>(g0, a.dq, a, a.q, st));
     } else {
-        DEC_HIP((launch_mix<K1, ST, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
+        DEC_HIP((launch_mix<K, ST, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
     }
     d = base;
     d.x = k; d.y = q; d.z = v; d.w = o;
@@ -1212,12 +1364,12 @@ int backward(const Args& a, hipStream_t st) {
     d.anchors = DOT ? reinterpret_cast<float*>(ws + l.anchors) : nullptr;
     if (shared(a, a.k) || shared(a, a.v)) {
         d.out = g0; d.out2 = g1;
-        DEC_HIP((launch_mix2<K2, float, NP, DOT>(d, st)));
+        DEC_HIP((launch_mix2<K, float, NP, DOT>(d, st)));
         DEC_HIP(launch_group<ST>(g0, a.dk, a, a.k, st));
         DEC_HIP(launch_group<ST>(g1, a.dv, a, a.v, st));
     } else {
         d.out = a.dk; d.out2 = a.dv;
-        DEC_HIP((launch_mix2<K2, ST, NP, DOT>(d, st)));
+        DEC_HIP((launch_mix2<K, ST, NP, DOT>(d, st)));
     }
     if constexpr (DOT) {
         d = base;
@@ -1226,7 +1378,7 @@ int backward(const Args& a, hipStream_t st) {
         d.anchors = reinterpret_cast<float*>(ws + l.anchors);
         double* sums = a.dg_heads ? reinterpret_cast<double*>(ws + l.sums) : nullptr;
         hipLaunchKernelGGL(kda_decay_dg_kernel, dim3((unsigned)(d.nslots * d.H)), dim3(DG_TH), 0, st, d, starts, dends, a.s_final,
-                           a.ds_final, sums ? nullptr : a.dg, sums, D * D, K1::C);
+                           a.ds_final, sums ? nullptr : a.dg, sums, D * D, K::C);
         DEC_HIP(hipGetLastError());
         if (sums) {
             hipLaunchKernelGGL(kda_decay_dg_sum_kernel, dim3((unsigned)d.H), dim3(64), 0, st, sums, a.dg, d.nslots, d.H);
@@ -1256,7 +1408,7 @@ hipError_t launch_step(const StepArgs& a, bool f32, hipStream_t st) {
 
 int check_common(const Args& a, bool bwd) {
     DEC_TRY(check_sizes(a));
-    const Plan p = plan_of(a, bwd && a.dg);
+    const Plan p = plan_of(a, bwd);
     if (p.nslots < 0) return api_fail(KDA_E_UNSUPPORTED, "B=%lld T=%lld H=%lld: too many workgroups", (long long)a.B, (long long)a.T, (long long)a.H);
     if (a.B * a.T > 0) {
         DEC_TRY(check_operand(a, a.q, "q"));
@@ -1286,7 +1438,7 @@ extern "C" {
 size_t kda_decay_workspace_size(int pass, const kda_decay_args* args) {
     if (!args || check_sizes(*args) != KDA_OK) return 0;
     const bool bwd = pass == KDA_PASS_BWD;
-    const Plan p = plan_of(*args, bwd && args->dg);
+    const Plan p = plan_of(*args, bwd);
     return p.nslots < 0 ? 0 : (size_t)layout_of(*args, p, bwd).bytes;
 }
 

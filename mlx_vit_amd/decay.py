@@ -33,13 +33,13 @@ from .linear import _grad_enabled, _is_tracing, _on, _raw_stream
 
 HEAD_DIMS = FWD_HEAD_DIMS
 _increment_version = torch._C._increment_version
-MAX_TOKENS = (1 << 31) - 8192
+MAX_TOKENS, MAX_TOKEN_STRIDE = (1 << 31) - 8192, 1 << 24
 
 
 def _pieces(t: torch.Tensor) -> torch.Tensor:
     """t (..., heads, D) as the kernels read it, rows in whole 16-byte pieces; a copy where it is not."""
     n = 16 // t.element_size()
-    if (t.data_ptr() & 15 or t.stride(-1) != 1
+    if (t.data_ptr() & 15 or t.stride(-1) != 1 or t.stride(-3) > MAX_TOKEN_STRIDE
             or any(s % n for s, m in zip(t.stride()[:-1], t.shape[:-1]) if m > 1)):
         return t.clone(memory_format=torch.contiguous_format)
     return t
