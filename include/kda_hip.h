@@ -433,9 +433,10 @@ int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const 
  * of exactly zero.  A value that is not finite reaches every output of its sequence from its
  * block of 32 tokens on (in a gradient: up to it).
  * Backward: gradients of <o, dout> + <s_final, ds_final>; reads s_final only for dg
- * beside ds_final.  Nothing else is kept between the calls.  workspace: at least
- * kda_decay_workspace_size(KDA_PASS_FWD or KDA_PASS_BWD, args) bytes for these sizes, heads, cu,
- * nseq, dtype, dg and dg_heads, 16-byte aligned.  Results do not depend on how the
+ * beside ds_final.  kda_decay_workspace_size(pass, args): bytes, 16-byte aligned, for these
+ * sizes, heads, cu, nseq, dtype, dg and dg_heads.  KDA_PASS_FWD: the forward pass' workspace;
+ * KDA_PASS_TRAIN: with train != 0, what it writes to kept instead, for a backward pass of the
+ * same arguments to read; KDA_PASS_BWD: the backward pass' workspace.  Results do not depend on how the
  * sequence is shared out beyond rounding, and are the same from call to call. */
 typedef struct kda_decay_rows {
     const void* p;
@@ -458,6 +459,8 @@ typedef struct kda_decay_args {
     int64_t B, T, H, D, dtype;
     void* workspace;
     int64_t ws_bytes;
+    void* kept;
+    int64_t kept_bytes, train;
 } kda_decay_args;
 size_t kda_decay_workspace_size(int pass, const kda_decay_args* args);
 int kda_decay_fwd(const kda_decay_args* args, void* stream);

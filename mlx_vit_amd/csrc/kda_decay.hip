@@ -42,8 +42,10 @@ struct DecayArgs {
     void *out, *out2;           // [B][T][H][D]
     const float* s_in;          // the state that a slot starts from, by slot or by sequence
     float* s_out;               // and ends with: by slot (states), by sequence (else); may be null
-    float *dots, *dots2;        // [H][B T]
-    float* anchors;             // [slot][H][its chunks]
+    float* dots;                // [H][B T]
+    const float *starts, *s_final;   // mix2: the state at the slots' starts, by slot, and at the sequences' ends
+    float* dg;                  // [B][T][H], or null
+    double* sums;               // or its sums by slot, [slot][H]
     float* seg;                 // states: e^{sum of g} of each slot and head
     const int4* tab;            // packed: the slots
     int in_by_slot;
@@ -111,50 +113,49 @@ struct Sw {
     }
 };
 
-// C tokens a chunk; a wave has CW tiles of 16 of W's channels (with two the LDS reads of
-// a chunk are half as many, but 65536 x 12 x 64 took 190 us instead of 175: too few
-// waves).  bf16 operands are one plane, fp32 ones three.  OCC: waves a SIMD that mix and
-// mix2 are held to.
-template <int D_, bool F32_, int C_ = 32, int CW_ = 1>
+// C tokens a chunk; a wave has 16 of W's channels (32, which halves the LDS reads, took
+// 190 us instead of 175 over 65536 x 12 x 64: too few waves), a workgroup a SPLIT-th of
+// them: the pairs are then formed SPLIT times, but by waves that would wait for them (20000
+// packed x 16 x 128: 115 instead of 128 us forward, dq 147 instead of 185).  bf16 operands are
+// one plane, fp32 ones three.  OCC, OCC2: waves a SIMD that mix and mix2 are held to.
+template <int D_, bool F32_, int SPLIT_ = 1, int C_ = 32>
 struct Cfg {
-    static constexpr int D = D_, C = C_, CW = CW_, NPL = F32_ ? 3 : 1, NW = D / (16 * CW), NTH = 64 * NW;
-    static constexpr int RB = 2 * D, PLANE = C * RB, TILE = NPL * PLANE;    // bytes
-    static constexpr int RP = 2 * C, PPL = C * RP;                          // of the pairs'
+    static constexpr int D = D_, C = C_, SPLIT = SPLIT_, DW = D / SPLIT, NPL = F32_ ? 3 : 1, NW = DW / 16, NTH = 64 * NW;
+    static constexpr int RB = 2 * D, PLANE = C * RB, TILE = NPL * PLANE;                       // bytes
+    static constexpr int RBW = (2 * DW + 63) / 64 * 64, PLANEW = C * RBW, TILEW = NPL * PLANEW;   // of DW channels
+    static constexpr int RP = 2 * C, PPL = C * RP;                                             // of the pairs'
     static constexpr int TT = C / 16, NT = TT * (TT + 1) / 2, DT = D / 16, KD = D / 32, KC = C / 32;
-    static constexpr int OCC = F32_ ? 1 : 4, OCC2 = F32_ ? 1 : D > 64 ? 2 : 3;
+    static constexpr int OCC = F32_ ? 1 : D > 64 ? 3 : 4, OCC2 = F32_ ? 1 : D > 64 ? 2 : 3;
     static constexpr bool F32 = F32_;
     typedef typename std::conditional<F32_, float, uint16_t>::type ST;
-    static constexpr int ES = (int)sizeof(ST), EPV = 16 / ES, VPR = D / EPV, NV = C * VPR, PER = NV / NTH;
-    static_assert(NV % NTH == 0 && C % 32 == 0 && D % (16 * CW) == 0, "whole pieces");
+    static constexpr int ES = (int)sizeof(ST), EPV = 16 / ES;
+    static_assert(C % 32 == 0 && D % (16 * SPLIT) == 0 && D % 32 == 0, "whole tiles");
 };
-// the channel of W that row m of tile c of wave w stands for: two tiles' four rows are
-// eight channels in a row
-template <class K>
-__device__ __forceinline__ int channel(int w, int c, int m) {
-    return K::CW == 2 ? 32 * w + 8 * (m >> 2) + 4 * c + (m & 3) : 16 * w + m;
-}
 
-// C rows on their way from memory to LDS, forwards or backwards in time
-template <class K, bool REV>
+// C rows of COLS channels on their way from memory to LDS, forwards or backwards in time
+template <class K, int COLS, bool REV>
 struct Stage {
-    uint4 r[K::PER];
+    static constexpr int VPR = COLS / K::EPV, NV = K::C * VPR, PER = NV / K::NTH;
+    static constexpr int RB = COLS == K::D ? K::RB : K::RBW, PLANE = K::C * RB;
+    static_assert(NV % K::NTH == 0, "whole pieces");
+    uint4 r[PER];
     // n >= 1 rows, the first in memory at p, `step` bytes apart; what is behind them reads the last
     __device__ __forceinline__ void load(const typename K::ST* p, uint32_t step, int n) {
 #pragma unroll
-        for (int i = 0; i < K::PER; ++i) {
-            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = v - row * K::VPR, m = min(row, n - 1);
+        for (int i = 0; i < PER; ++i) {
+            const int v = (int)threadIdx.x + K::NTH * i, row = v / VPR, c = v - row * VPR, m = min(row, n - 1);
             r[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + ((uint32_t)(REV ? n - 1 - m : m) * step + 16 * c));
         }
     }
     // ... and is stored as zeros
     __device__ __forceinline__ void store(char* t, int n) const {
 #pragma unroll
-        for (int i = 0; i < K::PER; ++i) {
-            const int v = (int)threadIdx.x + K::NTH * i, row = v / K::VPR, c = v - row * K::VPR;
+        for (int i = 0; i < PER; ++i) {
+            const int v = (int)threadIdx.x + K::NTH * i, row = v / VPR, c = v - row * VPR;
             uint4 x = r[i];
             if (n < K::C) x = row < n ? x : make_uint4(0u, 0u, 0u, 0u);
             if constexpr (!K::F32) {
-                *reinterpret_cast<uint4*>(t + Sw<K::RB>::at(row, c)) = x;
+                *reinterpret_cast<uint4*>(t + Sw<RB>::at(row, c)) = x;
             } else {
                 // each part the next 8 bits of 24, cut off, so that nothing overflows
                 const uint32_t b[4] = {x.x, x.y, x.z, x.w};
@@ -167,12 +168,12 @@ struct Stage {
                     l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
                 }
                 constexpr uint32_t HI = 0x07060302u;
-                char* q = t + Sw<K::RB>::at(row, c >> 1) + 8 * (c & 1);
+                char* q = t + Sw<RB>::at(row, c >> 1) + 8 * (c & 1);
                 *reinterpret_cast<uint2*>(q) =
                     make_uint2(__builtin_amdgcn_perm(h[1], h[0], HI), __builtin_amdgcn_perm(h[3], h[2], HI));
-                *reinterpret_cast<uint2*>(q + K::PLANE) =
+                *reinterpret_cast<uint2*>(q + PLANE) =
                     make_uint2(__builtin_amdgcn_perm(m[1], m[0], HI), __builtin_amdgcn_perm(m[3], m[2], HI));
-                *reinterpret_cast<uint2*>(q + 2 * K::PLANE) =
+                *reinterpret_cast<uint2*>(q + 2 * PLANE) =
                     make_uint2(__builtin_amdgcn_perm(l[1], l[0], HI), __builtin_amdgcn_perm(l[3], l[2], HI));
             }
         }
@@ -189,29 +190,24 @@ __device__ __forceinline__ void along(const char* t, int row0, int k, bf16x8 (&f
         f[p] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(t + p * PLANE + row0 * RB + o));
 }
 // and across them: 16 columns of rows 32 k .., the p-th four of them at o0 (o1: four rows on)
-template <class K>
-__device__ __forceinline__ void across(const char* t, int k, int o0, int o1, bf16x8 (&f)[K::NPL]) {
+template <int RB, int NPL, int PLANE>
+__device__ __forceinline__ void across(const char* t, int k, int o0, int o1, bf16x8 (&f)[NPL]) {
 #pragma unroll
-    for (int p = 0; p < K::NPL; ++p) {
-        const char* u = t + p * K::PLANE + 32 * k * K::RB;
+    for (int p = 0; p < NPL; ++p) {
+        const char* u = t + p * PLANE + 32 * k * RB;
         f[p] = cat4(ld_tr4(reinterpret_cast<const uint16_t*>(u + o0)), ld_tr4(reinterpret_cast<const uint16_t*>(u + o1)));
     }
 }
-// of W: tile c of the wave's; of Y: tile j, every other four of 32 channels
-template <class K>
-__device__ __forceinline__ void w_frag(const char* W, int k, int c, bf16x8 (&f)[K::NPL]) {
-    const int l = lane_id(), j = l & 15, row = 8 * (l >> 4) + (j >> 2), w = (int)(threadIdx.x >> 6);
-    if constexpr (K::CW == 2) {
-        across<K>(W, k, Sw<K::RB>::at(row, 4 * w + (j & 3)) + 8 * c, Sw<K::RB>::at(row + 4, 4 * w + (j & 3)) + 8 * c, f);
-    } else {
-        const int piece = 2 * w + ((j & 3) >> 1), b = 8 * (j & 1);
-        across<K>(W, k, Sw<K::RB>::at(row, piece) + b, Sw<K::RB>::at(row + 4, piece) + b, f);
-    }
+// of W, columns 16 w .. of rows of RB bytes; of Y, tile t: every other four of 32 channels
+template <class K, int RB>
+__device__ __forceinline__ void w_frag(const char* W, int k, int w, bf16x8 (&f)[K::NPL]) {
+    const int l = lane_id(), j = l & 15, row = 8 * (l >> 4) + (j >> 2), piece = 2 * w + ((j & 3) >> 1), b = 8 * (j & 1);
+    across<RB, K::NPL, K::C * RB>(W, k, Sw<RB>::at(row, piece) + b, Sw<RB>::at(row + 4, piece) + b, f);
 }
 template <class K>
 __device__ __forceinline__ void y_frag(const char* Y, int k, int t, bf16x8 (&f)[K::NPL]) {
-    const int l = lane_id(), j = l & 15, row = 8 * (l >> 4) + (j >> 2);
-    across<K>(Y, k, Sw<K::RB>::at(row, j & 3, t >> 1) + 8 * (t & 1), Sw<K::RB>::at(row + 4, j & 3, t >> 1) + 8 * (t & 1), f);
+    const int l = lane_id(), j = l & 15, row = 8 * (l >> 4) + (j >> 2), b = 8 * (t & 1);
+    across<K::RB, K::NPL, K::PLANE>(Y, k, Sw<K::RB>::at(row, j & 3, t >> 1) + b, Sw<K::RB>::at(row + 4, j & 3, t >> 1) + b, f);
 }
 
 // A chunk's decays.  Sums of g are formed in fp64 (a difference of two sums of
@@ -233,19 +229,24 @@ __device__ __forceinline__ double dpp(double x) {   // 0 where there is no sourc
     return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_update_dpp(0, u.x, CTRL, ROWS, 0xf, true),
                                                  __builtin_amdgcn_update_dpp(0, u.y, CTRL, ROWS, 0xf, true)));
 }
+// sums over the lanes up to each, of 32; and the last of those, for all lanes
+__device__ __forceinline__ double prefix32(double x) {
+    x += dpp<0x111, 0xf>(x);   // row_shr:1, 2, 4, 8
+    x += dpp<0x112, 0xf>(x);
+    x += dpp<0x114, 0xf>(x);
+    x += dpp<0x118, 0xf>(x);
+    return x + dpp<0x142, 0xa>(x);   // row_bcast:15, into rows 1 and 3
+}
+__device__ __forceinline__ double lane31(double x) {
+    const uint2 u = __builtin_bit_cast(uint2, x);
+    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(u.x, 31), __builtin_amdgcn_readlane(u.y, 31)));
+}
 // by one wave: lane r has g of row r (0 behind the last); returns G_C
 template <int C>
 __device__ __forceinline__ double fill_decays(Decays<C>* d, float g) {
     static_assert(C == 32, "two rows of 16 lanes");
     const int l = lane_id();
-    double x = (double)(g < G_MIN ? G_MIN : g) * LOG2E;
-    x += dpp<0x111, 0xf>(x);   // row_shr:1, 2, 4, 8
-    x += dpp<0x112, 0xf>(x);
-    x += dpp<0x114, 0xf>(x);
-    x += dpp<0x118, 0xf>(x);
-    x += dpp<0x142, 0xa>(x);   // row_bcast:15, into rows 1 and 3
-    const uint2 u = __builtin_bit_cast(uint2, x);
-    const double all = __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(u.x, 31), __builtin_amdgcn_readlane(u.y, 31)));
+    const double x = prefix32((double)(g < G_MIN ? G_MIN : g) * LOG2E), all = lane31(x);
     if (l < C) {
         const float h = (float)x;
         d->hi[l] = h;
@@ -310,130 +311,107 @@ __device__ __forceinline__ void clear_upper(char* P) {
     }
 }
 
-// The state, the channels of W that are the wave's: lane (m = l % 16, r = l / 16) holds
-// St[32 (j / 2) + 8 r + 4 (j % 2) + i][channel(w, c, m)] in s[c][j][i].  In memory [W's channel]
-// [Y's], or (swapped) [Y's][W's].
+// The state, channels 16 w .. + 15 of W for wave w of all: lane (m = l % 16, r = l / 16) holds
+// St[32 (j / 2) + 8 r + 4 (j % 2) + i][16 w + m] in s[j][i].  In memory [W's channel][Y's], or
+// (swapped) [Y's][W's].
 template <class K>
 struct State {
-    f32x4 s[K::CW][K::DT];
-    __device__ __forceinline__ void load(const float* p, bool swapped) {
-        const int l = lane_id(), r = l >> 4;
+    f32x4 s[K::DT];
+    __device__ __forceinline__ void load(const float* p, int w, bool swapped) {
+        const int l = lane_id(), r = l >> 4, dw = 16 * w + (l & 15);
 #pragma unroll
-        for (int c = 0; c < K::CW; ++c) {
-            const int dw = channel<K>(threadIdx.x >> 6, c, l & 15);
+        for (int j = 0; j < K::DT; ++j) {
+            const int dy = 32 * (j >> 1) + 8 * r + 4 * (j & 1);
+            if (!p) { s[j] = zero4(); continue; }
+            if (!swapped) {
+                const float4 v = *reinterpret_cast<const float4*>(p + dw * K::D + dy);
+                s[j] = f32x4{v.x, v.y, v.z, v.w};
+            } else {
 #pragma unroll
-            for (int j = 0; j < K::DT; ++j) {
-                const int dy = 32 * (j >> 1) + 8 * r + 4 * (j & 1);
-                if (!p) { s[c][j] = zero4(); continue; }
-                if (!swapped) {
-                    const float4 v = *reinterpret_cast<const float4*>(p + dw * K::D + dy);
-                    s[c][j] = f32x4{v.x, v.y, v.z, v.w};
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[c][j][i] = p[(dy + i) * K::D + dw];
-                }
+                for (int i = 0; i < 4; ++i) s[j][i] = p[(dy + i) * K::D + dw];
             }
         }
     }
-    __device__ __forceinline__ void store(float* p, float scale) const {
-        const int l = lane_id(), r = l >> 4;
+    __device__ __forceinline__ void store(float* p, int w, float scale) const {
+        const int l = lane_id(), r = l >> 4, dw = 16 * w + (l & 15);
 #pragma unroll
-        for (int c = 0; c < K::CW; ++c) {
-            const int dw = channel<K>(threadIdx.x >> 6, c, l & 15);
+        for (int j = 0; j < K::DT; ++j)
+            *reinterpret_cast<float4*>(p + dw * K::D + 32 * (j >> 1) + 8 * r + 4 * (j & 1)) =
+                make_float4(scale * s[j][0], scale * s[j][1], scale * s[j][2], scale * s[j][3]);
+    }
+    // sum of s p over the wave's part, for all lanes; p as load's, swapped
+    __device__ __forceinline__ double dot(const float* p, int w) const {
+        const int l = lane_id(), r = l >> 4, dw = 16 * w + (l & 15);
+        double x = 0.0;
 #pragma unroll
-            for (int j = 0; j < K::DT; ++j)
-                *reinterpret_cast<float4*>(p + dw * K::D + 32 * (j >> 1) + 8 * r + 4 * (j & 1)) =
-                    make_float4(scale * s[c][j][0], scale * s[c][j][1], scale * s[c][j][2], scale * s[c][j][3]);
-        }
+        for (int j = 0; j < K::DT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x += (double)p[(32 * (j >> 1) + 8 * r + 4 * (j & 1) + i) * K::D + dw] * s[j][i];
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
+        return x;
     }
     // S <- all S + Y^T (down W): the chunk's sum from zero, so that what the matrix unit
     // loses (it rounds sums downwards) does not add up over the chunks.  w: w_frag of W.
-    __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::KC][K::CW][K::NPL], const Decays<K::C>& d) {
+    __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::NPL], const Decays<K::C>& d) {
         static_assert(K::KC == 1, "one step of the contracted index");
         const int r = lane_id() >> 4;
         const float4 d0 = *reinterpret_cast<const float4*>(d.down + 8 * r), d1 = *reinterpret_cast<const float4*>(d.down + 8 * r + 4);
         const float dn[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
-        bf16x8 ws[K::CW][3];
+        bf16x8 ws[3];
+        float v[8];
 #pragma unroll
-        for (int c = 0; c < K::CW; ++c) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = (float)w[0][c][0][e];
-                if constexpr (K::NPL == 3) v[e] += (float)w[0][c][1][e] + (float)w[0][c][2][e];
-                v[e] *= dn[e];
-            }
-            planes8<3>(v, ws[c]);
+        for (int e = 0; e < 8; ++e) {
+            v[e] = (float)w[0][e];
+            if constexpr (K::NPL == 3) v[e] += (float)w[1][e] + (float)w[2][e];
+            v[e] *= dn[e];
         }
+        planes8<3>(v, ws);
         const float all = d.all;
 #pragma unroll
         for (int j = 0; j < K::DT; ++j) {
             bf16x8 y[K::NPL];
             y_frag<K>(Y, 0, j, y);
+            const f32x4 u = mmp(y, ws, zero4());
 #pragma unroll
-            for (int c = 0; c < K::CW; ++c) {
-                const f32x4 u = mmp(y, ws[c], zero4());
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[c][j][i] = fmaf(all, s[c][j][i], u[i]);
-            }
+            for (int i = 0; i < 4; ++i) s[j][i] = fmaf(all, s[j][i], u[i]);
         }
     }
-    // up_t (St^T X_t) for every row, the state as NS planes: lane (m, r) has row 16 i + m, the
-    // channels of rows 4 r .. of tile c
+    // up_t (St^T X_t) for every row, the state as NS planes: lane (m, r) has row 16 i + m,
+    // channels 16 w + 4 r ..
     template <int NS>
-    __device__ __forceinline__ void apply(const char* X, const Decays<K::C>& d, f32x4 (&o)[K::TT][K::CW]) const {
+    __device__ __forceinline__ void apply(const char* X, const Decays<K::C>& d, f32x4 (&o)[K::TT]) const {
 #pragma unroll
-        for (int i = 0; i < K::TT; ++i)
-#pragma unroll
-            for (int c = 0; c < K::CW; ++c) o[i][c] = zero4();
+        for (int i = 0; i < K::TT; ++i) o[i] = zero4();
 #pragma unroll
         for (int k = 0; k < K::KD; ++k) {
-            bf16x8 f[K::CW][NS];
-#pragma unroll
-            for (int c = 0; c < K::CW; ++c) {
-                const f32x4 &x = s[c][2 * k], &y = s[c][2 * k + 1];
-                const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-                planes8<NS>(v, f[c]);
-            }
+            const f32x4 &x = s[2 * k], &y = s[2 * k + 1];
+            const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            bf16x8 f[NS];
+            planes8<NS>(v, f);
 #pragma unroll
             for (int i = 0; i < K::TT; ++i) {
                 bf16x8 x[K::NPL];
                 along<K::RB, K::NPL, K::PLANE>(X, 16 * i, k, x);
-#pragma unroll
-                for (int c = 0; c < K::CW; ++c) o[i][c] = mmp(f[c], x, o[i][c]);
+                o[i] = mmp(f, x, o[i]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < K::TT; ++i) {
-            const float up = d.up[16 * i + (lane_id() & 15)];
-#pragma unroll
-            for (int c = 0; c < K::CW; ++c) o[i][c] *= up;
-        }
+        for (int i = 0; i < K::TT; ++i) o[i] *= d.up[16 * i + (lane_id() & 15)];
     }
 };
 
 // o_t += sum_s P[t][s] W_s, layout as State::apply
 template <class K, int NP>
-__device__ __forceinline__ void add_pairs(const char* P, const bf16x8 (&w)[K::KC][K::CW][K::NPL], f32x4 (&o)[K::TT][K::CW]) {
+__device__ __forceinline__ void add_pairs(const char* P, const bf16x8 (&w)[K::NPL], f32x4 (&o)[K::TT]) {
 #pragma unroll
-    for (int k = 0; k < K::KC; ++k)
-#pragma unroll
-        for (int i = 2 * k; i < K::TT; ++i) {
-            bf16x8 p[NP];
-            along<K::RP, NP, K::PPL>(P, 16 * i, k, p);
-#pragma unroll
-            for (int c = 0; c < K::CW; ++c) o[i][c] = mmp(w[k][c], p, o[i][c]);
-        }
-}
-template <class K>
-__device__ __forceinline__ void w_frags(const char* W, bf16x8 (&w)[K::KC][K::CW][K::NPL]) {
-#pragma unroll
-    for (int k = 0; k < K::KC; ++k)
-#pragma unroll
-        for (int c = 0; c < K::CW; ++c) w_frag<K>(W, k, c, w[k][c]);
+    for (int i = 0; i < K::TT; ++i) {
+        bf16x8 p[NP];
+        along<K::RP, NP, K::PPL>(P, 16 * i, 0, p);
+        o[i] = mmp(w, p, o[i]);
+    }
 }
 
-// a wave's channels of the rows of a chunk, the first in memory at out
 template <typename T>
 __device__ __forceinline__ void put4(T* p, const f32x4& v) {
     if constexpr (std::is_same<T, float>::value)
@@ -441,21 +419,14 @@ __device__ __forceinline__ void put4(T* p, const f32x4& v) {
     else
         *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
 }
+// wave w's channels of the rows of a chunk, the first in memory at out
 template <class K, typename OT, bool REV>
-__device__ __forceinline__ void put_rows(OT* out, uint32_t step, const f32x4 (&o)[K::TT][K::CW], int n) {
-    const int l = lane_id(), w = threadIdx.x >> 6, r = l >> 4;
+__device__ __forceinline__ void put_rows(OT* out, uint32_t step, const f32x4 (&o)[K::TT], int w, int n) {
+    const int l = lane_id();
 #pragma unroll
     for (int i = 0; i < K::TT; ++i) {
         const int t = 16 * i + (l & 15);
-        if (t >= n) continue;
-        OT* p = out + (uint32_t)(REV ? n - 1 - t : t) * step + channel<K>(w, 0, 4 * r);
-        if constexpr (K::CW == 2 && !std::is_same<OT, float>::value) {
-            *reinterpret_cast<uint4*>(p) = make_uint4(pack2bf(o[i][0][0], o[i][0][1]), pack2bf(o[i][0][2], o[i][0][3]),
-                                                      pack2bf(o[i][1][0], o[i][1][1]), pack2bf(o[i][1][2], o[i][1][3]));
-        } else {
-#pragma unroll
-            for (int c = 0; c < K::CW; ++c) put4<OT>(p + 4 * c, o[i][c]);
-        }
+        if (t < n) put4<OT>(out + (uint32_t)(REV ? n - 1 - t : t) * step + 16 * w + 4 * (l >> 4), o[i]);
     }
 }
 __device__ __forceinline__ float quad_sum(float x) {   // over the four lanes of equal l % 16
@@ -480,13 +451,14 @@ __device__ __forceinline__ void clear_rows(void* out, const DecayArgs& a, const 
 
 template <class K, int NP>
 constexpr size_t mix_lds(bool states, bool dot) {
-    return (states ? 2 : 3) * (size_t)K::TILE + (states ? 0 : (size_t)NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
+    return (states ? 1 : 2) * (size_t)K::TILE + K::TILEW + (states ? 0 : (size_t)NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
            (dot ? (size_t)K::NW * K::C * 4 : 0);
 }
 
 // mix: out = the operator over a slot's tokens (REV: backwards in time).  STATES: only
 // what the slot adds to the state, and its whole decay.  DOT: dots[t] = z_t . (the part
-// of out_t that comes from the state before the chunk), which NS = 3 keeps to fp32.
+// of out_t that comes from the state before the chunk), which NS = 3 keeps to fp32; by
+// parts of the channels.
 //
 // A chunk: pairs, state and the state's part of out from LDS; a barrier; the pairs'
 // part from P and registers, and the next chunk into LDS; a barrier.  Its loads are in
@@ -499,26 +471,28 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
     char* X = lds;
     char* Y = X + (STATES ? 0 : K::TILE);
     char* W = Y + K::TILE;
-    char* P = W + K::TILE;
+    char* P = W + K::TILEW;
     Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : NP * K::PPL));
     float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]
 
-    const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x), j = bid / a.H, h = bid - j * a.H;
+    const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x), cols = bid % K::SPLIT, jh = bid / K::SPLIT, j = jh / a.H, h = jh - j * a.H;
     const Slot s = slot_of(a, j);
     if (s.seq < 0) {
         if constexpr (!STATES) {
-            if (s.seq == -1) clear_rows<K::D, OT>(a.out, a, s, h);
+            if (s.seq == -1 && cols == 0) clear_rows<K::D, OT>(a.out, a, s, h);
         }
         return;
     }
     if (STATES && (REV ? s.first : s.last)) return;   // nothing follows
     const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+    const int wv = cols * K::NW + wave;   // of all
     constexpr int DD = K::D * K::D, LAST = K::NW - 1;
     State<K> st;
-    st.load(STATES || !a.s_in ? nullptr : a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD, swapped);
+    st.load(STATES || !a.s_in ? nullptr : a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD, wv, swapped);
 
     const float* g = a.g + b * a.gb + (int64_t)s.tok0 * a.gt + h * a.gh;
-    Stage<K, REV> sx, sy, sw;
+    Stage<K, K::D, REV> sx, sy;
+    Stage<K, K::DW, REV> sw;
     float gv = 0.f;
     // the first row in memory of the chunk at i0
     auto lowest = [&](int i0, int n) { return s.tok0 + (REV ? s.n - i0 - n : i0); };
@@ -526,7 +500,7 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
         const int n = min(K::C, s.n - i0), t = lowest(i0, n);
         if constexpr (!STATES) sx.load(at<ST>(a.x, b, t, h), (uint32_t)a.x.token * K::ES, n);
         sy.load(at<ST>(a.y, b, t, h), (uint32_t)a.y.token * K::ES, n);
-        sw.load(at<ST>(a.w, b, t, h), (uint32_t)a.w.token * K::ES, n);
+        sw.load(at<ST>(a.w, b, t, h) + cols * K::DW, (uint32_t)a.w.token * K::ES, n);
     };
     // backwards, row i decays by what its successor in time does; the first by nothing
     auto load_g = [&](int i0) {
@@ -555,17 +529,16 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
         const int n = min(K::C, s.n - i0);
         const Decays<K::C>& d = dec[i0 / K::C & 1];
         const bool more = i0 + K::C < s.n;
-        bf16x8 w[K::KC][K::CW][K::NPL];
-        f32x4 o[K::TT][K::CW];
-        w_frags<K>(W, w);
-        float4 z[DOT ? K::TT : 1][K::CW];
+        bf16x8 w[K::NPL];
+        f32x4 o[K::TT];
+        w_frag<K, K::RBW>(W, 0, wave, w);
+        float4 z[DOT ? K::TT : 1];
         if constexpr (DOT) {
-            const ST* p = at<ST>(a.z, b, lowest(i0, n), h) + channel<K>(wave, 0, 4 * (l >> 4));
+            const ST* p = at<ST>(a.z, b, lowest(i0, n), h) + 16 * wv + 4 * (l >> 4);
 #pragma unroll
             for (int i = 0; i < K::TT; ++i) {
                 const int m = min(16 * i + (l & 15), n - 1);
-#pragma unroll
-                for (int c = 0; c < K::CW; ++c) z[i][c] = ld4<ST>(p + (REV ? n - 1 - m : m) * (int)a.z.token + 4 * c);
+                z[i] = ld4<ST>(p + (REV ? n - 1 - m : m) * (int)a.z.token);
             }
         }
         if constexpr (!STATES) {
@@ -584,10 +557,7 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
             if constexpr (DOT) {
 #pragma unroll
                 for (int i = 0; i < K::TT; ++i) {
-                    float x = 0.f;
-#pragma unroll
-                    for (int c = 0; c < K::CW; ++c) x += dot4(z[i][c], o[i][c]);
-                    x = quad_sum(x);
+                    const float x = quad_sum(dot4(z[i], o[i]));
                     if (l < 16) part[wave * K::C + 16 * i + l] = x;
                 }
             }
@@ -605,14 +575,14 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
         if constexpr (!STATES) {
             const int64_t row = (int64_t)b * a.T + lowest(i0, n);
             add_pairs<K, NP>(P, w, o);
-            put_rows<K, OT, REV>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, n);
+            put_rows<K, OT, REV>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, wv, n);
             if constexpr (DOT) {
                 const int t = threadIdx.x;
                 if (t < n) {
                     float x = 0.f;
 #pragma unroll
                     for (int k = 0; k < K::NW; ++k) x += part[k * K::C + t];
-                    a.dots[(int64_t)h * a.B * a.T + row + (REV ? n - 1 - t : t)] = x;
+                    a.dots[((int64_t)cols * a.H + h) * a.B * a.T + row + (REV ? n - 1 - t : t)] = x;
                 }
             }
         }
@@ -622,12 +592,12 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
         // backwards: to before the slot's first token
         float last = 1.f;
         if constexpr (REV) last = decay(g[0]);
-        if (wave == LAST && l == 0) a.seg[(int64_t)j * a.H + h] = __builtin_amdgcn_exp2f((float)whole) * last;
-        st.store(a.s_out + ((int64_t)j * a.H + h) * DD, last);
+        if (wave == LAST && l == 0 && cols == 0) a.seg[(int64_t)j * a.H + h] = __builtin_amdgcn_exp2f((float)whole) * last;
+        st.store(a.s_out + ((int64_t)j * a.H + h) * DD, wv, last);
     } else if (a.s_out && (REV ? s.first : s.last)) {
         float last = 1.f;
         if constexpr (REV) last = s.n > 0 ? decay(g[0]) : 1.f;
-        st.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, last);
+        st.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, wv, last);
     }
 }
 
@@ -640,13 +610,18 @@ constexpr size_t mix2_lds(bool dot) {
 constexpr float ANCHOR_BELOW = 0x1p-32f;
 
 // mix2: dk and dv of a slot, backwards in time, from q (y), k (x), v (z) and do (w), with
-// dS in both orders: dv = mix(k, q, do), dk = mix(v, do, q).  DOT: dots[t] -= k_t . (the part
-// of dk_t from behind the chunk); dots2[t] = rows - columns of E, E_{ts} = e^{G_t - G_s}
-// (q_t . k_s) (do_t . v_s), whose sums over s and over t are what the chunk's own pairs
-// give q . dq and k . dk; and where nothing passes through a whole chunk anchors[chunk], all
-// that leaves it.
-template <class K, typename OT, int NP, int NS, bool DOT>
+// dS in both orders: dv = mix(k, q, do), dk = mix(v, do, q).
+// DOT: dg too, what passes from before token t to t or later.  With a_t and b_t the parts of
+// q_t . dq_t and k_t . dk_t that come through the state (a: dots, from mix), and E_{ts} =
+// e^{G_t - G_s} (q_t . k_s) (do_t . v_s) the chunk's own pairs, s < t,
+//   dg_t = <S, dS> behind the chunk + sum of a - b from t on + sum of E_{t' s}, t' >= t > s.
+// What the pairs give stays in their chunk, and where nothing passes through a chunk <S, dS>
+// behind it begins anew, as all that leaves it (the sum of b): with all of q . dq - k . dk in
+// one sum over the slot, dg of fast decays was 2 to 60 times as far off.  Sums in fp64.
+// PARTS: of dots, by channels.
+template <class K, typename OT, int NP, int NS, bool DOT, int PARTS>
 __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const DecayArgs a) {
+    static_assert(K::SPLIT == 1, "dg takes all channels");
     typedef typename K::ST ST;
     __shared__ __attribute__((aligned(16))) char lds[mix2_lds<K, NP>(DOT)];
     char* Kt = lds;
@@ -666,18 +641,34 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         if (s.seq == -1) {
             clear_rows<K::D, OT>(a.out, a, s, h);
             clear_rows<K::D, OT>(a.out2, a, s, h);
+            if (DOT && a.dg)
+                for (int i = threadIdx.x; i < s.n; i += K::NTH) a.dg[(int64_t)(s.tok0 + i) * a.H + h] = 0.f;
         }
+        if (DOT && a.sums && threadIdx.x == 0) a.sums[(int64_t)j * a.H + h] = 0.0;
         return;
     }
     const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
     constexpr int DD = K::D * K::D, LAST = K::NW - 1;
     const float* s_in = a.s_in ? a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD : nullptr;
     State<K> sv, sk;   // dv's: [do][q]; dk's: [q][do]
-    sv.load(s_in, false);
-    sk.load(s_in, true);
+    sv.load(s_in, wave, false);
+    sk.load(s_in, wave, true);
+    double passing = 0.0;   // <S, dS> behind the chunk
+    if constexpr (DOT) {
+        if (s_in && (!s.last || a.s_final)) {
+            const float* p = s.last ? a.s_final + ((int64_t)s.seq * a.H + h) * DD : a.starts + ((int64_t)(j + 1) * a.H + h) * DD;
+            double* sums = reinterpret_cast<double*>(lds);
+            const double x = sk.dot(p, wave);
+            if (l == 0) sums[wave] = x;
+            lds_barrier();
+#pragma unroll
+            for (int k = 0; k < K::NW; ++k) passing += sums[k];
+            lds_barrier();
+        }
+    }
 
     const float* g = a.g + b * a.gb + (int64_t)s.tok0 * a.gt + h * a.gh;
-    Stage<K, true> rk, rq, rv, ro;
+    Stage<K, K::D, true> rk, rq, rv, ro;
     float gv = 0.f;
     // the chunks are those of a pass forwards, so that dots and the sums of mix over them add up:
     // rows [i0, i0 + n) backwards, all but the first C of them
@@ -693,6 +684,20 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         const int i = i0 + l;
         gv = l < n && i > 0 && i < s.n ? g[(int64_t)(s.n - i) * a.gt] : 0.f;
     };
+    // dots and g of the chunk's tokens, in wave 0
+    float av = 0.f, gt = 0.f;
+    double whole = 0.0;
+    auto load_a = [&](int i0, int n) {
+        const int i = i0 + l, t = s.n - 1 - i;
+        if (DOT && wave == 0) {
+            const bool in = l < n && i < s.n;
+            av = 0.f;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                if (in) av += a.dots[((int64_t)p * a.H + h) * a.B * a.T + (int64_t)b * a.T + s.tok0 + t];
+            gt = in ? g[(int64_t)t * a.gt] : 0.f;
+        }
+    };
     auto store = [&](int n) {
         rk.store(Kt, n);
         rq.store(Q, n);
@@ -705,6 +710,7 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         for (int v = threadIdx.x; v < 2 * K::TT * K::C; v += K::NTH) e_own[v] = 0.f;
     if (s.n > 0) {
         load(0, n0);
+        load_a(0, n0);
         if (wave == LAST) {
             load_g(0, n0);
             fill_decays<K::C>(dec, gv);
@@ -718,9 +724,9 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
     for (int i0 = 0, n = n0; i0 < s.n; i0 += n, n = K::C, turn ^= 1) {
         const Decays<K::C>& d = dec[turn];
         const bool more = i0 + n < s.n;
-        bf16x8 wo[K::KC][K::CW][K::NPL], wq[K::KC][K::CW][K::NPL];
-        w_frags<K>(O, wo);
-        w_frags<K>(Q, wq);
+        bf16x8 wo[K::NPL], wq[K::NPL];
+        w_frag<K, K::RB>(O, 0, wave, wo);
+        w_frag<K, K::RB>(Q, 0, wave, wq);
 #pragma unroll
         for (int k = 0; k < (K::NT + K::NW - 1) / K::NW; ++k) {
             const int id = wave + K::NW * k;
@@ -749,30 +755,25 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
                 }
             }
         }
-        f32x4 o[K::TT][K::CW], o2[K::TT][K::CW];
-        sv.template apply<NS>(Kt, d, o);
+        f32x4 o[K::TT], o2[K::TT];
+        sv.template apply<K::NPL == 3 ? 3 : NP>(Kt, d, o);
+        sk.template apply<NS>(V, d, o2);
         if constexpr (DOT) {
-            const int ch = channel<K>(wave, 0, 4 * (l >> 4));
+            const int ch = 16 * wave + 4 * (l >> 4);
 #pragma unroll
             for (int i = 0; i < K::TT; ++i) {
                 const int t = 16 * i + (l & 15);
-                float x = 0.f;
-#pragma unroll
-                for (int c = 0; c < K::CW; ++c) {
-                    const char* p = V + Sw<K::RB>::at(t, (ch + 4 * c) >> 3) + 2 * ((ch + 4 * c) & 7);
-                    float4 v = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p));
-                    if constexpr (K::NPL == 3) {
-                        const float4 v1 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + K::PLANE)),
-                                     v2 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + 2 * K::PLANE));
-                        v = make_float4(v.x + (v1.x + v2.x), v.y + (v1.y + v2.y), v.z + (v1.z + v2.z), v.w + (v1.w + v2.w));
-                    }
-                    x += dot4(v, o[i][c]);
+                const char* p = Kt + Sw<K::RB>::at(t, ch >> 3) + 2 * (ch & 7);
+                float4 v = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p));
+                if constexpr (K::NPL == 3) {
+                    const float4 v1 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + K::PLANE)),
+                                 v2 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + 2 * K::PLANE));
+                    v = make_float4(v.x + (v1.x + v2.x), v.y + (v1.y + v2.y), v.z + (v1.z + v2.z), v.w + (v1.w + v2.w));
                 }
-                x = quad_sum(x);
+                const float x = quad_sum(dot4(v, o2[i]));
                 if (l < 16) part[wave * K::C + t] = x;
             }
         }
-        sk.template apply<K::NPL == 3 ? 3 : NP>(V, d, o2);
         sv.add(Q, wo, d);
         sk.add(O, wq, d);
         if (wave == LAST && more) {
@@ -788,35 +789,43 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         const int64_t row = (int64_t)b * a.T + s.tok0 + s.n - i0 - n, out = (row * a.H + h) * K::D;
         add_pairs<K, NP>(PA, wo, o);
         add_pairs<K, NP>(PD, wq, o2);
-        put_rows<K, OT, true>(static_cast<OT*>(a.out) + out, (uint32_t)(a.H * K::D), o2, n);
-        put_rows<K, OT, true>(static_cast<OT*>(a.out2) + out, (uint32_t)(a.H * K::D), o, n);
+        put_rows<K, OT, true>(static_cast<OT*>(a.out) + out, (uint32_t)(a.H * K::D), o2, wave, n);
+        put_rows<K, OT, true>(static_cast<OT*>(a.out2) + out, (uint32_t)(a.H * K::D), o, wave, n);
         if constexpr (DOT) {
             if (wave == 0) {
-                const int t = l;
-                float x = 0.f;
-                if (t < n) {
-                    float own = 0.f, oth = 0.f;
+                float x = 0.f, own = 0.f, oth = 0.f;
+                if (l < n) {
 #pragma unroll
                     for (int k = 0; k < K::TT; ++k) {
-                        own += e_own[k * K::C + t];
-                        oth += e_oth[k * K::C + t];
+                        own += e_own[k * K::C + l];
+                        oth += e_oth[k * K::C + l];
                     }
 #pragma unroll
-                    for (int k = 0; k < K::NW; ++k) x += part[k * K::C + t];
-                    const int64_t at = (int64_t)h * a.B * a.T + row + (n - 1 - t);
-                    a.dots[at] -= x;
-                    a.dots2[at] = oth - own;
+                    for (int k = 0; k < K::NW; ++k) x += part[k * K::C + l];
                 }
-#pragma unroll
-                for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k, 64);
-                if (l == 0)
-                    a.anchors[((int64_t)j * a.H + h) * (a.seg_tokens / K::C) + (s.n - i0 - 1) / K::C] =
-                        all < ANCHOR_BELOW ? x : __builtin_nanf("");
+                // lane l: token n - 1 - l of the chunk
+                const double pairs = prefix32((double)oth - (double)own), through = prefix32((double)av - (double)x);
+                if (all < ANCHOR_BELOW) passing = lane31(prefix32((double)x));
+                if (l < n) {
+                    // (nothing passes a decay of zero: exactly)
+                    const double v = gt < G_MIN ? 0.0 : (passing + through) + pairs;
+                    if (a.dg) a.dg[(row + (n - 1 - l)) * a.H + h] = (float)v;
+                    whole += v;
+                }
+                passing += lane31(through);
+                load_a(i0 + n, K::C);
             }
         }
         if (more) lds_barrier();
     }
-    if (a.s_out && s.first) sv.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, s.n > 0 ? decay(g[0]) : 1.f);
+    if constexpr (DOT) {
+        if (a.sums && wave == 0) {
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) whole += __shfl_xor(whole, m, 64);
+            if (l == 0) a.sums[(int64_t)j * a.H + h] = whole;
+        }
+    }
+    if (a.s_out && s.first) sv.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, wave, s.n > 0 ? decay(g[0]) : 1.f);
 }
 
 // ----------------------------------------------------------------------------
@@ -887,130 +896,46 @@ __global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, 
 }
 
 // The state at each slot's start (REV: its adjoint at each slot's end), in place of
-// what the slots add: one thread takes four elements through a sequence's slots, sixteen
+// what the slots add: one thread takes two elements through a sequence's slots, 16
 // loads at a time.
+constexpr int SCAN_PER = 2;
 template <bool REV>
 __global__ __launch_bounds__(256) void kda_decay_scan_kernel(float* u, const float* seg, const float* s0, const int* first,
                                                              int per_seq, int H, int DD, int parts) {
+    typedef float vec __attribute__((ext_vector_type(SCAN_PER)));
     const int part = blockIdx.x % parts, sh = blockIdx.x / parts, seq = sh / H, h = sh - seq * H;
-    const int e = 4 * (part * 256 + (int)threadIdx.x);
+    const int e = SCAN_PER * (part * 256 + (int)threadIdx.x);
     if (e >= DD) return;
     const int lo = first ? first[seq] : seq * per_seq, count = (first ? first[seq + 1] : lo + per_seq) - lo;
-    float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (s0) run = *reinterpret_cast<const float4*>(s0 + ((int64_t)seq * H + h) * DD + e);
+    vec run = 0.f;
+    if (s0) run = *reinterpret_cast<const vec*>(s0 + ((int64_t)seq * H + h) * DD + e);
     auto slot = [&](int i) { return (int64_t)(REV ? lo + count - 1 - i : lo + i) * H + h; };
-    constexpr int AHEAD = 16;
-    for (int i0 = 0; i0 < count; i0 += AHEAD) {
-        float4 v[AHEAD];
-        float f[AHEAD];
+    int i = 0;
+    // (the last one adds nothing to a start)
+    auto batch = [&](auto size) {
+        constexpr int N = size();
+        for (; i + N <= count - 1; i += N) {
+            vec v[N];
+            float f[N];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            // (the last one adds nothing to a start)
-            const int64_t at = slot(min(i0 + k, count - 1));
-            const bool any = i0 + k < count - 1;
-            v[k] = any ? *reinterpret_cast<const float4*>(u + at * DD + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-            f[k] = any ? seg[at] : 0.f;
-        }
+            for (int k = 0; k < N; ++k) {
+                v[k] = *reinterpret_cast<const vec*>(u + slot(i + k) * DD + e);
+                f[k] = seg[slot(i + k)];
+            }
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            if (i0 + k < count) {
-                *reinterpret_cast<float4*>(u + slot(i0 + k) * DD + e) = run;
-                run = make_float4(fmaf(f[k], run.x, v[k].x), fmaf(f[k], run.y, v[k].y), fmaf(f[k], run.z, v[k].z),
-                                  fmaf(f[k], run.w, v[k].w));
+            for (int k = 0; k < N; ++k) {
+                *reinterpret_cast<vec*>(u + slot(i + k) * DD + e) = run;
+#pragma unroll
+                for (int x = 0; x < SCAN_PER; ++x) run[x] = fmaf(f[k], run[x], v[k][x]);
             }
         }
-    }
+    };
+    batch(std::integral_constant<int, 16>());
+    batch(std::integral_constant<int, 4>());
+    batch(std::integral_constant<int, 1>());
+    if (count) *reinterpret_cast<vec*>(u + slot(count - 1) * DD + e) = run;
 }
 
-// dg of a slot: what passes from before token t to t or later,
-//   <S, dS> at the slot's end + sum_{s >= t} dots_s + sum_{s >= t, in t's chunk} dots2_s.
-// A chunk's dots2 add up to nothing, so their errors stay in it, and where nothing passes
-// through a chunk the first two begin anew at its end, with what leaves it: with all of
-// q . dq - k . dk in one sum over the slot, dg of fast decays was 2 to 60 times as far
-// off.  Sums in fp64.
-// s_end, ds_end: the state and its adjoint at a slot's end (the last slot's by sequence).
-// sums (not null): only the slot's whole sum.
-constexpr int DG_TH = 256;
-__global__ __launch_bounds__(DG_TH) void kda_decay_dg_kernel(const DecayArgs a, const float* starts, const float* dends,
-                                                             const float* s_final, const float* ds_final, float* dg,
-                                                             double* sums, int DD, int C) {
-    __shared__ double buf[DG_TH / 32];
-    const int j = blockIdx.x / a.H, h = blockIdx.x - j * a.H, t = threadIdx.x, l = t & 63, w = t >> 6;
-    const Slot s = slot_of(a, j);
-    if (s.seq < 0) {
-        if (s.seq == -1 && dg)
-            for (int i = t; i < s.n; i += DG_TH) dg[(int64_t)(s.tok0 + i) * a.H + h] = 0.f;
-        if (sums && t == 0) sums[(int64_t)j * a.H + h] = 0.0;
-        return;
-    }
-    auto all = [&](double x) {
-#pragma unroll
-        for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k, 64);
-        __syncthreads();
-        if (l == 0) buf[w] = x;
-        __syncthreads();
-        double y = 0.0;
-#pragma unroll
-        for (int k = 0; k < DG_TH / 64; ++k) y += buf[k];
-        return y;
-    };
-    const float *p = nullptr, *q = nullptr;
-    if (s.last) {
-        if (ds_final) {
-            p = s_final + ((int64_t)s.seq * a.H + h) * DD;
-            q = ds_final + ((int64_t)s.seq * a.H + h) * DD;
-        }
-    } else {
-        p = starts + ((int64_t)(j + 1) * a.H + h) * DD;
-        q = dends + ((int64_t)j * a.H + h) * DD;
-    }
-    double run = 0.0;
-    if (p) {
-        for (int e = 4 * t; e < DD; e += 4 * DG_TH) {
-            const float4 x = *reinterpret_cast<const float4*>(p + e), y = *reinterpret_cast<const float4*>(q + e);
-            run += ((double)x.x * y.x + (double)x.y * y.y) + ((double)x.z * y.z + (double)x.w * y.w);
-        }
-        run = all(run);
-    }
-    const int b = a.tab ? 0 : s.seq;
-    const int64_t base = (int64_t)h * a.B * a.T + (int64_t)b * a.T + s.tok0;
-    double whole = 0.0;
-    // 256 tokens a step from the last on; lane l of wave w has token i0 + 64 w + l
-    const float* anchors = a.anchors + ((int64_t)j * a.H + h) * (a.seg_tokens / C);
-    const int own = t / C;
-    for (int i0 = (s.n - 1) / DG_TH * DG_TH; i0 >= 0; i0 -= DG_TH) {
-        const int i = i0 + t;
-        double x = i < s.n ? (double)a.dots[base + i] : 0.0, e = i < s.n ? (double)a.dots2[base + i] : 0.0;
-#pragma unroll
-        for (int k = 1; k < 64; k <<= 1) {
-            const double y = __shfl_down(x, k, 64), f = __shfl_down(e, k, 64);
-            if ((l & (C - 1)) + k < C) { x += y; e += f; }
-        }
-        __syncthreads();
-        if (t % C == 0) buf[own] = x;
-        __syncthreads();
-        double behind = 0.0;
-        for (int k = DG_TH / C - 1; k >= 0; --k) {
-            if (i0 + k * C < s.n) {
-                const float anchor = anchors[i0 / C + k];
-                if (anchor == anchor) run = (double)anchor;
-            }
-            if (k == own) behind = run;
-            run += buf[k];
-        }
-        if (i < s.n) {
-            // (nothing passes a decay of zero: exactly)
-            const float g = a.g[b * a.gb + (int64_t)(s.tok0 + i) * a.gt + h * a.gh];
-            const double v = g < G_MIN ? 0.0 : (behind + x) + e;
-            if (dg) dg[((int64_t)b * a.T + s.tok0 + i) * a.H + h] = (float)v;
-            whole += v;
-        }
-    }
-    if (sums) {
-        whole = all(whole);
-        if (t == 0) sums[(int64_t)j * a.H + h] = whole;
-    }
-}
 // one decay a head: its gradient is the sum over the slots
 __global__ __launch_bounds__(64) void kda_decay_dg_sum_kernel(const double* sums, float* dg, int nslots, int H) {
     double x = 0.0;
@@ -1128,15 +1053,15 @@ struct Plan {
 // over them, and the workgroups come in rounds of as many as fit beside each other
 // (measured at D = 64: a chunk takes 0.4 of a full card's time in a workgroup alone, a
 // slot 1 / 40 of it in the scan): the least of all counts.
-Plan plan_of(const Args& a, bool bwd) {
+Plan plan_of(const Args& a, bool train) {
     Plan p;
     p.packed = a.cu != nullptr;
     const int64_t seqs = p.packed ? a.nseq : a.B, rows = p.packed ? 1 : a.B, chunks = std::max<int64_t>(1, (a.T + 63) / 64);
     // dg is a sum over a slot's tokens, whose errors add up
-    const int64_t most = bwd && a.dg ? 32 : chunks, fit = a.D <= 64 ? 1024 : 512;
+    const int64_t most = train ? 32 : chunks, fit = a.D <= 64 ? 1024 : 512;
     double best = 0.0;
     int64_t seg = 0;
-    for (int64_t c = 1; c <= most; c = c == chunks ? most + 1 : c >= 64 ? chunks : c + 1) {
+    for (int64_t c = 1; c <= most; c = c < 64 || c == chunks ? c + 1 : chunks) {
         const int64_t per = (chunks + c - 1) / c, n = (p.packed ? per + seqs / 2 : rows * per) * a.H, rest = n % fit;
         const double turns = (double)(n / fit) + (rest ? 0.4 + 0.6 * (double)rest / fit : 0.0);
         const double cost = (double)c * turns * (p.packed || per > 1 ? 1.5 : 1.0) + (per > 1 ? 0.5 + 0.025 * per : 0.0);
@@ -1148,43 +1073,39 @@ Plan plan_of(const Args& a, bool bwd) {
     p.seg_tokens = (int)(64 * seg);
     p.per_seq = p.packed ? 0 : (int)((chunks + seg - 1) / seg);
     const int64_t n = p.packed ? a.nseq + 2 + a.T / p.seg_tokens : a.B * p.per_seq;
-    p.nslots = n * a.H > 0x7fffffff ? -1 : (int)n;
+    p.nslots = n * a.H > 0x3fffffff ? -1 : (int)n;
     p.multi = p.packed || p.per_seq > 1;
     return p;
 }
 
-// the workspace's parts, offsets in bytes
+// Parts in bytes: the slots and the states at their starts, which the backward pass reads
+// again (kept); and the backward pass' own
 struct Layout {
-    int64_t tab = -1, first = -1, s = -1, seg = -1, ds = -1, segd = -1, dots = -1, anchors = -1, sums = -1, g0 = -1, g1 = -1, bytes = 0;
+    int64_t tab = -1, first = -1, s = -1, seg = -1, kept = 0;
+    int64_t ds = -1, segd = -1, dots = -1, sums = -1, g0 = -1, g1 = -1, bytes = 0;
 };
 bool shared(const Args& a, const kda_decay_rows& r) { return r.heads != a.H; }
-Layout layout_of(const Args& a, const Plan& p, bool bwd) {
+Layout layout_of(const Args& a, const Plan& p) {
     Layout l;
-    auto take = [&](int64_t n) { const int64_t at = l.bytes; l.bytes += up16(n); return at; };
+    auto take = [](int64_t& at, int64_t n) { const int64_t x = at; at += up16(n); return x; };
     if (p.packed) {
-        l.tab = take(16 * (int64_t)p.nslots);
-        l.first = take(4 * (a.nseq + 1));
+        l.tab = take(l.kept, 16 * (int64_t)p.nslots);
+        l.first = take(l.kept, 4 * (a.nseq + 1));
     }
-    const int64_t st = 4 * (int64_t)p.nslots * a.H * a.D * a.D, sg = 4 * (int64_t)p.nslots * a.H;
+    const int64_t st = 4 * (int64_t)p.nslots * a.H * a.D * a.D, sg = 4 * (int64_t)p.nslots * a.H, rows = 4 * a.B * a.T * a.H;
     if (p.multi) {
-        l.s = take(st);
-        l.seg = take(sg);
+        l.s = take(l.kept, st);
+        l.seg = take(l.kept, sg);
+        l.ds = take(l.bytes, st);
+        l.segd = take(l.bytes, sg);
     }
-    if (bwd) {
-        if (p.multi) {
-            l.ds = take(st);
-            l.segd = take(sg);
-        }
-        if (a.dg) {
-            l.dots = take(2 * 4 * a.H * a.B * a.T);
-            l.anchors = take(sg * (p.seg_tokens / 32));
-            if (a.dg_heads) l.sums = take(2 * sg);
-        }
-        const int64_t rows = 4 * a.B * a.T * a.H * a.D;
-        const bool kv = shared(a, a.k) || shared(a, a.v);
-        if (kv || shared(a, a.q)) l.g0 = take(rows);
-        if (kv) l.g1 = take(rows);
+    if (a.dg) {
+        l.dots = take(l.bytes, 2 * rows);   // (of two parts of the channels)
+        if (a.dg_heads) l.sums = take(l.bytes, 2 * sg);
     }
+    const bool kv = shared(a, a.k) || shared(a, a.v);
+    if (kv || shared(a, a.q)) l.g0 = take(l.bytes, rows * a.D);
+    if (kv) l.g1 = take(l.bytes, rows * a.D);
     return l;
 }
 
@@ -1236,43 +1157,34 @@ int check_ptr(const void* p, const char* name, int align) {
 
 Rows rows_of(const Args& a, const kda_decay_rows& r) { return {r.p, r.batch, r.token, r.head, (int)(a.H / r.heads)}; }
 
-DecayArgs base_of(const Args& a, const Plan& p, const Layout& l) {
+DecayArgs base_of(const Args& a, const Plan& p, const Layout& l, char* kept) {
     DecayArgs d = {};
-    char* ws = static_cast<char*>(a.workspace);
     d.g = a.g; d.gb = a.g_batch; d.gt = a.g_token; d.gh = a.g_head;
     d.B = (int)a.B; d.T = (int)a.T; d.H = (int)a.H;
     d.nseq = (int)(a.cu ? a.nseq : a.B);
     d.nslots = p.nslots; d.per_seq = p.per_seq; d.seg_tokens = p.seg_tokens;
-    d.tab = p.packed ? reinterpret_cast<const int4*>(ws + l.tab) : nullptr;
+    d.tab = p.packed ? reinterpret_cast<const int4*>(kept + l.tab) : nullptr;
     d.in_by_slot = p.multi;
     return d;
 }
 
 template <class K, typename OT, int NP, int NS, bool REV, bool STATES, bool DOT>
 hipError_t launch_mix(const DecayArgs& d, bool swapped, hipStream_t st) {
-    hipLaunchKernelGGL((kda_decay_mix_kernel<K, OT, NP, NS, REV, STATES, DOT>), dim3((unsigned)(d.nslots * d.H)), dim3(K::NTH), 0,
-                       st, d, swapped);
+    hipLaunchKernelGGL((kda_decay_mix_kernel<K, OT, NP, NS, REV, STATES, DOT>), dim3((unsigned)(d.nslots * d.H * K::SPLIT)),
+                       dim3(K::NTH), 0, st, d, swapped);
     return hipGetLastError();
 }
 
-hipError_t launch_plan(const Args& a, const Plan& p, const Layout& l, hipStream_t st) {
-    char* ws = static_cast<char*>(a.workspace);
-    hipLaunchKernelGGL(kda_decay_plan_kernel, dim3(1), dim3(PLAN_TH), 0, st, a.cu, (int)a.nseq, (int)a.T, p.seg_tokens,
-                       reinterpret_cast<int4*>(ws + l.tab), reinterpret_cast<int*>(ws + l.first), p.nslots);
-    return hipGetLastError();
-}
-
-// the states at the slots' limits: s at their starts, or (REV) their adjoints at the ends
+// the states at the slots' limits: their starts (u, seg: kept), or (REV) their adjoints at the ends
 template <class K, bool REV>
-hipError_t states(const Args& a, const Plan& p, const Layout& l, DecayArgs d, const float* s0, hipStream_t st) {
-    char* ws = static_cast<char*>(a.workspace);
-    d.s_out = reinterpret_cast<float*>(ws + (REV ? l.ds : l.s));
-    d.seg = reinterpret_cast<float*>(ws + (REV ? l.segd : l.seg));
+hipError_t states(DecayArgs d, float* u, float* seg, const int* first, const float* s0, hipStream_t st) {
+    d.s_out = u;
+    d.seg = seg;
     const hipError_t e = launch_mix<K, float, 1, 1, REV, true, false>(d, false, st);
     if (e != hipSuccess || d.nseq == 0) return e;
-    const int DD = K::D * K::D, parts = (DD / 4 + 255) / 256;
-    hipLaunchKernelGGL(kda_decay_scan_kernel<REV>, dim3((unsigned)(d.nseq * d.H * parts)), dim3(256), 0, st, d.s_out, d.seg, s0,
-                       p.packed ? reinterpret_cast<const int*>(ws + l.first) : nullptr, p.per_seq, d.H, DD, parts);
+    const int DD = K::D * K::D, parts = (DD / SCAN_PER + 255) / 256;
+    hipLaunchKernelGGL(kda_decay_scan_kernel<REV>, dim3((unsigned)(d.nseq * d.H * parts)), dim3(256), 0, st, u, seg, s0, first,
+                       d.per_seq, d.H, DD, parts);
     return hipGetLastError();
 }
 
@@ -1285,64 +1197,67 @@ hipError_t launch_group(const float* src, void* dst, const Args& a, const kda_de
     return hipGetLastError();
 }
 
+template <int D>
+constexpr int SPLIT_OF = D > 64 ? 2 : 1;
 // Planes of the pairs' products and of the state in bf16's products with it: two make
 // what is lost there small beside the output's own rounding.
 template <int D, bool F32>
 int forward(const Args& a, hipStream_t st) {
-    typedef Cfg<D, F32> K;
+    typedef Cfg<D, F32, SPLIT_OF<D>> K;
     constexpr int NP = F32 ? 3 : 2;
-    const Plan p = plan_of(a, false);
-    const Layout l = layout_of(a, p, false);
-    DecayArgs d = base_of(a, p, l);
-    if (p.packed) DEC_HIP(launch_plan(a, p, l, st));
+    const Plan p = plan_of(a, a.train != 0);
+    const Layout l = layout_of(a, p);
+    char* kept = static_cast<char*>(a.train ? a.kept : a.workspace);
+    DecayArgs d = base_of(a, p, l, kept);
+    int* first = p.packed ? reinterpret_cast<int*>(kept + l.first) : nullptr;
+    if (p.packed) {
+        hipLaunchKernelGGL(kda_decay_plan_kernel, dim3(1), dim3(PLAN_TH), 0, st, a.cu, (int)a.nseq, (int)a.T, p.seg_tokens,
+                           reinterpret_cast<int4*>(kept + l.tab), first, p.nslots);
+        DEC_HIP(hipGetLastError());
+    }
     if (p.multi) {
         DecayArgs m = d;
         m.y = rows_of(a, a.k);
         m.w = rows_of(a, a.v);
-        DEC_HIP((states<K, false>(a, p, l, m, a.s0, st)));
+        DEC_HIP((states<K, false>(m, reinterpret_cast<float*>(kept + l.s), reinterpret_cast<float*>(kept + l.seg), first, a.s0, st)));
     }
     d.x = rows_of(a, a.q);
     d.y = rows_of(a, a.k);
     d.w = rows_of(a, a.v);
     d.out = a.o;
-    d.s_in = p.multi ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + l.s) : a.s0;
+    d.s_in = p.multi ? reinterpret_cast<float*>(kept + l.s) : a.s0;
     d.s_out = a.s_final;
     DEC_HIP((launch_mix<K, typename K::ST, NP, NP, false, false, false>(d, false, st)));
     return KDA_OK;
 }
 
-template <class K, typename OT, int NP, bool DOT>
+template <class K, typename OT, int NP, bool DOT, int PARTS>
 hipError_t launch_mix2(const DecayArgs& d, hipStream_t st) {
-    hipLaunchKernelGGL((kda_decay_mix2_kernel<K, OT, NP, DOT ? 3 : NP, DOT>), dim3((unsigned)(d.nslots * d.H)), dim3(K::NTH), 0, st,
+    hipLaunchKernelGGL((kda_decay_mix2_kernel<K, OT, NP, DOT ? 3 : NP, DOT, PARTS>), dim3((unsigned)(d.nslots * d.H)), dim3(K::NTH), 0, st,
                        d);
     return hipGetLastError();
 }
 
 template <int D, bool F32, bool DOT>
 int backward(const Args& a, hipStream_t st) {
-    typedef Cfg<D, F32> K;
+    typedef Cfg<D, F32, SPLIT_OF<D>> K;
+    typedef Cfg<D, F32> K2;
     typedef typename K::ST ST;
     constexpr int NP = F32 ? 3 : 2;
     const Plan p = plan_of(a, true);
-    const Layout l = layout_of(a, p, true);
-    char* ws = static_cast<char*>(a.workspace);
-    const DecayArgs base = base_of(a, p, l);
+    const Layout l = layout_of(a, p);
+    char *ws = static_cast<char*>(a.workspace), *kept = static_cast<char*>(a.kept);
+    const DecayArgs base = base_of(a, p, l, kept);
     const Rows q = rows_of(a, a.q), k = rows_of(a, a.k), v = rows_of(a, a.v);
     kda_decay_rows dout = a.dout;
     dout.heads = a.H;
     const Rows o = rows_of(a, dout);
-    float* starts = p.multi ? reinterpret_cast<float*>(ws + l.s) : nullptr;
-    float* dends = p.multi ? reinterpret_cast<float*>(ws + l.ds) : nullptr;
-    float* dots = DOT ? reinterpret_cast<float*>(ws + l.dots) : nullptr;
-    float *g0 = l.g0 >= 0 ? reinterpret_cast<float*>(ws + l.g0) : nullptr,
-          *g1 = l.g1 >= 0 ? reinterpret_cast<float*>(ws + l.g1) : nullptr;
-    if (p.packed) DEC_HIP(launch_plan(a, p, l, st));
+    const auto part = [&](char* at, int64_t n) { return n < 0 ? nullptr : reinterpret_cast<float*>(at + n); };
+    float *starts = part(kept, l.s), *dends = part(ws, l.ds), *dots = part(ws, l.dots), *g0 = part(ws, l.g0), *g1 = part(ws, l.g1);
     if (p.multi) {
         DecayArgs m = base;
-        m.y = k; m.w = v;
-        DEC_HIP((states<K, false>(a, p, l, m, a.s0, st)));
         m.y = q; m.w = o;
-        DEC_HIP((states<K, true>(a, p, l, m, a.ds_final, st)));
+        DEC_HIP((states<K, true>(m, dends, part(ws, l.segd), reinterpret_cast<const int*>(part(kept, l.first)), a.ds_final, st)));
     }
     DecayArgs d = base;
     d.x = o; d.y = v; d.w = k; d.z = q;
@@ -1359,31 +1274,24 @@ int backward(const Args& a, hipStream_t st) {
     d.x = k; d.y = q; d.z = v; d.w = o;
     d.s_in = p.multi ? dends : a.ds_final;
     d.s_out = a.ds0;
+    double* sums = reinterpret_cast<double*>(part(ws, l.sums));
     d.dots = dots;
-    d.dots2 = DOT ? dots + a.H * a.B * a.T : nullptr;
-    d.anchors = DOT ? reinterpret_cast<float*>(ws + l.anchors) : nullptr;
+    d.starts = starts;
+    d.s_final = a.ds_final ? a.s_final : nullptr;
+    d.dg = sums ? nullptr : a.dg;
+    d.sums = sums;
     if (shared(a, a.k) || shared(a, a.v)) {
         d.out = g0; d.out2 = g1;
-        DEC_HIP((launch_mix2<K, float, NP, DOT>(d, st)));
+        DEC_HIP((launch_mix2<K2, float, NP, DOT, K::SPLIT>(d, st)));
         DEC_HIP(launch_group<ST>(g0, a.dk, a, a.k, st));
         DEC_HIP(launch_group<ST>(g1, a.dv, a, a.v, st));
     } else {
         d.out = a.dk; d.out2 = a.dv;
-        DEC_HIP((launch_mix2<K, ST, NP, DOT>(d, st)));
+        DEC_HIP((launch_mix2<K2, ST, NP, DOT, K::SPLIT>(d, st)));
     }
-    if constexpr (DOT) {
-        d = base;
-        d.dots = dots;
-        d.dots2 = dots + a.H * a.B * a.T;
-        d.anchors = reinterpret_cast<float*>(ws + l.anchors);
-        double* sums = a.dg_heads ? reinterpret_cast<double*>(ws + l.sums) : nullptr;
-        hipLaunchKernelGGL(kda_decay_dg_kernel, dim3((unsigned)(d.nslots * d.H)), dim3(DG_TH), 0, st, d, starts, dends, a.s_final,
-                           a.ds_final, sums ? nullptr : a.dg, sums, D * D, K::C);
+    if (sums) {
+        hipLaunchKernelGGL(kda_decay_dg_sum_kernel, dim3((unsigned)d.H), dim3(64), 0, st, sums, a.dg, d.nslots, d.H);
         DEC_HIP(hipGetLastError());
-        if (sums) {
-            hipLaunchKernelGGL(kda_decay_dg_sum_kernel, dim3((unsigned)d.H), dim3(64), 0, st, sums, a.dg, d.nslots, d.H);
-            DEC_HIP(hipGetLastError());
-        }
     }
     return KDA_OK;
 }
@@ -1406,9 +1314,15 @@ hipError_t launch_step(const StepArgs& a, bool f32, hipStream_t st) {
     return hipGetLastError();
 }
 
+int check_ws(const void* p, const char* name, int64_t have, int64_t need) {
+    if (!need) return KDA_OK;
+    DEC_TRY(check_ptr(p, name, 16));
+    if (have < need) return api_fail(KDA_E_WORKSPACE, "%s has %lld bytes, needs %lld", name, (long long)have, (long long)need);
+    return KDA_OK;
+}
 int check_common(const Args& a, bool bwd) {
     DEC_TRY(check_sizes(a));
-    const Plan p = plan_of(a, bwd);
+    const Plan p = plan_of(a, bwd || a.train);
     if (p.nslots < 0) return api_fail(KDA_E_UNSUPPORTED, "B=%lld T=%lld H=%lld: too many workgroups", (long long)a.B, (long long)a.T, (long long)a.H);
     if (a.B * a.T > 0) {
         DEC_TRY(check_operand(a, a.q, "q"));
@@ -1418,12 +1332,10 @@ int check_common(const Args& a, bool bwd) {
     }
     if (a.cu) DEC_TRY(check_ptr(a.cu, "cu", 4));
     if (a.s0) DEC_TRY(check_ptr(a.s0, "s0", 16));
-    const int64_t need = layout_of(a, p, bwd).bytes;
-    if (need) {
-        DEC_TRY(check_ptr(a.workspace, "workspace", 16));
-        if (a.ws_bytes < need)
-            return api_fail(KDA_E_WORKSPACE, "workspace has %lld bytes, needs %lld", (long long)a.ws_bytes, (long long)need);
-    }
+    const Layout l = layout_of(a, p);
+    if (bwd || a.train) DEC_TRY(check_ws(a.kept, "kept", a.kept_bytes, l.kept));
+    else DEC_TRY(check_ws(a.workspace, "workspace", a.ws_bytes, l.kept));
+    if (bwd) DEC_TRY(check_ws(a.workspace, "workspace", a.ws_bytes, l.bytes));
     return KDA_OK;
 }
 
@@ -1437,9 +1349,10 @@ extern "C" {
 
 size_t kda_decay_workspace_size(int pass, const kda_decay_args* args) {
     if (!args || check_sizes(*args) != KDA_OK) return 0;
-    const bool bwd = pass == KDA_PASS_BWD;
-    const Plan p = plan_of(*args, bwd);
-    return p.nslots < 0 ? 0 : (size_t)layout_of(*args, p, bwd).bytes;
+    const Plan p = plan_of(*args, pass != KDA_PASS_FWD);
+    if (p.nslots < 0) return 0;
+    const Layout l = layout_of(*args, p);
+    return (size_t)(pass == KDA_PASS_BWD ? l.bytes : l.kept);
 }
 
 int kda_decay_fwd(const kda_decay_args* args, void* stream) {

@@ -103,24 +103,18 @@ def _check_device(what: str, dev: torch.device) -> None:
 
 
 def _args(q, k, v, g, s0, cu, do=None, o=None, s_final=None, ds_final=None, dq=None, dk=None, dv=None, dg=None, ds0=None):
-    """``kda_decay_args`` as 64-bit fields (without the workspace, the last two)."""
+    """``kda_decay_args`` as 64-bit fields; the last five are the workspace, what is kept and train."""
     B, T, _, D = q.shape
     p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     gs = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
     return array("q", [*_field(q, 3), *_field(k, 3), *_field(v, 3), *_field(do, 3), p(g), *gs, p(s0), p(cu),
                        0 if cu is None else cu.numel() - 1, p(o), p(s_final), p(ds_final), p(dq), p(dk), p(dv), p(dg),
-                       int(g.dim() == 1), p(ds0), B, T, g.shape[-1], D, _DTYPE_CODE[q.dtype], 0, 0])
+                       int(g.dim() == 1), p(ds0), B, T, g.shape[-1], D, _DTYPE_CODE[q.dtype], 0, 0, 0, 0, 0])
 
 
-def _call(what: str, pass_: int, args: array, dev: torch.device) -> None:
-    lib, at = _lib.load(), args.buffer_info()[0]
+def _space(lib, pass_: int, at: int, dev: torch.device) -> Optional[torch.Tensor]:
     n = lib.kda_decay_workspace_size(pass_, at)
-    if n:
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        args[-2], args[-1] = ws.data_ptr(), n
-    rc = (lib.kda_decay_bwd if pass_ == _lib.KDA_PASS_BWD else lib.kda_decay_fwd)(at, _raw_stream(dev.index))
-    if rc:
-        _lib.check(rc, what)
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -130,24 +124,34 @@ def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _forward(q, k, v, g, s0, cu):
+def _forward(q, k, v, g, s0, cu, train: bool):
     B, T, _, D = q.shape
     H, dev = g.shape[-1], q.device
     with _on(dev):
         q, k, v, s0 = _pieces(q), _pieces(k), _pieces(v), _aligned(s0)
         o = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
         s_final = torch.empty((B if cu is None else cu.numel() - 1, H, D, D), dtype=torch.float32, device=dev)
-        _call("kda_decay_fwd", _lib.KDA_PASS_FWD, _args(q, k, v, g, s0, cu, o=o, s_final=s_final), dev)
-    return q, k, v, s0, o, s_final
+        args, lib = _args(q, k, v, g, s0, cu, o=o, s_final=s_final), _lib.load()
+        at = args.buffer_info()[0]
+        ws = _space(lib, _lib.KDA_PASS_TRAIN if train else _lib.KDA_PASS_FWD, at, dev)
+        if ws is not None:
+            i = -3 if train else -5
+            args[i], args[i + 1] = ws.data_ptr(), ws.numel()
+        args[-1] = int(train)
+        rc = lib.kda_decay_fwd(at, _raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, "kda_decay_fwd")
+    return q, k, v, s0, ws, o, s_final
 
 
 class ChunkDecayFunction(torch.autograd.Function):
-    """``chunk_decay`` as one node; keeps its inputs and the final state."""
+    """``chunk_decay`` as one node; keeps its inputs, the final state and the states that
+    the kernels share a sequence out by."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, s0, cu):
-        q, k, v, s0, o, s_final = _forward(q, k, v, g, s0, cu)
-        ctx.save_for_backward(q, k, v, g, s0, cu, s_final)
+        *kept, o, s_final = _forward(q, k, v, g, s0, cu, True)
+        ctx.save_for_backward(*kept, g, cu, s_final)
         # an unused output's cotangent comes as None
         ctx.set_materialize_grads(False)
         return o, s_final
@@ -155,18 +159,27 @@ class ChunkDecayFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do, ds):
-        q, k, v, g, s0, cu, s_final = ctx.saved_tensors
+        q, k, v, s0, kept, g, cu, s_final = ctx.saved_tensors
         need_g, need_s = ctx.needs_input_grad[3:5]
         B, T, _, D = q.shape
         H, dev = g.shape[-1], q.device
         with _on(dev):
             do = torch.zeros((B, T, H, D), dtype=q.dtype, device=dev) if do is None else _pieces(do)
+            ds = _aligned(ds)
             new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
             dq, dk, dv = new(q), new(k), new(v)
             dg = new(g) if need_g else None
             ds0 = new(s0) if need_s else None
-            _call("kda_decay_bwd", _lib.KDA_PASS_BWD,
-                  _args(q, k, v, g, s0, cu, do, None, s_final, _aligned(ds), dq, dk, dv, dg, ds0), dev)
+            args, lib = _args(q, k, v, g, s0, cu, do, None, s_final, ds, dq, dk, dv, dg, ds0), _lib.load()
+            at = args.buffer_info()[0]
+            ws = _space(lib, _lib.KDA_PASS_BWD, at, dev)
+            if ws is not None:
+                args[-5], args[-4] = ws.data_ptr(), ws.numel()
+            if kept is not None:
+                args[-3], args[-2] = kept.data_ptr(), kept.numel()
+            rc = lib.kda_decay_bwd(at, _raw_stream(dev.index))
+            if rc:
+                _lib.check(rc, "kda_decay_bwd")
         return dq, dk, dv, dg, ds0, None
 
 
@@ -208,7 +221,7 @@ def chunk_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     if (_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, initial_state))
             or forward_ad._current_level >= 0):
         return ChunkDecayFunction.apply(q, k, v, g, initial_state, cu_seqlens)
-    return _forward(q, k, v, g, initial_state, cu_seqlens)[4:]
+    return _forward(q, k, v, g, initial_state, cu_seqlens, False)[5:]
 
 
 def decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
@@ -247,7 +260,7 @@ def decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         gs = (0, g.stride(0)) if g.dim() == 1 else g.stride()
         rows = lambda t: (t.data_ptr(), t.stride(0) if B > 1 else 0, 0, t.stride(1) if t.shape[1] > 1 else 0, t.shape[1])  # noqa: E731
         args = array("q", [*rows(q), *rows(k), *rows(v), 0, 0, 0, 0, 0, g.data_ptr(), gs[0], 0, gs[1], state.data_ptr(), 0, 0,
-                           o.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, B, 1, H, D, _DTYPE_CODE[q.dtype], 0, 0])
+                           o.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, B, 1, H, D, _DTYPE_CODE[q.dtype], 0, 0, 0, 0, 0])
         rc = _lib.load().kda_decay_step(args.buffer_info()[0], None if slots is None else slots.data_ptr(), N,
                                         _raw_stream(dev.index))
         if rc:

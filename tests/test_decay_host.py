@@ -107,16 +107,16 @@ class Decay(ctypes.Structure):
                 + [("s0", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("nseq", ctypes.c_int64)]
                 + [(n, ctypes.c_void_p) for n in ("o", "s_final", "ds_final", "dq", "dk", "dv", "dg")]
                 + [("dg_heads", ctypes.c_int64), ("ds0", ctypes.c_void_p)]
-                + [(n, ctypes.c_int64) for n in ("B", "T", "H", "D", "dtype")] + [("workspace", ctypes.c_void_p), ("ws_bytes", ctypes.c_int64)])
+                + [(n, ctypes.c_int64) for n in ("B", "T", "H", "D", "dtype")] + [("workspace", ctypes.c_void_p), ("ws_bytes", ctypes.c_int64), ("kept", ctypes.c_void_p), ("kept_bytes", ctypes.c_int64), ("train", ctypes.c_int64)])
 
 
 def _decay(**kw):
     a = Decay(B=2, T=300, H=4, D=64, dtype=1)
     for i, n in enumerate(("q", "k", "v", "dout")):
         setattr(a, n, Rows(4096 * (i + 1), 300 * 256, 256, 64, 4))
-    for i, n in enumerate(("g", "o", "s_final", "dq", "dk", "dv", "dg", "workspace")):
+    for i, n in enumerate(("g", "o", "s_final", "dq", "dk", "dv", "dg", "workspace", "kept")):
         setattr(a, n, 65536 * (i + 1))
-    a.ws_bytes = 1 << 40
+    a.ws_bytes = a.kept_bytes = 1 << 40
     for n, v in kw.items():
         setattr(a, n, v)
     return a
@@ -136,6 +136,7 @@ def _decay(**kw):
     (dict(B=2, cu=4096, nseq=2), _lib.KDA_E_INVALID, "one row"),
     (dict(workspace=None), _lib.KDA_E_INVALID, "workspace"),
     (dict(ws_bytes=16), _lib.KDA_E_WORKSPACE, "needs"),
+    (dict(q=Rows(4096, 0, (1 << 24) + 8, 64, 4)), _lib.KDA_E_INVALID, "token stride"),
     (dict(B=1 << 30, T=4096), _lib.KDA_E_UNSUPPORTED, "too many workgroups"),
 ])
 def test_decay_abi_refuses(kw, code, match):
@@ -150,7 +151,9 @@ def test_decay_abi_refuses_its_own():
     lib = _lib.load()
     for f, kw, match in ((lib.kda_decay_fwd, dict(o=None), "o is NULL"), (lib.kda_decay_fwd, dict(s_final=4), "s_final"),
                          (lib.kda_decay_bwd, dict(dq=None), "dq"), (lib.kda_decay_bwd, dict(dg=2), "dg"),
-                         (lib.kda_decay_bwd, dict(ds_final=65536, s_final=None), "s_final (of the forward")):
+                         (lib.kda_decay_bwd, dict(ds_final=65536, s_final=None), "s_final (of the forward"),
+                         (lib.kda_decay_bwd, dict(B=1, T=100000, kept=None), "kept is NULL"),
+                         (lib.kda_decay_fwd, dict(B=1, T=100000, train=1, kept=None), "kept is NULL")):
         a = _decay(**kw)
         assert f(ctypes.addressof(a), None) == _lib.KDA_E_INVALID
         assert match in _lib.last_error()
@@ -171,8 +174,12 @@ def test_decay_workspace():
     assert size(_lib.KDA_PASS_FWD, B=1, T=64) == 0
     n = size(_lib.KDA_PASS_FWD, B=1, T=65536, H=12)
     assert n and n % (12 * 4) == 0 and n > 12 * 4 * 64 * 64 * 2
-    # a backward pass holds the adjoints beside the states
-    assert size(_lib.KDA_PASS_BWD, B=1, T=65536, H=12, dg=None) >= 2 * n
+    # a training pass keeps the states at its slots' starts, a backward pass makes as many adjoints
+    own = Rows(4096, 0, 768, 64, 12)
+    many = dict(B=1, T=65536, H=12, dg=None, q=own, k=own, v=own)
+    assert size(_lib.KDA_PASS_TRAIN, **many) == size(_lib.KDA_PASS_BWD, **many) > 12 * 4 * 64 * 64 * 2
+    assert size(_lib.KDA_PASS_BWD, **{**many, "dg": 64}) - size(_lib.KDA_PASS_BWD, **many) >= 4 * 65536 * 12
+    assert size(_lib.KDA_PASS_BWD, **{**many, "k": Rows(4096, 0, 64, 64, 1)}) - size(_lib.KDA_PASS_BWD, **many) == 2 * 4 * 65536 * 12 * 64
     assert size(_lib.KDA_PASS_FWD, dtype=5) == 0 and "dtype" in _lib.last_error()
     # packed: a slot for every sequence, and for what lies around them
     many = size(_lib.KDA_PASS_FWD, B=1, T=64, cu=4096, nseq=1000)
