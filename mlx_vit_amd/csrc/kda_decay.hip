@@ -1050,9 +1050,11 @@ struct Plan {
 };
 // How many chunks of 64 tokens a slot has.  Sequences that fill the card by themselves are
 // one slot each; else what is shared out costs a pass for the slots' states and a scan
-// over them, and the workgroups come in rounds of as many as fit beside each other
-// (measured at D = 64: a chunk takes 0.4 of a full card's time in a workgroup alone, a
-// slot 1 / 40 of it in the scan): the least of all counts.
+// over them, and the workgroups come in rounds of as many as fit beside each other: the
+// least of all counts.  (Measured at D = 64, bf16, in chunks' times of a full card, 7.5 us: a
+// chunk takes 0.33 in a workgroup alone; half as much again in the first pass; the two more
+// launches 0.9 and a slot of the scan 0.02.  8 x 1568 x 12 x 64 takes 42 us in slots of 3
+// chunks, 45 of 2 or 4, 68 whole; 196 x 6 x 64 14.5 of one chunk, 12.1 whole.)
 Plan plan_of(const Args& a, bool train) {
     Plan p;
     p.packed = a.cu != nullptr;
@@ -1063,8 +1065,8 @@ Plan plan_of(const Args& a, bool train) {
     int64_t seg = 0;
     for (int64_t c = 1; c <= most; c = c < 64 || c == chunks ? c + 1 : chunks) {
         const int64_t per = (chunks + c - 1) / c, n = (p.packed ? per + seqs / 2 : rows * per) * a.H, rest = n % fit;
-        const double turns = (double)(n / fit) + (rest ? 0.4 + 0.6 * (double)rest / fit : 0.0);
-        const double cost = (double)c * turns * (p.packed || per > 1 ? 1.5 : 1.0) + (per > 1 ? 0.5 + 0.025 * per : 0.0);
+        const double turns = (double)(n / fit) + (rest ? 0.33 + 0.67 * (double)rest / fit : 0.0);
+        const double cost = (double)c * turns * (p.packed || per > 1 ? 1.5 : 1.0) + (p.packed || per > 1 ? 0.9 + 0.02 * per : 0.0);
         if (!seg || cost < best) {
             best = cost;
             seg = c;

@@ -20,7 +20,8 @@ from before it, and those of shared heads are summed before they are rounded.
 """
 from __future__ import annotations
 
-from array import array
+from functools import lru_cache
+from struct import Struct
 from typing import Optional, Tuple
 
 import torch
@@ -38,23 +39,64 @@ MAX_TOKENS, MAX_TOKEN_STRIDE = (1 << 31) - 8192, 1 << 24
 
 def _pieces(t: torch.Tensor) -> torch.Tensor:
     """t (..., heads, D) as the kernels read it, rows in whole 16-byte pieces; a copy where it is not."""
-    n = 16 // t.element_size()
-    if (t.data_ptr() & 15 or t.stride(-1) != 1 or t.stride(-3) > MAX_TOKEN_STRIDE
-            or any(s % n for s, m in zip(t.stride()[:-1], t.shape[:-1]) if m > 1)):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    if not t.data_ptr() & 15:
+        if t.is_contiguous():
+            return t
+        n = 16 // t.element_size()
+        if (t.stride(-1) == 1 and t.stride(0 if t.dim() == 3 else 1) <= MAX_TOKEN_STRIDE
+                and not any(s % n for s, m in zip(t.stride()[:-1], t.shape[:-1]) if m > 1)):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _field(t: Optional[torch.Tensor], lead: int):
-    """Address, ``lead`` strides and the heads of an operand (zeros: not there).  Of a dimension of
-    one the stride does not count."""
-    if t is None:
-        return [0] * (lead + 2)
-    return [t.data_ptr(), *(s if n > 1 else 0 for s, n in zip(t.stride()[:lead], t.shape)), t.shape[lead - 1]]
+def _rows(t: torch.Tensor):
+    """kda_decay_rows of t (B, T, heads, D).  (Of a dimension of one the stride does not count.)"""
+    B, T, h, D = t.shape
+    if t.is_contiguous():
+        return t.data_ptr(), T * h * D, h * D, D, h
+    b, m, s, _ = t.stride()
+    return t.data_ptr(), b if B > 1 else 0, m if T > 1 else 0, s if h > 1 else 0, h
+
+
+_NONE = (0,) * 5
+_pack = Struct("46q").pack      # kda_decay_args
+
+
+@lru_cache(maxsize=1024)
+def _space(pass_: int, B: int, T: int, H: int, D: int, code: int, hq: int, hk: int, hv: int, nseq: int, dg: int) -> int:
+    """``kda_decay_workspace_size`` by sizes; nseq -1: not packed; dg 0: not wanted, 1 [B][T][H], 2 [H]."""
+    none = (0, 0, 0, 0)
+    return _lib.load().kda_decay_workspace_size(pass_, _pack(
+        *none, hq, *none, hk, *none, hv, *none, H, *none, 0, nseq >= 0, max(nseq, 0), 0, 0, 0, 0, 0, 0, dg > 0, dg == 2, 0, B, T, H, D,
+        code, *none, 0))
+
+
+def _new(n: int, dev: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _p(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _matches(n: int, q, k, v, g) -> bool:
+    """What ``_check_operands`` asks for, in one expression."""
+    try:
+        *head, hq, D = q.shape
+        *kh, hk, kd = k.shape
+        *vh, hv, vd = v.shape
+        H, dt, dev = g.shape[-1], q.dtype, q.get_device()
+        return (len(head) == n and head == kh == vh and D == kd == vd and D in HEAD_DIMS and dt in _DTYPE_CODE
+                and k.dtype is dt and v.dtype is dt and g.dtype in _DTYPE_CODE and not (H % hq or H % hk or H % hv) and H > 0
+                and (g.dim() == 1 or g.shape == (*head, H)) and dev == k.get_device() == v.get_device() == g.get_device())
+    except (AttributeError, TypeError, ValueError, IndexError, ZeroDivisionError):
+        return False
 
 
 def _check_operands(what: str, q, k, v, g, lead: Tuple[str, ...]) -> int:
     """Validate q, k, v (*lead, heads, D) and g (*lead, H) or (H,); returns H."""
+    if _matches(len(lead), q, k, v, g):
+        return g.shape[-1]
     for name, t in (("q", q), ("k", k), ("v", v), ("g", g)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: {name} must be a torch.Tensor")
@@ -102,21 +144,6 @@ def _check_device(what: str, dev: torch.device) -> None:
         raise RuntimeError(f"{what} cannot be traced: its launches are no part of a traced graph")
 
 
-def _args(q, k, v, g, s0, cu, do=None, o=None, s_final=None, ds_final=None, dq=None, dk=None, dv=None, dg=None, ds0=None):
-    """``kda_decay_args`` as 64-bit fields; the last five are the workspace, what is kept and train."""
-    B, T, _, D = q.shape
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    gs = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
-    return array("q", [*_field(q, 3), *_field(k, 3), *_field(v, 3), *_field(do, 3), p(g), *gs, p(s0), p(cu),
-                       0 if cu is None else cu.numel() - 1, p(o), p(s_final), p(ds_final), p(dq), p(dk), p(dv), p(dg),
-                       int(g.dim() == 1), p(ds0), B, T, g.shape[-1], D, _DTYPE_CODE[q.dtype], 0, 0, 0, 0, 0])
-
-
-def _space(lib, pass_: int, at: int, dev: torch.device) -> Optional[torch.Tensor]:
-    n = lib.kda_decay_workspace_size(pass_, at)
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-
-
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """States: contiguous, rows on 16 bytes."""
     if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
@@ -124,23 +151,30 @@ def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _forward(q, k, v, g, s0, cu, train: bool):
+def _call(fn, q, k, v, do, g, *rest):
+    one = g.dim() == 1
     B, T, _, D = q.shape
-    H, dev = g.shape[-1], q.device
+    s0, cu, o, s_final, ds, dq, dk, dv, dg, ds0, ws, kept, train = rest
+    rc = fn(_pack(*_rows(q), *_rows(k), *_rows(v), *(_NONE if do is None else _rows(do)), g.data_ptr(),
+                  *((0, 0, g.stride(0)) if one else g.stride()), _p(s0), _p(cu), 0 if cu is None else cu.numel() - 1, _p(o),
+                  _p(s_final), _p(ds), _p(dq), _p(dk), _p(dv), _p(dg), one, _p(ds0), B, T, g.shape[-1], D, _DTYPE_CODE[q.dtype],
+                  _p(ws), 0 if ws is None else ws.numel(), _p(kept), 0 if kept is None else kept.numel(), train),
+            _raw_stream(q.get_device()))
+    if rc:
+        _lib.check(rc, fn.__name__)
+
+
+def _forward(q, k, v, g, s0, cu, train: bool):
+    B, T, hq, D = q.shape
+    H, dev, nseq = g.shape[-1], q.device, -1 if cu is None else cu.numel() - 1
     with _on(dev):
         q, k, v, s0 = _pieces(q), _pieces(k), _pieces(v), _aligned(s0)
         o = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
-        s_final = torch.empty((B if cu is None else cu.numel() - 1, H, D, D), dtype=torch.float32, device=dev)
-        args, lib = _args(q, k, v, g, s0, cu, o=o, s_final=s_final), _lib.load()
-        at = args.buffer_info()[0]
-        ws = _space(lib, _lib.KDA_PASS_TRAIN if train else _lib.KDA_PASS_FWD, at, dev)
-        if ws is not None:
-            i = -3 if train else -5
-            args[i], args[i + 1] = ws.data_ptr(), ws.numel()
-        args[-1] = int(train)
-        rc = lib.kda_decay_fwd(at, _raw_stream(dev.index))
-        if rc:
-            _lib.check(rc, "kda_decay_fwd")
+        s_final = torch.empty((B if cu is None else nseq, H, D, D), dtype=torch.float32, device=dev)
+        ws = _new(_space(_lib.KDA_PASS_TRAIN if train else _lib.KDA_PASS_FWD, B, T, H, D, _DTYPE_CODE[q.dtype], hq, k.shape[2],
+                         v.shape[2], nseq, 0), dev)
+        _call(_lib.load().kda_decay_fwd, q, k, v, None, g, s0, cu, o, s_final, None, None, None, None, None, None,
+              None if train else ws, ws if train else None, train)
     return q, k, v, s0, ws, o, s_final
 
 
@@ -161,25 +195,16 @@ class ChunkDecayFunction(torch.autograd.Function):
     def backward(ctx, do, ds):
         q, k, v, s0, kept, g, cu, s_final = ctx.saved_tensors
         need_g, need_s = ctx.needs_input_grad[3:5]
-        B, T, _, D = q.shape
+        B, T, hq, D = q.shape
         H, dev = g.shape[-1], q.device
         with _on(dev):
             do = torch.zeros((B, T, H, D), dtype=q.dtype, device=dev) if do is None else _pieces(do)
-            ds = _aligned(ds)
-            new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
-            dq, dk, dv = new(q), new(k), new(v)
-            dg = new(g) if need_g else None
-            ds0 = new(s0) if need_s else None
-            args, lib = _args(q, k, v, g, s0, cu, do, None, s_final, ds, dq, dk, dv, dg, ds0), _lib.load()
-            at = args.buffer_info()[0]
-            ws = _space(lib, _lib.KDA_PASS_BWD, at, dev)
-            if ws is not None:
-                args[-5], args[-4] = ws.data_ptr(), ws.numel()
-            if kept is not None:
-                args[-3], args[-2] = kept.data_ptr(), kept.numel()
-            rc = lib.kda_decay_bwd(at, _raw_stream(dev.index))
-            if rc:
-                _lib.check(rc, "kda_decay_bwd")
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+            dg = torch.empty(g.shape, dtype=torch.float32, device=dev) if need_g else None
+            ds0 = torch.empty(s0.shape, dtype=torch.float32, device=dev) if need_s else None
+            ws = _new(_space(_lib.KDA_PASS_BWD, B, T, H, D, _DTYPE_CODE[q.dtype], hq, k.shape[2], v.shape[2],
+                             -1 if cu is None else cu.numel() - 1, (2 if g.dim() == 1 else 1) if need_g else 0), dev)
+            _call(_lib.load().kda_decay_bwd, q, k, v, do, g, s0, cu, None, s_final, _aligned(ds), dq, dk, dv, dg, ds0, ws, kept, 0)
         return dq, dk, dv, dg, ds0, None
 
 
@@ -257,12 +282,14 @@ def decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     with _on(dev):
         q, k, v = _pieces(q), _pieces(k), _pieces(v)
         o = torch.empty((B, H, D), dtype=q.dtype, device=dev)
-        gs = (0, g.stride(0)) if g.dim() == 1 else g.stride()
-        rows = lambda t: (t.data_ptr(), t.stride(0) if B > 1 else 0, 0, t.stride(1) if t.shape[1] > 1 else 0, t.shape[1])  # noqa: E731
-        args = array("q", [*rows(q), *rows(k), *rows(v), 0, 0, 0, 0, 0, g.data_ptr(), gs[0], 0, gs[1], state.data_ptr(), 0, 0,
-                           o.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, B, 1, H, D, _DTYPE_CODE[q.dtype], 0, 0, 0, 0, 0])
-        rc = _lib.load().kda_decay_step(args.buffer_info()[0], None if slots is None else slots.data_ptr(), N,
-                                        _raw_stream(dev.index))
+        gb, gh = (0, g.stride(0)) if g.dim() == 1 else g.stride()
+        fields = []
+        for t in (q, k, v):
+            b, h, _ = t.stride()
+            fields += (t.data_ptr(), b if B > 1 else 0, 0, h if t.shape[1] > 1 else 0, t.shape[1])
+        rc = _lib.load().kda_decay_step(
+            _pack(*fields, *_NONE, g.data_ptr(), gb, 0, gh, state.data_ptr(), 0, 0, o.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, B, 1, H, D,
+                  _DTYPE_CODE[q.dtype], 0, 0, 0, 0, 0), None if slots is None else slots.data_ptr(), N, _raw_stream(dev.index))
         if rc:
             _lib.check(rc, "kda_decay_step")
     if not state.is_inference():

@@ -26,6 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import forward_ad
 
+from .decay_layer import DecayAttentionLayer
 from .layer import GatedDeltaLayer
 from .layer_fused import _nn_module, _plain_module
 from .linear import mlp
@@ -216,17 +217,19 @@ class NoPEVideoEncoder(nn.Module):
 
 
 class HybridBlock(nn.Module):
-    """One processor block, GDN or NoPE attention (nope_gdn_mlx.py:4009-4091)."""
+    """One processor block, GDN or NoPE attention (nope_gdn_mlx.py:4009-4091); or ``decay``, linear
+    attention with rotary positions over frames of ``grid`` tokens, in the GDN's place."""
 
     fused_mlp = False   # set_fused_mlp
 
     def __init__(self, dim: int, num_heads: int, block_type: str = "gdn", head_dim: Optional[int] = None,
                  chunk_size: int = 64, mlp_ratio: float = 4.0, dropout: float = 0.0,
                  channel_wise_decay: bool = True, allow_neg_eigval: bool = False,
-                 spatial_tokens: Optional[int] = None, drop_path: float = 0.0, gdn_temporal_only: bool = False):
+                 spatial_tokens: Optional[int] = None, drop_path: float = 0.0, gdn_temporal_only: bool = False,
+                 grid: Tuple[int, int] = (14, 14)):
         super().__init__()
-        if block_type not in ("gdn", "nope"):
-            raise ValueError(f"block_type must be 'gdn' or 'nope'; got {block_type!r}")
+        if block_type not in ("gdn", "nope", "decay"):
+            raise ValueError(f"block_type must be 'gdn', 'nope' or 'decay'; got {block_type!r}")
         self.block_type = block_type
         self.spatial_tokens = spatial_tokens
         self.gdn_temporal_only = gdn_temporal_only
@@ -235,6 +238,10 @@ class HybridBlock(nn.Module):
         if block_type == "gdn":
             self.layer = GatedDeltaLayer(dim, num_heads, head_dim or dim // num_heads, chunk_size,
                                          channel_wise_decay=channel_wise_decay, allow_neg_eigval=allow_neg_eigval)
+        elif block_type == "decay":
+            # (a scan over time alone sees frames of one token)
+            time_only = gdn_temporal_only and spatial_tokens is not None
+            self.layer = DecayAttentionLayer(dim, num_heads, head_dim or dim // num_heads, grid=(1, 1) if time_only else grid)
         else:
             self.layer = NoPEMultiheadAttention(dim, num_heads, dropout)
         self.norm2 = nn.LayerNorm(dim, eps=1e-6)
@@ -244,7 +251,7 @@ class HybridBlock(nn.Module):
                 state: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         B, N, D = x.shape
         normed = self.norm1(x)
-        if self.block_type == "gdn":
+        if self.block_type != "nope":
             if self.gdn_temporal_only and self.spatial_tokens is not None:
                 # time-only scan: one recurrence per spatial location over T'
                 S = self.spatial_tokens
@@ -267,7 +274,7 @@ class HybridBlock(nn.Module):
 
 
 class NoPEGDNVideoBackbone(nn.Module):
-    """NoPE encoder + GDN:NoPE hybrid processor (nope_gdn_mlx.py:4097-4209)."""
+    """NoPE encoder + GDN:NoPE hybrid processor (nope_gdn_mlx.py:4097-4209); ``mixer``: see NoPEGDNClassifier."""
 
     def __init__(self, img_size: int = 224, num_frames: int = 32, tubelet_size=(2, 16, 16), in_channels: int = 3,
                  encoder_dim: int = 384, encoder_depth: int = 12, encoder_heads: int = 6,
@@ -275,8 +282,10 @@ class NoPEGDNVideoBackbone(nn.Module):
                  gdn_ratio: int = 3, chunk_size: int = 64, channel_wise_decay: bool = True,
                  allow_neg_eigval: bool = False, factorized_attention: bool = True,
                  gdn_temporal_only: bool = False, mlp_ratio: float = 4.0, dropout: float = 0.0,
-                 drop_path_rate: float = 0.0):
+                 drop_path_rate: float = 0.0, mixer: str = "gdn"):
         super().__init__()
+        if mixer not in ("gdn", "decay"):
+            raise ValueError(f"mixer must be 'gdn' or 'decay'; got {mixer!r}")
         total = encoder_depth + processor_depth
         dpr = [drop_path_rate * i / (total - 1) for i in range(total)] if drop_path_rate > 0 and total > 1 \
             else [0.0] * total
@@ -290,11 +299,11 @@ class NoPEGDNVideoBackbone(nn.Module):
         period = gdn_ratio + 1
         blocks = []
         for i in range(processor_depth):
-            bt = "nope" if (i + 1) % period == 0 else "gdn"
+            bt = "nope" if (i + 1) % period == 0 else mixer
             blocks.append(HybridBlock(processor_dim, processor_heads, bt, processor_dim // processor_heads,
                                       chunk_size, mlp_ratio, dropout, channel_wise_decay, allow_neg_eigval,
                                       spatial if (bt == "nope" or gdn_temporal_only) else None,
-                                      dpr[encoder_depth + i], gdn_temporal_only))
+                                      dpr[encoder_depth + i], gdn_temporal_only, (grid["H"], grid["W"])))
         self.processor_blocks = nn.ModuleList(blocks)
         self.processor_norm = nn.LayerNorm(processor_dim, eps=1e-6)
         self.encoder_dim, self.processor_dim = encoder_dim, processor_dim
@@ -358,7 +367,8 @@ class VideoClassificationHead(nn.Module):
 
 
 class NoPEGDNClassifier(nn.Module):
-    """End-to-end NoPE + GDN video classifier (nope_gdn_mlx.py:4285-4342)."""
+    """End-to-end NoPE + GDN video classifier (nope_gdn_mlx.py:4285-4342).  ``mixer``: "gdn",
+    or "decay" for DecayAttentionLayer in the GDN's place."""
 
     def __init__(self, img_size: int = 224, num_frames: int = 32, tubelet_size=(2, 16, 16), in_channels: int = 3,
                  encoder_dim: int = 384, encoder_depth: int = 12, encoder_heads: int = 6,
@@ -367,12 +377,12 @@ class NoPEGDNClassifier(nn.Module):
                  allow_neg_eigval: bool = False, factorized_attention: bool = True,
                  gdn_temporal_only: bool = False, head_type: str = "temporal", num_classes: int = 174,
                  mlp_ratio: float = 4.0, dropout: float = 0.0, head_dropout: float = 0.0,
-                 drop_path_rate: float = 0.0):
+                 drop_path_rate: float = 0.0, mixer: str = "gdn"):
         super().__init__()
         self.backbone = NoPEGDNVideoBackbone(
             img_size, num_frames, tubelet_size, in_channels, encoder_dim, encoder_depth, encoder_heads,
             processor_dim, processor_depth, processor_heads, gdn_ratio, chunk_size, channel_wise_decay,
-            allow_neg_eigval, factorized_attention, gdn_temporal_only, mlp_ratio, dropout, drop_path_rate)
+            allow_neg_eigval, factorized_attention, gdn_temporal_only, mlp_ratio, dropout, drop_path_rate, mixer)
         self.spatial_tokens = (img_size // tubelet_size[1]) * (img_size // tubelet_size[2])
         if head_type == "mean":
             self.head = VideoClassificationHead(processor_dim, num_classes, dropout=head_dropout)
