@@ -16,6 +16,7 @@ from __future__ import annotations
 import math
 from array import array
 from functools import lru_cache
+from struct import Struct
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -31,38 +32,49 @@ _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
 @lru_cache(maxsize=64)
-def _turns(sections: Tuple[int, ...], base: float) -> array:
-    """Turns a unit of position of every pair: base^(-2 i / section) / 2 pi."""
-    return array("d", [base ** (-2 * i / s) / (2 * math.pi) for s in sections for i in range(s // 2)])
+def _axes(D: int, sections, base: float) -> Tuple[int, Tuple[int, ...], array]:
+    """Validated: how many axes, their sections filled up with zeros, and turns a unit of position of
+    every pair, base^(-2 i / section) / 2 pi."""
+    given, sections = sections, (D,) if sections is None else tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= MAX_AXES or any(s < 0 or s % 2 for s in sections) or sum(sections) > D:
+        raise ValueError(f"rotary: sections={given}: expected 1 to {MAX_AXES} even numbers that make up at most {D}")
+    if not 0.0 < base < math.inf:
+        raise ValueError(f"rotary: base={base}: expected a positive number")
+    turns = array("d", [base ** (-2 * i / s) / (2 * math.pi) for s in sections for i in range(s // 2)])
+    return len(sections), sections + (0,) * (MAX_AXES - len(sections)), turns
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _rows(t: Optional[torch.Tensor]):
-    return (0, 0, 0, 0, 1) if t is None else (t.data_ptr(), *t.stride()[:3], t.shape[2])
+def _rows(t: torch.Tensor):
+    return (t.data_ptr(), *t.stride()[:3], t.shape[2])
+
+
+_NONE = (0, 0, 0, 0, 1)
+_pack = Struct("32q").pack      # kda_rotary_args
 
 
 def _turn(q, k, how, sign: int):
     """Queries and keys (either may be None) turned by ``how``, sign -1: back."""
-    positions, strides, grid, start, sections, base, interleaved = how
-    first = q if k is None or q is not None else k
+    positions, where, (axes, sections, turns), interleaved = how
+    first, second = (k, None) if q is None else (q, k)
     B, T, _, D = first.shape
     dev = first.device
     with _on(dev):
-        q, k = (None if t is None else _unit(t) for t in (q, k))
-        out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k)]
-        ins, outs = (q, k) if q is not None else (k, None), out if q is not None else (out[1], None)
-        turns = _turns(sections, base)
-        args = array("q", [*_rows(ins[0]), *_rows(ins[1]), *(0 if t is None else t.data_ptr() for t in outs),
-                           *((0, 0, 0, 0, 0) if positions is None else (positions.data_ptr(), _POSITIONS[positions.dtype], *strides)),
-                           *grid, start, len(sections), *sections, *([0] * (MAX_AXES - len(sections))),
-                           turns.buffer_info()[0], int(interleaved), sign, B, T, D, _DTYPE_CODE[first.dtype]])
-        rc = _lib.load().kda_rotary(args.buffer_info()[0], _raw_stream(dev.index))
+        first = _unit(first)
+        y, z = torch.empty(first.shape, dtype=first.dtype, device=dev), None
+        if second is not None:
+            second = _unit(second)
+            z = torch.empty(second.shape, dtype=second.dtype, device=dev)
+        rc = _lib.load().kda_rotary(
+            _pack(*_rows(first), *(_NONE if second is None else _rows(second)), y.data_ptr(), 0 if z is None else z.data_ptr(),
+                  0 if positions is None else positions.data_ptr(), *where, axes, *sections, turns.buffer_info()[0], interleaved, sign,
+                  B, T, D, _DTYPE_CODE[first.dtype]), _raw_stream(dev.index))
         if rc:
             _lib.check(rc, "kda_rotary")
-    return out
+    return (None, y) if q is None else (y, z)
 
 
 class RotaryFunction(torch.autograd.Function):
@@ -74,7 +86,7 @@ class RotaryFunction(torch.autograd.Function):
         ctx.how = how[1:]
         ctx.set_materialize_grads(False)
         y = _turn(q, k, how, 1)
-        return y[0] if k is None else tuple(y)
+        return y[0] if k is None else y
 
     @staticmethod
     @once_differentiable
@@ -118,26 +130,25 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optiona
             raise ValueError(f"{what}: k has dtype {k.dtype}; expected {q.dtype}")
         if k.device != dev:
             raise ValueError(f"{what}: k is on {k.device}, q on {dev}")
-    sections = (D,) if sections is None else tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= MAX_AXES or any(s < 0 or s % 2 for s in sections) or sum(sections) > D:
-        raise ValueError(f"{what}: sections={sections}: expected 1 to {MAX_AXES} even numbers that make up at most {D}")
-    base = float(base)
-    if not 0.0 < base < math.inf:
-        raise ValueError(f"{what}: base={base}: expected a positive number")
-    strides = None
+    how = _axes(D, sections if sections is None or type(sections) is tuple else tuple(sections), float(base))
+    n = how[0]
     if (positions is None) == (grid is None):
         raise ValueError(f"{what}: expected either positions or grid")
     if grid is not None:
-        grid = tuple(int(n) for n in grid)
-        if len(grid) != 2 or min(grid) < 1 or max(grid) >= 1 << 31 or len(sections) > 3 or not 0 <= start < 1 << 62:
-            raise ValueError(f"{what}: grid={grid}, start={start} with {len(sections)} sections: expected (height, width), "
+        try:
+            h, w = grid
+        except (TypeError, ValueError):
+            raise ValueError(f"{what}: grid={grid}: expected (height, width)") from None
+        if not (1 <= h < 1 << 31 and 1 <= w < 1 << 31 and n <= 3 and 0 <= start < 1 << 62):
+            raise ValueError(f"{what}: grid={grid}, start={start} with {n} sections: expected (height, width), "
                              "start >= 0 and at most 3 axes")
+        where = (0, 0, 0, 0, int(h), int(w), int(start))
     else:
         if not isinstance(positions, torch.Tensor):
             raise TypeError("rotary: positions must be a torch.Tensor")
         if start:
             raise ValueError(f"{what}: start={start} goes with grid, not with positions")
-        shape, n = tuple(positions.shape), len(sections)
+        shape = tuple(positions.shape)
         if shape not in ((n, T), (n, B, T)) and not (n == 1 and shape == (T,)):
             raise ValueError(f"{what}: positions shape {shape}: expected ({n}, {T}) or ({n}, {B}, {T})")
         if positions.dtype not in _POSITIONS:
@@ -147,13 +158,13 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optiona
         if positions.requires_grad and _grad_enabled():
             raise ValueError(f"{what} has no gradient for positions")
         s = positions.stride()
-        strides = (0, 0, s[0]) if len(s) == 1 else (s[0], 0, s[1]) if len(s) == 2 else s
+        where = (_POSITIONS[positions.dtype], *((0, 0, s[0]) if len(s) == 1 else (s[0], 0, s[1]) if len(s) == 2 else s), 1, 1, 0)
     if dev.type != "cuda":
         raise ValueError(f"{what} runs on a ROCm device; got tensors on {dev}")
     if _is_tracing():
         raise RuntimeError(f"{what} cannot be traced: its launches are no part of a traced graph")
-    how = positions, strides, grid or (1, 1), int(start), sections, base, bool(interleaved)
+    how = positions, where, how, bool(interleaved)
     if _grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or forward_ad._current_level >= 0:
         return RotaryFunction.apply(q, k, how)
     y = _turn(q, k, how, 1)
-    return y[0] if k is None else tuple(y)
+    return y[0] if k is None else y
