@@ -901,9 +901,9 @@ __global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, 
 constexpr int SCAN_PER = 2;
 template <bool REV>
 __global__ __launch_bounds__(256) void kda_decay_scan_kernel(float* u, const float* seg, const float* s0, const int* first,
-                                                             int per_seq, int H, int DD, int parts) {
+                                                             int per_seq, int H, int DD, int parts, int seq0) {
     typedef float vec __attribute__((ext_vector_type(SCAN_PER)));
-    const int part = blockIdx.x % parts, sh = blockIdx.x / parts, seq = sh / H, h = sh - seq * H;
+    const int part = blockIdx.x % parts, sh = blockIdx.x / parts, in = sh / H, h = sh - in * H, seq = seq0 + in;
     const int e = SCAN_PER * (part * 256 + (int)threadIdx.x);
     if (e >= DD) return;
     const int lo = first ? first[seq] : seq * per_seq, count = (first ? first[seq + 1] : lo + per_seq) - lo;
@@ -1042,6 +1042,8 @@ __global__ __launch_bounds__(256) void kda_decay_step_kernel(const StepArgs a) {
 // ----------------------------------------------------------------------------
 typedef kda_decay_args Args;
 
+constexpr int64_t MAX_THREADS = (int64_t)1 << 32;   // of a launch: fewer
+
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Plan {
@@ -1075,7 +1077,7 @@ Plan plan_of(const Args& a, bool train) {
     p.seg_tokens = (int)(64 * seg);
     p.per_seq = p.packed ? 0 : (int)((chunks + seg - 1) / seg);
     const int64_t n = p.packed ? a.nseq + 2 + a.T / p.seg_tokens : a.B * p.per_seq;
-    p.nslots = n * a.H > 0x3fffffff ? -1 : (int)n;
+    p.nslots = n * a.H >= MAX_THREADS / (4 * a.D) ? -1 : (int)n;   // (4 D threads a slot and head)
     p.multi = p.packed || p.per_seq > 1;
     return p;
 }
@@ -1185,8 +1187,18 @@ hipError_t states(DecayArgs d, float* u, float* seg, const int* first, const flo
     const hipError_t e = launch_mix<K, float, 1, 1, REV, true, false>(d, false, st);
     if (e != hipSuccess || d.nseq == 0) return e;
     const int DD = K::D * K::D, parts = (DD / SCAN_PER + 255) / 256;
-    hipLaunchKernelGGL(kda_decay_scan_kernel<REV>, dim3((unsigned)(d.nseq * d.H * parts)), dim3(256), 0, st, u, seg, s0, first,
-                       d.per_seq, d.H, DD, parts);
+    const int most = std::max(1, (int)((MAX_THREADS - 1) / 256 / ((int64_t)parts * d.H)));   // sequences a launch
+    for (int seq0 = 0; seq0 < d.nseq; seq0 += std::min(most, d.nseq - seq0)) {
+        hipLaunchKernelGGL(kda_decay_scan_kernel<REV>, dim3((unsigned)(std::min(most, d.nseq - seq0) * d.H * parts)), dim3(256), 0, st, u,
+                           seg, s0, first, d.per_seq, d.H, DD, parts, seq0);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_dg_sum(const double* sums, float* dg, int nslots, int H, hipStream_t st) {
+    hipLaunchKernelGGL(kda_decay_dg_sum_kernel, dim3((unsigned)H), dim3(64), 0, st, sums, dg, nslots, H);
     return hipGetLastError();
 }
 
@@ -1291,10 +1303,7 @@ int backward(const Args& a, hipStream_t st) {
         d.out = a.dk; d.out2 = a.dv;
         DEC_HIP((launch_mix2<K2, ST, NP, DOT, K::SPLIT>(d, st)));
     }
-    if (sums) {
-        hipLaunchKernelGGL(kda_decay_dg_sum_kernel, dim3((unsigned)d.H), dim3(64), 0, st, sums, a.dg, d.nslots, d.H);
-        DEC_HIP(hipGetLastError());
-    }
+    if (sums) DEC_HIP(launch_dg_sum(sums, a.dg, d.nslots, d.H, st));
     return KDA_OK;
 }
 
@@ -1389,8 +1398,11 @@ int kda_decay_bwd(const kda_decay_args* args, void* stream) {
         DEC_TRY(check_ptr(a.dg, "dg", 4));
         if (a.ds_final) DEC_TRY(check_ptr(a.s_final, "s_final (of the forward pass, for dg)", 16));
     }
-    if (a.B == 0) return KDA_OK;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.B == 0) {
+        if (a.dg && a.dg_heads) DEC_HIP(launch_dg_sum(nullptr, a.dg, 0, (int)a.H, st));   // zeros
+        return KDA_OK;
+    }
     switch (a.D) {
         case 32: return backward_of<32>(a, st);
         case 64: return backward_of<64>(a, st);
@@ -1407,7 +1419,7 @@ int kda_decay_step(const kda_decay_args* args, const int32_t* slots, int64_t sta
     if (a.B == 0) return KDA_OK;
     if (states < 0 || states > 0x7fffffff || (!slots && states != a.B))
         return api_fail(KDA_E_INVALID, "%lld states for %lld rows", (long long)states, (long long)a.B);
-    if (a.B * a.H > (1 << 28)) return api_fail(KDA_E_UNSUPPORTED, "B=%lld H=%lld: too many workgroups", (long long)a.B, (long long)a.H);
+    if (a.B * a.H >= MAX_THREADS / 512) return api_fail(KDA_E_UNSUPPORTED, "B=%lld H=%lld: too many workgroups", (long long)a.B, (long long)a.H);
     DEC_TRY(check_operand(a, a.q, "q"));
     DEC_TRY(check_operand(a, a.k, "k"));
     DEC_TRY(check_operand(a, a.v, "v"));

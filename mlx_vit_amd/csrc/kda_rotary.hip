@@ -28,7 +28,7 @@ struct RotaryArgs {
     int type;
     uint32_t grid_h, grid_w;
     int64_t start;
-    uint32_t T, groups, parts, units;  // groups of V pairs a row; parts of `per` heads each; B T parts
+    uint32_t T, groups, parts, unit0, units;  // groups of V pairs a row; parts of `per` heads each; units [unit0, units) of B T parts
     int D, per;
     float sign;
     int axes, ends[AXES];              // pairs before each axis' end
@@ -86,7 +86,7 @@ struct Row {
 
 template <typename ST, int V, bool HALVES>
 __global__ __launch_bounds__(256) void kda_rotary_kernel(const RotaryArgs a) {
-    const uint32_t rows = 256u / a.groups, group = threadIdx.x % a.groups, unit = blockIdx.x * rows + threadIdx.x / a.groups;
+    const uint32_t rows = 256u / a.groups, group = threadIdx.x % a.groups, unit = a.unit0 + blockIdx.x * rows + threadIdx.x / a.groups;
     if (threadIdx.x >= rows * a.groups || unit >= a.units) return;
     const uint32_t tok = a.parts == 1 ? unit : unit / a.parts, part = unit - tok * a.parts;
     const uint32_t b = tok / a.T, t = tok - b * a.T;
@@ -154,10 +154,18 @@ __global__ __launch_bounds__(256) void kda_rotary_kernel(const RotaryArgs a) {
 }
 
 template <typename ST, int V, bool HALVES>
-hipError_t launch(const RotaryArgs& a, hipStream_t st) {
+hipError_t launch(RotaryArgs a, hipStream_t st) {
     const uint32_t rows = 256u / a.groups;
-    hipLaunchKernelGGL((kda_rotary_kernel<ST, V, HALVES>), dim3((a.units + rows - 1) / rows), dim3(256), 0, st, a);
-    return hipGetLastError();
+    // (a launch has fewer than 2^32 threads)
+    for (uint32_t blocks = (a.units + rows - 1) / rows; blocks;) {
+        const uint32_t n = std::min(blocks, 1u << 23);
+        hipLaunchKernelGGL((kda_rotary_kernel<ST, V, HALVES>), dim3(n), dim3(256), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        a.unit0 += n * rows;
+        blocks -= n;
+    }
+    return hipSuccess;
 }
 
 }  // namespace

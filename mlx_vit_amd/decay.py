@@ -15,7 +15,8 @@ the recurrence of ``chunk_gdn`` without the delta rule (nope_gdn_mlx.py:641-650)
 
 Differentiable in every tensor but ``cu_seqlens``; a second derivative and tracing are
 refused.  Sums and states are fp32; each output is rounded once, to its input's dtype.
-There is no CPU path.  Gradients of g are fp32 sums of what reaches the tokens from one on
+There is no CPU path.  A backward pass is captured into a graph as torch's own nodes are: while no
+eager graph of the same leaves is alive.  Gradients of g are fp32 sums of what reaches the tokens from one on
 from before it, and those of shared heads are summed before they are rounded.
 """
 from __future__ import annotations
@@ -217,7 +218,7 @@ def chunk_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     q, k, v (B, T, heads, D), bf16 or fp32, D 32, 64, 96 or 128, any strides (rows that
     are not whole 16-byte pieces are copied first).  g (B, T, H) or (H,), fp32 or bf16;
     g = -inf starts the state anew, and so does everything below -200.  A
-    value that is not finite reaches all outputs of its sequence from its 64 tokens on.
+    value that is not finite reaches all outputs of its sequence from its 32 tokens on.
 
     ``cu_seqlens`` (N + 1,) int32 on the same device: token cu[i] to cu[i + 1] - 1 of the one
     row (B = 1) are sequence i; states are then (N, H, D, D).  The limits are read on the

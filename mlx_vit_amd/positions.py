@@ -9,7 +9,8 @@ reference's model has no positions; this is for what is built beside it.
 
 Angles are formed in fp64 (at a position p they are within 2^-52 p), rows in fp32 and
 rounded once.  Differentiable in q and k, by turning back; a second derivative and tracing are
-refused.  There is no CPU path.
+refused.  A backward pass is captured into a graph as torch's own nodes are: while no eager graph
+of the same leaves is alive.  There is no CPU path.
 """
 from __future__ import annotations
 

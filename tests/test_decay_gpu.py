@@ -117,6 +117,19 @@ def test_packed_long():
     check(inputs(1, 2600, 1, 32, BF, state=True, n=4), [3, 3, 2200, 2201, 2590])
 
 
+def test_more_sequences_than_a_scan_takes_at_once():
+    """2^19 states of 128 x 128: the scan over their slots in two launches.  A sequence of one
+    token, of values that a launch too few would not give."""
+    n, D = (1 << 19) + 3, 128
+    k = torch.ones(1, n, 1, D, dtype=BF, device=DEV)
+    v = (torch.arange(n, device=DEV) % 251).to(BF)[None, :, None, None].expand(1, n, 1, D)
+    with torch.no_grad():
+        o, s = chunk_decay(k, k, v, torch.zeros(1, n, 1, device=DEV), None, torch.arange(n + 1, dtype=torch.int32, device=DEV))
+    assert torch.equal(s[:, 0, 5, 7], v[0, :, 0, 0].float())
+    # (128 times an integer below 251, in bf16)
+    assert torch.equal(o[0, :, 0, 3], (128 * v[0, :, 0, 0].float()).to(BF))
+
+
 def test_many_sequences():
     lens = [(7 * i) % 13 for i in range(1500)]
     cu = [0]
@@ -312,10 +325,12 @@ def test_nothing_to_do():
         assert [g.shape for g in got] == [t.shape for t in leaves] and torch.equal(got[4], x["ds"])
         o, s = chunk_decay(*leaves[:4])
         assert not s.any()
-    x = inputs(2, 0, 3, 32, BF, one=True)
-    g = x["g"].requires_grad_(True)
-    dg, = torch.autograd.grad(chunk_decay(x["q"], x["k"], x["v"], g)[0], g, x["do"])
-    assert dg.shape == (3,) and not dg.any()
+    for B, T in ((2, 0), (0, 3)):
+        x = inputs(B, T, 300, 32, BF, one=True)
+        g = x["g"].requires_grad_(True)
+        torch.full((300,), math.nan, device=DEV)   # what freed memory holds
+        dg, = torch.autograd.grad(chunk_decay(x["q"], x["k"], x["v"], g)[0], g, x["do"])
+        assert dg.shape == (300,) and not dg.any()
 
 
 def test_the_same_twice_and_on_another_stream():

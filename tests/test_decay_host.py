@@ -138,6 +138,7 @@ def _decay(**kw):
     (dict(ws_bytes=16), _lib.KDA_E_WORKSPACE, "needs"),
     (dict(q=Rows(4096, 0, (1 << 24) + 8, 64, 4)), _lib.KDA_E_INVALID, "token stride"),
     (dict(B=1 << 30, T=4096), _lib.KDA_E_UNSUPPORTED, "too many workgroups"),
+    (dict(B=1 << 22, T=1), _lib.KDA_E_UNSUPPORTED, "too many workgroups"),   # 2^32 threads
 ])
 def test_decay_abi_refuses(kw, code, match):
     lib = _lib.load()
@@ -162,6 +163,8 @@ def test_decay_abi_refuses_its_own():
     assert lib.kda_decay_step(ctypes.addressof(a), None, 2, None) == _lib.KDA_E_INVALID and "T=2" in _lib.last_error()
     a = _decay(T=1)
     assert lib.kda_decay_step(ctypes.addressof(a), None, 3, None) == _lib.KDA_E_INVALID and "3 states" in _lib.last_error()
+    a = _decay(T=1, B=1 << 21)
+    assert lib.kda_decay_step(ctypes.addressof(a), None, 1 << 21, None) == _lib.KDA_E_UNSUPPORTED
     a = _decay(T=1, s0=None)
     assert lib.kda_decay_step(ctypes.addressof(a), None, 2, None) == _lib.KDA_E_INVALID and "s0" in _lib.last_error()
 

@@ -197,6 +197,17 @@ def test_past_two_to_the_31():
         near(y[:, lo:lo + 40], turned(q[:, lo:lo + 40], (torch.arange(40) + lo)[None, None], (128,)), lo)
 
 
+def test_more_tokens_than_a_launch_takes():
+    """2^24 tokens of 256 single channels: two launches.  One row for all of them, off its pieces' alignment."""
+    T, D = (1 << 24) + 3, 256
+    row = torch.randn(D + 1, device=DEV).to(BF)[1:]
+    y = rotary(row.expand(1, T, 1, D), grid=(64, 64), sections=(128, 64, 64))
+    for lo in (0, (1 << 24) - 2):
+        n = torch.arange(5) + lo
+        at = torch.stack([n // 4096, n // 64 % 64, n % 64])[:, None]
+        near(y[:, lo:lo + 5], turned(row.expand(1, 5, 1, D), at, (128, 64, 64)), lo)
+
+
 def test_together():
     """Positions, then the attention over a clip, then a token at a time: one rotation and one recurrence over it all."""
     from mlx_vit_amd import decay_step
