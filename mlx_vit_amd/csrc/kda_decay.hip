@@ -126,7 +126,7 @@ struct Cfg {
     static constexpr int RP = 2 * C, PPL = C * RP;                                             // of the pairs'
     static constexpr int TT = C / 16, NT = TT * (TT + 1) / 2, DT = D / 16, KD = D / 32, KC = C / 32;
     static constexpr int OCC = F32_ ? 1 : D > 64 ? 3 : 4, OCC2 = F32_ ? 1 : D > 64 ? 2 : 3;
-    static constexpr bool F32 = F32_;
+    static constexpr bool F32 = F32_, WITH_DS = D <= 64;
     typedef typename std::conditional<F32_, float, uint16_t>::type ST;
     static constexpr int ES = (int)sizeof(ST), EPV = 16 / ES;
     static_assert(C % 32 == 0 && D % (16 * SPLIT) == 0 && D % 32 == 0, "whole tiles");
@@ -354,9 +354,13 @@ struct State {
     // S <- all S + Y^T (down W): the chunk's sum from zero, so that what the matrix unit
     // loses (it rounds sums downwards) does not add up over the chunks.  w: w_frag of W.
     __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::NPL], const Decays<K::C>& d) {
+        add(Y, w, d.down, d.all, 1.f);
+    }
+    // S <- own S + all Y^T (weights W)
+    __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::NPL], const float* weights, float own, float all) {
         static_assert(K::KC == 1, "one step of the contracted index");
         const int r = lane_id() >> 4;
-        const float4 d0 = *reinterpret_cast<const float4*>(d.down + 8 * r), d1 = *reinterpret_cast<const float4*>(d.down + 8 * r + 4);
+        const float4 d0 = *reinterpret_cast<const float4*>(weights + 8 * r), d1 = *reinterpret_cast<const float4*>(weights + 8 * r + 4);
         const float dn[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
         bf16x8 ws[3];
         float v[8];
@@ -367,14 +371,13 @@ struct State {
             v[e] *= dn[e];
         }
         planes8<3>(v, ws);
-        const float all = d.all;
 #pragma unroll
         for (int j = 0; j < K::DT; ++j) {
             bf16x8 y[K::NPL];
             y_frag<K>(Y, 0, j, y);
             const f32x4 u = mmp(y, ws, zero4());
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = fmaf(all, s[j][i], u[i]);
+            for (int i = 0; i < 4; ++i) s[j][i] = fmaf(own, s[j][i], all * u[i]);
         }
     }
     // up_t (St^T X_t) for every row, the state as NS planes: lane (m, r) has row 16 i + m,
@@ -450,27 +453,43 @@ __device__ __forceinline__ void clear_rows(void* out, const DecayArgs& a, const 
 }
 
 template <class K, int NP>
-constexpr size_t mix_lds(bool states, bool dot) {
-    return (states ? 1 : 2) * (size_t)K::TILE + K::TILEW + (states ? 0 : (size_t)NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
+constexpr size_t mix_lds(bool states, bool grad, bool dot) {
+    return (states ? 1 : grad ? 3 : 2) * (size_t)K::TILE + K::TILEW + (states ? 0 : (size_t)NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
            (dot ? (size_t)K::NW * K::C * 4 : 0);
 }
+// four channels of a row of a tile
+template <class K>
+__device__ __forceinline__ float4 tile4(const char* p) {
+    float4 v = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p));
+    if constexpr (K::NPL == 3) {
+        const float4 v1 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + K::PLANE)),
+                     v2 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + 2 * K::PLANE));
+        v = make_float4(v.x + (v1.x + v2.x), v.y + (v1.y + v2.y), v.z + (v1.z + v2.z), v.w + (v1.w + v2.w));
+    }
+    return v;
+}
 
-// mix: out = the operator over a slot's tokens (REV: backwards in time).  STATES: only
-// what the slot adds to the state, and its whole decay.  DOT: dots[t] = z_t . (the part
-// of out_t that comes from the state before the chunk), which NS = 3 keeps to fp32; by
+// mix: out = the operator over a slot's tokens.  STATES: only what the slot adds to the state,
+// and its whole decay.  GRAD: out is dq, z is q, and the slots' s_out and seg take what they
+// add to dS as well, sum of e^{G_t} do_t q_t^T (WITH_DS: 8 x 1568 x 12 x 64 34 us, by a pass of its
+// own 27 + 15; at D = 128 that leaves registers for two waves a SIMD instead of three, 213 us of
+// 20000 packed x 16, by itself 148 + 64); STATES and GRAD: dS alone.  DOT: dots[t] = q_t . (the
+// part of out_t that comes from the state before the chunk), which NS = 3 keeps to fp32; by
 // parts of the channels.
 //
 // A chunk: pairs, state and the state's part of out from LDS; a barrier; the pairs'
 // part from P and registers, and the next chunk into LDS; a barrier.  Its loads are in
 // flight for a whole chunk.  The last wave, which has the fewest pairs, forms the next
 // chunk's decays.
-template <class K, typename OT, int NP, int NS, bool REV, bool STATES, bool DOT>
-__global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const DecayArgs a, const bool swapped) {
+template <class K, typename OT, int NP, int NS, bool STATES, bool GRAD, bool DOT>
+__global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K::OCC) void kda_decay_mix_kernel(const DecayArgs a) {
     typedef typename K::ST ST;
-    __shared__ __attribute__((aligned(16))) char lds[mix_lds<K, NP>(STATES, DOT)];
+    constexpr bool DQ = GRAD && !STATES, DS = DQ && K::WITH_DS;
+    __shared__ __attribute__((aligned(16))) char lds[mix_lds<K, NP>(STATES, DS, DOT)];
     char* X = lds;
     char* Y = X + (STATES ? 0 : K::TILE);
-    char* W = Y + K::TILE;
+    char* Z = Y + K::TILE;
+    char* W = Z + (DS ? K::TILE : 0);
     char* P = W + K::TILEW;
     Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : NP * K::PPL));
     float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]
@@ -483,33 +502,35 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
         }
         return;
     }
-    if (STATES && (REV ? s.first : s.last)) return;   // nothing follows
+    if (STATES && (GRAD ? s.first : s.last)) return;   // no slot needs it
     const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
     const int wv = cols * K::NW + wave;   // of all
     constexpr int DD = K::D * K::D, LAST = K::NW - 1;
-    State<K> st;
-    st.load(STATES || !a.s_in ? nullptr : a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD, wv, swapped);
+    State<K> st, ds;
+    st.load(STATES || !a.s_in ? nullptr : a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD, wv, DQ);
+    const bool adjoint = DS && a.s_out && !s.first;
+    if constexpr (DS) ds.load(nullptr, wv, false);
+    float before = 1.f;   // e^{sum of g before the chunk}
 
     const float* g = a.g + b * a.gb + (int64_t)s.tok0 * a.gt + h * a.gh;
-    Stage<K, K::D, REV> sx, sy;
-    Stage<K, K::DW, REV> sw;
+    Stage<K, K::D, false> sx, sy, sz;
+    Stage<K, K::DW, false> sw;
     float gv = 0.f;
-    // the first row in memory of the chunk at i0
-    auto lowest = [&](int i0, int n) { return s.tok0 + (REV ? s.n - i0 - n : i0); };
     auto load = [&](int i0) {
-        const int n = min(K::C, s.n - i0), t = lowest(i0, n);
+        const int n = min(K::C, s.n - i0), t = s.tok0 + i0;
         if constexpr (!STATES) sx.load(at<ST>(a.x, b, t, h), (uint32_t)a.x.token * K::ES, n);
         sy.load(at<ST>(a.y, b, t, h), (uint32_t)a.y.token * K::ES, n);
+        if constexpr (DS) sz.load(at<ST>(a.z, b, t, h), (uint32_t)a.z.token * K::ES, n);
         sw.load(at<ST>(a.w, b, t, h) + cols * K::DW, (uint32_t)a.w.token * K::ES, n);
     };
-    // backwards, row i decays by what its successor in time does; the first by nothing
     auto load_g = [&](int i0) {
         const int i = i0 + l;
-        gv = l < K::C && i < s.n && !(REV && i == 0) ? g[(int64_t)(REV ? s.n - i : i) * a.gt] : 0.f;
+        gv = l < K::C && i < s.n ? g[(int64_t)i * a.gt] : 0.f;
     };
     auto store = [&](int n) {
         if constexpr (!STATES) sx.store(X, n);
         sy.store(Y, n);
+        if constexpr (DS) sz.store(Z, n);
         sw.store(W, n);
     };
     if constexpr (!STATES) clear_upper<K, NP>(P);
@@ -532,14 +553,12 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
         bf16x8 w[K::NPL];
         f32x4 o[K::TT];
         w_frag<K, K::RBW>(W, 0, wave, w);
-        float4 z[DOT ? K::TT : 1];
-        if constexpr (DOT) {
-            const ST* p = at<ST>(a.z, b, lowest(i0, n), h) + 16 * wv + 4 * (l >> 4);
+        const int ch = 16 * wv + 4 * (l >> 4);
+        float4 z[DOT && !DS ? K::TT : 1];
+        if constexpr (DOT && !DS) {
+            const ST* p = at<ST>(a.z, b, s.tok0 + i0, h) + ch;
 #pragma unroll
-            for (int i = 0; i < K::TT; ++i) {
-                const int m = min(16 * i + (l & 15), n - 1);
-                z[i] = ld4<ST>(p + (REV ? n - 1 - m : m) * (int)a.z.token);
-            }
+            for (int i = 0; i < K::TT; ++i) z[i] = ld4<ST>(p + min(16 * i + (l & 15), n - 1) * (int)a.z.token);
         }
         if constexpr (!STATES) {
 #pragma unroll
@@ -557,12 +576,27 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
             if constexpr (DOT) {
 #pragma unroll
                 for (int i = 0; i < K::TT; ++i) {
-                    const float x = quad_sum(dot4(z[i], o[i]));
-                    if (l < 16) part[wave * K::C + 16 * i + l] = x;
+                    const int t = 16 * i + (l & 15);
+                    if constexpr (DS) z[0] = tile4<K>(Z + Sw<K::RB>::at(t, ch >> 3) + 2 * (ch & 7));
+                    const float x = quad_sum(dot4(z[DS ? 0 : i], o[i]));
+                    if (l < 16) part[wave * K::C + t] = x;
                 }
             }
         }
-        st.add(Y, w, d);
+        if constexpr (STATES && GRAD) {
+            st.add(Y, w, d.up, 1.f, before);
+            before *= d.all;
+        } else {
+            st.add(Y, w, d);
+        }
+        if constexpr (DS) {
+            if (adjoint) {
+                bf16x8 x[K::NPL];
+                w_frag<K, K::RB>(X, 0, wv, x);
+                ds.add(Z, x, d.up, 1.f, before);
+                before *= d.all;
+            }
+        }
         if (wave == LAST && more) {
             whole += fill_decays<K::C>(dec + ((i0 / K::C + 1) & 1), gv);
             load_g(i0 + 2 * K::C);
@@ -573,31 +607,26 @@ __global__ __launch_bounds__(K::NTH, K::OCC) void kda_decay_mix_kernel(const Dec
             if (i0 + 2 * K::C < s.n) load(i0 + 2 * K::C);
         }
         if constexpr (!STATES) {
-            const int64_t row = (int64_t)b * a.T + lowest(i0, n);
+            const int64_t row = (int64_t)b * a.T + s.tok0 + i0;
             add_pairs<K, NP>(P, w, o);
-            put_rows<K, OT, REV>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, wv, n);
+            put_rows<K, OT, false>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, wv, n);
             if constexpr (DOT) {
                 const int t = threadIdx.x;
                 if (t < n) {
                     float x = 0.f;
 #pragma unroll
                     for (int k = 0; k < K::NW; ++k) x += part[k * K::C + t];
-                    a.dots[((int64_t)cols * a.H + h) * a.B * a.T + row + (REV ? n - 1 - t : t)] = x;
+                    a.dots[((int64_t)cols * a.H + h) * a.B * a.T + row + t] = x;
                 }
             }
         }
         if (more) lds_barrier();
     }
-    if constexpr (STATES) {
-        // backwards: to before the slot's first token
-        float last = 1.f;
-        if constexpr (REV) last = decay(g[0]);
-        if (wave == LAST && l == 0 && cols == 0) a.seg[(int64_t)j * a.H + h] = __builtin_amdgcn_exp2f((float)whole) * last;
-        st.store(a.s_out + ((int64_t)j * a.H + h) * DD, wv, last);
-    } else if (a.s_out && (REV ? s.first : s.last)) {
-        float last = 1.f;
-        if constexpr (REV) last = s.n > 0 ? decay(g[0]) : 1.f;
-        st.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, wv, last);
+    if (STATES || adjoint) {
+        if (wave == LAST && l == 0 && cols == 0) a.seg[(int64_t)j * a.H + h] = __builtin_amdgcn_exp2f((float)whole);
+        (STATES ? st : ds).store(a.s_out + ((int64_t)j * a.H + h) * DD, wv, 1.f);
+    } else if (!GRAD && a.s_out && s.last) {
+        st.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, wv, 1.f);
     }
 }
 
@@ -764,13 +793,7 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
             for (int i = 0; i < K::TT; ++i) {
                 const int t = 16 * i + (l & 15);
                 const char* p = Kt + Sw<K::RB>::at(t, ch >> 3) + 2 * (ch & 7);
-                float4 v = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p));
-                if constexpr (K::NPL == 3) {
-                    const float4 v1 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + K::PLANE)),
-                                 v2 = ld4<uint16_t>(reinterpret_cast<const uint16_t*>(p + 2 * K::PLANE));
-                    v = make_float4(v.x + (v1.x + v2.x), v.y + (v1.y + v2.y), v.z + (v1.z + v2.z), v.w + (v1.w + v2.w));
-                }
-                const float x = quad_sum(dot4(v, o2[i]));
+                const float x = quad_sum(dot4(tile4<K>(p), o2[i]));
                 if (l < 16) part[wave * K::C + t] = x;
             }
         }
@@ -1172,21 +1195,17 @@ DecayArgs base_of(const Args& a, const Plan& p, const Layout& l, char* kept) {
     return d;
 }
 
-template <class K, typename OT, int NP, int NS, bool REV, bool STATES, bool DOT>
-hipError_t launch_mix(const DecayArgs& d, bool swapped, hipStream_t st) {
-    hipLaunchKernelGGL((kda_decay_mix_kernel<K, OT, NP, NS, REV, STATES, DOT>), dim3((unsigned)(d.nslots * d.H * K::SPLIT)),
-                       dim3(K::NTH), 0, st, d, swapped);
+template <class K, typename OT, int NP, int NS, bool STATES, bool GRAD, bool DOT>
+hipError_t launch_mix(const DecayArgs& d, hipStream_t st) {
+    hipLaunchKernelGGL((kda_decay_mix_kernel<K, OT, NP, NS, STATES, GRAD, DOT>), dim3((unsigned)(d.nslots * d.H * K::SPLIT)),
+                       dim3(K::NTH), 0, st, d);
     return hipGetLastError();
 }
 
 // the states at the slots' limits: their starts (u, seg: kept), or (REV) their adjoints at the ends
-template <class K, bool REV>
-hipError_t states(DecayArgs d, float* u, float* seg, const int* first, const float* s0, hipStream_t st) {
-    d.s_out = u;
-    d.seg = seg;
-    const hipError_t e = launch_mix<K, float, 1, 1, REV, true, false>(d, false, st);
-    if (e != hipSuccess || d.nseq == 0) return e;
-    const int DD = K::D * K::D, parts = (DD / SCAN_PER + 255) / 256;
+template <bool REV>
+hipError_t launch_scan(const DecayArgs& d, int D, float* u, const float* seg, const int* first, const float* s0, hipStream_t st) {
+    const int DD = D * D, parts = (DD / SCAN_PER + 255) / 256;
     const int most = std::max(1, (int)((MAX_THREADS - 1) / 256 / ((int64_t)parts * d.H)));   // sequences a launch
     for (int seq0 = 0; seq0 < d.nseq; seq0 += std::min(most, d.nseq - seq0)) {
         hipLaunchKernelGGL(kda_decay_scan_kernel<REV>, dim3((unsigned)(std::min(most, d.nseq - seq0) * d.H * parts)), dim3(256), 0, st, u,
@@ -1233,7 +1252,10 @@ int forward(const Args& a, hipStream_t st) {
         DecayArgs m = d;
         m.y = rows_of(a, a.k);
         m.w = rows_of(a, a.v);
-        DEC_HIP((states<K, false>(m, reinterpret_cast<float*>(kept + l.s), reinterpret_cast<float*>(kept + l.seg), first, a.s0, st)));
+        m.s_out = reinterpret_cast<float*>(kept + l.s);
+        m.seg = reinterpret_cast<float*>(kept + l.seg);
+        DEC_HIP((launch_mix<K, float, 1, 1, true, false, false>(m, st)));
+        DEC_HIP(launch_scan<false>(m, D, m.s_out, m.seg, first, a.s0, st));
     }
     d.x = rows_of(a, a.q);
     d.y = rows_of(a, a.k);
@@ -1241,7 +1263,7 @@ int forward(const Args& a, hipStream_t st) {
     d.out = a.o;
     d.s_in = p.multi ? reinterpret_cast<float*>(kept + l.s) : a.s0;
     d.s_out = a.s_final;
-    DEC_HIP((launch_mix<K, typename K::ST, NP, NP, false, false, false>(d, false, st)));
+    DEC_HIP((launch_mix<K, typename K::ST, NP, NP, false, false, false>(d, st)));
     return KDA_OK;
 }
 
@@ -1268,22 +1290,29 @@ int backward(const Args& a, hipStream_t st) {
     const Rows o = rows_of(a, dout);
     const auto part = [&](char* at, int64_t n) { return n < 0 ? nullptr : reinterpret_cast<float*>(at + n); };
     float *starts = part(kept, l.s), *dends = part(ws, l.ds), *dots = part(ws, l.dots), *g0 = part(ws, l.g0), *g1 = part(ws, l.g1);
-    if (p.multi) {
-        DecayArgs m = base;
-        m.y = q; m.w = o;
-        DEC_HIP((states<K, true>(m, dends, part(ws, l.segd), reinterpret_cast<const int*>(part(kept, l.first)), a.ds_final, st)));
-    }
     DecayArgs d = base;
     d.x = o; d.y = v; d.w = k; d.z = q;
     d.s_in = p.multi ? starts : a.s0;
     d.dots = dots;
+    d.s_out = dends;
+    d.seg = part(ws, l.segd);
+    const auto scan = [&] {
+        return launch_scan<true>(base, D, dends, d.seg, reinterpret_cast<const int*>(part(kept, l.first)), a.ds_final, st);
+    };
+    if (p.multi && !K::WITH_DS) {   // dS of the slots by itself; else with dq
+        DecayArgs m = d;
+        m.y = q; m.w = o;
+        DEC_HIP((launch_mix<K, float, 1, 1, true, true, false>(m, st)));
+        DEC_HIP(scan());
+    }
     d.out = shared(a, a.q) ? g0 : a.dq;
     if (shared(a, a.q)) {
-        DEC_HIP((launch_mix<K, float, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
+        DEC_HIP((launch_mix<K, float, NP, DOT ? 3 : NP, false, true, DOT>(d, st)));
         DEC_HIP(launch_group<ST>(g0, a.dq, a, a.q, st));
     } else {
-        DEC_HIP((launch_mix<K, ST, NP, DOT ? 3 : NP, false, false, DOT>(d, true, st)));
+        DEC_HIP((launch_mix<K, ST, NP, DOT ? 3 : NP, false, true, DOT>(d, st)));
     }
+    if (p.multi && K::WITH_DS) DEC_HIP(scan());
     d = base;
     d.x = k; d.y = q; d.z = v; d.w = o;
     d.s_in = p.multi ? dends : a.ds_final;
