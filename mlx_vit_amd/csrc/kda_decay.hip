@@ -14,6 +14,10 @@
 //       behind, the state then being dS, the adjoint of S;
 //   dg_t = <S_T, dS_T> + sum_{s >= t} (q_s . dq_s - k_s . dk_s),
 // which is what reaches tokens from t on from before t.
+//
+// A long sequence is shared out into slots of whole chunks, a workgroup each: a pass for what
+// every slot adds to the state, a scan over the slots, and the pass for the output.  That
+// reads k and v twice, and gives a few long sequences the whole card.
 #include "kda_hip.h"
 #include "kda_internal.h"
 
@@ -481,6 +485,12 @@ __device__ __forceinline__ float4 tile4(const char* p) {
 // part from P and registers, and the next chunk into LDS; a barrier.  Its loads are in
 // flight for a whole chunk.  The last wave, which has the fewest pairs, forms the next
 // chunk's decays.
+//
+// Measured, bf16: 65536 x 12 x 64 STATES 51 us (201 MB at 3.9 TB/s, all that a sum which only
+// reads reaches), output 100 us (403 MB at 4.0 TB/s); 8 x 1568 x 12 x 64 15 and 20 us; 20000
+// packed x 16 x 128 62 and 117 us.  What bounds the output's pass is the chain through a chunk,
+// not one unit: of the 117 us the state's sum and its product, most of the matrix work, are worth
+// 15 each and 26 together, then stores 28, loads 18, and 34 are left without anything else.
 template <class K, typename OT, int NP, int NS, bool STATES, bool GRAD, bool DOT>
 __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K::OCC) void kda_decay_mix_kernel(const DecayArgs a) {
     typedef typename K::ST ST;
@@ -648,6 +658,11 @@ constexpr float ANCHOR_BELOW = 0x1p-32f;
 // behind it begins anew, as all that leaves it (the sum of b): with all of q . dq - k . dk in
 // one sum over the slot, dg of fast decays was 2 to 60 times as far off.  Sums in fp64.
 // PARTS: of dots, by channels.
+//
+// Measured, bf16: 8 x 1568 x 12 x 64 45 us; 20000 packed x 16 x 128 325 us, where four heads share
+// a key and 328 MB of fp32 parts are written, 64 us of it.  Two states of D x D in registers
+// leave two waves a SIMD (D <= 64: three), so a chunk's chain of products is seen in full; parts of
+// the channels as in mix would form both kinds of pairs twice (343 us).
 template <class K, typename OT, int NP, int NS, bool DOT, int PARTS>
 __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const DecayArgs a) {
     static_assert(K::SPLIT == 1, "dg takes all channels");
@@ -920,7 +935,8 @@ __global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, 
 
 // The state at each slot's start (REV: its adjoint at each slot's end), in place of
 // what the slots add: one thread takes two elements through a sequence's slots, 16
-// loads at a time.
+// loads at a time.  Bound by the latency of its rounds of loads: 12 heads of 64
+// over 79 slots (15.5 MB, read and written) 14 us, 32 loads at a time no less.
 constexpr int SCAN_PER = 2;
 template <bool REV>
 __global__ __launch_bounds__(256) void kda_decay_scan_kernel(float* u, const float* seg, const float* s0, const int* first,
@@ -968,7 +984,9 @@ __global__ __launch_bounds__(64) void kda_decay_dg_sum_kernel(const double* sums
     if (threadIdx.x == 0) dg[blockIdx.x] = (float)x;
 }
 
-// gradients of a tensor whose heads are shared: sums over the state's heads, rounded once
+// gradients of a tensor whose heads are shared: sums over the state's heads, rounded once.
+// Bound by its bytes: 20000 x 16 x 128 to 4 heads 31 us, 5.9 TB/s (what mix2 has just written
+// is partly still in a cache).
 template <typename OT>
 __global__ __launch_bounds__(256) void kda_decay_group_kernel(const float* src, OT* dst, int64_t n4, int share, int D) {
     const int per = D / 4;
@@ -1000,7 +1018,8 @@ struct StepArgs {
 
 // A wave takes R rows of a state (rows of v's channels) through one token: loads of
 // 16 bytes a lane, L lanes a row, all in flight together.  The states' bytes, read and
-// written once, are all that counts.
+// written once, are all that counts: 256 x 32 x 128 x 128 (1.07 GB both ways) 215 us, 5.0 TB/s;
+// 200 of 12 x 64 x 64 (79 MB) 16 us.
 template <int D>
 struct StepCfg {
     static constexpr int L = D == 32 ? 8 : D == 64 ? 16 : 32, RP = 64 / L, R = D == 32 ? 32 : 16, NP = R / RP, PARTS = D / R;
