@@ -21,6 +21,8 @@
 #include "kda_hip.h"
 #include "kda_internal.h"
 
+#include <cmath>
+
 namespace kda {
 
 namespace {
@@ -51,7 +53,8 @@ struct DecayArgs {
     float* dg;                  // [B][T][H], or null
     double* sums;               // or its sums by slot, [slot][H]
     float* seg;                 // states: e^{sum of g} of each slot and head
-    const int4* tab;            // packed: the slots
+    const int4* tab;            // packed: the slots, and the order in which they are taken
+    const int* order;
     int in_by_slot;
     int B, T, H, nseq, nslots, per_seq, seg_tokens;
 };
@@ -70,6 +73,30 @@ __device__ __forceinline__ Slot slot_of(const DecayArgs& a, int j) {
         s.last = i == a.per_seq - 1;
     }
     return s;
+}
+// The slot, head and part of the columns of a workgroup.  Workgroups go to the 8 XCDs in
+// turn: neighbours, which read the same tokens' keys, are put into one XCD's cache; of
+// packed sequences, whose slots differ in length, only the parts of one slot and head are,
+// so that each XCD begins with whole slots and ends with short ones (20000 in 10 sequences x
+// 16 x 128, forward and backward: 806 us in the slots' own order, 779 so, 727 with lengths
+// chosen for it).
+template <int SPLIT>
+__device__ __forceinline__ void work_of(const DecayArgs& a, int& j, int& h, int& cols) {
+    int at;
+    if (a.tab) {
+        constexpr int GROUP = 8 * SPLIT;
+        const int b = (int)blockIdx.x, r = b % GROUP, g = b - r;
+        const bool full = g + GROUP <= (int)gridDim.x;
+        at = g / SPLIT + (full ? r % 8 : r / SPLIT);
+        cols = full ? r / 8 : r % SPLIT;
+    } else {
+        const int b = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+        at = b / SPLIT;
+        cols = b % SPLIT;
+    }
+    j = at / a.H;
+    h = at - j * a.H;
+    if (a.tab) j = a.order[j];
 }
 
 // Products of two operands given as sums of bf16 planes, down to 2^-16 of the
@@ -488,9 +515,10 @@ __device__ __forceinline__ float4 tile4(const char* p) {
 //
 // Measured, bf16: 65536 x 12 x 64 STATES 51 us (201 MB at 3.9 TB/s, all that a sum which only
 // reads reaches), output 100 us (403 MB at 4.0 TB/s); 8 x 1568 x 12 x 64 15 and 20 us; 20000
-// packed x 16 x 128 62 and 117 us.  What bounds the output's pass is the chain through a chunk,
-// not one unit: of the 117 us the state's sum and its product, most of the matrix work, are worth
-// 15 each and 26 together, then stores 28, loads 18, and 34 are left without anything else.
+// packed x 16 x 128 57 and 106 us.  What bounds the output's pass is the chain through a chunk,
+// not one unit: of the latter (117 us when that was measured) the state's sum and its product, most
+// of the matrix work, are worth 15 each and 26 together, then stores 28, loads 18, and 34 are
+// left without anything else.
 template <class K, typename OT, int NP, int NS, bool STATES, bool GRAD, bool DOT>
 __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K::OCC) void kda_decay_mix_kernel(const DecayArgs a) {
     typedef typename K::ST ST;
@@ -504,7 +532,8 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
     Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : NP * K::PPL));
     float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]
 
-    const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x), cols = bid % K::SPLIT, jh = bid / K::SPLIT, j = jh / a.H, h = jh - j * a.H;
+    int j, h, cols;
+    work_of<K::SPLIT>(a, j, h, cols);
     const Slot s = slot_of(a, j);
     if (s.seq < 0) {
         if constexpr (!STATES) {
@@ -659,10 +688,10 @@ constexpr float ANCHOR_BELOW = 0x1p-32f;
 // one sum over the slot, dg of fast decays was 2 to 60 times as far off.  Sums in fp64.
 // PARTS: of dots, by channels.
 //
-// Measured, bf16: 8 x 1568 x 12 x 64 45 us; 20000 packed x 16 x 128 325 us, where four heads share
+// Measured, bf16: 8 x 1568 x 12 x 64 45 us; 20000 packed x 16 x 128 291 us, where four heads share
 // a key and 328 MB of fp32 parts are written, 64 us of it.  Two states of D x D in registers
 // leave two waves a SIMD (D <= 64: three), so a chunk's chain of products is seen in full; parts of
-// the channels as in mix would form both kinds of pairs twice (343 us).
+// the channels as in mix would form both kinds of pairs twice (343 us for 325 then).
 template <class K, typename OT, int NP, int NS, bool DOT, int PARTS>
 __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const DecayArgs a) {
     static_assert(K::SPLIT == 1, "dg takes all channels");
@@ -679,7 +708,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
     float* e_own = part + K::NW * K::C;                // sums over the other tokens, of X rows (k, v)
     float* e_oth = e_own + K::TT * K::C;               // and of Y rows (q, do)
 
-    const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x), j = bid / a.H, h = bid - j * a.H;
+    int j, h, cols;
+    work_of<1>(a, j, h, cols);
     const Slot s = slot_of(a, j);
     if (s.seq < 0) {
         if (s.seq == -1) {
@@ -873,17 +903,20 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
 // Slots of packed sequences, cu[0 .. nseq] their limits (taken as rising and within
 // [0, T], whatever they hold): tab as slot_of reads it, first[i] sequence i's first
 // slot.  What lies before the first and behind the last sequence becomes slots of
-// no sequence, after the others.
+// no sequence, after the others.  order: the slots as workgroups take them, whole ones
+// first, so that the last round is of short ones.
 constexpr int PLAN_TH = 1024;
 __global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, int nseq, int T, int seg_tokens, int4* tab,
-                                                                 int* first, int nslots) {
+                                                                 int* first, int* order, int nslots) {
     __shared__ int buf[PLAN_TH];
-    __shared__ int carry_end, carry_slots;
+    __shared__ int carry_end, carry_slots, carry_whole;
     const int t = threadIdx.x;
     if (t == 0) {
         carry_end = min(max(cu[0], 0), T);
         carry_slots = 0;
+        carry_whole = 0;
     }
+    __syncthreads();   // (without sequences the next read is behind the loop)
     const int begin = min(max(cu[0], 0), T);
     for (int i0 = 0; i0 < nseq; i0 += PLAN_TH) {
         const int i = i0 + t;
@@ -908,20 +941,35 @@ __global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, 
             __syncthreads();
         }
         const int at = carry_slots + buf[t] - slots, total = carry_slots + buf[PLAN_TH - 1];
+        __syncthreads();
+        const int whole = n / seg_tokens;
+        buf[t] = whole;
+        __syncthreads();
+        for (int k = 1; k < PLAN_TH; k <<= 1) {
+            const int x = t >= k ? buf[t - k] : 0;
+            __syncthreads();
+            buf[t] += x;
+            __syncthreads();
+        }
+        const int whole_at = carry_whole + buf[t] - whole, whole_total = carry_whole + buf[PLAN_TH - 1];
         if (i < nseq) {
             first[i] = at;
-            for (int k = 0; k < slots; ++k)
+            for (int k = 0; k < slots; ++k) {
                 tab[at + k] = make_int4(lo + k * seg_tokens, min(seg_tokens, n - k * seg_tokens), i,
                                         (k == 0) | (k == slots - 1) << 1);
+                // whole ones from the front; the others, of which at - whole_at came before, from behind
+                order[k < whole ? whole_at + k : nslots - 1 - (at - whole_at)] = at + k;
+            }
         }
         __syncthreads();
         if (t == 0) {
             carry_end = top;
             carry_slots = total;
+            carry_whole = whole_total;
         }
         __syncthreads();
     }
-    const int used = carry_slots, end = carry_end;
+    const int used = carry_slots, end = carry_end, wholes = carry_whole;
     if (t == 0) first[nseq] = used;
     const int lead = (begin + seg_tokens - 1) / seg_tokens, trail = (T - end + seg_tokens - 1) / seg_tokens;
     for (int k = t; k < nslots - used; k += PLAN_TH) {
@@ -930,6 +978,7 @@ __global__ __launch_bounds__(PLAN_TH) void kda_decay_plan_kernel(const int* cu, 
         else if (k - lead < trail)
             v = make_int4(end + (k - lead) * seg_tokens, min(seg_tokens, T - end - (k - lead) * seg_tokens), -1, 0);
         tab[used + k] = v;
+        order[wholes + k] = used + k;
     }
 }
 
@@ -985,8 +1034,8 @@ __global__ __launch_bounds__(64) void kda_decay_dg_sum_kernel(const double* sums
 }
 
 // gradients of a tensor whose heads are shared: sums over the state's heads, rounded once.
-// Bound by its bytes: 20000 x 16 x 128 to 4 heads 31 us, 5.9 TB/s (what mix2 has just written
-// is partly still in a cache).
+// Bound by its bytes: 20000 x 16 x 128 to 4 heads 31 to 33 us, 5.8 TB/s (what mix2 has just
+// written is partly still in a cache).
 template <typename OT>
 __global__ __launch_bounds__(256) void kda_decay_group_kernel(const float* src, OT* dst, int64_t n4, int share, int D) {
     const int per = D / 4;
@@ -1095,22 +1144,38 @@ struct Plan {
 // How many chunks of 64 tokens a slot has.  Sequences that fill the card by themselves are
 // one slot each; else what is shared out costs a pass for the slots' states and a scan
 // over them, and the workgroups come in rounds of as many as fit beside each other: the
-// least of all counts.  (Measured at D = 64, bf16, in chunks' times of a full card, 7.5 us: a
-// chunk takes 0.33 in a workgroup alone; half as much again in the first pass; the two more
-// launches 0.9 and a slot of the scan 0.02.  8 x 1568 x 12 x 64 takes 42 us in slots of 3
-// chunks, 45 of 2 or 4, 68 whole; 196 x 6 x 64 14.5 of one chunk, 12.1 whole.)
+// least of all counts.  (In chunks' times of a full card, 7.5 us at D = 64, bf16, where it was
+// measured: a chunk takes 0.33 in a workgroup alone, a slot's beginning a third of a chunk;
+// the pass for the states half of the forward pass, dq 1.2 of it and mix2, of which fewer
+// fit, 2.1; the two more launches 0.9 and a slot of the scan 0.02.  8 x 1568 x 12 x 64 takes 42 us
+// in slots of 3 chunks, 45 of 2 or 4, 68 whole; 196 x 6 x 64 14.5 of one chunk, 12.1 whole; 20000
+// packed x 16 x 128 forward and backward 724 of 7, 769 of 5, 779 of 6, 754 of 12, 835 of 3.)
 Plan plan_of(const Args& a, bool train) {
     Plan p;
     p.packed = a.cu != nullptr;
-    const int64_t seqs = p.packed ? a.nseq : a.B, rows = p.packed ? 1 : a.B, chunks = std::max<int64_t>(1, (a.T + 63) / 64);
+    const int64_t rows = p.packed ? 1 : a.B, chunks = std::max<int64_t>(1, (a.T + 63) / 64);
     // dg is a sum over a slot's tokens, whose errors add up
-    const int64_t most = train ? 32 : chunks, fit = a.D <= 64 ? 1024 : 512;
+    const int64_t most = train ? 32 : chunks;
+    const double fit = a.D <= 64 ? 1024 : 384, fit2 = a.D <= 64 ? 768 : 256;
+    // rounds of `fit` that `whole` slots and `parts` slots of a `rest` of their length take
+    const auto turns = [](double whole, double parts, double rest, double fit) {
+        const double full = std::floor(whole / fit), left = whole - full * fit;
+        const auto round = [&](double n) { return n > 0.0 ? 0.33 + 0.67 * std::min(1.0, n / fit) : 0.0; };
+        if (left == 0.0) return full + rest * round(parts);
+        return left + parts <= fit ? full + round(left + rest * parts) : full + 1.0 + rest * round(left + parts - fit);
+    };
     double best = 0.0;
     int64_t seg = 0;
     for (int64_t c = 1; c <= most; c = c < 64 || c == chunks ? c + 1 : chunks) {
-        const int64_t per = (chunks + c - 1) / c, n = (p.packed ? per + seqs / 2 : rows * per) * a.H, rest = n % fit;
-        const double turns = (double)(n / fit) + (rest ? 0.33 + 0.67 * (double)rest / fit : 0.0);
-        const double cost = (double)c * turns * (p.packed || per > 1 ? 1.5 : 1.0) + (p.packed || per > 1 ? 0.9 + 0.02 * per : 0.0);
+        const int64_t per = (chunks + c - 1) / c;
+        const bool multi = p.packed || per > 1;
+        // (packed sequences' last slots, of unknown lengths, are taken last and fill a round)
+        const double slots = (double)a.T / (64 * c), all = p.packed ? slots : std::floor(slots), n = (double)rows * a.H;
+        const auto t = [&](double f) { return turns(n * all, slots > all ? n : 0.0, slots - all, f); };
+        double cost = t(fit) * (multi ? 1.5 : 1.0);
+        if (train) cost += t(fit) * (multi ? 1.7 : 1.2) + t(fit2) * 2.1;
+        cost *= c + 0.35;
+        if (multi) cost += (0.9 + 0.02 * a.D / 64 * per) * (train ? 2 : 1);
         if (!seg || cost < best) {
             best = cost;
             seg = c;
@@ -1127,7 +1192,7 @@ Plan plan_of(const Args& a, bool train) {
 // Parts in bytes: the slots and the states at their starts, which the backward pass reads
 // again (kept); and the backward pass' own
 struct Layout {
-    int64_t tab = -1, first = -1, s = -1, seg = -1, kept = 0;
+    int64_t tab = -1, first = -1, order = -1, s = -1, seg = -1, kept = 0;
     int64_t ds = -1, segd = -1, dots = -1, sums = -1, g0 = -1, g1 = -1, bytes = 0;
 };
 bool shared(const Args& a, const kda_decay_rows& r) { return r.heads != a.H; }
@@ -1137,6 +1202,7 @@ Layout layout_of(const Args& a, const Plan& p) {
     if (p.packed) {
         l.tab = take(l.kept, 16 * (int64_t)p.nslots);
         l.first = take(l.kept, 4 * (a.nseq + 1));
+        l.order = take(l.kept, 4 * (int64_t)p.nslots);
     }
     const int64_t st = 4 * (int64_t)p.nslots * a.H * a.D * a.D, sg = 4 * (int64_t)p.nslots * a.H, rows = 4 * a.B * a.T * a.H;
     if (p.multi) {
@@ -1210,6 +1276,7 @@ DecayArgs base_of(const Args& a, const Plan& p, const Layout& l, char* kept) {
     d.nseq = (int)(a.cu ? a.nseq : a.B);
     d.nslots = p.nslots; d.per_seq = p.per_seq; d.seg_tokens = p.seg_tokens;
     d.tab = p.packed ? reinterpret_cast<const int4*>(kept + l.tab) : nullptr;
+    d.order = p.packed ? reinterpret_cast<const int*>(kept + l.order) : nullptr;
     d.in_by_slot = p.multi;
     return d;
 }
@@ -1264,7 +1331,7 @@ int forward(const Args& a, hipStream_t st) {
     int* first = p.packed ? reinterpret_cast<int*>(kept + l.first) : nullptr;
     if (p.packed) {
         hipLaunchKernelGGL(kda_decay_plan_kernel, dim3(1), dim3(PLAN_TH), 0, st, a.cu, (int)a.nseq, (int)a.T, p.seg_tokens,
-                           reinterpret_cast<int4*>(kept + l.tab), first, p.nslots);
+                           reinterpret_cast<int4*>(kept + l.tab), first, reinterpret_cast<int*>(kept + l.order), p.nslots);
         DEC_HIP(hipGetLastError());
     }
     if (p.multi) {

@@ -158,7 +158,7 @@ def test_limits_out_of_order():
 
 
 def test_sequences_do_not_meet():
-    """Values that are not finite stay in their sequence, and behind its 64 tokens; the gradients before."""
+    """Values that are not finite stay in their sequence, and behind the start of its 32 tokens; the gradients before."""
     x = inputs(1, 300, 2, 64, BF, state=True, n=3)
     cu = torch.tensor([0, 100, 230, 300], dtype=torch.int32, device=DEV)
     clean = chunk_decay(x["q"], x["k"], x["v"], x["g"], x["s0"], cu)
