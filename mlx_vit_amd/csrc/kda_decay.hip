@@ -148,10 +148,13 @@ struct Sw {
 // 190 us instead of 175 over 65536 x 12 x 64: too few waves), a workgroup a SPLIT-th of
 // them: the pairs are then formed SPLIT times, but by waves that would wait for them (20000
 // packed x 16 x 128: 115 instead of 128 us forward, dq 147 instead of 185).  bf16 operands are
-// one plane, fp32 ones three.  OCC, OCC2: waves a SIMD that mix and mix2 are held to.
+// one plane, fp32 ones three, and so are the pairs' weights and the state as factors (NP): with two,
+// 16 bits, one bf16 output in 450 is rounded the other way, so one in 6000 to 18000, for 1 to 3%
+// of the time (65536 x 12 x 64 153.1 -> 154.7 us, 20000 packed x 16 x 128 forward and backward 726 -> 747).
+// OCC, OCC2: waves a SIMD that mix and mix2 are held to.
 template <int D_, bool F32_, int SPLIT_ = 1, int C_ = 32>
 struct Cfg {
-    static constexpr int D = D_, C = C_, SPLIT = SPLIT_, DW = D / SPLIT, NPL = F32_ ? 3 : 1, NW = DW / 16, NTH = 64 * NW;
+    static constexpr int D = D_, C = C_, SPLIT = SPLIT_, DW = D / SPLIT, NPL = F32_ ? 3 : 1, NP = 3, NW = DW / 16, NTH = 64 * NW;
     static constexpr int RB = 2 * D, PLANE = C * RB, TILE = NPL * PLANE;                       // bytes
     static constexpr int RBW = (2 * DW + 63) / 64 * 64, PLANEW = C * RBW, TILEW = NPL * PLANEW;   // of DW channels
     static constexpr int RP = 2 * C, PPL = C * RP;                                             // of the pairs'
@@ -320,23 +323,23 @@ __device__ __forceinline__ f32x4 mask_tile(const Decays<K::C>& d, int ti, int si
     for (int i = 0; i < 4; ++i) m[i] = s0 + i <= t ? __builtin_amdgcn_exp2f((h - hv[i]) + (o - lv[i])) : 0.f;
     return m;
 }
-// a tile of NP planes into P[t][s]
-template <class K, int NP>
+// a tile into P[t][s]
+template <class K>
 __device__ __forceinline__ void put_pair(char* P, const f32x4& v, int ti, int si) {
     const int l = lane_id(), g = l >> 4;
     char* p = P + Sw<K::RP>::at(16 * ti + (l & 15), 2 * si + (g >> 1)) + 8 * (g & 1);
     float x[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
+    for (int i = 0; i < K::NP; ++i) {
         const uint32_t a = pack2bf(x[0], x[1]), b = pack2bf(x[2], x[3]);
         *reinterpret_cast<uint2*>(p + i * K::PPL) = make_uint2(a, b);
-        if (i + 1 < NP) { x[0] -= bf_lo(a); x[1] -= bf_hi(a); x[2] -= bf_lo(b); x[3] -= bf_hi(b); }
+        if (i + 1 < K::NP) { x[0] -= bf_lo(a); x[1] -= bf_hi(a); x[2] -= bf_lo(b); x[3] -= bf_hi(b); }
     }
 }
 // the tiles above the diagonal that products of 32 columns read
-template <class K, int NP>
+template <class K>
 __device__ __forceinline__ void clear_upper(char* P) {
-    for (int v = threadIdx.x; v < NP * (K::TT / 2) * 16 * 2; v += K::NTH) {
+    for (int v = threadIdx.x; v < K::NP * (K::TT / 2) * 16 * 2; v += K::NTH) {
         const int c = v & 1, row = (v >> 1) & 15, b = (v >> 5) % (K::TT / 2), p = (v >> 5) / (K::TT / 2);
         *reinterpret_cast<uint4*>(P + p * K::PPL + Sw<K::RP>::at(32 * b + row, 4 * b + 2 + c)) = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -411,9 +414,7 @@ struct State {
             for (int i = 0; i < 4; ++i) s[j][i] = fmaf(own, s[j][i], all * u[i]);
         }
     }
-    // up_t (St^T X_t) for every row, the state as NS planes: lane (m, r) has row 16 i + m,
-    // channels 16 w + 4 r ..
-    template <int NS>
+    // up_t (St^T X_t) for every row: lane (m, r) has row 16 i + m, channels 16 w + 4 r ..
     __device__ __forceinline__ void apply(const char* X, const Decays<K::C>& d, f32x4 (&o)[K::TT]) const {
 #pragma unroll
         for (int i = 0; i < K::TT; ++i) o[i] = zero4();
@@ -421,8 +422,8 @@ struct State {
         for (int k = 0; k < K::KD; ++k) {
             const f32x4 &x = s[2 * k], &y = s[2 * k + 1];
             const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            bf16x8 f[NS];
-            planes8<NS>(v, f);
+            bf16x8 f[K::NP];
+            planes8<K::NP>(v, f);
 #pragma unroll
             for (int i = 0; i < K::TT; ++i) {
                 bf16x8 x[K::NPL];
@@ -436,12 +437,12 @@ struct State {
 };
 
 // o_t += sum_s P[t][s] W_s, layout as State::apply
-template <class K, int NP>
+template <class K>
 __device__ __forceinline__ void add_pairs(const char* P, const bf16x8 (&w)[K::NPL], f32x4 (&o)[K::TT]) {
 #pragma unroll
     for (int i = 0; i < K::TT; ++i) {
-        bf16x8 p[NP];
-        along<K::RP, NP, K::PPL>(P, 16 * i, 0, p);
+        bf16x8 p[K::NP];
+        along<K::RP, K::NP, K::PPL>(P, 16 * i, 0, p);
         o[i] = mmp(w, p, o[i]);
     }
 }
@@ -483,9 +484,9 @@ __device__ __forceinline__ void clear_rows(void* out, const DecayArgs& a, const 
         static_cast<OT*>(out)[((int64_t)(s.tok0 + v / D) * a.H + h) * D + v % D] = OT(0);
 }
 
-template <class K, int NP>
+template <class K>
 constexpr size_t mix_lds(bool states, bool grad, bool dot) {
-    return (states ? 1 : grad ? 3 : 2) * (size_t)K::TILE + K::TILEW + (states ? 0 : (size_t)NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
+    return (states ? 1 : grad ? 3 : 2) * (size_t)K::TILE + K::TILEW + (states ? 0 : (size_t)K::NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
            (dot ? (size_t)K::NW * K::C * 4 : 0);
 }
 // four channels of a row of a tile
@@ -505,8 +506,7 @@ __device__ __forceinline__ float4 tile4(const char* p) {
 // add to dS as well, sum of e^{G_t} do_t q_t^T (WITH_DS: 8 x 1568 x 12 x 64 34 us, by a pass of its
 // own 27 + 15; at D = 128 that leaves registers for two waves a SIMD instead of three, 213 us of
 // 20000 packed x 16, by itself 148 + 64); STATES and GRAD: dS alone.  DOT: dots[t] = q_t . (the
-// part of out_t that comes from the state before the chunk), which NS = 3 keeps to fp32; by
-// parts of the channels.
+// part of out_t that comes from the state before the chunk), by parts of the channels.
 //
 // A chunk: pairs, state and the state's part of out from LDS; a barrier; the pairs'
 // part from P and registers, and the next chunk into LDS; a barrier.  Its loads are in
@@ -519,17 +519,17 @@ __device__ __forceinline__ float4 tile4(const char* p) {
 // not one unit: of the latter (117 us when that was measured) the state's sum and its product, most
 // of the matrix work, are worth 15 each and 26 together, then stores 28, loads 18, and 34 are
 // left without anything else.
-template <class K, typename OT, int NP, int NS, bool STATES, bool GRAD, bool DOT>
+template <class K, typename OT, bool STATES, bool GRAD, bool DOT>
 __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K::OCC) void kda_decay_mix_kernel(const DecayArgs a) {
     typedef typename K::ST ST;
     constexpr bool DQ = GRAD && !STATES, DS = DQ && K::WITH_DS;
-    __shared__ __attribute__((aligned(16))) char lds[mix_lds<K, NP>(STATES, DS, DOT)];
+    __shared__ __attribute__((aligned(16))) char lds[mix_lds<K>(STATES, DS, DOT)];
     char* X = lds;
     char* Y = X + (STATES ? 0 : K::TILE);
     char* Z = Y + K::TILE;
     char* W = Z + (DS ? K::TILE : 0);
     char* P = W + K::TILEW;
-    Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : NP * K::PPL));
+    Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : K::NP * K::PPL));
     float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]
 
     int j, h, cols;
@@ -572,7 +572,7 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
         if constexpr (DS) sz.store(Z, n);
         sw.store(W, n);
     };
-    if constexpr (!STATES) clear_upper<K, NP>(P);
+    if constexpr (!STATES) clear_upper<K>(P);
     double whole = 0.0;
     if (s.n > 0) {
         load(0);
@@ -608,10 +608,10 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
                     tile_of(id, ti, si);
                     f32x4 p = pair_tile<K>(X, Y, ti, si);
                     p *= mask_tile<K>(d, ti, si);
-                    put_pair<K, NP>(P, p, ti, si);
+                    put_pair<K>(P, p, ti, si);
                 }
             }
-            st.template apply<NS>(X, d, o);
+            st.apply(X, d, o);
             if constexpr (DOT) {
 #pragma unroll
                 for (int i = 0; i < K::TT; ++i) {
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
         }
         if constexpr (!STATES) {
             const int64_t row = (int64_t)b * a.T + s.tok0 + i0;
-            add_pairs<K, NP>(P, w, o);
+            add_pairs<K>(P, w, o);
             put_rows<K, OT, false>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, wv, n);
             if constexpr (DOT) {
                 const int t = threadIdx.x;
@@ -669,9 +669,9 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
     }
 }
 
-template <class K, int NP>
+template <class K>
 constexpr size_t mix2_lds(bool dot) {
-    return 4 * (size_t)K::TILE + 2 * (size_t)NP * K::PPL + 2 * sizeof(Decays<K::C>) +
+    return 4 * (size_t)K::TILE + 2 * (size_t)K::NP * K::PPL + 2 * sizeof(Decays<K::C>) +
            (dot ? (size_t)(K::NW + 2 * K::TT) * K::C * 4 : 0);
 }
 // e^{sum of g over a chunk} below which what passes through it is nothing beside what begins in it
@@ -692,18 +692,18 @@ constexpr float ANCHOR_BELOW = 0x1p-32f;
 // a key and 328 MB of fp32 parts are written, 64 us of it.  Two states of D x D in registers
 // leave two waves a SIMD (D <= 64: three), so a chunk's chain of products is seen in full; parts of
 // the channels as in mix would form both kinds of pairs twice (343 us for 325 then).
-template <class K, typename OT, int NP, int NS, bool DOT, int PARTS>
+template <class K, typename OT, bool DOT, int PARTS>
 __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const DecayArgs a) {
     static_assert(K::SPLIT == 1, "dg takes all channels");
     typedef typename K::ST ST;
-    __shared__ __attribute__((aligned(16))) char lds[mix2_lds<K, NP>(DOT)];
+    __shared__ __attribute__((aligned(16))) char lds[mix2_lds<K>(DOT)];
     char* Kt = lds;
     char* Q = Kt + K::TILE;
     char* V = Q + K::TILE;
     char* O = V + K::TILE;
     char* PA = O + K::TILE;
-    char* PD = PA + NP * K::PPL;
-    Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(PD + NP * K::PPL);
+    char* PD = PA + K::NP * K::PPL;
+    Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(PD + K::NP * K::PPL);
     float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]; then E's [TT column tiles][C] and [TT row tiles][C]
     float* e_own = part + K::NW * K::C;                // sums over the other tokens, of X rows (k, v)
     float* e_oth = e_own + K::TT * K::C;               // and of Y rows (q, do)
@@ -778,8 +778,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         rv.store(V, n);
         ro.store(O, n);
     };
-    clear_upper<K, NP>(PA);
-    clear_upper<K, NP>(PD);
+    clear_upper<K>(PA);
+    clear_upper<K>(PD);
     if constexpr (DOT)
         for (int v = threadIdx.x; v < 2 * K::TT * K::C; v += K::NTH) e_own[v] = 0.f;
     if (s.n > 0) {
@@ -809,8 +809,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
                 tile_of(id, ti, si);
                 const f32x4 m = mask_tile<K>(d, ti, si);
                 const f32x4 pa = pair_tile<K>(Kt, Q, ti, si) * m, pd = pair_tile<K>(V, O, ti, si);
-                put_pair<K, NP>(PA, pa, ti, si);
-                put_pair<K, NP>(PD, pd * m, ti, si);
+                put_pair<K>(PA, pa, ti, si);
+                put_pair<K>(PD, pd * m, ti, si);
                 if constexpr (DOT) {
                     // a token's own pair passes no decay, and would drown what does where decays are fast
                     f32x4 e = pa * pd;
@@ -830,8 +830,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
             }
         }
         f32x4 o[K::TT], o2[K::TT];
-        sv.template apply<K::NPL == 3 ? 3 : NP>(Kt, d, o);
-        sk.template apply<NS>(V, d, o2);
+        sv.apply(Kt, d, o);
+        sk.apply(V, d, o2);
         if constexpr (DOT) {
             const int ch = 16 * wave + 4 * (l >> 4);
 #pragma unroll
@@ -855,8 +855,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
             if (i0 + n + K::C < s.n) load(i0 + n + K::C, K::C);
         }
         const int64_t row = (int64_t)b * a.T + s.tok0 + s.n - i0 - n, out = (row * a.H + h) * K::D;
-        add_pairs<K, NP>(PA, wo, o);
-        add_pairs<K, NP>(PD, wq, o2);
+        add_pairs<K>(PA, wo, o);
+        add_pairs<K>(PD, wq, o2);
         put_rows<K, OT, true>(static_cast<OT*>(a.out) + out, (uint32_t)(a.H * K::D), o2, wave, n);
         put_rows<K, OT, true>(static_cast<OT*>(a.out2) + out, (uint32_t)(a.H * K::D), o, wave, n);
         if constexpr (DOT) {
@@ -1281,9 +1281,9 @@ DecayArgs base_of(const Args& a, const Plan& p, const Layout& l, char* kept) {
     return d;
 }
 
-template <class K, typename OT, int NP, int NS, bool STATES, bool GRAD, bool DOT>
+template <class K, typename OT, bool STATES, bool GRAD, bool DOT>
 hipError_t launch_mix(const DecayArgs& d, hipStream_t st) {
-    hipLaunchKernelGGL((kda_decay_mix_kernel<K, OT, NP, NS, STATES, GRAD, DOT>), dim3((unsigned)(d.nslots * d.H * K::SPLIT)),
+    hipLaunchKernelGGL((kda_decay_mix_kernel<K, OT, STATES, GRAD, DOT>), dim3((unsigned)(d.nslots * d.H * K::SPLIT)),
                        dim3(K::NTH), 0, st, d);
     return hipGetLastError();
 }
@@ -1318,12 +1318,9 @@ hipError_t launch_group(const float* src, void* dst, const Args& a, const kda_de
 
 template <int D>
 constexpr int SPLIT_OF = D > 64 ? 2 : 1;
-// Planes of the pairs' products and of the state in bf16's products with it: two make
-// what is lost there small beside the output's own rounding.
 template <int D, bool F32>
 int forward(const Args& a, hipStream_t st) {
     typedef Cfg<D, F32, SPLIT_OF<D>> K;
-    constexpr int NP = F32 ? 3 : 2;
     const Plan p = plan_of(a, a.train != 0);
     const Layout l = layout_of(a, p);
     char* kept = static_cast<char*>(a.train ? a.kept : a.workspace);
@@ -1340,7 +1337,7 @@ int forward(const Args& a, hipStream_t st) {
         m.w = rows_of(a, a.v);
         m.s_out = reinterpret_cast<float*>(kept + l.s);
         m.seg = reinterpret_cast<float*>(kept + l.seg);
-        DEC_HIP((launch_mix<K, float, 1, 1, true, false, false>(m, st)));
+        DEC_HIP((launch_mix<K, float, true, false, false>(m, st)));
         DEC_HIP(launch_scan<false>(m, D, m.s_out, m.seg, first, a.s0, st));
     }
     d.x = rows_of(a, a.q);
@@ -1349,14 +1346,13 @@ int forward(const Args& a, hipStream_t st) {
     d.out = a.o;
     d.s_in = p.multi ? reinterpret_cast<float*>(kept + l.s) : a.s0;
     d.s_out = a.s_final;
-    DEC_HIP((launch_mix<K, typename K::ST, NP, NP, false, false, false>(d, st)));
+    DEC_HIP((launch_mix<K, typename K::ST, false, false, false>(d, st)));
     return KDA_OK;
 }
 
-template <class K, typename OT, int NP, bool DOT, int PARTS>
+template <class K, typename OT, bool DOT, int PARTS>
 hipError_t launch_mix2(const DecayArgs& d, hipStream_t st) {
-    hipLaunchKernelGGL((kda_decay_mix2_kernel<K, OT, NP, DOT ? 3 : NP, DOT, PARTS>), dim3((unsigned)(d.nslots * d.H)), dim3(K::NTH), 0, st,
-                       d);
+    hipLaunchKernelGGL((kda_decay_mix2_kernel<K, OT, DOT, PARTS>), dim3((unsigned)(d.nslots * d.H)), dim3(K::NTH), 0, st, d);
     return hipGetLastError();
 }
 
@@ -1365,7 +1361,6 @@ int backward(const Args& a, hipStream_t st) {
     typedef Cfg<D, F32, SPLIT_OF<D>> K;
     typedef Cfg<D, F32> K2;
     typedef typename K::ST ST;
-    constexpr int NP = F32 ? 3 : 2;
     const Plan p = plan_of(a, true);
     const Layout l = layout_of(a, p);
     char *ws = static_cast<char*>(a.workspace), *kept = static_cast<char*>(a.kept);
@@ -1388,15 +1383,15 @@ int backward(const Args& a, hipStream_t st) {
     if (p.multi && !K::WITH_DS) {   // dS of the slots by itself; else with dq
         DecayArgs m = d;
         m.y = q; m.w = o;
-        DEC_HIP((launch_mix<K, float, 1, 1, true, true, false>(m, st)));
+        DEC_HIP((launch_mix<K, float, true, true, false>(m, st)));
         DEC_HIP(scan());
     }
     d.out = shared(a, a.q) ? g0 : a.dq;
     if (shared(a, a.q)) {
-        DEC_HIP((launch_mix<K, float, NP, DOT ? 3 : NP, false, true, DOT>(d, st)));
+        DEC_HIP((launch_mix<K, float, false, true, DOT>(d, st)));
         DEC_HIP(launch_group<ST>(g0, a.dq, a, a.q, st));
     } else {
-        DEC_HIP((launch_mix<K, ST, NP, DOT ? 3 : NP, false, true, DOT>(d, st)));
+        DEC_HIP((launch_mix<K, ST, false, true, DOT>(d, st)));
     }
     if (p.multi && K::WITH_DS) DEC_HIP(scan());
     d = base;
@@ -1411,12 +1406,12 @@ int backward(const Args& a, hipStream_t st) {
     d.sums = sums;
     if (shared(a, a.k) || shared(a, a.v)) {
         d.out = g0; d.out2 = g1;
-        DEC_HIP((launch_mix2<K2, float, NP, DOT, K::SPLIT>(d, st)));
+        DEC_HIP((launch_mix2<K2, float, DOT, K::SPLIT>(d, st)));
         DEC_HIP(launch_group<ST>(g0, a.dk, a, a.k, st));
         DEC_HIP(launch_group<ST>(g1, a.dv, a, a.v, st));
     } else {
         d.out = a.dk; d.out2 = a.dv;
-        DEC_HIP((launch_mix2<K2, ST, NP, DOT, K::SPLIT>(d, st)));
+        DEC_HIP((launch_mix2<K2, ST, DOT, K::SPLIT>(d, st)));
     }
     if (sums) DEC_HIP(launch_dg_sum(sums, a.dg, d.nslots, d.H, st));
     return KDA_OK;
