@@ -1,7 +1,7 @@
 """DecayAttentionLayer: linear attention with a decay for each head and rotary positions.
 
-The place of ``GatedDeltaLayer`` in a block (the same call, the same state), without the delta
-rule and the short convolutions, so without a write gate, and with positions on a video's
+The place of ``GatedDeltaLayer`` in a block (the same state, the same call but for the tokens'
+numbers), without the delta rule and the short convolutions, so without a write gate, and with positions on a video's
 axes instead: queries and keys are turned (``rotary``), mixed by ``chunk_decay`` and
 normalised and gated by ``RMSNormGated`` (nope_gdn_mlx.py:340-366).  The decay is the
 reference's decay gate for one head (nope_gdn_mlx.py:812-819),
@@ -27,8 +27,10 @@ def video_sections(head_dim: int) -> Tuple[int, int, int]:
 
 
 class DecayAttentionLayer(nn.Module):
-    """``forward(x, state=None, start=0) -> (out, new_state)``, x (B, L, hidden_size), state
-    (B, H, D, D) fp32 or None; ``start``: the first token's number in its video.
+    """``forward(x, state=None, start=None) -> (out, new_state)``, x (B, L, hidden_size), state
+    (B, H, D, D) fp32 or None; ``start``: the first token's number in its video, of all rows (a
+    number, which a captured graph keeps).  A state holds keys turned by their positions, so whoever
+    goes on from one says from where; without a state it is 0.
     ``grid`` = (height, width): the tokens of a frame.  ``num_kv_heads``: key and value heads, each
     shared by num_heads / num_kv_heads heads (default: one each)."""
 
@@ -65,13 +67,17 @@ class DecayAttentionLayer(nn.Module):
         return q, k, v, g
 
     def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None,
-                start: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+                start: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        if start is None:
+            if state is not None:
+                raise ValueError("a state was given without start, the number of the first token in its video")
+            start = 0
         o, new_state = chunk_decay(*self._operands(x, start), state)
         return self.o_proj(self.o_norm(o, self.g_proj(x))), new_state
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, state: torch.Tensor, start: int) -> torch.Tensor:
-        """The next token of each row, x (B, 1, hidden_size), number ``start`` of its video; ``state`` is updated."""
+        """The next token of each row, x (B, 1, hidden_size), number ``start`` of its video, in all rows; ``state`` is updated."""
         q, k, v, g = self._operands(x, start)
         if x.shape[1] != 1:
             raise ValueError(f"a step takes one token of each row; got {x.shape[1]}")

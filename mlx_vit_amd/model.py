@@ -218,7 +218,9 @@ class NoPEVideoEncoder(nn.Module):
 
 class HybridBlock(nn.Module):
     """One processor block, GDN or NoPE attention (nope_gdn_mlx.py:4009-4091); or ``decay``, linear
-    attention with rotary positions over frames of ``grid`` tokens, in the GDN's place."""
+    attention with rotary positions over frames of ``grid`` tokens, in the GDN's place.  A decay
+    block that goes on from a state takes ``start``, the number of x's first token in its video;
+    the others have no positions and leave it."""
 
     fused_mlp = False   # set_fused_mlp
 
@@ -248,7 +250,8 @@ class HybridBlock(nn.Module):
         self.mlp = _mlp(dim, mlp_ratio, dropout)
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None,
-                state: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+                state: Optional[torch.Tensor] = None,
+                start: Optional[int] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         B, N, D = x.shape
         normed = self.norm1(x)
         if self.block_type != "nope":
@@ -260,6 +263,8 @@ class HybridBlock(nn.Module):
                 out_t, _ = self.layer(xt, None)
                 out = out_t.reshape(B, S, T, D).transpose(1, 2).reshape(B, N, D)
                 new_state = state
+            elif self.block_type == "decay":
+                out, new_state = self.layer(normed, state, start)
             else:
                 out, new_state = self.layer(normed, state)
         elif self.spatial_tokens is not None:
