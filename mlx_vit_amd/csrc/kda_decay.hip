@@ -12,8 +12,8 @@
 //   dq  (do, v, k), the state transposed;
 //   dk  (v, do, q) and dv (k, q, do), backwards in time with the decay of the token
 //       behind, the state then being dS, the adjoint of S;
-//   dg_t = <S_T, dS_T> + sum_{s >= t} (q_s . dq_s - k_s . dk_s),
-// which is what reaches tokens from t on from before t.
+//   dg_t = e^{g_t} <S_{t-1}, dS_t>, what reaches tokens from t on from before t,
+// put together from what enters, leaves, crosses and passes a chunk (mix2).
 //
 // A long sequence is shared out into slots of whole chunks, a workgroup each: a pass for what
 // every slot adds to the state, a scan over the slots, and the pass for the output.  That
@@ -49,7 +49,8 @@ struct DecayArgs {
     const float* s_in;          // the state that a slot starts from, by slot or by sequence
     float* s_out;               // and ends with: by slot (states), by sequence (else); may be null
     float* dots;                // [H][B T]
-    const float *starts, *s_final;   // mix2: the state at the slots' starts, by slot, and at the sequences' ends
+    float* peaks;               // [H][chunk_count]: the largest |S| at each chunk's start
+    const float *starts, *s_final;   // mix2: the state at the starts (as s_in), and at the sequences' ends
     float* dg;                  // [B][T][H], or null
     double* sums;               // or its sums by slot, [slot][H]
     float* seg;                 // states: e^{sum of g} of each slot and head
@@ -74,6 +75,10 @@ __device__ __forceinline__ Slot slot_of(const DecayArgs& a, int j) {
     }
     return s;
 }
+// Chunks are numbered in their tokens' order, with a gap where a slot's last one is not whole:
+// chunk c of slot j, whose first token is number `tok` of all rows
+__device__ __forceinline__ int64_t chunk_number(int64_t tok, int j, int c) { return tok / 32 + j + c; }
+__host__ __device__ __forceinline__ int64_t chunk_count(int64_t B, int64_t T, int64_t nslots) { return B * T / 32 + nslots + 1; }
 // The slot, head and part of the columns of a workgroup.  Workgroups go to the 8 XCDs in
 // turn: neighbours, which read the same tokens' keys, are put into one XCD's cache; of
 // packed sequences, whose slots differ in length, only the parts of one slot and head are,
@@ -263,17 +268,34 @@ __device__ __forceinline__ double dpp(double x) {   // 0 where there is no sourc
     return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_update_dpp(0, u.x, CTRL, ROWS, 0xf, true),
                                                  __builtin_amdgcn_update_dpp(0, u.y, CTRL, ROWS, 0xf, true)));
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ float lane(float x, int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l)); }
 // sums over the lanes up to each, of 32; and the last of those, for all lanes
-__device__ __forceinline__ double prefix32(double x) {
+template <typename T>
+__device__ __forceinline__ T prefix32(T x) {
     x += dpp<0x111, 0xf>(x);   // row_shr:1, 2, 4, 8
     x += dpp<0x112, 0xf>(x);
     x += dpp<0x114, 0xf>(x);
     x += dpp<0x118, 0xf>(x);
     return x + dpp<0x142, 0xa>(x);   // row_bcast:15, into rows 1 and 3
 }
-__device__ __forceinline__ double lane31(double x) {
+__device__ __forceinline__ double lane(double x, int l) {
     const uint2 u = __builtin_bit_cast(uint2, x);
-    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(u.x, 31), __builtin_amdgcn_readlane(u.y, 31)));
+    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(u.x, l), __builtin_amdgcn_readlane(u.y, l)));
+}
+__device__ __forceinline__ double lane31(double x) { return lane(x, 31); }
+// sums over the lanes behind each, of 32, and over all of them
+__device__ __forceinline__ double behind32(double x, double& all) {
+    x += dpp<0x101, 0xf>(x);   // row_shl:1, 2, 4, 8
+    x += dpp<0x102, 0xf>(x);
+    x += dpp<0x104, 0xf>(x);
+    x += dpp<0x108, 0xf>(x);
+    const double row1 = lane(x, 16);
+    all = lane(x, 0) + row1;
+    return dpp<0x101, 0xf>(x) + (lane_id() < 16 ? row1 : 0.0);
 }
 // by one wave: lane r has g of row r (0 behind the last); returns G_C
 template <int C>
@@ -385,6 +407,29 @@ struct State {
         for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
         return x;
     }
+    // the largest magnitude of the wave's part, and the sum of them, in lane 63
+    __device__ __forceinline__ float peak() const {
+        float x = 0.f;
+#pragma unroll
+        for (int j = 0; j < K::DT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x = fmaxf(x, fabsf(s[j][i]));
+        x = fmaxf(x, dpp<0x111, 0xf>(x));
+        x = fmaxf(x, dpp<0x112, 0xf>(x));
+        x = fmaxf(x, dpp<0x114, 0xf>(x));
+        x = fmaxf(x, dpp<0x118, 0xf>(x));
+        x = fmaxf(x, dpp<0x142, 0xa>(x));
+        return fmaxf(x, dpp<0x143, 0xc>(x));   // row_bcast:31, into rows 2 and 3
+    }
+    __device__ __forceinline__ float weight() const {
+        float x = 0.f;
+#pragma unroll
+        for (int j = 0; j < K::DT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x += fabsf(s[j][i]);
+        x = prefix32(x);
+        return x + dpp<0x143, 0xc>(x);
+    }
     // S <- all S + Y^T (down W): the chunk's sum from zero, so that what the matrix unit
     // loses (it rounds sums downwards) does not add up over the chunks.  w: w_frag of W.
     __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::NPL], const Decays<K::C>& d) {
@@ -487,7 +532,7 @@ __device__ __forceinline__ void clear_rows(void* out, const DecayArgs& a, const 
 template <class K>
 constexpr size_t mix_lds(bool states, bool grad, bool dot) {
     return (states ? 1 : grad ? 3 : 2) * (size_t)K::TILE + K::TILEW + (states ? 0 : (size_t)K::NP * K::PPL) + 2 * sizeof(Decays<K::C>) +
-           (dot ? (size_t)K::NW * K::C * 4 : 0);
+           (dot ? (size_t)K::NW * (K::C + 1) * 4 : 0);
 }
 // four channels of a row of a tile
 template <class K>
@@ -531,6 +576,7 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
     char* P = W + K::TILEW;
     Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(P + (STATES ? 0 : K::NP * K::PPL));
     float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]
+    float* peak = part + K::NW * K::C;                 // [NW]
 
     int j, h, cols;
     work_of<K::SPLIT>(a, j, h, cols);
@@ -613,6 +659,8 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
             }
             st.apply(X, d, o);
             if constexpr (DOT) {
+                const float top = st.peak();
+                if (l == 63) peak[wave] = top;
 #pragma unroll
                 for (int i = 0; i < K::TT; ++i) {
                     const int t = 16 * i + (l & 15);
@@ -657,6 +705,13 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
                     for (int k = 0; k < K::NW; ++k) x += part[k * K::C + t];
                     a.dots[((int64_t)cols * a.H + h) * a.B * a.T + row + t] = x;
                 }
+                if (t == 0) {
+                    float x = peak[0];
+#pragma unroll
+                    for (int k = 1; k < K::NW; ++k) x = fmaxf(x, peak[k]);
+                    a.peaks[((int64_t)cols * a.H + h) * chunk_count(a.B, a.T, a.nslots) +
+                            chunk_number((int64_t)b * a.T + s.tok0, j, i0 / K::C)] = x;
+                }
             }
         }
         if (more) lds_barrier();
@@ -669,24 +724,41 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
     }
 }
 
+// What mix2 keeps of a chunk for dg
+struct Chunk {
+    double enter, leave;      // sums over its tokens: of what comes from before it, of what goes behind it
+    double pass;              // what passes it, counted from the slot's end
+    float entered, left;      // the first two of magnitudes
+    float off, most;          // what pass may be off by; what it cannot exceed
+    uint32_t live;            // bit i: token n - 1 - i has a decay that is not zero
+    float pad;
+};
+constexpr int SLOT_CHUNKS = 64;   // of a slot in training: a lane each
 template <class K>
 constexpr size_t mix2_lds(bool dot) {
     return 4 * (size_t)K::TILE + 2 * (size_t)K::NP * K::PPL + 2 * sizeof(Decays<K::C>) +
-           (dot ? (size_t)(K::NW + 2 * K::TT) * K::C * 4 : 0);
+           (dot ? SLOT_CHUNKS * sizeof(Chunk) + 2 * (2 * K::TT * K::C * 8 + K::NW * (K::C + 1) * 4) : 0);
 }
-// e^{sum of g over a chunk} below which what passes through it is nothing beside what begins in it
-constexpr float ANCHOR_BELOW = 0x1p-32f;
-
+// What rounding leaves open in a sum of such magnitudes
+constexpr float SUM_OFF = 0x1p-22f;
+// a number within +-most, and NaN as it is
+__device__ __forceinline__ double within(double x, float most) { return x > most ? most : x < -most ? -most : x; }
 // mix2: dk and dv of a slot, backwards in time, from q (y), k (x), v (z) and do (w), with
 // dS in both orders: dv = mix(k, q, do), dk = mix(v, do, q).
 // DOT: dg too, what passes from before token t to t or later.  With a_t and b_t the parts of
-// q_t . dq_t and k_t . dk_t that come through the state (a: dots, from mix), and E_{ts} =
-// e^{G_t - G_s} (q_t . k_s) (do_t . v_s) the chunk's own pairs, s < t,
-//   dg_t = <S, dS> behind the chunk + sum of a - b from t on + sum of E_{t' s}, t' >= t > s.
-// What the pairs give stays in their chunk, and where nothing passes through a chunk <S, dS>
-// behind it begins anew, as all that leaves it (the sum of b): with all of q . dq - k . dk in
-// one sum over the slot, dg of fast decays was 2 to 60 times as far off.  Sums in fp64.
-// PARTS: of dots, by channels.
+// q_t . dq_t and k_t . dk_t that come through the state (a: dots, from mix), E_{ts} =
+// e^{G_t - G_s} (q_t . k_s) (do_t . v_s) the chunk's own pairs, s < t, and P what passes all of
+// the chunk,
+//   dg_t = P + sum of a from t on + sum of b before t + sum of E_{t' s}, t' >= t > s:
+// no difference of large sums but in P.  Behind the chunk passes P + sum of b, before it P + sum
+// of a, so P follows from <S, dS> at the slot's end, chunk by chunk backwards, and from that
+// at its start forwards: each off by what the sums on its way are off by, the smaller is
+// taken.  (From one side alone dg is lost where little gets through: with a loss on the last
+// token and g = -0.2, 100 tokens before it.)  Nor can P exceed e^{G_C} max|S| sum|dS|,
+// which ends what came from large sums nearby: with all of q . dq - k . dk in one sum over
+// the slot, dg of fast decays was 2 to 60 times as far off.  Sums in fp64, E's too: in their
+// differences a token with a decay of its own would drown in the rounding of the rest.
+// PARTS: of dots and peaks, by channels.
 //
 // Measured, bf16: 8 x 1568 x 12 x 64 45 us; 20000 packed x 16 x 128 291 us, where four heads share
 // a key and 328 MB of fp32 parts are written, 64 us of it.  Two states of D x D in registers
@@ -704,9 +776,14 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
     char* PA = O + K::TILE;
     char* PD = PA + K::NP * K::PPL;
     Decays<K::C>* dec = reinterpret_cast<Decays<K::C>*>(PD + K::NP * K::PPL);
-    float* part = reinterpret_cast<float*>(dec + 2);   // DOT: [NW][C]; then E's [TT column tiles][C] and [TT row tiles][C]
-    float* e_own = part + K::NW * K::C;                // sums over the other tokens, of X rows (k, v)
-    float* e_oth = e_own + K::TT * K::C;               // and of Y rows (q, do)
+    Chunk* chunks = reinterpret_cast<Chunk*>(dec + 2);                        // DOT: by number in the slot
+    // of a chunk and the one before: E's sums over the other tokens, of X rows (k, v), [TT column tiles][C], and of Y
+    // rows (q, do), [TT row tiles][C]; k . dk by waves, [NW][C]; sum |dS| by waves
+    constexpr int EN = K::TT * K::C, PN = K::NW * K::C;
+    double* e_own = reinterpret_cast<double*>(chunks + SLOT_CHUNKS);
+    double* e_oth = e_own + 2 * EN;
+    float* part = reinterpret_cast<float*>(e_oth + 2 * EN);
+    float* weight = part + 2 * PN;
 
     int j, h, cols;
     work_of<1>(a, j, h, cols);
@@ -722,24 +799,30 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         return;
     }
     const int b = a.tab ? 0 : s.seq, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
-    constexpr int DD = K::D * K::D, LAST = K::NW - 1;
+    // dg's wave: the first one without a tile of pairs, if there is one
+    constexpr int DD = K::D * K::D, LAST = K::NW - 1, DGW = K::NT < LAST ? K::NT : LAST;
     const float* s_in = a.s_in ? a.s_in + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD : nullptr;
     State<K> sv, sk;   // dv's: [do][q]; dk's: [q][do]
     sv.load(s_in, wave, false);
     sk.load(s_in, wave, true);
+    auto dot_all = [&](const float* p) {   // <p, dS>, for all threads
+        double* sums = reinterpret_cast<double*>(lds);
+        const double x = sk.dot(p, wave);
+        if (l == 0) sums[wave] = x;
+        lds_barrier();
+        double y = 0.0;
+#pragma unroll
+        for (int k = 0; k < K::NW; ++k) y += sums[k];
+        return y;
+    };
     double passing = 0.0;   // <S, dS> behind the chunk
     if constexpr (DOT) {
         if (s_in && (!s.last || a.s_final)) {
-            const float* p = s.last ? a.s_final + ((int64_t)s.seq * a.H + h) * DD : a.starts + ((int64_t)(j + 1) * a.H + h) * DD;
-            double* sums = reinterpret_cast<double*>(lds);
-            const double x = sk.dot(p, wave);
-            if (l == 0) sums[wave] = x;
-            lds_barrier();
-#pragma unroll
-            for (int k = 0; k < K::NW; ++k) passing += sums[k];
+            passing = dot_all(s.last ? a.s_final + ((int64_t)s.seq * a.H + h) * DD : a.starts + ((int64_t)(j + 1) * a.H + h) * DD);
             lds_barrier();
         }
     }
+    float off = SUM_OFF * fabsf((float)passing);   // of it
 
     const float* g = a.g + b * a.gb + (int64_t)s.tok0 * a.gt + h * a.gh;
     Stage<K, K::D, true> rk, rq, rv, ro;
@@ -758,19 +841,18 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         const int i = i0 + l;
         gv = l < n && i > 0 && i < s.n ? g[(int64_t)(s.n - i) * a.gt] : 0.f;
     };
-    // dots and g of the chunk's tokens, in wave 0
-    float av = 0.f, gt = 0.f;
+    // dots, peaks and g of the chunk's tokens (those behind the last: of that), on their way until settle
+    float av[PARTS], top[PARTS], gt = 0.f;
     double whole = 0.0;
     auto load_a = [&](int i0, int n) {
-        const int i = i0 + l, t = s.n - 1 - i;
-        if (DOT && wave == 0) {
-            const bool in = l < n && i < s.n;
-            av = 0.f;
+        const int t = s.n - 1 - i0 - min(l, n - 1);
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-                if (in) av += a.dots[((int64_t)p * a.H + h) * a.B * a.T + (int64_t)b * a.T + s.tok0 + t];
-            gt = in ? g[(int64_t)t * a.gt] : 0.f;
+        for (int p = 0; p < PARTS; ++p) {
+            av[p] = a.dots[((int64_t)p * a.H + h) * a.B * a.T + (int64_t)b * a.T + s.tok0 + t];
+            top[p] = a.peaks[((int64_t)p * a.H + h) * chunk_count(a.B, a.T, a.nslots) +
+                             chunk_number((int64_t)b * a.T + s.tok0, j, (s.n - 1 - i0) / K::C)];
         }
+        gt = g[(int64_t)t * a.gt];
     };
     auto store = [&](int n) {
         rk.store(Kt, n);
@@ -781,10 +863,9 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
     clear_upper<K>(PA);
     clear_upper<K>(PD);
     if constexpr (DOT)
-        for (int v = threadIdx.x; v < 2 * K::TT * K::C; v += K::NTH) e_own[v] = 0.f;
+        for (int v = threadIdx.x; v < 4 * EN; v += K::NTH) e_own[v] = 0.0;
     if (s.n > 0) {
         load(0, n0);
-        load_a(0, n0);
         if (wave == LAST) {
             load_g(0, n0);
             fill_decays<K::C>(dec, gv);
@@ -794,10 +875,57 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         if (n0 < s.n) load(n0, K::C);
         lds_barrier();
     }
+    // dg of the chunk of rows [i0, i0 + n), but for what passes it: one chunk late, beside the next one's pairs
+    float all = 1.f;   // e^{sum of g over it}
+    auto settle = [&](int i0, int n, int turn) {
+        // lane l: token n - 1 - l of the chunk
+        float x = 0.f, y = 0.f, size = 0.f, peak = 0.f;
+        double cross = 0.0;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            y += av[p];
+            peak = fmaxf(peak, top[p]);
+        }
+        if (l >= n) y = 0.f;
+        if (l < n) {
+#pragma unroll
+            for (int k = 0; k < K::TT; ++k) cross += e_oth[turn * EN + k * K::C + l] - e_own[turn * EN + k * K::C + l];
+#pragma unroll
+            for (int k = 0; k < K::NW; ++k) x += part[turn * PN + k * K::C + l];
+        }
+#pragma unroll
+        for (int k = 0; k < K::NW; ++k) size += weight[turn * K::NW + k];
+        Chunk c;
+        const double pairs = prefix32(cross), enter = prefix32((double)y), before = behind32((double)x, c.leave);
+        c.enter = lane31(enter);
+        c.entered = lane(prefix32(fabsf(y)), 31);
+        c.left = lane(prefix32(fabsf(x)), 31);
+        c.most = decay(lane(gt, n - 1)) * all * (peak * size);
+        c.pass = within(passing - c.leave, c.most);
+        c.off = off + SUM_OFF * c.left;
+        if (c.most < c.off) c.off = c.most;
+        c.live = (uint32_t)__ballot(l < n && !(gt < G_MIN));
+        passing = c.pass + c.enter;
+        off = c.off + SUM_OFF * c.entered;
+        if (l == 0) chunks[(s.n - 1 - i0) / K::C] = c;
+        if (l < n) {
+            // (nothing passes a decay of zero: exactly; nor do pairs cross the chunk's first token)
+            const double v = gt < G_MIN ? 0.0 : enter + before + (l < n - 1 ? pairs : 0.0);
+            if (a.dg) a.dg[((int64_t)b * a.T + s.tok0 + s.n - 1 - i0 - l) * a.H + h] = (float)v;
+            whole += v;
+        }
+    };
     int turn = 0;
     for (int i0 = 0, n = n0; i0 < s.n; i0 += n, n = K::C, turn ^= 1) {
         const Decays<K::C>& d = dec[turn];
         const bool more = i0 + n < s.n;
+        if constexpr (DOT) {
+            if (wave == DGW) {
+                if (i0) settle(i0 == n0 ? 0 : i0 - K::C, i0 == n0 ? n0 : K::C, turn ^ 1);
+                load_a(i0, n);
+                all = d.all;
+            }
+        }
         bf16x8 wo[K::NPL], wq[K::NPL];
         w_frag<K, K::RB>(O, 0, wave, wo);
         w_frag<K, K::RB>(Q, 0, wave, wq);
@@ -813,19 +941,21 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
                 put_pair<K>(PD, pd * m, ti, si);
                 if constexpr (DOT) {
                     // a token's own pair passes no decay, and would drown what does where decays are fast
-                    f32x4 e = pa * pd;
+                    double e[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (ti == si && 4 * (l >> 4) + i == (l & 15)) e[i] = 0.f;
-                    const float own = quad_sum((e[0] + e[1]) + (e[2] + e[3]));
-                    if (l < 16) e_own[si * K::C + 16 * ti + l] = own;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x = e[i];
-#pragma unroll
-                        for (int q = 1; q < 16; q <<= 1) x += __shfl_xor(x, q, 64);
-                        if ((l & 15) == 0) e_oth[ti * K::C + 16 * si + 4 * (l >> 4) + i] = x;
-                    }
+                    for (int i = 0; i < 4; ++i) e[i] = ti == si && 4 * (l >> 4) + i == (l & 15) ? 0.0 : (double)(pa[i] * pd[i]);
+                    double own = (e[0] + e[1]) + (e[2] + e[3]);
+                    own += __shfl_xor(own, 16, 64);
+                    own += __shfl_xor(own, 32, 64);
+                    if (l < 16) e_own[turn * EN + si * K::C + 16 * ti + l] = own;
+                    // sums over 16 lanes of four numbers, which the first two steps share out
+                    const bool b0 = l & 1, b1 = l & 2;
+                    const double x = (b0 ? e[2] : e[0]) + dpp<0xb1, 0xf>(b0 ? e[0] : e[2]),   // quad_perm: the other one,
+                                 y = (b0 ? e[3] : e[1]) + dpp<0xb1, 0xf>(b0 ? e[1] : e[3]);
+                    double oth = (b1 ? y : x) + dpp<0x4e, 0xf>(b1 ? x : y);                   // and the other two
+                    oth += dpp<0x128, 0xf>(oth);                                              // row_ror:8, 4
+                    oth += dpp<0x124, 0xf>(oth);
+                    if ((l & 15) < 4) e_oth[turn * EN + ti * K::C + 16 * si + 4 * (l >> 4) + 2 * b0 + b1] = oth;
                 }
             }
         }
@@ -833,13 +963,15 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         sv.apply(Kt, d, o);
         sk.apply(V, d, o2);
         if constexpr (DOT) {
+            const float x = sk.weight();
+            if (l == 63) weight[turn * K::NW + wave] = x;
             const int ch = 16 * wave + 4 * (l >> 4);
 #pragma unroll
             for (int i = 0; i < K::TT; ++i) {
                 const int t = 16 * i + (l & 15);
                 const char* p = Kt + Sw<K::RB>::at(t, ch >> 3) + 2 * (ch & 7);
                 const float x = quad_sum(dot4(tile4<K>(p), o2[i]));
-                if (l < 16) part[wave * K::C + t] = x;
+                if (l < 16) part[turn * PN + wave * K::C + t] = x;
             }
         }
         sv.add(Q, wo, d);
@@ -848,7 +980,6 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
             fill_decays<K::C>(dec + (turn ^ 1), gv);
             load_g(i0 + n + K::C, K::C);
         }
-        const float all = d.all;
         lds_barrier();
         if (more) {
             store(K::C);
@@ -859,38 +990,46 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         add_pairs<K>(PD, wq, o2);
         put_rows<K, OT, true>(static_cast<OT*>(a.out) + out, (uint32_t)(a.H * K::D), o2, wave, n);
         put_rows<K, OT, true>(static_cast<OT*>(a.out2) + out, (uint32_t)(a.H * K::D), o, wave, n);
-        if constexpr (DOT) {
-            if (wave == 0) {
-                float x = 0.f, own = 0.f, oth = 0.f;
-                if (l < n) {
-#pragma unroll
-                    for (int k = 0; k < K::TT; ++k) {
-                        own += e_own[k * K::C + l];
-                        oth += e_oth[k * K::C + l];
-                    }
-#pragma unroll
-                    for (int k = 0; k < K::NW; ++k) x += part[k * K::C + l];
-                }
-                // lane l: token n - 1 - l of the chunk
-                const double pairs = prefix32((double)oth - (double)own), through = prefix32((double)av - (double)x);
-                if (all < ANCHOR_BELOW) passing = lane31(prefix32((double)x));
-                if (l < n) {
-                    // (nothing passes a decay of zero: exactly)
-                    const double v = gt < G_MIN ? 0.0 : (passing + through) + pairs;
-                    if (a.dg) a.dg[(row + (n - 1 - l)) * a.H + h] = (float)v;
-                    whole += v;
-                }
-                passing += lane31(through);
-                load_a(i0 + n, K::C);
-            }
-        }
         if (more) lds_barrier();
     }
     if constexpr (DOT) {
-        if (a.sums && wave == 0) {
+        const float* p = !a.starts ? nullptr : a.starts + ((int64_t)(a.in_by_slot ? j : s.seq) * a.H + h) * DD;
+        double from = 0.0;   // what passes the slot's start
+        if (p && s.n > 0) from = (double)decay(g[0]) * dot_all(p);
+        if (wave == DGW) {
+            if (s.n > 0) settle(s.n > n0 ? s.n - K::C : 0, s.n > n0 ? K::C : n0, turn ^ 1);
+            float open = SUM_OFF * fabsf((float)from);
+            double pass = 0.0;   // lane l: of chunk l
+            const int count = (s.n + K::C - 1) / K::C;
+            for (int i = 0; i < count; ++i) {
+                const Chunk c = chunks[i];
+                double x = within(from - c.enter, c.most);
+                float o = open + SUM_OFF * c.entered;
+                if (c.most < o) o = c.most;
+                from = x + c.leave;
+                open = o + SUM_OFF * c.left;
+                if (c.off <= o) x = c.pass;
+                if (l == i) {
+                    pass = x;
+                    whole += x * __popc(c.live);
+                }
+            }
+            if (a.dg) {
+                __threadfence_block();   // its other lanes' stores
+                for (int i = l; i - l < s.n; i += 64) {
+                    const double x = __shfl(pass, min(i, s.n - 1) / K::C, 64);
+                    const int k = i / K::C, n = min(K::C, s.n - k * K::C);
+                    if (i < s.n && (chunks[k].live >> (n - 1 - (i - k * K::C)) & 1)) {
+                        float* d = a.dg + ((int64_t)b * a.T + s.tok0 + i) * a.H + h;
+                        *d = (float)(*d + x);
+                    }
+                }
+            }
+            if (a.sums) {
 #pragma unroll
-            for (int m = 1; m < 64; m <<= 1) whole += __shfl_xor(whole, m, 64);
-            if (l == 0) a.sums[(int64_t)j * a.H + h] = whole;
+                for (int m = 1; m < 64; m <<= 1) whole += __shfl_xor(whole, m, 64);
+                if (l == 0) a.sums[(int64_t)j * a.H + h] = whole;
+            }
         }
     }
     if (a.s_out && s.first) sv.store(a.s_out + ((int64_t)s.seq * a.H + h) * DD, wave, s.n > 0 ? decay(g[0]) : 1.f);
@@ -1154,8 +1293,8 @@ Plan plan_of(const Args& a, bool train) {
     Plan p;
     p.packed = a.cu != nullptr;
     const int64_t rows = p.packed ? 1 : a.B, chunks = std::max<int64_t>(1, (a.T + 63) / 64);
-    // dg is a sum over a slot's tokens, whose errors add up
-    const int64_t most = train ? 32 : chunks;
+    // dg goes from chunk to chunk of a slot, whose errors add up, and has a lane for each
+    const int64_t most = train ? SLOT_CHUNKS / 2 : chunks;
     const double fit = a.D <= 64 ? 1024 : 384, fit2 = a.D <= 64 ? 768 : 256;
     // rounds of `fit` that `whole` slots and `parts` slots of a `rest` of their length take
     const auto turns = [](double whole, double parts, double rest, double fit) {
@@ -1193,7 +1332,7 @@ Plan plan_of(const Args& a, bool train) {
 // again (kept); and the backward pass' own
 struct Layout {
     int64_t tab = -1, first = -1, order = -1, s = -1, seg = -1, kept = 0;
-    int64_t ds = -1, segd = -1, dots = -1, sums = -1, g0 = -1, g1 = -1, bytes = 0;
+    int64_t ds = -1, segd = -1, dots = -1, peaks = -1, sums = -1, g0 = -1, g1 = -1, bytes = 0;
 };
 bool shared(const Args& a, const kda_decay_rows& r) { return r.heads != a.H; }
 Layout layout_of(const Args& a, const Plan& p) {
@@ -1213,6 +1352,7 @@ Layout layout_of(const Args& a, const Plan& p) {
     }
     if (a.dg) {
         l.dots = take(l.bytes, 2 * rows);   // (of two parts of the channels)
+        l.peaks = take(l.bytes, 2 * 4 * a.H * chunk_count(a.B, a.T, p.nslots));
         if (a.dg_heads) l.sums = take(l.bytes, 2 * sg);
     }
     const bool kv = shared(a, a.k) || shared(a, a.v);
@@ -1375,6 +1515,7 @@ int backward(const Args& a, hipStream_t st) {
     d.x = o; d.y = v; d.w = k; d.z = q;
     d.s_in = p.multi ? starts : a.s0;
     d.dots = dots;
+    d.peaks = part(ws, l.peaks);
     d.s_out = dends;
     d.seg = part(ws, l.segd);
     const auto scan = [&] {
@@ -1400,7 +1541,8 @@ int backward(const Args& a, hipStream_t st) {
     d.s_out = a.ds0;
     double* sums = reinterpret_cast<double*>(part(ws, l.sums));
     d.dots = dots;
-    d.starts = starts;
+    d.peaks = part(ws, l.peaks);
+    d.starts = p.multi ? starts : a.s0;
     d.s_final = a.ds_final ? a.s_final : nullptr;
     d.dg = sums ? nullptr : a.dg;
     d.sums = sums;
