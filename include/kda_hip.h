@@ -430,7 +430,8 @@ int kda_adamw_moments(const void* m, const void* v, const float* m_scale, const 
  * or with dg_heads != 0 [H], the sum over all tokens; NULL: not wanted.
  * Sums and states are fp32, and enter the products with all their bits.  What a token gets
  * from itself alone (T = 1, no s0) has a dg of exactly zero.  A value that is not finite
- * reaches every output of its sequence from its block of 32 tokens on (in a gradient: up to it).
+ * reaches what the recurrence takes it to: o and dq from its token on, dk and dv up to it; of dg
+ * all of its sequence.
  * Backward: gradients of <o, dout> + <s_final, ds_final>; reads s_final only for dg
  * beside ds_final.  kda_decay_workspace_size(pass, args): bytes, 16-byte aligned, for these
  * sizes, heads, cu, nseq, dtype, dg and dg_heads.  KDA_PASS_FWD: the forward pass' workspace;

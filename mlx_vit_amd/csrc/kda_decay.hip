@@ -334,6 +334,7 @@ __device__ __forceinline__ f32x4 pair_tile(const char* X, const char* Y, int ti,
     }
     return acc;
 }
+// their weights, and the product with them: nothing of a later token, whatever it is
 template <class K>
 __device__ __forceinline__ f32x4 mask_tile(const Decays<K::C>& d, int ti, int si) {
     const int l = lane_id(), t = 16 * ti + (l & 15), s0 = 16 * si + 4 * (l >> 4);
@@ -342,8 +343,14 @@ __device__ __forceinline__ f32x4 mask_tile(const Decays<K::C>& d, int ti, int si
     const float hv[4] = {hs.x, hs.y, hs.z, hs.w}, lv[4] = {ls.x, ls.y, ls.z, ls.w};
     f32x4 m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = s0 + i <= t ? __builtin_amdgcn_exp2f((h - hv[i]) + (o - lv[i])) : 0.f;
+    for (int i = 0; i < 4; ++i) m[i] = __builtin_amdgcn_exp2f((h - hv[i]) + (o - lv[i]));
     return m;
+}
+__device__ __forceinline__ f32x4 masked(const f32x4& p, const f32x4& m, int ti, int si) {
+    f32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = ti == si && 4 * (lane_id() >> 4) + i > (lane_id() & 15) ? 0.f : p[i] * m[i];
+    return x;
 }
 // a tile into P[t][s]
 template <class K>
@@ -481,14 +488,49 @@ struct State {
     }
 };
 
-// o_t += sum_s P[t][s] W_s, layout as State::apply
+// o_t += sum_s P[t][s] W_s, layout as State::apply.  A value of W that is not finite would reach
+// the rows before its own too, whose weights are zero: there, seldom, it is taken out of the
+// product and put into its channel's rows from its own on.
 template <class K>
-__device__ __forceinline__ void add_pairs(const char* P, const bf16x8 (&w)[K::NPL], f32x4 (&o)[K::TT]) {
+__device__ __forceinline__ void add_pairs(const char* P, bf16x8 (&w)[K::NPL], f32x4 (&o)[K::TT]) {
+    uint4 u = __builtin_bit_cast(uint4, w[0]);   // (the first plane has the exponent)
+    // bit 15 of a half whose exponent is all ones, carried there
+    const auto ends = [](uint32_t x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
+    const bool bad = __any((int)(ends(u.x) | ends(u.y) | ends(u.z) | ends(u.w)));
+    int first = K::C;   // of this lane's channel of W, the first such row
+    if (bad) {
+        const int l = lane_id();
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 7; e >= 0; --e)
+            if (ends(x[e >> 1]) & (e & 1 ? 0x80000000u : 0x8000u)) first = 8 * (l >> 4) + e;
+        first = min(first, __shfl_xor(first, 16, 64));
+        first = min(first, __shfl_xor(first, 32, 64));
+#pragma unroll
+        for (int p = 0; p < K::NPL; ++p) {
+            uint4 v = __builtin_bit_cast(uint4, w[p]);
+            uint32_t y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (8 * (l >> 4) + e >= first) y[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+            w[p] = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
+        }
+    }
 #pragma unroll
     for (int i = 0; i < K::TT; ++i) {
         bf16x8 p[K::NP];
         along<K::RP, K::NP, K::PPL>(P, 16 * i, 0, p);
         o[i] = mmp(w, p, o[i]);
+    }
+    if (bad) {
+        const int l = lane_id();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int row = __shfl(first, 4 * (l >> 4) + c, 64);
+#pragma unroll
+            for (int i = 0; i < K::TT; ++i)
+                if (16 * i + (l & 15) >= row) o[i][c] = __builtin_nanf("");
+        }
     }
 }
 
@@ -652,9 +694,7 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
                 if (id < K::NT) {
                     int ti, si;
                     tile_of(id, ti, si);
-                    f32x4 p = pair_tile<K>(X, Y, ti, si);
-                    p *= mask_tile<K>(d, ti, si);
-                    put_pair<K>(P, p, ti, si);
+                    put_pair<K>(P, masked(pair_tile<K>(X, Y, ti, si), mask_tile<K>(d, ti, si), ti, si), ti, si);
                 }
             }
             st.apply(X, d, o);
@@ -936,14 +976,14 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
                 int ti, si;
                 tile_of(id, ti, si);
                 const f32x4 m = mask_tile<K>(d, ti, si);
-                const f32x4 pa = pair_tile<K>(Kt, Q, ti, si) * m, pd = pair_tile<K>(V, O, ti, si);
+                const f32x4 pa = masked(pair_tile<K>(Kt, Q, ti, si), m, ti, si), pd = pair_tile<K>(V, O, ti, si);
                 put_pair<K>(PA, pa, ti, si);
-                put_pair<K>(PD, pd * m, ti, si);
+                put_pair<K>(PD, masked(pd, m, ti, si), ti, si);
                 if constexpr (DOT) {
                     // a token's own pair passes no decay, and would drown what does where decays are fast
                     double e[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[i] = ti == si && 4 * (l >> 4) + i == (l & 15) ? 0.0 : (double)(pa[i] * pd[i]);
+                    for (int i = 0; i < 4; ++i) e[i] = ti == si && 4 * (l >> 4) + i >= (l & 15) ? 0.0 : (double)(pa[i] * pd[i]);
                     double own = (e[0] + e[1]) + (e[2] + e[3]);
                     own += __shfl_xor(own, 16, 64);
                     own += __shfl_xor(own, 32, 64);

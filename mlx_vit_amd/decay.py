@@ -217,8 +217,8 @@ def chunk_decay(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
 
     q, k, v (B, T, heads, D), bf16 or fp32, D 32, 64, 96 or 128, any strides (rows that
     are not whole 16-byte pieces are copied first).  g (B, T, H) or (H,), fp32 or bf16;
-    g = -inf starts the state anew, and so does everything below -200.  A
-    value that is not finite reaches all outputs of its sequence from its 32 tokens on.
+    g = -inf starts the state anew, and so does everything below -200.  A value that is not
+    finite reaches the outputs of its sequence from its token on, and all of its dg.
 
     ``cu_seqlens`` (N + 1,) int32 on the same device: token cu[i] to cu[i + 1] - 1 of the one
     row (B = 1) are sequence i; states are then (N, H, D, D).  The limits are read on the
