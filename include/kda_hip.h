@@ -477,10 +477,10 @@ int kda_decay_step(const kda_decay_args* args, const int32_t* slots, int64_t sta
  * position_a 2 pi turns[...], the pairs numbered through all axes; channels behind
  * the last axis are copied.  Pairs of an axis: (i, sections[a] / 2 + i), or with
  * interleaved (2 i, 2 i + 1).  Angles are formed in fp64, rows in fp32.  turns: host memory,
- * one for every pair.  Positions: of type 0 int32, 1 int64 or 2 fp32 with strides (axis,
- * batch, token), or NULL: axes 0 to 2 are n / (grid_h grid_w), n / grid_w mod grid_h and n mod
- * grid_w of n = start + token.  q and k (k.p NULL: none): as kda_decay's operands, of any alignment
- * to their element; q_out, k_out contiguous [B][T][heads][D]. */
+ * one for every pair (NULL where there is none).  Positions: of type 0 int32, 1 int64 or 2 fp32
+ * with strides (axis, batch, token), or NULL: axes 0 to 2 are n / (grid_h grid_w), n / grid_w mod
+ * grid_h and n mod grid_w of n = start + token.  q and k (k.p NULL: none): as kda_decay's operands, of
+ * any alignment to their element; q_out, k_out contiguous [B][T][heads][D]. */
 #define KDA_ROTARY_AXES 4
 typedef struct kda_rotary_args {
     kda_decay_rows q, k;

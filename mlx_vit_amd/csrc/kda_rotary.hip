@@ -189,7 +189,6 @@ extern "C" int kda_rotary(const kda_rotary_args* args, void* stream) {
         return api_fail(KDA_E_INVALID, "grid %lld x %lld from %lld, and no positions", (long long)r.grid_h, (long long)r.grid_w,
                         (long long)r.start);
     if (r.positions && (r.type < 0 || r.type > 2)) return api_fail(KDA_E_UNSUPPORTED, "type=%lld: expected 0, 1 or 2", (long long)r.type);
-    if (!r.turns) return api_fail(KDA_E_INVALID, "turns is NULL");
     RotaryArgs a = {};
     const int es = r.dtype == KDA_DTYPE_BF16 ? 2 : 4, halves = !r.interleaved;
     // the widest pieces that every operand and section is made of
@@ -203,6 +202,7 @@ extern "C" int kda_rotary(const kda_rotary_args* args, void* stream) {
         a.ends[x] = at / 2;
         if (halves) fits(r.sections[x] / 2);
     }
+    if (at && !r.turns) return api_fail(KDA_E_INVALID, "turns is NULL");
     fits(halves ? (r.D - at) / 2 : r.D);
     const kda_decay_rows* in[2] = {&r.q, &r.k};
     void* out[2] = {r.q_out, r.k_out};
