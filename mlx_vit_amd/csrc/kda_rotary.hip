@@ -52,9 +52,9 @@ __device__ __forceinline__ ST of_f(float x) {
     else return f2bf(x);
 }
 
-// (x, y) turned.  No angle: copied, whatever the other one is.
+// (x, y) turned.  No angle: copied, whatever the other one is, and a zero with its sign.
 __device__ __forceinline__ void turned(float& x, float& y, float c, float s) {
-    const float u = fmaf(x, c, s == 0.f ? 0.f : -(y * s)), v = fmaf(y, c, s == 0.f ? 0.f : x * s);
+    const float u = s == 0.f ? x * c : fmaf(x, c, -(y * s)), v = s == 0.f ? y * c : fmaf(y, c, x * s);
     x = u;
     y = v;
 }

@@ -21,3 +21,13 @@ def test_no_channels_turn(sections, interleaved, dt):
         y, z = rotary(q, k, sections=sections, interleaved=interleaved, **where)
         d, = torch.autograd.grad(y, q, y)
         assert torch.equal(y, q) and torch.equal(z, k) and torch.equal(d, y)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_channels_behind_the_axes_keep_their_bits(interleaved, dt):
+    """A zero's sign among them."""
+    q = torch.randn(1, 5, 2, 64, device=DEV).to(dt)
+    q[..., 33:50:3], q[..., 34:50:3] = -0.0, 0.0
+    y = rotary(q, grid=(2, 2), start=9, sections=(16, 8, 8), interleaved=interleaved)
+    assert torch.equal(y[..., 32:].contiguous().view(BITS[dt]), q[..., 32:].contiguous().view(BITS[dt]))
