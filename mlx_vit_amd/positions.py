@@ -17,6 +17,7 @@ from __future__ import annotations
 import math
 from array import array
 from functools import lru_cache
+from operator import index
 from struct import Struct
 from typing import Optional, Sequence, Tuple, Union
 
@@ -36,13 +37,20 @@ _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 def _axes(D: int, sections, base: float) -> Tuple[int, Tuple[int, ...], array]:
     """Validated: how many axes, their sections filled up with zeros, and turns a unit of position of
     every pair, base^(-2 i / section) / 2 pi."""
-    given, sections = sections, (D,) if sections is None else tuple(int(s) for s in sections)
+    given, sections = sections, (D,) if sections is None else sections
     if not 1 <= len(sections) <= MAX_AXES or any(s < 0 or s % 2 for s in sections) or sum(sections) > D:
         raise ValueError(f"rotary: sections={given}: expected 1 to {MAX_AXES} even numbers that make up at most {D}")
     if not 0.0 < base < math.inf:
         raise ValueError(f"rotary: base={base}: expected a positive number")
     turns = array("d", [base ** (-2 * i / s) / (2 * math.pi) for s in sections for i in range(s // 2)])
     return len(sections), sections + (0,) * (MAX_AXES - len(sections)), turns
+
+
+def _whole(sections) -> Optional[Tuple[int, ...]]:
+    try:
+        return sections if sections is None else tuple(map(index, sections))
+    except TypeError:
+        raise ValueError(f"rotary: sections={sections}: expected 1 to {MAX_AXES} even numbers") from None
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
@@ -131,19 +139,20 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optiona
             raise ValueError(f"{what}: k has dtype {k.dtype}; expected {q.dtype}")
         if k.device != dev:
             raise ValueError(f"{what}: k is on {k.device}, q on {dev}")
-    how = _axes(D, sections if sections is None or type(sections) is tuple else tuple(sections), float(base))
+    how = _axes(D, _whole(sections), float(base))
     n = how[0]
     if (positions is None) == (grid is None):
         raise ValueError(f"{what}: expected either positions or grid")
     if grid is not None:
         try:
             h, w = grid
+            h, w, first = index(h), index(w), index(start)
         except (TypeError, ValueError):
-            raise ValueError(f"{what}: grid={grid}: expected (height, width)") from None
-        if not (1 <= h < 1 << 31 and 1 <= w < 1 << 31 and n <= 3 and 0 <= start < 1 << 62):
+            raise ValueError(f"{what}: grid={grid}, start={start}: expected (height, width) and a number, whole numbers") from None
+        if not (1 <= h < 1 << 31 and 1 <= w < 1 << 31 and n <= 3 and 0 <= first < 1 << 62):
             raise ValueError(f"{what}: grid={grid}, start={start} with {n} sections: expected (height, width), "
                              "start >= 0 and at most 3 axes")
-        where = (0, 0, 0, 0, int(h), int(w), int(start))
+        where = (0, 0, 0, 0, h, w, first)
     else:
         if not isinstance(positions, torch.Tensor):
             raise TypeError("rotary: positions must be a torch.Tensor")
