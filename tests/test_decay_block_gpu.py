@@ -39,3 +39,40 @@ def test_blocks_without_positions_leave_start():
         block = HybridBlock(64, 2, kind).cuda().eval()
         with torch.no_grad():
             assert all(torch.equal(a, b) if a is not None else b is None for a, b in zip(block(x, **kw), block(x, start=5, **kw)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("time_only", [False, True])
+def test_block_against_64_bits(time_only):
+    """The whole block, and of a scan over time alone each location's own sequence, with its gradients: 2e-4 of the
+    largest, the layer's 1e-4 and as much for the norms and the MLP."""
+    from test_decay_layer_gpu import plain
+    torch.manual_seed(0)
+    block = HybridBlock(48, 2, "decay", 32, spatial_tokens=6 if time_only else None, gdn_temporal_only=time_only, grid=(2, 3)).cuda()
+    x = torch.randn(2, 30, 48, device="cuda", requires_grad=True)
+    y, _ = block(x)
+    dy = torch.randn_like(y)
+    names = ["x", *(n for n, _ in block.named_parameters())]
+    got = [y, *torch.autograd.grad(y, [x, *block.parameters()], dy)]
+    p = {n: t.detach().double().requires_grad_(True) for n, t in block.named_parameters()}
+    wx = x.detach().double().requires_grad_(True)
+    n1 = torch.nn.functional.layer_norm(wx, (48,), p["norm1.weight"], p["norm1.bias"], 1e-6)
+    rows = n1.reshape(2, 5, 6, 48).transpose(1, 2).reshape(12, 5, 48) if time_only else n1
+    # (the layer in 64 bits has leaves of its own: its gradients are asked for with what reaches its output)
+    ly, _, lx, lp = plain(block.layer, rows.detach())
+    at = ly.detach().requires_grad_(True)
+    mixed = at.reshape(2, 6, 5, 48).transpose(1, 2).reshape(2, 30, 48) if time_only else at
+    h = wx + mixed
+    n2 = torch.nn.functional.layer_norm(h, (48,), p["norm2.weight"], p["norm2.bias"], 1e-6)
+    mlp = block.mlp
+    ps = [p["mlp." + n] for n, _ in mlp.named_parameters()]
+    f = torch.nn.functional
+    wy = h + f.linear(f.gelu(f.linear(n2, ps[0], ps[1])), ps[2], ps[3])
+    leaves = [wx, at, p["norm2.weight"], p["norm2.bias"], *ps]
+    gx, ga, g2w, g2b, *gp = torch.autograd.grad(wy, leaves, dy.double(), retain_graph=True)
+    gl = torch.autograd.grad(ly, [lx, *lp.values()], ga)
+    more = torch.autograd.grad(rows, [wx, p["norm1.weight"], p["norm1.bias"]], gl[0])
+    want = {"x": gx + more[0], "norm1.weight": more[1], "norm1.bias": more[2], "norm2.weight": g2w, "norm2.bias": g2b,
+            **{"layer." + n: t for n, t in zip(lp, gl[1:])}, **{"mlp." + n: t for (n, _), t in zip(mlp.named_parameters(), gp)}}
+    for name, a, b in zip(["y", *names], got, [wy, *(want[n] for n in names)]):
+        assert float((a.double() - b).abs().max()) <= 2e-4 * float(b.abs().max()), name
