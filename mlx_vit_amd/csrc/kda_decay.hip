@@ -493,14 +493,21 @@ struct State {
 // product and put into its channel's rows from its own on.
 template <class K>
 __device__ __forceinline__ void add_pairs(const char* P, bf16x8 (&w)[K::NPL], f32x4 (&o)[K::TT]) {
-    uint4 u = __builtin_bit_cast(uint4, w[0]);   // (the first plane has the exponent)
+    const uint4 u = __builtin_bit_cast(uint4, w[0]);   // (the first plane has the exponent)
     // bit 15 of a half whose exponent is all ones, carried there
     const auto ends = [](uint32_t x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
-    const bool bad = __any((int)(ends(u.x) | ends(u.y) | ends(u.z) | ends(u.w)));
-    int first = K::C;   // of this lane's channel of W, the first such row
-    if (bad) {
+    const auto product = [&] {
+#pragma unroll
+        for (int i = 0; i < K::TT; ++i) {
+            bf16x8 p[K::NP];
+            along<K::RP, K::NP, K::PPL>(P, 16 * i, 0, p);
+            o[i] = mmp(w, p, o[i]);
+        }
+    };
+    if (__builtin_expect(__any((int)(ends(u.x) | ends(u.y) | ends(u.z) | ends(u.w))), 0)) {
         const int l = lane_id();
         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        int first = K::C;   // of this lane's channel of W, the first such row
 #pragma unroll
         for (int e = 7; e >= 0; --e)
             if (ends(x[e >> 1]) & (e & 1 ? 0x80000000u : 0x8000u)) first = 8 * (l >> 4) + e;
@@ -508,22 +515,14 @@ __device__ __forceinline__ void add_pairs(const char* P, bf16x8 (&w)[K::NPL], f3
         first = min(first, __shfl_xor(first, 32, 64));
 #pragma unroll
         for (int p = 0; p < K::NPL; ++p) {
-            uint4 v = __builtin_bit_cast(uint4, w[p]);
+            const uint4 v = __builtin_bit_cast(uint4, w[p]);
             uint32_t y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (8 * (l >> 4) + e >= first) y[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
             w[p] = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
         }
-    }
-#pragma unroll
-    for (int i = 0; i < K::TT; ++i) {
-        bf16x8 p[K::NP];
-        along<K::RP, K::NP, K::PPL>(P, 16 * i, 0, p);
-        o[i] = mmp(w, p, o[i]);
-    }
-    if (bad) {
-        const int l = lane_id();
+        product();
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int row = __shfl(first, 4 * (l >> 4) + c, 64);
@@ -531,6 +530,8 @@ __device__ __forceinline__ void add_pairs(const char* P, bf16x8 (&w)[K::NPL], f3
             for (int i = 0; i < K::TT; ++i)
                 if (16 * i + (l & 15) >= row) o[i][c] = __builtin_nanf("");
         }
+    } else {
+        product();
     }
 }
 
