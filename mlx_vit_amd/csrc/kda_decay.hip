@@ -156,7 +156,8 @@ struct Sw {
 // one plane, fp32 ones three, and so are the pairs' weights and the state as factors (NP): with two,
 // 16 bits, one bf16 output in 450 is rounded the other way, so one in 6000 to 18000, for 1 to 3%
 // of the time (65536 x 12 x 64 153.1 -> 154.7 us, 20000 packed x 16 x 128 forward and backward 726 -> 747).
-// OCC, OCC2: waves a SIMD that mix and mix2 are held to.
+// OCC, OCC2: waves a SIMD that mix and mix2 are held to (fp32, D = 64: mix2 takes registers for
+// one where it is let, and the training call 254 us instead of 220, 8 x 1568 x 12).
 template <int D_, bool F32_, int SPLIT_ = 1, int C_ = 32>
 struct Cfg {
     static constexpr int D = D_, C = C_, SPLIT = SPLIT_, DW = D / SPLIT, NPL = F32_ ? 3 : 1, NP = 3, NW = DW / 16, NTH = 64 * NW;
@@ -164,7 +165,7 @@ struct Cfg {
     static constexpr int RBW = (2 * DW + 63) / 64 * 64, PLANEW = C * RBW, TILEW = NPL * PLANEW;   // of DW channels
     static constexpr int RP = 2 * C, PPL = C * RP;                                             // of the pairs'
     static constexpr int TT = C / 16, NT = TT * (TT + 1) / 2, DT = D / 16, KD = D / 32, KC = C / 32;
-    static constexpr int OCC = F32_ ? 1 : D > 64 ? 3 : 4, OCC2 = F32_ ? 1 : D > 64 ? 2 : 3;
+    static constexpr int OCC = F32_ ? 1 : D > 64 ? 3 : 4, OCC2 = F32_ ? (D > 32 ? 2 : 1) : D > 64 ? 2 : 3;
     static constexpr bool F32 = F32_, WITH_DS = D <= 64;
     typedef typename std::conditional<F32_, float, uint16_t>::type ST;
     static constexpr int ES = (int)sizeof(ST), EPV = 16 / ES;
@@ -488,50 +489,69 @@ struct State {
     }
 };
 
-// o_t += sum_s P[t][s] W_s, layout as State::apply.  A value of W that is not finite would reach
-// the rows before its own too, whose weights are zero: there, seldom, it is taken out of the
-// product and put into its channel's rows from its own on.
+// A value of W that is not finite would reach the rows before its own too, whose weights are zero:
+// seldom, so all of it lies behind a branch, it is taken out of W (w: w_frag) ...
+struct Ends {
+    bool any;    // in the wave's channels
+    int first;   // the first such row of this lane's (C: none)
+};
 template <class K>
-__device__ __forceinline__ void add_pairs(const char* P, bf16x8 (&w)[K::NPL], f32x4 (&o)[K::TT]) {
+__device__ __forceinline__ Ends take_ends(bf16x8 (&w)[K::NPL]) {
     const uint4 u = __builtin_bit_cast(uint4, w[0]);   // (the first plane has the exponent)
     // bit 15 of a half whose exponent is all ones, carried there
     const auto ends = [](uint32_t x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
-    const auto product = [&] {
-#pragma unroll
-        for (int i = 0; i < K::TT; ++i) {
-            bf16x8 p[K::NP];
-            along<K::RP, K::NP, K::PPL>(P, 16 * i, 0, p);
-            o[i] = mmp(w, p, o[i]);
-        }
-    };
-    if (__builtin_expect(__any((int)(ends(u.x) | ends(u.y) | ends(u.z) | ends(u.w))), 0)) {
-        const int l = lane_id();
+    Ends r = {(bool)__any((int)(ends(u.x) | ends(u.y) | ends(u.z) | ends(u.w))), K::C};
+    if (__builtin_expect(r.any, 0)) {
+        const int row = 8 * (lane_id() >> 4);
         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-        int first = K::C;   // of this lane's channel of W, the first such row
 #pragma unroll
         for (int e = 7; e >= 0; --e)
-            if (ends(x[e >> 1]) & (e & 1 ? 0x80000000u : 0x8000u)) first = 8 * (l >> 4) + e;
-        first = min(first, __shfl_xor(first, 16, 64));
-        first = min(first, __shfl_xor(first, 32, 64));
+            if (ends(x[e >> 1]) & (e & 1 ? 0x80000000u : 0x8000u)) r.first = row + e;
+        r.first = min(r.first, __shfl_xor(r.first, 16, 64));
+        r.first = min(r.first, __shfl_xor(r.first, 32, 64));
 #pragma unroll
         for (int p = 0; p < K::NPL; ++p) {
             const uint4 v = __builtin_bit_cast(uint4, w[p]);
             uint32_t y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (8 * (l >> 4) + e >= first) y[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+                if (row + e >= r.first) y[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
             w[p] = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
         }
-        product();
+    }
+    return r;
+}
+// ... and put into its channel of the state behind the chunk, and of the rows from its own on
+template <class K>
+__device__ __forceinline__ void put_ends(const Ends& r, State<K>& s) {
+    if (__builtin_expect(r.any, 0) && r.first < K::C)
+#pragma unroll
+        for (int j = 0; j < K::DT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s.s[j][i] = __builtin_nanf("");
+}
+template <class K>
+__device__ __forceinline__ void put_ends(const Ends& r, f32x4 (&o)[K::TT]) {
+    if (__builtin_expect(r.any, 0)) {
+        const int l = lane_id();
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const int row = __shfl(first, 4 * (l >> 4) + c, 64);
+            const int row = __shfl(r.first, 4 * (l >> 4) + c, 64);
 #pragma unroll
             for (int i = 0; i < K::TT; ++i)
                 if (16 * i + (l & 15) >= row) o[i][c] = __builtin_nanf("");
         }
-    } else {
-        product();
+    }
+}
+
+// o_t += sum_s P[t][s] W_s, layout as State::apply
+template <class K>
+__device__ __forceinline__ void add_pairs(const char* P, const bf16x8 (&w)[K::NPL], f32x4 (&o)[K::TT]) {
+#pragma unroll
+    for (int i = 0; i < K::TT; ++i) {
+        bf16x8 p[K::NP];
+        along<K::RP, K::NP, K::PPL>(P, 16 * i, 0, p);
+        o[i] = mmp(w, p, o[i]);
     }
 }
 
@@ -681,6 +701,8 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
         bf16x8 w[K::NPL];
         f32x4 o[K::TT];
         w_frag<K, K::RBW>(W, 0, wave, w);
+        Ends ends;
+        if constexpr (!STATES) ends = take_ends<K>(w);
         const int ch = 16 * wv + 4 * (l >> 4);
         float4 z[DOT && !DS ? K::TT : 1];
         if constexpr (DOT && !DS) {
@@ -716,6 +738,7 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
             before *= d.all;
         } else {
             st.add(Y, w, d);
+            if constexpr (!STATES) put_ends<K>(ends, st);
         }
         if constexpr (DS) {
             if (adjoint) {
@@ -737,6 +760,7 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
         if constexpr (!STATES) {
             const int64_t row = (int64_t)b * a.T + s.tok0 + i0;
             add_pairs<K>(P, w, o);
+            put_ends<K>(ends, o);
             put_rows<K, OT, false>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, wv, n);
             if constexpr (DOT) {
                 const int t = threadIdx.x;
@@ -970,6 +994,7 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         bf16x8 wo[K::NPL], wq[K::NPL];
         w_frag<K, K::RB>(O, 0, wave, wo);
         w_frag<K, K::RB>(Q, 0, wave, wq);
+        const Ends ends_o = take_ends<K>(wo), ends_q = take_ends<K>(wq);
 #pragma unroll
         for (int k = 0; k < (K::NT + K::NW - 1) / K::NW; ++k) {
             const int id = wave + K::NW * k;
@@ -1017,6 +1042,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         }
         sv.add(Q, wo, d);
         sk.add(O, wq, d);
+        put_ends<K>(ends_o, sv);
+        put_ends<K>(ends_q, sk);
         if (wave == LAST && more) {
             fill_decays<K::C>(dec + (turn ^ 1), gv);
             load_g(i0 + n + K::C, K::C);
@@ -1029,6 +1056,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
         const int64_t row = (int64_t)b * a.T + s.tok0 + s.n - i0 - n, out = (row * a.H + h) * K::D;
         add_pairs<K>(PA, wo, o);
         add_pairs<K>(PD, wq, o2);
+        put_ends<K>(ends_o, o);
+        put_ends<K>(ends_q, o2);
         put_rows<K, OT, true>(static_cast<OT*>(a.out) + out, (uint32_t)(a.H * K::D), o2, wave, n);
         put_rows<K, OT, true>(static_cast<OT*>(a.out2) + out, (uint32_t)(a.H * K::D), o, wave, n);
         if (more) lds_barrier();
