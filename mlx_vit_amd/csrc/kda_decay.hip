@@ -438,12 +438,8 @@ struct State {
         x = prefix32(x);
         return x + dpp<0x143, 0xc>(x);
     }
-    // S <- all S + Y^T (down W): the chunk's sum from zero, so that what the matrix unit
-    // loses (it rounds sums downwards) does not add up over the chunks.  w: w_frag of W.
-    __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::NPL], const Decays<K::C>& d) {
-        add(Y, w, d.down, d.all, 1.f);
-    }
-    // S <- own S + all Y^T (weights W)
+    // S <- own S + all Y^T (weights W): the chunk's sum from zero, so that what the matrix unit loses
+    // (it rounds sums downwards) does not add up over the chunks.  w: w_frag of W.
     __device__ __forceinline__ void add(const char* Y, const bf16x8 (&w)[K::NPL], const float* weights, float own, float all) {
         static_assert(K::KC == 1, "one step of the contracted index");
         const int r = lane_id() >> 4;
@@ -521,15 +517,13 @@ __device__ __forceinline__ Ends take_ends(bf16x8 (&w)[K::NPL]) {
     }
     return r;
 }
-// ... and put into its channel of the state behind the chunk, and of the rows from its own on
+// ... and put into its channel of the state behind the chunk, as its decay (no branch: the compiler may
+// move what reads a matrix product behind one and then leave out the wait for it), ...
 template <class K>
-__device__ __forceinline__ void put_ends(const Ends& r, State<K>& s) {
-    if (__builtin_expect(r.any, 0) && r.first < K::C)
-#pragma unroll
-        for (int j = 0; j < K::DT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s.s[j][i] = __builtin_nanf("");
+__device__ __forceinline__ float own_of(const Ends& r, float own) {
+    return r.first < K::C ? __builtin_nanf("") : own;
 }
+// ... and of the rows from its own on, before the pairs' part is added
 template <class K>
 __device__ __forceinline__ void put_ends(const Ends& r, f32x4 (&o)[K::TT]) {
     if (__builtin_expect(r.any, 0)) {
@@ -737,8 +731,7 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
             st.add(Y, w, d.up, 1.f, before);
             before *= d.all;
         } else {
-            st.add(Y, w, d);
-            if constexpr (!STATES) put_ends<K>(ends, st);
+            st.add(Y, w, d.down, STATES ? d.all : own_of<K>(ends, d.all), 1.f);
         }
         if constexpr (DS) {
             if (adjoint) {
@@ -759,8 +752,8 @@ __global__ __launch_bounds__(K::NTH, GRAD && !STATES && K::WITH_DS ? K::OCC2 : K
         }
         if constexpr (!STATES) {
             const int64_t row = (int64_t)b * a.T + s.tok0 + i0;
-            add_pairs<K>(P, w, o);
             put_ends<K>(ends, o);
+            add_pairs<K>(P, w, o);
             put_rows<K, OT, false>(static_cast<OT*>(a.out) + (row * a.H + h) * K::D, (uint32_t)(a.H * K::D), o, wv, n);
             if constexpr (DOT) {
                 const int t = threadIdx.x;
@@ -1040,10 +1033,8 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
                 if (l < 16) part[turn * PN + wave * K::C + t] = x;
             }
         }
-        sv.add(Q, wo, d);
-        sk.add(O, wq, d);
-        put_ends<K>(ends_o, sv);
-        put_ends<K>(ends_q, sk);
+        sv.add(Q, wo, d.down, own_of<K>(ends_o, d.all), 1.f);
+        sk.add(O, wq, d.down, own_of<K>(ends_q, d.all), 1.f);
         if (wave == LAST && more) {
             fill_decays<K::C>(dec + (turn ^ 1), gv);
             load_g(i0 + n + K::C, K::C);
@@ -1054,10 +1045,10 @@ __global__ __launch_bounds__(K::NTH, K::OCC2) void kda_decay_mix2_kernel(const D
             if (i0 + n + K::C < s.n) load(i0 + n + K::C, K::C);
         }
         const int64_t row = (int64_t)b * a.T + s.tok0 + s.n - i0 - n, out = (row * a.H + h) * K::D;
-        add_pairs<K>(PA, wo, o);
-        add_pairs<K>(PD, wq, o2);
         put_ends<K>(ends_o, o);
         put_ends<K>(ends_q, o2);
+        add_pairs<K>(PA, wo, o);
+        add_pairs<K>(PD, wq, o2);
         put_rows<K, OT, true>(static_cast<OT*>(a.out) + out, (uint32_t)(a.H * K::D), o2, wave, n);
         put_rows<K, OT, true>(static_cast<OT*>(a.out2) + out, (uint32_t)(a.H * K::D), o, wave, n);
         if (more) lds_barrier();

@@ -65,3 +65,18 @@ def test_padding_may_hold_anything(dt):
     with torch.no_grad():
         a, b = (chunk_decay(*(t[n] for n in NAMES)) for t in (x, y))
     assert torch.equal(a[0][0], b[0][0]) and torch.equal(a[0][1, :77], b[0][1, :77]) and torch.equal(a[1][0], b[1][0])
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("g_too", [True, False])
+def test_the_same_bits(g_too, D, dt):
+    """Twenty calls on the same inputs, of several slots and chunks, with and without dg."""
+    x = inputs(2, 333, 3, D, dt, state=True, seed=D)
+    first = None
+    for _ in range(20):
+        leaves = [x[n].detach().requires_grad_(g_too or n != "g") for n in NAMES]
+        o, s = chunk_decay(*leaves)
+        out = [o, s, *torch.autograd.grad((o, s), [t for t in leaves if t.requires_grad], (x["do"], x["ds"]))]
+        first = first or out
+        assert all(torch.equal(a, b) for a, b in zip(first, out))
