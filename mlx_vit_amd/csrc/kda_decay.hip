@@ -80,11 +80,11 @@ __device__ __forceinline__ Slot slot_of(const DecayArgs& a, int j) {
 __device__ __forceinline__ int64_t chunk_number(int64_t tok, int j, int c) { return tok / 32 + j + c; }
 __host__ __device__ __forceinline__ int64_t chunk_count(int64_t B, int64_t T, int64_t nslots) { return B * T / 32 + nslots + 1; }
 // The slot, head and part of the columns of a workgroup.  Workgroups go to the 8 XCDs in
-// turn: neighbours, which read the same tokens' keys, are put into one XCD's cache; of
-// packed sequences, whose slots differ in length, only the parts of one slot and head are,
-// so that each XCD begins with whole slots and ends with short ones (20000 in 10 sequences x
-// 16 x 128, forward and backward: 806 us in the slots' own order, 779 so, 727 with lengths
-// chosen for it).
+// turn: neighbours, which read the same tokens' keys, are put into one XCD's cache where the grid is
+// a multiple of 8 (else they stay as they come); of packed sequences, whose slots differ in
+// length, only the parts of one slot and head are, for any grid, so that each XCD begins with whole
+// slots and ends with short ones (20000 in 10 sequences x 16 x 128, forward and backward, when it was
+// chosen: 806 us in the slots' own order, 779 so, 727 with lengths chosen for it).
 template <int SPLIT>
 __device__ __forceinline__ void work_of(const DecayArgs& a, int& j, int& h, int& cols) {
     int at;
@@ -152,7 +152,7 @@ struct Sw {
 // C tokens a chunk; a wave has 16 of W's channels (32, which halves the LDS reads, took
 // 190 us instead of 175 over 65536 x 12 x 64: too few waves), a workgroup a SPLIT-th of
 // them: the pairs are then formed SPLIT times, but by waves that would wait for them (20000
-// packed x 16 x 128: 115 instead of 128 us forward, dq 147 instead of 185).  bf16 operands are
+// packed x 16 x 128, when it was chosen: 115 instead of 128 us forward, dq 147 instead of 185).  bf16 operands are
 // one plane, fp32 ones three, and so are the pairs' weights and the state as factors (NP): with two,
 // 16 bits, one bf16 output in 450 is rounded the other way, so one in 6000 to 18000, for 1 to 3%
 // of the time (65536 x 12 x 64 153.1 -> 154.7 us, 20000 packed x 16 x 128 forward and backward 726 -> 747).
@@ -605,8 +605,8 @@ __device__ __forceinline__ float4 tile4(const char* p) {
 
 // mix: out = the operator over a slot's tokens.  STATES: only what the slot adds to the state,
 // and its whole decay.  GRAD: out is dq, z is q, and the slots' s_out and seg take what they
-// add to dS as well, sum of e^{G_t} do_t q_t^T (WITH_DS: 8 x 1568 x 12 x 64 34 us, by a pass of its
-// own 27 + 15; at D = 128 that leaves registers for two waves a SIMD instead of three, 213 us of
+// add to dS as well, sum of e^{G_t} do_t q_t^T (WITH_DS, when it was chosen: 8 x 1568 x 12 x 64 34 us, by a pass
+// of its own 27 + 15; at D = 128 that leaves registers for two waves a SIMD instead of three, 213 us of
 // 20000 packed x 16, by itself 148 + 64); STATES and GRAD: dS alone.  DOT: dots[t] = q_t . (the
 // part of out_t that comes from the state before the chunk), by parts of the channels.
 //
@@ -615,9 +615,9 @@ __device__ __forceinline__ float4 tile4(const char* p) {
 // flight for a whole chunk.  The last wave, which has the fewest pairs, forms the next
 // chunk's decays.
 //
-// Measured, bf16: 65536 x 12 x 64 STATES 51 us (201 MB at 3.9 TB/s, all that a sum which only
-// reads reaches), output 100 us (403 MB at 4.0 TB/s); 8 x 1568 x 12 x 64 15 and 20 us; 20000
-// packed x 16 x 128 57 and 106 us.  What bounds the output's pass is the chain through a chunk,
+// Measured, bf16: 65536 x 12 x 64 STATES 50 us (201 MB at 4.0 TB/s, all that a sum which only
+// reads reaches), output 108 us (403 MB at 3.7 TB/s); 8 x 1568 x 12 x 64 15 and 24 us; 20000
+// packed x 16 x 128 56 and 122 us.  What bounds the output's pass is the chain through a chunk,
 // not one unit: of the latter (117 us when that was measured) the state's sum and its product, most
 // of the matrix work, are worth 15 each and 26 together, then stores 28, loads 18, and 34 are
 // left without anything else.
@@ -818,7 +818,10 @@ __device__ __forceinline__ double within(double x, float most) { return x > most
 // differences a token with a decay of its own would drown in the rounding of the rest.
 // PARTS: of dots and peaks, by channels.
 //
-// Measured, bf16: 8 x 1568 x 12 x 64 45 us; 20000 packed x 16 x 128 291 us, where four heads share
+// dg's work goes on beside the next chunk's pairs, in a wave that has none of them: 20000 packed
+// x 16 x 128 326 us, in the last wave but one 353, at the end of a chunk 357.
+//
+// Measured, bf16: 8 x 1568 x 12 x 64 50 us; 20000 packed x 16 x 128 332 us, where four heads share
 // a key and 328 MB of fp32 parts are written, 64 us of it.  Two states of D x D in registers
 // leave two waves a SIMD (D <= 64: three), so a chunk's chain of products is seen in full; parts of
 // the channels as in mix would form both kinds of pairs twice (343 us for 325 then).
@@ -1267,8 +1270,10 @@ struct StepArgs {
 
 // A wave takes R rows of a state (rows of v's channels) through one token: loads of
 // 16 bytes a lane, L lanes a row, all in flight together.  The states' bytes, read and
-// written once, are all that counts: 256 x 32 x 128 x 128 (1.07 GB both ways) 215 us, 5.0 TB/s;
-// 200 of 12 x 64 x 64 (79 MB) 16 us.
+// written once, are all that counts up to about a thousand rows: 256 x 32 x 128 x 128 (1.07 GB both
+// ways) 215 us, 5.0 TB/s; 200 of 12 x 64 x 64 (79 MB) 16 us.  With slots every wave looks through
+// all rows for its own, B / 64 rounds of loads, which many small states do not hide: 1024 rows of 12 x
+// 64 x 64 74 us (without slots 63), 4096 of 6 x 64 x 64 317 (147), 8192 944 (301).
 template <int D>
 struct StepCfg {
     static constexpr int L = D == 32 ? 8 : D == 64 ? 16 : 32, RP = 64 / L, R = D == 32 ? 32 : 16, NP = R / RP, PARTS = D / R;
@@ -1347,9 +1352,13 @@ struct Plan {
 // least of all counts.  (In chunks' times of a full card, 7.5 us at D = 64, bf16, where it was
 // measured: a chunk takes 0.33 in a workgroup alone, a slot's beginning a third of a chunk;
 // the pass for the states half of the forward pass, dq 1.2 of it and mix2, of which fewer
-// fit, 2.1; the two more launches 0.9 and a slot of the scan 0.02.  8 x 1568 x 12 x 64 takes 42 us
-// in slots of 3 chunks, 45 of 2 or 4, 68 whole; 196 x 6 x 64 14.5 of one chunk, 12.1 whole; 20000
-// packed x 16 x 128 forward and backward 724 of 7, 769 of 5, 779 of 6, 754 of 12, 835 of 3.)
+// fit, 2.1; the two more launches 0.9 and a slot of the scan 0.02.  8 x 1568 x 12 x 64 takes 48 us
+// in slots of 3 chunks, 51 of 2, 50 of 4, 47 of 5, 81 whole, and with gradients 136, 154, 149, 144 and 392;
+// 196 x 6 x 64 19 whole or of one chunk; 20000 packed x 16 x 128 forward and backward 792 of 7, 838 of 5,
+// 848 of 6, 824 of 12, 906 of 3.  The figures are bf16's at D = 64 and 128; fp32 and heads of 32 and 96
+// take them over.  At 8 x 1568 and one sequence of 2048 to 8192 their choice was within 6% of the
+// best length for heads of 32 and 96 and small fp32 calls; 12% above it for fp32 8 x 1568 x 12 x 64
+// with gradients, 235 us against 209, and 20% for fp32 8 x 1568 x 8 x 128 forward, 145 against 122.)
 Plan plan_of(const Args& a, bool train) {
     Plan p;
     p.packed = a.cu != nullptr;

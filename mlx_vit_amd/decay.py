@@ -258,7 +258,8 @@ def decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     q, k, v (B, heads, D), g (B, H) or (H,), types and heads as in ``chunk_decay``, whose
     final_state a sequence goes on from.  ``slots`` (B,) int32 on the same device: the state of each
     row (without it row b's is b, N = B).  A row whose slot is none of 0 to N - 1 is left out, its o
-    zero; rows of one slot follow each other.  No gradients: ``chunk_decay`` with T = 1 has them."""
+    zero; rows of one slot follow each other (which is looked for among all rows: thousands of them
+    cost more than their states).  No gradients: ``chunk_decay`` with T = 1 has them."""
     H = _check_operands("decay_step", q, k, v, g, ("B",))
     B, _, D = q.shape
     dev = q.device
