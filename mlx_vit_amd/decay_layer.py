@@ -9,7 +9,7 @@ g = -exp(A_log) softplus(a_proj(x) + dt_bias).
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -28,9 +28,10 @@ def video_sections(head_dim: int) -> Tuple[int, int, int]:
 
 class DecayAttentionLayer(nn.Module):
     """``forward(x, state=None, start=None) -> (out, new_state)``, x (B, L, hidden_size), state
-    (B, H, D, D) fp32 or None; ``start``: the first token's number in its video, of all rows (a
-    number, which a captured graph keeps).  A state holds keys turned by their positions, so whoever
-    goes on from one says from where; without a state it is 0.
+    (B, H, D, D) fp32 or None; ``start``: the first token's number in its video, a number for all rows
+    (a captured graph keeps it) or (B,) int32 or int64 on x's device, each row's (a graph reads it
+    anew).  A state holds keys turned by their positions, so whoever goes on from one says from
+    where; without a state it is 0.
     ``grid`` = (height, width): the tokens of a frame.  ``num_kv_heads``: key and value heads, each
     shared by num_heads / num_kv_heads heads (default: one each)."""
 
@@ -57,17 +58,28 @@ class DecayAttentionLayer(nn.Module):
         self.o_norm = RMSNormGated(head_dim, eps=1e-5)
         self.o_proj = nn.Linear(total, hidden_size, bias=False)
 
-    def _operands(self, x: torch.Tensor, start: int):
+    def _where(self, x: torch.Tensor, start: Union[int, torch.Tensor]) -> dict:
+        """rotary's positions of x's tokens."""
+        if not isinstance(start, torch.Tensor) or not start.dim():
+            return dict(grid=self.grid, start=start)
+        if start.shape != x.shape[:1] or start.dtype not in (torch.int32, torch.int64) or start.device != x.device:
+            raise ValueError(f"start must be a number or ({x.shape[0]},) int32 or int64 on {x.device}; "
+                             f"got {tuple(start.shape)} {start.dtype} on {start.device}")
+        h, w = self.grid
+        n = start[:, None] + torch.arange(x.shape[1], device=x.device)
+        return dict(positions=torch.stack([n // (h * w), n // w % h, n % w][:len(self.sections)]))
+
+    def _operands(self, x: torch.Tensor, start: Union[int, torch.Tensor]):
         if x.dim() != 3 or x.shape[-1] != self.hidden_size:
             raise ValueError(f"x must be (B, L, {self.hidden_size}); got {tuple(x.shape)}")
         D = self.head_dim
         q, k, v = (p(x).unflatten(-1, (-1, D)) for p in (self.q_proj, self.k_proj, self.v_proj))
-        q, k = rotary(q * self.scale, k, grid=self.grid, start=start, sections=self.sections, base=self.base)
+        q, k = rotary(q * self.scale, k, **self._where(x, start), sections=self.sections, base=self.base)
         g = -torch.exp(self.A_log.float()) * F.softplus(self.a_proj(x).float() + self.dt_bias.float())
         return q, k, v, g
 
     def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None,
-                start: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                start: Union[None, int, torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         if start is None:
             if state is not None:
                 raise ValueError("a state was given without start, the number of the first token in its video")
@@ -76,10 +88,12 @@ class DecayAttentionLayer(nn.Module):
         return self.o_proj(self.o_norm(o, self.g_proj(x))), new_state
 
     @torch.no_grad()
-    def step(self, x: torch.Tensor, state: torch.Tensor, start: int) -> torch.Tensor:
-        """The next token of each row, x (B, 1, hidden_size), number ``start`` of its video, in all rows; ``state`` is updated."""
+    def step(self, x: torch.Tensor, state: torch.Tensor, start: Union[int, torch.Tensor],
+             slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The next token of each row, x (B, 1, hidden_size), number ``start`` of its video, as in forward; ``state``
+        is updated: (B, H, D, D), or (N, H, D, D) with ``slots`` (B,) int32, the state of each row (``decay_step``)."""
         q, k, v, g = self._operands(x, start)
         if x.shape[1] != 1:
             raise ValueError(f"a step takes one token of each row; got {x.shape[1]}")
-        o = decay_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], state)
+        o = decay_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], state, slots)
         return self.o_proj(self.o_norm(o[:, None], self.g_proj(x)))

@@ -19,7 +19,7 @@ Differences of form, not of function:
 """
 from __future__ import annotations
 
-from typing import List, Optional, Tuple
+from typing import List, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -219,8 +219,8 @@ class NoPEVideoEncoder(nn.Module):
 class HybridBlock(nn.Module):
     """One processor block, GDN or NoPE attention (nope_gdn_mlx.py:4009-4091); or ``decay``, linear
     attention with rotary positions over frames of ``grid`` tokens, in the GDN's place.  A decay
-    block that goes on from a state takes ``start``, the number of x's first token in its video;
-    the others have no positions and leave it."""
+    block that goes on from a state takes ``start``, the number of x's first token in its video, of
+    all rows or of each; the others have no positions and leave it."""
 
     fused_mlp = False   # set_fused_mlp
 
@@ -251,7 +251,7 @@ class HybridBlock(nn.Module):
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None,
                 state: Optional[torch.Tensor] = None,
-                start: Optional[int] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+                start: Union[None, int, torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         B, N, D = x.shape
         normed = self.norm1(x)
         if self.block_type != "nope":

@@ -76,3 +76,65 @@ def test_block_against_64_bits(time_only):
             **{"layer." + n: t for n, t in zip(lp, gl[1:])}, **{"mlp." + n: t for (n, _), t in zip(mlp.named_parameters(), gp)}}
     for name, a, b in zip(["y", *names], got, [wy, *(want[n] for n in names)]):
         assert float((a.double() - b).abs().max()) <= 2e-4 * float(b.abs().max()), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(sections=(64,)), dict(sections=(32, 32))])
+def test_streams_at_different_times(kw):
+    """Rows with numbers and states of their own, in a prompt and token by token, as each alone."""
+    torch.manual_seed(0)
+    layer = DecayAttentionLayer(48, 2, 64, grid=(3, 4), **kw).cuda()
+    x, starts = torch.randn(3, 20, 48, device="cuda"), [0, 31, 12 * 700 + 5]
+    at = torch.tensor(starts, device="cuda")
+    near = dict(rtol=1e-4, atol=1e-4)
+    with torch.no_grad():
+        state = 0.1 * torch.randn(5, 2, 64, 64, device="cuda")
+        slots = [4, 0, 2]
+        y, s = layer(x[:, :18], state[slots], start=at)
+        pool = state.clone()
+        pool[slots] = s
+        tails = [layer.step(x[:, t:t + 1], pool, (at + t).int(), torch.tensor(slots, dtype=torch.int32, device="cuda")) for t in (18, 19)]
+        for b, n in enumerate(starts):
+            one, last = layer(x[b:b + 1, :18], state[slots[b]:slots[b] + 1], start=n)
+            torch.testing.assert_close(y[b:b + 1], one, **near)
+            for i, t in enumerate((18, 19)):
+                torch.testing.assert_close(tails[i][b:b + 1], layer.step(x[b:b + 1, t:t + 1], last, n + t), **near)
+            torch.testing.assert_close(pool[slots[b]:slots[b] + 1], last, **near)
+        assert torch.equal(pool[[1, 3]], state[[1, 3]])
+
+
+@pytest.mark.gpu
+def test_a_captured_step_goes_on():
+    """Its numbers are read anew with every replay."""
+    torch.manual_seed(0)
+    layer = DecayAttentionLayer(48, 2, 64, grid=(3, 4)).cuda()
+    x, at = torch.randn(2, 1, 48, device="cuda"), torch.tensor([3, 90], device="cuda")
+    state = 0.1 * torch.randn(2, 2, 64, 64, device="cuda")
+    twin = state.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.step(x, state.clone(), at)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer.step(x, state, at)
+    for i in range(4):
+        x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        # (the projections' products may be made by another of torch's kernels in a graph)
+        torch.testing.assert_close(y, layer.step(x, twin, torch.tensor([3 + i, 90 + i], device="cuda")), rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(state, twin, rtol=1e-5, atol=1e-5)
+        at += 1
+
+
+def test_start_is_refused():
+    layer = DecayAttentionLayer(64, 2, 32)
+    x, state = torch.zeros(2, 6, 64), torch.zeros(2, 2, 32, 32)
+    for start in (torch.zeros(3, dtype=torch.int64), torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2)):
+        with pytest.raises(ValueError, match="start must be"):
+            layer(x, state, start)
+    for start in (1.5, torch.tensor(1.5)):
+        with pytest.raises(ValueError, match="whole numbers"):
+            layer(x, state, start)
